@@ -233,6 +233,16 @@ def _rows_of(s, b):
     return s["kv"][s["row_at"][b]:s["row_at"][b + 1]]
 
 
+def _tiles(k, v, r):
+    """Keys, values and rope keys (rows, .., dims) padded with zeros to tiles of 64 rows, their indices split."""
+    pad = -k.shape[0] % 64
+    if pad:
+        k, v, r = (torch.cat([x, x.new_zeros(pad, *x.shape[1:])]) for x in (k, v, r))
+    heads = k.shape[1]
+    return (k.reshape(-1, 2, 32, heads, 8, 2, 2, 4), v.reshape(-1, 4, 2, 2, 4, heads, 4, 32),
+            r.reshape(-1, 2, 32, 4, 2, 2, 4))
+
+
 def _decompress(rows, W, heads):
     """c_t W^T per head: (heads, rows, 128)."""
     return torch.matmul(rows[:, :DC], W.float().view(heads, -1, DC).transpose(1, 2))
@@ -270,9 +280,9 @@ def _run_plain(s):
     heads, kind, cos, sin = case["heads"], case["kind"], s["cos"], s["sin"]
     if kind == "expand":
         rows = s["rows"].float()
-        return (_decompress(rows, s["W_UK"], heads).transpose(0, 1).to(s["model"]),
-                _decompress(rows, s["W_UV"], heads).transpose(0, 1).to(s["model"]),
-                _rotate(rows[:, DC:], cos, sin).to(s["model"]))
+        return _tiles(_decompress(rows, s["W_UK"], heads).transpose(0, 1).to(s["model"]),
+                      _decompress(rows, s["W_UV"], heads).transpose(0, 1).to(s["model"]),
+                      _rotate(rows[:, DC:], cos, sin).to(s["model"]))
     outs = []
     if kind == "prefill":
         q = s["q"].float()
@@ -373,7 +383,12 @@ def exact(case, seed):
         latent = r[:, :DC].T.contiguous()
         k = torch.matmul(s["W_UK"].double(), latent).view(heads, DN, -1).permute(2, 0, 1)
         v = torch.matmul(s["W_UV"].double(), latent).view(heads, DV, -1).permute(2, 0, 1)
-        return k, v, turned(r[:, DC:], turn)
+        whole = -(-k.shape[0] // 64) * 64  # zeros up to whole tiles, the indices split as SharedPrefix has them
+        out = [torch.zeros(whole, *x.shape[1:], dtype=x.dtype, device="cuda") for x in (k, v, r[:, DC:])]
+        for x, y in zip(out, (k, v, turned(r[:, DC:], turn))):
+            x[:y.shape[0]] = y
+        return (out[0].view(-1, 2, 32, heads, 8, 2, 2, 4), out[1].view(-1, 4, 2, 2, 4, heads, 4, 32),
+                out[2].view(-1, 2, 32, 4, 2, 2, 4))
     pairs = sum(n * (o + n + case.get("prefix_rows", 0)) for n, o, _ in s["lens"])
     if pairs * heads > 2.0e10:
         return None
