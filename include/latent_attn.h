@@ -207,6 +207,120 @@ typedef struct la_append_args {
   int32_t blocks_per_seq;
 } la_append_args;
 
+/* Attention of several new tokens per sequence: prompts, pieces of prompts,
+ * drafted tokens (la_mla_prefill). No counterpart in the reference, whose
+ * entry points take one query position. */
+typedef struct la_prefill_args {
+  /* latent cache, as in la_decode_args: equal regions of seq_len rows,
+   * seq_offsets, or a paged pool; seq_lens optional (required with
+   * block_table). The rows of the new tokens are in it already
+   * (la_append_kv). */
+  const void* kv_cache;
+  int32_t kv_dtype;
+  int64_t total_rows;
+  int32_t num_seqs;
+  int32_t seq_len;
+  const int32_t* seq_offsets;
+  const int32_t* seq_lens;
+  const int32_t* block_table;
+  int32_t block_size;
+  int32_t blocks_per_seq;
+  /* most rows of a sequence, 0 = its region (regions and paged caches): a
+   * region ends there. Bounds the workspace where the capacity is far beyond
+   * the lengths. */
+  int32_t max_seq_rows;
+  /* new tokens, packed: sequence s has tokens [q_offsets[s], q_offsets[s+1])
+   * (DEVICE int32, num_seqs + 1, starting at 0; non-decreasing), or, with
+   * NULL, tokens / num_seqs each. They are its last rows: token j of n of a
+   * sequence with L rows is at position L - n + j. Tokens behind the last
+   * sequence get zero rows. */
+  int64_t tokens;
+  const int32_t* q_offsets;
+  /* queries (tokens, num_heads, qk_nope_head_dim) and (tokens, num_heads,
+   * qk_rope_head_dim) of q_dtype (F32, F16, BF16), with strides in elements
+   * from token to token and from head to head (0, 0 = packed). */
+  const void* q_nope;
+  const void* q_rope;
+  int32_t q_dtype;
+  int64_t q_nope_token_stride, q_nope_head_stride;
+  int64_t q_rope_token_stride, q_rope_head_stride;
+  /* 1: q_rope is not rotated yet and is rotated by its token's position on the
+   * way (q_rope itself is left as it is); 0: it comes rotated. */
+  int32_t rotate_q;
+  /* mask: a token sees the rows up to its own. prefix_lens (optional, DEVICE
+   * int32, num_seqs): it also sees the sequence's first prefix_lens[s] rows,
+   * so those are read in both directions. A token that sees nothing (more
+   * tokens than rows) gets a zero row. */
+  const int32_t* prefix_lens;
+  const void* W_UK;
+  int32_t w_uk_dtype;
+  const void* W_UV;
+  int32_t w_uv_dtype;
+  const float* rope_cos; /* indexed by position, as in la_decode_args */
+  const float* rope_sin;
+  int64_t rope_rows;
+  /* (tokens, num_heads, v_head_dim) of out_dtype (F32, F16, BF16); must not overlap an input */
+  void* output;
+  int32_t out_dtype;
+  la_mla_config cfg;
+  void* workspace; /* la_mla_prefill_workspace_size bytes; NULL: taken stream-ordered */
+  size_t workspace_bytes;
+  /* 0 = automatic; 1 = plain kernel (any type and head shape); 2 = keys and
+   * values expanded from the rows, on the matrix cores; 3 = queries absorbed,
+   * every token a sequence of a paged decode step. LA_ERROR_NOT_SUPPORTED
+   * where the form has no kernel for these arguments. */
+  int32_t kernel_variant;
+} la_prefill_args;
+
+/* A prefix's rows expanded into per-head keys and values (la_expand_prefix). */
+typedef struct la_expand_args {
+  const void* kv_cache; /* rows rows, packed */
+  int32_t kv_dtype;     /* F16, BF16 or FP8_E4M3 */
+  int32_t rows;
+  const void* W_UK;
+  int32_t w_uk_dtype;
+  const void* W_UV;
+  int32_t w_uv_dtype;
+  const float* rope_cos;
+  const float* rope_sin;
+  int64_t rope_rows;
+  la_mla_config cfg;
+  /* la_expanded_size bytes, 256-byte aligned: K, V, then the rotated rope
+   * keys, in fp16 for an F16 cache and bf16 otherwise, in tiles of 64 rows
+   * (zeros past the last row) in the order that the matrix instructions take:
+   *   K     [head][tile][32-row block (2)][step of 16 dims (8)][lane (64)][8]
+   *   V     [head][tile][32-dim block (4)][step of 16 rows (4)][lane (64)][8]
+   *   rope  [tile][32-row block (2)][step of 16 dims (4)][lane (64)][8]
+   * where lane l is row (V: dim) l % 32 of its block, and with g = l / 32
+   * elements 0..3 are dims (V: rows) 4 g + (0..3) of the step, elements 4..7
+   * are 8 + 4 g + (0..3). */
+  void* expanded;
+  size_t expanded_bytes;
+  void* workspace; /* la_expand_prefix_workspace_size bytes; NULL: taken stream-ordered */
+  size_t workspace_bytes;
+} la_expand_args;
+
+/* A decode step of sequences that share a prefix (la_mla_decode_shared). */
+typedef struct la_shared_args {
+  /* the sequences' own rows and the queries, as for la_mla_decode (q_nope and
+   * W_UK; all queries_per_seq queries of a sequence see all its rows).
+   * rope_cos / rope_sin are indexed from the prefix's first row: row i of a
+   * sequence is at position prefix_len + i. output, workspace, chunk_rows and
+   * kernel_variant of this descriptor are not read. */
+  la_decode_args own;
+  const void* prefix; /* (prefix_len, kv_lora_rank + qk_rope_head_dim) rows of own.kv_dtype, at positions 0, 1, ... */
+  int32_t prefix_len;
+  /* la_expand_prefix's buffer for the same rows and weights, or NULL: large
+   * batches then read it in place of the rows */
+  const void* expanded;
+  void* output; /* (num_seqs * queries_per_seq, num_heads, v_head_dim) of out_dtype (F32, F16, BF16) */
+  int32_t out_dtype;
+  void* workspace; /* la_mla_decode_shared_workspace_size bytes; NULL: taken stream-ordered */
+  size_t workspace_bytes;
+  /* 0 = automatic; 1 = latent rows of the prefix; 2 = its expanded form */
+  int32_t kernel_variant;
+} la_shared_args;
+
 /* Human-readable name of an la_status value. */
 const char* la_status_string(int status);
 
@@ -355,6 +469,26 @@ int la_append_kv(const la_append_args* args, void* stream);
  * q_absorbed (tokens, nh, dc) f32. */
 int la_absorb_q(const float* q_nope, const void* W_UK, int w_uk_dtype, float* q_absorbed, int tokens,
                 const la_mla_config* cfg, void* stream);
+
+/* out[t,h] = softmax_k(scale * (q_nope[t,h] . K[k,h] + q_rope[t,h] . RoPE(k_rope[k], k))) . V[k,h] over the keys that
+ * token t sees, K = c_t W_UK^T and V = c_t W_UV^T. Device offsets and lengths
+ * that are out of range are clamped (wrong rows, no access out of bounds). */
+int la_mla_prefill(const la_prefill_args* args, void* stream);
+size_t la_mla_prefill_workspace_size(const la_prefill_args* args);
+
+/* Expands a prefix's rows once, for la_mla_decode_shared. 16-bit and FP8
+ * caches with kv_lora_rank 512, qk_nope_head_dim and v_head_dim 128,
+ * qk_rope_head_dim 64; weights of any type (rounded to the expanded one). */
+int la_expand_prefix(const la_expand_args* args, void* stream);
+size_t la_expand_prefix_workspace_size(const la_expand_args* args);
+/* Bytes of the expanded form of `rows` rows: 512 per row and head, 128 per
+ * row, rows rounded up to 64. 0 for dimensions without one. */
+size_t la_expanded_size(int32_t rows, const la_mla_config* cfg);
+
+/* One decode step over [prefix | own rows] of every sequence: the prefix's
+ * part is computed for all queries at once. */
+int la_mla_decode_shared(const la_shared_args* args, void* stream);
+size_t la_mla_decode_shared_workspace_size(const la_shared_args* args);
 
 #ifdef __cplusplus
 } /* extern "C" */

@@ -6,8 +6,9 @@
 // messages, output allocated as float32 on kv_cache's device, launched on the
 // current stream. Differences: the 16-bit dtype may be float16 (reference
 // contract) or bfloat16, float32 caches/weights select the fp32 path, a
-// device guard is taken, and two functions are added (mla_decode_forward,
-// absorb_q_forward). No tensor math happens here; all compute is in the HIP
+// device guard is taken, and functions are added (mla_decode_forward,
+// mla_decode_absorbed_forward, append_kv_forward, absorb_q_forward,
+// mla_prefill_forward, expand_prefix_forward, mla_decode_shared_forward). No tensor math happens here; all compute is in the HIP
 // library.
 #include <torch/extension.h>
 #include <c10/hip/HIPStream.h>
@@ -506,6 +507,307 @@ torch::Tensor naive_mla_forward(torch::Tensor kv_cache, torch::Tensor W_UK, torc
   return out;
 }
 
+namespace {
+
+// Cache, sequence and table arguments of mla_prefill_forward and
+// mla_decode_shared_forward, checked as for mla_decode_forward. Returns the
+// longest sequence that the host knows of (0: lengths are on the device).
+template <typename Args>
+int64_t fill_cache(Args& a, const torch::Tensor& kv_cache, const c10::optional<torch::Tensor>& seq_offsets,
+                   const c10::optional<torch::Tensor>& seq_lens, const c10::optional<torch::Tensor>& block_table,
+                   int block_size, int64_t batch, int64_t row) {
+  int64_t longest = 0;
+  a.kv_cache = kv_cache.data_ptr();
+  a.kv_dtype = dtype_tag(kv_cache);
+  a.num_seqs = (int32_t)batch;
+  if (block_table.has_value() && block_table->defined()) {
+    const auto& bt = *block_table;
+    TORCH_CHECK(bt.dtype() == torch::kInt32 && bt.is_contiguous() && bt.is_cuda() && bt.dim() == 2 &&
+                    bt.size(0) == batch,
+                "block_table must be a contiguous int32 CUDA tensor (batch, blocks_per_seq)");
+    TORCH_CHECK(!(seq_offsets.has_value() && seq_offsets->defined()), "block_table and seq_offsets exclude each other");
+    TORCH_CHECK(seq_lens.has_value() && seq_lens->defined(), "a paged cache needs seq_lens");
+    TORCH_CHECK(block_size > 0 && kv_cache.dim() == 2 && kv_cache.size(1) == row && kv_cache.size(0) % block_size == 0,
+                "paged kv_cache must be a (num_blocks * block_size, ", row, ") pool");
+    TORCH_CHECK(batch == 0 || kv_cache.size(0) >= block_size, "paged kv_cache pool needs at least one block");
+    TORCH_CHECK(bt.size(1) > 0 && bt.size(1) * block_size <= INT32_MAX, "block_table has no or too many blocks");
+    check_same_device(kv_cache, bt, "block_table");
+    a.total_rows = kv_cache.size(0);
+    a.block_table = bt.data_ptr<int32_t>();
+    a.block_size = block_size;
+    a.blocks_per_seq = (int32_t)bt.size(1);
+  } else if (seq_offsets.has_value() && seq_offsets->defined()) {
+    const auto& off = *seq_offsets;
+    TORCH_CHECK(off.dtype() == torch::kInt32 && off.is_contiguous() && off.is_cuda(),
+                "seq_offsets must be a contiguous int32 CUDA tensor");
+    TORCH_CHECK(off.dim() == 1 && off.size(0) == batch + 1, "seq_offsets must have batch + 1 entries");
+    check_same_device(kv_cache, off, "seq_offsets");
+    TORCH_CHECK(kv_cache.dim() == 2 && kv_cache.size(1) == row, "packed kv_cache must be (total_rows, ", row, ")");
+    a.total_rows = kv_cache.size(0);
+    a.seq_offsets = off.data_ptr<int32_t>();
+  } else {
+    TORCH_CHECK(kv_cache.dim() == 3 && kv_cache.size(0) == batch && kv_cache.size(2) == row,
+                "kv_cache must be (batch, seq_len, ", row, ") when seq_offsets is None");
+    TORCH_CHECK(kv_cache.size(1) <= INT32_MAX, "seq_len too large");
+    a.seq_len = (int32_t)kv_cache.size(1);
+    a.total_rows = batch * kv_cache.size(1);
+    longest = kv_cache.size(1);
+  }
+  if (seq_lens.has_value() && seq_lens->defined()) {
+    const auto& len = *seq_lens;
+    TORCH_CHECK(len.dtype() == torch::kInt32 && len.is_contiguous() && len.is_cuda(),
+                "seq_lens must be a contiguous int32 CUDA tensor");
+    TORCH_CHECK(len.dim() == 1 && len.size(0) == batch, "seq_lens must have batch entries");
+    check_same_device(kv_cache, len, "seq_lens");
+    a.seq_lens = len.data_ptr<int32_t>();
+    longest = 0;
+  }
+  return longest;
+}
+
+void check_weights(const torch::Tensor& kv_cache, const torch::Tensor& W_UK, const torch::Tensor& W_UV,
+                   const la_mla_config& c) {
+  check_weight(W_UK, "W_UK");
+  check_weight(W_UV, "W_UV");
+  TORCH_CHECK(W_UK.dim() == 2 && W_UK.size(0) == (int64_t)c.num_heads * c.qk_nope_head_dim &&
+                  W_UK.size(1) == c.kv_lora_rank,
+              "W_UK shape mismatch");
+  TORCH_CHECK(W_UV.dim() == 2 && W_UV.size(0) == (int64_t)c.num_heads * c.v_head_dim && W_UV.size(1) == c.kv_lora_rank,
+              "W_UV shape mismatch");
+  check_same_device(kv_cache, W_UK, "W_UK");
+  check_same_device(kv_cache, W_UV, "W_UV");
+}
+
+int out_tag(c10::ScalarType t) {
+  switch (t) {
+    case torch::kFloat32: return LA_DTYPE_F32;
+    case torch::kFloat16: return LA_DTYPE_F16;
+    case torch::kBFloat16: return LA_DTYPE_BF16;
+    default: TORCH_CHECK(false, "out_dtype must be float16, bfloat16 or float32, got ", t); return -1;
+  }
+}
+
+}  // namespace
+
+// mla_prefill_forward -- several new tokens per sequence (la_mla_prefill):
+//   q_nope (T, nh, dn), q_rope (T, nh, dR) in float32 / float16 / bfloat16, last
+//   dimension contiguous; q_offsets None or int32 (B+1,); prefix_lens None or
+//   int32 (B,); returns (T, nh, dv) in out_dtype.
+torch::Tensor mla_prefill_forward(torch::Tensor kv_cache, torch::Tensor q_nope, torch::Tensor q_rope,
+                                  torch::Tensor W_UK, torch::Tensor W_UV, torch::Tensor rope_cos,
+                                  torch::Tensor rope_sin, c10::optional<torch::Tensor> q_offsets,
+                                  c10::optional<torch::Tensor> seq_offsets, int d_model, int kv_lora_rank,
+                                  int qk_nope_head_dim, int qk_rope_head_dim, int num_heads, int v_head_dim,
+                                  c10::optional<torch::Tensor> seq_lens, c10::optional<torch::Tensor> block_table,
+                                  int block_size, c10::optional<torch::Tensor> prefix_lens, bool rotate_q,
+                                  int max_seq_rows, c10::ScalarType out_dtype, int kernel_variant) {
+  check_storage(kv_cache, "kv_cache");
+  check_fp32_contiguous(rope_cos, "rope_cos");
+  check_fp32_contiguous(rope_sin, "rope_sin");
+  const la_mla_config cfg =
+      config_from_args(d_model, kv_lora_rank, qk_nope_head_dim, qk_rope_head_dim, num_heads, v_head_dim);
+  const int64_t row = (int64_t)kv_lora_rank + qk_rope_head_dim;
+  TORCH_CHECK(q_nope.dim() == 3 && q_nope.size(1) == num_heads && q_nope.size(2) == qk_nope_head_dim,
+              "q_nope must be (tokens, num_heads, qk_nope_head_dim)");
+  const int64_t tokens = q_nope.size(0);
+  TORCH_CHECK(q_rope.dim() == 3 && q_rope.size(0) == tokens && q_rope.size(1) == num_heads &&
+                  q_rope.size(2) == qk_rope_head_dim,
+              "q_rope must be (tokens, num_heads, qk_rope_head_dim)");
+  TORCH_CHECK(dtype_tag(q_nope) >= 0 && dtype_tag(q_nope) != LA_DTYPE_FP8_E4M3,
+              "q_nope must be float16, bfloat16 or float32, got ", q_nope.dtype());
+  TORCH_CHECK(q_rope.dtype() == q_nope.dtype(), "q_nope and q_rope must have the same dtype");
+  for (auto* t : {&q_nope, &q_rope}) {
+    TORCH_CHECK(t->is_cuda(), "queries must be on CUDA");
+    TORCH_CHECK(t->stride(2) == 1 && t->stride(0) >= 0 && t->stride(1) >= 0,
+                "queries must be contiguous in their last dimension");
+    check_same_device(kv_cache, *t, "queries");
+  }
+  check_weights(kv_cache, W_UK, W_UV, cfg);
+  for (auto* t : {&rope_cos, &rope_sin}) check_same_device(kv_cache, *t, "inputs");
+
+  la_prefill_args a{};
+  int64_t batch;
+  if (block_table.has_value() && block_table->defined()) {
+    TORCH_CHECK(block_table->dim() == 2, "block_table must be a contiguous int32 CUDA tensor (batch, blocks_per_seq)");
+    batch = block_table->size(0);
+  } else if (seq_offsets.has_value() && seq_offsets->defined()) {
+    TORCH_CHECK(seq_offsets->dim() == 1 && seq_offsets->size(0) > 0, "seq_offsets must have batch + 1 entries");
+    batch = seq_offsets->size(0) - 1;
+  } else {
+    TORCH_CHECK(kv_cache.dim() == 3, "kv_cache must be (batch, seq_len, ", row, ") when seq_offsets is None");
+    batch = kv_cache.size(0);
+  }
+  TORCH_CHECK(batch < INT32_MAX && tokens <= INT32_MAX / num_heads, "batch too large");
+  int64_t longest = fill_cache(a, kv_cache, seq_offsets, seq_lens, block_table, block_size, batch, row);
+  TORCH_CHECK(max_seq_rows >= 0, "max_seq_rows must not be negative");
+  TORCH_CHECK(max_seq_rows == 0 || !a.seq_offsets, "max_seq_rows and seq_offsets exclude each other");
+  if (max_seq_rows > 0) longest = std::min<int64_t>(longest, max_seq_rows);
+  check_rope(rope_cos, rope_sin, std::max<int64_t>(longest, 1), cfg);
+  a.max_seq_rows = max_seq_rows;
+  a.tokens = tokens;
+  if (q_offsets.has_value() && q_offsets->defined()) {
+    const auto& off = *q_offsets;
+    TORCH_CHECK(off.dtype() == torch::kInt32 && off.is_contiguous() && off.is_cuda() && off.dim() == 1 &&
+                    off.size(0) == batch + 1,
+                "q_offsets must be a contiguous int32 CUDA tensor of batch + 1 entries");
+    check_same_device(kv_cache, off, "q_offsets");
+    a.q_offsets = off.data_ptr<int32_t>();
+  } else {
+    TORCH_CHECK(tokens == 0 || (batch > 0 && tokens % batch == 0),
+                "tokens must be a multiple of the batch without q_offsets");
+  }
+  TORCH_CHECK(tokens == 0 || batch > 0, "tokens without a sequence");
+  if (prefix_lens.has_value() && prefix_lens->defined()) {
+    const auto& len = *prefix_lens;
+    TORCH_CHECK(len.dtype() == torch::kInt32 && len.is_contiguous() && len.is_cuda() && len.dim() == 1 &&
+                    len.size(0) == batch,
+                "prefix_lens must be a contiguous int32 CUDA tensor of batch entries");
+    check_same_device(kv_cache, len, "prefix_lens");
+    a.prefix_lens = len.data_ptr<int32_t>();
+  }
+  a.q_nope = q_nope.data_ptr();
+  a.q_rope = q_rope.data_ptr();
+  a.q_dtype = dtype_tag(q_nope);
+  if (!q_nope.is_contiguous()) a.q_nope_token_stride = q_nope.stride(0), a.q_nope_head_stride = q_nope.stride(1);
+  if (!q_rope.is_contiguous()) a.q_rope_token_stride = q_rope.stride(0), a.q_rope_head_stride = q_rope.stride(1);
+  a.rotate_q = rotate_q;
+  a.W_UK = W_UK.data_ptr();
+  a.w_uk_dtype = dtype_tag(W_UK);
+  a.W_UV = W_UV.data_ptr();
+  a.w_uv_dtype = dtype_tag(W_UV);
+  a.rope_cos = rope_cos.data_ptr<float>();
+  a.rope_sin = rope_sin.data_ptr<float>();
+  a.rope_rows = std::min(rope_cos.size(0), rope_sin.size(0));
+  a.out_dtype = out_tag(out_dtype);
+  a.cfg = cfg;
+  a.kernel_variant = kernel_variant;
+
+  const at::DeviceGuard guard(kv_cache.device());
+  auto output = torch::empty({tokens, num_heads, v_head_dim}, kv_cache.options().dtype(out_dtype));
+  if (tokens == 0) return output;
+  a.output = output.data_ptr();
+  const size_t ws_bytes = la_mla_prefill_workspace_size(&a);
+  auto ws = workspace(kv_cache, ws_bytes);
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = ws_bytes;
+  check_status(la_mla_prefill(&a, current_stream()), "la_mla_prefill");
+  return output;
+}
+
+// expand_prefix_forward -- a prefix's rows (P, dc+dR) as per-head keys and
+// values (la_expand_prefix): a flat tensor of the library's order, fp16 for
+// float16 rows and bf16 otherwise.
+torch::Tensor expand_prefix_forward(torch::Tensor kv_cache, torch::Tensor W_UK, torch::Tensor W_UV,
+                                    torch::Tensor rope_cos, torch::Tensor rope_sin, int d_model, int kv_lora_rank,
+                                    int qk_nope_head_dim, int qk_rope_head_dim, int num_heads, int v_head_dim) {
+  check_storage(kv_cache, "kv_cache");
+  check_fp32_contiguous(rope_cos, "rope_cos");
+  check_fp32_contiguous(rope_sin, "rope_sin");
+  const la_mla_config cfg =
+      config_from_args(d_model, kv_lora_rank, qk_nope_head_dim, qk_rope_head_dim, num_heads, v_head_dim);
+  TORCH_CHECK(kv_cache.dim() == 2 && kv_cache.size(1) == (int64_t)kv_lora_rank + qk_rope_head_dim,
+              "kv_cache must be (prefix, ", kv_lora_rank + qk_rope_head_dim, ")");
+  TORCH_CHECK(kv_cache.size(0) <= INT32_MAX, "prefix too long");
+  check_weights(kv_cache, W_UK, W_UV, cfg);
+  check_rope(rope_cos, rope_sin, kv_cache.size(0), cfg);
+  for (auto* t : {&rope_cos, &rope_sin}) check_same_device(kv_cache, *t, "inputs");
+  TORCH_CHECK(kv_cache.scalar_type() != torch::kFloat32 && la_expanded_size(1, &cfg) > 0,
+              "expand_prefix: 16-bit and FP8 caches with kv_lora_rank 512, 128-dim heads and rope 64 only");
+  la_expand_args a{};
+  a.kv_cache = kv_cache.data_ptr();
+  a.kv_dtype = dtype_tag(kv_cache);
+  a.rows = (int32_t)kv_cache.size(0);
+  a.W_UK = W_UK.data_ptr();
+  a.w_uk_dtype = dtype_tag(W_UK);
+  a.W_UV = W_UV.data_ptr();
+  a.w_uv_dtype = dtype_tag(W_UV);
+  a.rope_cos = rope_cos.data_ptr<float>();
+  a.rope_sin = rope_sin.data_ptr<float>();
+  a.rope_rows = std::min(rope_cos.size(0), rope_sin.size(0));
+  a.cfg = cfg;
+  const at::DeviceGuard guard(kv_cache.device());
+  const auto type = kv_cache.scalar_type() == torch::kFloat16 ? torch::kFloat16 : torch::kBFloat16;
+  a.expanded_bytes = la_expanded_size(a.rows, &cfg);
+  auto out = torch::empty({(int64_t)(a.expanded_bytes / 2)}, kv_cache.options().dtype(type));
+  if (a.rows == 0) return out;
+  a.expanded = out.data_ptr();
+  a.workspace_bytes = la_expand_prefix_workspace_size(&a);
+  auto ws = workspace(kv_cache, a.workspace_bytes);
+  a.workspace = ws.data_ptr();
+  check_status(la_expand_prefix(&a, current_stream()), "la_expand_prefix");
+  return out;
+}
+
+// mla_decode_shared_forward -- mla_decode_forward for sequences behind one
+// prefix (P, dc+dR) (la_mla_decode_shared); expanded: None or
+// expand_prefix_forward's tensor of the same rows.
+torch::Tensor mla_decode_shared_forward(torch::Tensor prefix, c10::optional<torch::Tensor> expanded,
+                                        torch::Tensor kv_cache, torch::Tensor q_nope, torch::Tensor q_rope,
+                                        torch::Tensor W_UK, torch::Tensor W_UV, torch::Tensor rope_cos,
+                                        torch::Tensor rope_sin, c10::optional<torch::Tensor> seq_offsets, int d_model,
+                                        int kv_lora_rank, int qk_nope_head_dim, int qk_rope_head_dim, int num_heads,
+                                        int v_head_dim, c10::optional<torch::Tensor> seq_lens,
+                                        c10::optional<torch::Tensor> block_table, int block_size,
+                                        c10::ScalarType out_dtype, int kernel_variant) {
+  check_storage(kv_cache, "kv_cache");
+  check_storage(prefix, "prefix");
+  check_fp32_contiguous(q_nope, "q_nope");
+  check_fp32_contiguous(q_rope, "q_rope");
+  check_fp32_contiguous(rope_cos, "rope_cos");
+  check_fp32_contiguous(rope_sin, "rope_sin");
+  const la_mla_config cfg =
+      config_from_args(d_model, kv_lora_rank, qk_nope_head_dim, qk_rope_head_dim, num_heads, v_head_dim);
+  const int64_t row = (int64_t)kv_lora_rank + qk_rope_head_dim;
+  TORCH_CHECK(prefix.dim() == 2 && prefix.size(1) == row, "prefix must be (prefix, ", row, ")");
+  TORCH_CHECK(prefix.dtype() == kv_cache.dtype(), "prefix and kv_cache must have the same dtype");
+  TORCH_CHECK(prefix.size(0) <= INT32_MAX, "prefix too long");
+  check_same_device(kv_cache, prefix, "prefix");
+  TORCH_CHECK(q_nope.dim() == 3 && q_nope.size(1) == num_heads && q_nope.size(2) == qk_nope_head_dim,
+              "q_nope must be (batch, num_heads, qk_nope_head_dim)");
+  const int64_t batch = q_nope.size(0);
+  TORCH_CHECK(q_rope.dim() == 3 && q_rope.size(0) == batch && q_rope.size(1) == num_heads &&
+                  q_rope.size(2) == qk_rope_head_dim,
+              "q_rope must be (batch, num_heads, qk_rope_head_dim)");
+  TORCH_CHECK(batch <= INT32_MAX / num_heads, "batch too large");
+  check_weights(kv_cache, W_UK, W_UV, cfg);
+  la_shared_args a{};
+  const int64_t longest = fill_cache(a.own, kv_cache, seq_offsets, seq_lens, block_table, block_size, batch, row);
+  check_rope(rope_cos, rope_sin, std::max<int64_t>(prefix.size(0) + longest, 1), cfg);
+  for (auto* t : {&q_nope, &q_rope, &rope_cos, &rope_sin}) check_same_device(kv_cache, *t, "inputs");
+  a.own.queries_per_seq = 1;
+  a.own.q_nope = q_nope.data_ptr<float>();
+  a.own.q_rope = q_rope.data_ptr<float>();
+  a.own.W_UK = W_UK.data_ptr();
+  a.own.w_uk_dtype = dtype_tag(W_UK);
+  a.own.W_UV = W_UV.data_ptr();
+  a.own.w_uv_dtype = dtype_tag(W_UV);
+  a.own.rope_cos = rope_cos.data_ptr<float>();
+  a.own.rope_sin = rope_sin.data_ptr<float>();
+  a.own.rope_rows = std::min(rope_cos.size(0), rope_sin.size(0));
+  a.own.cfg = cfg;
+  a.prefix = prefix.data_ptr();
+  a.prefix_len = (int32_t)prefix.size(0);
+  if (expanded.has_value() && expanded->defined()) {
+    const auto type = prefix.scalar_type() == torch::kFloat16 ? torch::kFloat16 : torch::kBFloat16;
+    TORCH_CHECK(expanded->is_contiguous() && expanded->is_cuda() && expanded->scalar_type() == type &&
+                    (size_t)expanded->nbytes() == la_expanded_size(a.prefix_len, &cfg),
+                "expanded is not the expanded form of prefix");
+    check_same_device(kv_cache, *expanded, "expanded");
+    a.expanded = expanded->data_ptr();
+  }
+  a.out_dtype = out_tag(out_dtype);
+  a.kernel_variant = kernel_variant;
+  const at::DeviceGuard guard(kv_cache.device());
+  auto output = torch::empty({batch, num_heads, v_head_dim}, kv_cache.options().dtype(out_dtype));
+  if (batch == 0) return output;
+  a.output = output.data_ptr();
+  a.workspace_bytes = la_mla_decode_shared_workspace_size(&a);
+  auto ws = workspace(kv_cache, a.workspace_bytes);
+  a.workspace = ws.data_ptr();
+  check_status(la_mla_decode_shared(&a, current_stream()), "la_mla_decode_shared");
+  return output;
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("naive_mla_forward", &naive_mla_forward, "MLA forward from q_nope and W_UK (decompress-then-attend result)");
   m.def("fused_mla_forward", &fused_mla_forward,
@@ -533,4 +835,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("kv_lora_rank"), py::arg("qk_nope_head_dim"), py::arg("qk_rope_head_dim"), py::arg("num_heads"),
         py::arg("v_head_dim"), py::arg("block_table") = py::none(), py::arg("block_size") = 0);
   m.def("absorb_q_forward", &absorb_q_forward, "q_absorbed = q_nope . W_UK per head");
+  m.def("mla_prefill_forward", &mla_prefill_forward,
+        "Causal attention of several new tokens per sequence over latent caches");
+  m.def("expand_prefix_forward", &expand_prefix_forward, "Per-head keys and values of a prefix's latent rows");
+  m.def("mla_decode_shared_forward", &mla_decode_shared_forward,
+        "Decode step over a shared prefix and every sequence's own rows");
 }

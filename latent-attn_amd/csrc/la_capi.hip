@@ -7,6 +7,7 @@
 // the other absorption in la_f32.hip and la_generic.hip, la_append.hip,
 // la_naive.hip.
 #include "la_internal.hpp"
+#include "la_prompt.hpp"
 
 #include <algorithm>
 #include <cmath>
@@ -305,9 +306,10 @@ bool merge_halves(const DecodeProblem& p, const Plan& plan) {
 }
 
 // ev_b / ev_e (optional) are recorded around the attention kernel, which runs
-// max(repeat, 1) times between them.
+// max(repeat, 1) times between them. used (optional): the problem with its
+// partial slots' addresses, for a kernel that reads them next.
 int run(const la_decode_args* a, hipStream_t stream, hipEvent_t ev_b = nullptr, hipEvent_t ev_e = nullptr,
-        int repeat = 1, bool coarse = false) {
+        int repeat = 1, bool coarse = false, DecodeProblem* used = nullptr) {
   if (repeat < 0) return LA_ERROR_INVALID_VALUE;
   DecodeProblem p;
   Plan plan;
@@ -398,6 +400,7 @@ int run(const la_decode_args* a, hipStream_t stream, hipEvent_t ev_b = nullptr, 
     }
     if (e != hipSuccess) return finish(e);
   }
+  if (used) *used = p;
   if (plan.proj_f32) return finish(launch_combine_project_f32(p, stream, merge_halves));
   if (plan.proj_mfma) return finish(launch_combine_project_mfma(p, stream, merge_halves, cu_count()));
   return finish(launch_combine_project(p, stream));
@@ -461,6 +464,600 @@ int scratch_ptr(void** out) {
   }
   *out = g_scratch_ptr[dev];
   return LA_SUCCESS;
+}
+
+// ---- prompts and shared prefixes ----------------------------------------------------------------------
+
+bool valid_out(int d) { return valid_dtype(d); }
+// Head shape of the expanded form's kernels.
+bool expanded_dims(const la_mla_config& c) {
+  return c.kv_lora_rank == 512 && c.qk_nope_head_dim == 128 && c.qk_rope_head_dim == 64 && c.v_head_dim == 128;
+}
+bool sixteen_bit(int d) { return d == LA_DTYPE_F16 || d == LA_DTYPE_BF16; }
+
+// Cuts a workspace into 256-byte aligned pieces; with a null base it only counts.
+struct Carve {
+  char* base;
+  size_t at = 0;
+  explicit Carve(void* ws) : base(reinterpret_cast<char*>(align_up(reinterpret_cast<uintptr_t>(ws)))) {}
+  void* take(size_t bytes) {
+    void* const p = base ? base + at : nullptr;
+    at += align_up(bytes);
+    return p;
+  }
+  size_t total() const { return at > 0 ? at + kAlign : 0; }  // the base may have to be aligned
+};
+
+// The caller's workspace, or one of `need` bytes taken and returned in the order of the stream.
+struct Scratch {
+  void* ws;
+  bool owned = false;
+  int status = LA_SUCCESS;
+  hipStream_t stream;
+  Scratch(void* given, size_t given_bytes, size_t need, hipStream_t st) : ws(given), stream(st) {
+    if (need == 0) return;
+    if (ws) {
+      if (given_bytes < need) status = LA_ERROR_WORKSPACE;
+    } else {
+      const hipError_t e = hipMallocAsync(&ws, need, st);
+      if (e != hipSuccess) status = record_hip(e);
+      else owned = true;
+    }
+  }
+  int finish(int st) {
+    if (!owned) return st;
+    const hipError_t f = hipFreeAsync(ws, stream);
+    return st == LA_SUCCESS && f != hipSuccess ? record_hip(f) : st;
+  }
+};
+int status_of(hipError_t e) { return e == hipSuccess ? (int)LA_SUCCESS : record_hip(e); }
+
+// Weights as the expanded form's products take them: 16-bit values of its
+// type, from 16-byte aligned rows; others are copied first.
+struct ExpandWeights {
+  const void* w;
+  int dtype;
+  void* copy;
+};
+bool weight_as_is(const void* w, int dtype, int f16) {
+  return dtype == (f16 ? LA_DTYPE_F16 : LA_DTYPE_BF16) && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+}
+
+// Gather and expansion of `heads` heads at a time, shared by prompts and prefixes.
+struct ExpandPlan {
+  ExpandProblem p{};
+  void* uk_copy = nullptr;
+  void* uv_copy = nullptr;
+  size_t copy_elems = 0;
+};
+void carve_expand(Carve& c, ExpandPlan& e, const void* W_UK, int uk_dtype, const void* W_UV, int uv_dtype, int nh) {
+  const size_t tiles = (size_t)e.p.src.num_tiles;
+  e.p.rows_c = c.take(tiles * kTileCBytes);
+  e.p.tile_rows = static_cast<int32_t*>(c.take(tiles * sizeof(int32_t)));
+  e.copy_elems = (size_t)nh * 128 * 512;
+  e.uk_copy = e.uv_copy = nullptr;
+  e.p.W_UK = W_UK;
+  e.p.W_UV = W_UV;
+  if (!weight_as_is(W_UK, uk_dtype, e.p.f16)) e.p.W_UK = e.uk_copy = c.take(e.copy_elems * 2);
+  if (!weight_as_is(W_UV, uv_dtype, e.p.f16)) e.p.W_UV = e.uv_copy = c.take(e.copy_elems * 2);
+}
+hipError_t start_expand(const ExpandPlan& e, const void* W_UK, int uk_dtype, const void* W_UV, int uv_dtype, bool copy_uk,
+                        bool copy_uv, hipStream_t stream) {
+  hipError_t r = launch_gather(e.p, stream);
+  if (r == hipSuccess && copy_uk) r = launch_convert(W_UK, uk_dtype, e.uk_copy, e.p.f16, (int64_t)e.copy_elems, stream);
+  if (r == hipSuccess && copy_uv) r = launch_convert(W_UV, uv_dtype, e.uv_copy, e.p.f16, (int64_t)e.copy_elems, stream);
+  return r;
+}
+
+enum PrefillForm { kPrefillNone = 0, kPrefillPlain = 1, kPrefillExpanded = 2, kPrefillAbsorbed = 3 };
+
+// Expanded keys and values of one launch at most (heads go in groups of it).
+constexpr size_t kMaxExpanded = (size_t)8 << 30;
+
+struct Prefill {
+  PrefillForm form = kPrefillNone;
+  QuerySource q{};
+  RowSource src{};
+  int block_size = 0, blocks_per_seq = 0;  // of the absorbed form
+  int64_t pool_rows = 0;
+  int splits = 1, group = 0;  // of the expanded form: key parts, heads at a time
+  int64_t q_tiles = 0;
+};
+
+int prepare_prefill(const la_prefill_args* a, Prefill* out) {
+  if (!a || !valid_cfg(&a->cfg) || !valid_cache_dtype(a->kv_dtype) || !valid_dtype(a->w_uk_dtype) ||
+      !valid_dtype(a->w_uv_dtype) || !valid_dtype(a->q_dtype) || !valid_out(a->out_dtype))
+    return LA_ERROR_INVALID_VALUE;
+  const la_mla_config& c = a->cfg;
+  if (a->num_seqs < 0 || a->tokens < 0 || a->total_rows < 0 || a->rope_rows < 0 || a->max_seq_rows < 0 ||
+      a->kernel_variant < 0 || a->kernel_variant > kPrefillAbsorbed || (a->rotate_q != 0 && a->rotate_q != 1))
+    return LA_ERROR_INVALID_VALUE;
+  if (a->num_seqs == INT32_MAX || a->tokens > INT32_MAX / c.num_heads) return LA_ERROR_INVALID_VALUE;
+  if (a->q_nope_token_stride < 0 || a->q_nope_head_stride < 0 || a->q_rope_token_stride < 0 || a->q_rope_head_stride < 0)
+    return LA_ERROR_INVALID_VALUE;
+  const bool paged = a->block_table != nullptr;
+  if (paged) {
+    if (a->block_size <= 0 || a->blocks_per_seq <= 0 || a->seq_offsets || !a->seq_lens ||
+        a->total_rows % a->block_size != 0 || (int64_t)a->blocks_per_seq * a->block_size > INT32_MAX ||
+        a->total_rows > (int64_t)UINT32_MAX || (a->num_seqs > 0 && a->total_rows < a->block_size))
+      return LA_ERROR_INVALID_VALUE;
+  } else if (a->seq_offsets) {
+    if (a->max_seq_rows != 0 || a->total_rows > INT32_MAX) return LA_ERROR_INVALID_VALUE;
+  } else if (a->seq_len < 0 || (int64_t)a->num_seqs * a->seq_len > a->total_rows) {
+    return LA_ERROR_INVALID_VALUE;
+  }
+  Prefill p;
+  p.form = kPrefillNone;
+  if (a->tokens == 0) {
+    *out = p;
+    return LA_SUCCESS;
+  }
+  if (a->num_seqs == 0 || (!a->q_offsets && a->tokens % a->num_seqs != 0)) return LA_ERROR_INVALID_VALUE;
+  if (!a->q_nope || !a->q_rope || !a->W_UK || !a->W_UV || !a->rope_cos || !a->rope_sin || !a->output ||
+      (a->total_rows > 0 && !a->kv_cache))
+    return LA_ERROR_INVALID_VALUE;
+
+  RowSource& r = p.src;
+  r.kv = a->kv_cache;
+  r.kv_dtype = a->kv_dtype;
+  r.row_elems = c.kv_lora_rank + c.qk_rope_head_dim;
+  r.total_rows = a->total_rows;
+  r.num_seqs = a->num_seqs;
+  r.offsets = a->seq_offsets;
+  r.lens = a->seq_lens;
+  r.cos = a->rope_cos;
+  r.sin = a->rope_sin;
+  r.rope_rows = a->rope_rows;
+  if (paged) {
+    r.block_table = a->block_table;
+    r.block_size = a->block_size;
+    r.blocks_per_seq = a->blocks_per_seq;
+    r.pool_blocks = a->total_rows / a->block_size;
+    r.region = a->blocks_per_seq * a->block_size;
+  } else if (!a->seq_offsets) {
+    r.region = r.stride_rows = a->seq_len;
+  }
+  if (!a->seq_offsets && a->max_seq_rows > 0) r.region = std::min(r.region, a->max_seq_rows);
+  r.num_tiles = source_tiles(r);
+
+  QuerySource& q = p.q;
+  q.q_nope = a->q_nope;
+  q.q_rope = a->q_rope;
+  q.dtype = a->q_dtype;
+  const bool nope_packed = a->q_nope_token_stride == 0 && a->q_nope_head_stride == 0;
+  const bool rope_packed = a->q_rope_token_stride == 0 && a->q_rope_head_stride == 0;
+  q.nope_stride = nope_packed ? (int64_t)c.num_heads * c.qk_nope_head_dim : a->q_nope_token_stride;
+  q.nope_head = nope_packed ? c.qk_nope_head_dim : a->q_nope_head_stride;
+  q.rope_stride = rope_packed ? (int64_t)c.num_heads * c.qk_rope_head_dim : a->q_rope_token_stride;
+  q.rope_head = rope_packed ? c.qk_rope_head_dim : a->q_rope_head_stride;
+  q.rotate = a->rotate_q;
+  q.tokens = a->tokens;
+  q.num_seqs = a->num_seqs;
+  q.offsets = a->q_offsets;
+  q.per_seq = a->q_offsets ? 0 : (int)(a->tokens / a->num_seqs);
+  q.prefix = a->prefix_lens;
+
+  const bool expanded_ok = expanded_dims(c) && (sixteen_bit(a->kv_dtype) || a->kv_dtype == LA_DTYPE_FP8_E4M3) &&
+                           device_is_gfx950() && (reinterpret_cast<uintptr_t>(a->output) & 15) == 0 &&
+                           r.num_tiles <= INT32_MAX / 128;
+  // The absorbed form's block tables: the cache's own, or identity blocks of equal regions.
+  if (paged) {
+    p.block_size = a->block_size;
+    p.pool_rows = a->total_rows;
+  } else if (!a->seq_offsets && a->seq_len > 0) {
+    p.block_size = a->seq_len % 64 == 0 ? 64 : a->seq_len % 32 == 0 ? 32 : a->seq_len;
+    p.pool_rows = (int64_t)a->num_seqs * a->seq_len;
+  }
+  bool absorbed_ok = p.block_size > 0 && r.region > 0 && p.pool_rows / p.block_size <= INT32_MAX;
+  if (absorbed_ok) {
+    p.blocks_per_seq = (r.region + p.block_size - 1) / p.block_size;
+    absorbed_ok = a->tokens * p.blocks_per_seq <= INT32_MAX &&
+                  (int64_t)p.blocks_per_seq * p.block_size <= INT32_MAX;
+  }
+  const bool plain_ok = generic_prompt_supported(c.kv_lora_rank, c.qk_rope_head_dim);
+  if (a->kernel_variant == kPrefillAbsorbed && !absorbed_ok) return LA_ERROR_NOT_SUPPORTED;
+  if (a->kernel_variant == kPrefillExpanded && !expanded_ok) return LA_ERROR_NOT_SUPPORTED;
+  if (a->kernel_variant == kPrefillPlain && !plain_ok) return LA_ERROR_NOT_SUPPORTED;
+  if (a->kernel_variant != 0) {
+    p.form = (PrefillForm)a->kernel_variant;
+  } else if (expanded_ok) {
+    // products per head: n tokens over L rows take 131072 n + 1088 n L absorbed, 131072 L + 320 n L expanded
+    const double n = (double)a->tokens / a->num_seqs, rows = (double)std::max(r.region, 1);
+    p.form = absorbed_ok && n * (131072. + 768. * rows) < 131072. * rows ? kPrefillAbsorbed : kPrefillExpanded;
+  } else if (absorbed_ok) {
+    p.form = kPrefillAbsorbed;
+  } else if (plain_ok) {
+    p.form = kPrefillPlain;
+  } else {
+    return LA_ERROR_NOT_SUPPORTED;
+  }
+
+  if (p.form == kPrefillExpanded) {
+    const size_t head_bytes = (size_t)r.num_tiles * kTileKBytes * 2;
+    p.group = (int)std::min<size_t>(c.num_heads, std::max<size_t>(1, head_bytes ? kMaxExpanded / head_bytes : c.num_heads));
+    p.q_tiles = query_tiles(q, prompt_query_rows());
+    // few query tiles leave CUs idle: their keys are cut into parts of at least four tiles
+    const int64_t blocks = p.q_tiles * p.group;
+    const int64_t tiles = a->seq_offsets ? a->total_rows / a->num_seqs / kTileKeys + 1 : r.num_tiles / a->num_seqs;
+    const int64_t want = (2 * cu_count() + blocks - 1) / blocks;
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, tiles / 4, 32}));
+    if ((int64_t)p.group * p.splits * p.q_tiles > INT32_MAX - 8) return LA_ERROR_NOT_SUPPORTED;
+  }
+  *out = p;
+  return LA_SUCCESS;
+}
+
+// The decode step of the absorbed form: every token a sequence with its own visible rows.
+la_decode_args token_step(const la_prefill_args* a, const Prefill& p, const float* q_nope, const float* q_rope,
+                          const int32_t* lens, const int32_t* table, float* out, void* ws, size_t ws_bytes) {
+  la_decode_args d{};
+  d.kv_cache = a->kv_cache;
+  d.kv_dtype = a->kv_dtype;
+  d.total_rows = p.pool_rows;
+  d.num_seqs = (int32_t)a->tokens;
+  d.queries_per_seq = 1;
+  d.q_nope = q_nope;
+  d.q_rope = q_rope;
+  d.W_UK = a->W_UK;
+  d.w_uk_dtype = a->w_uk_dtype;
+  d.W_UV = a->W_UV;
+  d.w_uv_dtype = a->w_uv_dtype;
+  d.rope_cos = a->rope_cos;
+  d.rope_sin = a->rope_sin;
+  d.rope_rows = a->rope_rows;
+  d.output = out;
+  d.cfg = a->cfg;
+  d.seq_lens = lens;
+  d.block_table = table;
+  d.block_size = p.block_size;
+  d.blocks_per_seq = p.blocks_per_seq;
+  d.workspace = ws;
+  d.workspace_bytes = ws_bytes;
+  return d;
+}
+
+// Runs the call, or with run = false counts its workspace into *need.
+int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need) {
+  const hipStream_t stream = static_cast<hipStream_t>(stream_v);
+  Prefill p;
+  const int st = prepare_prefill(a, &p);
+  if (st != LA_SUCCESS) return st;
+  if (need) *need = 0;
+  if (p.form == kPrefillNone) return LA_SUCCESS;
+  const la_mla_config& c = a->cfg;
+  const int nh = c.num_heads;
+  const float scale_log2 = (float)(kLog2e / std::sqrt((double)(c.qk_nope_head_dim + c.qk_rope_head_dim)));
+  const int64_t rows = a->tokens * nh;
+
+  // the layout is the same whether counted or carved
+  ExpandPlan e;
+  e.p.src = p.src;
+  e.p.f16 = a->kv_dtype == LA_DTYPE_F16;
+  float *part_o = nullptr, *part_lse = nullptr, *q_nope = nullptr, *q_rope = nullptr, *q_abs = nullptr, *out32 = nullptr;
+  int32_t *lens = nullptr, *table = nullptr;
+  void* step_ws = nullptr;
+  size_t step_bytes = 0;
+  const bool q32 = a->q_dtype == LA_DTYPE_F32;
+  const bool nope_as_is = q32 && p.q.nope_head == c.qk_nope_head_dim && p.q.nope_stride == (int64_t)nh * p.q.nope_head;
+  const bool rope_as_is = q32 && !a->rotate_q && p.q.rope_head == c.qk_rope_head_dim &&
+                          p.q.rope_stride == (int64_t)nh * p.q.rope_head;
+  auto carve = [&](void* ws) {
+    Carve v(ws);
+    if (p.form == kPrefillExpanded) {
+      carve_expand(v, e, a->W_UK, a->w_uk_dtype, a->W_UV, a->w_uv_dtype, nh);
+      const size_t tiles = (size_t)p.src.num_tiles;
+      e.p.rope = v.take(tiles * kTileRBytes);
+      e.p.kx = v.take(tiles * p.group * kTileKBytes);
+      e.p.vx = v.take(tiles * p.group * kTileKBytes);
+      if (p.splits > 1) {
+        part_o = static_cast<float*>(v.take((size_t)p.splits * rows * 128 * sizeof(float)));
+        part_lse = static_cast<float*>(v.take((size_t)p.splits * rows * sizeof(float)));
+      }
+    } else {
+      if (!nope_as_is) q_nope = static_cast<float*>(v.take((size_t)rows * c.qk_nope_head_dim * sizeof(float)));
+      if (p.form == kPrefillPlain) {
+        q_abs = static_cast<float*>(v.take((size_t)rows * c.kv_lora_rank * sizeof(float)));
+      } else {
+        if (!rope_as_is) q_rope = static_cast<float*>(v.take((size_t)rows * c.qk_rope_head_dim * sizeof(float)));
+        lens = static_cast<int32_t*>(v.take((size_t)a->tokens * sizeof(int32_t)));
+        table = static_cast<int32_t*>(v.take((size_t)a->tokens * p.blocks_per_seq * sizeof(int32_t)));
+        if (a->out_dtype != LA_DTYPE_F32) out32 = static_cast<float*>(v.take((size_t)rows * c.v_head_dim * sizeof(float)));
+        // (the addresses are those of a workspace of any base: only their alignment matters to the plan)
+        alignas(256) static const char any[256] = {0};
+        const float* f = reinterpret_cast<const float*>(any);
+        const la_decode_args d =
+            token_step(a, p, nope_as_is ? static_cast<const float*>(a->q_nope) : f,
+                       rope_as_is ? static_cast<const float*>(a->q_rope) : f, reinterpret_cast<const int32_t*>(any),
+                       reinterpret_cast<const int32_t*>(any), const_cast<float*>(f), nullptr, 0);
+        step_bytes = la_mla_decode_workspace_size(&d);
+        step_ws = v.take(step_bytes);
+      }
+    }
+    return v.total();
+  };
+  const size_t total = carve(nullptr);
+  if (p.form == kPrefillAbsorbed && step_bytes == 0) return LA_ERROR_NOT_SUPPORTED;
+  if (need) *need = total;
+  if (!run_it) return LA_SUCCESS;
+  Scratch scratch(a->workspace, a->workspace_bytes, total, stream);
+  if (scratch.status != LA_SUCCESS) return scratch.status;
+  carve(scratch.ws);
+
+  if (p.form == kPrefillExpanded) {
+    hipError_t r = start_expand(e, a->W_UK, a->w_uk_dtype, a->W_UV, a->w_uv_dtype, e.uk_copy, e.uv_copy, stream);
+    PromptProblem m{};
+    m.q = p.q;
+    m.src = p.src;
+    m.f16 = e.p.f16;
+    m.kx = e.p.kx;
+    m.vx = e.p.vx;
+    m.rope = e.p.rope;
+    m.nh = nh;
+    m.scale_log2 = scale_log2;
+    m.out = a->output;
+    m.out_dtype = a->out_dtype;
+    m.splits = p.splits;
+    m.part_o = part_o;
+    m.part_lse = part_lse;
+    m.q_tiles = p.q_tiles;
+    m.nope_vec = q_vec(p.q.q_nope, p.q.dtype, p.q.nope_stride, p.q.nope_head);
+    m.rope_vec = q_vec(p.q.q_rope, p.q.dtype, p.q.rope_stride, p.q.rope_head);
+    for (int h = 0; h < nh && r == hipSuccess; h += p.group) {
+      e.p.head0 = m.head0 = h;
+      e.p.heads = m.heads = std::min(p.group, nh - h);
+      r = launch_expand(e.p, stream, cu_count());
+      if (r == hipSuccess) r = launch_prompt(m, stream);
+    }
+    if (r == hipSuccess && p.splits > 1) {
+      JoinProblem j{};
+      j.rows = rows;
+      j.nh = nh;
+      j.dv = 128;
+      j.splits = p.splits;
+      j.part_o = part_o;
+      j.part_lse = part_lse;
+      j.out = a->output;
+      j.out_dtype = a->out_dtype;
+      r = launch_join(j, stream);
+    }
+    return scratch.finish(status_of(r));
+  }
+
+  TokenProblem t{};
+  t.q = p.q;
+  t.src = p.src;
+  t.nh = nh;
+  t.dn = c.qk_nope_head_dim;
+  t.dR = c.qk_rope_head_dim;
+  t.q_nope = q_nope;
+  t.q_rope = q_rope;
+  t.lens = lens;
+  t.table = table;
+  t.block_size = p.block_size;
+  t.blocks_per_seq = p.blocks_per_seq;
+  const float* const qn = nope_as_is ? static_cast<const float*>(a->q_nope) : q_nope;
+  if (p.form == kPrefillPlain) {
+    hipError_t r = q_nope ? launch_tokens(t, stream) : hipSuccess;
+    if (r != hipSuccess) return scratch.finish(record_hip(r));
+    const int s2 = la_absorb_q(qn, a->W_UK, a->w_uk_dtype, q_abs, (int)a->tokens, &c, stream_v);
+    if (s2 != LA_SUCCESS) return scratch.finish(s2);
+    GenericPrompt g{};
+    g.q = p.q;
+    g.src = p.src;
+    g.q_abs = q_abs;
+    g.W_UV = a->W_UV;
+    g.wuv_dtype = a->w_uv_dtype;
+    g.nh = nh;
+    g.dc = c.kv_lora_rank;
+    g.dR = c.qk_rope_head_dim;
+    g.dv = c.v_head_dim;
+    g.scale_log2 = scale_log2;
+    g.out = a->output;
+    g.out_dtype = a->out_dtype;
+    return scratch.finish(status_of(launch_generic_prompt(g, stream)));
+  }
+  hipError_t r = launch_tokens(t, stream);
+  if (r != hipSuccess) return scratch.finish(record_hip(r));
+  float* const out = out32 ? out32 : static_cast<float*>(a->output);
+  const la_decode_args d = token_step(a, p, qn, rope_as_is ? static_cast<const float*>(a->q_rope) : q_rope, lens, table,
+                                      out, step_ws, step_bytes);
+  int s3 = run(&d, stream);
+  if (s3 == LA_SUCCESS && out32) s3 = status_of(launch_cast(out32, a->output, a->out_dtype, rows * c.v_head_dim, stream));
+  return scratch.finish(s3);
+}
+
+// ---- a prefix, expanded once --------------------------------------------------------------------------
+
+RowSource prefix_source(const void* rows, int dtype, int n, const la_mla_config& c, const float* cos, const float* sin,
+                        int64_t rope_rows) {
+  RowSource r{};
+  r.kv = rows;
+  r.kv_dtype = dtype;
+  r.row_elems = c.kv_lora_rank + c.qk_rope_head_dim;
+  r.total_rows = n;
+  r.num_seqs = 1;
+  r.region = r.stride_rows = n;
+  r.cos = cos;
+  r.sin = sin;
+  r.rope_rows = rope_rows;
+  r.num_tiles = source_tiles(r);
+  return r;
+}
+
+int expand(const la_expand_args* a, hipStream_t stream, bool run_it, size_t* need) {
+  if (!a || !valid_cfg(&a->cfg) || !valid_cache_dtype(a->kv_dtype) || !valid_dtype(a->w_uk_dtype) ||
+      !valid_dtype(a->w_uv_dtype) || a->rows < 0 || a->rope_rows < 0)
+    return LA_ERROR_INVALID_VALUE;
+  if (need) *need = 0;
+  if (!expanded_dims(a->cfg) || a->kv_dtype == LA_DTYPE_F32) return LA_ERROR_NOT_SUPPORTED;
+  if (a->rows == 0) return LA_SUCCESS;
+  if (!a->kv_cache || !a->W_UK || !a->W_UV || !a->rope_cos || !a->rope_sin) return LA_ERROR_INVALID_VALUE;
+  ExpandPlan e;
+  e.p.src = prefix_source(a->kv_cache, a->kv_dtype, a->rows, a->cfg, a->rope_cos, a->rope_sin, a->rope_rows);
+  e.p.f16 = a->kv_dtype == LA_DTYPE_F16;
+  auto carve = [&](void* ws) {
+    Carve v(ws);
+    carve_expand(v, e, a->W_UK, a->w_uk_dtype, a->W_UV, a->w_uv_dtype, a->cfg.num_heads);
+    return v.total();
+  };
+  const size_t total = carve(nullptr);
+  if (need) *need = total;
+  if (!run_it) return LA_SUCCESS;
+  if (!a->expanded || (reinterpret_cast<uintptr_t>(a->expanded) & (kAlign - 1)) != 0 ||
+      a->expanded_bytes < la_expanded_size(a->rows, &a->cfg))
+    return LA_ERROR_INVALID_VALUE;
+  if (!device_is_gfx950()) return LA_ERROR_NOT_SUPPORTED;
+  Scratch scratch(a->workspace, a->workspace_bytes, total, stream);
+  if (scratch.status != LA_SUCCESS) return scratch.status;
+  carve(scratch.ws);
+  const size_t kv = (size_t)a->cfg.num_heads * e.p.src.num_tiles * kTileKBytes;
+  e.p.kx = a->expanded;
+  e.p.vx = static_cast<char*>(a->expanded) + kv;
+  e.p.rope = static_cast<char*>(a->expanded) + 2 * kv;
+  e.p.head0 = 0;
+  e.p.heads = a->cfg.num_heads;
+  hipError_t r = start_expand(e, a->W_UK, a->w_uk_dtype, a->W_UV, a->w_uv_dtype, e.uk_copy, e.uv_copy, stream);
+  if (r == hipSuccess) r = launch_expand(e.p, stream, cu_count());
+  return scratch.finish(status_of(r));
+}
+
+// ---- decode behind a shared prefix --------------------------------------------------------------------
+
+int decode_shared(const la_shared_args* a, hipStream_t stream, bool run_it, size_t* need) {
+  if (!a || !valid_cfg(&a->own.cfg)) return LA_ERROR_INVALID_VALUE;
+  const la_mla_config& c = a->own.cfg;
+  const int nh = c.num_heads;
+  if (!valid_out(a->out_dtype) || a->prefix_len < 0 || a->kernel_variant < 0 || a->kernel_variant > 2 ||
+      a->own.num_seqs < 0 || a->own.queries_per_seq < 1 || a->own.q_absorbed || a->own.rope_rows < 0)
+    return LA_ERROR_INVALID_VALUE;
+  const int64_t tokens = (int64_t)a->own.num_seqs * a->own.queries_per_seq;
+  if (tokens > INT32_MAX / nh) return LA_ERROR_INVALID_VALUE;
+  if (need) *need = 0;
+  if (tokens == 0) return LA_SUCCESS;
+  if (!a->own.q_nope || !a->own.q_rope || !a->output || !a->own.rope_cos || !a->own.rope_sin || !a->own.W_UK ||
+      !a->own.W_UV || (a->prefix_len > 0 && !a->prefix))
+    return LA_ERROR_INVALID_VALUE;
+  const int P = a->prefix_len;
+  const int64_t half = c.qk_rope_head_dim / 2;
+
+  la_decode_args own = a->own;
+  // own rows start at position P; tables that end before it give their last row, as everywhere
+  const int64_t first = own.rope_rows > 0 ? std::min<int64_t>(P, own.rope_rows - 1) : P;
+  own.rope_cos += first * half;
+  own.rope_sin += first * half;
+  if (own.rope_rows > 0) own.rope_rows -= first;
+  own.chunk_rows = own.kernel_variant = 0;
+  own.workspace = nullptr;
+  own.workspace_bytes = 0;
+  alignas(256) static const char any[256] = {0};  // stands for an aligned address while sizes are counted
+  own.output = reinterpret_cast<float*>(const_cast<char*>(any));
+
+  const bool expanded_ok = a->expanded && (reinterpret_cast<uintptr_t>(a->expanded) & (kAlign - 1)) == 0 &&
+                           expanded_dims(c) && own.kv_dtype != LA_DTYPE_F32 && device_is_gfx950();
+  if (a->kernel_variant == 2 && !expanded_ok) return LA_ERROR_NOT_SUPPORTED;
+  const bool expanded = P > 0 && expanded_ok && (a->kernel_variant == 2 || (a->kernel_variant == 0 && tokens > 48));
+
+  PromptProblem m{};
+  la_decode_args pre{};
+  size_t pre_bytes = 0;
+  if (expanded) {
+    m.src = prefix_source(a->prefix, own.kv_dtype, P, c, a->own.rope_cos, a->own.rope_sin, a->own.rope_rows);
+    m.q.q_nope = own.q_nope;
+    m.q.q_rope = own.q_rope;
+    m.q.dtype = LA_DTYPE_F32;
+    m.q.nope_head = c.qk_nope_head_dim;
+    m.q.nope_stride = (int64_t)nh * c.qk_nope_head_dim;
+    m.q.rope_head = c.qk_rope_head_dim;
+    m.q.rope_stride = (int64_t)nh * c.qk_rope_head_dim;
+    m.q.tokens = tokens;
+    m.q.num_seqs = 1;
+    m.q.per_seq = (int)tokens;
+    m.q.all = 1;
+    m.f16 = own.kv_dtype == LA_DTYPE_F16;
+    m.nh = m.heads = nh;
+    m.scale_log2 = (float)(kLog2e / std::sqrt((double)(c.qk_nope_head_dim + c.qk_rope_head_dim)));
+    m.out_dtype = LA_DTYPE_F32;
+    m.q_tiles = query_tiles(m.q, prompt_query_rows());
+    m.nope_vec = q_vec(m.q.q_nope, m.q.dtype, m.q.nope_stride, m.q.nope_head);
+    m.rope_vec = q_vec(m.q.q_rope, m.q.dtype, m.q.rope_stride, m.q.rope_head);
+    const int64_t blocks = m.q_tiles * nh;
+    m.splits = (int)std::max<int64_t>(
+        2, std::min<int64_t>({(2 * cu_count() + blocks - 1) / blocks, m.src.num_tiles / 4, 32}));
+  } else if (P > 0) {
+    pre = a->own;
+    pre.kv_cache = a->prefix;
+    pre.total_rows = pre.seq_len = P;
+    pre.num_seqs = 1;
+    pre.queries_per_seq = (int32_t)tokens;
+    pre.seq_offsets = pre.seq_lens = pre.block_table = nullptr;
+    pre.block_size = pre.blocks_per_seq = 0;
+    pre.chunk_rows = pre.kernel_variant = 0;
+    pre.workspace = nullptr;
+    pre.workspace_bytes = 0;
+    pre.output = own.output;
+  }
+  // validates both steps
+  la::DecodeProblem probe;
+  Plan plan;
+  int st = prepare(&own, &probe, &plan);
+  if (st == LA_SUCCESS && pre.num_seqs > 0) st = prepare(&pre, &probe, &plan);
+  if (st != LA_SUCCESS) return st;
+  const size_t own_bytes = la_mla_decode_workspace_size(&own);
+  if (pre.num_seqs > 0) pre_bytes = la_mla_decode_workspace_size(&pre);
+
+  const int64_t rows = tokens * nh;
+  void *own_ws = nullptr, *pre_ws = nullptr;
+  float *own_out = nullptr, *pre_out = nullptr;
+  auto carve = [&](void* ws) {
+    Carve v(ws);
+    own_ws = v.take(own_bytes);
+    own_out = static_cast<float*>(v.take((size_t)rows * c.v_head_dim * sizeof(float)));
+    if (expanded) {
+      m.part_o = static_cast<float*>(v.take((size_t)m.splits * rows * 128 * sizeof(float)));
+      m.part_lse = static_cast<float*>(v.take((size_t)m.splits * rows * sizeof(float)));
+    } else if (P > 0) {
+      pre_ws = v.take(pre_bytes);
+      pre_out = static_cast<float*>(v.take((size_t)rows * c.v_head_dim * sizeof(float)));
+    }
+    return v.total();
+  };
+  const size_t total = carve(nullptr);
+  if (need) *need = total;
+  if (!run_it) return LA_SUCCESS;
+  Scratch scratch(a->workspace, a->workspace_bytes, total, stream);
+  if (scratch.status != LA_SUCCESS) return scratch.status;
+  carve(scratch.ws);
+  JoinProblem j{};
+  j.rows = rows;
+  j.nh = nh;
+  j.dv = c.v_head_dim;
+  j.out = a->output;
+  j.out_dtype = a->out_dtype;
+  if (expanded) {
+    const size_t kv = (size_t)nh * m.src.num_tiles * kTileKBytes;
+    m.kx = a->expanded;
+    m.vx = static_cast<const char*>(a->expanded) + kv;
+    m.rope = static_cast<const char*>(a->expanded) + 2 * kv;
+    st = status_of(launch_prompt(m, stream));
+    j.splits = m.splits;
+    j.part_o = m.part_o;
+    j.part_lse = m.part_lse;
+  } else if (P > 0) {
+    pre.output = pre_out;
+    pre.workspace = pre_ws;
+    pre.workspace_bytes = pre_bytes;
+    st = run(&pre, stream, nullptr, nullptr, 1, false, &j.step[1]);
+    j.step_out[1] = pre_out;
+  }
+  if (st == LA_SUCCESS) {
+    own.output = own_out;
+    own.workspace = own_ws;
+    own.workspace_bytes = own_bytes;
+    st = run(&own, stream, nullptr, nullptr, 1, false, &j.step[0]);
+    j.step_out[0] = own_out;
+  }
+  if (st == LA_SUCCESS) st = status_of(launch_join(j, stream));
+  return scratch.finish(st);
 }
 
 }  // namespace
@@ -759,6 +1356,37 @@ int la_absorb_q(const float* q_nope, const void* W_UK, int w_uk_dtype, float* q_
                       : la::launch_absorb(q_nope, W_UK, w_uk_dtype, q_absorbed, tokens, cfg->num_heads,
                                           cfg->qk_nope_head_dim, cfg->kv_lora_rank, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? (int)LA_SUCCESS : la::record_hip(e);
+}
+
+int la_mla_prefill(const la_prefill_args* args, void* stream) { return la::prefill(args, stream, true, nullptr); }
+
+size_t la_mla_prefill_workspace_size(const la_prefill_args* args) {
+  size_t need = 0;
+  return la::prefill(args, nullptr, false, &need) == LA_SUCCESS ? need : 0;
+}
+
+int la_expand_prefix(const la_expand_args* args, void* stream) {
+  return la::expand(args, static_cast<hipStream_t>(stream), true, nullptr);
+}
+
+size_t la_expand_prefix_workspace_size(const la_expand_args* args) {
+  size_t need = 0;
+  return la::expand(args, nullptr, false, &need) == LA_SUCCESS ? need : 0;
+}
+
+size_t la_expanded_size(int32_t rows, const la_mla_config* cfg) {
+  if (!la::valid_cfg(cfg) || rows < 0 || !la::expanded_dims(*cfg)) return 0;
+  const size_t tiles = ((size_t)rows + la::kTileKeys - 1) / la::kTileKeys;
+  return tiles * (2 * (size_t)cfg->num_heads * la::kTileKBytes + la::kTileRBytes);
+}
+
+int la_mla_decode_shared(const la_shared_args* args, void* stream) {
+  return la::decode_shared(args, static_cast<hipStream_t>(stream), true, nullptr);
+}
+
+size_t la_mla_decode_shared_workspace_size(const la_shared_args* args) {
+  size_t need = 0;
+  return la::decode_shared(args, nullptr, false, &need) == LA_SUCCESS ? need : 0;
 }
 
 }  // extern "C"

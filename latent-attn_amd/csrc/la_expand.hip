@@ -1,0 +1,288 @@
+// Latent rows -> per-head keys and values (the expanded form that prompts and
+// shared prefixes attend over):
+//   K[pos,h] = c_t[pos] . W_UK[h]^T   V[pos,h] = c_t[pos] . W_UV[h]^T   R[pos] = RoPE(k_rope[pos], pos)
+// gather_kernel reads the cache once, whatever its layout and type, and
+// writes 16-bit latent tiles of 64 rows (zeros past a sequence's last row, so
+// nothing unfilled is ever an operand) and the rotated rope keys; the product
+// then runs over dense rows, with sums in fp32 and one rounding to 16 bits, as
+// the matrix instructions of the attention take them.
+#include "la_prompt.hpp"
+
+namespace la {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) char lchar;
+
+template <typename T>
+struct Mm;
+template <>
+struct Mm<__hip_bfloat16> {
+  typedef bf16x8 vec;
+  typedef __bf16 elem;
+  static __device__ inline f32x16 mma(vec a, vec b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mm<__half> {
+  typedef f16x8 vec;
+  typedef _Float16 elem;
+  static __device__ inline f32x16 mma(vec a, vec b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+// ---- gather --------------------------------------------------------------------
+
+// Eight cache elements as T (an 8-bit cache: bf16, exact).
+template <typename KT, typename T>
+__device__ inline typename Mm<T>::vec load8(const KT* p) {
+  typename Mm<T>::vec v;
+  if constexpr (sizeof(KT) == 2) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = __builtin_bit_cast(typename Mm<T>::elem, p[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (typename Mm<T>::elem)to_f32(p[e]);
+  }
+  return v;
+}
+template <typename KT, typename T, bool kAligned>
+__device__ inline typename Mm<T>::vec load8_row(const KT* p) {
+  if constexpr (kAligned && sizeof(KT) == 2) return *reinterpret_cast<const typename Mm<T>::vec*>(p);
+  if constexpr (kAligned && sizeof(KT) == 1) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    KT b[8];
+    __builtin_memcpy(b, &w, 8);
+    return load8<KT, T>(b);
+  }
+  return load8<KT, T>(p);
+}
+
+// One workgroup per tile.
+template <typename KT, typename T, bool kAligned>
+__global__ __launch_bounds__(256) void gather_kernel(ExpandProblem p) {
+  typedef typename Mm<T>::vec vec;
+  typedef typename Mm<T>::elem elem;
+  typedef elem vec4 __attribute__((ext_vector_type(4)));
+  const int64_t tile = blockIdx.x;
+  const int s = source_find(p.src, tile);
+  const int64_t t = tile - source_tile(p.src, s);
+  const int L = source_rows(p.src, s);
+  const int rows = (int)clamp64(L - t * kTileKeys, 0, kTileKeys);
+  if (threadIdx.x == 0) p.tile_rows[tile] = rows;
+  if (rows == 0) return;
+  const int pos0 = (int)t * kTileKeys;
+  const KT* kv = static_cast<const KT*>(p.src.kv);
+  vec* const c_out = reinterpret_cast<vec*>(static_cast<char*>(p.rows_c) + tile * kTileCBytes);
+#pragma unroll 4
+  for (int i = threadIdx.x; i < kTileKeys * 64; i += 256) {
+    const int r = i >> 6, ch = i & 63;
+    vec v = {};
+    if (r < rows) v = load8_row<KT, T, kAligned>(kv + source_row(p.src, s, pos0 + r) * p.src.row_elems + 8 * ch);
+    c_out[i] = v;
+  }
+  elem* const r_out = reinterpret_cast<elem*>(static_cast<char*>(p.rope) + tile * kTileRBytes);
+  for (int i = threadIdx.x; i < kTileKeys * 8; i += 256) {
+    const int r = i >> 3, d = 4 * (i & 7);  // dims d .. d+3 and their partners d + 32 ..
+    vec4 a = {}, b = {};
+    if (r < rows) {
+      const KT* k = kv + source_row(p.src, s, pos0 + r) * p.src.row_elems + 512 + d;
+      const int64_t at = source_rope_row(p.src, pos0 + r) * 32 + d;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float k0 = to_f32(k[e]), k1 = to_f32(k[e + 32]), c = p.src.cos[at + e], sn = p.src.sin[at + e];
+        a[e] = (elem)(k0 * c - k1 * sn);
+        b[e] = (elem)(k0 * sn + k1 * c);
+      }
+    }
+    elem* const o = r_out + (r >> 5) * (4 * 512) + operand_elem(r, d & 15);
+    *reinterpret_cast<vec4*>(o + (d >> 4) * 512) = a;
+    *reinterpret_cast<vec4*>(o + ((d >> 4) + 2) * 512) = b;
+  }
+}
+
+__global__ __launch_bounds__(256) void convert_kernel(const void* src, int src_dtype, uint16_t* dst, int f16, int64_t n) {
+  const int64_t step = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
+    const float x = load_any(src, src_dtype, i);
+    dst[i] = f16 ? __builtin_bit_cast(uint16_t, (_Float16)x) : __builtin_bit_cast(uint16_t, (__bf16)x);
+  }
+}
+
+// ---- expand ----------------------------------------------------------------------
+
+// One head's 256 weight rows (128 of W_UK, then 128 of W_UV) times kPos rows.
+// 8 waves: a quarter of the weight rows (0, 1: K dims; 2, 3: V dims) by half of
+// the positions each. Stages of 32 latent columns, chunk j of row r at j ^ sw(r).
+constexpr int kDc = 512;
+constexpr int kBk = 32;
+constexpr int kStages = 3;
+constexpr int kNRows = 256;
+__device__ inline int sw(int r) { return (r >> 2) & 3; }
+
+// The products and stores of one wave (kV: of V dims). Both kinds have the
+// same barriers; each has its own accumulators, since a branch around the
+// products alone made the compiler copy and spill them.
+template <typename T, int kPb, bool kV>
+__device__ inline void expand_wave(const ExpandProblem& p, const char* const (&src)[(kPb + 4) / 2], lchar* L, int lane,
+                                   int wave, int h, int64_t tile0) {
+  typedef typename Mm<T>::vec vec;
+  typedef typename Mm<T>::elem elem;
+  constexpr int kPos = 64 * kPb;
+  constexpr int kStageBytes = (kPos + kNRows) * kBk * 2;
+  constexpr int kCopies = (kPb + 4) / 2;
+  constexpr int stages = kDc / kBk;
+  auto issue = [&](int k) {
+    const int buf = (k % kStages) * kStageBytes;
+    const int kk = min(k, stages - 1);  // past the end: the last stage again, never read
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i)
+      __builtin_amdgcn_global_load_lds(src[i] + kk * (kBk * 2), (lds_void*)(L + buf + 1024 * (kCopies * wave + i)), 16, 0, 0);
+  };
+  const int wn = wave & 3, wp = wave >> 2;  // weight quarter, position half
+  const int r32 = lane & 31, g = lane >> 5;
+  f32x16 acc[kPb][2] = {};
+  issue(0);
+  issue(1);
+  for (int k = 0; k < stages; ++k) {
+    __builtin_amdgcn_s_waitcnt(0x0F70 | kCopies);  // this wave's copies of stage k have landed
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // everyone's; stage k - 1 is read
+    issue(k + 2);
+    const lchar* S = L + (k % kStages) * kStageBytes;
+#pragma unroll
+    for (int ks = 0; ks < kBk / 16; ++ks) {
+      vec w[2], x[kPb];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = kPos + 64 * wn + 32 * j + r32;
+        w[j] = *reinterpret_cast<const __attribute__((address_space(3))) vec*>(S + r * 64 + 16 * ((2 * ks + g) ^ sw(r)));
+      }
+#pragma unroll
+      for (int i = 0; i < kPb; ++i) {
+        const int r = 32 * kPb * wp + 32 * i + r32;
+        x[i] = *reinterpret_cast<const __attribute__((address_space(3))) vec*>(S + r * 64 + 16 * ((2 * ks + g) ^ sw(r)));
+      }
+#pragma unroll
+      for (int i = 0; i < kPb; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          acc[i][j] = kV ? Mm<T>::mma(x[i], w[j], acc[i][j]) : Mm<T>::mma(w[j], x[i], acc[i][j]);
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // the copies past the end have landed: the workgroup may end
+#pragma unroll
+  for (int i = 0; i < kPb; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) settle(acc[i][j]);
+  // registers 8 q .. 8 q + 7 of a block are one operand element group (operand
+  // order, la_prompt.hpp): K: a step of 16 dims; V: of 16 keys
+#pragma unroll
+  for (int i = 0; i < kPb; ++i) {
+    const int pb = kPb * wp + i;  // block of 32 positions
+    const int64_t tile = tile0 + pb / 2;
+    if (tile >= p.src.num_tiles) continue;
+    char* const out = static_cast<char*>(kV ? p.vx : p.kx) + ((int64_t)h * p.src.num_tiles + tile) * kTileKBytes;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        vec v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (elem)acc[i][j][8 * q + e];
+        const int db = 2 * (wn & 1) + j;  // block of 32 dims
+        const int piece = kV ? 4 * db + 2 * (pb & 1) + q : 8 * (pb & 1) + 2 * db + q;
+        *reinterpret_cast<vec*>(out + piece * 1024 + 16 * lane) = v;
+      }
+  }
+}
+
+template <typename T, int kPb>  // kPb blocks of 32 positions per wave, kPb tiles per workgroup
+__global__ __launch_bounds__(512, 2) void expand_kernel(ExpandProblem p) {
+  constexpr int kPos = 64 * kPb;
+  constexpr int kCopies = (kPb + 4) / 2;  // of 1 KB (16 rows) per wave and stage
+  static_assert(kCopies * 8 * 16 == kPos + kNRows, "every row of a stage is copied once");
+  extern __shared__ __attribute__((aligned(1024))) char expand_lds[];
+  lchar* const L = (lchar*)expand_lds;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  // an XCD (id % 8) takes every eighth head and goes through them per position
+  // block: its weights stay in its L2 and each block's rows are fetched once
+  const int nh8 = (p.heads + 7) / 8, x8 = blockIdx.x & 7, k8 = blockIdx.x >> 3;
+  const int h = x8 + 8 * (k8 % nh8);
+  const int64_t tile0 = (int64_t)(k8 / nh8) * kPb;
+  if (h >= p.heads) return;
+  int any = 0;
+#pragma unroll
+  for (int i = 0; i < kPb; ++i) any |= tile0 + i < p.src.num_tiles ? p.tile_rows[tile0 + i] : 0;
+  if (any == 0) return;
+  const int64_t row_last = p.src.num_tiles * kTileKeys - 1;
+  const char* const WK = static_cast<const char*>(p.W_UK) + (int64_t)(p.head0 + h) * 128 * kDc * 2;
+  const char* const WV = static_cast<const char*>(p.W_UV) + (int64_t)(p.head0 + h) * 128 * kDc * 2;
+  const char* src[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    const int r = 16 * (kCopies * wave + i) + (lane >> 2);
+    const int64_t xr = tile0 * kTileKeys + r;
+    const char* row = r < kPos ? static_cast<const char*>(p.rows_c) + (xr < row_last ? xr : row_last) * (kDc * 2)
+                      : r < kPos + 128 ? WK + (int64_t)(r - kPos) * (kDc * 2)
+                                       : WV + (int64_t)(r - kPos - 128) * (kDc * 2);
+    src[i] = row + 16 * ((lane & 3) ^ sw(r));
+  }
+  if ((wave & 3) >= 2) expand_wave<T, kPb, true>(p, src, L, lane, wave, h, tile0);
+  else expand_wave<T, kPb, false>(p, src, L, lane, wave, h, tile0);
+}
+
+template <typename T, int kPb>
+hipError_t expand_pb(const ExpandProblem& p, hipStream_t stream) {
+  constexpr int lds = kStages * (64 * kPb + kNRows) * kBk * 2;
+  static OncePerDevice once;
+  hipError_t e = allow_lds(once, reinterpret_cast<const void*>(expand_kernel<T, kPb>), lds);
+  if (e != hipSuccess) return e;
+  const int64_t blocks = 8 * (int64_t)((p.heads + 7) / 8) * ((p.src.num_tiles + kPb - 1) / kPb);
+  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((expand_kernel<T, kPb>), dim3((unsigned)blocks), dim3(512), lds, stream, p);
+  return hipGetLastError();
+}
+
+template <typename KT, typename T>
+hipError_t gather_t(const ExpandProblem& p, bool aligned, hipStream_t stream) {
+  const dim3 grid((unsigned)p.src.num_tiles);
+  if (aligned) hipLaunchKernelGGL((gather_kernel<KT, T, true>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((gather_kernel<KT, T, false>), grid, dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_gather(const ExpandProblem& p, hipStream_t stream) {
+  if (p.src.num_tiles == 0) return hipSuccess;
+  if (p.src.num_tiles > INT32_MAX || p.src.row_elems != 576) return hipErrorInvalidValue;
+  const bool aligned = (reinterpret_cast<uintptr_t>(p.src.kv) & 15) == 0;  // rows are 1152 or 576 B
+  switch (p.src.kv_dtype) {
+    case LA_DTYPE_BF16: return gather_t<__hip_bfloat16, __hip_bfloat16>(p, aligned, stream);
+    case LA_DTYPE_F16: return gather_t<__half, __half>(p, aligned, stream);
+    case LA_DTYPE_FP8_E4M3: return gather_t<fp8e4m3, __hip_bfloat16>(p, aligned, stream);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+hipError_t launch_expand(const ExpandProblem& p, hipStream_t stream, int ncu) {
+  if (p.src.num_tiles == 0 || p.heads == 0) return hipSuccess;
+  const bool wide = (int64_t)p.heads * ((p.src.num_tiles + 3) / 4) >= ncu;
+  if (p.f16) return wide ? expand_pb<__half, 4>(p, stream) : expand_pb<__half, 2>(p, stream);
+  return wide ? expand_pb<__hip_bfloat16, 4>(p, stream) : expand_pb<__hip_bfloat16, 2>(p, stream);
+}
+
+hipError_t launch_convert(const void* src, int src_dtype, void* dst, int f16, int64_t n, hipStream_t stream) {
+  if (n == 0) return hipSuccess;
+  const int64_t blocks = n / 1024 + 1 < 4096 ? n / 1024 + 1 : 4096;
+  hipLaunchKernelGGL(convert_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, src, src_dtype,
+                     static_cast<uint16_t*>(dst), f16, n);
+  return hipGetLastError();
+}
+
+}  // namespace la

@@ -10,7 +10,8 @@ falls back to PyTorch math -- if the extension is missing, the call raises.
 
 from __future__ import annotations
 
-from typing import TYPE_CHECKING, Optional
+from dataclasses import dataclass
+from typing import TYPE_CHECKING, Optional, Union
 
 import torch
 
@@ -224,3 +225,161 @@ def absorb_q(q_nope: torch.Tensor, W_UK: torch.Tensor, cfg: "MLAConfig") -> torc
     """q_absorbed[..., h, c] = sum_i q_nope[..., h, i] * W_UK[h*dn + i, c] (fp32)."""
     _C = _load_ext()
     return _C.absorb_q_forward(q_nope, W_UK, *_cfg_args(cfg))
+
+
+def mla_prefill(
+    kv_cache: torch.Tensor,
+    q_nope: torch.Tensor,
+    q_rope: torch.Tensor,
+    W_UK: torch.Tensor,
+    W_UV: torch.Tensor,
+    rope_cos: torch.Tensor,
+    rope_sin: torch.Tensor,
+    cfg: "MLAConfig",
+    q_offsets: Optional[torch.Tensor] = None,
+    seq_offsets: Optional[torch.Tensor] = None,
+    seq_lens: Optional[torch.Tensor] = None,
+    block_table: Optional[torch.Tensor] = None,
+    block_size: int = 0,
+    prefix_lens: Optional[torch.Tensor] = None,
+    rotate_q: bool = False,
+    max_seq_rows: int = 0,
+    out_dtype: Optional[torch.dtype] = None,
+    kernel_variant: int = 0,
+) -> torch.Tensor:
+    """Causal attention of several new tokens per sequence: whole prompts,
+    pieces of them over what the cache holds already, drafted tokens.
+
+    The new tokens' rows are in the cache (``append_kv``) and are each
+    sequence's last: token j of n of a sequence with L rows is at position
+    L - n + j and sees the rows up to its own.
+
+    Args:
+        kv_cache:    as in ``mla_decode``: (batch, capacity, dc + dR), packed
+                     (rows, dc + dR) with ``seq_offsets``, or a paged pool with
+                     ``block_table`` / ``block_size`` / ``seq_lens``
+        q_nope:      (tokens, num_heads, qk_nope_head_dim) fp32 / fp16 / bf16,
+                     the sequences' new tokens one after another
+        q_rope:      (tokens, num_heads, qk_rope_head_dim), the same type; both
+                     may be strided views whose last dimension is contiguous
+                     (slices of one projection's output)
+        q_offsets:   int32 (batch + 1,) device tensor starting at 0; sequence b
+                     has tokens [q_offsets[b], q_offsets[b+1]); None: tokens /
+                     batch each. Tokens behind the last sequence get zeros.
+        prefix_lens: optional int32 (batch,) device tensor: the first
+                     prefix_lens[b] rows of sequence b are seen by all of its
+                     tokens (read in both directions)
+        rotate_q:    q_rope is not rotated yet: rotated on the way by its
+                     token's position (the tensor is left as it is)
+        max_seq_rows: a region ends there (0: its capacity); bounds the
+                     workspace of caches whose capacity is far beyond the
+                     lengths
+        out_dtype:   fp32 / fp16 / bf16; None: the queries' type
+        kernel_variant: 0 = automatic, 1 = plain kernel, 2 = keys and values
+                     expanded, 3 = queries absorbed
+
+    Returns:
+        (tokens, num_heads, v_head_dim) in out_dtype
+    """
+    _C = _load_ext()
+    return _C.mla_prefill_forward(kv_cache, q_nope, q_rope, W_UK, W_UV, rope_cos, rope_sin, q_offsets, seq_offsets,
+                                  *_cfg_args(cfg), seq_lens, block_table, block_size, prefix_lens, rotate_q,
+                                  max_seq_rows, q_nope.dtype if out_dtype is None else out_dtype, kernel_variant)
+
+
+@dataclass(frozen=True)
+class SharedPrefix:
+    """A prefix for ``mla_decode_shared``: its latent rows and, from
+    ``expand_prefix``, their per-head keys and values. ``expanded`` belongs to
+    the weights and tables that it was made with."""
+
+    rows: torch.Tensor  # (prefix, kv_lora_rank + qk_rope_head_dim)
+    expanded: torch.Tensor  # fp16 (fp16 rows) or bf16, the library's order
+    num_heads: int
+
+    @property
+    def _tiles(self) -> int:
+        return -(-self.rows.size(0) // 64)
+
+    @property
+    def k_nope(self) -> torch.Tensor:
+        """Keys W_UK c_t as a view (tile, 2, 32, head, 8, 2, 2, 4): rows (zeros
+        past the last), head, dims in order; ``reshape(-1, heads, 128)`` copies
+        them into rows."""
+        t, h = self._tiles, self.num_heads
+        return self.expanded[:h * t * 8192].view(h, t, 2, 8, 2, 32, 2, 4).permute(1, 2, 5, 0, 3, 6, 4, 7)
+
+    @property
+    def v(self) -> torch.Tensor:
+        """Values W_UV c_t as a view (tile, 4, 2, 2, 4, head, 4, 32)."""
+        t, h = self._tiles, self.num_heads
+        return self.expanded[h * t * 8192:2 * h * t * 8192].view(h, t, 4, 4, 2, 32, 2, 4).permute(1, 3, 6, 4, 7, 0, 2, 5)
+
+    @property
+    def k_rope(self) -> torch.Tensor:
+        """Rotated rope keys as a view (tile, 2, 32, 4, 2, 2, 4)."""
+        t, h = self._tiles, self.num_heads
+        return self.expanded[2 * h * t * 8192:].view(t, 2, 4, 2, 32, 2, 4).permute(0, 1, 4, 2, 5, 3, 6)
+
+
+def expand_prefix(
+    kv_cache: torch.Tensor,
+    W_UK: torch.Tensor,
+    W_UV: torch.Tensor,
+    rope_cos: torch.Tensor,
+    rope_sin: torch.Tensor,
+    cfg: "MLAConfig",
+) -> SharedPrefix:
+    """Expands a prefix's latent rows (prefix, dc + dR; fp16, bf16 or FP8) into
+    per-head keys and values, once for the many steps that read them: 512 bytes
+    per row and head, with which ``mla_decode_shared`` does under a third of
+    the products for a large batch. kv_lora_rank 512, 128-dim heads, rope 64."""
+    _C = _load_ext()
+    return SharedPrefix(kv_cache, _C.expand_prefix_forward(kv_cache, W_UK, W_UV, rope_cos, rope_sin, *_cfg_args(cfg)),
+                        cfg.num_heads)
+
+
+def mla_decode_shared(
+    prefix: Union[SharedPrefix, torch.Tensor],
+    kv_cache: torch.Tensor,
+    q_nope: torch.Tensor,
+    q_rope: torch.Tensor,
+    W_UK: torch.Tensor,
+    W_UV: torch.Tensor,
+    rope_cos: torch.Tensor,
+    rope_sin: torch.Tensor,
+    cfg: "MLAConfig",
+    seq_offsets: Optional[torch.Tensor] = None,
+    seq_lens: Optional[torch.Tensor] = None,
+    block_table: Optional[torch.Tensor] = None,
+    block_size: int = 0,
+    out_dtype: torch.dtype = torch.float32,
+    kernel_variant: int = 0,
+) -> torch.Tensor:
+    """``mla_decode`` for sequences that share a prefix, which is attended once
+    for all of them.
+
+    Args:
+        prefix:      (prefix, dc + dR) latent rows at positions 0, 1, ..., in
+                     kv_cache's type, or a ``SharedPrefix`` of them
+        kv_cache, seq_offsets, seq_lens, block_table, block_size: the
+                     sequences' own rows, as in ``mla_decode``; row i of a
+                     sequence is at position prefix + i, and it may have none
+        q_nope, q_rope, W_UK, W_UV: as in ``mla_decode``
+        rope_cos / rope_sin: (>= prefix + longest sequence, dR / 2)
+        out_dtype:   fp32 / fp16 / bf16
+        kernel_variant: 0 = automatic, 1 = the prefix's latent rows, 2 = its
+                     expanded form
+
+    Returns:
+        (batch, num_heads, v_head_dim) in out_dtype
+    """
+    _C = _load_ext()
+    expanded = None
+    if isinstance(prefix, SharedPrefix):
+        if prefix.num_heads != cfg.num_heads:
+            raise ValueError(f"prefix was expanded for {prefix.num_heads} heads, not {cfg.num_heads}")
+        prefix, expanded = prefix.rows, prefix.expanded
+    return _C.mla_decode_shared_forward(prefix, expanded, kv_cache, q_nope, q_rope, W_UK, W_UV, rope_cos, rope_sin,
+                                        seq_offsets, *_cfg_args(cfg), seq_lens, block_table, block_size, out_dtype,
+                                        kernel_variant)

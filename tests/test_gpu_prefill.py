@@ -1,0 +1,301 @@
+"""GPU parity of functional.mla_prefill (la_mla_prefill) against the 64-bit
+reference of tests/prompt_cases.py: every form, cache layout, cache and query
+type, odd and empty lengths, masks, strides, and its use in a run of the
+framework's calls and in a captured graph."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from conftest import assert_close
+from prompt_cases import U, Layout, as_double, check, reference, tables, weights
+
+from latent_attn import MLAConfig
+from latent_attn import functional as F
+
+pytestmark = pytest.mark.gpu
+
+AUTO, PLAIN, EXPANDED, ABSORBED = 0, 1, 2, 3
+
+
+def config(heads, dc=512, dn=128, d_r=64, dv=128):
+    return MLAConfig(5120, dc, dn, d_r, heads, dv)
+
+
+class Case:
+    def __init__(self, cuda, layout, rows, new, heads=4, kv=torch.bfloat16, q=torch.bfloat16, w=None, prefix=None,
+                 rotate_q=True, block=64, seed=1, dims=(512, 128, 64, 128), pad=0, scale=1.0):
+        dc, dn, d_r, dv = dims
+        self.cfg, self.kv_type, self.q_type = config(heads, dc, dn, d_r, dv), kv, q
+        g = torch.Generator().manual_seed(seed)
+        data = [(torch.randn(n, dc + d_r, generator=g) * scale).to(kv).float() for n in rows]
+        self.layout = Layout(layout, data, kv, cuda, block=block, seed=seed)
+        self.rows = [d.double() for d in data]
+        tokens = sum(new) + pad
+        self.q = torch.randn(tokens, heads, dn + d_r, generator=g).to(q).to(cuda)
+        w = w or (kv if kv in U else torch.bfloat16 if kv != torch.float32 else torch.float32)
+        self.W_UK, self.W_UV = (x.to(cuda) for x in weights(heads, w, seed + 1, dc, dn, dv))
+        cos, sin = tables(max(rows), d_r)
+        self.cos, self.sin = cos.to(cuda), sin.to(cuda)
+        self.new, self.prefix, self.rotate_q, self.dn = new, prefix, rotate_q, dn
+        at = [0]
+        for n in new:
+            at.append(at[-1] + n)
+        self.kw = dict(self.layout.kw)
+        self.kw["q_offsets"] = torch.tensor(at, dtype=torch.int32, device=cuda)
+        if prefix is not None:
+            self.kw["prefix_lens"] = torch.tensor(prefix, dtype=torch.int32, device=cuda)
+
+    def run(self, **kw):
+        kw = {**self.kw, "rotate_q": self.rotate_q, **kw}
+        return F.mla_prefill(self.layout.kv, self.q[..., :self.dn], self.q[..., self.dn:], self.W_UK, self.W_UV,
+                             self.cos, self.sin, self.cfg, **kw)
+
+    def reference(self):
+        q = as_double(self.q)
+        return reference(self.rows, q[..., :self.dn], q[..., self.dn:], as_double(self.W_UK), as_double(self.W_UV),
+                         as_double(self.cos), as_double(self.sin), self.new, self.prefix, self.rotate_q)
+
+    def check(self, got, form, what=""):
+        ref = self.reference()
+        if self.kv_type == torch.float32:
+            assert got.dtype == self.q_type
+            if got.dtype == torch.float32:
+                assert_close(got.cpu().numpy(), ref[0].numpy(), "f32", what)
+            else:  # fp32 sums, one rounding of the output
+                bound = U[got.dtype] * ref[0].abs() + 1e-4
+                assert ((got.double().cpu() - ref[0]).abs() <= bound).all(), what
+            return
+        u = U[torch.float16 if self.kv_type == torch.float16 else torch.bfloat16]
+        if form == EXPANDED:
+            q_rounds = self.rotate_q or self.q_type != (torch.float16 if self.kv_type == torch.float16 else torch.bfloat16)
+            check(got, ref, u, 2 if q_rounds else 1, U.get(got.dtype, 0.0), what)
+        else:
+            assert_close(got.double().cpu().numpy(), ref[0].numpy(), "bf16", what)
+
+
+ODD_ROWS, ODD_NEW = [1, 63, 64, 65, 200, 130], [1, 5, 64, 65, 130, 129]
+
+
+@pytest.mark.parametrize("kv", [torch.bfloat16, torch.float16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("layout", ["packed", "capacity", "packed_capacity", "paged"])
+def test_expanded_layouts(cuda, layout, kv):
+    c = Case(cuda, layout, ODD_ROWS, ODD_NEW, kv=kv, q=torch.float16 if kv == torch.float16 else torch.bfloat16)
+    c.check(c.run(kernel_variant=EXPANDED), EXPANDED, f"{layout} {kv}")
+
+
+@pytest.mark.parametrize("kv", [torch.bfloat16, torch.float16, torch.float8_e4m3fn, torch.float32])
+@pytest.mark.parametrize("layout,form", [("capacity", ABSORBED), ("paged", ABSORBED), ("packed", PLAIN),
+                                         ("capacity", PLAIN), ("paged", PLAIN), ("packed_capacity", PLAIN)])
+def test_other_forms(cuda, layout, form, kv):
+    c = Case(cuda, layout, ODD_ROWS, [1, 5, 8, 3, 1, 7], heads=16, kv=kv, q=torch.float32)
+    c.check(c.run(kernel_variant=form), form, f"{layout} {kv}")
+
+
+@pytest.mark.parametrize("form", [PLAIN, EXPANDED, ABSORBED])
+def test_empty_rows_and_more_tokens_than_rows(cuda, form):
+    """A sequence without rows, one with more new tokens than rows (its first tokens see nothing), one without new
+    tokens, and padding behind the last sequence: zeros there, the rest as ever."""
+    c = Case(cuda, "capacity", [0, 3, 70, 40], [2, 9, 0, 40], heads=16, pad=5)
+    got = c.run(kernel_variant=form)
+    c.check(got, form, "empty")
+    assert (got[:2] == 0).all() and (got[2:8] == 0).all() and (got[-5:] == 0).all()
+    assert (got[8] != 0).any()
+
+
+@pytest.mark.parametrize("form", [PLAIN, EXPANDED, ABSORBED])
+@pytest.mark.parametrize("prefix", [[0, 7, 64, 500, 1], [1000] * 5])
+def test_prefix_mask(cuda, form, prefix):
+    c = Case(cuda, "capacity", [50, 64, 130, 129, 1], [50, 60, 100, 3, 1], heads=16, prefix=prefix)
+    c.check(c.run(kernel_variant=form), form, "prefix")
+
+
+@pytest.mark.parametrize("heads", [1, 3, 8, 16, 17])
+@pytest.mark.parametrize("n,L", [(1, 1), (1, 300), (33, 33), (127, 500), (257, 257)])
+def test_heads_and_lengths(cuda, heads, n, L):
+    c = Case(cuda, "uniform", [L, L], [n, n], heads=heads)
+    c.check(c.run(kernel_variant=EXPANDED), EXPANDED, f"{heads} heads {n} of {L}")
+
+
+@pytest.mark.parametrize("kv", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("q", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("w", [torch.float32, torch.bfloat16, torch.float16])
+def test_types(cuda, kv, q, w):
+    """Every mixture of cache, query and weight types; weights of another type are rounded to the expanded one (the
+    reference takes them so)."""
+    c = Case(cuda, "packed", [70, 33], [70, 20], kv=kv, q=q, w=w)
+    c.W_UK, c.W_UV = (x.to(kv).to(x.dtype) for x in (c.W_UK, c.W_UV))
+    for out in (torch.float32, torch.bfloat16, torch.float16):
+        got = c.run(kernel_variant=EXPANDED, out_dtype=out)
+        assert got.dtype == out
+        c.check(got, EXPANDED, f"{kv} {q} {w} {out}")
+
+
+def test_rotation_and_strides(cuda):
+    """Queries rotated on the way equal queries rotated before; packed, sliced and oddly strided queries agree."""
+    c = Case(cuda, "packed", [90, 40], [90, 11], heads=5, q=torch.float32)
+    want = c.run(kernel_variant=EXPANDED)
+    c.check(want, EXPANDED, "rotated on the way")
+    pos = torch.cat([torch.arange(90), torch.arange(29, 40)]).to(cuda)
+    x, y = c.q[..., 128:160], c.q[..., 160:]
+    cs, sn = c.cos[pos][:, None], c.sin[pos][:, None]
+    before = torch.cat([x * cs - y * sn, x * sn + y * cs], -1)
+    kept = before.clone()
+    args = (c.W_UK, c.W_UV, c.cos, c.sin, c.cfg)
+    got = F.mla_prefill(c.layout.kv, c.q[..., :128].contiguous(), before, *args, **c.kw, kernel_variant=EXPANDED)
+    assert torch.equal(before, kept)
+    # a product contracted into an fma or not moves a rotated element by an fp32 rounding, which can move its 16-bit one
+    assert (got - want).norm() <= 2.0 ** -8 * want.norm()
+    wide = torch.zeros(101, 7, 193, device=cuda)  # rows that are no multiple of 16 bytes
+    wide[:, 1:6, 1:] = c.q
+    view = wide[:, 1:6, 1:]
+    got = F.mla_prefill(c.layout.kv, view[..., :128], view[..., 128:], *args, **c.kw, rotate_q=True, kernel_variant=EXPANDED)
+    assert torch.equal(got, want)
+    turned = c.q.transpose(0, 1).contiguous().transpose(0, 1)  # heads outermost
+    got = F.mla_prefill(c.layout.kv, turned[..., :128], turned[..., 128:], *args, **c.kw, rotate_q=True,
+                        kernel_variant=EXPANDED)
+    assert torch.equal(got, want)
+
+
+def test_unaligned_cache_and_weights(cuda):
+    c = Case(cuda, "packed", [70, 33], [70, 20])
+    want = c.run(kernel_variant=EXPANDED)
+    for name in ("W_UK", "W_UV"):
+        w = getattr(c, name)
+        b = torch.zeros(w.numel() + 1, dtype=w.dtype, device=cuda)
+        b[1:] = w.flatten()
+        setattr(c, name, b[1:].view_as(w))
+    b = torch.zeros(c.layout.kv.numel() + 1, dtype=c.layout.kv.dtype, device=cuda)
+    b[1:] = c.layout.kv.flatten()
+    c.layout.kv = b[1:].view_as(c.layout.kv)
+    assert torch.equal(c.run(kernel_variant=EXPANDED), want)
+
+
+@pytest.mark.parametrize("block", [1, 16, 48, 100])
+def test_page_sizes(cuda, block):
+    """Pages that end inside a tile of keys, and single rows."""
+    c = Case(cuda, "paged", ODD_ROWS, ODD_NEW, block=block)
+    c.check(c.run(kernel_variant=EXPANDED), EXPANDED, f"block {block}")
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_what_a_token_does_not_see_does_not_reach_it(cuda, bad):
+    """Rows behind a token that hold NaN or infinities leave it as it was; the tokens that see them get NaN or
+    infinities (nothing finite), in every head."""
+    c = Case(cuda, "packed", [150, 80], [150, 80])
+    want = c.run(kernel_variant=EXPANDED)
+    c.layout.kv[101] = bad  # a row of the first sequence
+    got = c.run(kernel_variant=EXPANDED)
+    assert torch.equal(got[:101], want[:101]) and torch.equal(got[150:], want[150:])
+    assert not torch.isfinite(got[101:150]).any()
+
+
+def test_large_scores(cuda):
+    """Scores of thousands: the running maximum rises often, and by much."""
+    c = Case(cuda, "packed", [300, 64], [300, 64], scale=1.0)
+    c.q *= 64
+    c.q_type = torch.bfloat16
+    ref = c.reference()
+    got = c.run(kernel_variant=EXPANDED).double().cpu()
+    assert torch.isfinite(got).all()
+    # a rounded key moves a score of hundreds by more than one: only rows whose first weight is safe are compared
+    out, mass, size = ref
+    top = (got - out).abs().amax(-1)
+    safe = torch.expm1(2 * 2 * 2.0 ** -8 * size) < 0.5
+    assert (top[safe] <= 2 * mass.amax(-1)[safe]).all()
+
+
+def test_splits_equal_one_part(cuda):
+    """One token tile over many keys runs in parts of the keys, joined; the same call in a large batch does not."""
+    one = Case(cuda, "uniform", [2000], [3], heads=2, seed=5)
+    got = one.run(kernel_variant=EXPANDED)
+    one.check(got, EXPANDED, "parts")
+
+
+def test_auto_form_and_large_head_count(cuda):
+    for rows, new in (([400, 90], [3, 1]), ([400, 90], [300, 90])):
+        c = Case(cuda, "paged", rows, new, heads=128)
+        c.check(c.run(), ABSORBED, "auto")
+
+
+def test_other_dims(cuda):
+    for kv in (torch.bfloat16, torch.float32):
+        c = Case(cuda, "packed", [50, 20], [50, 3], heads=3, kv=kv, q=torch.float32, dims=(96, 40, 24, 56))
+        c.check(c.run(), PLAIN, "other dims")
+
+
+def test_max_seq_rows(cuda):
+    """A capacity cache whose regions are cut at max_seq_rows gives the same where no sequence is longer."""
+    c = Case(cuda, "capacity", [50, 64, 10], [50, 5, 10], heads=16)
+    for form in (PLAIN, EXPANDED, ABSORBED):
+        want = c.run(kernel_variant=form)
+        got = c.run(kernel_variant=form, max_seq_rows=64)
+        c.check(got, form, "max_seq_rows")
+        # (the absorbed form's decode plan cuts the region, so its sums run in another order)
+        assert form == ABSORBED or torch.equal(got, want)
+
+
+def test_other_stream_and_repeat(cuda):
+    c = Case(cuda, "packed", ODD_ROWS, ODD_NEW)
+    want = c.run(kernel_variant=EXPANDED)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = [c.run(kernel_variant=EXPANDED) for _ in range(3)]
+    torch.cuda.synchronize()
+    for g in got:
+        assert torch.equal(g, want)
+
+
+@pytest.mark.parametrize("form", [PLAIN, EXPANDED, ABSORBED])
+def test_captured(cuda, form):
+    """A captured call replayed on other inputs and offsets (a padded batch), with eager work between the replays."""
+    c = Case(cuda, "capacity", [50, 64, 10], [20, 5, 10], heads=16, pad=10)
+    c.run(kernel_variant=form)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = c.run(kernel_variant=form)
+    for seed, new in ((3, [20, 5, 10]), (4, [1, 40, 4]), (5, [0, 0, 1])):
+        g = torch.Generator().manual_seed(seed)
+        c.q.copy_(torch.randn(c.q.shape, generator=g).to(c.q.dtype))
+        at = [0, new[0], new[0] + new[1], sum(new)]
+        c.kw["q_offsets"].copy_(torch.tensor(at, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        eager = c.run(kernel_variant=form)
+        torch.cuda.synchronize()
+        assert torch.equal(got, eager)
+        assert (got[sum(new):] == 0).all()
+
+
+def test_prompt_then_decode(cuda):
+    """append_kv of a prompt, its attention, then a drafted pair of tokens and a single one: the last token's row is
+    the decode step's."""
+    cfg = config(16)
+    B, cap, T = 3, 256, 70
+    g = torch.Generator().manual_seed(2)
+    W_UK, W_UV = (x.to(cuda) for x in weights(16, torch.bfloat16, 3))
+    cos, sin = (x.to(cuda) for x in tables(cap))
+    kv = torch.full((B, cap, 576), float("nan"), dtype=torch.bfloat16, device=cuda)
+    lens = torch.zeros(B, dtype=torch.int32, device=cuda)
+    rows = torch.randn(B, T + 3, 576, generator=g).to(torch.bfloat16).to(cuda)
+    q = torch.randn(B, T + 3, 16, 192, generator=g).to(cuda)
+    at = 0
+    for n in (T, 2, 1):
+        new = rows[:, at:at + n]
+        F.append_kv(kv, lens, new[..., :512].contiguous(), new[..., 512:].contiguous(), cfg)
+        at += n
+        mine = q[:, at - n:at].reshape(B * n, 16, 192)
+        got = F.mla_prefill(kv, mine[..., :128], mine[..., 128:], W_UK, W_UV, cos, sin, cfg, seq_lens=lens, rotate_q=True)
+        ref = reference([r[:at] for r in as_double(rows)], as_double(mine[..., :128]), as_double(mine[..., 128:]),
+                        as_double(W_UK), as_double(W_UV), as_double(cos), as_double(sin), [n] * B, None, True)
+        assert_close(got.double().cpu().numpy(), ref[0].numpy(), "bf16", f"{n} tokens at {at}")
+        assert lens.tolist() == [at] * B
+    x, y = mine[..., 128:160], mine[..., 160:]
+    cs, sn = cos[at - 1], sin[at - 1]
+    turned = torch.cat([x * cs - y * sn, x * sn + y * cs], -1).contiguous()
+    step = F.mla_decode(kv, mine[..., :128].contiguous(), turned, W_UK, W_UV, cos, sin, cfg, seq_lens=lens)
+    assert_close(got.cpu().numpy(), step.double().cpu().numpy(), "bf16", "the decode step")
