@@ -63,7 +63,10 @@ __device__ inline typename Mm<T>::vec load8_row(const KT* p) {
   return load8<KT, T>(p);
 }
 
-// One workgroup per tile.
+// One workgroup per tile. A row whose latent holds an infinity or NaN gets zeros
+// there and NaN as its rope key: the tokens that see it get NaN through their
+// scores, as from its values, and those that do not (their weight is zero, and
+// zero times NaN is NaN) are left alone.
 template <typename KT, typename T, bool kAligned>
 __global__ __launch_bounds__(256) void gather_kernel(ExpandProblem p) {
   typedef typename Mm<T>::vec vec;
@@ -79,13 +82,21 @@ __global__ __launch_bounds__(256) void gather_kernel(ExpandProblem p) {
   const int pos0 = (int)t * kTileKeys;
   const KT* kv = static_cast<const KT*>(p.src.kv);
   vec* const c_out = reinterpret_cast<vec*>(static_cast<char*>(p.rows_c) + tile * kTileCBytes);
+  __shared__ int bad[kTileKeys];
 #pragma unroll 4
   for (int i = threadIdx.x; i < kTileKeys * 64; i += 256) {
-    const int r = i >> 6, ch = i & 63;
+    const int r = i >> 6, ch = i & 63;  // a wave takes one row
     vec v = {};
     if (r < rows) v = load8_row<KT, T, kAligned>(kv + source_row(p.src, s, pos0 + r) * p.src.row_elems + 8 * ch);
+    float z = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z = __builtin_fmaf((float)v[e], 0.f, z);
+    const bool any = __builtin_amdgcn_ballot_w64(!(z == 0.f)) != 0;
+    if (any) v = vec{};
+    if (ch == 0) bad[r] = any;
     c_out[i] = v;
   }
+  __syncthreads();
   elem* const r_out = reinterpret_cast<elem*>(static_cast<char*>(p.rope) + tile * kTileRBytes);
   for (int i = threadIdx.x; i < kTileKeys * 8; i += 256) {
     const int r = i >> 3, d = 4 * (i & 7);  // dims d .. d+3 and their partners d + 32 ..
@@ -99,6 +110,7 @@ __global__ __launch_bounds__(256) void gather_kernel(ExpandProblem p) {
         a[e] = (elem)(k0 * c - k1 * sn);
         b[e] = (elem)(k0 * sn + k1 * c);
       }
+      if (bad[r]) a = b = vec4{(elem)__builtin_nanf(""), (elem)__builtin_nanf(""), (elem)__builtin_nanf(""), (elem)__builtin_nanf("")};
     }
     elem* const o = r_out + (r >> 5) * (4 * 512) + operand_elem(r, d & 15);
     *reinterpret_cast<vec4*>(o + (d >> 4) * 512) = a;
