@@ -468,6 +468,9 @@ int scratch_ptr(void** out) {
 
 // ---- prompts and shared prefixes ----------------------------------------------------------------------
 
+bool tables_aligned(const RowSource& r) {
+  return ((reinterpret_cast<uintptr_t>(r.cos) | reinterpret_cast<uintptr_t>(r.sin)) & 15) == 0;
+}
 bool valid_out(int d) { return valid_dtype(d); }
 // Head shape of the expanded form's kernels.
 bool expanded_dims(const la_mla_config& c) {
@@ -746,6 +749,7 @@ int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need)
     if (p.form == kPrefillExpanded) {
       carve_expand(v, e, a->W_UK, a->w_uk_dtype, a->W_UV, a->w_uv_dtype, nh);
       const size_t tiles = (size_t)p.src.num_tiles;
+      e.p.q_info = static_cast<QueryTile*>(v.take((size_t)p.q_tiles * sizeof(QueryTile)));
       e.p.rope = v.take(tiles * kTileRBytes);
       e.p.kx = v.take(tiles * p.group * kTileKBytes);
       e.p.vx = v.take(tiles * p.group * kTileKBytes);
@@ -784,6 +788,9 @@ int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need)
   carve(scratch.ws);
 
   if (p.form == kPrefillExpanded) {
+    e.p.q = p.q;
+    e.p.q_tiles = p.q_tiles;
+    e.p.query_rows = prompt_query_rows();
     hipError_t r = start_expand(e, a->W_UK, a->w_uk_dtype, a->W_UV, a->w_uv_dtype, e.uk_copy, e.uv_copy, stream);
     PromptProblem m{};
     m.q = p.q;
@@ -792,6 +799,7 @@ int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need)
     m.kx = e.p.kx;
     m.vx = e.p.vx;
     m.rope = e.p.rope;
+    m.q_info = e.p.q_info;
     m.nh = nh;
     m.scale_log2 = scale_log2;
     m.out = a->output;
@@ -802,6 +810,7 @@ int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need)
     m.q_tiles = p.q_tiles;
     m.nope_vec = q_vec(p.q.q_nope, p.q.dtype, p.q.nope_stride, p.q.nope_head);
     m.rope_vec = q_vec(p.q.q_rope, p.q.dtype, p.q.rope_stride, p.q.rope_head);
+    m.table_vec = tables_aligned(p.src);
     for (int h = 0; h < nh && r == hipSuccess; h += p.group) {
       e.p.head0 = m.head0 = h;
       e.p.heads = m.heads = std::min(p.group, nh - h);
@@ -980,6 +989,7 @@ int decode_shared(const la_shared_args* a, hipStream_t stream, bool run_it, size
     m.q_tiles = query_tiles(m.q, prompt_query_rows());
     m.nope_vec = q_vec(m.q.q_nope, m.q.dtype, m.q.nope_stride, m.q.nope_head);
     m.rope_vec = q_vec(m.q.q_rope, m.q.dtype, m.q.rope_stride, m.q.rope_head);
+    m.table_vec = tables_aligned(m.src);
     const int64_t blocks = m.q_tiles * nh;
     m.splits = (int)std::max<int64_t>(
         2, std::min<int64_t>({(2 * cu_count() + blocks - 1) / blocks, m.src.num_tiles / 4, 32}));

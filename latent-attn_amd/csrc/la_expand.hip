@@ -63,59 +63,72 @@ __device__ inline typename Mm<T>::vec load8_row(const KT* p) {
   return load8<KT, T>(p);
 }
 
-// One workgroup per tile. A row whose latent holds an infinity or NaN gets zeros
-// there and NaN as its rope key: the tokens that see it get NaN through their
-// scores, as from its values, and those that do not (their weight is zero, and
-// zero times NaN is NaN) are left alone.
+// kGatherRows rows of a tile per workgroup, a row per wave at a time; the
+// workgroups behind the tiles find the query tiles. A row whose latent holds an
+// infinity or NaN gets zeros there and NaN as its rope key: the tokens that see
+// it get NaN through their scores, as from its values, and those that do not
+// (their weight is zero, and zero times NaN is NaN) are left alone.
+constexpr int kGatherRows = 16;
+constexpr int kGatherParts = kTileKeys / kGatherRows;
 template <typename KT, typename T, bool kAligned>
 __global__ __launch_bounds__(256) void gather_kernel(ExpandProblem p) {
   typedef typename Mm<T>::vec vec;
   typedef typename Mm<T>::elem elem;
   typedef elem vec4 __attribute__((ext_vector_type(4)));
-  const int64_t tile = blockIdx.x;
+  const int64_t tile = blockIdx.x / kGatherParts;
+  if (tile >= p.src.num_tiles) {
+    const int64_t qt = ((int64_t)blockIdx.x - p.src.num_tiles * kGatherParts) * 256 + threadIdx.x;
+    if (qt < p.q_tiles) p.q_info[qt] = make_query_tile(p.q, p.src, qt, p.query_rows);
+    return;
+  }
   const int s = source_find(p.src, tile);
   const int64_t t = tile - source_tile(p.src, s);
   const int L = source_rows(p.src, s);
   const int rows = (int)clamp64(L - t * kTileKeys, 0, kTileKeys);
-  if (threadIdx.x == 0) p.tile_rows[tile] = rows;
+  const int part = blockIdx.x % kGatherParts * kGatherRows;
+  if (threadIdx.x == 0 && part == 0) p.tile_rows[tile] = rows;
   if (rows == 0) return;
   const int pos0 = (int)t * kTileKeys;
   const KT* kv = static_cast<const KT*>(p.src.kv);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   vec* const c_out = reinterpret_cast<vec*>(static_cast<char*>(p.rows_c) + tile * kTileCBytes);
-  __shared__ int bad[kTileKeys];
-#pragma unroll 4
-  for (int i = threadIdx.x; i < kTileKeys * 64; i += 256) {
-    const int r = i >> 6, ch = i & 63;  // a wave takes one row
-    vec v = {};
-    if (r < rows) v = load8_row<KT, T, kAligned>(kv + source_row(p.src, s, pos0 + r) * p.src.row_elems + 8 * ch);
+  __shared__ int bad[kGatherRows];
+  vec v[kGatherRows / 4] = {};
+#pragma unroll
+  for (int i = 0; i < kGatherRows / 4; ++i) {
+    const int r = part + wave + 4 * i;
+    if (r < rows) v[i] = load8_row<KT, T, kAligned>(kv + source_row(p.src, s, pos0 + r) * p.src.row_elems + 8 * lane);
+  }
+#pragma unroll
+  for (int i = 0; i < kGatherRows / 4; ++i) {
     float z = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) z = __builtin_fmaf((float)v[e], 0.f, z);
+    for (int e = 0; e < 8; ++e) z = __builtin_fmaf((float)v[i][e], 0.f, z);
     const bool any = __builtin_amdgcn_ballot_w64(!(z == 0.f)) != 0;
-    if (any) v = vec{};
-    if (ch == 0) bad[r] = any;
-    c_out[i] = v;
+    if (any) v[i] = vec{};
+    if (lane == 0) bad[wave + 4 * i] = any;
+    c_out[(part + wave + 4 * i) * 64 + lane] = v[i];
   }
   __syncthreads();
+  if (threadIdx.x >= kGatherRows * 8) return;
   elem* const r_out = reinterpret_cast<elem*>(static_cast<char*>(p.rope) + tile * kTileRBytes);
-  for (int i = threadIdx.x; i < kTileKeys * 8; i += 256) {
-    const int r = i >> 3, d = 4 * (i & 7);  // dims d .. d+3 and their partners d + 32 ..
-    vec4 a = {}, b = {};
-    if (r < rows) {
-      const KT* k = kv + source_row(p.src, s, pos0 + r) * p.src.row_elems + 512 + d;
-      const int64_t at = source_rope_row(p.src, pos0 + r) * 32 + d;
+  const int r = part + (threadIdx.x >> 3), d = 4 * (threadIdx.x & 7);  // dims d .. d+3 and their partners d + 32 ..
+  vec4 a = {}, b = {};
+  if (r < rows) {
+    const KT* k = kv + source_row(p.src, s, pos0 + r) * p.src.row_elems + 512 + d;
+    const int64_t at = source_rope_row(p.src, pos0 + r) * 32 + d;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float k0 = to_f32(k[e]), k1 = to_f32(k[e + 32]), c = p.src.cos[at + e], sn = p.src.sin[at + e];
-        a[e] = (elem)(k0 * c - k1 * sn);
-        b[e] = (elem)(k0 * sn + k1 * c);
-      }
-      if (bad[r]) a = b = vec4{(elem)__builtin_nanf(""), (elem)__builtin_nanf(""), (elem)__builtin_nanf(""), (elem)__builtin_nanf("")};
+    for (int e = 0; e < 4; ++e) {
+      const float k0 = to_f32(k[e]), k1 = to_f32(k[e + 32]), c = p.src.cos[at + e], sn = p.src.sin[at + e];
+      a[e] = (elem)(k0 * c - k1 * sn);
+      b[e] = (elem)(k0 * sn + k1 * c);
     }
-    elem* const o = r_out + (r >> 5) * (4 * 512) + operand_elem(r, d & 15);
-    *reinterpret_cast<vec4*>(o + (d >> 4) * 512) = a;
-    *reinterpret_cast<vec4*>(o + ((d >> 4) + 2) * 512) = b;
+    const elem nan = (elem)__builtin_nanf("");
+    if (bad[r - part]) a = b = vec4{nan, nan, nan, nan};
   }
+  elem* const o = r_out + (r >> 5) * (4 * 512) + operand_elem(r, d & 15);
+  *reinterpret_cast<vec4*>(o + (d >> 4) * 512) = a;
+  *reinterpret_cast<vec4*>(o + ((d >> 4) + 2) * 512) = b;
 }
 
 __global__ __launch_bounds__(256) void convert_kernel(const void* src, int src_dtype, uint16_t* dst, int f16, int64_t n) {
@@ -262,7 +275,7 @@ hipError_t expand_pb(const ExpandProblem& p, hipStream_t stream) {
 
 template <typename KT, typename T>
 hipError_t gather_t(const ExpandProblem& p, bool aligned, hipStream_t stream) {
-  const dim3 grid((unsigned)p.src.num_tiles);
+  const dim3 grid((unsigned)(p.src.num_tiles * kGatherParts + (p.q_tiles + 255) / 256));
   if (aligned) hipLaunchKernelGGL((gather_kernel<KT, T, true>), grid, dim3(256), 0, stream, p);
   else hipLaunchKernelGGL((gather_kernel<KT, T, false>), grid, dim3(256), 0, stream, p);
   return hipGetLastError();
@@ -271,8 +284,8 @@ hipError_t gather_t(const ExpandProblem& p, bool aligned, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_gather(const ExpandProblem& p, hipStream_t stream) {
-  if (p.src.num_tiles == 0) return hipSuccess;
-  if (p.src.num_tiles > INT32_MAX || p.src.row_elems != 576) return hipErrorInvalidValue;
+  if (p.src.num_tiles == 0 && p.q_tiles == 0) return hipSuccess;
+  if (p.src.num_tiles > INT32_MAX / 8 || p.q_tiles > INT32_MAX || p.src.row_elems != 576) return hipErrorInvalidValue;
   const bool aligned = (reinterpret_cast<uintptr_t>(p.src.kv) & 15) == 0;  // rows are 1152 or 576 B
   switch (p.src.kv_dtype) {
     case LA_DTYPE_BF16: return gather_t<__hip_bfloat16, __hip_bfloat16>(p, aligned, stream);

@@ -65,6 +65,87 @@ __device__ inline void store1(void* out, int dtype, int64_t i, float v) {
   else static_cast<_Float16*>(out)[i] = (_Float16)v;
 }
 
+// The query of one lane as operands: 12 steps of 8 elements, step by step {16 k +
+// 4 g + (0..3), 16 k + 8 + 4 g + (0..3)}. All loads go out before the first is
+// waited for, so the type decides around them, not between them.
+enum QueryLoad { kScalar, kVec16, kVec32 };
+template <typename T, QueryLoad kLoad>
+__device__ inline void load_query_as(const PromptProblem& p, int64_t an, int64_t ar, int64_t pos, int g,
+                                     typename Mm<T>::vec (&qn)[8], typename Mm<T>::vec (&qr)[4]) {
+  typedef typename Mm<T>::elem elem;
+  float x[24][4];  // 16 pieces of the nope part, 8 of the rope part
+  auto at = [&](int i) { return i < 16 ? an + 8 * i + 4 * g : ar + 8 * (i - 16) + 4 * g; };
+  if constexpr (kLoad == kVec16) {
+    uint2 w[24];
+#pragma unroll
+    for (int i = 0; i < 24; ++i)
+      w[i] = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(i < 16 ? p.q.q_nope : p.q.q_rope) + at(i));
+    const bool bf16 = p.q.dtype == LA_DTYPE_BF16;
+#pragma unroll
+    for (int i = 0; i < 24; ++i) {
+      const uint32_t b[4] = {w[i].x & 0xFFFF, w[i].x >> 16, w[i].y & 0xFFFF, w[i].y >> 16};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        x[i][e] = bf16 ? f_of(b[e] << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)b[e]);
+    }
+  } else if constexpr (kLoad == kVec32) {
+#pragma unroll
+    for (int i = 0; i < 24; ++i) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(static_cast<const float*>(i < 16 ? p.q.q_nope : p.q.q_rope) + at(i));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[i][e] = v[e];
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < 24; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float v = load_any(i < 16 ? p.q.q_nope : p.q.q_rope, p.q.dtype, at(i) + e);
+#pragma unroll
+        for (int k = 0; k < 24; ++k) x[k][e] = k == i ? v : x[k][e];
+      }
+  }
+  if (p.q.rotate) {
+    f32x4 c[4], s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float* const cp = p.src.cos + pos + 8 * i + 4 * g;
+      const float* const sp = p.src.sin + pos + 8 * i + 4 * g;
+      if (p.table_vec) {
+        c[i] = *reinterpret_cast<const f32x4*>(cp);
+        s[i] = *reinterpret_cast<const f32x4*>(sp);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[i][e] = cp[e], s[i][e] = sp[e];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = x[16 + i][e], b = x[20 + i][e];
+        x[16 + i][e] = a * c[i][e] - b * s[i][e];
+        x[20 + i][e] = a * s[i][e] + b * c[i][e];
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 24; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (i < 16) qn[i >> 1][4 * (i & 1) + e] = (elem)x[i][e];
+      else qr[(i - 16) >> 1][4 * (i & 1) + e] = (elem)x[i][e];
+    }
+}
+template <typename T>
+__device__ inline void load_query(const PromptProblem& p, int64_t token, int h, int64_t pos, int g,
+                                  typename Mm<T>::vec (&qn)[8], typename Mm<T>::vec (&qr)[4]) {
+  const int64_t an = token * p.q.nope_stride + h * p.q.nope_head, ar = token * p.q.rope_stride + h * p.q.rope_head;
+  const int64_t at = source_rope_row(p.src, pos) * 32;
+  if (!(p.nope_vec && p.rope_vec)) load_query_as<T, kScalar>(p, an, ar, at, g, qn, qr);
+  else if (p.q.dtype == LA_DTYPE_F32) load_query_as<T, kVec32>(p, an, ar, at, g, qn, qr);
+  else load_query_as<T, kVec16>(p, an, ar, at, g, qn, qr);
+}
+
 // One workgroup: kQBlock tokens of one sequence, one head, one of `splits`
 // parts of the keys that they see. Scores come out transposed (keys in
 // registers, a query per lane), so the softmax's maximum and sum are per lane
@@ -86,20 +167,18 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(PromptProblem p) {
   if ((int64_t)(blockIdx.x >> 3) >= per || item >= items) return;
   const int64_t qt = p.q_tiles - 1 - item % p.q_tiles;
   const int hs = (int)(item / p.q_tiles), part = hs % p.splits, h = hs / p.splits;
-  const int s = query_find(p.q, qt, kQBlock);
-  const int n = query_count(p.q, s);
-  const int64_t j0l = (qt - query_tile(p.q, s, kQBlock)) * kQBlock;
-  if (j0l < 0 || j0l >= n) return;
-  const int j0 = (int)j0l;
-  const int L = source_rows(p.src, s);
-  const int64_t tile0 = L > 0 ? source_tile(p.src, s) : 0;
+  QueryTile q;
+  if (p.q_info) q = p.q_info[qt];
+  else q = QueryTile{(int)qt * kQBlock, (int)p.q.tokens, p.src.region, p.src.region, 0, 0};
+  if (q.j0 < 0) return;
   // visible keys grow with the token
-  const int jw = j0 + kQRows * wave;  // this wave's first token
-  const int j = min(jw + r32, n - 1);
-  const int lim = visible_keys(p.q, s, j, n, L);
-  const int wave_max = jw < n ? visible_keys(p.q, s, min(jw + kQRows, n) - 1, n, L) : 0;
-  const int wave_min = visible_keys(p.q, s, min(jw, n - 1), n, L);
-  const int block_max = visible_keys(p.q, s, min(j0 + kQBlock, n) - 1, n, L);
+  const int jw = q.j0 + kQRows * wave;  // this wave's first token
+  const int j = min(jw + r32, q.n - 1);
+  const int lim = tile_visible(q, j);
+  const int wave_max = jw < q.n ? tile_visible(q, min(jw + kQRows, q.n) - 1) : 0;
+  const int wave_min = tile_visible(q, min(jw, q.n - 1));
+  const int block_max = tile_visible(q, min(q.j0 + kQBlock, q.n) - 1);
+  const int64_t tile0 = q.tile0;
   const int nt = (int)clamp64((block_max + kTileKeys - 1) / kTileKeys, 0, p.src.num_tiles - tile0);
   const int t0 = (int)((int64_t)nt * part / p.splits), t1 = (int)((int64_t)nt * (part + 1) / p.splits);
 
@@ -122,42 +201,9 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(PromptProblem p) {
   };
   if (t0 < t1) issue(t0);
 
-  const int64_t token = query_begin(p.q, s) + j;
+  const int64_t token = q.token0 + j;
   vec qn[8], qr[4];
-  {
-    const int64_t at = token * p.q.nope_stride + (p.head0 + h) * p.q.nope_head;
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk)
-#pragma unroll
-      for (int e4 = 0; e4 < 2; ++e4) {
-        float x[4];
-        load_q4(p.q.q_nope, p.q.dtype, at + 16 * kk + 8 * e4 + 4 * g, p.nope_vec, x);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) qn[kk][4 * e4 + e] = (elem)x[e];
-      }
-    const int64_t ar = token * p.q.rope_stride + (p.head0 + h) * p.q.rope_head;
-    const int64_t pos = L == 0 ? 0 : source_rope_row(p.src, clamp64(L - n + j, 0, INT32_MAX)) * 32;
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-      for (int e4 = 0; e4 < 2; ++e4) {
-        const int d = 16 * kk + 8 * e4 + 4 * g;
-        float x[4], y[4];
-        load_q4(p.q.q_rope, p.q.dtype, ar + d, p.rope_vec, x);
-        load_q4(p.q.q_rope, p.q.dtype, ar + d + 32, p.rope_vec, y);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float a = x[e], b = y[e];
-          if (p.q.rotate) {
-            const float c = p.src.cos[pos + d + e], sn = p.src.sin[pos + d + e];
-            a = x[e] * c - y[e] * sn;
-            b = x[e] * sn + y[e] * c;
-          }
-          qr[kk][4 * e4 + e] = (elem)a;
-          qr[kk + 2][4 * e4 + e] = (elem)b;
-        }
-      }
-  }
+  load_query<T>(p, token, p.head0 + h, clamp64(q.L - q.n + j, 0, INT32_MAX), g, qn, qr);
 
   f32x16 o[4] = {};
   float m = kNoScore, l = 0.f;  // m in base-2 units of the scaled scores; l: this lane half's keys
@@ -169,16 +215,32 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(PromptProblem p) {
     if (t * kTileKeys >= wave_max) continue;
     const lchar* const b = lds + (t & 1) * kBufBytes + 16 * lane;
     auto operand = [&](int at) { return *reinterpret_cast<const __attribute__((address_space(3))) vec*>(b + at); };
+    // products in groups of four, the operands of the next group read before them
+    auto key = [&](int i) {  // operand i: step i / 2, key block i % 2
+      return operand(i < 16 ? 1024 * (8 * (i & 1) + (i >> 1)) : 2 * kTileKBytes + 1024 * (4 * (i & 1) + (i >> 1) - 8));
+    };
     f32x16 x[2] = {};
+    vec w[2][4];
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk)
+    for (int k = 0; k < 4; ++k) w[0][k] = key(k);
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) x[kb] = Mm<T>::mma(operand(1024 * (8 * kb + kk)), qn[kk], x[kb]);
+    for (int i = 0; i < 6; ++i) {
+      if (i < 5) {
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk)
+        for (int k = 0; k < 4; ++k) w[(i + 1) & 1][k] = key(4 * (i + 1) + k);
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-        x[kb] = Mm<T>::mma(operand(2 * kTileKBytes + 1024 * (4 * kb + kk)), qr[kk], x[kb]);
+      for (int k = 0; k < 4; ++k) {
+        const int st = (4 * i + k) >> 1;
+        x[k & 1] = Mm<T>::mma(w[i & 1][k], st < 8 ? qn[st] : qr[st - 8], x[k & 1]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    vec v[2][4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) v[0][d] = operand(kTileKBytes + 1024 * (4 * d));
+    __builtin_amdgcn_sched_barrier(0);
     settle2(x[0], x[1]);
     if ((t + 1) * kTileKeys > wave_min) {
 #pragma unroll
@@ -213,12 +275,18 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(PromptProblem p) {
         pr[ks][e] = (elem)w;
       }
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
+    for (int ks = 0; ks < 4; ++ks) {
+      if (ks < 3) {
 #pragma unroll
-      for (int d = 0; d < 4; ++d)
-        o[d] = Mm<T>::mma(operand(kTileKBytes + 1024 * (4 * d + ks)), pr[ks], o[d]);
+        for (int d = 0; d < 4; ++d) v[(ks + 1) & 1][d] = operand(kTileKBytes + 1024 * (4 * d + ks + 1));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) o[d] = Mm<T>::mma(v[ks & 1][d], pr[ks], o[d]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
-  if (jw + r32 >= n) return;
+  if (jw + r32 >= q.n) return;
   l = sum_halves(l);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   settle2(o[0], o[1]);
@@ -344,15 +412,18 @@ __global__ __launch_bounds__(256) void generic_prompt_kernel(GenericPrompt p) {
 
 // ---- queries of the absorbed forms ------------------------------------------------------------------
 
-// One workgroup per token.
+// kTokenElems elements of a token's queries per workgroup (x: token, y: share);
+// the first also writes its length and table.
+constexpr int kTokenElems = 2048;
 __global__ __launch_bounds__(256) void tokens_kernel(TokenProblem p) {
   const int64_t token = blockIdx.x;
   const int s = query_seq(p.q, token);
   const int n = query_count(p.q, s);
   const int64_t j = token - query_begin(p.q, s);
   const int L = j >= 0 && j < n ? source_rows(p.src, s) : 0;  // malformed offsets leave tokens without a sequence
-  if (p.lens && threadIdx.x == 0) p.lens[token] = L > 0 ? visible_keys(p.q, s, (int)j, n, L) : 0;
-  if (p.table) {
+  const int first = blockIdx.y * kTokenElems + threadIdx.x, last = (blockIdx.y + 1) * kTokenElems;
+  if (p.lens && first == 0) p.lens[token] = L > 0 ? visible_keys(p.q, s, (int)j, n, L) : 0;
+  if (p.table && blockIdx.y == 0) {
     int32_t* const t = p.table + token * p.blocks_per_seq;
     for (int i = threadIdx.x; i < p.blocks_per_seq; i += 256)
       t[i] = L == 0                 ? 0
@@ -360,13 +431,13 @@ __global__ __launch_bounds__(256) void tokens_kernel(TokenProblem p) {
                                  : (int32_t)((int64_t)s * p.src.stride_rows / p.block_size + i);
   }
   if (p.q_nope)
-    for (int i = threadIdx.x; i < p.nh * p.dn; i += 256)
+    for (int i = first; i < min(p.nh * p.dn, last); i += 256)
       p.q_nope[token * p.nh * p.dn + i] =
           load_any(p.q.q_nope, p.q.dtype, token * p.q.nope_stride + (i / p.dn) * p.q.nope_head + i % p.dn);
   if (p.q_rope) {
     const int half = p.dR / 2;
     const int64_t at = L == 0 ? 0 : source_rope_row(p.src, clamp64(L - n + j, 0, INT32_MAX)) * half;
-    for (int i = threadIdx.x; i < p.nh * half; i += 256) {
+    for (int i = first; i < min(p.nh * half, last); i += 256) {
       const int h = i / half, d = i % half;
       const int64_t ar = token * p.q.rope_stride + h * p.q.rope_head + d;
       float a = load_any(p.q.q_rope, p.q.dtype, ar), b = load_any(p.q.q_rope, p.q.dtype, ar + half);
@@ -409,7 +480,10 @@ hipError_t launch_generic_prompt(const GenericPrompt& p, hipStream_t stream) {
 hipError_t launch_tokens(const TokenProblem& p, hipStream_t stream) {
   if (p.q.tokens == 0) return hipSuccess;
   if (p.q.tokens > INT32_MAX) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(tokens_kernel, dim3((unsigned)p.q.tokens), dim3(256), 0, stream, p);
+  const int elems = p.nh * (p.dn > p.dR / 2 ? p.dn : p.dR / 2);
+  const unsigned shares = (unsigned)((elems + kTokenElems - 1) / kTokenElems);
+  if (shares > 65535) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(tokens_kernel, dim3((unsigned)p.q.tokens, shares), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 

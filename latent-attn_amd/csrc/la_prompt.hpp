@@ -184,6 +184,31 @@ inline bool q_vec(const void* base, int dtype, int64_t stride, int64_t head) {
   return reinterpret_cast<uintptr_t>(base) % align == 0 && stride % 4 == 0 && head % 4 == 0;
 }
 
+// A query tile as prompt_kernel takes it, found once per call by gather_kernel:
+// binary searches over device offsets in every workgroup were a chain of
+// dependent loads at its start.
+struct alignas(16) QueryTile {
+  int32_t j0;       // its first token within the sequence, < 0: no tokens
+  int32_t n, L;     // tokens and rows of the sequence
+  int32_t prefix;   // rows that every token sees
+  int64_t token0;   // first token of the sequence
+  int64_t tile0;    // first key tile of the sequence
+};
+__device__ inline QueryTile make_query_tile(const QuerySource& q, const RowSource& r, int64_t tile, int rows) {
+  const int s = query_find(q, tile, rows);
+  const int64_t j0 = (tile - query_tile(q, s, rows)) * rows;
+  QueryTile t{};
+  t.n = query_count(q, s);
+  t.j0 = j0 >= 0 && j0 < t.n ? (int)j0 : -1;
+  t.L = source_rows(r, s);
+  t.prefix = q.all ? t.L : q.prefix && t.L > 0 ? min(q.prefix[s], t.L) : 0;
+  t.token0 = query_begin(q, s);
+  t.tile0 = t.L > 0 ? source_tile(r, s) : 0;
+  return t;
+}
+// Keys that token j sees (visible_keys).
+__device__ inline int tile_visible(const QueryTile& t, int j) { return t.L == 0 ? 0 : max(max(t.L - t.n + j + 1, t.prefix), 0); }
+
 // Gather + expand: the source's rows as 16-bit latent tiles and rotated rope
 // keys (rows_c, rope), then K and V of `heads` heads from row `head0` of the
 // weights (16-bit, the tiles' type; kx and vx hold those heads only).
@@ -193,6 +218,10 @@ struct ExpandProblem {
   void* rows_c;     // [tile][64][512]
   void* rope;       // [tile] operand order
   int32_t* tile_rows;  // rows of each tile
+  QuerySource q;       // its tiles of query_rows tokens go to q_info (q_tiles = 0: none)
+  QueryTile* q_info;
+  int64_t q_tiles;
+  int query_rows;
   const void* W_UK;
   const void* W_UV;
   void* kx;  // [head][tile] operand order
@@ -212,6 +241,7 @@ struct PromptProblem {
   const void* kx;
   const void* vx;
   const void* rope;
+  const QueryTile* q_info;  // q_tiles of them, or nullptr: one sequence, every token sees every row
   int nh, head0, heads;  // weight heads; this launch's
   float scale_log2;
   void* out;  // (tokens, nh, 128) in out_dtype
@@ -220,7 +250,7 @@ struct PromptProblem {
   float* part_o;    // [split][token][nh][128], normalised
   float* part_lse;  // [split][token][nh], base 2
   int64_t q_tiles;
-  int nope_vec, rope_vec;
+  int nope_vec, rope_vec, table_vec;  // 16-byte (queries: whole-vector) aligned
 };
 int prompt_query_rows();  // query tokens per workgroup
 hipError_t launch_prompt(const PromptProblem& p, hipStream_t stream);
