@@ -678,7 +678,7 @@ int prepare_prefill(const la_prefill_args* a, Prefill* out) {
   if (p.form == kPrefillExpanded) {
     const size_t head_bytes = (size_t)r.num_tiles * kTileKBytes * 2;
     p.group = (int)std::min<size_t>(c.num_heads, std::max<size_t>(1, head_bytes ? kMaxExpanded / head_bytes : c.num_heads));
-    p.q_tiles = query_tiles(q, prompt_query_rows());
+        p.q_tiles = query_tiles(q, prompt_query_rows());
     // few query tiles leave CUs idle: their keys are cut into parts of at least four tiles
     const int64_t blocks = p.q_tiles * p.group;
     const int64_t tiles = a->seq_offsets ? a->total_rows / a->num_seqs / kTileKeys + 1 : r.num_tiles / a->num_seqs;
@@ -791,6 +791,7 @@ int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need)
     e.p.q = p.q;
     e.p.q_tiles = p.q_tiles;
     e.p.query_rows = prompt_query_rows();
+    e.p.k_scale = scale_log2;  // the softmax's scale goes into the keys before their one rounding
     hipError_t r = start_expand(e, a->W_UK, a->w_uk_dtype, a->W_UV, a->w_uv_dtype, e.uk_copy, e.uv_copy, stream);
     PromptProblem m{};
     m.q = p.q;
@@ -801,7 +802,7 @@ int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need)
     m.rope = e.p.rope;
     m.q_info = e.p.q_info;
     m.nh = nh;
-    m.scale_log2 = scale_log2;
+    m.q_scale = 1.f;
     m.out = a->output;
     m.out_dtype = a->out_dtype;
     m.splits = p.splits;
@@ -923,6 +924,7 @@ int expand(const la_expand_args* a, hipStream_t stream, bool run_it, size_t* nee
   e.p.kx = a->expanded;
   e.p.vx = static_cast<char*>(a->expanded) + kv;
   e.p.rope = static_cast<char*>(a->expanded) + 2 * kv;
+  e.p.k_scale = 1.f;
   e.p.head0 = 0;
   e.p.heads = a->cfg.num_heads;
   hipError_t r = start_expand(e, a->W_UK, a->w_uk_dtype, a->W_UV, a->w_uv_dtype, e.uk_copy, e.uv_copy, stream);
@@ -984,7 +986,7 @@ int decode_shared(const la_shared_args* a, hipStream_t stream, bool run_it, size
     m.q.all = 1;
     m.f16 = own.kv_dtype == LA_DTYPE_F16;
     m.nh = m.heads = nh;
-    m.scale_log2 = (float)(kLog2e / std::sqrt((double)(c.qk_nope_head_dim + c.qk_rope_head_dim)));
+    m.q_scale = (float)(kLog2e / std::sqrt((double)(c.qk_nope_head_dim + c.qk_rope_head_dim)));
     m.out_dtype = LA_DTYPE_F32;
     m.q_tiles = query_tiles(m.q, prompt_query_rows());
     m.nope_vec = q_vec(m.q.q_nope, m.q.dtype, m.q.nope_stride, m.q.nope_head);

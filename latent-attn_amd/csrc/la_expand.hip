@@ -120,8 +120,8 @@ __global__ __launch_bounds__(256) void gather_kernel(ExpandProblem p) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float k0 = to_f32(k[e]), k1 = to_f32(k[e + 32]), c = p.src.cos[at + e], sn = p.src.sin[at + e];
-      a[e] = (elem)(k0 * c - k1 * sn);
-      b[e] = (elem)(k0 * sn + k1 * c);
+      a[e] = (elem)((k0 * c - k1 * sn) * p.k_scale);
+      b[e] = (elem)((k0 * sn + k1 * c) * p.k_scale);
     }
     const elem nan = (elem)__builtin_nanf("");
     if (bad[r - part]) a = b = vec4{nan, nan, nan, nan};
@@ -218,7 +218,7 @@ __device__ inline void expand_wave(const ExpandProblem& p, const char* const (&s
       for (int q = 0; q < 2; ++q) {
         vec v;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (elem)acc[i][j][8 * q + e];
+        for (int e = 0; e < 8; ++e) v[e] = (elem)(kV ? acc[i][j][8 * q + e] : acc[i][j][8 * q + e] * p.k_scale);
         const int db = 2 * (wn & 1) + j;  // block of 32 dims
         const int piece = kV ? 4 * db + 2 * (pb & 1) + q : 8 * (pb & 1) + 2 * db + q;
         *reinterpret_cast<vec*>(out + piece * 1024 + 16 * lane) = v;

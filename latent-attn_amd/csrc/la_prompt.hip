@@ -132,8 +132,8 @@ __device__ inline void load_query_as(const PromptProblem& p, int64_t an, int64_t
   for (int i = 0; i < 24; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (i < 16) qn[i >> 1][4 * (i & 1) + e] = (elem)x[i][e];
-      else qr[(i - 16) >> 1][4 * (i & 1) + e] = (elem)x[i][e];
+      if (i < 16) qn[i >> 1][4 * (i & 1) + e] = (elem)(x[i][e] * p.q_scale);
+      else qr[(i - 16) >> 1][4 * (i & 1) + e] = (elem)(x[i][e] * p.q_scale);
     }
 }
 template <typename T>
@@ -146,152 +146,20 @@ __device__ inline void load_query(const PromptProblem& p, int64_t token, int h, 
   else load_query_as<T, kVec16>(p, an, ar, at, g, qn, qr);
 }
 
-// One workgroup: kQBlock tokens of one sequence, one head, one of `splits`
-// parts of the keys that they see. Scores come out transposed (keys in
-// registers, a query per lane), so the softmax's maximum and sum are per lane
-// (and one exchange between the lane halves), and their exponentials are the
-// second product's operand as they are.
-template <typename T>
-__global__ __launch_bounds__(256, 2) void prompt_kernel(PromptProblem p) {
-  typedef typename Mm<T>::vec vec;
-  typedef typename Mm<T>::elem elem;
-  extern __shared__ __attribute__((aligned(1024))) char prompt_lds[];
-  lchar* const lds = (lchar*)prompt_lds;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int r32 = lane & 31, g = lane >> 5;
-  // Items in order of head, part and query tile (the last, with the most keys
-  // to see, first), an eighth of them to each XCD: the workgroups that read
-  // one head's keys share an L2.
-  const int64_t items = (int64_t)p.heads * p.splits * p.q_tiles, per = (items + 7) / 8;
-  const int64_t item = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int64_t)(blockIdx.x >> 3) >= per || item >= items) return;
-  const int64_t qt = p.q_tiles - 1 - item % p.q_tiles;
-  const int hs = (int)(item / p.q_tiles), part = hs % p.splits, h = hs / p.splits;
-  QueryTile q;
-  if (p.q_info) q = p.q_info[qt];
-  else q = QueryTile{(int)qt * kQBlock, (int)p.q.tokens, p.src.region, p.src.region, 0, 0};
-  if (q.j0 < 0) return;
-  // visible keys grow with the token
-  const int jw = q.j0 + kQRows * wave;  // this wave's first token
-  const int j = min(jw + r32, q.n - 1);
-  const int lim = tile_visible(q, j);
-  const int wave_max = jw < q.n ? tile_visible(q, min(jw + kQRows, q.n) - 1) : 0;
-  const int wave_min = tile_visible(q, min(jw, q.n - 1));
-  const int block_max = tile_visible(q, min(q.j0 + kQBlock, q.n) - 1);
-  const int64_t tile0 = q.tile0;
-  const int nt = (int)clamp64((block_max + kTileKeys - 1) / kTileKeys, 0, p.src.num_tiles - tile0);
-  const int t0 = (int)((int64_t)nt * part / p.splits), t1 = (int)((int64_t)nt * (part + 1) / p.splits);
+__device__ inline float max3(float a, float b, float c) {  // (fmaxf first quiets every operand: two instructions more)
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 
-  const char* const kx = static_cast<const char*>(p.kx) + ((int64_t)h * p.src.num_tiles + tile0) * kTileKBytes;
-  const char* const vx = static_cast<const char*>(p.vx) + ((int64_t)h * p.src.num_tiles + tile0) * kTileKBytes;
-  const char* const rx = static_cast<const char*>(p.rope) + tile0 * kTileRBytes;
-  // A tile is three runs of 16, 16 and 8 KB, copied as they lie: 1 KB per wave and instruction.
-  auto issue = [&](int t) {
-    lchar* const b = lds + (t & 1) * kBufBytes;
-    const char* k = kx + (int64_t)t * kTileKBytes + 16 * lane;
-    const char* v = vx + (int64_t)t * kTileKBytes + 16 * lane;
-    const char* r = rx + (int64_t)t * kTileRBytes + 16 * lane;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = 1024 * (4 * i + wave);
-      __builtin_amdgcn_global_load_lds(k + c, (lds_void*)(b + c), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(v + c, (lds_void*)(b + kTileKBytes + c), 16, 0, 0);
-      if (i < 2) __builtin_amdgcn_global_load_lds(r + c, (lds_void*)(b + 2 * kTileKBytes + c), 16, 0, 0);
-    }
-  };
-  if (t0 < t1) issue(t0);
-
-  const int64_t token = q.token0 + j;
-  vec qn[8], qr[4];
-  load_query<T>(p, token, p.head0 + h, clamp64(q.L - q.n + j, 0, INT32_MAX), g, qn, qr);
-
-  f32x16 o[4] = {};
-  float m = kNoScore, l = 0.f;  // m in base-2 units of the scaled scores; l: this lane half's keys
-  const float sc = p.scale_log2;
-  for (int t = t0; t < t1; ++t) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // this wave's copies of tile t have landed
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // everyone's; tile t - 1 is read
-    if (t + 1 < t1) issue(t + 1);
-    if (t * kTileKeys >= wave_max) continue;
-    const lchar* const b = lds + (t & 1) * kBufBytes + 16 * lane;
-    auto operand = [&](int at) { return *reinterpret_cast<const __attribute__((address_space(3))) vec*>(b + at); };
-    // products in groups of four, the operands of the next group read before them
-    auto key = [&](int i) {  // operand i: step i / 2, key block i % 2
-      return operand(i < 16 ? 1024 * (8 * (i & 1) + (i >> 1)) : 2 * kTileKBytes + 1024 * (4 * (i & 1) + (i >> 1) - 8));
-    };
-    f32x16 x[2] = {};
-    vec w[2][4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) w[0][k] = key(k);
-#pragma unroll
-    for (int i = 0; i < 6; ++i) {
-      if (i < 5) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[(i + 1) & 1][k] = key(4 * (i + 1) + k);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int st = (4 * i + k) >> 1;
-        x[k & 1] = Mm<T>::mma(w[i & 1][k], st < 8 ? qn[st] : qr[st - 8], x[k & 1]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    vec v[2][4];
-#pragma unroll
-    for (int d = 0; d < 4; ++d) v[0][d] = operand(kTileKBytes + 1024 * (4 * d));
-    __builtin_amdgcn_sched_barrier(0);
-    settle2(x[0], x[1]);
-    if ((t + 1) * kTileKeys > wave_min) {
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          x[kb][e] = t * kTileKeys + 32 * kb + 8 * (e >> 2) + 4 * g + (e & 3) < lim ? x[kb][e] : -INFINITY;
-    }
-    float top = x[0][0];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) top = fmaxf(top, fmaxf(x[0][e], x[1][e]));
-    const auto sw = __builtin_amdgcn_permlane32_swap(u_of(top), u_of(top), false, false);
-    top = fmaxf(f_of(sw[0]), f_of(sw[1])) * sc;
-    if (__builtin_amdgcn_ballot_w64(top > m + kSlack)) {
-      const float up = fmaxf(m, top), a = exp2f(m - up);
-      m = up;
-      l *= a;
-      settle2(o[0], o[1]);
-      settle2(o[2], o[3]);
-#pragma unroll
-      for (int d = 0; d < 4; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[d][e] *= a;
-    }
-    vec pr[4];
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[ks >> 1][8 * (ks & 1) + e], sc, -m));
-        l += w;
-        pr[ks][e] = (elem)w;
-      }
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      if (ks < 3) {
-#pragma unroll
-        for (int d = 0; d < 4; ++d) v[(ks + 1) & 1][d] = operand(kTileKBytes + 1024 * (4 * d + ks + 1));
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int d = 0; d < 4; ++d) o[d] = Mm<T>::mma(v[ks & 1][d], pr[ks], o[d]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
-  if (jw + r32 >= q.n) return;
+// One lane's half of its query's row: the output, or the part of it over one split's keys.
+__device__ inline void store_rows(const PromptProblem& p, int64_t token, int h, int part, int g, f32x16 (&o)[4], float m,
+                                  float l) {
   l = sum_halves(l);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   settle2(o[0], o[1]);
   settle2(o[2], o[3]);
-  const int64_t row = token * p.nh + p.head0 + h;
+  const int64_t row = token * p.nh + h;
   const bool whole = p.splits == 1;
   float* const po = whole ? nullptr : p.part_o + (int64_t)part * p.q.tokens * p.nh * 128;
 #pragma unroll
@@ -308,11 +176,214 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(PromptProblem p) {
   if (!whole && g == 0) p.part_lse[(int64_t)part * p.q.tokens * p.nh + row] = l == 0.f ? -INFINITY : m + log2f(l);
 }
 
+// What one wave holds of its 32 queries. Scores come out transposed (keys in
+// registers, a query per lane), so the softmax's maximum and sum are per lane
+// (and one exchange between the lane halves), and their exponentials are the
+// second product's operand as they are.
+template <typename T>
+struct Wave {
+  typedef typename Mm<T>::vec vec;
+  typedef typename Mm<T>::elem elem;
+  typedef const __attribute__((address_space(3))) vec lvec;
+  vec qn[8], qr[4];
+  vec w[3][4];  // operands of four products, and of the next eight
+  f32x16 x[2];  // scores of a tile, less m
+  vec pr[4];    // their exponentials
+  f32x16 o[4];
+  float m, l;   // running maximum, in base-2 units of the scaled scores; sum over this lane half's keys
+  f32x16 start; // -m: the scores' sums begin with it, so no instruction subtracts it
+
+  __device__ inline void clear() {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) o[d] = f32x16{};
+    start = f32x16{};
+    m = l = 0.f;
+  }
+  // Operand k of group i: groups 0..3 are V (group = step of 16 keys, k = block
+  // of 32 dims), 4..9 the keys (steps 2 (i - 4) + k / 2, key block k % 2).
+  static __device__ inline vec operand(const lchar* b, int i, int k) {
+    if (i < 4) return *reinterpret_cast<lvec*>(b + kTileKBytes + 1024 * (4 * k + i));
+    const int st = 2 * (i - 4) + (k >> 1), kb = k & 1;
+    return *reinterpret_cast<lvec*>(b + (st < 8 ? 1024 * (8 * kb + st) : 2 * kTileKBytes + 1024 * (4 * kb + st - 8)));
+  }
+  __device__ inline void read(const lchar* b, int i) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[i % 3][k] = operand(b, i, k);
+  }
+  // Groups kFrom .. kTo - 1, the operands of each read two groups ahead (those
+  // of the first two are there). V comes from tile bv, keys from bk.
+  template <int kFrom, int kTo>
+  __device__ inline void products(const lchar* bv, const lchar* bk) {
+    if constexpr (kTo > 4) x[0] = x[1] = start;
+#pragma unroll
+    for (int i = kFrom; i < kTo; ++i) {
+      if (i + 2 < kTo) read(i + 2 < 4 ? bv : bk, i + 2);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int st = 2 * (i - 4) + (k >> 1);
+        if (i < 4) o[k] = Mm<T>::mma(w[i % 3][k], pr[i & 3], o[k]);
+        else x[k & 1] = Mm<T>::mma(w[i % 3][k], st < 8 ? qn[st & 7] : qr[st & 3], x[k & 1]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  // Scores -> exponentials. masked: the tile has keys that a token does not see,
+  // from number `see` (less 4 per lane half) on. first: the first tile, which
+  // sets the maximum whatever it is; later ones raise it where theirs is larger
+  // by more than the slack (rarely).
+  __device__ inline void softmax(bool masked, int see, bool first) {
+    settle2(x[0], x[1]);
+    if (masked) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[kb][e] = 32 * kb + 8 * (e >> 2) + (e & 3) < see ? x[kb][e] : -INFINITY;
+    }
+    float a = max3(x[0][0], x[0][1], x[0][2]), b = max3(x[1][0], x[1][1], x[1][2]);
+#pragma unroll
+    for (int e = 3; e < 15; e += 2) {
+      a = max3(a, x[0][e], x[0][e + 1]);
+      b = max3(b, x[1][e], x[1][e + 1]);
+    }
+    a = max3(a, x[0][15], x[1][15]);
+    a = max3(a, b, b);
+    const auto sw = __builtin_amdgcn_permlane32_swap(u_of(a), u_of(a), false, false);
+    const float top = max3(f_of(sw[0]), f_of(sw[1]), f_of(sw[1]));  // less m
+    if (first || __builtin_amdgcn_ballot_w64(top > kSlack)) {
+      const float up = first ? (top == -INFINITY ? 0.f : top) : fmaxf(top, 0.f), f = exp2f(-up);
+      m += up;
+      if (!first) l *= f;  // (f may be infinite then)
+      settle2(o[0], o[1]);
+      settle2(o[2], o[3]);
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          if (!first) o[d][e] *= f;
+          start[e] = -m;
+        }
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[kb][e] -= up;
+    }
+    float sum[4] = {};
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = __builtin_amdgcn_exp2f(x[ks >> 1][8 * (ks & 1) + e]);
+        sum[e & 3] += v;
+        pr[ks][e] = (elem)v;
+      }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  }
+};
+
+// A workgroup's share of the work: kQBlock tokens of one sequence, one head, one
+// of `splits` parts of the keys that they see.
+struct Item {
+  QueryTile q;
+  int h, part, t0, t1;  // head of this launch; key tiles [t0, t1) of the sequence
+  const char *kx, *vx, *rx;
+};
+__device__ inline bool find_item(const PromptProblem& p, Item& it) {
+  // Items in order of head, part and query tile (the last, with the most keys
+  // to see, first), an eighth of them to each XCD: the workgroups that read
+  // one head's keys share an L2.
+  const int64_t items = (int64_t)p.heads * p.splits * p.q_tiles, per = (items + 7) / 8;
+  const int64_t item = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int64_t)(blockIdx.x >> 3) >= per || item >= items) return false;
+  const uint32_t qts = (uint32_t)p.q_tiles, hs = (uint32_t)item / qts;
+  const int qt = (int)(qts - 1 - ((uint32_t)item - hs * qts));
+  it.part = (int)(hs % (uint32_t)p.splits);
+  it.h = (int)(hs / (uint32_t)p.splits);
+  if (p.q_info) it.q = p.q_info[qt];
+  else it.q = QueryTile{qt * kQBlock, (int)p.q.tokens, p.src.region, p.src.region, 0, 0};
+  if (it.q.j0 < 0) return false;
+  const int most = tile_visible(it.q, min(it.q.j0 + kQBlock, it.q.n) - 1);  // visible keys grow with the token
+  const int nt = (int)clamp64((most + kTileKeys - 1) / kTileKeys, 0, p.src.num_tiles - it.q.tile0);
+  it.t0 = (int)((int64_t)nt * it.part / p.splits);
+  it.t1 = (int)((int64_t)nt * (it.part + 1) / p.splits);
+  const int64_t at = (int64_t)it.h * p.src.num_tiles + it.q.tile0;
+  it.kx = static_cast<const char*>(p.kx) + at * kTileKBytes;
+  it.vx = static_cast<const char*>(p.vx) + at * kTileKBytes;
+  it.rx = static_cast<const char*>(p.rope) + it.q.tile0 * kTileRBytes;
+  return true;
+}
+// HBM -> LDS copy of kPieces KB, 1 KB per instruction, as they lie (an
+// instruction's offset moves both addresses). Inline asm without outputs: with
+// the builtin the compiler takes every LDS read behind it to be out of order
+// and waits for all of them where it needs one (5 of 40 products went unhidden).
+// It does not count these copies either: landed() waits for them.
+template <int kPieces>
+__device__ inline void copy_run(lchar* to, const char* from, int lane) {
+  const uint32_t dst = (uint32_t)(uintptr_t)to, off = 16 * lane;
+  static_assert(kPieces == 2 || kPieces == 4, "");
+  if constexpr (kPieces == 4)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024\n\t"
+                 "global_load_lds_dwordx4 %1, %2 offset:2048\n\tglobal_load_lds_dwordx4 %1, %2 offset:3072"
+                 ::"s"(dst), "v"(off), "s"(from) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024"
+                 ::"s"(dst), "v"(off), "s"(from) : "memory", "m0");
+}
+// Tile t into a buffer: K, V and the rope keys, a quarter of each per wave.
+__device__ inline void copy_tile(const Item& it, lchar* b, int t, int wave, int lane) {
+  const int c = kTileKBytes / 4 * wave, r = kTileRBytes / 4 * wave;
+  copy_run<4>(b + c, it.kx + (int64_t)t * kTileKBytes + c, lane);
+  copy_run<4>(b + kTileKBytes + c, it.vx + (int64_t)t * kTileKBytes + c, lane);
+  copy_run<2>(b + 2 * kTileKBytes + r, it.rx + (int64_t)t * kTileRBytes + r, lane);
+}
+__device__ inline void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// 4 waves, two workgroups per CU, whose waves overlap each other's softmax and products.
+template <typename T>
+__global__ __launch_bounds__(256, 2) void prompt_kernel(PromptProblem p) {
+  extern __shared__ __attribute__((aligned(1024))) char prompt_lds[];
+  lchar* const lds = (lchar*)prompt_lds;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int r32 = lane & 31, g = lane >> 5;
+  Item it;
+  if (!find_item(p, it)) return;
+  const int jw = it.q.j0 + kQRows * wave;  // this wave's first token
+  const int j = min(jw + r32, it.q.n - 1);
+  const int lim = tile_visible(it.q, j);
+  const int wave_max = jw < it.q.n ? tile_visible(it.q, min(jw + kQRows, it.q.n) - 1) : 0;
+  const int wave_min = tile_visible(it.q, min(jw, it.q.n - 1));
+  if (it.t0 < it.t1) copy_tile(it, lds + (it.t0 & 1) * kBufBytes, it.t0, wave, lane);
+  const int64_t token = it.q.token0 + j;
+  Wave<T> w;
+  load_query<T>(p, token, p.head0 + it.h, clamp64(it.q.L - it.q.n + j, 0, INT32_MAX), g, w.qn, w.qr);
+  w.clear();
+  for (int t = it.t0; t < it.t1; ++t) {
+    landed();  // this wave's copies of tile t
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // everyone's; tile t - 1 is read
+    if (t + 1 < it.t1) copy_tile(it, lds + ((t + 1) & 1) * kBufBytes, t + 1, wave, lane);
+    if (t * kTileKeys >= wave_max) continue;
+    const lchar* const b = lds + (t & 1) * kBufBytes + 16 * lane;
+    w.read(b, 4);
+    w.read(b, 5);
+    __builtin_amdgcn_s_setprio(1);  // products first: the other wave of the SIMD has vector work in their shadow
+    w.template products<4, 10>(b, b);
+    __builtin_amdgcn_s_setprio(0);
+    w.read(b, 0);
+    w.read(b, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    w.softmax((t + 1) * kTileKeys > wave_min, lim - t * kTileKeys - 4 * g, t == it.t0);
+    __builtin_amdgcn_s_setprio(1);
+    w.template products<0, 4>(b, b);
+    __builtin_amdgcn_s_setprio(0);
+  }
+  if (jw + r32 < it.q.n) store_rows(p, token, p.head0 + it.h, it.part, g, w.o, w.m, w.l);
+}
+
 template <typename T>
 hipError_t prompt_t(const PromptProblem& p, hipStream_t stream) {
   constexpr int lds = 2 * kBufBytes;
   static OncePerDevice once;
-  hipError_t e = allow_lds(once, reinterpret_cast<const void*>(prompt_kernel<T>), lds);
+  const hipError_t e = allow_lds(once, reinterpret_cast<const void*>(prompt_kernel<T>), lds);
   if (e != hipSuccess) return e;
   const int64_t items = (int64_t)p.heads * p.splits * p.q_tiles;
   if (items > INT32_MAX - 8) return hipErrorInvalidValue;

@@ -226,6 +226,7 @@ struct ExpandProblem {
   const void* W_UV;
   void* kx;  // [head][tile] operand order
   void* vx;
+  float k_scale;  // times K and the rope keys
   int head0, heads;
 };
 hipError_t launch_gather(const ExpandProblem& p, hipStream_t stream);
@@ -243,7 +244,7 @@ struct PromptProblem {
   const void* rope;
   const QueryTile* q_info;  // q_tiles of them, or nullptr: one sequence, every token sees every row
   int nh, head0, heads;  // weight heads; this launch's
-  float scale_log2;
+  float q_scale;  // times the queries (1: the keys are scaled already)
   void* out;  // (tokens, nh, 128) in out_dtype
   int out_dtype;
   int splits;  // > 1: partial sums below, joined by launch_join
