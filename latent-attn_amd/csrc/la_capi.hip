@@ -561,11 +561,40 @@ struct Prefill {
   PrefillForm form = kPrefillNone;
   QuerySource q{};
   RowSource src{};
-  int block_size = 0, blocks_per_seq = 0;  // of the absorbed form
+  int block_size = 0, blocks_per_seq = 0, used_blocks = 0;  // of the absorbed form
   int64_t pool_rows = 0;
   int splits = 1, group = 0;  // of the expanded form: key parts, heads at a time
   int64_t q_tiles = 0;
 };
+
+// The decode step of the absorbed form: every token a sequence with its own visible rows.
+la_decode_args token_step(const la_prefill_args* a, const Prefill& p, const float* q_nope, const float* q_rope,
+                          const int32_t* lens, const int32_t* table, float* out, void* ws, size_t ws_bytes) {
+  la_decode_args d{};
+  d.kv_cache = a->kv_cache;
+  d.kv_dtype = a->kv_dtype;
+  d.total_rows = p.pool_rows;
+  d.num_seqs = (int32_t)a->tokens;
+  d.queries_per_seq = 1;
+  d.q_nope = q_nope;
+  d.q_rope = q_rope;
+  d.W_UK = a->W_UK;
+  d.w_uk_dtype = a->w_uk_dtype;
+  d.W_UV = a->W_UV;
+  d.w_uv_dtype = a->w_uv_dtype;
+  d.rope_cos = a->rope_cos;
+  d.rope_sin = a->rope_sin;
+  d.rope_rows = a->rope_rows;
+  d.output = out;
+  d.cfg = a->cfg;
+  d.seq_lens = lens;
+  d.block_table = table;
+  d.block_size = p.block_size;
+  d.blocks_per_seq = p.blocks_per_seq;
+  d.workspace = ws;
+  d.workspace_bytes = ws_bytes;
+  return d;
+}
 
 int prepare_prefill(const la_prefill_args* a, Prefill* out) {
   if (!a || !valid_cfg(&a->cfg) || !valid_cache_dtype(a->kv_dtype) || !valid_dtype(a->w_uk_dtype) ||
@@ -653,7 +682,7 @@ int prepare_prefill(const la_prefill_args* a, Prefill* out) {
   }
   bool absorbed_ok = p.block_size > 0 && r.region > 0 && p.pool_rows / p.block_size <= INT32_MAX;
   if (absorbed_ok) {
-    p.blocks_per_seq = (r.region + p.block_size - 1) / p.block_size;
+    p.blocks_per_seq = p.used_blocks = (r.region + p.block_size - 1) / p.block_size;
     absorbed_ok = a->tokens * p.blocks_per_seq <= INT32_MAX &&
                   (int64_t)p.blocks_per_seq * p.block_size <= INT32_MAX;
   }
@@ -675,6 +704,25 @@ int prepare_prefill(const la_prefill_args* a, Prefill* out) {
     return LA_ERROR_NOT_SUPPORTED;
   }
 
+  if (p.form == kPrefillAbsorbed) {
+    // The decode plan cuts filled rows where it has four chunks per sequence,
+    // which the rounding of its chunks can miss by little (16 x 4 tokens over 500
+    // to 6000 rows: 251 chunks for 64 sequences; attention 99.5 us over the
+    // regions): longer regions, whose further blocks are never read, reach it.
+    alignas(256) static const char any[256] = {0};
+    float* const f = reinterpret_cast<float*>(const_cast<char*>(any));
+    const int32_t* const ids = reinterpret_cast<const int32_t*>(any);
+    bool filled = false;
+    for (int more = 0; more < 8 && !filled && a->tokens <= cu_count() / 2; ++more) {
+      p.blocks_per_seq = p.used_blocks + more;
+      if (a->tokens * p.blocks_per_seq > INT32_MAX || (int64_t)p.blocks_per_seq * p.block_size > INT32_MAX) break;
+      const la_decode_args d = token_step(a, p, f, f, ids, ids, f, nullptr, 0);
+      DecodeProblem step;
+      Plan plan;
+      filled = prepare(&d, &step, &plan) == LA_SUCCESS && step.chunk_len < 0;
+    }
+    if (!filled) p.blocks_per_seq = p.used_blocks;
+  }
   if (p.form == kPrefillExpanded) {
     const size_t head_bytes = (size_t)r.num_tiles * kTileKBytes * 2;
     p.group = (int)std::min<size_t>(c.num_heads, std::max<size_t>(1, head_bytes ? kMaxExpanded / head_bytes : c.num_heads));
@@ -688,35 +736,6 @@ int prepare_prefill(const la_prefill_args* a, Prefill* out) {
   }
   *out = p;
   return LA_SUCCESS;
-}
-
-// The decode step of the absorbed form: every token a sequence with its own visible rows.
-la_decode_args token_step(const la_prefill_args* a, const Prefill& p, const float* q_nope, const float* q_rope,
-                          const int32_t* lens, const int32_t* table, float* out, void* ws, size_t ws_bytes) {
-  la_decode_args d{};
-  d.kv_cache = a->kv_cache;
-  d.kv_dtype = a->kv_dtype;
-  d.total_rows = p.pool_rows;
-  d.num_seqs = (int32_t)a->tokens;
-  d.queries_per_seq = 1;
-  d.q_nope = q_nope;
-  d.q_rope = q_rope;
-  d.W_UK = a->W_UK;
-  d.w_uk_dtype = a->w_uk_dtype;
-  d.W_UV = a->W_UV;
-  d.w_uv_dtype = a->w_uv_dtype;
-  d.rope_cos = a->rope_cos;
-  d.rope_sin = a->rope_sin;
-  d.rope_rows = a->rope_rows;
-  d.output = out;
-  d.cfg = a->cfg;
-  d.seq_lens = lens;
-  d.block_table = table;
-  d.block_size = p.block_size;
-  d.blocks_per_seq = p.blocks_per_seq;
-  d.workspace = ws;
-  d.workspace_bytes = ws_bytes;
-  return d;
 }
 
 // Runs the call, or with run = false counts its workspace into *need.
@@ -845,6 +864,8 @@ int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need)
   t.table = table;
   t.block_size = p.block_size;
   t.blocks_per_seq = p.blocks_per_seq;
+  t.used_blocks = p.used_blocks;
+  t.vec = q_vec(p.q.q_nope, p.q.dtype, p.q.nope_stride, p.q.nope_head) && q_vec(p.q.q_rope, p.q.dtype, p.q.rope_stride, p.q.rope_head);
   const float* const qn = nope_as_is ? static_cast<const float*>(a->q_nope) : q_nope;
   if (p.form == kPrefillPlain) {
     hipError_t r = q_nope ? launch_tokens(t, stream) : hipSuccess;

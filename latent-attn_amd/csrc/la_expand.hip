@@ -141,65 +141,94 @@ __global__ __launch_bounds__(256) void convert_kernel(const void* src, int src_d
 
 // ---- expand ----------------------------------------------------------------------
 
-// One head's 256 weight rows (128 of W_UK, then 128 of W_UV) times kPos rows.
-// 8 waves: a quarter of the weight rows (0, 1: K dims; 2, 3: V dims) by half of
-// the positions each. Stages of 32 latent columns, chunk j of row r at j ^ sw(r).
+// One head's K or V (128 weight rows) of kPos rows: 4 waves, half of the weight
+// rows by half of the positions each, and two workgroups per CU, so that one's
+// products run under the other's stores (a quarter as many cycles) and first
+// copies. Stages of kBk latent columns in LDS, in a ring of three: one is read,
+// two are on their way. 16-byte chunk j of row r lies at j ^ (r / 4 % 4), which
+// the copies' addresses apply, so that 16 rows' chunks fill all banks.
 constexpr int kDc = 512;
 constexpr int kBk = 32;
-constexpr int kStages = 3;
-constexpr int kNRows = 256;
+constexpr int kRing = 3;
+constexpr int kRowBytes = kBk * 2;
+constexpr int kNRows = 128;
 __device__ inline int sw(int r) { return (r >> 2) & 3; }
 
-// The products and stores of one wave (kV: of V dims). Both kinds have the
-// same barriers; each has its own accumulators, since a branch around the
-// products alone made the compiler copy and spill them.
+// kPb blocks of 32 positions per wave, kPb tiles per workgroup; kV: V (the
+// accumulators hold positions by dims), else K (dims by positions).
 template <typename T, int kPb, bool kV>
-__device__ inline void expand_wave(const ExpandProblem& p, const char* const (&src)[(kPb + 4) / 2], lchar* L, int lane,
-                                   int wave, int h, int64_t tile0) {
+__device__ inline void expand_block(const ExpandProblem& p, int h, int64_t tile0) {
   typedef typename Mm<T>::vec vec;
   typedef typename Mm<T>::elem elem;
+  typedef const __attribute__((address_space(3))) vec lvec;
   constexpr int kPos = 64 * kPb;
-  constexpr int kStageBytes = (kPos + kNRows) * kBk * 2;
-  constexpr int kCopies = (kPb + 4) / 2;
+  constexpr int kStageBytes = (kPos + kNRows) * kRowBytes;
+  constexpr int kCopies = kStageBytes / 1024 / 4;  // of 1 KB (16 rows) per wave and stage
+  static_assert(kCopies * 4 * 16 == kPos + kNRows, "every row of a stage is copied once");
   constexpr int stages = kDc / kBk;
+  extern __shared__ __attribute__((aligned(1024))) char expand_lds[];
+  lchar* const L = (lchar*)expand_lds;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  // rows past the last tile (whose products nobody stores) read the last row
+  const int rows = (int)clamp64((p.src.num_tiles - tile0) * kTileKeys, 0, kPos);
+  const char* const X = static_cast<const char*>(p.rows_c) + tile0 * kTileCBytes;
+  const char* const W = static_cast<const char*>(kV ? p.W_UV : p.W_UK) + (int64_t)(p.head0 + h) * 128 * kDc * 2;
+  const char* base[kCopies];
+  uint32_t off[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    const int r0 = 16 * (kCopies * wave + i);  // a copy's rows are all X's or all W's
+    const int r = lane >> 2;
+    base[i] = r0 < kPos ? X : W + (r0 - kPos) * (kDc * 2);
+    off[i] = (uint32_t)((r0 < kPos ? min(r0 + r, rows - 1) : r) * (kDc * 2) + 16 * ((lane & 3) ^ sw(r)));
+  }
+  // inline asm without outputs: behind the builtin the compiler waits for every LDS read at once
   auto issue = [&](int k) {
-    const int buf = (k % kStages) * kStageBytes;
+    const uint32_t buf = (uint32_t)(uintptr_t)L + k % kRing * kStageBytes + 1024 * kCopies * wave;
     const int kk = min(k, stages - 1);  // past the end: the last stage again, never read
 #pragma unroll
     for (int i = 0; i < kCopies; ++i)
-      __builtin_amdgcn_global_load_lds(src[i] + kk * (kBk * 2), (lds_void*)(L + buf + 1024 * (kCopies * wave + i)), 16, 0, 0);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(buf + 1024 * i), "v"(off[i]),
+                   "s"(base[i] + kk * kRowBytes)
+                   : "memory", "m0");
   };
-  const int wn = wave & 3, wp = wave >> 2;  // weight quarter, position half
+  const int wn = wave & 1, wp = wave >> 1;  // half of the weight rows, half of the positions
   const int r32 = lane & 31, g = lane >> 5;
+  const lchar* const wr = L + (kPos + 64 * wn + r32) * kRowBytes;
+  const lchar* const xr = L + (32 * kPb * wp + r32) * kRowBytes;
   f32x16 acc[kPb][2] = {};
+  vec w[2][2], x[2][kPb];
   issue(0);
   issue(1);
+#pragma unroll 1
   for (int k = 0; k < stages; ++k) {
-    __builtin_amdgcn_s_waitcnt(0x0F70 | kCopies);  // this wave's copies of stage k have landed
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // everyone's; stage k - 1 is read
+    // this wave's copies of stage k have landed (those of the next are on their way)
+    if constexpr (kCopies == 6) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    static_assert(kCopies == 6 || kCopies == 4, "the waits above");
+    asm volatile("s_barrier" ::: "memory");  // everyone's; stage k - 1 is read
     issue(k + 2);
-    const lchar* S = L + (k % kStages) * kStageBytes;
+    const int at = k % kRing * kStageBytes;
+    auto read = [&](int ks) {
+      const int c = at + 16 * ((2 * ks + g) ^ sw(r32));
 #pragma unroll
-    for (int ks = 0; ks < kBk / 16; ++ks) {
-      vec w[2], x[kPb];
+      for (int j = 0; j < 2; ++j) w[ks][j] = *reinterpret_cast<lvec*>(wr + 32 * j * kRowBytes + c);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int r = kPos + 64 * wn + 32 * j + r32;
-        w[j] = *reinterpret_cast<const __attribute__((address_space(3))) vec*>(S + r * 64 + 16 * ((2 * ks + g) ^ sw(r)));
-      }
+      for (int i = 0; i < kPb; ++i) x[ks][i] = *reinterpret_cast<lvec*>(xr + 32 * i * kRowBytes + c);
+    };
+    read(0);
 #pragma unroll
-      for (int i = 0; i < kPb; ++i) {
-        const int r = 32 * kPb * wp + 32 * i + r32;
-        x[i] = *reinterpret_cast<const __attribute__((address_space(3))) vec*>(S + r * 64 + 16 * ((2 * ks + g) ^ sw(r)));
-      }
+    for (int ks = 0; ks < 2; ++ks) {
+      if (ks == 0) read(1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < kPb; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          acc[i][j] = kV ? Mm<T>::mma(x[i], w[j], acc[i][j]) : Mm<T>::mma(w[j], x[i], acc[i][j]);
+        for (int j = 0; j < 2; ++j) acc[i][j] = kV ? Mm<T>::mma(x[ks][i], w[ks][j], acc[i][j]) : Mm<T>::mma(w[ks][j], x[ks][i], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // the copies past the end have landed: the workgroup may end
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end have landed: the workgroup may end
 #pragma unroll
   for (int i = 0; i < kPb; ++i)
 #pragma unroll
@@ -219,57 +248,50 @@ __device__ inline void expand_wave(const ExpandProblem& p, const char* const (&s
         vec v;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = (elem)(kV ? acc[i][j][8 * q + e] : acc[i][j][8 * q + e] * p.k_scale);
-        const int db = 2 * (wn & 1) + j;  // block of 32 dims
+        const int db = 2 * wn + j;  // block of 32 dims
         const int piece = kV ? 4 * db + 2 * (pb & 1) + q : 8 * (pb & 1) + 2 * db + q;
         *reinterpret_cast<vec*>(out + piece * 1024 + 16 * lane) = v;
       }
   }
 }
 
-template <typename T, int kPb>  // kPb blocks of 32 positions per wave, kPb tiles per workgroup
-__global__ __launch_bounds__(512, 2) void expand_kernel(ExpandProblem p) {
-  constexpr int kPos = 64 * kPb;
-  constexpr int kCopies = (kPb + 4) / 2;  // of 1 KB (16 rows) per wave and stage
-  static_assert(kCopies * 8 * 16 == kPos + kNRows, "every row of a stage is copied once");
-  extern __shared__ __attribute__((aligned(1024))) char expand_lds[];
-  lchar* const L = (lchar*)expand_lds;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  // an XCD (id % 8) takes every eighth head and goes through them per position
-  // block: its weights stay in its L2 and each block's rows are fetched once
-  const int nh8 = (p.heads + 7) / 8, x8 = blockIdx.x & 7, k8 = blockIdx.x >> 3;
-  const int h = x8 + 8 * (k8 % nh8);
-  const int64_t tile0 = (int64_t)(k8 / nh8) * kPb;
+// Heads that an XCD takes together.
+__host__ __device__ inline int head_group(int heads) { return heads > 24 ? 4 : (heads + 7) / 8; }
+template <typename T, int kPb>
+__global__ __launch_bounds__(256, 2) void expand_kernel(ExpandProblem p) {
+  // An XCD (id % 8) takes every eighth head, `group` of them through all
+  // positions before the next: their weights (1 MB) stay in its L2, and the rows
+  // pass it once per group (all heads per position block read 16 heads' weights,
+  // more than an L2 holds, again for every block: 13,060 rows of 12 documents, 128
+  // heads, a call 1817 us against 1727).
+  const int64_t blocks = (p.src.num_tiles + kPb - 1) / kPb;
+  const int group = head_group(p.heads);
+  int64_t k = blockIdx.x >> 3;
+  const bool v = k & 1;
+  k >>= 1;
+  const int in_group = (int)(k % group);
+  k /= group;
+  const int64_t tile0 = k % blocks * kPb;
+  const int h = (int)(blockIdx.x & 7) + 8 * ((int)(k / blocks) * group + in_group);
   if (h >= p.heads) return;
   int any = 0;
 #pragma unroll
   for (int i = 0; i < kPb; ++i) any |= tile0 + i < p.src.num_tiles ? p.tile_rows[tile0 + i] : 0;
   if (any == 0) return;
-  const int64_t row_last = p.src.num_tiles * kTileKeys - 1;
-  const char* const WK = static_cast<const char*>(p.W_UK) + (int64_t)(p.head0 + h) * 128 * kDc * 2;
-  const char* const WV = static_cast<const char*>(p.W_UV) + (int64_t)(p.head0 + h) * 128 * kDc * 2;
-  const char* src[kCopies];
-#pragma unroll
-  for (int i = 0; i < kCopies; ++i) {
-    const int r = 16 * (kCopies * wave + i) + (lane >> 2);
-    const int64_t xr = tile0 * kTileKeys + r;
-    const char* row = r < kPos ? static_cast<const char*>(p.rows_c) + (xr < row_last ? xr : row_last) * (kDc * 2)
-                      : r < kPos + 128 ? WK + (int64_t)(r - kPos) * (kDc * 2)
-                                       : WV + (int64_t)(r - kPos - 128) * (kDc * 2);
-    src[i] = row + 16 * ((lane & 3) ^ sw(r));
-  }
-  if ((wave & 3) >= 2) expand_wave<T, kPb, true>(p, src, L, lane, wave, h, tile0);
-  else expand_wave<T, kPb, false>(p, src, L, lane, wave, h, tile0);
+  if (v) expand_block<T, kPb, true>(p, h, tile0);
+  else expand_block<T, kPb, false>(p, h, tile0);
 }
 
 template <typename T, int kPb>
 hipError_t expand_pb(const ExpandProblem& p, hipStream_t stream) {
-  constexpr int lds = kStages * (64 * kPb + kNRows) * kBk * 2;
+  constexpr int lds = kRing * (64 * kPb + kNRows) * kRowBytes;
   static OncePerDevice once;
   hipError_t e = allow_lds(once, reinterpret_cast<const void*>(expand_kernel<T, kPb>), lds);
   if (e != hipSuccess) return e;
-  const int64_t blocks = 8 * (int64_t)((p.heads + 7) / 8) * ((p.src.num_tiles + kPb - 1) / kPb);
+  const int group = head_group(p.heads);
+  const int64_t blocks = 16LL * ((p.heads + 8 * group - 1) / (8 * group) * group) * ((p.src.num_tiles + kPb - 1) / kPb);
   if (blocks > INT32_MAX) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((expand_kernel<T, kPb>), dim3((unsigned)blocks), dim3(512), lds, stream, p);
+  hipLaunchKernelGGL((expand_kernel<T, kPb>), dim3((unsigned)blocks), dim3(256), lds, stream, p);
   return hipGetLastError();
 }
 

@@ -38,14 +38,30 @@ __device__ inline float step_lse(const DecodeProblem& p, int64_t row, int l32) {
   return m + log2f(sum32(l));
 }
 
-// 32 lanes per query row, four values each at a time where rows are whole vectors.
+// 32 lanes per query row, four values each at a time where rows are whole
+// vectors. The decode results go out before the log-sum-exps are known: those
+// take several dependent loads, which are most of the kernel's time.
 template <bool kVec>
 __global__ __launch_bounds__(256) void join_kernel(JoinProblem p) {
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int l32 = threadIdx.x & 31;
   if (row >= p.rows) return;
+  constexpr int kN = kVec ? 4 : 1;
+  struct Part {
+    float v[kN];
+  };
+  auto load = [](const float* o) {
+    Part r;
+    if constexpr (kVec) __builtin_memcpy(r.v, __builtin_assume_aligned(o, 16), 16);
+    else r.v[0] = *o;
+    return r;
+  };
+  Part first[2] = {};
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (p.step[i].num_seqs > 0 && l32 * kN < p.dv) first[i] = load(p.step_out[i] + row * p.dv + l32 * kN);
   // lane i holds part i's weight
-  float e = l32 < p.splits ? p.part_lse[(int64_t)l32 * p.rows + row] : -INFINITY;
+  const float e = l32 < p.splits ? p.part_lse[(int64_t)l32 * p.rows + row] : -INFINITY;
   float es[2] = {-INFINITY, -INFINITY};
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -57,23 +73,18 @@ __global__ __launch_bounds__(256) void join_kernel(JoinProblem p) {
   const float total = sum32(w) + ws[0] + ws[1];
   const float inv = total == 0.f ? 0.f : 1.f / total;
   const int base = threadIdx.x & 32;
-  constexpr int kN = kVec ? 4 : 1;
   for (int d = l32 * kN; d < p.dv; d += 32 * kN) {
     float acc[kN] = {};
-    auto add = [&](float f, const float* o) {
-      if (f == 0.f) return;  // its values may be anything
-      if constexpr (kVec) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(o);
+    auto add = [&](float f, const Part& o) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) acc[k] += f * v[k];
-      } else {
-        acc[0] += f * o[0];
-      }
+      for (int k = 0; k < kN; ++k) acc[k] += f == 0.f ? 0.f : f * o.v[k];  // (a part without weight may hold anything)
     };
-    for (int i = 0; i < p.splits; ++i) add(__shfl(w, base + i, 64), p.part_o + ((int64_t)i * p.rows + row) * p.dv + d);
+#pragma unroll 4
+    for (int i = 0; i < p.splits; ++i)
+      add(__shfl(w, base + i, 64), load(p.part_o + ((int64_t)i * p.rows + row) * p.dv + d));
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      if (p.step[i].num_seqs > 0) add(ws[i], p.step_out[i] + row * p.dv + d);
+      if (p.step[i].num_seqs > 0) add(ws[i], d == l32 * kN ? first[i] : load(p.step_out[i] + row * p.dv + d));
     const int64_t at = row * p.dv + d;
 #pragma unroll
     for (int k = 0; k < kN; ++k) {

@@ -483,43 +483,59 @@ __global__ __launch_bounds__(256) void generic_prompt_kernel(GenericPrompt p) {
 
 // ---- queries of the absorbed forms ------------------------------------------------------------------
 
-// kTokenElems elements of a token's queries per workgroup (x: token, y: share);
-// the first also writes its length and table.
+// kTokenElems elements of a token's nope queries, and as many pairs of rope
+// ones, per workgroup (x: token, y: share), four at a time where heads and
+// strides are whole vectors; the first also writes its length and table.
 constexpr int kTokenElems = 2048;
+template <int kN>
+__device__ inline void load_n(const void* base, int dtype, int64_t i, float (&x)[kN]) {
+  if constexpr (kN == 4) load_q4(base, dtype, i, true, x);
+  else x[0] = load_any(base, dtype, i);
+}
+template <int kN>
 __global__ __launch_bounds__(256) void tokens_kernel(TokenProblem p) {
   const int64_t token = blockIdx.x;
   const int s = query_seq(p.q, token);
   const int n = query_count(p.q, s);
   const int64_t j = token - query_begin(p.q, s);
   const int L = j >= 0 && j < n ? source_rows(p.src, s) : 0;  // malformed offsets leave tokens without a sequence
-  const int first = blockIdx.y * kTokenElems + threadIdx.x, last = (blockIdx.y + 1) * kTokenElems;
+  const int first = blockIdx.y * kTokenElems + kN * threadIdx.x, last = (blockIdx.y + 1) * kTokenElems;
   if (p.lens && first == 0) p.lens[token] = L > 0 ? visible_keys(p.q, s, (int)j, n, L) : 0;
   if (p.table && blockIdx.y == 0) {
     int32_t* const t = p.table + token * p.blocks_per_seq;
     for (int i = threadIdx.x; i < p.blocks_per_seq; i += 256)
-      t[i] = L == 0                 ? 0
-             : p.src.block_table ? p.src.block_table[(int64_t)s * p.src.blocks_per_seq + i]
-                                 : (int32_t)((int64_t)s * p.src.stride_rows / p.block_size + i);
+      t[i] = L == 0 || i >= p.used_blocks ? 0
+             : p.src.block_table         ? p.src.block_table[(int64_t)s * p.src.blocks_per_seq + i]
+                                         : (int32_t)((int64_t)s * p.src.stride_rows / p.block_size + i);
   }
   if (p.q_nope)
-    for (int i = first; i < min(p.nh * p.dn, last); i += 256)
-      p.q_nope[token * p.nh * p.dn + i] =
-          load_any(p.q.q_nope, p.q.dtype, token * p.q.nope_stride + (i / p.dn) * p.q.nope_head + i % p.dn);
+    for (int i = first; i < min(p.nh * p.dn, last); i += 256 * kN) {
+      float x[kN];
+      load_n<kN>(p.q.q_nope, p.q.dtype, token * p.q.nope_stride + (i / p.dn) * p.q.nope_head + i % p.dn, x);
+#pragma unroll
+      for (int e = 0; e < kN; ++e) p.q_nope[token * p.nh * p.dn + i + e] = x[e];
+    }
   if (p.q_rope) {
     const int half = p.dR / 2;
     const int64_t at = L == 0 ? 0 : source_rope_row(p.src, clamp64(L - n + j, 0, INT32_MAX)) * half;
-    for (int i = first; i < min(p.nh * half, last); i += 256) {
+    for (int i = first; i < min(p.nh * half, last); i += 256 * kN) {
       const int h = i / half, d = i % half;
       const int64_t ar = token * p.q.rope_stride + h * p.q.rope_head + d;
-      float a = load_any(p.q.q_rope, p.q.dtype, ar), b = load_any(p.q.q_rope, p.q.dtype, ar + half);
-      if (p.q.rotate) {
-        const float c = p.src.cos[at + d], sn = p.src.sin[at + d], x = a, y = b;
-        a = x * c - y * sn;
-        b = x * sn + y * c;
-      }
+      float a[kN], b[kN];
+      load_n<kN>(p.q.q_rope, p.q.dtype, ar, a);
+      load_n<kN>(p.q.q_rope, p.q.dtype, ar + half, b);
       float* const o = p.q_rope + (token * p.nh + h) * p.dR + d;
-      o[0] = a;
-      o[half] = b;
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        const float x = a[e], y = b[e];
+        if (p.q.rotate) {
+          const float c = p.src.cos[at + d + e], sn = p.src.sin[at + d + e];
+          a[e] = x * c - y * sn;
+          b[e] = x * sn + y * c;
+        }
+        o[e] = a[e];
+        o[half + e] = b[e];
+      }
     }
   }
 }
@@ -554,7 +570,9 @@ hipError_t launch_tokens(const TokenProblem& p, hipStream_t stream) {
   const int elems = p.nh * (p.dn > p.dR / 2 ? p.dn : p.dR / 2);
   const unsigned shares = (unsigned)((elems + kTokenElems - 1) / kTokenElems);
   if (shares > 65535) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(tokens_kernel, dim3((unsigned)p.q.tokens, shares), dim3(256), 0, stream, p);
+  const dim3 grid((unsigned)p.q.tokens, shares);
+  if (p.vec && p.dn % 4 == 0 && p.dR % 8 == 0) hipLaunchKernelGGL(tokens_kernel<4>, grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL(tokens_kernel<1>, grid, dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 

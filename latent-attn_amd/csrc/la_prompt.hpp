@@ -298,8 +298,9 @@ struct TokenProblem {
   float* q_nope;   // (tokens, nh, dn), or nullptr
   float* q_rope;   // (tokens, nh, dR), or nullptr
   int32_t* lens;   // (tokens), or nullptr
-  int32_t* table;  // (tokens, blocks_per_seq)
-  int block_size, blocks_per_seq;
+  int32_t* table;  // (tokens, blocks_per_seq), entries past used_blocks are never read
+  int block_size, blocks_per_seq, used_blocks;
+  int vec;  // queries are whole-vector aligned
 };
 hipError_t launch_tokens(const TokenProblem& p, hipStream_t stream);
 // fp32 -> out_dtype
