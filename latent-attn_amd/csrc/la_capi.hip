@@ -471,6 +471,17 @@ int scratch_ptr(void** out) {
 bool tables_aligned(const RowSource& r) {
   return ((reinterpret_cast<uintptr_t>(r.cos) | reinterpret_cast<uintptr_t>(r.sin)) & 15) == 0;
 }
+// Parts that the keys of `tiles` tiles are cut into when `blocks` workgroups
+// would run: one workgroup per CU, down to two tiles each, and two per CU where
+// each keeps 16 tiles (partial rows cost a workgroup and the join as much as
+// several tiles; a step of 32 tokens over 16 heads x 8192 shared rows 50 us with
+// 32 parts, 46 with 16; 64 tokens over 128 heads 177 with 4, 183 with 2).
+int key_splits(int64_t blocks, int64_t tiles, int least) {
+  const int64_t ncu = cu_count();
+  const int64_t two = (2 * ncu + blocks - 1) / blocks, one = (ncu + blocks - 1) / blocks;
+  const int64_t n = tiles >= 16 * two ? two : std::min(one, tiles / 2);
+  return (int)std::max<int64_t>(least, std::min<int64_t>(n, 32));
+}
 bool valid_out(int d) { return valid_dtype(d); }
 // Head shape of the expanded form's kernels.
 bool expanded_dims(const la_mla_config& c) {
@@ -727,11 +738,8 @@ int prepare_prefill(const la_prefill_args* a, Prefill* out) {
     const size_t head_bytes = (size_t)r.num_tiles * kTileKBytes * 2;
     p.group = (int)std::min<size_t>(c.num_heads, std::max<size_t>(1, head_bytes ? kMaxExpanded / head_bytes : c.num_heads));
         p.q_tiles = query_tiles(q, prompt_query_rows());
-    // few query tiles leave CUs idle: their keys are cut into parts of at least four tiles
-    const int64_t blocks = p.q_tiles * p.group;
     const int64_t tiles = a->seq_offsets ? a->total_rows / a->num_seqs / kTileKeys + 1 : r.num_tiles / a->num_seqs;
-    const int64_t want = (2 * cu_count() + blocks - 1) / blocks;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, tiles / 4, 32}));
+    p.splits = key_splits(p.q_tiles * p.group, tiles, 1);
     if ((int64_t)p.group * p.splits * p.q_tiles > INT32_MAX - 8) return LA_ERROR_NOT_SUPPORTED;
   }
   *out = p;
@@ -987,7 +995,14 @@ int decode_shared(const la_shared_args* a, hipStream_t stream, bool run_it, size
   const bool expanded_ok = a->expanded && (reinterpret_cast<uintptr_t>(a->expanded) & (kAlign - 1)) == 0 &&
                            expanded_dims(c) && own.kv_dtype != LA_DTYPE_F32 && device_is_gfx950();
   if (a->kernel_variant == 2 && !expanded_ok) return LA_ERROR_NOT_SUPPORTED;
-  const bool expanded = P > 0 && expanded_ok && (a->kernel_variant == 2 || (a->kernel_variant == 0 && tokens > 48));
+  // Microseconds beside the own rows': over latent rows 25 of launches (queries
+  // absorbed, a merge) and 2.3e-6 per (token, head, row); over the expanded form
+  // its bytes at 5 TB/s (128 heads x 8192 rows, a step with 16 / 32 / 48 / 64
+  // tokens: 97 / 131 / 189 / 218 over latent rows, 131 / 140 / 157 / 163 expanded;
+  // 2000 rows, 16 tokens 74 / 58; 16 heads x 8192 rows, 32 tokens 66 / 50).
+  const double pairs = (double)nh * P;
+  const bool expanded = P > 0 && expanded_ok &&
+                        (a->kernel_variant == 2 || (a->kernel_variant == 0 && pairs * 512. / 5e6 < 25. + 2.3e-6 * pairs * tokens));
 
   PromptProblem m{};
   la_decode_args pre{};
@@ -1013,9 +1028,7 @@ int decode_shared(const la_shared_args* a, hipStream_t stream, bool run_it, size
     m.nope_vec = q_vec(m.q.q_nope, m.q.dtype, m.q.nope_stride, m.q.nope_head);
     m.rope_vec = q_vec(m.q.q_rope, m.q.dtype, m.q.rope_stride, m.q.rope_head);
     m.table_vec = tables_aligned(m.src);
-    const int64_t blocks = m.q_tiles * nh;
-    m.splits = (int)std::max<int64_t>(
-        2, std::min<int64_t>({(2 * cu_count() + blocks - 1) / blocks, m.src.num_tiles / 4, 32}));
+    m.splits = key_splits(m.q_tiles * nh, m.src.num_tiles, 2);  // 2: a join follows either way
   } else if (P > 0) {
     pre = a->own;
     pre.kv_cache = a->prefix;
