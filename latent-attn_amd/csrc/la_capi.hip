@@ -704,9 +704,16 @@ int prepare_prefill(const la_prefill_args* a, Prefill* out) {
   if (a->kernel_variant != 0) {
     p.form = (PrefillForm)a->kernel_variant;
   } else if (expanded_ok) {
-    // products per head: n tokens over L rows take 131072 n + 1088 n L absorbed, 131072 L + 320 n L expanded
-    const double n = (double)a->tokens / a->num_seqs, rows = (double)std::max(r.region, 1);
-    p.form = absorbed_ok && n * (131072. + 768. * rows) < 131072. * rows ? kPrefillAbsorbed : kPrefillExpanded;
+    // Microseconds of both forms: launches, then absorption and projection per
+    // (token, head) and 1088 products per pair of a token and a row, or expansion
+    // per (row, head) and 320 products per pair (a query tile's worth at least).
+    // Measured (absorbed / expanded, 128 heads): 1 x 16 of 1000 rows 48 / 76, 64 of
+    // 1000 76 / 75, 128 of 1000 111 / 76, 128 of 8192 318 / 475, 200 of 8192 540 /
+    // 560, 16 x 16 of 2000 256 / 1900; 16 heads, 17 of 100 28 / 23.
+    const double heads = c.num_heads, seqs = a->num_seqs, n = (double)a->tokens / seqs, rows = std::max(r.region, 1);
+    const double absorbed_us = 27. + a->tokens * heads * (2e-3 + 2.3e-6 * rows);
+    const double expanded_us = 20. + 1.2 * heads * seqs * rows * (3.1e-4 + 7e-7 * std::max(n, 64.));
+    p.form = absorbed_ok && absorbed_us < expanded_us ? kPrefillAbsorbed : kPrefillExpanded;
   } else if (absorbed_ok) {
     p.form = kPrefillAbsorbed;
   } else if (plain_ok) {
