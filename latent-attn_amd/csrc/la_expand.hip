@@ -39,28 +39,24 @@ struct Mm<__half> {
 // ---- gather --------------------------------------------------------------------
 
 // Eight cache elements as T (an 8-bit cache: bf16, exact).
-template <typename KT, typename T>
-__device__ inline typename Mm<T>::vec load8(const KT* p) {
-  typename Mm<T>::vec v;
-  if constexpr (sizeof(KT) == 2) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = __builtin_bit_cast(typename Mm<T>::elem, p[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (typename Mm<T>::elem)to_f32(p[e]);
-  }
-  return v;
-}
 template <typename KT, typename T, bool kAligned>
-__device__ inline typename Mm<T>::vec load8_row(const KT* p) {
-  if constexpr (kAligned && sizeof(KT) == 2) return *reinterpret_cast<const typename Mm<T>::vec*>(p);
-  if constexpr (kAligned && sizeof(KT) == 1) {
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
-    KT b[8];
-    __builtin_memcpy(b, &w, 8);
-    return load8<KT, T>(b);
+__device__ inline typename Mm<T>::vec load8(const KT* p) {
+  typedef typename Mm<T>::vec vec;
+  KT b[8];
+  if constexpr (kAligned) __builtin_memcpy(b, __builtin_assume_aligned(p, 8 * sizeof(KT)), sizeof(b));
+  else __builtin_memcpy(b, p, sizeof(b));
+  if constexpr (sizeof(KT) == 2) {
+    return __builtin_bit_cast(vec, b);
+  } else {
+    uint32_t w[2], y[4];
+    __builtin_memcpy(w, b, 8);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      y[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], 1.f, false));
+      y[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], 1.f, true));
+    }
+    return __builtin_bit_cast(vec, y);
   }
-  return load8<KT, T>(p);
 }
 
 // kGatherRows rows of a tile per workgroup, a row per wave at a time; the
@@ -97,7 +93,7 @@ __global__ __launch_bounds__(256) void gather_kernel(ExpandProblem p) {
 #pragma unroll
   for (int i = 0; i < kGatherRows / 4; ++i) {
     const int r = part + wave + 4 * i;
-    if (r < rows) v[i] = load8_row<KT, T, kAligned>(kv + source_row(p.src, s, pos0 + r) * p.src.row_elems + 8 * lane);
+    if (r < rows) v[i] = load8<KT, T, kAligned>(kv + source_row(p.src, s, pos0 + r) * p.src.row_elems + 8 * lane);
   }
 #pragma unroll
   for (int i = 0; i < kGatherRows / 4; ++i) {
@@ -141,157 +137,204 @@ __global__ __launch_bounds__(256) void convert_kernel(const void* src, int src_d
 
 // ---- expand ----------------------------------------------------------------------
 
-// One head's K or V (128 weight rows) of kPos rows: 4 waves, half of the weight
-// rows by half of the positions each, and two workgroups per CU, so that one's
-// products run under the other's stores (a quarter as many cycles) and first
-// copies. Stages of kBk latent columns in LDS, in a ring of three: one is read,
-// two are on their way. 16-byte chunk j of row r lies at j ^ (r / 4 % 4), which
-// the copies' addresses apply, so that 16 rows' chunks fill all banks.
+// One head's 256 weight rows (128 of W_UK, then 128 of W_UV) times 64 kPb
+// positions per workgroup of 8 waves: a quarter of the weight rows (0, 1: K
+// dims; 2, 3: V dims) by half of the positions each. Stages of kBk latent
+// columns in a ring in LDS: one is read, the others are on their way. 16-byte
+// chunk j of row r lies at j ^ (r % 8), which the copies' addresses apply, so
+// that 8 rows' chunks fill all banks.
+//
+// The rows and weights that pass the L2 bound it, not its products (with the
+// copies left out 8192 rows x 128 heads took 234 us for 334, with the products
+// left out 301): hence the large tile, and the order in which an XCD takes its
+// items. Large calls run a workgroup per CU, which takes items in turn and has
+// the next one's first stage on its way while it stores (4 tiles); small ones
+// a workgroup per item and tile, with three stages on their way.
 constexpr int kDc = 512;
-constexpr int kBk = 32;
-constexpr int kRing = 3;
+constexpr int kBk = 64;
+constexpr int kStages = kDc / kBk;
 constexpr int kRowBytes = kBk * 2;
-constexpr int kNRows = 128;
-__device__ inline int sw(int r) { return (r >> 2) & 3; }
+constexpr int kNRows = 256;
+template <int kPb>
+struct Geometry {  // kPb tiles per item, blocks of 32 positions per wave
+  static constexpr int kPos = 64 * kPb;
+  static constexpr int kRing = kPb == 4 ? 2 : 4;
+  static constexpr int kStageBytes = (kPos + kNRows) * kRowBytes;
+  static constexpr int kCopies = kStageBytes / 1024 / 8;  // of 1 KB (8 rows) per wave and stage
+  static constexpr int kStores = 4 * kPb;                  // of a wave and item
+  static_assert(kCopies * 8 * 8 == kPos + kNRows, "every row of a stage is copied once");
+};
+// Heads that an XCD takes together: their weights (1 MB) stay in its L2 while
+// all rows pass, once per group (all 16 heads of an XCD per block of rows: more
+// weights than an L2 holds, again for every block).
+__host__ __device__ inline int head_group(int heads) { return heads > 24 ? 4 : (heads + 7) / 8; }
+__host__ __device__ inline int64_t items_per_xcd(int heads, int64_t tiles, int pb) {
+  const int group = head_group(heads);
+  return (int64_t)((heads + 8 * group - 1) / (8 * group) * group) * ((tiles + pb - 1) / pb);
+}
 
-// kPb blocks of 32 positions per wave, kPb tiles per workgroup; kV: V (the
-// accumulators hold positions by dims), else K (dims by positions).
+template <int N>
+__device__ inline void wait_copies() {
+  static_assert(N == 0 || N == 10 || N == 16, "");
+  if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  else if constexpr (N == 10) asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+}
+
+// The work of one wave (kV: of V dims). Both kinds have the same barriers; each
+// has its own accumulators, since a branch around the products alone made the
+// compiler copy and spill them.
 template <typename T, int kPb, bool kV>
-__device__ inline void expand_block(const ExpandProblem& p, int h, int64_t tile0) {
+__device__ inline void expand_wave(const ExpandProblem& p, int64_t step, lchar* L, int lane, int wave) {
   typedef typename Mm<T>::vec vec;
   typedef typename Mm<T>::elem elem;
   typedef const __attribute__((address_space(3))) vec lvec;
-  constexpr int kPos = 64 * kPb;
-  constexpr int kStageBytes = (kPos + kNRows) * kRowBytes;
-  constexpr int kCopies = kStageBytes / 1024 / 4;  // of 1 KB (16 rows) per wave and stage
-  static_assert(kCopies * 4 * 16 == kPos + kNRows, "every row of a stage is copied once");
-  constexpr int stages = kDc / kBk;
-  extern __shared__ __attribute__((aligned(1024))) char expand_lds[];
-  lchar* const L = (lchar*)expand_lds;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  // rows past the last tile (whose products nobody stores) read the last row
-  const int rows = (int)clamp64((p.src.num_tiles - tile0) * kTileKeys, 0, kPos);
-  const char* const X = static_cast<const char*>(p.rows_c) + tile0 * kTileCBytes;
-  const char* const W = static_cast<const char*>(kV ? p.W_UV : p.W_UK) + (int64_t)(p.head0 + h) * 128 * kDc * 2;
-  const char* base[kCopies];
-  uint32_t off[kCopies];
+  typedef Geometry<kPb> G;
+  // Items of an XCD (id % 8), every step-th from id / 8 on: head of the group
+  // fastest, then rows, then groups; heads past the last and empty tiles are no items.
+  const int64_t blocks = (p.src.num_tiles + kPb - 1) / kPb, items = items_per_xcd(p.heads, p.src.num_tiles, kPb);
+  const int group = head_group(p.heads);
+  int64_t item = blockIdx.x >> 3, tile0 = 0;
+  int h = 0;
+  auto find = [&]() {  // the first item from `item` on, or items
+    for (; item < items; item += step) {
+      h = (int)(blockIdx.x & 7) + 8 * ((int)(item / group / blocks) * group + (int)(item % group));
+      tile0 = item / group % blocks * kPb;
+      int any = 0;
 #pragma unroll
-  for (int i = 0; i < kCopies; ++i) {
-    const int r0 = 16 * (kCopies * wave + i);  // a copy's rows are all X's or all W's
-    const int r = lane >> 2;
-    base[i] = r0 < kPos ? X : W + (r0 - kPos) * (kDc * 2);
-    off[i] = (uint32_t)((r0 < kPos ? min(r0 + r, rows - 1) : r) * (kDc * 2) + 16 * ((lane & 3) ^ sw(r)));
-  }
+      for (int i = 0; i < kPb; ++i) any |= tile0 + i < p.src.num_tiles ? p.tile_rows[tile0 + i] : 0;
+      if (h < p.heads && any != 0) return;
+    }
+  };
+  const char* base[G::kCopies];
+  uint32_t off[G::kCopies];
+  auto sources = [&] {
+    // rows past the last tile (whose products nobody stores) read the last row
+    const int rows = (int)clamp64((p.src.num_tiles - tile0) * kTileKeys, 0, G::kPos);
+    const char* const X = static_cast<const char*>(p.rows_c) + tile0 * kTileCBytes;
+    const char* const WK = static_cast<const char*>(p.W_UK) + (int64_t)(p.head0 + h) * 128 * kDc * 2;
+    const char* const WV = static_cast<const char*>(p.W_UV) + (int64_t)(p.head0 + h) * 128 * kDc * 2;
+    const int r = lane >> 3;
+#pragma unroll
+    for (int i = 0; i < G::kCopies; ++i) {
+      const int r0 = 8 * (G::kCopies * wave + i);  // a copy's rows are all X's, W_UK's or W_UV's
+      base[i] = r0 < G::kPos ? X : r0 < G::kPos + 128 ? WK + (r0 - G::kPos) * (kDc * 2) : WV + (r0 - G::kPos - 128) * (kDc * 2);
+      off[i] = (uint32_t)((r0 < G::kPos ? min(r0 + r, rows - 1) : r) * (kDc * 2) + 16 * ((lane & 7) ^ r));
+    }
+  };
   // inline asm without outputs: behind the builtin the compiler waits for every LDS read at once
   auto issue = [&](int k) {
-    const uint32_t buf = (uint32_t)(uintptr_t)L + k % kRing * kStageBytes + 1024 * kCopies * wave;
-    const int kk = min(k, stages - 1);  // past the end: the last stage again, never read
+    const uint32_t buf = (uint32_t)(uintptr_t)L + k % G::kRing * G::kStageBytes + 1024 * G::kCopies * wave;
+    const int kk = min(k, kStages - 1);  // past the end (small calls): the last stage again, never read
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i)
+    for (int i = 0; i < G::kCopies; ++i)
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(buf + 1024 * i), "v"(off[i]),
                    "s"(base[i] + kk * kRowBytes)
                    : "memory", "m0");
   };
-  const int wn = wave & 1, wp = wave >> 1;  // half of the weight rows, half of the positions
+  const int wn = wave & 3, wp = wave >> 2;  // weight quarter, position half
   const int r32 = lane & 31, g = lane >> 5;
-  const lchar* const wr = L + (kPos + 64 * wn + r32) * kRowBytes;
+  const lchar* const wr = L + (G::kPos + 64 * wn + r32) * kRowBytes;
   const lchar* const xr = L + (32 * kPb * wp + r32) * kRowBytes;
-  f32x16 acc[kPb][2] = {};
-  vec w[2][2], x[2][kPb];
-  issue(0);
-  issue(1);
+  find();
+  if (item >= items) return;
+  sources();
+#pragma unroll
+  for (int k = 0; k < G::kRing - 1; ++k) issue(k);
+  bool stored = false;  // the copies on their way are behind kStores stores
+  while (true) {
+    f32x16 acc[kPb][2] = {};
+    vec w[2][2], x[2][kPb];
+    const int64_t out_tile = tile0;
+    const int out_h = h;
+    bool more = false;
 #pragma unroll 1
-  for (int k = 0; k < stages; ++k) {
-    // this wave's copies of stage k have landed (those of the next are on their way)
-    if constexpr (kCopies == 6) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
-    else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-    static_assert(kCopies == 6 || kCopies == 4, "the waits above");
-    asm volatile("s_barrier" ::: "memory");  // everyone's; stage k - 1 is read
-    issue(k + 2);
-    const int at = k % kRing * kStageBytes;
-    auto read = [&](int ks) {
-      const int c = at + 16 * ((2 * ks + g) ^ sw(r32));
-#pragma unroll
-      for (int j = 0; j < 2; ++j) w[ks][j] = *reinterpret_cast<lvec*>(wr + 32 * j * kRowBytes + c);
-#pragma unroll
-      for (int i = 0; i < kPb; ++i) x[ks][i] = *reinterpret_cast<lvec*>(xr + 32 * i * kRowBytes + c);
-    };
-    read(0);
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      if (ks == 0) read(1);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < kPb; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = kV ? Mm<T>::mma(x[ks][i], w[ks][j], acc[i][j]) : Mm<T>::mma(w[ks][j], x[ks][i], acc[i][j]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end have landed: the workgroup may end
-#pragma unroll
-  for (int i = 0; i < kPb; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) settle(acc[i][j]);
-  // registers 8 q .. 8 q + 7 of a block are one operand element group (operand
-  // order, la_prompt.hpp): K: a step of 16 dims; V: of 16 keys
-#pragma unroll
-  for (int i = 0; i < kPb; ++i) {
-    const int pb = kPb * wp + i;  // block of 32 positions
-    const int64_t tile = tile0 + pb / 2;
-    if (tile >= p.src.num_tiles) continue;
-    char* const out = static_cast<char*>(kV ? p.vx : p.kx) + ((int64_t)h * p.src.num_tiles + tile) * kTileKBytes;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        vec v;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (elem)(kV ? acc[i][j][8 * q + e] : acc[i][j][8 * q + e] * p.k_scale);
-        const int db = 2 * wn + j;  // block of 32 dims
-        const int piece = kV ? 4 * db + 2 * (pb & 1) + q : 8 * (pb & 1) + 2 * db + q;
-        *reinterpret_cast<vec*>(out + piece * 1024 + 16 * lane) = v;
+    for (int k = 0; k < kStages; ++k) {
+      // this wave's copies of stage k have landed; everyone's, and stage k - 1 is read
+      if (kPb == 4 && k == 0 && stored) wait_copies<G::kRing == 2 ? 16 : 0>();
+      else wait_copies<(G::kRing - 2) * G::kCopies>();
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (kPb == 4 && k == kStages - 1) {
+        item += step;
+        find();
+        more = item < items;
+        if (more) {
+          sources();
+          issue(0);
+        }
+      } else {
+        issue(k + G::kRing - 1);
       }
-  }
-}
-
-// Heads that an XCD takes together.
-__host__ __device__ inline int head_group(int heads) { return heads > 24 ? 4 : (heads + 7) / 8; }
-template <typename T, int kPb>
-__global__ __launch_bounds__(256, 2) void expand_kernel(ExpandProblem p) {
-  // An XCD (id % 8) takes every eighth head, `group` of them through all
-  // positions before the next: their weights (1 MB) stay in its L2, and the rows
-  // pass it once per group (all heads per position block read 16 heads' weights,
-  // more than an L2 holds, again for every block: 13,060 rows of 12 documents, 128
-  // heads, a call 1817 us against 1727).
-  const int64_t blocks = (p.src.num_tiles + kPb - 1) / kPb;
-  const int group = head_group(p.heads);
-  int64_t k = blockIdx.x >> 3;
-  const bool v = k & 1;
-  k >>= 1;
-  const int in_group = (int)(k % group);
-  k /= group;
-  const int64_t tile0 = k % blocks * kPb;
-  const int h = (int)(blockIdx.x & 7) + 8 * ((int)(k / blocks) * group + in_group);
-  if (h >= p.heads) return;
-  int any = 0;
+      const int at = k % G::kRing * G::kStageBytes;
+      auto read = [&](int ks) {
+        const int c = at + 16 * ((2 * ks + g) ^ (r32 & 7));
 #pragma unroll
-  for (int i = 0; i < kPb; ++i) any |= tile0 + i < p.src.num_tiles ? p.tile_rows[tile0 + i] : 0;
-  if (any == 0) return;
-  if (v) expand_block<T, kPb, true>(p, h, tile0);
-  else expand_block<T, kPb, false>(p, h, tile0);
+        for (int j = 0; j < 2; ++j) w[ks & 1][j] = *reinterpret_cast<lvec*>(wr + 32 * j * kRowBytes + c);
+#pragma unroll
+        for (int i = 0; i < kPb; ++i) x[ks & 1][i] = *reinterpret_cast<lvec*>(xr + 32 * i * kRowBytes + c);
+      };
+      read(0);
+#pragma unroll
+      for (int ks = 0; ks < kBk / 16; ++ks) {
+        if (ks + 1 < kBk / 16) read(ks + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < kPb; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            acc[i][j] = kV ? Mm<T>::mma(x[ks & 1][i], w[ks & 1][j], acc[i][j]) : Mm<T>::mma(w[ks & 1][j], x[ks & 1][i], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kPb; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) settle(acc[i][j]);
+    // registers 8 q .. 8 q + 7 of a block are one operand element group (operand
+    // order, la_prompt.hpp): K: a step of 16 dims; V: of 16 keys
+#pragma unroll
+    for (int i = 0; i < kPb; ++i) {
+      const int pb = kPb * wp + i;  // block of 32 positions
+      const int64_t tile = out_tile + pb / 2;
+      if (tile >= p.src.num_tiles) continue;
+      char* const out = static_cast<char*>(kV ? p.vx : p.kx) + ((int64_t)out_h * p.src.num_tiles + tile) * kTileKBytes;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          vec v;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = (elem)(kV ? acc[i][j][8 * q + e] : acc[i][j][8 * q + e] * p.k_scale);
+          const int db = 2 * (wn & 1) + j;  // block of 32 dims
+          const int piece = kV ? 4 * db + 2 * (pb & 1) + q : 8 * (pb & 1) + 2 * db + q;
+          *reinterpret_cast<vec*>(out + piece * 1024 + 16 * lane) = v;
+        }
+    }
+    if (kPb != 4 || !more) break;
+    stored = out_tile + kPb <= p.src.num_tiles;  // all of them: else the next wait takes everything
+  }
+  wait_copies<0>();  // the copies past the end have landed: the workgroup may end
 }
 
 template <typename T, int kPb>
-hipError_t expand_pb(const ExpandProblem& p, hipStream_t stream) {
-  constexpr int lds = kRing * (64 * kPb + kNRows) * kRowBytes;
+__global__ __launch_bounds__(512, 2) void expand_kernel(ExpandProblem p, int64_t step) {
+  extern __shared__ __attribute__((aligned(1024))) char expand_lds[];
+  lchar* const L = (lchar*)expand_lds;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  if ((wave & 3) >= 2) expand_wave<T, kPb, true>(p, step, L, lane, wave);
+  else expand_wave<T, kPb, false>(p, step, L, lane, wave);
+}
+
+template <typename T, int kPb>
+hipError_t expand_pb(const ExpandProblem& p, hipStream_t stream, int ncu) {
+  constexpr int lds = Geometry<kPb>::kRing * Geometry<kPb>::kStageBytes;
   static OncePerDevice once;
   hipError_t e = allow_lds(once, reinterpret_cast<const void*>(expand_kernel<T, kPb>), lds);
   if (e != hipSuccess) return e;
-  const int group = head_group(p.heads);
-  const int64_t blocks = 16LL * ((p.heads + 8 * group - 1) / (8 * group) * group) * ((p.src.num_tiles + kPb - 1) / kPb);
-  if (blocks > INT32_MAX) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((expand_kernel<T, kPb>), dim3((unsigned)blocks), dim3(256), lds, stream, p);
+  int64_t per_xcd = items_per_xcd(p.heads, p.src.num_tiles, kPb);
+  if (kPb == 4) per_xcd = per_xcd < (ncu + 7) / 8 ? per_xcd : (ncu + 7) / 8;
+  if (8 * per_xcd > INT32_MAX) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((expand_kernel<T, kPb>), dim3((unsigned)(8 * per_xcd)), dim3(512), lds, stream, p, per_xcd);
   return hipGetLastError();
 }
 
@@ -320,8 +363,8 @@ hipError_t launch_gather(const ExpandProblem& p, hipStream_t stream) {
 hipError_t launch_expand(const ExpandProblem& p, hipStream_t stream, int ncu) {
   if (p.src.num_tiles == 0 || p.heads == 0) return hipSuccess;
   const bool wide = (int64_t)p.heads * ((p.src.num_tiles + 3) / 4) >= ncu;
-  if (p.f16) return wide ? expand_pb<__half, 4>(p, stream) : expand_pb<__half, 2>(p, stream);
-  return wide ? expand_pb<__hip_bfloat16, 4>(p, stream) : expand_pb<__hip_bfloat16, 2>(p, stream);
+  if (p.f16) return wide ? expand_pb<__half, 4>(p, stream, ncu) : expand_pb<__half, 1>(p, stream, ncu);
+  return wide ? expand_pb<__hip_bfloat16, 4>(p, stream, ncu) : expand_pb<__hip_bfloat16, 1>(p, stream, ncu);
 }
 
 hipError_t launch_convert(const void* src, int src_dtype, void* dst, int f16, int64_t n, hipStream_t stream) {
