@@ -849,6 +849,9 @@ int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need)
     for (int h = 0; h < nh && r == hipSuccess; h += p.group) {
       e.p.head0 = m.head0 = h;
       e.p.heads = m.heads = std::min(p.group, nh - h);
+      // (128 heads, a call by head / by tile: 300 rows 45 / 41 us, 1001 121 / 112, 2000 293 / 284, 16 x 300 438 / 413,
+      // 4000 854 / 843, 12 documents of 13,060 rows 1610 / 1629, 8192 2765 / 3165; 16 heads x 2000 73 / 68)
+      m.by_tile = m.heads % 8 == 0 && p.src.num_tiles <= 96;
       r = launch_expand(e.p, stream, cu_count());
       if (r == hipSuccess) r = launch_prompt(m, stream);
     }

@@ -289,16 +289,28 @@ struct Item {
   const char *kx, *vx, *rx;
 };
 __device__ inline bool find_item(const PromptProblem& p, Item& it) {
-  // Items in order of head, part and query tile (the last, with the most keys
-  // to see, first), an eighth of them to each XCD: the workgroups that read
-  // one head's keys share an L2.
+  // Long sequences: items in order of head, part and query tile (the last, with
+  // the most keys to see, first), an eighth of them to each XCD, so that the
+  // workgroups that read one head's keys share an L2. Where a head's keys are few
+  // (by_tile), the last tiles of all of an XCD's heads (every eighth) first: a
+  // late long tile is what the call ends with otherwise.
   const int64_t items = (int64_t)p.heads * p.splits * p.q_tiles, per = (items + 7) / 8;
-  const int64_t item = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int64_t)(blockIdx.x >> 3) >= per || item >= items) return false;
-  const uint32_t qts = (uint32_t)p.q_tiles, hs = (uint32_t)item / qts;
-  const int qt = (int)(qts - 1 - ((uint32_t)item - hs * qts));
-  it.part = (int)(hs % (uint32_t)p.splits);
-  it.h = (int)(hs / (uint32_t)p.splits);
+  if ((int64_t)(blockIdx.x >> 3) >= per) return false;
+  int qt;
+  if (p.by_tile) {
+    const uint32_t heads = (uint32_t)p.heads / 8, k = blockIdx.x >> 3, rest = k / heads;
+    it.h = (int)((k - rest * heads) * 8 + (blockIdx.x & 7));
+    const uint32_t r = rest / (uint32_t)p.splits;
+    it.part = (int)(rest - r * (uint32_t)p.splits);
+    qt = (int)((uint32_t)p.q_tiles - 1 - r);
+  } else {
+    const int64_t item = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (item >= items) return false;
+    const uint32_t qts = (uint32_t)p.q_tiles, hs = (uint32_t)item / qts;
+    qt = (int)(qts - 1 - ((uint32_t)item - hs * qts));
+    it.part = (int)(hs % (uint32_t)p.splits);
+    it.h = (int)(hs / (uint32_t)p.splits);
+  }
   if (p.q_info) it.q = p.q_info[qt];
   else it.q = QueryTile{qt * kQBlock, (int)p.q.tokens, p.src.region, p.src.region, 0, 0};
   if (it.q.j0 < 0) return false;
