@@ -621,6 +621,8 @@ torch::Tensor mla_prefill_forward(torch::Tensor kv_cache, torch::Tensor q_nope, 
     TORCH_CHECK(t->stride(2) == 1 && t->stride(0) >= 0 && t->stride(1) >= 0,
                 "queries must be contiguous in their last dimension");
     check_same_device(kv_cache, *t, "queries");
+    // one row broadcast to all tokens and heads: strides of 0, which mean packed below
+    if (t->stride(0) == 0 && t->stride(1) == 0) *t = t->contiguous();
   }
   check_weights(kv_cache, W_UK, W_UV, cfg);
   for (auto* t : {&rope_cos, &rope_sin}) check_same_device(kv_cache, *t, "inputs");

@@ -691,7 +691,7 @@ int prepare_prefill(const la_prefill_args* a, Prefill* out) {
     p.block_size = a->seq_len % 64 == 0 ? 64 : a->seq_len % 32 == 0 ? 32 : a->seq_len;
     p.pool_rows = (int64_t)a->num_seqs * a->seq_len;
   }
-  bool absorbed_ok = p.block_size > 0 && r.region > 0 && p.pool_rows / p.block_size <= INT32_MAX;
+  bool absorbed_ok = p.block_size > 0 && r.region > 0 && p.pool_rows <= (int64_t)UINT32_MAX;  // as la_mla_decode takes
   if (absorbed_ok) {
     p.blocks_per_seq = p.used_blocks = (r.region + p.block_size - 1) / p.block_size;
     absorbed_ok = a->tokens * p.blocks_per_seq <= INT32_MAX &&
@@ -744,7 +744,7 @@ int prepare_prefill(const la_prefill_args* a, Prefill* out) {
   if (p.form == kPrefillExpanded) {
     const size_t head_bytes = (size_t)r.num_tiles * kTileKBytes * 2;
     p.group = (int)std::min<size_t>(c.num_heads, std::max<size_t>(1, head_bytes ? kMaxExpanded / head_bytes : c.num_heads));
-        p.q_tiles = query_tiles(q, prompt_query_rows());
+    p.q_tiles = query_tiles(q, prompt_query_rows());
     const int64_t tiles = a->seq_offsets ? a->total_rows / a->num_seqs / kTileKeys + 1 : r.num_tiles / a->num_seqs;
     p.splits = key_splits(p.q_tiles * p.group, tiles, 1);
     if ((int64_t)p.group * p.splits * p.q_tiles > INT32_MAX - 8) return LA_ERROR_NOT_SUPPORTED;

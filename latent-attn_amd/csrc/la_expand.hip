@@ -78,9 +78,9 @@ __global__ __launch_bounds__(256) void gather_kernel(ExpandProblem p) {
     return;
   }
   const int s = source_find(p.src, tile);
-  const int64_t t = tile - source_tile(p.src, s);
-  const int L = source_rows(p.src, s);
-  const int rows = (int)clamp64(L - t * kTileKeys, 0, kTileKeys);
+  const int64_t t = tile - source_tile(p.src, s);  // < 0: rows before the first sequence
+  const int L = t < 0 ? 0 : source_rows(p.src, s);
+  const int rows = (int)clamp64(L - t * kTileKeys, 0, L > 0 ? kTileKeys : 0);
   const int part = blockIdx.x % kGatherParts * kGatherRows;
   if (threadIdx.x == 0 && part == 0) p.tile_rows[tile] = rows;
   if (rows == 0) return;

@@ -31,11 +31,14 @@ __device__ inline float step_lse(const DecodeProblem& p, int64_t row, int l32) {
   const int64_t cf = lo / len, cl = (hi - 1) / len;
   float m = -INFINITY;
   for (int64_t c = cf + l32; c <= cl; c += 32) m = fmaxf(m, p.part_lse[slot_of(p, c, s) * p.Hq + hq]);
-  m = max32(m);
-  if (m == -INFINITY) return m;
+  m = max32(m);  // (maxima pass over NaN, the sum below does not)
   float l = 0.f;
-  for (int64_t c = cf + l32; c <= cl; c += 32) l += exp2f(p.part_lse[slot_of(p, c, s) * p.Hq + hq] - m);
-  return m + log2f(sum32(l));
+  for (int64_t c = cf + l32; c <= cl; c += 32) {
+    const float e = p.part_lse[slot_of(p, c, s) * p.Hq + hq];
+    l += e == -INFINITY ? 0.f : exp2f(e - m);
+  }
+  l = sum32(l);
+  return l == 0.f ? -INFINITY : m + log2f(l);
 }
 
 // 32 lanes per query row, four values each at a time where rows are whole

@@ -172,6 +172,72 @@ def test_unaligned_cache_and_weights(cuda):
     assert torch.equal(c.run(kernel_variant=EXPANDED), want)
 
 
+@pytest.mark.parametrize("form", [PLAIN, EXPANDED])
+def test_rows_before_the_first_sequence(cuda, form):
+    """Packed sequences that begin past the cache's first rows, which hold NaN."""
+    c = Case(cuda, "packed", [70, 130], [70, 20])
+    lead = torch.full((200, 576), float("nan"), dtype=c.layout.kv.dtype, device=cuda)
+    want = c.run(kernel_variant=form)
+    c.layout.kv = torch.cat([lead, c.layout.kv])
+    c.kw["seq_offsets"] = c.kw["seq_offsets"] + 200
+    got = c.run(kernel_variant=form)
+    c.check(got, form, "rows before the first sequence")
+    # the longer cache may cut its keys into more parts, whose sums are taken in another order
+    assert form == EXPANDED or torch.equal(got, want)
+
+
+@pytest.mark.parametrize("form", [PLAIN, EXPANDED, ABSORBED])
+def test_broadcast_queries(cuda, form):
+    """One query row for all tokens and heads, and one per token or head."""
+    c = Case(cuda, "capacity", [40, 9], [3, 4], heads=16)
+    for shape in ((1, 1), (7, 1), (1, 16)):
+        one = c.q[:shape[0], :shape[1]].clone().expand(7, 16, 192)
+        c.q = one.contiguous()
+        want = c.run(kernel_variant=form)
+        c.check(want, form, f"broadcast {shape}")
+        c.q = one
+        assert torch.equal(c.run(kernel_variant=form), want)
+        c.q = one.contiguous()
+
+
+@pytest.mark.parametrize("kv", [torch.bfloat16, torch.float32])
+def test_no_rows_at_all(cuda, kv):
+    cfg, q = config(4), torch.randn(6, 4, 192, device=cuda)
+    W = torch.zeros(512, 512, device=cuda, dtype=kv)
+    t = torch.zeros(8, 32, device=cuda)
+    got = F.mla_prefill(torch.zeros(2, 0, 576, device=cuda, dtype=kv), q[..., :128], q[..., 128:], W, W, t, t, cfg)
+    assert got.shape == (6, 4, 128) and (got == 0).all()
+    off = torch.zeros(3, dtype=torch.int32, device=cuda)
+    got = F.mla_prefill(torch.zeros(0, 576, device=cuda, dtype=kv), q[..., :128], q[..., 128:], W, W, t, t, cfg,
+                        seq_offsets=off, q_offsets=off)
+    assert (got == 0).all()
+    got = F.mla_prefill(torch.zeros(2, 8, 576, device=cuda, dtype=kv), q[:0, :, :128], q[:0, :, 128:], W, W, t, t, cfg)
+    assert got.shape == (0, 4, 128)
+
+
+@pytest.mark.parametrize("kv", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("L", [50, 96])
+def test_absorbed_over_equal_regions(cuda, L, kv):
+    """Identity block tables: regions that are whole blocks of 32 rows, and one block each where they are not."""
+    c = Case(cuda, "uniform", [L, L, L], [5, 5, 5], heads=16, kv=kv, q=torch.float32)
+    c.check(c.run(kernel_variant=ABSORBED), ABSORBED, f"{kv} {L}")
+
+
+def test_offsets_past_32_bits(cuda):
+    """A cache whose expanded keys pass 2^31 elements and 2^32 bytes, in two groups of heads, against the absorbed form
+    (both within 1e-2 of the exact result normwise, so within 2e-2 of each other)."""
+    heads, L = 128, 140000
+    cfg = config(heads)
+    g = torch.Generator(device=cuda).manual_seed(1)
+    kv = torch.randn(1, L, 576, generator=g, device=cuda).bfloat16()
+    W_UK, W_UV = (w.to(cuda) for w in weights(heads, torch.bfloat16, 2))
+    cos, sin = (t.to(cuda) for t in tables(L))
+    q = torch.randn(3, heads, 192, generator=g, device=cuda)
+    run = lambda form: F.mla_prefill(kv, q[..., :128], q[..., 128:], W_UK, W_UV, cos, sin, cfg, kernel_variant=form).double()
+    a, b = run(ABSORBED), run(EXPANDED)
+    assert (a - b).norm() <= 2e-2 * a.norm()
+
+
 @pytest.mark.parametrize("block", [1, 16, 48, 100])
 def test_page_sizes(cuda, block):
     """Pages that end inside a tile of keys, and single rows."""

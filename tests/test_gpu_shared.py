@@ -133,6 +133,73 @@ def test_equals_decode_over_whole_caches(cuda):
         assert_close(got.double().cpu().numpy(), step.double().cpu().numpy(), "bf16", "decode over whole caches")
 
 
+@pytest.mark.parametrize("form", [LATENT, EXPANDED])
+def test_several_queries_per_sequence(cuda, form):
+    """The C entry's queries_per_seq, on packed own rows and a caller's workspace, an odd address among them."""
+    import ctypes
+
+    from latent_attn import capi
+
+    lib, heads, own, P = capi.load(), 16, [7, 0, 40], 100
+    c = Case(cuda, P, own, heads=heads, layout="packed")
+    g = torch.Generator().manual_seed(9)
+    q_nope, q_rope = (torch.randn(6, heads, d, generator=g).to(cuda) for d in (128, 64))
+    out = torch.empty(6, heads, 128, device=cuda)
+    expanded = c.expand().expanded
+    a = capi.SharedArgs(prefix=c.front.data_ptr(), prefix_len=P, expanded=expanded.data_ptr(), output=out.data_ptr(),
+                        out_dtype=capi.LA_DTYPE_F32, kernel_variant=form)
+    a.own = capi.DecodeArgs(kv_cache=c.layout.kv.data_ptr(), kv_dtype=capi.LA_DTYPE_BF16, total_rows=47, num_seqs=3,
+                            seq_offsets=c.layout.kw["seq_offsets"].data_ptr(), queries_per_seq=2,
+                            q_nope=q_nope.data_ptr(), q_rope=q_rope.data_ptr(), W_UK=c.W_UK.data_ptr(),
+                            w_uk_dtype=capi.LA_DTYPE_BF16, W_UV=c.W_UV.data_ptr(), w_uv_dtype=capi.LA_DTYPE_BF16,
+                            rope_cos=c.cos.data_ptr(), rope_sin=c.sin.data_ptr(), rope_rows=c.cos.shape[0],
+                            cfg=capi.config(c.cfg))
+    stream = torch.cuda.current_stream().cuda_stream
+    need = lib.la_mla_decode_shared_workspace_size(ctypes.byref(a))
+    ws = torch.full((need + 64,), 255, dtype=torch.uint8, device=cuda)
+    ref = reference([r for r in c.rows for _ in range(2)], as_double(q_nope), as_double(q_rope), as_double(c.W_UK),
+                    as_double(c.W_UV), as_double(c.cos), as_double(c.sin), [1] * 6)[0]
+    for at in (0, 16):
+        out.fill_(float("nan"))
+        a.workspace, a.workspace_bytes = ws.data_ptr() + at, need
+        assert lib.la_mla_decode_shared(ctypes.byref(a), stream) == capi.LA_SUCCESS
+        assert_close(out.double().cpu().numpy(), ref.numpy(), "bf16", f"two queries, workspace + {at}")
+    assert (ws[need + 16:] == 255).all()
+    a.workspace, a.workspace_bytes = None, 0  # taken in the order of the stream
+    assert lib.la_mla_decode_shared(ctypes.byref(a), stream) == capi.LA_SUCCESS
+    assert_close(out.double().cpu().numpy(), ref.numpy(), "bf16", "own memory")
+
+
+def test_a_row_that_is_not_finite(cuda):
+    """An infinity or NaN in the prefix reaches every token, in one sequence's own rows that sequence's only."""
+    for bad in (float("nan"), float("inf")):
+        c = Case(cuda, 130, [5, 40, 0], layout="capacity")
+        p = c.expand()
+        want = c.run(p, kernel_variant=EXPANDED)
+        c.layout.kv[1, 3] = bad
+        got = c.run(p, kernel_variant=EXPANDED)
+        assert not torch.isfinite(got[1]).any() and torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+        c = Case(cuda, 130, [5, 40, 0], layout="capacity")
+        c.front[77] = bad
+        assert not torch.isfinite(c.run(c.expand(), kernel_variant=EXPANDED)).any()
+
+
+def test_tables_that_end_early(cuda):
+    """Positions past the tables take their last row, as everywhere."""
+    c = Case(cuda, 100, [30, 64, 7], layout="capacity")
+    full_cos, full_sin = c.cos, c.sin
+    for rows in (110, 60):
+        c.cos, c.sin = full_cos[:rows].contiguous(), full_sin[:rows].contiguous()
+        ends = torch.arange(full_cos.shape[0]).clamp(max=rows - 1)
+        ref = reference(c.rows, as_double(c.q_nope), as_double(c.q_rope), as_double(c.W_UK), as_double(c.W_UV),
+                        as_double(full_cos)[ends], as_double(full_sin)[ends], [1] * 3)[0]
+        if rows == 60:  # the extension asks for a table over the prefix; the C entry clamps
+            with pytest.raises(RuntimeError, match="need at least"):
+                c.run()
+            continue
+        assert_close(c.run().double().cpu().numpy(), ref.numpy(), "bf16", "clamped tables")
+
+
 def test_other_dims(cuda):
     for kv in (torch.bfloat16, torch.float32):
         c = Case(cuda, 70, [5, 0, 30], heads=3, kv=kv, layout="packed", dims=(96, 40, 24, 56))
