@@ -327,19 +327,20 @@ __device__ inline bool find_item(const PromptProblem& p, Item& it) {
 // HBM -> LDS copy of kPieces KB, 1 KB per instruction, as they lie (an
 // instruction's offset moves both addresses). Inline asm without outputs: with
 // the builtin the compiler takes every LDS read behind it to be out of order
-// and waits for all of them where it needs one (5 of 40 products went unhidden).
-// It does not count these copies either: landed() waits for them.
+// and waits for all of them where it needs one (8192 tokens x 128 heads, a call:
+// 3018 us so, 2828 with these). It does not count these copies either: landed()
+// waits for them.
 template <int kPieces>
 __device__ inline void copy_run(lchar* to, const char* from, int lane) {
   const uint32_t dst = (uint32_t)(uintptr_t)to, off = 16 * lane;
   static_assert(kPieces == 2 || kPieces == 4, "");
   if constexpr (kPieces == 4)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024\n\t"
-                 "global_load_lds_dwordx4 %1, %2 offset:2048\n\tglobal_load_lds_dwordx4 %1, %2 offset:3072"
-                 ::"s"(dst), "v"(off), "s"(from) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3\n\t"
+                 "global_load_lds_dwordx4 %1, %2 offset:%4\n\tglobal_load_lds_dwordx4 %1, %2 offset:%5"
+                 ::"s"(dst), "v"(off), "s"(from), "i"(1 << 10), "i"(2 << 10), "i"(3 << 10) : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024"
-                 ::"s"(dst), "v"(off), "s"(from) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3"
+                 ::"s"(dst), "v"(off), "s"(from), "i"(1 << 10) : "memory", "m0");
 }
 // Tile t into a buffer: K, V and the rope keys, a quarter of each per wave.
 __device__ inline void copy_tile(const Item& it, lchar* b, int t, int wave, int lane) {

@@ -238,6 +238,127 @@ def test_offsets_past_32_bits(cuda):
     assert (a - b).norm() <= 2e-2 * a.norm()
 
 
+@pytest.mark.parametrize("form", [PLAIN, EXPANDED, ABSORBED])
+def test_lengths_outside_their_regions(cuda, form):
+    """A length beyond its region counts as the region, a negative one as none; as where they say so themselves."""
+    c = Case(cuda, "capacity", [96, 96, 40], [3, 9, 5], heads=16)
+    cap = c.layout.kv.shape[1]
+    c.layout.kv[0, 96:] = c.layout.kv[0, :cap - 96]
+    for given, meant in (([cap, 96, 40], [cap + 1000, 96, 40]), ([96, 0, 40], [96, -5, 40]), ([96, 96, 0], [96, 96, -2 ** 31])):
+        out = []
+        for lens in (given, meant):
+            c.kw["seq_lens"] = torch.tensor(lens, dtype=torch.int32, device=cuda)
+            out.append(c.run(kernel_variant=form))
+        assert torch.isfinite(out[0]).all() and torch.equal(*out), (given, meant)
+
+
+@pytest.mark.parametrize("form", [PLAIN, EXPANDED, ABSORBED])
+def test_blocks_outside_the_pool(cuda, form):
+    """Block numbers past the pool or below it take its last or first block (a row of which the sequence has)."""
+    c = Case(cuda, "paged", [40, 64], [3, 9], heads=16, block=64)
+    table, blocks = c.kw["block_table"], c.layout.kv.shape[0] // 64
+    c.layout.kv.copy_(torch.randn(c.layout.kv.shape, generator=torch.Generator().manual_seed(4)).to(c.layout.kv.dtype))
+    out = []
+    for ids in ([blocks - 1, 0], [blocks + 5, -7], [2 ** 31 - 1, -2 ** 31]):
+        table[:, 0] = torch.tensor(ids, dtype=torch.int32)
+        out.append(c.run(kernel_variant=form))
+    assert torch.isfinite(out[0]).all() and torch.equal(out[0], out[1]) and torch.equal(out[0], out[2])
+
+
+@pytest.mark.parametrize("form", [PLAIN, EXPANDED, ABSORBED])
+def test_tables_that_end_early(cuda, form):
+    """Positions past the tables take their last row: keys' and queries'."""
+    c = Case(cuda, "capacity", [100, 30], [20, 4], heads=16)
+    cos, sin = c.cos, c.sin
+    ends = torch.arange(cos.shape[0], device=cuda).clamp(max=69)
+    c.cos, c.sin = cos[ends], sin[ends]
+    ref = c.reference()
+    c.cos, c.sin = cos[:70].contiguous(), sin[:70].contiguous()
+    got = c.run(kernel_variant=form)
+    assert_close(got.double().cpu().numpy(), ref[0].numpy(), "bf16", "short tables")
+
+
+@pytest.mark.parametrize("rows,new,prefix", [([2000], [3], [1500]), ([6300], [200], None), ([6300], [200], [6250]),
+                                             ([64 * 97, 5], [130, 5], None)])
+def test_long_caches(cuda, rows, new, prefix):
+    """Parts of the keys under a prefix mask, and both orders of the workgroups. (A term of an output passes at most
+    6300 / 16 additions of an instruction's 16 keys, one of a sum of weights 6300 / 8 of a lane's: the bound's fp32
+    part, for 1000, holds.)"""
+    for heads in (2, 8):
+        c = Case(cuda, "capacity", rows, new, heads=heads, prefix=prefix)
+        c.check(c.run(kernel_variant=EXPANDED), EXPANDED, f"{rows} {heads}")
+
+
+def test_pages_cut_at_max_seq_rows(cuda):
+    """Regions of whole and of cut blocks: rows past max_seq_rows are not seen."""
+    c = Case(cuda, "paged", [130, 70, 200], [5, 3, 8], heads=16, block=48)
+    held = c.rows
+    for cut in (144, 100):
+        c.rows = [r[:cut] for r in held]
+        for form in (PLAIN, EXPANDED, ABSORBED):
+            c.check(c.run(kernel_variant=form, max_seq_rows=cut), form, f"cut at {cut}")
+
+
+def test_two_streams_at_once(cuda):
+    """Two prompts on two streams, several times over: each has its own workspace."""
+    cases = [Case(cuda, "packed", [700, 64], [700, 64], heads=16, seed=s) for s in (1, 2)]
+    want = [c.run(kernel_variant=EXPANDED) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(5):
+        for i, c in enumerate(cases):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(c.run(kernel_variant=EXPANDED))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in (0, 1) for g in got[i])
+
+
+def test_inputs_are_left_as_they_were(cuda):
+    c = Case(cuda, "paged", ODD_ROWS, [1, 5, 8, 3, 1, 7], heads=16)
+    tensors = [c.layout.kv, c.q, c.W_UK, c.W_UV, c.cos, c.sin, *[t for t in c.kw.values() if torch.is_tensor(t)]]
+    before = [t.clone() for t in tensors]
+    for form in (PLAIN, EXPANDED, ABSORBED):
+        c.run(kernel_variant=form)
+    for t, b in zip(tensors, before):
+        assert torch.equal(t.view(torch.uint8) if t.is_floating_point() else t, b.view(torch.uint8) if b.is_floating_point() else b)
+
+
+def test_c_entry_and_its_workspaces(cuda):
+    """The C entry with a workspace of just its size at an odd address, with none, and twice over the same one."""
+    import ctypes
+
+    from latent_attn import capi
+
+    lib = capi.load()
+    c = Case(cuda, "capacity", [70, 9, 130], [20, 9, 1], heads=16, q=torch.float32)
+    for form in (PLAIN, EXPANDED, ABSORBED):
+        want = c.run(kernel_variant=form)
+        out = torch.empty_like(want)
+        q_nope, q_rope = c.q[..., :128].contiguous(), c.q[..., 128:].contiguous()
+        a = capi.PrefillArgs(kv_cache=c.layout.kv.data_ptr(), kv_dtype=capi.LA_DTYPE_BF16, num_seqs=3,
+                             seq_len=c.layout.kv.shape[1], total_rows=3 * c.layout.kv.shape[1],
+                             seq_lens=c.kw["seq_lens"].data_ptr(), q_offsets=c.kw["q_offsets"].data_ptr(), tokens=30,
+                             q_nope=q_nope.data_ptr(), q_rope=q_rope.data_ptr(), q_dtype=capi.LA_DTYPE_F32, rotate_q=1,
+                             W_UK=c.W_UK.data_ptr(), w_uk_dtype=capi.LA_DTYPE_BF16, W_UV=c.W_UV.data_ptr(),
+                             w_uv_dtype=capi.LA_DTYPE_BF16, rope_cos=c.cos.data_ptr(), rope_sin=c.sin.data_ptr(),
+                             rope_rows=c.cos.shape[0], output=out.data_ptr(), out_dtype=capi.LA_DTYPE_F32,
+                             cfg=capi.config(c.cfg), kernel_variant=form)
+        stream = torch.cuda.current_stream().cuda_stream
+        need = lib.la_mla_prefill_workspace_size(ctypes.byref(a))
+        ws = torch.full((need + 64,), 255, dtype=torch.uint8, device=cuda)
+        for at in (0, 16, 16):
+            out.fill_(float("nan"))
+            a.workspace, a.workspace_bytes = ws.data_ptr() + at, need
+            assert lib.la_mla_prefill(ctypes.byref(a), stream) == capi.LA_SUCCESS
+            assert torch.equal(out, want), (form, at)
+        assert (ws[need + 16:] == 255).all()
+        out.fill_(float("nan"))
+        a.workspace, a.workspace_bytes = None, 0
+        assert lib.la_mla_prefill(ctypes.byref(a), stream) == capi.LA_SUCCESS
+        assert torch.equal(out, want), form
+
+
 @pytest.mark.parametrize("block", [1, 16, 48, 100])
 def test_page_sizes(cuda, block):
     """Pages that end inside a tile of keys, and single rows."""

@@ -47,7 +47,8 @@ def test_expand(cuda, rows, heads, kv):
 
 
 class Case:
-    def __init__(self, cuda, prefix, own, heads=16, kv=torch.bfloat16, layout="paged", seed=1, dims=(512, 128, 64, 128)):
+    def __init__(self, cuda, prefix, own, heads=16, kv=torch.bfloat16, layout="paged", seed=1, dims=(512, 128, 64, 128),
+                 model=None):
         dc, dn, d_r, dv = dims
         self.cfg, self.kv_type = config(heads, dc, dn, d_r, dv), kv
         g = torch.Generator().manual_seed(seed)
@@ -56,7 +57,7 @@ class Case:
         self.layout = Layout(layout, data, kv, cuda, seed=seed)
         self.front = front.to(kv).to(cuda)
         self.rows = [torch.cat([front, d]).double() for d in data]
-        model = kv if kv in U else torch.float32 if kv == torch.float32 else torch.bfloat16
+        model = model or (kv if kv in U else torch.float32 if kv == torch.float32 else torch.bfloat16)
         self.W_UK, self.W_UV = (w.to(cuda) for w in weights(heads, model, seed + 1, dc, dn, dv))
         self.cos, self.sin = (t.to(cuda) for t in tables(prefix + max(own), d_r))
         self.q_nope = torch.randn(len(own), heads, dn, generator=g).to(cuda)
@@ -198,6 +199,46 @@ def test_tables_that_end_early(cuda):
                 c.run()
             continue
         assert_close(c.run().double().cpu().numpy(), ref.numpy(), "bf16", "clamped tables")
+
+
+@pytest.mark.parametrize("model", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kv", [torch.float16, torch.bfloat16, torch.float8_e4m3fn])
+def test_weight_types(cuda, kv, model):
+    c = Case(cuda, 150, [5, 0, 40], kv=kv, layout="capacity", model=model)
+    for form in (LATENT, EXPANDED):
+        c.check(c.run(c.expand(), kernel_variant=form), f"{kv} {model} {form}")
+
+
+def test_lengths_outside_their_regions(cuda):
+    c = Case(cuda, 100, [64, 9], layout="capacity")
+    cap = c.layout.kv.shape[1]
+    c.layout.kv[0, 64:] = c.layout.kv[0, :cap - 64]
+    p = c.expand()
+    for form in (LATENT, EXPANDED):
+        for given, meant in (([cap, 9], [cap + 1, 9]), ([64, 0], [64, -3])):
+            out = []
+            for lens in (given, meant):
+                c.layout.kw["seq_lens"] = torch.tensor(lens, dtype=torch.int32, device=cuda)
+                out.append(c.run(p, kernel_variant=form))
+            assert torch.isfinite(out[0]).all() and torch.equal(*out)
+
+
+@pytest.mark.parametrize("form", [LATENT, EXPANDED])
+def test_two_streams_at_once(cuda, form):
+    """Two batches behind one expanded prefix, on two streams."""
+    cases = [Case(cuda, 500, [20, 0, 40], heads=32, layout="capacity", seed=s) for s in (1, 2)]
+    p = cases[0].expand()
+    cases[1].W_UK, cases[1].W_UV = cases[0].W_UK, cases[0].W_UV
+    want = [c.run(p, kernel_variant=form) for c in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cases], [[], []]
+    for _ in range(5):
+        for i, c in enumerate(cases):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(c.run(p, kernel_variant=form))
+    torch.cuda.synchronize()
+    # few query rows: two halves of a row are added into zeros with atomics, in either order the same sum
+    assert all(torch.equal(g, want[i]) for i in (0, 1) for g in got[i])
 
 
 def test_other_dims(cuda):
