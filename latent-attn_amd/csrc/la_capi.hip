@@ -306,10 +306,15 @@ bool merge_halves(const DecodeProblem& p, const Plan& plan) {
 }
 
 // ev_b / ev_e (optional) are recorded around the attention kernel, which runs
-// max(repeat, 1) times between them. used (optional): the problem with its
-// partial slots' addresses, for a kernel that reads them next.
+// max(repeat, 1) times between them. tail (optional): what a kernel that reads
+// the step's partial slots next takes from it and leaves to it.
+struct StepTail {
+  DecodeProblem p;               // out: the problem with its slots' addresses
+  bool merge = true;             // false: the slots stay as they are, nothing is written to the output
+  const void* q_prep = nullptr;  // the same queries' 16-bit rows in a layout that is this step's too
+};
 int run(const la_decode_args* a, hipStream_t stream, hipEvent_t ev_b = nullptr, hipEvent_t ev_e = nullptr,
-        int repeat = 1, bool coarse = false, DecodeProblem* used = nullptr) {
+        int repeat = 1, bool coarse = false, StepTail* tail = nullptr) {
   if (repeat < 0) return LA_ERROR_INVALID_VALUE;
   DecodeProblem p;
   Plan plan;
@@ -345,10 +350,12 @@ int run(const la_decode_args* a, hipStream_t stream, hipEvent_t ev_b = nullptr, 
   // the two latent halves, which add into the output. The kernel that writes
   // the attention kernel's 16-bit queries (the absorb kernel, or prep_q when
   // the queries come absorbed) runs first and zeroes the output.
-  const bool merge_halves = la::merge_halves(p, plan);
+  const bool merge_halves = (!tail || tail->merge) && la::merge_halves(p, plan);
   float* const zero_out = merge_halves ? a->output : nullptr;
   const int64_t zero_n = merge_halves ? tokens * c.num_heads * c.v_head_dim : 0;
-  if (a->q_nope) {
+  if (tail && tail->q_prep && plan.absorb_prep) {
+    p.q_prep = const_cast<void*>(tail->q_prep);
+  } else if (a->q_nope) {
     hipError_t e = hipSuccess;
     if (plan.absorb_prep) {
       // absorbed, scaled 16-bit Q rows for the attention kernel in one pass
@@ -400,7 +407,8 @@ int run(const la_decode_args* a, hipStream_t stream, hipEvent_t ev_b = nullptr, 
     }
     if (e != hipSuccess) return finish(e);
   }
-  if (used) *used = p;
+  if (tail) tail->p = p;
+  if (tail && !tail->merge) return finish(hipSuccess);
   if (plan.proj_f32) return finish(launch_combine_project_f32(p, stream, merge_halves));
   if (plan.proj_mfma) return finish(launch_combine_project_mfma(p, stream, merge_halves, cu_count()));
   return finish(launch_combine_project(p, stream));
@@ -774,6 +782,7 @@ int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need)
   int32_t *lens = nullptr, *table = nullptr;
   void* step_ws = nullptr;
   size_t step_bytes = 0;
+  bool cast_merge = false;
   const bool q32 = a->q_dtype == LA_DTYPE_F32;
   const bool nope_as_is = q32 && p.q.nope_head == c.qk_nope_head_dim && p.q.nope_stride == (int64_t)nh * p.q.nope_head;
   const bool rope_as_is = q32 && !a->rotate_q && p.q.rope_head == c.qk_rope_head_dim &&
@@ -799,7 +808,6 @@ int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need)
         if (!rope_as_is) q_rope = static_cast<float*>(v.take((size_t)rows * c.qk_rope_head_dim * sizeof(float)));
         lens = static_cast<int32_t*>(v.take((size_t)a->tokens * sizeof(int32_t)));
         table = static_cast<int32_t*>(v.take((size_t)a->tokens * p.blocks_per_seq * sizeof(int32_t)));
-        if (a->out_dtype != LA_DTYPE_F32) out32 = static_cast<float*>(v.take((size_t)rows * c.v_head_dim * sizeof(float)));
         // (the addresses are those of a workspace of any base: only their alignment matters to the plan)
         alignas(256) static const char any[256] = {0};
         const float* f = reinterpret_cast<const float*>(any);
@@ -809,6 +817,14 @@ int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need)
                        reinterpret_cast<const int32_t*>(any), const_cast<float*>(f), nullptr, 0);
         step_bytes = la_mla_decode_workspace_size(&d);
         step_ws = v.take(step_bytes);
+        DecodeProblem step;
+        Plan plan;
+        // The merge that ends the step writes 16-bit rows itself, but not the half-row one (16 x 4 tokens x 128 heads
+        // with a cast / so 118.7 / 116.7 us, 16 x 8 112.2 / 109.5; 2 x 2, half rows, 32.3 / 32.7 as full rows)
+        cast_merge = a->out_dtype != LA_DTYPE_F32 && prepare(&d, &step, &plan) == LA_SUCCESS &&
+                     merge_join_supported(step) && !merge_halves(step, plan);
+        if (a->out_dtype != LA_DTYPE_F32 && !cast_merge)
+          out32 = static_cast<float*>(v.take((size_t)rows * c.v_head_dim * sizeof(float)));
       }
     }
     return v.total();
@@ -907,10 +923,22 @@ int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need)
   }
   hipError_t r = launch_tokens(t, stream);
   if (r != hipSuccess) return scratch.finish(record_hip(r));
-  float* const out = out32 ? out32 : static_cast<float*>(a->output);
+  float* const out = out32 ? out32 : static_cast<float*>(a->output);  // (cast_merge: the step leaves it alone)
   const la_decode_args d = token_step(a, p, qn, rope_as_is ? static_cast<const float*>(a->q_rope) : q_rope, lens, table,
                                       out, step_ws, step_bytes);
-  int s3 = run(&d, stream);
+  StepTail tail;
+  tail.merge = !cast_merge;
+  int s3 = run(&d, stream, nullptr, nullptr, 1, false, &tail);
+  if (s3 == LA_SUCCESS && cast_merge) {
+    JoinProblem j{};
+    j.rows = rows;
+    j.nh = nh;
+    j.dv = c.v_head_dim;
+    j.step[0] = tail.p;
+    j.out = a->output;
+    j.out_dtype = a->out_dtype;
+    s3 = status_of(launch_merge_join(j, stream, cu_count()));
+  }
   if (s3 == LA_SUCCESS && out32) s3 = status_of(launch_cast(out32, a->output, a->out_dtype, rows * c.v_head_dim, stream));
   return scratch.finish(s3);
 }
@@ -1005,14 +1033,19 @@ int decode_shared(const la_shared_args* a, hipStream_t stream, bool run_it, size
   const bool expanded_ok = a->expanded && (reinterpret_cast<uintptr_t>(a->expanded) & (kAlign - 1)) == 0 &&
                            expanded_dims(c) && own.kv_dtype != LA_DTYPE_F32 && device_is_gfx950();
   if (a->kernel_variant == 2 && !expanded_ok) return LA_ERROR_NOT_SUPPORTED;
-  // Microseconds beside the own rows': over latent rows 25 of launches (queries
-  // absorbed, a merge) and 2.3e-6 per (token, head, row); over the expanded form
-  // its bytes at 5 TB/s (128 heads x 8192 rows, a step with 16 / 32 / 48 / 64
-  // tokens: 97 / 131 / 189 / 218 over latent rows, 131 / 140 / 157 / 163 expanded;
-  // 2000 rows, 16 tokens 74 / 58; 16 heads x 8192 rows, 32 tokens 66 / 50).
-  const double pairs = (double)nh * P;
-  const bool expanded = P > 0 && expanded_ok &&
-                        (a->kernel_variant == 2 || (a->kernel_variant == 0 && pairs * 512. / 5e6 < 25. + 2.3e-6 * pairs * tokens));
+  // Microseconds beside the own rows': over latent rows 1.75e-6 per (token, head,
+  // row) and 5 to 27 of launches (a second attention and its slots); over the
+  // expanded form its bytes at 5 TB/s. A step over latent rows / expanded: 128
+  // heads, 8192 rows with 16, 32, 48, 64 tokens 75 / 126, 112 / 134, 162 / 154,
+  // 196 / 159; 2000 rows with 8, 16, 32 51 / 59, 53 / 54, 68 / 58; 500 rows with 1,
+  // 4, 16 33 / 36, 41 / 44, 41 / 39; 16 heads, 512 rows with 2 32 / 28; 8192 with
+  // 1, 8, 32 36 / 39, 41 / 38, 56 / 42; 32768 with 8, 32, 100 61 / 73, 76 / 78,
+  // 157 / 110.
+  const double pairs = (double)nh * P, all = pairs * tokens;
+  const bool expanded =
+      P > 0 && expanded_ok &&
+      (a->kernel_variant == 2 ||
+       (a->kernel_variant == 0 && pairs * 512. / 5e6 < std::min(27., 5. + 4e-6 * all) + 1.75e-6 * all));
 
   PromptProblem m{};
   la_decode_args pre{};
@@ -1052,12 +1085,25 @@ int decode_shared(const la_shared_args* a, hipStream_t stream, bool run_it, size
     pre.workspace_bytes = 0;
     pre.output = own.output;
   }
-  // validates both steps
+  // Validates both steps. One kernel merges their slots, projects and joins
+  // where the slots are the MFMA kernels', unless many rows of many parts wait
+  // for its one workgroup per CU (a step, us, with launches of their own / with
+  // the one: 16 heads, 200 sequences and 16 parts 69.9 / 73.6, 130 and 8 parts
+  // 52.0 / 55.2; 4 and 15 parts 34.7 / 29.8; 128 heads, 200 and 2 parts 181 / 177).
+  // Heads in whole blocks of 32 query rows lie alike in both steps, which then
+  // share the absorbed queries.
   la::DecodeProblem probe;
   Plan plan;
   int st = prepare(&own, &probe, &plan);
-  if (st == LA_SUCCESS && pre.num_seqs > 0) st = prepare(&pre, &probe, &plan);
   if (st != LA_SUCCESS) return st;
+  const bool few = !expanded || m.splits <= 4 || (int64_t)((nh + 7) / 8 * 8) * ((tokens + 7) / 8) <= cu_count();
+  bool one = P > 0 && few && merge_join_supported(probe), share = nh % 32 == 0 && plan.absorb_prep;
+  if (pre.num_seqs > 0) {
+    st = prepare(&pre, &probe, &plan);
+    if (st != LA_SUCCESS) return st;
+    one = one && merge_join_supported(probe);
+    share = share && plan.absorb_prep;
+  }
   const size_t own_bytes = la_mla_decode_workspace_size(&own);
   if (pre.num_seqs > 0) pre_bytes = la_mla_decode_workspace_size(&pre);
 
@@ -1067,13 +1113,13 @@ int decode_shared(const la_shared_args* a, hipStream_t stream, bool run_it, size
   auto carve = [&](void* ws) {
     Carve v(ws);
     own_ws = v.take(own_bytes);
-    own_out = static_cast<float*>(v.take((size_t)rows * c.v_head_dim * sizeof(float)));
+    if (!one) own_out = static_cast<float*>(v.take((size_t)rows * c.v_head_dim * sizeof(float)));
     if (expanded) {
       m.part_o = static_cast<float*>(v.take((size_t)m.splits * rows * 128 * sizeof(float)));
       m.part_lse = static_cast<float*>(v.take((size_t)m.splits * rows * sizeof(float)));
     } else if (P > 0) {
       pre_ws = v.take(pre_bytes);
-      pre_out = static_cast<float*>(v.take((size_t)rows * c.v_head_dim * sizeof(float)));
+      if (!one) pre_out = static_cast<float*>(v.take((size_t)rows * c.v_head_dim * sizeof(float)));
     }
     return v.total();
   };
@@ -1099,20 +1145,27 @@ int decode_shared(const la_shared_args* a, hipStream_t stream, bool run_it, size
     j.part_o = m.part_o;
     j.part_lse = m.part_lse;
   } else if (P > 0) {
-    pre.output = pre_out;
+    if (!one) pre.output = pre_out;
     pre.workspace = pre_ws;
     pre.workspace_bytes = pre_bytes;
-    st = run(&pre, stream, nullptr, nullptr, 1, false, &j.step[1]);
+    StepTail tail;
+    tail.merge = !one;
+    st = run(&pre, stream, nullptr, nullptr, 1, false, &tail);
+    j.step[1] = tail.p;
     j.step_out[1] = pre_out;
   }
   if (st == LA_SUCCESS) {
-    own.output = own_out;
+    if (!one) own.output = own_out;
     own.workspace = own_ws;
     own.workspace_bytes = own_bytes;
-    st = run(&own, stream, nullptr, nullptr, 1, false, &j.step[0]);
+    StepTail tail;
+    tail.merge = !one;
+    if (share && !expanded && P > 0) tail.q_prep = j.step[1].q_prep;
+    st = run(&own, stream, nullptr, nullptr, 1, false, &tail);
+    j.step[0] = tail.p;
     j.step_out[0] = own_out;
   }
-  if (st == LA_SUCCESS) st = status_of(launch_join(j, stream));
+  if (st == LA_SUCCESS) st = status_of(one ? launch_merge_join(j, stream, cu_count()) : launch_join(j, stream));
   return scratch.finish(st);
 }
 

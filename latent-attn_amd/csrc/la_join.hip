@@ -9,8 +9,6 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kMaxSplits = 32;
-
 __device__ inline float max32(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
@@ -104,7 +102,7 @@ __global__ __launch_bounds__(256) void join_kernel(JoinProblem p) {
 hipError_t launch_join(const JoinProblem& p, hipStream_t stream) {
   if (p.rows == 0) return hipSuccess;
   const int64_t blocks = (p.rows + 7) / 8;
-  if (blocks > INT32_MAX || p.splits > kMaxSplits) return hipErrorInvalidValue;
+  if (blocks > INT32_MAX || p.splits > kJoinSplits) return hipErrorInvalidValue;
   if (p.dv % 4 == 0) hipLaunchKernelGGL(join_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
   else hipLaunchKernelGGL(join_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
   return hipGetLastError();

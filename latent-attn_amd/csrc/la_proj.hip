@@ -27,7 +27,7 @@
 //          splits each over the two latent halves, which add into the output
 //          (zeroed earlier in the same call by the kernel that writes the
 //          attention kernel's 16-bit queries).
-#include "la_internal.hpp"
+#include "la_prompt.hpp"
 
 #include <type_traits>
 
@@ -417,10 +417,11 @@ __device__ inline MergeTask merge_task(const DecodeProblem& p, int t, int h, int
 // most 64 takes one memory round trip. Longer merges loop over further
 // groups of NB rows (and of 64 slots). Lane i's weights are broadcast with
 // v_readlane.
-// kHalf: half-row merge of latent half c (o[k][1] stays 0).
+// kHalf: half-row merge of latent half c (o[k][1] stays 0). row_lse (optional):
+// each row's base-2 log-sum-exp over all of its slots, -infinity without any.
 template <bool F16, bool kHalf, int NB, int kTasks>
 __device__ inline void merge_tasks(const DecodeProblem& p, const int (&t)[kTasks], int h, int g, int G, int lane,
-                                   f32x4 (&o)[kTasks][2], int c = 0) {
+                                   f32x4 (&o)[kTasks][2], int c = 0, float* row_lse = nullptr) {
   typedef typename std::conditional<F16, _Float16, float>::type PT;
   typedef typename std::conditional<kHalf, SlotRowHalf<F16>, SlotRow<F16>>::type SR;
   const int64_t sstride = (int64_t)p.Hq * kDcP;
@@ -455,6 +456,7 @@ __device__ inline void merge_tasks(const DecodeProblem& p, const int (&t)[kTasks
     o[k][0] = f32x4{0.f, 0.f, 0.f, 0.f};
     o[k][1] = o[k][0];
     const int n = mt[k].n, ns = mt[k].ns;
+    if (row_lse) row_lse[k] = -INFINITY;
     if (n == 0) continue;  // wave-uniform
     const float* lse = p.part_lse + mt[k].row0;
     // M and the denominator over every slot of the row
@@ -463,7 +465,9 @@ __device__ inline void merge_tasks(const DecodeProblem& p, const int (&t)[kTasks
     mx = wave_max(mx);
     float den = lane < n ? exp2f(ls_all[k] - mx) : 0.f;
     for (int i = lane + 64; i < n; i += 64) den += exp2f(lse[(int64_t)i * p.Hq] - mx);
-    const float inv = 1.f / wave_sum(den);
+    den = wave_sum(den);
+    if (row_lse) row_lse[k] = mx + log2f(den);
+    const float inv = 1.f / den;
     for (int i0 = 0; i0 < ns; i0 += 64) {
       const int nb = min(64, ns - i0);
       // this lane's slot: g + G (i0 + lane)
@@ -758,6 +762,163 @@ __global__ __launch_bounds__(kMPWaves * 64) void merge_project_half_kernel(Decod
   LA_RSTAMP_WRITE(1);
 }
 
+// Merge + W_UV projection + join (JoinProblem): a row's latent part is the sum
+// of up to two decode steps' slots (both before W_UV, so one projection serves
+// both), each step's merge weighted by its share of the whole softmax; parts
+// that are projected already (prompt_kernel's) are added to the product with
+// their own shares, and the row goes out in its type. One launch for two
+// merges, a join and a cast, and neither step's rows in between.
+// A workgroup of 8 waves per (head, 16 query rows, or fewer while the launch
+// leaves CUs idle; a CU holds one): up to 8 rows share the waves, more are two
+// per wave. A step, us, with the merges and the join as launches of their own /
+// with this: 12 sequences behind 32768 rows, 128 heads 153 / 132; 8 behind 4000
+// 75 / 57; 4 behind 2000, 16 heads 34.7 / 29.8; 64 behind 8192 expanded, 128
+// heads 178 / 173. Two workgroups of half the rows per CU: 149, 65, 29.3, 175.
+template <typename WT>
+__global__ __launch_bounds__(kMPWaves * 64) void merge_join_kernel(JoinProblem j, int rpb_log2) {
+  const DecodeProblem& p = j.step[0];
+  typedef Mma16<WT> M;
+  typedef typename M::vec vec;
+  constexpr float kLoScale = Mma<WT>::kLoScale;
+  __shared__ __attribute__((aligned(16))) short oh[kMPRows * kMPOPitch];  // joined O rows, high parts
+  __shared__ __attribute__((aligned(16))) short ol[kMPRows * kMPOPitch];  // and residuals
+  __shared__ __attribute__((aligned(16))) float gp[kMPWaves * kMPPitch];  // slot-group sums
+  __shared__ __attribute__((aligned(8))) float gq[kMPRows][128];          // the projected parts' weighted sums
+  const int R = p.num_seqs * p.qps, rpb = 1 << rpb_log2;
+  const int nrb = (R + rpb - 1) >> rpb_log2;
+  const int x = blockIdx.x & 7, k = blockIdx.x >> 3;
+  const int h = (k / nrb) * 8 + x, rb = k % nrb;
+  if (h >= p.nh) return;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int rows = min(rpb, R - rb * rpb);
+
+  // W_UV operands: B[k = 32 ks + 8 (lane / 16) + j][n = lane % 16]
+  const WT* wrow = reinterpret_cast<const WT*>(p.W_UV) + ((int64_t)h * p.dv + 16 * wave + (lane & 15)) * kDcP +
+                   8 * (lane >> 4);
+  vec bw[16];
+#pragma unroll
+  for (int ks = 0; ks < 16; ++ks) bw[ks] = __builtin_bit_cast(vec, *reinterpret_cast<const i16x8*>(wrow + 32 * ks));
+
+  // This wave's rows t[k] (< 0: none): o[k] <- the latent row, gq[row[k]] <- the
+  // projected parts, each the share of group g of G (slots and parts g, g + G, ...).
+  // The first parts' loads go out with the slots'.
+  f32x4 o[2][2];
+  auto merge = [&](const auto& t, const int* row, int g, int G) {
+    constexpr int kTasks = sizeof(t) / sizeof(int);
+    constexpr int kAhead = 8;
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    float part[kTasks], own[kTasks], front[kTasks];
+    f32x4 a[kTasks][2], b[kTasks][2];
+    f32x2 q[kTasks][kAhead];
+    auto load = [&](int i, int s) {
+      return *reinterpret_cast<const f32x2*>(j.part_o + ((int64_t)s * j.rows + (int64_t)t[i] * p.nh + h) * 128 + 2 * lane);
+    };
+#pragma unroll
+    for (int i = 0; i < kTasks; ++i) {
+      part[i] = t[i] >= 0 && lane < j.splits ? j.part_lse[(int64_t)lane * j.rows + (int64_t)t[i] * p.nh + h] : -INFINITY;
+      front[i] = -INFINITY;
+      b[i][0] = b[i][1] = f32x4{};
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (t[i] >= 0 && g + G * u < j.splits) q[i][u] = load(i, g + G * u);
+    }
+    merge_tasks<true, false, kMPSlots, kTasks>(p, t, h, g, G, lane, a, 0, own);
+    if (j.step[1].num_seqs > 0) merge_tasks<true, false, kMPSlots, kTasks>(j.step[1], t, h, g, G, lane, b, 0, front);
+#pragma unroll
+    for (int i = 0; i < kTasks; ++i) {
+      const float m = fmaxf(wave_max(part[i]), fmaxf(own[i], front[i]));
+      // rows that see nothing have no part with a weight; a NaN stays one
+      const auto weight = [&](float e) { return e == -INFINITY ? 0.f : exp2f(e - m); };
+      const float w = weight(part[i]), wa = weight(own[i]), wb = weight(front[i]);
+      const float total = wave_sum(w) + wa + wb, inv = total == 0.f ? 0.f : 1.f / total;
+      o[i][0] = wa * inv * a[i][0] + wb * inv * b[i][0];
+      o[i][1] = wa * inv * a[i][1] + wb * inv * b[i][1];
+      const float wi = w * inv;
+      f32x2 sum = {};
+      for (int s0 = g; s0 < j.splits; s0 += kAhead * G) {
+        if (s0 > g) {
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u)
+            if (t[i] >= 0 && s0 + G * u < j.splits) q[i][u] = load(i, s0 + G * u);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (s0 + G * u < j.splits) {
+            const float ws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wi), s0 + G * u));
+            if (ws != 0.f) sum += ws * q[i][u];  // (a part without weight may hold anything)
+          }
+      }
+      *reinterpret_cast<f32x2*>(&gq[row[i]][2 * lane]) = sum;
+    }
+  };
+  // row r, columns c0 .. c0 + 7 of O -> high and low operand rows
+  auto put8 = [&](int r, int c0, const f32x4& v0, const f32x4& v1) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = v0[e], v[4 + e] = v1[e];
+    vec hi, lo;
+    split8<WT>(v, hi, lo);
+    *reinterpret_cast<vec*>(&oh[r * kMPOPitch + c0]) = hi;
+    *reinterpret_cast<vec*>(&ol[r * kMPOPitch + c0]) = lo;
+  };
+  if (rows > kMPWaves) {
+    const int row[2] = {wave, wave + kMPWaves};
+    const int t[2] = {rb * rpb + wave, wave + kMPWaves < rows ? rb * rpb + wave + kMPWaves : -1};
+    merge(t, row, 0, 1);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) put8(row[q], 8 * lane, o[q][0], o[q][1]);  // 0 without a second row
+  } else {
+    const int G = kMPWaves / rows;
+    const int row[1] = {wave}, t[1] = {wave / G < rows ? rb * rpb + wave / G : -1};
+    merge(t, row, wave % G, G);
+    *reinterpret_cast<f32x4*>(&gp[wave * kMPPitch + 8 * lane]) = o[0][0];
+    *reinterpret_cast<f32x4*>(&gp[wave * kMPPitch + 8 * lane + 4]) = o[0][1];
+    __syncthreads();
+    for (int i = tid; i < kMPRows * (kDcP / 8); i += kMPWaves * 64) {
+      const int rr = i / (kDcP / 8), c8 = i % (kDcP / 8);
+      f32x4 v0 = {}, v1 = {};
+      if (rr < rows)
+        for (int q = 0; q < G; ++q) {
+          v0 += *reinterpret_cast<const f32x4*>(&gp[(rr * G + q) * kMPPitch + 8 * c8]);
+          v1 += *reinterpret_cast<const f32x4*>(&gp[(rr * G + q) * kMPPitch + 8 * c8 + 4]);
+        }
+      put8(rr, 8 * c8, v0, v1);
+    }
+  }
+  __syncthreads();
+
+  // A[m = lane % 16][k = 32 ks + 8 (lane / 16) + j] = O[m][k] (high, low)
+  f32x4 acc_hi = {}, acc_lo = {};
+  const int a0 = (lane & 15) * kMPOPitch + 8 * (lane >> 4);
+#pragma unroll
+  for (int ks = 0; ks < 16; ++ks) {
+    const vec hi = *reinterpret_cast<const vec*>(&oh[a0 + 32 * ks]);
+    const vec lo = *reinterpret_cast<const vec*>(&ol[a0 + 32 * ks]);
+    acc_hi = M::mma(hi, bw[ks], acc_hi);
+    acc_lo = M::mma(lo, bw[ks], acc_lo);
+  }
+  // D[m = 4 (lane / 16) + i][n = lane % 16]
+  const int r0 = 4 * (lane >> 4);
+  if (r0 >= rows) return;
+  const int64_t at = ((int64_t)(rb * rpb + r0) * p.nh + h) * p.dv + 16 * wave + (lane & 15);
+  const int64_t step = (int64_t)p.nh * p.dv;  // from one query row's output of head h to the next's
+  f32x4 v = acc_hi + acc_lo * (1.f / kLoScale);
+  if (j.splits > 0) {
+    const int G = rows > kMPWaves ? 1 : kMPWaves / rows;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (r0 + i < rows)
+        for (int q = 0; q < G; ++q) v[i] += gq[(r0 + i) * G + q][16 * wave + (lane & 15)];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (r0 + i < rows) {
+      if (j.out_dtype == LA_DTYPE_F32) static_cast<float*>(j.out)[at + i * step] = v[i];
+      else if (j.out_dtype == LA_DTYPE_BF16) static_cast<__bf16*>(j.out)[at + i * step] = (__bf16)v[i];
+      else static_cast<_Float16*>(j.out)[at + i * step] = (_Float16)v[i];
+    }
+}
+
 // The same for float32 weights, all in fp32 (v_mfma_f32_16x16x4_f32): one
 // workgroup of 8 waves per (head h, 16 query rows), or, with kHalf and an
 // output zeroed earlier in the call, per latent half of it, the halves added
@@ -977,6 +1138,27 @@ hipError_t launch_combine_project_mfma(const DecodeProblem& p, hipStream_t strea
     else
       hipLaunchKernelGGL((merge_project_kernel<__half, false>), grid, dim3(kMPWaves * 64), 0, stream, p);
   }
+  return hipGetLastError();
+}
+
+bool merge_join_supported(const DecodeProblem& p) { return p.part_f16 && project_mfma_supported(p); }
+
+hipError_t launch_merge_join(const JoinProblem& j, hipStream_t stream, int ncu) {
+  const DecodeProblem& p = j.step[0];
+  const int R = p.num_seqs * p.qps, hb = 8 * ((p.nh + 7) / 8);
+  if (R == 0) return hipSuccess;
+  if (j.rows != (int64_t)R * p.nh || j.splits > kJoinSplits || !merge_join_supported(p) ||
+      (j.step[1].num_seqs > 0 && (!merge_join_supported(j.step[1]) || j.step[1].num_seqs * j.step[1].qps != R ||
+                                  j.step[1].nh != p.nh)))
+    return hipErrorInvalidValue;
+  int rpb_log2 = 4;
+  while (rpb_log2 > 0 && (int64_t)hb * ((R + (1 << rpb_log2) - 1) >> rpb_log2) < ncu) --rpb_log2;
+  const int64_t blocks = (int64_t)hb * ((R + (1 << rpb_log2) - 1) >> rpb_log2);
+  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  if (p.wuv_dtype == LA_DTYPE_BF16)
+    hipLaunchKernelGGL(merge_join_kernel<__hip_bfloat16>, dim3((unsigned)blocks), dim3(kMPWaves * 64), 0, stream, j, rpb_log2);
+  else
+    hipLaunchKernelGGL(merge_join_kernel<__half>, dim3((unsigned)blocks), dim3(kMPWaves * 64), 0, stream, j, rpb_log2);
   return hipGetLastError();
 }
 

@@ -258,6 +258,7 @@ int prompt_query_rows();  // query tokens per workgroup
 hipError_t launch_prompt(const PromptProblem& p, hipStream_t stream);
 
 // Joins partial results of the same (token, head) rows by their log-sum-exps.
+constexpr int kJoinSplits = 32;  // at most
 struct JoinProblem {
   int64_t rows;  // tokens * nh
   int nh, dv;
@@ -272,6 +273,11 @@ struct JoinProblem {
   int out_dtype;
 };
 hipError_t launch_join(const JoinProblem& p, hipStream_t stream);
+// The same from the steps' partial slots (step[0] is there; step_out unused):
+// merge, W_UV and join in one (la_proj.hip). Both steps hold fp16 slots and
+// have 16-bit W_UV.
+bool merge_join_supported(const DecodeProblem& p);
+hipError_t launch_merge_join(const JoinProblem& j, hipStream_t stream, int ncu);
 
 // Any type and head shape: absorbed queries (fp32), one workgroup per (token, head).
 struct GenericPrompt {
