@@ -819,10 +819,9 @@ int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need)
         step_ws = v.take(step_bytes);
         DecodeProblem step;
         Plan plan;
-        // The merge that ends the step writes 16-bit rows itself, but not the half-row one (16 x 4 tokens x 128 heads
-        // with a cast / so 118.7 / 116.7 us, 16 x 8 112.2 / 109.5; 2 x 2, half rows, 32.3 / 32.7 as full rows)
-        cast_merge = a->out_dtype != LA_DTYPE_F32 && prepare(&d, &step, &plan) == LA_SUCCESS &&
-                     merge_join_supported(step) && !merge_halves(step, plan);
+        // The merge that ends the step writes 16-bit rows itself (the step's own merge and a cast / so: 16 x 4 tokens x
+        // 128 heads 119 / 109 us a call, 16 x 8 112 / 94, 2 x 2 33.0 / 30.9, 1 token 33.2 / 31.3)
+        cast_merge = a->out_dtype != LA_DTYPE_F32 && prepare(&d, &step, &plan) == LA_SUCCESS && merge_join_supported(step);
         if (a->out_dtype != LA_DTYPE_F32 && !cast_merge)
           out32 = static_cast<float*>(v.take((size_t)rows * c.v_head_dim * sizeof(float)));
       }
@@ -1086,18 +1085,13 @@ int decode_shared(const la_shared_args* a, hipStream_t stream, bool run_it, size
     pre.output = own.output;
   }
   // Validates both steps. One kernel merges their slots, projects and joins
-  // where the slots are the MFMA kernels', unless many rows of many parts wait
-  // for its one workgroup per CU (a step, us, with launches of their own / with
-  // the one: 16 heads, 200 sequences and 16 parts 69.9 / 73.6, 130 and 8 parts
-  // 52.0 / 55.2; 4 and 15 parts 34.7 / 29.8; 128 heads, 200 and 2 parts 181 / 177).
-  // Heads in whole blocks of 32 query rows lie alike in both steps, which then
-  // share the absorbed queries.
+  // where the slots are the MFMA kernels'. Heads in whole blocks of 32 query rows
+  // lie alike in both steps, which then share the absorbed queries.
   la::DecodeProblem probe;
   Plan plan;
   int st = prepare(&own, &probe, &plan);
   if (st != LA_SUCCESS) return st;
-  const bool few = !expanded || m.splits <= 4 || (int64_t)((nh + 7) / 8 * 8) * ((tokens + 7) / 8) <= cu_count();
-  bool one = P > 0 && few && merge_join_supported(probe), share = nh % 32 == 0 && plan.absorb_prep;
+  bool one = P > 0 && merge_join_supported(probe), share = nh % 32 == 0 && plan.absorb_prep;
   if (pre.num_seqs > 0) {
     st = prepare(&pre, &probe, &plan);
     if (st != LA_SUCCESS) return st;

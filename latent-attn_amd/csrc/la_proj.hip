@@ -769,13 +769,18 @@ __global__ __launch_bounds__(kMPWaves * 64) void merge_project_half_kernel(Decod
 // their own shares, and the row goes out in its type. One launch for two
 // merges, a join and a cast, and neither step's rows in between.
 // A workgroup of 8 waves per (head, 16 query rows, or fewer while the launch
-// leaves CUs idle; a CU holds one): up to 8 rows share the waves, more are two
-// per wave. A step, us, with the merges and the join as launches of their own /
-// with this: 12 sequences behind 32768 rows, 128 heads 153 / 132; 8 behind 4000
-// 75 / 57; 4 behind 2000, 16 heads 34.7 / 29.8; 64 behind 8192 expanded, 128
-// heads 178 / 173. Two workgroups of half the rows per CU: 149, 65, 29.3, 175.
+// leaves CUs idle): up to 8 rows share the waves, more are two per wave. It
+// waits on one chain of loads (sequence, slots, weights), so two per CU count
+// for more than loads ahead: 5 slots at once and the weights behind the merge
+// (121 VGPRs) against 8 and the weights before it (229): 200 sequences behind
+// 2000 rows, 128 heads, a step 147 us for 176; 64 behind 8192 166 for 173; 16 x
+// 4 drafted tokens a call 109 for 119. A step with the merges and the join as
+// launches of their own / with this: 12 sequences behind 32768 rows, 128 heads
+// 153 / 134; 8 behind 4000 75 / 57; 4 behind 2000, 16 heads 34.7 / 29.8; 200
+// behind 4001 70 / 65.5.
+constexpr int kMJSlots = 5;
 template <typename WT>
-__global__ __launch_bounds__(kMPWaves * 64) void merge_join_kernel(JoinProblem j, int rpb_log2) {
+__global__ __launch_bounds__(kMPWaves * 64, 4) void merge_join_kernel(JoinProblem j, int rpb_log2) {
   const DecodeProblem& p = j.step[0];
   typedef Mma16<WT> M;
   typedef typename M::vec vec;
@@ -795,9 +800,6 @@ __global__ __launch_bounds__(kMPWaves * 64) void merge_join_kernel(JoinProblem j
   // W_UV operands: B[k = 32 ks + 8 (lane / 16) + j][n = lane % 16]
   const WT* wrow = reinterpret_cast<const WT*>(p.W_UV) + ((int64_t)h * p.dv + 16 * wave + (lane & 15)) * kDcP +
                    8 * (lane >> 4);
-  vec bw[16];
-#pragma unroll
-  for (int ks = 0; ks < 16; ++ks) bw[ks] = __builtin_bit_cast(vec, *reinterpret_cast<const i16x8*>(wrow + 32 * ks));
 
   // This wave's rows t[k] (< 0: none): o[k] <- the latent row, gq[row[k]] <- the
   // projected parts, each the share of group g of G (slots and parts g, g + G, ...).
@@ -805,7 +807,7 @@ __global__ __launch_bounds__(kMPWaves * 64) void merge_join_kernel(JoinProblem j
   f32x4 o[2][2];
   auto merge = [&](const auto& t, const int* row, int g, int G) {
     constexpr int kTasks = sizeof(t) / sizeof(int);
-    constexpr int kAhead = 8;
+    constexpr int kAhead = 4;  // parts at once
     typedef float f32x2 __attribute__((ext_vector_type(2)));
     float part[kTasks], own[kTasks], front[kTasks];
     f32x4 a[kTasks][2], b[kTasks][2];
@@ -822,8 +824,8 @@ __global__ __launch_bounds__(kMPWaves * 64) void merge_join_kernel(JoinProblem j
       for (int u = 0; u < kAhead; ++u)
         if (t[i] >= 0 && g + G * u < j.splits) q[i][u] = load(i, g + G * u);
     }
-    merge_tasks<true, false, kMPSlots, kTasks>(p, t, h, g, G, lane, a, 0, own);
-    if (j.step[1].num_seqs > 0) merge_tasks<true, false, kMPSlots, kTasks>(j.step[1], t, h, g, G, lane, b, 0, front);
+    merge_tasks<true, false, kMJSlots, kTasks>(p, t, h, g, G, lane, a, 0, own);
+    if (j.step[1].num_seqs > 0) merge_tasks<true, false, kMJSlots, kTasks>(j.step[1], t, h, g, G, lane, b, 0, front);
 #pragma unroll
     for (int i = 0; i < kTasks; ++i) {
       const float m = fmaxf(wave_max(part[i]), fmaxf(own[i], front[i]));
@@ -885,6 +887,11 @@ __global__ __launch_bounds__(kMPWaves * 64) void merge_join_kernel(JoinProblem j
       put8(rr, 8 * c8, v0, v1);
     }
   }
+  // the weights only now: held through the merge beside the slot rows they cost
+  // the second workgroup per CU
+  vec bw[16];
+#pragma unroll
+  for (int ks = 0; ks < 16; ++ks) bw[ks] = __builtin_bit_cast(vec, *reinterpret_cast<const i16x8*>(wrow + 32 * ks));
   __syncthreads();
 
   // A[m = lane % 16][k = 32 ks + 8 (lane / 16) + j] = O[m][k] (high, low)
