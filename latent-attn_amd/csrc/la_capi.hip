@@ -490,6 +490,22 @@ int key_splits(int64_t blocks, int64_t tiles, int least) {
   const int64_t n = tiles >= 16 * two ? two : std::min(one, tiles / 2);
   return (int)std::max<int64_t>(least, std::min<int64_t>(n, 32));
 }
+// Heads of an XCD that prompt_kernel takes together: as many as fill its CUs'
+// two workgroups each, four at least (their keys and values share its L2, and
+// the long query tiles of several heads do not end the call); with all 16 of
+// 128 heads / 8 / 4 / one after another, a call, us: 300 rows 42.4 / 46.1 / 46.4 /
+// 47.5, 600 78.1 / 72.5 / 75.2 / 83.1, 1001 113 / 110 / 115 / 122, 2000 273 / 274 /
+// 268 / 280, 4000 811 / 798 / 795 / 819, 16 x 300 431 / 431 / 431 / 455, 8192 3019 /
+// 2782 / 2644 / 2679; 16 heads, both / one: 2000 rows 68.9 / 73.7, 8000 339 / 346.
+// 0: heads that the XCDs do not share evenly, in order.
+int head_order(int heads, int64_t blocks) {
+  if (heads % 8 != 0) return 0;
+  const int64_t most = std::max<int64_t>(4, 64 / blocks);
+  int group = 1;
+  for (int g = 2; g <= heads / 8 && g <= most; ++g)
+    if (heads / 8 % g == 0) group = g;
+  return group;
+}
 bool valid_out(int d) { return valid_dtype(d); }
 // Head shape of the expanded form's kernels.
 bool expanded_dims(const la_mla_config& c) {
@@ -864,9 +880,7 @@ int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need)
     for (int h = 0; h < nh && r == hipSuccess; h += p.group) {
       e.p.head0 = m.head0 = h;
       e.p.heads = m.heads = std::min(p.group, nh - h);
-      // (128 heads, a call by head / by tile: 300 rows 45 / 41 us, 1001 121 / 112, 2000 293 / 284, 16 x 300 438 / 413,
-      // 4000 854 / 843, 12 documents of 13,060 rows 1610 / 1629, 8192 2765 / 3165; 16 heads x 2000 73 / 68)
-      m.by_tile = m.heads % 8 == 0 && p.src.num_tiles <= 96;
+      m.group = head_order(m.heads, (a->tokens + prompt_query_rows() - 1) / prompt_query_rows() * m.splits);
       r = launch_expand(e.p, stream, cu_count());
       if (r == hipSuccess) r = launch_prompt(m, stream);
     }

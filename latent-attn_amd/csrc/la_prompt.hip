@@ -289,19 +289,19 @@ struct Item {
   const char *kx, *vx, *rx;
 };
 __device__ inline bool find_item(const PromptProblem& p, Item& it) {
-  // Long sequences: items in order of head, part and query tile (the last, with
-  // the most keys to see, first), an eighth of them to each XCD, so that the
-  // workgroups that read one head's keys share an L2. Where a head's keys are few
-  // (by_tile), the last tiles of all of an XCD's heads (every eighth) first: a
-  // late long tile is what the call ends with otherwise.
+  // An eighth of the items to each XCD, so that the workgroups that read one
+  // head's keys share an L2: groups of its heads (every eighth), within them the
+  // last query tiles, with the most keys to see, of all heads first. Without
+  // groups: an eighth of all, in order of head, part and query tile.
   const int64_t items = (int64_t)p.heads * p.splits * p.q_tiles, per = (items + 7) / 8;
   if ((int64_t)(blockIdx.x >> 3) >= per) return false;
   int qt;
-  if (p.by_tile) {
-    const uint32_t heads = (uint32_t)p.heads / 8, k = blockIdx.x >> 3, rest = k / heads;
-    it.h = (int)((k - rest * heads) * 8 + (blockIdx.x & 7));
-    const uint32_t r = rest / (uint32_t)p.splits;
-    it.part = (int)(rest - r * (uint32_t)p.splits);
+  if (p.group) {
+    const uint32_t group = (uint32_t)p.group, one = group * (uint32_t)p.splits * (uint32_t)p.q_tiles;
+    const uint32_t k = blockIdx.x >> 3, first = k / one, rest = k - first * one, t = rest / group;
+    it.h = (int)((first * group + rest - t * group) * 8 + (blockIdx.x & 7));
+    const uint32_t r = t / (uint32_t)p.splits;
+    it.part = (int)(t - r * (uint32_t)p.splits);
     qt = (int)((uint32_t)p.q_tiles - 1 - r);
   } else {
     const int64_t item = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);

@@ -251,7 +251,7 @@ struct PromptProblem {
   float* part_o;    // [split][token][nh][128], normalised
   float* part_lse;  // [split][token][nh], base 2
   int64_t q_tiles;
-  int by_tile;  // order of the workgroups (heads a multiple of 8)
+  int group;  // order of the workgroups: heads of an XCD taken together (a divisor of heads / 8), or 0
   int nope_vec, rope_vec, table_vec;  // 16-byte (queries: whole-vector) aligned
 };
 int prompt_query_rows();  // query tokens per workgroup
