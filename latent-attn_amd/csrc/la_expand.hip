@@ -141,8 +141,8 @@ __global__ __launch_bounds__(256) void convert_kernel(const void* src, int src_d
 // positions per workgroup of 8 waves: a quarter of the weight rows (0, 1: K
 // dims; 2, 3: V dims) by half of the positions each. Stages of kBk latent
 // columns in a ring in LDS: one is read, the others are on their way. 16-byte
-// chunk j of row r lies at j ^ (r % 8), which the copies' addresses apply, so
-// that 8 rows' chunks fill all banks.
+// chunk j of row r lies at j ^ (r / 2 % 8), which the copies' addresses apply:
+// rows are half as long as all banks, so 16 rows' chunks fill them.
 //
 // The rows and weights that pass the L2 bound it, not its products (with the
 // copies left out 8192 rows x 128 heads took 234 us for 334, with the products
@@ -219,7 +219,8 @@ __device__ inline void expand_wave(const ExpandProblem& p, int64_t step, lchar* 
     for (int i = 0; i < G::kCopies; ++i) {
       const int r0 = 8 * (G::kCopies * wave + i);  // a copy's rows are all X's, W_UK's or W_UV's
       base[i] = r0 < G::kPos ? X : r0 < G::kPos + 128 ? WK + (r0 - G::kPos) * (kDc * 2) : WV + (r0 - G::kPos - 128) * (kDc * 2);
-      off[i] = (uint32_t)((r0 < G::kPos ? min(r0 + r, rows - 1) : r) * (kDc * 2) + 16 * ((lane & 7) ^ r));
+      off[i] = (uint32_t)((r0 < G::kPos ? min(r0 + r, rows - 1) : r) * (kDc * 2) +
+                          16 * ((lane & 7) ^ (4 * ((G::kCopies * wave + i) & 1) + (r >> 1))));
     }
   };
   // inline asm without outputs: behind the builtin the compiler waits for every LDS read at once
@@ -267,7 +268,7 @@ __device__ inline void expand_wave(const ExpandProblem& p, int64_t step, lchar* 
       }
       const int at = k % G::kRing * G::kStageBytes;
       auto read = [&](int ks) {
-        const int c = at + 16 * ((2 * ks + g) ^ (r32 & 7));
+        const int c = at + 16 * ((2 * ks + g) ^ (r32 >> 1 & 7));
 #pragma unroll
         for (int j = 0; j < 2; ++j) w[ks & 1][j] = *reinterpret_cast<lvec*>(wr + 32 * j * kRowBytes + c);
 #pragma unroll
