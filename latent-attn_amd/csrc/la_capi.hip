@@ -1100,7 +1100,8 @@ int decode_shared(const la_shared_args* a, hipStream_t stream, bool run_it, size
   }
   // Validates both steps. One kernel merges their slots, projects and joins
   // where the slots are the MFMA kernels'. Heads in whole blocks of 32 query rows
-  // lie alike in both steps, which then share the absorbed queries.
+  // lie alike in both steps, which then share the absorbed queries (steps that
+  // merge by themselves do not: their absorption zeroes the output of a half-row merge).
   la::DecodeProblem probe;
   Plan plan;
   int st = prepare(&own, &probe, &plan);
@@ -1110,7 +1111,7 @@ int decode_shared(const la_shared_args* a, hipStream_t stream, bool run_it, size
     st = prepare(&pre, &probe, &plan);
     if (st != LA_SUCCESS) return st;
     one = one && merge_join_supported(probe);
-    share = share && plan.absorb_prep;
+    share = share && one && plan.absorb_prep;
   }
   const size_t own_bytes = la_mla_decode_workspace_size(&own);
   if (pre.num_seqs > 0) pre_bytes = la_mla_decode_workspace_size(&pre);

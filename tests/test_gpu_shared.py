@@ -209,6 +209,23 @@ def test_weight_types(cuda, kv, model):
         c.check(c.run(c.expand(), kernel_variant=form), f"{kv} {model} {form}")
 
 
+@pytest.mark.parametrize("kv", [torch.float16, torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("model", [(torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16),
+                                   (torch.float16, torch.bfloat16)])
+@pytest.mark.parametrize("heads", [16, 32, 128])
+def test_weights_of_two_types(cuda, kv, model, heads):
+    """Absorption and projection weights of their own types, with heads that share their absorbed queries between the
+    two steps and others; into a workspace that holds NaN."""
+    c = Case(cuda, 150, [5, 0, 40], heads=heads, kv=kv, layout="capacity", model=torch.float32)
+    c.W_UK, c.W_UV = c.W_UK.to(model[0]), c.W_UV.to(model[1])
+    p = c.expand()
+    for form in (LATENT, EXPANDED):
+        for _ in range(2):
+            junk = torch.full((64 << 20,), float("nan"), device=cuda)  # what the allocator gives out next
+            del junk
+            c.check(c.run(p, kernel_variant=form), f"{kv} {model} {form}")
+
+
 def test_lengths_outside_their_regions(cuda):
     c = Case(cuda, 100, [64, 9], layout="capacity")
     cap = c.layout.kv.shape[1]
