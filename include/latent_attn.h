@@ -25,6 +25,11 @@
  *                            (host-to-device copies of one row plus a stream
  *                            synchronize per token), done on the device for
  *                            every sequence at once, with the query's RoPE
+ * Beside them, without a counterpart there:
+ *   la_mla_prefill        attention of several new tokens per sequence under a
+ *                         causal or prefix mask (prompts, chunks, drafted tokens)
+ *   la_expand_prefix      a shared prefix's keys and values, expanded once
+ *   la_mla_decode_shared  a decode step of sequences behind one prefix
  *
  * Layouts (all row-major, contiguous):
  *   latent cache row   [c_t (kv_lora_rank) | k_rope (qk_rope_head_dim)]
@@ -268,7 +273,9 @@ typedef struct la_prefill_args {
   /* 0 = automatic; 1 = plain kernel (any type and head shape); 2 = keys and
    * values expanded from the rows, on the matrix cores; 3 = queries absorbed,
    * every token a sequence of a paged decode step. LA_ERROR_NOT_SUPPORTED
-   * where the form has no kernel for these arguments. */
+   * where the form has no kernel for these arguments. Form 2 holds keys,
+   * values and queries in 16 bits: bf16, or fp16 for an F16 cache, whose
+   * range they then have to keep to. */
   int32_t kernel_variant;
 } la_prefill_args;
 

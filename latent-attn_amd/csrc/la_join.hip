@@ -39,9 +39,12 @@ __device__ inline float step_lse(const DecodeProblem& p, int64_t row, int l32) {
   return l == 0.f ? -INFINITY : m + log2f(l);
 }
 
-// 32 lanes per query row, four values each at a time where rows are whole
-// vectors. The decode results go out before the log-sum-exps are known: those
-// take several dependent loads, which are most of the kernel's time.
+// For parts that no merge can take along: key splits of a prompt, and decode
+// steps of the VALU or fp32 kernels. 32 lanes per query row, four values each at
+// a time where rows are whole vectors; bound by latency, then by the parts'
+// bytes (1024 tokens x 16 heads x 3 parts 7.5 us, 25 MB). The decode results go
+// out before the log-sum-exps are known: those take several dependent loads,
+// which are most of the kernel's time.
 template <bool kVec>
 __global__ __launch_bounds__(256) void join_kernel(JoinProblem p) {
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);

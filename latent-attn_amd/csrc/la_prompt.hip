@@ -351,7 +351,23 @@ __device__ inline void copy_tile(const Item& it, lchar* b, int t, int wave, int 
 }
 __device__ inline void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// 4 waves, two workgroups per CU, whose waves overlap each other's softmax and products.
+// 4 waves of 32 tokens over 64 keys at a time, two buffers of 40 KB, two
+// workgroups per CU, whose waves overlap each other's softmax and products.
+// Bound by its products and, through them, by power: 8192 tokens x 128 heads,
+// 2.75 TFLOP, take 2.35 ms, 1.17 PFLOP/s, the matrix cores 68 % busy at the 1.66
+// GHz that the card then holds (a whole call 2.62 ms with random numbers, 2.2
+// with zeros). Every operand byte serves 32 tokens, so LDS reads (40 KB per wave
+// and tile) take as long as the products do; they and the vector work hide
+// behind the other waves. Not taken, a call (2743 us then): two groups of four
+// waves in step, one in its products while the other is in its softmax, 2716 to
+// 2772; 64 tokens per wave, half the reads but one wave per SIMD, 2960 to 3160.
+// 64 tokens of one step over 8192 shared rows: 512 MB of keys and values in 105
+// us, 5.1 TB/s.
+// Roundings to 16 bits, the products' operand type: expanded keys and values,
+// the queries (rotated first) and a tile's exponentials, as the decode kernels
+// round rows, queries and exponentials; scores, maxima, sums and outputs are
+// fp32. The scale goes into one side before its rounding, and the running
+// maximum lets exponentials reach 2^8, which fp16 holds.
 template <typename T>
 __global__ __launch_bounds__(256, 2) void prompt_kernel(PromptProblem p) {
   extern __shared__ __attribute__((aligned(1024))) char prompt_lds[];
@@ -408,7 +424,9 @@ hipError_t prompt_t(const PromptProblem& p, hipStream_t stream) {
 
 // One workgroup of 4 waves per (token, head) over absorbed fp32 queries: wave w
 // takes rows w, w + 4, ... with a running maximum of its own, lanes share a
-// row's elements; the waves' sums are joined and projected by W_UV.
+// row's elements; the waves' sums are joined and projected by W_UV. Everything
+// fp32. Rows come from L2 once per head and token, which bounds it; it is there
+// for shapes and types that the others do not take.
 constexpr int kGenericLatent = 1024;  // kv_lora_rank at most: 16 elements per lane
 constexpr int kGenericRope = 256;
 __global__ __launch_bounds__(256) void generic_prompt_kernel(GenericPrompt p) {

@@ -4,7 +4,9 @@ Same entry points and argument order as the reference
 (latent_attn/functional.py:24-116 in the reference repo): ``fused_mla``,
 ``naive_mla``, ``batched_fused_mla``; plus ``mla_decode`` (per-sequence and
 ragged caches with query absorption, split-KV and the W_UV projection in one
-call) and ``absorb_q``. All compute runs in the HIP library; nothing here
+call) and ``absorb_q``; ``append_kv``; ``mla_prefill`` (several new tokens per
+sequence: prompts, chunks, drafted tokens), ``expand_prefix`` and
+``mla_decode_shared`` (decode behind one prefix of the whole batch). All compute runs in the HIP library; nothing here
 falls back to PyTorch math -- if the extension is missing, the call raises.
 """
 
