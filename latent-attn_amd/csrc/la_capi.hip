@@ -581,7 +581,7 @@ void carve_expand(Carve& c, ExpandPlan& e, const void* W_UK, int uk_dtype, const
 }
 hipError_t start_expand(const ExpandPlan& e, const void* W_UK, int uk_dtype, const void* W_UV, int uv_dtype, bool copy_uk,
                         bool copy_uv, hipStream_t stream) {
-  hipError_t r = launch_gather(e.p, stream);
+  hipError_t r = launch_gather(e.p, stream, cu_count());
   if (r == hipSuccess && copy_uk) r = launch_convert(W_UK, uk_dtype, e.uk_copy, e.p.f16, (int64_t)e.copy_elems, stream);
   if (r == hipSuccess && copy_uv) r = launch_convert(W_UV, uv_dtype, e.uv_copy, e.p.f16, (int64_t)e.copy_elems, stream);
   return r;
@@ -857,6 +857,7 @@ int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need)
     e.p.q_tiles = p.q_tiles;
     e.p.query_rows = prompt_query_rows();
     e.p.k_scale = scale_log2;  // the softmax's scale goes into the keys before their one rounding
+    e.p.heads = p.group;
     hipError_t r = start_expand(e, a->W_UK, a->w_uk_dtype, a->W_UV, a->w_uv_dtype, e.uk_copy, e.uv_copy, stream);
     PromptProblem m{};
     m.q = p.q;

@@ -68,65 +68,99 @@ __device__ inline typename Mm<T>::vec load8(const KT* p) {
 // 13 us.
 constexpr int kGatherRows = 16;
 constexpr int kGatherParts = kTileKeys / kGatherRows;
-template <typename KT, typename T, bool kAligned>
-__global__ __launch_bounds__(256) void gather_kernel(ExpandProblem p) {
+// Sequence of a tile, the position of its first row and its rows.
+struct TileRows {
+  int s, pos0, rows;
+};
+__device__ inline TileRows tile_rows_of(const RowSource& src, int64_t tile) {
+  const int s = source_find(src, tile);
+  const int64_t t = tile - source_tile(src, s);  // < 0: rows before the first sequence
+  const int L = t < 0 ? 0 : source_rows(src, s);
+  return TileRows{s, (int)t * kTileKeys, (int)clamp64(L - t * kTileKeys, 0, L > 0 ? kTileKeys : 0)};
+}
+// Rows r0 + step i (i < kN) of a tile by one wave, eight elements per lane, to
+// put(row, elements); bit i of the result: row i was not finite.
+template <typename KT, typename T, bool kAligned, int kN, typename Put>
+__device__ inline uint32_t latent_rows(const RowSource& src, const TileRows& tr, int r0, int step, int lane, Put put) {
   typedef typename Mm<T>::vec vec;
-  typedef typename Mm<T>::elem elem;
-  typedef elem vec4 __attribute__((ext_vector_type(4)));
-  const int64_t tile = blockIdx.x / kGatherParts;
-  if (tile >= p.src.num_tiles) {
-    const int64_t qt = ((int64_t)blockIdx.x - p.src.num_tiles * kGatherParts) * 256 + threadIdx.x;
-    if (qt < p.q_tiles) p.q_info[qt] = make_query_tile(p.q, p.src, qt, p.query_rows);
-    return;
-  }
-  const int s = source_find(p.src, tile);
-  const int64_t t = tile - source_tile(p.src, s);  // < 0: rows before the first sequence
-  const int L = t < 0 ? 0 : source_rows(p.src, s);
-  const int rows = (int)clamp64(L - t * kTileKeys, 0, L > 0 ? kTileKeys : 0);
-  const int part = blockIdx.x % kGatherParts * kGatherRows;
-  if (threadIdx.x == 0 && part == 0) p.tile_rows[tile] = rows;
-  if (rows == 0) return;
-  const int pos0 = (int)t * kTileKeys;
-  const KT* kv = static_cast<const KT*>(p.src.kv);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  vec* const c_out = reinterpret_cast<vec*>(static_cast<char*>(p.rows_c) + tile * kTileCBytes);
-  __shared__ int bad[kGatherRows];
-  vec v[kGatherRows / 4] = {};
+  const KT* const kv = static_cast<const KT*>(src.kv);
+  vec v[kN] = {};
 #pragma unroll
-  for (int i = 0; i < kGatherRows / 4; ++i) {
-    const int r = part + wave + 4 * i;
-    if (r < rows) v[i] = load8<KT, T, kAligned>(kv + source_row(p.src, s, pos0 + r) * p.src.row_elems + 8 * lane);
+  for (int i = 0; i < kN; ++i) {
+    const int r = r0 + step * i;
+    if (r < tr.rows) v[i] = load8<KT, T, kAligned>(kv + source_row(src, tr.s, tr.pos0 + r) * src.row_elems + 8 * lane);
   }
+  uint32_t bad = 0;
 #pragma unroll
-  for (int i = 0; i < kGatherRows / 4; ++i) {
+  for (int i = 0; i < kN; ++i) {
     float z = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) z = __builtin_fmaf((float)v[i][e], 0.f, z);
-    const bool any = __builtin_amdgcn_ballot_w64(!(z == 0.f)) != 0;
-    if (any) v[i] = vec{};
-    if (lane == 0) bad[wave + 4 * i] = any;
-    c_out[(part + wave + 4 * i) * 64 + lane] = v[i];
-  }
-  __syncthreads();
-  if (threadIdx.x >= kGatherRows * 8) return;
-  elem* const r_out = reinterpret_cast<elem*>(static_cast<char*>(p.rope) + tile * kTileRBytes);
-  const int r = part + (threadIdx.x >> 3), d = 4 * (threadIdx.x & 7);  // dims d .. d+3 and their partners d + 32 ..
-  vec4 a = {}, b = {};
-  if (r < rows) {
-    const KT* k = kv + source_row(p.src, s, pos0 + r) * p.src.row_elems + 512 + d;
-    const int64_t at = source_rope_row(p.src, pos0 + r) * 32 + d;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float k0 = to_f32(k[e]), k1 = to_f32(k[e + 32]), c = p.src.cos[at + e], sn = p.src.sin[at + e];
-      a[e] = (elem)((k0 * c - k1 * sn) * p.k_scale);
-      b[e] = (elem)((k0 * sn + k1 * c) * p.k_scale);
+    if (__builtin_amdgcn_ballot_w64(!(z == 0.f)) != 0) {
+      v[i] = vec{};
+      bad |= 1u << i;
     }
-    const elem nan = (elem)__builtin_nanf("");
-    if (bad[r - part]) a = b = vec4{nan, nan, nan, nan};
+    put(r0 + step * i, v[i]);
   }
+  return bad;
+}
+// Piece `block` of the gather by 4 waves: kGatherRows rows of a tile, or 256 query
+// tiles. kRows: the latent rows and the tile's row count are stored, not the rope keys alone.
+template <typename KT, typename T, bool kAligned, bool kRows>
+__device__ inline void gather_piece(const ExpandProblem& p, int64_t block, int wave, int lane) {
+  typedef typename Mm<T>::vec vec;
+  typedef typename Mm<T>::elem elem;
+  typedef elem vec4 __attribute__((ext_vector_type(4)));
+  const int64_t tile = block / kGatherParts;
+  if (tile >= p.src.num_tiles) {
+    const int64_t qt = (block - p.src.num_tiles * kGatherParts) * 256 + 64 * wave + lane;
+    if (qt < p.q_tiles) p.q_info[qt] = make_query_tile(p.q, p.src, qt, p.query_rows);
+    return;
+  }
+  const TileRows tr = tile_rows_of(p.src, tile);
+  const int r0 = (int)(block % kGatherParts) * kGatherRows + wave;
+  if (kRows && r0 == 0 && lane == 0) p.tile_rows[tile] = tr.rows;
+  if (tr.rows == 0) return;
+  // the wave's rope keys, 8 lanes a row: dims d .. d + 3 and their partners d + 32 ..
+  const int r = r0 + 4 * (lane >> 3 & 3), d = 4 * (lane & 7);
+  float k0[4] = {}, k1[4] = {}, c[4] = {}, sn[4] = {};
+  if (r < tr.rows) {
+    const KT* const k = static_cast<const KT*>(p.src.kv) + source_row(p.src, tr.s, tr.pos0 + r) * p.src.row_elems + 512 + d;
+    const int64_t at = source_rope_row(p.src, tr.pos0 + r) * 32 + d;
+    KT b0[4], b1[4];
+    if constexpr (kAligned) {
+      __builtin_memcpy(b0, __builtin_assume_aligned(k, sizeof(b0)), sizeof(b0));
+      __builtin_memcpy(b1, __builtin_assume_aligned(k + 32, sizeof(b1)), sizeof(b1));
+    } else {
+      __builtin_memcpy(b0, k, sizeof(b0));
+      __builtin_memcpy(b1, k + 32, sizeof(b1));
+    }
+    __builtin_memcpy(c, p.src.cos + at, sizeof(c));
+    __builtin_memcpy(sn, p.src.sin + at, sizeof(sn));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) k0[e] = to_f32(b0[e]), k1[e] = to_f32(b1[e]);
+  }
+  vec* const c_out = reinterpret_cast<vec*>(static_cast<char*>(p.rows_c) + tile * kTileCBytes);
+  const uint32_t bad = latent_rows<KT, T, kAligned, kGatherRows / 4>(p.src, tr, r0, 4, lane, [&](int row, const vec& v) {
+    if constexpr (kRows) c_out[row * 64 + lane] = v;
+  });
+  if (lane >= 32) return;
+  vec4 a, b;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    a[e] = (elem)((k0[e] * c[e] - k1[e] * sn[e]) * p.k_scale);
+    b[e] = (elem)((k0[e] * sn[e] + k1[e] * c[e]) * p.k_scale);
+  }
+  const elem nan = (elem)__builtin_nanf("");
+  if (bad >> (lane >> 3) & 1) a = b = vec4{nan, nan, nan, nan};
+  elem* const r_out = reinterpret_cast<elem*>(static_cast<char*>(p.rope) + tile * kTileRBytes);
   elem* const o = r_out + (r >> 5) * (4 * 512) + operand_elem(r, d & 15);
   *reinterpret_cast<vec4*>(o + (d >> 4) * 512) = a;
   *reinterpret_cast<vec4*>(o + ((d >> 4) + 2) * 512) = b;
+}
+template <typename KT, typename T, bool kAligned>
+__global__ __launch_bounds__(256) void gather_kernel(ExpandProblem p) {
+  gather_piece<KT, T, kAligned, true>(p, blockIdx.x, __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), threadIdx.x & 63);
 }
 
 __global__ __launch_bounds__(256) void convert_kernel(const void* src, int src_dtype, uint16_t* dst, int f16, int64_t n) {
@@ -180,8 +214,9 @@ __host__ __device__ inline int64_t items_per_xcd(int heads, int64_t tiles, int p
 
 template <int N>
 __device__ inline void wait_copies() {
-  static_assert(N == 0 || N == 10 || N == 16, "");
+  static_assert(N == 0 || N == 4 || N == 10 || N == 16, "");
   if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  else if constexpr (N == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
   else if constexpr (N == 10) asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
   else asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
 }
@@ -344,6 +379,126 @@ hipError_t expand_pb(const ExpandProblem& p, hipStream_t stream, int ncu) {
   return hipGetLastError();
 }
 
+// ---- gather and expand in one: small calls ---------------------------------------------
+
+// A workgroup of 8 waves per (head, tile): its 64 latent rows to LDS, then the
+// product as in expand_kernel, the weights in a ring of three stages whose
+// copies are on their way before the rows are looked up. The workgroups behind
+// the items write the rope keys and query tiles, two pieces of the gather each.
+// Latency of its loads: 17 rows x 16 heads 8 us (gather and expansion one after
+// the other 12), 300 x 16 a call 9.3 (11.2).
+constexpr int kSmallW = kNRows * kRowBytes;  // a stage of weights
+constexpr int kSmallRing = 3;
+constexpr int kSmallX = kTileKeys * kDc * 2;
+constexpr int kSmallLds = kSmallX + kSmallRing * kSmallW;
+static_assert(kSmallLds <= 160 * 1024, "LDS of a CU");
+
+// Stage k of the weights into its part of the ring: four copies of 8 rows per
+// wave (32 rows from W on); past the end the last stage again, never read.
+__device__ inline void small_issue(lchar* L, const char* W, uint32_t off, int k, int wave) {
+  const uint32_t buf = (uint32_t)(uintptr_t)L + kSmallX + k % kSmallRing * kSmallW + 4096 * wave;
+  const char* const from = W + min(k, kStages - 1) * kRowBytes;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)  // (odd groups of 8 rows: 4 in the swizzle's row pairs)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(buf + 1024 * i),
+                 "v"(off ^ (i & 1 ? 64u : 0u)), "s"(from + i * 8 * (kDc * 2))
+                 : "memory", "m0");
+}
+template <typename T, bool kV>
+__device__ inline void small_products(const ExpandProblem& p, lchar* L, int64_t tile, int h, int lane, int wave,
+                                      const char* W, uint32_t off) {
+  typedef typename Mm<T>::vec vec;
+  typedef typename Mm<T>::elem elem;
+  typedef const __attribute__((address_space(3))) vec lvec;
+  const int wn = wave & 3, wp = wave >> 2, r32 = lane & 31, g = lane >> 5;
+  f32x16 acc[2] = {};
+  const lchar* const xr = L + (32 * wp + r32) * (kDc * 2);
+  const lchar* const wr = L + kSmallX + (64 * wn + r32) * kRowBytes;
+#pragma unroll 1
+  for (int k = 0; k < kStages; ++k) {
+    wait_copies<4>();  // this wave's of stage k have landed, those of the next may be on their way
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    small_issue(L, W, off, k + kSmallRing - 1, wave);
+    const lchar* const w0 = wr + k % kSmallRing * kSmallW;
+#pragma unroll
+    for (int ks = 0; ks < kBk / 16; ++ks) {
+      vec w[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        w[j] = *reinterpret_cast<lvec*>(w0 + 32 * j * kRowBytes + 16 * ((2 * ks + g) ^ (r32 >> 1 & 7)));
+      const vec x = *reinterpret_cast<lvec*>(xr + 16 * ((8 * k + 2 * ks + g) ^ (r32 & 15)));
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[j] = kV ? Mm<T>::mma(x, w[j], acc[j]) : Mm<T>::mma(w[j], x, acc[j]);
+    }
+  }
+  char* const out = static_cast<char*>(kV ? p.vx : p.kx) + ((int64_t)h * p.src.num_tiles + tile) * kTileKBytes;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    settle(acc[j]);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      vec v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (elem)(kV ? acc[j][8 * q + e] : acc[j][8 * q + e] * p.k_scale);
+      const int db = 2 * (wn & 1) + j;  // block of 32 dims
+      const int piece = kV ? 4 * db + 2 * wp + q : 8 * wp + 2 * db + q;
+      *reinterpret_cast<vec*>(out + piece * 1024 + 16 * lane) = v;
+    }
+  }
+}
+
+template <typename KT, typename T, bool kAligned>
+__global__ __launch_bounds__(512, 2) void gather_expand_kernel(ExpandProblem p, int64_t items) {
+  extern __shared__ __attribute__((aligned(1024))) char small_lds[];
+  typedef typename Mm<T>::vec vec;
+  lchar* const L = (lchar*)small_lds;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  if (blockIdx.x >= items) {
+    const int64_t pieces = p.src.num_tiles * kGatherParts + (p.q_tiles + 255) / 256;
+    const int64_t piece = 2 * ((int64_t)blockIdx.x - items) + (wave >> 2);
+    if (piece < pieces) gather_piece<KT, T, kAligned, false>(p, piece, wave & 3, lane);
+    return;
+  }
+  const int per = (p.heads + 7) / 8, k = blockIdx.x >> 3, h = k % per * 8 + (blockIdx.x & 7);  // a head's on one XCD
+  const int64_t tile = k / per;
+  if (h >= p.heads) return;
+  // Copies of a stage: 4 of a wave's, 8 weight rows of 128 B each; its rows are all W_UK's or W_UV's.
+  const char* const W = static_cast<const char*>(wave < 4 ? p.W_UK : p.W_UV) +
+                        ((int64_t)(p.head0 + h) * 128 + 32 * (wave & 3)) * (kDc * 2);
+  const int r = lane >> 3;
+  const uint32_t off = (uint32_t)(r * (kDc * 2)) + 16 * ((lane & 7) ^ (r >> 1));  // of an even group of 8 rows
+#pragma unroll
+  for (int i = 0; i < kSmallRing - 1; ++i) small_issue(L, W, off, i, wave);
+  const TileRows tr = tile_rows_of(p.src, tile);
+  if (tr.rows > 0) {
+    latent_rows<KT, T, kAligned, 8>(p.src, tr, wave, 8, lane, [&](int row, const vec& v) {
+      typedef __attribute__((address_space(3))) vec lvec;
+      *reinterpret_cast<lvec*>(L + row * (kDc * 2) + 16 * (lane ^ (row & 15))) = v;
+    });
+    if ((wave & 3) >= 2) small_products<T, true>(p, L, tile, h, lane, wave, W, off);
+    else small_products<T, false>(p, L, tile, h, lane, wave, W, off);
+  }
+  wait_copies<0>();  // all copies have landed: the workgroup may end
+}
+
+template <typename KT, typename T>
+hipError_t gather_expand_t(const ExpandProblem& p, bool aligned, hipStream_t stream) {
+  const void* const k = aligned ? reinterpret_cast<const void*>(gather_expand_kernel<KT, T, true>)
+                                : reinterpret_cast<const void*>(gather_expand_kernel<KT, T, false>);
+  static OncePerDevice once[2];
+  const hipError_t e = allow_lds(once[aligned], k, kSmallLds);
+  if (e != hipSuccess) return e;
+  const int64_t items = 8 * (int64_t)((p.heads + 7) / 8) * p.src.num_tiles;
+  const int64_t pieces = p.src.num_tiles * kGatherParts + (p.q_tiles + 255) / 256;
+  const int64_t blocks = items + (pieces + 1) / 2;
+  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  if (aligned)
+    hipLaunchKernelGGL((gather_expand_kernel<KT, T, true>), dim3((unsigned)blocks), dim3(512), kSmallLds, stream, p, items);
+  else
+    hipLaunchKernelGGL((gather_expand_kernel<KT, T, false>), dim3((unsigned)blocks), dim3(512), kSmallLds, stream, p, items);
+  return hipGetLastError();
+}
+
 template <typename KT, typename T>
 hipError_t gather_t(const ExpandProblem& p, bool aligned, hipStream_t stream) {
   const dim3 grid((unsigned)(p.src.num_tiles * kGatherParts + (p.q_tiles + 255) / 256));
@@ -352,10 +507,18 @@ hipError_t gather_t(const ExpandProblem& p, bool aligned, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// Gathers in the expansion's workgroups, one per (head, tile), where half the
+// CUs hold them (us a call, three launches / two: 17 tokens x 16 heads 20.4 /
+// 17.4, x 128 22.8 / 18.5, 256 x 16 29.6 / 27.5; one per CU, 1000 x 16 43.9 / 45.0;
+// two per CU, 250 x 128 38.4 / 44.4: every head reads and converts the rows).
+bool small_call(const ExpandProblem& p, int ncu) {
+  return p.src.num_tiles > 0 && 2 * (int64_t)p.heads * p.src.num_tiles <= ncu;
+}
+
 }  // namespace
 
-hipError_t launch_gather(const ExpandProblem& p, hipStream_t stream) {
-  if (p.src.num_tiles == 0 && p.q_tiles == 0) return hipSuccess;
+hipError_t launch_gather(const ExpandProblem& p, hipStream_t stream, int ncu) {
+  if (small_call(p, ncu) || (p.src.num_tiles == 0 && p.q_tiles == 0)) return hipSuccess;
   if (p.src.num_tiles > INT32_MAX / 8 || p.q_tiles > INT32_MAX || p.src.row_elems != 576) return hipErrorInvalidValue;
   const bool aligned = (reinterpret_cast<uintptr_t>(p.src.kv) & 15) == 0;  // rows are 1152 or 576 B
   switch (p.src.kv_dtype) {
@@ -368,6 +531,16 @@ hipError_t launch_gather(const ExpandProblem& p, hipStream_t stream) {
 
 hipError_t launch_expand(const ExpandProblem& p, hipStream_t stream, int ncu) {
   if (p.src.num_tiles == 0 || p.heads == 0) return hipSuccess;
+  if (small_call(p, ncu)) {
+    if (p.src.num_tiles > INT32_MAX / 8 || p.q_tiles > INT32_MAX || p.src.row_elems != 576) return hipErrorInvalidValue;
+    const bool aligned = (reinterpret_cast<uintptr_t>(p.src.kv) & 15) == 0;
+    switch (p.src.kv_dtype) {
+      case LA_DTYPE_BF16: return gather_expand_t<__hip_bfloat16, __hip_bfloat16>(p, aligned, stream);
+      case LA_DTYPE_F16: return gather_expand_t<__half, __half>(p, aligned, stream);
+      case LA_DTYPE_FP8_E4M3: return gather_expand_t<fp8e4m3, __hip_bfloat16>(p, aligned, stream);
+      default: return hipErrorInvalidValue;
+    }
+  }
   const bool wide = (int64_t)p.heads * ((p.src.num_tiles + 3) / 4) >= ncu;
   if (p.f16) return wide ? expand_pb<__half, 4>(p, stream, ncu) : expand_pb<__half, 1>(p, stream, ncu);
   return wide ? expand_pb<__hip_bfloat16, 4>(p, stream, ncu) : expand_pb<__hip_bfloat16, 1>(p, stream, ncu);

@@ -229,7 +229,7 @@ struct ExpandProblem {
   float k_scale;  // times K and the rope keys
   int head0, heads;
 };
-hipError_t launch_gather(const ExpandProblem& p, hipStream_t stream);
+hipError_t launch_gather(const ExpandProblem& p, hipStream_t stream, int ncu);
 hipError_t launch_expand(const ExpandProblem& p, hipStream_t stream, int ncu);
 // 16-bit copy of n weights of another type.
 hipError_t launch_convert(const void* src, int src_dtype, void* dst, int f16, int64_t n, hipStream_t stream);

@@ -172,6 +172,30 @@ def test_unaligned_cache_and_weights(cuda):
     assert torch.equal(c.run(kernel_variant=EXPANDED), want)
 
 
+@pytest.mark.parametrize("kv", [torch.bfloat16, torch.float16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("layout", ["capacity", "packed_capacity", "paged"])
+@pytest.mark.parametrize("heads", [32, 128])
+@pytest.mark.parametrize("aligned", [True, False])
+def test_many_heads(cuda, heads, layout, kv, aligned):
+    """The expansion's other tiles (few heads gather in its own workgroups), over caches that begin at any element."""
+    c = Case(cuda, layout, [1, 63, 65, 200], [1, 5, 65, 30], heads=heads, kv=kv)
+    if not aligned:
+        b = torch.zeros(c.layout.kv.numel() + 1, dtype=torch.float32, device=cuda).to(kv)
+        b.view(torch.uint8)[kv.itemsize:] = c.layout.kv.flatten().view(torch.uint8)
+        c.layout.kv = b[1:].view_as(c.layout.kv)
+    c.check(c.run(kernel_variant=EXPANDED), EXPANDED, f"{heads} {layout} {kv}")
+
+
+@pytest.mark.parametrize("heads", [4, 32, 128])
+def test_a_row_that_is_not_finite_by_size(cuda, heads):
+    c = Case(cuda, "packed", [150, 80], [150, 80], heads=heads)
+    want = c.run(kernel_variant=EXPANDED)
+    c.layout.kv[101, 300], c.layout.kv[160, 7] = float("inf"), float("nan")
+    got = c.run(kernel_variant=EXPANDED)
+    assert torch.equal(got[:101], want[:101]) and torch.equal(got[150:160], want[150:160])
+    assert not torch.isfinite(got[101:150]).any() and not torch.isfinite(got[160:]).any()
+
+
 @pytest.mark.parametrize("form", [PLAIN, EXPANDED])
 def test_rows_before_the_first_sequence(cuda, form):
     """Packed sequences that begin past the cache's first rows, which hold NaN."""

@@ -14,7 +14,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 HIPCC = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
 
 
-@pytest.mark.parametrize("source,least", [("la_prompt", 6), ("la_expand", 11), ("la_join", 2)])
+@pytest.mark.parametrize("source,least", [("la_prompt", 6), ("la_expand", 17), ("la_join", 2)])
 def test_no_scratch(source, least, tmp_path):
     if not os.path.exists(HIPCC):
         pytest.skip("hipcc not available")
