@@ -132,6 +132,23 @@ def test_types(cuda, kv, q, w):
         c.check(got, EXPANDED, f"{kv} {q} {w} {out}")
 
 
+@pytest.mark.parametrize("form", [PLAIN, ABSORBED])
+@pytest.mark.parametrize("kv", [torch.bfloat16, torch.float16, torch.float8_e4m3fn, torch.float32])
+@pytest.mark.parametrize("q", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("w", [torch.float32, torch.bfloat16])
+def test_types_of_the_other_forms(cuda, form, kv, q, w):
+    """Every mixture that the plain and the absorbed form take, with 3 heads (no matrix instructions) and 32."""
+    for heads in (3, 32):
+        c = Case(cuda, "capacity", [70, 0, 33], [2, 1, 5], heads=heads, kv=kv, q=q, w=w, pad=1)
+        full = c.run(kernel_variant=form, out_dtype=torch.float32)
+        for out in (torch.float32, torch.bfloat16, torch.float16):
+            got = c.run(kernel_variant=form, out_dtype=out)
+            assert got.dtype == out
+            # the merges of the two outputs may add in different orders: 2^-11 of the value, and one rounding
+            assert ((got.float() - full).abs() <= (2.0 ** -11 + U.get(out, 0.0)) * full.abs() + 1e-4).all()
+        assert_close(full.cpu().numpy(), c.reference()[0].numpy(), "bf16", f"{kv} {q} {w} {heads}")
+
+
 def test_rotation_and_strides(cuda):
     """Queries rotated on the way equal queries rotated before; packed, sliced and oddly strided queries agree."""
     c = Case(cuda, "packed", [90, 40], [90, 11], heads=5, q=torch.float32)
