@@ -877,6 +877,7 @@ int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need)
     m.q_tiles = p.q_tiles;
     m.nope_vec = q_vec(p.q.q_nope, p.q.dtype, p.q.nope_stride, p.q.nope_head);
     m.rope_vec = q_vec(p.q.q_rope, p.q.dtype, p.q.rope_stride, p.q.rope_head);
+    m.q_wide = q_wide(p.q.q_nope, p.q.nope_stride, p.q.nope_head) && q_wide(p.q.q_rope, p.q.rope_stride, p.q.rope_head);
     m.table_vec = tables_aligned(p.src);
     for (int h = 0; h < nh && r == hipSuccess; h += p.group) {
       e.p.head0 = m.head0 = h;

@@ -184,6 +184,10 @@ inline bool q_vec(const void* base, int dtype, int64_t stride, int64_t head) {
   return reinterpret_cast<uintptr_t>(base) % align == 0 && stride % 4 == 0 && head % 4 == 0;
 }
 
+inline bool q_wide(const void* base, int64_t stride, int64_t head) {
+  return reinterpret_cast<uintptr_t>(base) % 16 == 0 && stride % 8 == 0 && head % 8 == 0;
+}
+
 // A query tile as prompt_kernel takes it, found once per call by gather_kernel:
 // binary searches over device offsets in every workgroup were a chain of
 // dependent loads at its start.
@@ -253,6 +257,7 @@ struct PromptProblem {
   int64_t q_tiles;
   int group;  // order of the workgroups: heads of an XCD taken together (a divisor of heads / 8), or 0
   int nope_vec, rope_vec, table_vec;  // 16-byte (queries: whole-vector) aligned
+  int q_wide;  // 16-bit queries: 16-byte aligned
 };
 int prompt_query_rows();  // query tokens per workgroup
 hipError_t launch_prompt(const PromptProblem& p, hipStream_t stream);

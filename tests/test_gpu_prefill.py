@@ -175,6 +175,20 @@ def test_rotation_and_strides(cuda):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("q", [torch.bfloat16, torch.float16])
+def test_queries_by_alignment(cuda, q):
+    """16-bit queries on 16, 8 and 2 bytes, and with strides that are no multiple of 16 bytes: the same numbers."""
+    c = Case(cuda, "packed", [90, 40], [90, 11], heads=5, q=q)
+    want = c.run(kernel_variant=EXPANDED)
+    c.check(want, EXPANDED, f"{q}")
+    kept = c.q
+    for lead, pad in ((0, 0), (8, 0), (4, 0), (1, 0), (0, 4), (0, 1)):
+        wide = torch.zeros(101 * 5 * (192 + pad) + lead, dtype=q, device=cuda)[lead:].view(101, 5, 192 + pad)
+        wide[..., :192] = kept
+        c.q = wide[..., :192]
+        assert torch.equal(c.run(kernel_variant=EXPANDED), want), (lead, pad)
+
+
 def test_unaligned_cache_and_weights(cuda):
     c = Case(cuda, "packed", [70, 33], [70, 20])
     want = c.run(kernel_variant=EXPANDED)
