@@ -387,7 +387,7 @@ __device__ inline void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"
 // 4 waves of 32 tokens over 64 keys at a time, two buffers of 40 KB, two
 // workgroups per CU, whose waves overlap each other's softmax and products.
 // Bound by its products and, through them, by power: 8192 tokens x 128 heads,
-// 2.75 TFLOP, take 2.35 ms, 1.17 PFLOP/s, the matrix cores 68 % busy at the 1.66
+// 2.75 TFLOP, take 2.33 ms, 1.18 PFLOP/s, the matrix cores 69 % busy at the 1.64
 // GHz that the card then holds (a whole call 2.62 ms with random numbers, 2.2
 // with zeros). Every operand byte serves 32 tokens, so LDS reads (40 KB per wave
 // and tile) take as long as the products do; they and the vector work hide
