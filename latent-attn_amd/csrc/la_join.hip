@@ -7,8 +7,6 @@
 namespace la {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
 __device__ inline float max32(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));

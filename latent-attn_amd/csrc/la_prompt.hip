@@ -17,7 +17,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) char lchar;
 
 template <typename T>
@@ -553,7 +552,7 @@ __global__ __launch_bounds__(256) void generic_prompt_kernel(GenericPrompt p) {
 constexpr int kTokenElems = 2048;
 template <int kN>
 __device__ inline void load_n(const void* base, int dtype, int64_t i, float (&x)[kN]) {
-  if constexpr (kN == 4) load_q4(base, dtype, i, true, x);
+  if constexpr (kN == 4) load_q4(base, dtype, i, x);
   else x[0] = load_any(base, dtype, i);
 }
 template <int kN>

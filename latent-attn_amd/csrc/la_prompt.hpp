@@ -160,23 +160,17 @@ inline int64_t source_tiles(const RowSource& r) {
                    : (int64_t)r.num_seqs * ((r.region + kTileKeys - 1) / kTileKeys);
 }
 
-// Four consecutive elements of a query tensor of any type. vec: base and
-// strides keep them aligned to their 8 or 16 bytes.
-__device__ inline void load_q4(const void* base, int dtype, int64_t i, bool vec, float (&x)[4]) {
-  if (vec) {
-    if (dtype == LA_DTYPE_F32) {
-      const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + i);
-      x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-    } else {
-      const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + i);
-      const uint32_t w[4] = {v.x & 0xFFFF, v.x >> 16, v.y & 0xFFFF, v.y >> 16};
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        x[e] = dtype == LA_DTYPE_BF16 ? f_of(w[e] << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
-    }
+// Four consecutive elements of a query tensor of any type, aligned to their 8 or 16 bytes.
+__device__ inline void load_q4(const void* base, int dtype, int64_t i, float (&x)[4]) {
+  if (dtype == LA_DTYPE_F32) {
+    const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + i);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
   } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + i);
+    const uint32_t w[4] = {v.x & 0xFFFF, v.x >> 16, v.y & 0xFFFF, v.y >> 16};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = load_any(base, dtype, i + e);
+    for (int e = 0; e < 4; ++e)
+      x[e] = dtype == LA_DTYPE_BF16 ? f_of(w[e] << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
   }
 }
 inline bool q_vec(const void* base, int dtype, int64_t stride, int64_t head) {
