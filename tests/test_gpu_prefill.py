@@ -513,6 +513,27 @@ def test_captured(cuda, form):
         assert (got[sum(new):] == 0).all()
 
 
+@pytest.mark.parametrize("heads,cap", [(2, 2048), (64, 256)])
+def test_captured_by_size(cuda, heads, cap):
+    """Parts of the keys and their join, and the expansion in a launch of its own, in a graph; lengths that change."""
+    c = Case(cuda, "capacity", [cap - 40, 70], [3, 60], heads=heads)
+    c.run(kernel_variant=EXPANDED)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = c.run(kernel_variant=EXPANDED)
+    c.layout.kv.copy_(torch.randn(c.layout.kv.shape, generator=torch.Generator().manual_seed(7)).to(c.layout.kv.dtype))
+    for lens, new in (([cap - 40, 70], [3, 60]), ([1, cap], [1, 62]), ([0, 65], [60, 3]), ([64, 128], [0, 63])):
+        c.kw["seq_lens"].copy_(torch.tensor(lens, dtype=torch.int32))
+        c.kw["q_offsets"].copy_(torch.tensor([0, new[0], sum(new)], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        eager = c.run(kernel_variant=EXPANDED)
+        torch.cuda.synchronize()
+        assert torch.equal(got, eager) and torch.isfinite(got).all()
+
+
 def test_prompt_then_decode(cuda):
     """append_kv of a prompt, its attention, then a drafted pair of tokens and a single one: the last token's row is
     the decode step's."""

@@ -289,6 +289,28 @@ def test_captured(cuda, form):
         assert torch.equal(got, eager)
 
 
+@pytest.mark.parametrize("rows,heads", [(130, 16), (700, 128)])
+def test_captured_with_its_expansion(cuda, rows, heads):
+    """A prefix that is expanded and read in one graph, replayed over other rows, with eager work between the replays."""
+    c = Case(cuda, rows, [5, 20, 60], heads=heads, layout="capacity")
+    run = lambda: c.run(c.expand(), kernel_variant=EXPANDED)
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for seed in (3, 4, 5):
+        g = torch.Generator().manual_seed(seed)
+        c.front.copy_(torch.randn(c.front.shape, generator=g).to(c.front.dtype))
+        c.W_UV.copy_(torch.randn(c.W_UV.shape, generator=g) / 22)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        eager = run()
+        torch.cuda.synchronize()
+        assert torch.equal(got, eager)
+
+
 def test_a_batch_served(cuda):
     """A server's round: the prefix expanded once, then every sequence's question appended and attended, and single
     tokens after it; each against the reference."""
