@@ -598,6 +598,7 @@ struct Prefill {
   RowSource src{};
   int block_size = 0, blocks_per_seq = 0, used_blocks = 0;  // of the absorbed form
   int64_t pool_rows = 0;
+  bool nope_as_is = false, rope_as_is = false;  // queries that the other forms' kernels take where they lie
   int splits = 1, group = 0;  // of the expanded form: key parts, heads at a time
   int64_t q_tiles = 0;
 };
@@ -703,6 +704,13 @@ int prepare_prefill(const la_prefill_args* a, Prefill* out) {
   q.offsets = a->q_offsets;
   q.per_seq = a->q_offsets ? 0 : (int)(a->tokens / a->num_seqs);
   q.prefix = a->prefix_lens;
+  // (those that are not aligned are copied: a step over them would run on the VALU)
+  const auto as_is = [&](const void* base, int64_t stride, int64_t head, int dim) {
+    return a->q_dtype == LA_DTYPE_F32 && head == dim && stride == (int64_t)c.num_heads * dim &&
+           (reinterpret_cast<uintptr_t>(base) & 15) == 0;
+  };
+  p.nope_as_is = as_is(q.q_nope, q.nope_stride, q.nope_head, c.qk_nope_head_dim);
+  p.rope_as_is = !a->rotate_q && as_is(q.q_rope, q.rope_stride, q.rope_head, c.qk_rope_head_dim);
 
   const bool expanded_ok = expanded_dims(c) && (sixteen_bit(a->kv_dtype) || a->kv_dtype == LA_DTYPE_FP8_E4M3) &&
                            device_is_gfx950() && (reinterpret_cast<uintptr_t>(a->output) & 15) == 0 &&
@@ -799,10 +807,7 @@ int prefill(const la_prefill_args* a, void* stream_v, bool run_it, size_t* need)
   void* step_ws = nullptr;
   size_t step_bytes = 0;
   bool cast_merge = false;
-  const bool q32 = a->q_dtype == LA_DTYPE_F32;
-  const bool nope_as_is = q32 && p.q.nope_head == c.qk_nope_head_dim && p.q.nope_stride == (int64_t)nh * p.q.nope_head;
-  const bool rope_as_is = q32 && !a->rotate_q && p.q.rope_head == c.qk_rope_head_dim &&
-                          p.q.rope_stride == (int64_t)nh * p.q.rope_head;
+  const bool nope_as_is = p.nope_as_is, rope_as_is = p.rope_as_is;
   auto carve = [&](void* ws) {
     Carve v(ws);
     if (p.form == kPrefillExpanded) {
