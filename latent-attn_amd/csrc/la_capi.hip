@@ -729,6 +729,18 @@ int prepare_prefill(const la_prefill_args* a, Prefill* out) {
     absorbed_ok = a->tokens * p.blocks_per_seq <= INT32_MAX &&
                   (int64_t)p.blocks_per_seq * p.block_size <= INT32_MAX;
   }
+  // The token step's plan, with aligned addresses in place of what lies in the
+  // workspace then.
+  alignas(256) static const char any[256] = {0};
+  float* const f = reinterpret_cast<float*>(const_cast<char*>(any));
+  const int32_t* const ids = reinterpret_cast<const int32_t*>(any);
+  DecodeProblem step;
+  Plan plan;
+  const auto plan_step = [&] {
+    const la_decode_args d = token_step(a, p, f, f, ids, ids, f, nullptr, 0);
+    return prepare(&d, &step, &plan) == LA_SUCCESS;
+  };
+  absorbed_ok = absorbed_ok && plan_step();
   const bool plain_ok = generic_prompt_supported(c.kv_lora_rank, c.qk_rope_head_dim);
   if (a->kernel_variant == kPrefillAbsorbed && !absorbed_ok) return LA_ERROR_NOT_SUPPORTED;
   if (a->kernel_variant == kPrefillExpanded && !expanded_ok) return LA_ERROR_NOT_SUPPORTED;
@@ -741,10 +753,20 @@ int prepare_prefill(const la_prefill_args* a, Prefill* out) {
     // per (row, head) and 320 products per pair (a query tile's worth at least).
     // Measured (absorbed / expanded, 128 heads): 1 x 16 of 1000 rows 48 / 76, 64 of
     // 1000 76 / 75, 128 of 1000 111 / 76, 128 of 8192 318 / 475, 200 of 8192 540 /
-    // 560, 16 x 16 of 2000 256 / 1900; 16 heads, 17 of 100 28 / 23.
+    // 560, 16 x 16 of 2000 256 / 1900; 16 heads, 17 of 100 28 / 23. Where the step
+    // has no matrix kernel (pages or regions that are no multiple of 32 rows, heads
+    // no multiple of 16, an unaligned cache) the VALU's takes 0.8 ns per pair and
+    // head, and the expanded form, whose gather takes any of these, is faster but
+    // for a head or two of one token (its workgroups of a head share an XCD, so
+    // fewer than 8 heads cost what 8 do): 128 heads, 16-row pages, 1 x 4 of 2000
+    // rows 780 / 109, 16 x 4 9180 / 1610, 1 x 128 of 8192 100,400 / 448; regions of
+    // 1000 rows, 1 token 122 / 64; 8 heads, 16 x 4 of 2000 848 / 126, 1 x 64 of 8192
+    // 3121 / 58, 1 token of 200 49 / 23, of 131,072 853 / 540; 1 head, 1 token of
+    // 32,768 101 / 154, of 131,072 189 / 386, 16 x 4 of 2000 144 / 137.
     const double heads = c.num_heads, seqs = a->num_seqs, n = (double)a->tokens / seqs, rows = std::max(r.region, 1);
-    const double absorbed_us = 27. + a->tokens * heads * (2e-3 + 2.3e-6 * rows);
-    const double expanded_us = 20. + 1.2 * heads * seqs * rows * (3.1e-4 + 7e-7 * std::max(n, 64.));
+    const double absorbed_us = absorbed_ok && plan.mfma ? 27. + a->tokens * heads * (2e-3 + 2.3e-6 * rows)
+                                                        : 45. + a->tokens * heads * 8e-4 * rows;
+    const double expanded_us = 20. + 1.2 * ((c.num_heads + 7) / 8 * 8) * seqs * rows * (3.1e-4 + 7e-7 * std::max(n, 64.));
     p.form = absorbed_ok && absorbed_us < expanded_us ? kPrefillAbsorbed : kPrefillExpanded;
   } else if (absorbed_ok) {
     p.form = kPrefillAbsorbed;
@@ -759,17 +781,11 @@ int prepare_prefill(const la_prefill_args* a, Prefill* out) {
     // which the rounding of its chunks can miss by little (16 x 4 tokens over 500
     // to 6000 rows: 251 chunks for 64 sequences; attention 99.5 us over the
     // regions): longer regions, whose further blocks are never read, reach it.
-    alignas(256) static const char any[256] = {0};
-    float* const f = reinterpret_cast<float*>(const_cast<char*>(any));
-    const int32_t* const ids = reinterpret_cast<const int32_t*>(any);
-    bool filled = false;
-    for (int more = 0; more < 8 && !filled && a->tokens <= cu_count() / 2; ++more) {
+    bool filled = step.chunk_len < 0;
+    for (int more = 1; more < 8 && !filled && a->tokens <= cu_count() / 2; ++more) {
       p.blocks_per_seq = p.used_blocks + more;
       if (a->tokens * p.blocks_per_seq > INT32_MAX || (int64_t)p.blocks_per_seq * p.block_size > INT32_MAX) break;
-      const la_decode_args d = token_step(a, p, f, f, ids, ids, f, nullptr, 0);
-      DecodeProblem step;
-      Plan plan;
-      filled = prepare(&d, &step, &plan) == LA_SUCCESS && step.chunk_len < 0;
+      filled = plan_step() && step.chunk_len < 0;
     }
     if (!filled) p.blocks_per_seq = p.used_blocks;
   }

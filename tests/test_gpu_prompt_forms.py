@@ -1,22 +1,99 @@
-"""Prompt and shared-prefix calls whose form and kernels the library chooses."""
+"""The form that an automatic mla_prefill call takes. A call's workspace size tells its form: each
+carves other pieces. (Sizes are counted on the host, from the descriptor alone, on the device that would run the call.)"""
 
 from __future__ import annotations
+
+import ctypes
 
 import pytest
 import torch
 
-from prompt_cases import tables, weights
+from conftest import assert_close
+from prompt_cases import Layout, as_double, reference, tables, weights
 
-from latent_attn import MLAConfig
+from latent_attn import MLAConfig, capi
 from latent_attn import functional as F
 
 pytestmark = pytest.mark.gpu
 
-ABSORBED = 3
+EXPANDED, ABSORBED = 2, 3
+AT = 1 << 20  # an aligned address that sizes are counted with and nothing reads
 
 
 def config(heads):
     return MLAConfig(5120, 512, 128, 64, heads, 128)
+
+
+def prefill_size(form, heads, batch, new, rows, block=0, kv=AT, dtype=capi.LA_DTYPE_BF16):
+    a = capi.PrefillArgs(kv_dtype=dtype, num_seqs=batch, tokens=batch * new, q_dtype=capi.LA_DTYPE_BF16, rotate_q=1,
+                         w_uk_dtype=capi.LA_DTYPE_BF16, w_uv_dtype=capi.LA_DTYPE_BF16, out_dtype=capi.LA_DTYPE_BF16,
+                         rope_rows=rows, cfg=capi.config(config(heads)), kernel_variant=form)
+    for f in ("q_nope", "q_rope", "W_UK", "W_UV", "rope_cos", "rope_sin", "output"):
+        setattr(a, f, AT)
+    a.kv_cache = kv
+    if block:
+        per = -(-rows // block)
+        a.block_table = a.seq_lens = AT
+        a.block_size, a.blocks_per_seq, a.total_rows = block, per, batch * per * block
+    else:
+        a.seq_len, a.total_rows = rows, batch * rows
+    return capi.load().la_mla_prefill_workspace_size(ctypes.byref(a))
+
+
+@pytest.mark.parametrize("case", [
+    dict(heads=128, batch=16, new=4, rows=2000, block=16),
+    dict(heads=128, batch=16, new=4, rows=2000, block=16, dtype=capi.LA_DTYPE_FP8_E4M3),
+    dict(heads=128, batch=1, new=128, rows=8192, block=16),
+    dict(heads=16, batch=16, new=4, rows=2000, block=48),
+    dict(heads=128, batch=1, new=4, rows=2000, block=1),
+    dict(heads=128, batch=4, new=16, rows=1000),
+    dict(heads=128, batch=1, new=1, rows=8200),
+    dict(heads=8, batch=16, new=4, rows=2000, block=64),
+    dict(heads=8, batch=1, new=64, rows=8192),
+    dict(heads=17, batch=1, new=8, rows=4000, block=64),
+    dict(heads=1, batch=16, new=4, rows=2000, block=64),
+    dict(heads=128, batch=16, new=4, rows=2048, block=64, kv=AT + 2),
+])
+def test_no_valu_step_beside_the_expanded_form(cuda, case):
+    """Pages, regions, heads and addresses without a matrix kernel for the absorbed form's step."""
+    auto, expanded, absorbed = (prefill_size(form, **case) for form in (0, EXPANDED, ABSORBED))
+    assert expanded != absorbed and absorbed > 0
+    assert auto == expanded
+
+
+@pytest.mark.parametrize("case", [
+    dict(heads=128, batch=16, new=4, rows=2000, block=64),
+    dict(heads=128, batch=16, new=4, rows=2000, block=32),
+    dict(heads=128, batch=1, new=4, rows=1024),
+    dict(heads=128, batch=1, new=4, rows=1024 + 32),
+    dict(heads=16, batch=16, new=4, rows=4096, block=128),
+    dict(heads=48, batch=16, new=2, rows=4096, block=64),
+    dict(heads=1, batch=1, new=1, rows=131072, block=64),  # on the VALU, which beats the expansion for one head
+])
+def test_a_few_tokens_stay_absorbed(cuda, case):
+    auto, expanded, absorbed = (prefill_size(form, **case) for form in (0, EXPANDED, ABSORBED))
+    assert expanded != absorbed and absorbed > 0
+    assert auto == absorbed
+
+
+@pytest.mark.parametrize("heads,rows,new,block", [(16, [300, 90], [3, 1], 16), (128, [200, 33], [2, 4], 48),
+                                                  (8, [700, 1], [4, 1], 64), (17, [260, 64], [4, 4], 64)])
+def test_automatic_calls(cuda, heads, rows, new, block):
+    """Such calls themselves: the expanded form's bits, and right."""
+    g = torch.Generator().manual_seed(heads)
+    data = [torch.randn(n, 576, generator=g).bfloat16().float() for n in rows]
+    layout = Layout("paged", data, torch.bfloat16, cuda, block=block)
+    q = torch.randn(sum(new), heads, 192, generator=g).bfloat16().to(cuda)
+    W_UK, W_UV = (w.to(cuda) for w in weights(heads, torch.bfloat16, 2))
+    cos, sin = (t.to(cuda) for t in tables(max(rows)))
+    off = torch.tensor([0, new[0], sum(new)], dtype=torch.int32, device=cuda)
+    run = lambda form: F.mla_prefill(layout.kv, q[..., :128], q[..., 128:], W_UK, W_UV, cos, sin, config(heads),
+                                     q_offsets=off, rotate_q=True, kernel_variant=form, **layout.kw)
+    got = run(0)
+    assert torch.equal(got, run(EXPANDED))
+    ref = reference([d.double() for d in data], as_double(q[..., :128]), as_double(q[..., 128:]), as_double(W_UK),
+                    as_double(W_UV), as_double(cos), as_double(sin), new, None, True)
+    assert_close(got.double().cpu().numpy(), ref[0].numpy(), "bf16", f"{heads} heads, pages of {block}")
 
 
 @pytest.mark.parametrize("kv", [torch.bfloat16, torch.float32])
