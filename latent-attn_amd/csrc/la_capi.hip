@@ -1076,17 +1076,39 @@ int decode_shared(const la_shared_args* a, hipStream_t stream, bool run_it, size
   // 196 / 159; 2000 rows with 8, 16, 32 51 / 59, 53 / 54, 68 / 58; 500 rows with 1,
   // 4, 16 33 / 36, 41 / 44, 41 / 39; 16 heads, 512 rows with 2 32 / 28; 8192 with
   // 1, 8, 32 36 / 39, 41 / 38, 56 / 42; 32768 with 8, 32, 100 61 / 73, 76 / 78,
-  // 157 / 110.
+  // 157 / 110. Where the latent rows have no matrix kernel (query heads of all
+  // tokens no multiple of 16, unaligned rows), always the expanded form: 8 heads, 1
+  // behind 64 rows 85 / 50, behind 32768 279 / 104; 17 heads, 2 behind 4000 225 / 84,
+  // 8 behind 32768 3480 / 151.
+  la_decode_args pre{};
+  DecodeProblem pre_step;
+  Plan pre_plan;
+  int pre_st = LA_SUCCESS;
+  if (P > 0) {
+    pre = a->own;
+    pre.kv_cache = a->prefix;
+    pre.total_rows = pre.seq_len = P;
+    pre.num_seqs = 1;
+    pre.queries_per_seq = (int32_t)tokens;
+    pre.seq_offsets = pre.seq_lens = pre.block_table = nullptr;
+    pre.block_size = pre.blocks_per_seq = 0;
+    pre.chunk_rows = pre.kernel_variant = 0;
+    pre.workspace = nullptr;
+    pre.workspace_bytes = 0;
+    pre.output = own.output;
+    pre_st = prepare(&pre, &pre_step, &pre_plan);
+  }
   const double pairs = (double)nh * P, all = pairs * tokens;
   const bool expanded =
       P > 0 && expanded_ok &&
       (a->kernel_variant == 2 ||
-       (a->kernel_variant == 0 && pairs * 512. / 5e6 < std::min(27., 5. + 4e-6 * all) + 1.75e-6 * all));
+       (a->kernel_variant == 0 && (pre_st != LA_SUCCESS || !pre_plan.mfma ||
+                                   pairs * 512. / 5e6 < std::min(27., 5. + 4e-6 * all) + 1.75e-6 * all)));
 
   PromptProblem m{};
-  la_decode_args pre{};
   size_t pre_bytes = 0;
   if (expanded) {
+    pre.num_seqs = 0;
     m.src = prefix_source(a->prefix, own.kv_dtype, P, c, a->own.rope_cos, a->own.rope_sin, a->own.rope_rows);
     m.q.q_nope = own.q_nope;
     m.q.q_rope = own.q_rope;
@@ -1108,33 +1130,21 @@ int decode_shared(const la_shared_args* a, hipStream_t stream, bool run_it, size
     m.rope_vec = q_vec(m.q.q_rope, m.q.dtype, m.q.rope_stride, m.q.rope_head);
     m.table_vec = tables_aligned(m.src);
     m.splits = key_splits(m.q_tiles * nh, m.src.num_tiles, 2);  // 2: a join follows either way
-  } else if (P > 0) {
-    pre = a->own;
-    pre.kv_cache = a->prefix;
-    pre.total_rows = pre.seq_len = P;
-    pre.num_seqs = 1;
-    pre.queries_per_seq = (int32_t)tokens;
-    pre.seq_offsets = pre.seq_lens = pre.block_table = nullptr;
-    pre.block_size = pre.blocks_per_seq = 0;
-    pre.chunk_rows = pre.kernel_variant = 0;
-    pre.workspace = nullptr;
-    pre.workspace_bytes = 0;
-    pre.output = own.output;
+  } else if (pre_st != LA_SUCCESS) {
+    return pre_st;
   }
-  // Validates both steps. One kernel merges their slots, projects and joins
+  // Validates the own rows' step. One kernel merges their slots, projects and joins
   // where the slots are the MFMA kernels'. Heads in whole blocks of 32 query rows
   // lie alike in both steps, which then share the absorbed queries (steps that
   // merge by themselves do not: their absorption zeroes the output of a half-row merge).
-  la::DecodeProblem probe;
-  Plan plan;
-  int st = prepare(&own, &probe, &plan);
+  DecodeProblem own_step;
+  Plan own_plan;
+  int st = prepare(&own, &own_step, &own_plan);
   if (st != LA_SUCCESS) return st;
-  bool one = P > 0 && merge_join_supported(probe), share = nh % 32 == 0 && plan.absorb_prep;
+  bool one = P > 0 && merge_join_supported(own_step), share = nh % 32 == 0 && own_plan.absorb_prep;
   if (pre.num_seqs > 0) {
-    st = prepare(&pre, &probe, &plan);
-    if (st != LA_SUCCESS) return st;
-    one = one && merge_join_supported(probe);
-    share = share && one && plan.absorb_prep;
+    one = one && merge_join_supported(pre_step);
+    share = share && one && pre_plan.absorb_prep;
   }
   const size_t own_bytes = la_mla_decode_workspace_size(&own);
   if (pre.num_seqs > 0) pre_bytes = la_mla_decode_workspace_size(&pre);

@@ -1,4 +1,4 @@
-"""The form that an automatic mla_prefill call takes. A call's workspace size tells its form: each
+"""The form that an automatic mla_prefill or mla_decode_shared call takes. A call's workspace size tells its form: each
 carves other pieces. (Sizes are counted on the host, from the descriptor alone, on the device that would run the call.)"""
 
 from __future__ import annotations
@@ -17,6 +17,7 @@ from latent_attn import functional as F
 pytestmark = pytest.mark.gpu
 
 EXPANDED, ABSORBED = 2, 3
+LATENT, OF_EXPANDED = 1, 2
 AT = 1 << 20  # an aligned address that sizes are counted with and nothing reads
 
 
@@ -74,6 +75,36 @@ def test_a_few_tokens_stay_absorbed(cuda, case):
     auto, expanded, absorbed = (prefill_size(form, **case) for form in (0, EXPANDED, ABSORBED))
     assert expanded != absorbed and absorbed > 0
     assert auto == absorbed
+
+
+def shared_size(form, heads, batch, prefix, at=AT):
+    a = capi.SharedArgs(prefix=at, prefix_len=prefix, expanded=AT, output=AT, out_dtype=capi.LA_DTYPE_BF16,
+                        kernel_variant=form)
+    a.own = capi.DecodeArgs(kv_dtype=capi.LA_DTYPE_BF16, num_seqs=batch, seq_len=64, total_rows=64 * batch,
+                            queries_per_seq=1, w_uk_dtype=capi.LA_DTYPE_BF16, w_uv_dtype=capi.LA_DTYPE_BF16,
+                            rope_rows=prefix + 64, cfg=capi.config(config(heads)))
+    for f in ("kv_cache", "q_nope", "q_rope", "W_UK", "W_UV", "rope_cos", "rope_sin"):
+        setattr(a.own, f, AT)
+    return capi.load().la_mla_decode_shared_workspace_size(ctypes.byref(a))
+
+
+@pytest.mark.parametrize("case", [
+    dict(heads=8, batch=1, prefix=64), dict(heads=8, batch=1, prefix=32768), dict(heads=17, batch=2, prefix=4000),
+    dict(heads=17, batch=8, prefix=32768), dict(heads=1, batch=8, prefix=32768), dict(heads=24, batch=1, prefix=32768),
+    dict(heads=128, batch=1, prefix=8192, at=AT + 2),
+])
+def test_no_valu_step_over_an_expanded_prefix(cuda, case):
+    auto, latent, expanded = (shared_size(form, **case) for form in (0, LATENT, OF_EXPANDED))
+    assert latent != expanded and latent > 0
+    assert auto == expanded
+
+
+@pytest.mark.parametrize("case", [dict(heads=128, batch=1, prefix=8192), dict(heads=8, batch=8, prefix=32768),
+                                  dict(heads=16, batch=1, prefix=8192)])
+def test_a_few_queries_read_the_latent_rows(cuda, case):
+    auto, latent, expanded = (shared_size(form, **case) for form in (0, LATENT, OF_EXPANDED))
+    assert latent != expanded and latent > 0
+    assert auto == latent
 
 
 @pytest.mark.parametrize("heads,rows,new,block", [(16, [300, 90], [3, 1], 16), (128, [200, 33], [2, 4], 48),
