@@ -712,9 +712,11 @@ int prepare_prefill(const la_prefill_args* a, Prefill* out) {
   p.nope_as_is = as_is(q.q_nope, q.nope_stride, q.nope_head, c.qk_nope_head_dim);
   p.rope_as_is = !a->rotate_q && as_is(q.q_rope, q.rope_stride, q.rope_head, c.qk_rope_head_dim);
 
+  const int64_t q_tiles = query_tiles(q, prompt_query_rows());
   const bool expanded_ok = expanded_dims(c) && (sixteen_bit(a->kv_dtype) || a->kv_dtype == LA_DTYPE_FP8_E4M3) &&
                            device_is_gfx950() && (reinterpret_cast<uintptr_t>(a->output) & 15) == 0 &&
-                           r.num_tiles <= INT32_MAX / 128;
+                           r.num_tiles <= INT32_MAX / 128 && expand_fits(r.num_tiles, q_tiles) &&
+                           q_tiles <= kMostPromptItems;
   // The absorbed form's block tables: the cache's own, or identity blocks of equal regions.
   if (paged) {
     p.block_size = a->block_size;
@@ -792,10 +794,11 @@ int prepare_prefill(const la_prefill_args* a, Prefill* out) {
   if (p.form == kPrefillExpanded) {
     const size_t head_bytes = (size_t)r.num_tiles * kTileKBytes * 2;
     p.group = (int)std::min<size_t>(c.num_heads, std::max<size_t>(1, head_bytes ? kMaxExpanded / head_bytes : c.num_heads));
-    p.q_tiles = query_tiles(q, prompt_query_rows());
+    p.q_tiles = q_tiles;
     const int64_t tiles = a->seq_offsets ? a->total_rows / a->num_seqs / kTileKeys + 1 : r.num_tiles / a->num_seqs;
     p.splits = key_splits(p.q_tiles * p.group, tiles, 1);
-    if ((int64_t)p.group * p.splits * p.q_tiles > INT32_MAX - 8) return LA_ERROR_NOT_SUPPORTED;
+    // (parts only where there are few items)
+    p.group = (int)std::min<int64_t>(p.group, kMostPromptItems / (p.splits * p.q_tiles));
   }
   *out = p;
   return LA_SUCCESS;
@@ -1007,6 +1010,7 @@ int expand(const la_expand_args* a, hipStream_t stream, bool run_it, size_t* nee
   if (!a->kv_cache || !a->W_UK || !a->W_UV || !a->rope_cos || !a->rope_sin) return LA_ERROR_INVALID_VALUE;
   ExpandPlan e;
   e.p.src = prefix_source(a->kv_cache, a->kv_dtype, a->rows, a->cfg, a->rope_cos, a->rope_sin, a->rope_rows);
+  if (!expand_fits(e.p.src.num_tiles, 0)) return LA_ERROR_NOT_SUPPORTED;
   e.p.f16 = a->kv_dtype == LA_DTYPE_F16;
   auto carve = [&](void* ws) {
     Carve v(ws);
@@ -1130,6 +1134,7 @@ int decode_shared(const la_shared_args* a, hipStream_t stream, bool run_it, size
     m.rope_vec = q_vec(m.q.q_rope, m.q.dtype, m.q.rope_stride, m.q.rope_head);
     m.table_vec = tables_aligned(m.src);
     m.splits = key_splits(m.q_tiles * nh, m.src.num_tiles, 2);  // 2: a join follows either way
+    if (m.q_tiles * nh * m.splits > kMostPromptItems) return LA_ERROR_NOT_SUPPORTED;
   } else if (pre_st != LA_SUCCESS) {
     return pre_st;
   }

@@ -373,7 +373,7 @@ hipError_t expand_pb(const ExpandProblem& p, hipStream_t stream, int ncu) {
   if (e != hipSuccess) return e;
   int64_t per_xcd = items_per_xcd(p.heads, p.src.num_tiles, kPb);
   if (kPb == 4) per_xcd = per_xcd < (ncu + 7) / 8 ? per_xcd : (ncu + 7) / 8;
-  if (8 * per_xcd > INT32_MAX) return hipErrorInvalidValue;
+  if (8 * per_xcd > most_blocks(512)) return hipErrorInvalidValue;
   hipLaunchKernelGGL((expand_kernel<T, kPb>), dim3((unsigned)(8 * per_xcd)), dim3(512), lds, stream, p, per_xcd);
   return hipGetLastError();
 }
@@ -490,7 +490,7 @@ hipError_t gather_expand_t(const ExpandProblem& p, bool aligned, hipStream_t str
   const int64_t items = 8 * (int64_t)((p.heads + 7) / 8) * p.src.num_tiles;
   const int64_t pieces = p.src.num_tiles * kGatherParts + (p.q_tiles + 255) / 256;
   const int64_t blocks = items + (pieces + 1) / 2;
-  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  if (blocks > most_blocks(512)) return hipErrorInvalidValue;
   if (aligned)
     hipLaunchKernelGGL((gather_expand_kernel<KT, T, true>), dim3((unsigned)blocks), dim3(512), kSmallLds, stream, p, items);
   else
@@ -498,9 +498,11 @@ hipError_t gather_expand_t(const ExpandProblem& p, bool aligned, hipStream_t str
   return hipGetLastError();
 }
 
+int64_t gather_blocks(int64_t tiles, int64_t q_tiles) { return tiles * kGatherParts + (q_tiles + 255) / 256; }
+
 template <typename KT, typename T>
 hipError_t gather_t(const ExpandProblem& p, bool aligned, hipStream_t stream) {
-  const dim3 grid((unsigned)(p.src.num_tiles * kGatherParts + (p.q_tiles + 255) / 256));
+  const dim3 grid((unsigned)gather_blocks(p.src.num_tiles, p.q_tiles));
   if (aligned) hipLaunchKernelGGL((gather_kernel<KT, T, true>), grid, dim3(256), 0, stream, p);
   else hipLaunchKernelGGL((gather_kernel<KT, T, false>), grid, dim3(256), 0, stream, p);
   return hipGetLastError();
@@ -516,9 +518,11 @@ bool small_call(const ExpandProblem& p, int ncu) {
 
 }  // namespace
 
+bool expand_fits(int64_t tiles, int64_t q_tiles) { return gather_blocks(tiles, q_tiles) <= most_blocks(256); }
+
 hipError_t launch_gather(const ExpandProblem& p, hipStream_t stream, int ncu) {
   if (small_call(p, ncu) || (p.src.num_tiles == 0 && p.q_tiles == 0)) return hipSuccess;
-  if (p.src.num_tiles > INT32_MAX / 8 || p.q_tiles > INT32_MAX || p.src.row_elems != 576) return hipErrorInvalidValue;
+  if (!expand_fits(p.src.num_tiles, p.q_tiles) || p.src.row_elems != 576) return hipErrorInvalidValue;
   const bool aligned = (reinterpret_cast<uintptr_t>(p.src.kv) & 15) == 0;  // rows are 1152 or 576 B
   switch (p.src.kv_dtype) {
     case LA_DTYPE_BF16: return gather_t<__hip_bfloat16, __hip_bfloat16>(p, aligned, stream);
@@ -531,7 +535,7 @@ hipError_t launch_gather(const ExpandProblem& p, hipStream_t stream, int ncu) {
 hipError_t launch_expand(const ExpandProblem& p, hipStream_t stream, int ncu) {
   if (p.src.num_tiles == 0 || p.heads == 0) return hipSuccess;
   if (small_call(p, ncu)) {
-    if (p.src.num_tiles > INT32_MAX / 8 || p.q_tiles > INT32_MAX || p.src.row_elems != 576) return hipErrorInvalidValue;
+    if (!expand_fits(p.src.num_tiles, p.q_tiles) || p.src.row_elems != 576) return hipErrorInvalidValue;
     const bool aligned = (reinterpret_cast<uintptr_t>(p.src.kv) & 15) == 0;
     switch (p.src.kv_dtype) {
       case LA_DTYPE_BF16: return gather_expand_t<__hip_bfloat16, __hip_bfloat16>(p, aligned, stream);

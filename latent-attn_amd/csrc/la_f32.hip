@@ -350,11 +350,11 @@ bool absorb_f32_supported(const void* q_nope, const void* W, int w_dtype, const 
 
 hipError_t launch_absorb_f32(const float* q_nope, const void* W, float* q_abs, int tokens, int nh, int dn, int dc,
                              hipStream_t stream) {
-  const dim3 grid((unsigned)((nh * (dc / 64) + 3) / 4), (unsigned)((tokens + 15) / 16));
   auto k = dn == 128 ? absorb_f32_kernel<8> : absorb_f32_kernel<0>;
-  hipLaunchKernelGGL(k, grid, dim3(256), 0, stream, q_nope, reinterpret_cast<const float*>(W), q_abs,
-                     tokens, nh, dn, dc);
-  return hipGetLastError();
+  return in_grids(tokens, kMostBlocksYZ * 16, [&](int64_t t, unsigned n) {
+    hipLaunchKernelGGL(k, dim3((unsigned)((nh * (dc / 64) + 3) / 4), (n + 15) / 16), dim3(256), 0, stream,
+                       q_nope + t * nh * dn, reinterpret_cast<const float*>(W), q_abs + t * nh * dc, (int)n, nh, dn, dc);
+  });
 }
 
 }  // namespace la

@@ -23,14 +23,14 @@ namespace {
 constexpr int kGenericThreads = 256;  // 4 waves
 constexpr int kGenericWaves = kGenericThreads / 64;
 
-// Grid (num_chunks, Hq). Each block walks the segments of its chunk for one
-// query head; wave w takes rows lo+w, lo+w+4, ...; lane owns latent columns
+// Grid (num_chunks, heads from hq0 on). Each block walks the segments of its chunk
+// for one query head; wave w takes rows lo+w, lo+w+4, ...; lane owns latent columns
 // lane + 64*j. Per segment the four waves' (max, sum, acc) are merged in LDS
 // and written as one partial slot.
 template <typename KT, int NC>
-__global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(DecodeProblem p) {
+__global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(DecodeProblem p, int hq0) {
   const int chunk = blockIdx.x;
-  const int hq = blockIdx.y;
+  const int hq = hq0 + blockIdx.y;
   const int tid = threadIdx.x;
   const int wave = tid >> 6, lane = tid & 63;
   const int dc = p.dc, dR = p.dR, half = dR >> 1;
@@ -139,19 +139,20 @@ __global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(DecodeP
 
 template <typename KT>
 hipError_t launch_generic_t(const DecodeProblem& p, hipStream_t stream) {
-  dim3 grid(p.num_chunks, p.Hq);
   const size_t smem = sizeof(float) * (p.dc + p.dR + kGenericWaves * (p.dc + 2));
   const int nc = (p.dc + 63) / 64;
-  if (nc <= 1) hipLaunchKernelGGL((decode_generic_kernel<KT, 1>), grid, dim3(kGenericThreads), smem, stream, p);
-  else if (nc <= 2) hipLaunchKernelGGL((decode_generic_kernel<KT, 2>), grid, dim3(kGenericThreads), smem, stream, p);
-  else if (nc <= 4) hipLaunchKernelGGL((decode_generic_kernel<KT, 4>), grid, dim3(kGenericThreads), smem, stream, p);
-  else if (nc <= 8) hipLaunchKernelGGL((decode_generic_kernel<KT, 8>), grid, dim3(kGenericThreads), smem, stream, p);
-  else hipLaunchKernelGGL((decode_generic_kernel<KT, 16>), grid, dim3(kGenericThreads), smem, stream, p);
-  return hipGetLastError();
+  const auto k = nc <= 1   ? decode_generic_kernel<KT, 1>
+                 : nc <= 2 ? decode_generic_kernel<KT, 2>
+                 : nc <= 4 ? decode_generic_kernel<KT, 4>
+                 : nc <= 8 ? decode_generic_kernel<KT, 8>
+                           : decode_generic_kernel<KT, 16>;
+  return in_grids(p.Hq, kMostBlocksYZ, [&](int64_t h, unsigned n) {
+    hipLaunchKernelGGL(k, dim3(p.num_chunks, n), dim3(kGenericThreads), smem, stream, p, (int)h);
+  });
 }
 
 // ---------------------------------------------------------------------------
-// Combine + projection. Grid (nh, ceil(R / kRowsPerBlock)) with
+// Combine + projection. Grid (nh, blocks of kRowsPerBlock tokens from rb0 on) of
 // R = num_seqs * qps query tokens; block (h, rb) handles tokens
 // [rb*kRowsPerBlock, ...) for weight head h, so W_UV[h] is read once per
 // block. Token r lives in sequence s = r / qps with query head
@@ -160,9 +161,9 @@ hipError_t launch_generic_t(const DecodeProblem& p, hipStream_t stream) {
 constexpr int kRowsPerBlock = 8;
 constexpr int kCombineThreads = 256;
 
-__global__ __launch_bounds__(kCombineThreads) void combine_project_kernel(DecodeProblem p) {
+__global__ __launch_bounds__(kCombineThreads) void combine_project_kernel(DecodeProblem p, int rb0) {
   const int h = blockIdx.x;
-  const int r0 = blockIdx.y * kRowsPerBlock;
+  const int r0 = (rb0 + (int)blockIdx.y) * kRowsPerBlock;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int dc = p.dc, dv = p.dv;
   const int R = p.num_seqs * p.qps;
@@ -220,7 +221,7 @@ __global__ __launch_bounds__(kCombineThreads) void combine_project_kernel(Decode
 }
 
 // ---------------------------------------------------------------------------
-// Absorption. Grid (nh, ceil(dc/256), ceil(tokens/kAbsTok)); thread = latent
+// Absorption. Grid (nh, ceil(dc/256), blocks of kAbsTok tokens); thread = latent
 // column c, so W_UK rows are read coalesced and once per token block.
 // ---------------------------------------------------------------------------
 constexpr int kAbsTok = 16;
@@ -274,18 +275,20 @@ hipError_t launch_decode_generic(const DecodeProblem& p, hipStream_t stream) {
 
 hipError_t launch_combine_project(const DecodeProblem& p, hipStream_t stream) {
   const int R = p.num_seqs * p.qps;
-  dim3 grid(p.nh, (R + kRowsPerBlock - 1) / kRowsPerBlock);
+  const int64_t blocks = ((int64_t)R + kRowsPerBlock - 1) / kRowsPerBlock;
   const size_t smem = sizeof(float) * kRowsPerBlock * p.dc;
-  hipLaunchKernelGGL(combine_project_kernel, grid, dim3(kCombineThreads), smem, stream, p);
-  return hipGetLastError();
+  return in_grids(blocks, kMostBlocksYZ, [&](int64_t b, unsigned n) {
+    hipLaunchKernelGGL(combine_project_kernel, dim3(p.nh, n), dim3(kCombineThreads), smem, stream, p, (int)b);
+  });
 }
 
 hipError_t launch_absorb(const float* q_nope, const void* W_UK, int w_dtype, float* q_abs, int tokens, int nh, int dn,
                          int dc, hipStream_t stream) {
-  dim3 grid(nh, (dc + 255) / 256, (tokens + kAbsTok - 1) / kAbsTok);
   const size_t smem = sizeof(float) * kAbsTok * dn;
-  hipLaunchKernelGGL(absorb_kernel, grid, dim3(256), smem, stream, q_nope, W_UK, w_dtype, q_abs, tokens, nh, dn, dc);
-  return hipGetLastError();
+  return in_grids(tokens, kMostBlocksYZ * kAbsTok, [&](int64_t t, unsigned n) {
+    hipLaunchKernelGGL(absorb_kernel, dim3(nh, (dc + 255) / 256, (n + kAbsTok - 1) / kAbsTok), dim3(256), smem, stream,
+                       q_nope + t * nh * dn, W_UK, w_dtype, q_abs + t * nh * dc, (int)n, nh, dn, dc);
+  });
 }
 
 }  // namespace la

@@ -560,6 +560,21 @@ inline hipError_t allow_lds(OncePerDevice& once, const void* fn, int bytes) {
 // Whether the current device runs the MFMA kernels.
 bool device_is_gfx950();
 
+// Workgroups of a launch: a grid dimension holds fewer than 2^32 threads, and y
+// and z at most 65,536 workgroups.
+constexpr int64_t most_blocks(int threads) { return (int64_t)UINT32_MAX / threads; }
+constexpr int kMostBlocksYZ = 65535;
+// Calls launch(first, n) for pieces of `blocks`, `most` at a time.
+template <typename Launch>
+hipError_t in_grids(int64_t blocks, int64_t most, Launch launch) {
+  hipError_t e = hipSuccess;
+  for (int64_t first = 0; first < blocks && e == hipSuccess; first += most) {
+    launch(first, (unsigned)(blocks - first < most ? blocks - first : most));
+    e = hipGetLastError();
+  }
+  return e;
+}
+
 // fp32 split-KV decode and absorption on the fp32 MFMA (la_f32.hip): float32
 // caches with kv_lora_rank 512, qk_rope_head_dim 64; float32 weights. zero_out
 // (optional): zero_n floats the attention kernel zeroes for a half-row merge.

@@ -44,8 +44,8 @@ __device__ inline float step_lse(const DecodeProblem& p, int64_t row, int l32) {
 // out before the log-sum-exps are known: those take several dependent loads,
 // which are most of the kernel's time.
 template <bool kVec>
-__global__ __launch_bounds__(256) void join_kernel(JoinProblem p) {
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+__global__ __launch_bounds__(256) void join_kernel(JoinProblem p, int64_t block0) {
+  const int64_t row = (block0 + blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int l32 = threadIdx.x & 31;
   if (row >= p.rows) return;
   constexpr int kN = kVec ? 4 : 1;
@@ -101,12 +101,11 @@ __global__ __launch_bounds__(256) void join_kernel(JoinProblem p) {
 }  // namespace
 
 hipError_t launch_join(const JoinProblem& p, hipStream_t stream) {
-  if (p.rows == 0) return hipSuccess;
-  const int64_t blocks = (p.rows + 7) / 8;
-  if (blocks > INT32_MAX || p.splits > kJoinSplits) return hipErrorInvalidValue;
-  if (p.dv % 4 == 0) hipLaunchKernelGGL(join_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL(join_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
-  return hipGetLastError();
+  if (p.splits > kJoinSplits) return hipErrorInvalidValue;
+  const auto k = p.dv % 4 == 0 ? join_kernel<true> : join_kernel<false>;
+  return in_grids((p.rows + 7) / 8, most_blocks(256), [&](int64_t first, unsigned blocks) {
+    hipLaunchKernelGGL(k, dim3(blocks), dim3(256), 0, stream, p, first);
+  });
 }
 
 }  // namespace la

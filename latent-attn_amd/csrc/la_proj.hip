@@ -1039,6 +1039,14 @@ hipError_t launch_absorb_mfma(const float* q_nope, const void* W_UK, int w_dtype
   // one block per (token block, head, column block), ordered for the XCDs:
   // groups of (token block, 8 heads) with 8 * (dc / 128) blocks each
   const int64_t groups = (int64_t)((tokens + 31) / 32) * ((nh + 7) / 8);
+  if (64 * (dc / kAbsCols) * ((groups + 7) / 8) > most_blocks(kAbsThreads)) {
+    if (out_mode != 0 || tokens <= 32) return hipErrorInvalidValue;
+    const int half = tokens / 64 * 32;  // plain rows: two launches
+    const hipError_t e = launch_absorb_mfma(q_nope, W_UK, w_dtype, out, 0, nullptr, 1.f, 0, half, nh, dn, dc, 1, stream, nullptr, 0);
+    if (e != hipSuccess) return e;
+    return launch_absorb_mfma(q_nope + (int64_t)half * nh * dn, W_UK, w_dtype, static_cast<float*>(out) + (int64_t)half * nh * dc,
+                              0, nullptr, 1.f, 0, tokens - half, nh, dn, dc, 1, stream, nullptr, 0);
+  }
   dim3 grid((unsigned)(8 * 8 * (dc / kAbsCols) * ((groups + 7) / 8)));
   const bool d128 = dn == 128;
   if (w_dtype == LA_DTYPE_BF16) {
@@ -1161,7 +1169,7 @@ hipError_t launch_merge_join(const JoinProblem& j, hipStream_t stream, int ncu) 
   int rpb_log2 = 4;
   while (rpb_log2 > 0 && (int64_t)hb * ((R + (1 << rpb_log2) - 1) >> rpb_log2) < ncu) --rpb_log2;
   const int64_t blocks = (int64_t)hb * ((R + (1 << rpb_log2) - 1) >> rpb_log2);
-  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  if (blocks > most_blocks(kMPWaves * 64)) return hipErrorInvalidValue;
   if (p.wuv_dtype == LA_DTYPE_BF16)
     hipLaunchKernelGGL(merge_join_kernel<__hip_bfloat16>, dim3((unsigned)blocks), dim3(kMPWaves * 64), 0, stream, j, rpb_log2);
   else

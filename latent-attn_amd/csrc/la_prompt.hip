@@ -447,26 +447,27 @@ hipError_t prompt_t(const PromptProblem& p, hipStream_t stream) {
   const hipError_t e = allow_lds(once, reinterpret_cast<const void*>(prompt_kernel<T>), lds);
   if (e != hipSuccess) return e;
   const int64_t items = (int64_t)p.heads * p.splits * p.q_tiles;
-  if (items > INT32_MAX - 8) return hipErrorInvalidValue;
+  if (items > kMostPromptItems) return hipErrorInvalidValue;
   hipLaunchKernelGGL(prompt_kernel<T>, dim3((unsigned)(8 * ((items + 7) / 8))), dim3(256), lds, stream, p);
   return hipGetLastError();
 }
 
 // ---- the plain form: any type and head shape ------------------------------------------------------
 
-// One workgroup of 4 waves per (token, head) over absorbed fp32 queries: wave w
+// One workgroup of 4 waves per (token, head), from number first on, over absorbed fp32 queries: wave w
 // takes rows w, w + 4, ... with a running maximum of its own, lanes share a
 // row's elements; the waves' sums are joined and projected by W_UV. Everything
 // fp32. Rows come from L2 once per head and token, which bounds it; it is there
 // for shapes and types that the others do not take.
 constexpr int kGenericLatent = 1024;  // kv_lora_rank at most: 16 elements per lane
 constexpr int kGenericRope = 256;
-__global__ __launch_bounds__(256) void generic_prompt_kernel(GenericPrompt p) {
+__global__ __launch_bounds__(256) void generic_prompt_kernel(GenericPrompt p, int64_t first) {
   __shared__ float q_l[kGenericRope];
   __shared__ float acc_l[4][kGenericLatent];
   __shared__ float ml[4][2];
-  const int64_t token = blockIdx.x / p.nh;
-  const int h = (int)(blockIdx.x % p.nh);
+  const uint32_t item = (uint32_t)first + blockIdx.x;  // (tokens x heads stay below 2^31)
+  const int64_t token = item / p.nh;
+  const int h = (int)(item % p.nh);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int s = query_seq(p.q, token);
   const int n = query_count(p.q, s);
@@ -547,7 +548,7 @@ __global__ __launch_bounds__(256) void generic_prompt_kernel(GenericPrompt p) {
 // ---- queries of the absorbed forms ------------------------------------------------------------------
 
 // kTokenElems elements of a token's nope queries, and as many pairs of rope
-// ones, per workgroup (x: token, y: share), four at a time where heads and
+// ones, per workgroup (x: token from number token0 on, y: share), four at a time where heads and
 // strides are whole vectors; the first also writes its length and table.
 constexpr int kTokenElems = 2048;
 template <int kN>
@@ -556,8 +557,8 @@ __device__ inline void load_n(const void* base, int dtype, int64_t i, float (&x)
   else x[0] = load_any(base, dtype, i);
 }
 template <int kN>
-__global__ __launch_bounds__(256) void tokens_kernel(TokenProblem p) {
-  const int64_t token = blockIdx.x;
+__global__ __launch_bounds__(256) void tokens_kernel(TokenProblem p, int64_t token0) {
+  const int64_t token = token0 + blockIdx.x;
   const int s = query_seq(p.q, token);
   const int n = query_count(p.q, s);
   const int64_t j = token - query_begin(p.q, s);
@@ -620,23 +621,21 @@ hipError_t launch_prompt(const PromptProblem& p, hipStream_t stream) {
 bool generic_prompt_supported(int dc, int dR) { return dc <= kGenericLatent && dR <= kGenericRope; }
 
 hipError_t launch_generic_prompt(const GenericPrompt& p, hipStream_t stream) {
-  const int64_t blocks = p.q.tokens * p.nh;
-  if (blocks == 0) return hipSuccess;
-  if (blocks > INT32_MAX) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(generic_prompt_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p);
-  return hipGetLastError();
+  const int64_t items = p.q.tokens * p.nh;
+  if (items > INT32_MAX) return hipErrorInvalidValue;
+  return in_grids(items, most_blocks(256), [&](int64_t first, unsigned blocks) {
+    hipLaunchKernelGGL(generic_prompt_kernel, dim3(blocks), dim3(256), 0, stream, p, first);
+  });
 }
 
 hipError_t launch_tokens(const TokenProblem& p, hipStream_t stream) {
-  if (p.q.tokens == 0) return hipSuccess;
-  if (p.q.tokens > INT32_MAX) return hipErrorInvalidValue;
   const int elems = p.nh * (p.dn > p.dR / 2 ? p.dn : p.dR / 2);
   const unsigned shares = (unsigned)((elems + kTokenElems - 1) / kTokenElems);
-  if (shares > 65535) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)p.q.tokens, shares);
-  if (p.vec && p.dn % 4 == 0 && p.dR % 8 == 0) hipLaunchKernelGGL(tokens_kernel<4>, grid, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL(tokens_kernel<1>, grid, dim3(256), 0, stream, p);
-  return hipGetLastError();
+  if (shares > kMostBlocksYZ) return hipErrorInvalidValue;
+  const auto k = p.vec && p.dn % 4 == 0 && p.dR % 8 == 0 ? tokens_kernel<4> : tokens_kernel<1>;
+  return in_grids(p.q.tokens, most_blocks(256), [&](int64_t first, unsigned blocks) {
+    hipLaunchKernelGGL(k, dim3(blocks, shares), dim3(256), 0, stream, p, first);
+  });
 }
 
 hipError_t launch_cast(const float* src, void* dst, int out_dtype, int64_t n, hipStream_t stream) {

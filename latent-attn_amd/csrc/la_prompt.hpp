@@ -227,6 +227,7 @@ struct ExpandProblem {
   float k_scale;  // times K and the rope keys
   int head0, heads;
 };
+bool expand_fits(int64_t tiles, int64_t q_tiles);  // one launch of the gather takes them
 hipError_t launch_gather(const ExpandProblem& p, hipStream_t stream, int ncu);
 hipError_t launch_expand(const ExpandProblem& p, hipStream_t stream, int ncu);
 // 16-bit copy of n weights of another type.
@@ -254,6 +255,8 @@ struct PromptProblem {
   int q_wide;  // 16-bit queries: 16-byte aligned
 };
 int prompt_query_rows();  // query tokens per workgroup
+// Most items (query tile, head, key part) of a launch.
+constexpr int64_t kMostPromptItems = most_blocks(256) - 8;
 hipError_t launch_prompt(const PromptProblem& p, hipStream_t stream);
 
 // Joins partial results of the same (token, head) rows by their log-sum-exps.

@@ -147,3 +147,80 @@ def test_queries_at_any_address(cuda, kv):
 
     for a, b in ((moved(q_nope), q_rope), (q_nope, moved(q_rope)), (moved(q_nope), moved(q_rope))):
         assert torch.equal(run(a, b), want)
+
+
+def small_reference(rows, q, W_UK, W_UV, heads, dn, dv):
+    """One sequence's causal attention from the definition, float64, without rotation; q (n, heads, dn + dR), the last n
+    rows' queries."""
+    dc = W_UK.shape[1]
+    c, r = rows[:, :dc].double(), rows[:, dc:].double()
+    K = (c @ W_UK.double().T).view(-1, heads, dn)
+    V = (c @ W_UV.double().T).view(-1, heads, dv)
+    q = q.double()
+    x = torch.matmul(q[..., :dn].transpose(0, 1), K.permute(1, 2, 0).contiguous())
+    x = x + torch.matmul(q[..., dn:].transpose(0, 1), r.T.contiguous())
+    x /= (q.shape[2]) ** 0.5
+    n, L = q.shape[0], rows.shape[0]
+    x = x.masked_fill(torch.arange(L, device=x.device) > torch.arange(L - n, L, device=x.device)[:, None], -float("inf"))
+    return torch.matmul(torch.softmax(x, -1), V.transpose(0, 1).contiguous()).transpose(0, 1)
+
+
+def unrotated(rows, d_r, device):
+    return torch.ones(rows, d_r // 2, device=device), torch.zeros(rows, d_r // 2, device=device)
+
+
+# float32 throughout. A score sums at most dc + dn + dR = 88 rounded products, whose magnitudes here add up to less than
+# 60 (after the scale), so it is off by at most 88 x 2^-24 x 60 = 3.2e-4, a weight by a factor within 1 +- 6.4e-4, and an
+# output by that of sum w |V| < 6: 3.9e-3. (V's own sums of 64 products add 64 x 2^-24 x 10 = 4e-5.)
+CLOSE = 4e-3
+
+
+@pytest.mark.parametrize("heads,tokens,dims,doc", [
+    (128, 1 << 17, (16, 8, 8, 8), 64),     # 2^24 workgroups of 256 threads: one more than a grid holds
+    (1, (1 << 20) + 640, (16, 8, 8, 8), 64),  # absorption in blocks of 16 tokens: more than 65,535 of them
+    (1, (1 << 20) + 640, (64, 16, 8, 8), 64),  # ... on the matrix cores
+])
+def test_plain_calls_past_one_grid(cuda, heads, tokens, dims, doc):
+    dc, dn, d_r, dv = dims
+    cfg = MLAConfig(64, dc, dn, d_r, heads, dv)
+    g = torch.Generator(device=cuda).manual_seed(1)
+    kv = torch.randn(tokens, dc + d_r, generator=g, device=cuda)
+    W_UK, W_UV = (torch.randn(heads * d, dc, generator=g, device=cuda) / dc ** 0.5 for d in (dn, dv))
+    q = torch.randn(tokens, heads, dn + d_r, generator=g, device=cuda)
+    off = torch.arange(0, tokens + 1, doc, device=cuda).int()
+    cos, sin = unrotated(doc, d_r, cuda)
+    got = F.mla_prefill(kv, q[..., :dn], q[..., dn:], W_UK, W_UV, cos, sin, cfg, q_offsets=off, seq_offsets=off,
+                        kernel_variant=1)
+    for at in (0, tokens // doc // 2 * doc, tokens - doc):
+        ref = small_reference(kv[at:at + doc], q[at:at + doc], W_UK, W_UV, heads, dn, dv)
+        assert (got[at:at + doc].double() - ref).abs().max() <= CLOSE, at
+
+
+def test_an_absorbed_call_past_one_grid(cuda):
+    """600,000 tokens' projections in blocks of 8: more than 65,535 of them."""
+    B, n, cap, (dc, dn, d_r, dv) = 10000, 60, 64, (16, 8, 8, 8)
+    cfg = MLAConfig(64, dc, dn, d_r, 1, dv)
+    g = torch.Generator(device=cuda).manual_seed(2)
+    kv = torch.randn(B, cap, dc + d_r, generator=g, device=cuda)
+    W_UK, W_UV = (torch.randn(d, dc, generator=g, device=cuda) / dc ** 0.5 for d in (dn, dv))
+    q = torch.randn(B * n, 1, dn + d_r, generator=g, device=cuda)
+    cos, sin = unrotated(cap, d_r, cuda)
+    got = F.mla_prefill(kv, q[..., :dn], q[..., dn:], W_UK, W_UV, cos, sin, cfg, kernel_variant=ABSORBED)
+    for b in (0, 8737, 8738, B - 1):
+        ref = small_reference(kv[b], q[b * n:(b + 1) * n], W_UK, W_UV, 1, dn, dv)
+        assert (got[b * n:(b + 1) * n].double() - ref).abs().max() <= CLOSE, b
+
+
+def test_a_shared_step_past_one_grid(cuda):
+    """The prefix's step has batch x heads query heads: 76,800 where a grid's y holds 65,535."""
+    B, heads, P, own, (dc, dn, d_r, dv) = 600, 128, 70, 5, (16, 8, 8, 8)
+    cfg = MLAConfig(64, dc, dn, d_r, heads, dv)
+    g = torch.Generator(device=cuda).manual_seed(3)
+    front, kv = torch.randn(P, dc + d_r, generator=g, device=cuda), torch.randn(B, own, dc + d_r, generator=g, device=cuda)
+    W_UK, W_UV = (torch.randn(heads * d, dc, generator=g, device=cuda) / dc ** 0.5 for d in (dn, dv))
+    q_nope, q_rope = (torch.randn(B, heads, d, generator=g, device=cuda) for d in (dn, d_r))
+    cos, sin = unrotated(P + own, d_r, cuda)
+    got = F.mla_decode_shared(front, kv, q_nope, q_rope, W_UK, W_UV, cos, sin, cfg)
+    for b in (0, 511, 512, B - 1):
+        ref = small_reference(torch.cat([front, kv[b]]), torch.cat([q_nope, q_rope], -1)[b:b + 1], W_UK, W_UV, heads, dn, dv)
+        assert (got[b:b + 1].double() - ref).abs().max() <= CLOSE, b
