@@ -275,7 +275,8 @@ typedef struct la_prefill_args {
    * every token a sequence of a paged decode step. LA_ERROR_NOT_SUPPORTED
    * where the form has no kernel for these arguments. Form 2 holds keys,
    * values and queries in 16 bits: bf16, or fp16 for an F16 cache, whose
-   * range they then have to keep to. */
+   * range they then have to keep to: tokens that see a row past it get NaN
+   * or infinities, the others are left as they are. */
   int32_t kernel_variant;
 } la_prefill_args;
 

@@ -8,6 +8,8 @@
 // the matrix instructions of the attention take them.
 #include "la_prompt.hpp"
 
+#include <type_traits>
+
 namespace la {
 namespace {
 
@@ -34,6 +36,32 @@ struct Mm<__half> {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
 };
+
+// Values past fp16's range. A weight of zero times infinity is NaN, so an
+// infinite value would reach the tokens that do not see its row. It becomes the
+// largest number, and over(row of the block) is called by a lane that holds one,
+// for a NaN in the row's key: that reaches the tokens that see it, through their
+// scores. (bf16 has fp32's range, whose end no other form passes either.)
+constexpr float kHalfMost = 65504.f, kHalfOver = 65520.f;  // from kHalfOver on fp16 rounds to infinity
+template <int kBlocks>
+__device__ inline bool past_half(const f32x16 (&v)[kBlocks]) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; e += 2)
+      asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(top) : "v"(top), "v"(v[i][e]), "v"(v[i][e + 1]));
+  return __builtin_amdgcn_ballot_w64(top >= kHalfOver) != 0;
+}
+template <typename Over>
+__device__ inline void hold_half(f32x16& v, int g, Over over) {  // a block of 32 rows: 8 (e / 4) + 4 g + e % 4 in register e
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (fabsf(v[e]) >= kHalfOver) {
+      v[e] = copysignf(kHalfMost, v[e]);
+      over(8 * (e >> 2) + 4 * g + (e & 3));
+    }
+}
 
 // ---- gather --------------------------------------------------------------------
 
@@ -330,6 +358,19 @@ __device__ inline void expand_wave(const ExpandProblem& p, int64_t step, lchar* 
     for (int i = 0; i < kPb; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) settle(acc[i][j]);
+    if constexpr (kV && std::is_same<T, __half>::value) {
+#pragma unroll
+      for (int i = 0; i < kPb; ++i) {
+        const int pb = kPb * wp + i;
+        const int64_t tile = out_tile + pb / 2;
+        if (tile < p.src.num_tiles && past_half(acc[i])) {
+          _Float16* const rope = static_cast<_Float16*>(p.rope) + tile * (kTileRBytes / 2) + (pb & 1) * (4 * 512);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            hold_half(acc[i][j], g, [&](int row) { rope[operand_elem(row, 0)] = (_Float16)__builtin_nanf(""); });
+        }
+      }
+    }
     // registers 8 q .. 8 q + 7 of a block are one operand element group (operand
     // order, la_prompt.hpp): K: a step of 16 dims; V: of 16 keys
 #pragma unroll
@@ -430,10 +471,18 @@ __device__ inline void small_products(const ExpandProblem& p, lchar* L, int64_t 
       for (int j = 0; j < 2; ++j) acc[j] = kV ? Mm<T>::mma(x, w[j], acc[j]) : Mm<T>::mma(w[j], x, acc[j]);
     }
   }
-  char* const out = static_cast<char*>(kV ? p.vx : p.kx) + ((int64_t)h * p.src.num_tiles + tile) * kTileKBytes;
+  const int64_t at = ((int64_t)h * p.src.num_tiles + tile) * kTileKBytes;
+  char* const out = static_cast<char*>(kV ? p.vx : p.kx) + at;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) settle(acc[j]);
+  uint32_t over = 0;  // fp16: this lane's rows of the block with a value past the range
+  if constexpr (kV && std::is_same<T, __half>::value) {
+    if (past_half(acc))
+#pragma unroll
+      for (int j = 0; j < 2; ++j) hold_half(acc[j], g, [&](int row) { over |= 1u << row; });
+  }
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    settle(acc[j]);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       vec v;
@@ -443,6 +492,12 @@ __device__ inline void small_products(const ExpandProblem& p, lchar* L, int64_t 
       const int piece = kV ? 4 * db + 2 * wp + q : 8 * wp + 2 * db + q;
       *reinterpret_cast<vec*>(out + piece * 1024 + 16 * lane) = v;
     }
+  }
+  if constexpr (std::is_same<T, __half>::value) {
+    // the rope keys are other workgroups', so a NaN goes into this head's key, behind the stores of the keys
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    _Float16* const key = reinterpret_cast<_Float16*>(static_cast<char*>(p.kx) + at) + wp * (8 * 512);
+    for (; over; over &= over - 1) key[operand_elem(__builtin_ctz(over), 0)] = (_Float16)__builtin_nanf("");
   }
 }
 
