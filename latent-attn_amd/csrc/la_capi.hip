@@ -552,11 +552,6 @@ int status_of(hipError_t e) { return e == hipSuccess ? (int)LA_SUCCESS : record_
 
 // Weights as the expanded form's products take them: 16-bit values of its
 // type, from 16-byte aligned rows; others are copied first.
-struct ExpandWeights {
-  const void* w;
-  int dtype;
-  void* copy;
-};
 bool weight_as_is(const void* w, int dtype, int f16) {
   return dtype == (f16 ? LA_DTYPE_F16 : LA_DTYPE_BF16) && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
 }
