@@ -213,9 +213,9 @@ __global__ __launch_bounds__(256) void convert_kernel(const void* src, int src_d
 // items. Large calls run a workgroup per CU, which takes items in turn and has
 // the next one's first stage on its way while it stores (4 tiles); small ones
 // a workgroup per item and tile, with three stages on their way. 8192 rows x
-// 128 heads: 275 GFLOP in 280 us, 0.98 PFLOP/s (a library product of the shape,
-// which writes them in no such order, 371); 1001 rows 39 us, of 47 in workgroups
-// of one tile and 51 in two of them per CU.
+// 128 heads: 275 GFLOP in 275 us, 1.0 PFLOP/s (a library product of the shape,
+// which writes them in no such order, 371); 1001 rows 36 us (when it was chosen 39,
+// of 47 in workgroups of one tile and 51 in two of them per CU).
 constexpr int kDc = 512;
 constexpr int kBk = 64;
 constexpr int kStages = kDc / kBk;

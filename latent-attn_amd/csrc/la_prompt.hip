@@ -386,15 +386,15 @@ __device__ inline void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"
 // 4 waves of 32 tokens over 64 keys at a time, two buffers of 40 KB, two
 // workgroups per CU, whose waves overlap each other's softmax and products.
 // Bound by its products and, through them, by power: 8192 tokens x 128 heads,
-// 2.75 TFLOP, take 2.33 ms, 1.18 PFLOP/s, the matrix cores 69 % busy at the 1.64
-// GHz that the card then holds (a whole call 2.62 ms with random numbers, 2.2
+// 2.75 TFLOP, take 2.26 ms, 1.22 PFLOP/s, the matrix cores 69 % busy at the 1.70
+// GHz that the card then holds (a whole call 2.54 ms with random numbers, 1.91
 // with zeros). Every operand byte serves 32 tokens, so LDS reads (40 KB per wave
 // and tile) take as long as the products do; they and the vector work hide
 // behind the other waves. Not taken, a call (2743 us then): two groups of four
 // waves in step, one in its products while the other is in its softmax, 2716 to
 // 2772; 64 tokens per wave, half the reads but one wave per SIMD, 2960 to 3160.
-// 64 tokens of one step over 8192 shared rows: 512 MB of keys and values in 105
-// us, 5.1 TB/s.
+// 64 tokens of one step over 8192 shared rows: 537 MB of keys and values in 107
+// us, 5.0 TB/s.
 // Roundings to 16 bits, the products' operand type: expanded keys and values,
 // the queries (rotated first) and a tile's exponentials, as the decode kernels
 // round rows, queries and exponentials; scores, maxima, sums and outputs are
