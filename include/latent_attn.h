@@ -65,7 +65,7 @@ typedef enum la_status {
   LA_SUCCESS = 0,
   LA_ERROR_INVALID_VALUE = 1, /* null pointer, bad shape or config         */
   LA_ERROR_NOT_SUPPORTED = 2, /* no kernel for this dtype / dims / device   */
-  LA_ERROR_WORKSPACE = 3,     /* caller workspace smaller than required     */
+  LA_ERROR_WORKSPACE = 3,     /* caller workspace smaller than required, or none where one is required */
   LA_ERROR_HIP = 4            /* a HIP call failed: see la_last_hip_error() */
 } la_status;
 
@@ -268,7 +268,7 @@ typedef struct la_prefill_args {
   void* output;
   int32_t out_dtype;
   la_mla_config cfg;
-  void* workspace; /* la_mla_prefill_workspace_size bytes; NULL: taken stream-ordered */
+  void* workspace; /* la_mla_prefill_workspace_size bytes; NULL: taken stream-ordered (not under capture) */
   size_t workspace_bytes;
   /* 0 = automatic; 1 = plain kernel (any type and head shape); 2 = keys and
    * values expanded from the rows, on the matrix cores; 3 = queries absorbed,
@@ -304,7 +304,7 @@ typedef struct la_expand_args {
    * are 8 + 4 g + (0..3). */
   void* expanded;
   size_t expanded_bytes;
-  void* workspace; /* la_expand_prefix_workspace_size bytes; NULL: taken stream-ordered */
+  void* workspace; /* la_expand_prefix_workspace_size bytes; NULL: taken stream-ordered (not under capture) */
   size_t workspace_bytes;
 } la_expand_args;
 
@@ -323,7 +323,7 @@ typedef struct la_shared_args {
   const void* expanded;
   void* output; /* (num_seqs * queries_per_seq, num_heads, v_head_dim) of out_dtype (F32, F16, BF16) */
   int32_t out_dtype;
-  void* workspace; /* la_mla_decode_shared_workspace_size bytes; NULL: taken stream-ordered */
+  void* workspace; /* la_mla_decode_shared_workspace_size bytes; NULL: taken stream-ordered (not under capture) */
   size_t workspace_bytes;
   /* 0 = automatic; 1 = latent rows of the prefix; 2 = its expanded form */
   int32_t kernel_variant;

@@ -526,7 +526,9 @@ struct Carve {
   size_t total() const { return at > 0 ? at + kAlign : 0; }  // the base may have to be aligned
 };
 
-// The caller's workspace, or one of `need` bytes taken and returned in the order of the stream.
+// The caller's workspace, or one of `need` bytes taken and returned in the order
+// of the stream. Under capture it has to be the caller's: whatever replays the
+// graph then owns the memory that its kernels write.
 struct Scratch {
   void* ws;
   bool owned = false;
@@ -537,7 +539,13 @@ struct Scratch {
     if (ws) {
       if (given_bytes < need) status = LA_ERROR_WORKSPACE;
     } else {
-      const hipError_t e = hipMallocAsync(&ws, need, st);
+      hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+      hipError_t e = st ? hipStreamIsCapturing(st, &capture) : hipSuccess;  // (the default stream is never captured)
+      if (e == hipSuccess && capture != hipStreamCaptureStatusNone) {
+        status = LA_ERROR_WORKSPACE;
+        return;
+      }
+      if (e == hipSuccess) e = hipMallocAsync(&ws, need, st);
       if (e != hipSuccess) status = record_hip(e);
       else owned = true;
     }

@@ -224,3 +224,23 @@ def test_a_shared_step_past_one_grid(cuda):
     for b in (0, 511, 512, B - 1):
         ref = small_reference(torch.cat([front, kv[b]]), torch.cat([q_nope, q_rope], -1)[b:b + 1], W_UK, W_UV, heads, dn, dv)
         assert (got[b:b + 1].double() - ref).abs().max() <= CLOSE, b
+
+
+@pytest.mark.parametrize("heads", [16, 3])
+@pytest.mark.parametrize("kv", [torch.bfloat16, torch.float32])
+def test_a_prefix_and_no_room_for_own_rows(cuda, heads, kv):
+    """Own caches of no rows at all: the prefix alone."""
+    g = torch.Generator().manual_seed(5)
+    front = torch.randn(90, 576, generator=g).to(kv).to(cuda)
+    W_UK, W_UV = (w.to(cuda) for w in weights(heads, kv, 6))
+    cos, sin = (t.to(cuda) for t in tables(90))
+    q_nope, q_rope = (torch.randn(2, heads, d, generator=g).to(cuda) for d in (128, 64))
+    args = (torch.zeros(2, 0, 576, dtype=kv, device=cuda), q_nope, q_rope, W_UK, W_UV, cos, sin, config(heads))
+    ref = reference([as_double(front)] * 2, as_double(q_nope), as_double(q_rope), as_double(W_UK), as_double(W_UV),
+                    as_double(cos), as_double(sin), [1, 1])[0]
+    got = [F.mla_decode_shared(front, *args)]
+    if kv == torch.bfloat16:
+        prefix = F.expand_prefix(front, W_UK, W_UV, cos, sin, config(heads))
+        got += [F.mla_decode_shared(prefix, *args, kernel_variant=form) for form in (LATENT, OF_EXPANDED)]
+    for x in got:
+        assert_close(x.double().cpu().numpy(), ref.numpy(), "bf16" if kv == torch.bfloat16 else "f32", f"{heads} {kv}")
