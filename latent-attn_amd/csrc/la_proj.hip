@@ -1041,7 +1041,7 @@ hipError_t launch_absorb_mfma(const float* q_nope, const void* W_UK, int w_dtype
   const int64_t groups = (int64_t)((tokens + 31) / 32) * ((nh + 7) / 8);
   if (64 * (dc / kAbsCols) * ((groups + 7) / 8) > most_blocks(kAbsThreads)) {
     if (out_mode != 0 || tokens <= 32) return hipErrorInvalidValue;
-    const int half = tokens / 64 * 32;  // plain rows: two launches
+    const int half = tokens < 64 ? 32 : tokens / 64 * 32;  // plain rows: two launches
     const hipError_t e = launch_absorb_mfma(q_nope, W_UK, w_dtype, out, 0, nullptr, 1.f, 0, half, nh, dn, dc, 1, stream, nullptr, 0);
     if (e != hipSuccess) return e;
     return launch_absorb_mfma(q_nope + (int64_t)half * nh * dn, W_UK, w_dtype, static_cast<float*>(out) + (int64_t)half * nh * dc,
