@@ -30,6 +30,10 @@
  *                         causal or prefix mask (prompts, chunks, drafted tokens)
  *   la_expand_prefix      a shared prefix's keys and values, expanded once
  *   la_mla_decode_shared  a decode step of sequences behind one prefix
+ *   la_mla_decode_tree    attention of a tree of drafted tokens per sequence
+ *   la_accept_kv          keeps the rows of a tree's accepted path
+ *   la_weigh_kv           adds up the attention weight that cache rows get
+ *   la_evict_kv           cuts sequences back to their heaviest rows
  *
  * Layouts (all row-major, contiguous):
  *   latent cache row   [c_t (kv_lora_rank) | k_rope (qk_rope_head_dim)]
@@ -329,6 +333,155 @@ typedef struct la_shared_args {
   int32_t kernel_variant;
 } la_shared_args;
 
+/* Attention of a tree of drafted tokens per sequence (la_mla_decode_tree). */
+typedef struct la_tree_args {
+  /* latent cache, as in la_prefill_args: equal regions of seq_len rows,
+   * seq_offsets, or a paged pool; seq_lens optional (required with
+   * block_table). The nodes' rows are in it already (la_append_kv): they are
+   * the sequence's last `nodes` rows, in the nodes' order. */
+  const void* kv_cache;
+  int32_t kv_dtype;
+  int64_t total_rows;
+  int32_t num_seqs;
+  int32_t seq_len;
+  const int32_t* seq_offsets;
+  const int32_t* seq_lens;
+  const int32_t* block_table;
+  int32_t block_size;
+  int32_t blocks_per_seq;
+  /* drafted tokens of every sequence, 1 .. LA_TREE_MAX_NODES. parents (DEVICE
+   * int32, num_seqs * nodes): node j's parent, an earlier node, or -1 (any
+   * other value counts as -1): it follows the sequence's last row before the
+   * nodes'. With L rows in the sequence node j is at position L - nodes +
+   * depth(j), depth 0 for a child of -1, and so is its key; it sees the first L
+   * - nodes rows, its ancestors and itself. A sequence with fewer rows than
+   * nodes has no tree: its tokens get zero rows. */
+  int32_t nodes;
+  const int32_t* parents;
+  /* queries (num_seqs * nodes, num_heads, .) and their strides, as in
+   * la_prefill_args; rotate_q = 1 rotates q_rope by its node's position */
+  const void* q_nope;
+  const void* q_rope;
+  int32_t q_dtype;
+  int64_t q_nope_token_stride, q_nope_head_stride;
+  int64_t q_rope_token_stride, q_rope_head_stride;
+  int32_t rotate_q;
+  const void* W_UK;
+  int32_t w_uk_dtype;
+  const void* W_UV;
+  int32_t w_uv_dtype;
+  const float* rope_cos;
+  const float* rope_sin;
+  int64_t rope_rows;
+  /* (num_seqs * nodes, num_heads, v_head_dim) of out_dtype (F32, F16, BF16); must not overlap an input */
+  void* output;
+  int32_t out_dtype;
+  la_mla_config cfg;
+  void* workspace; /* la_mla_decode_tree_workspace_size bytes; NULL: taken stream-ordered (not under capture) */
+  size_t workspace_bytes;
+  /* 0 = automatic; 1 = plain kernel (any type and head shape); 2 = matrix
+   * cores (LA_ERROR_NOT_SUPPORTED where la_mla_decode has no MFMA kernel for
+   * nodes * num_heads query heads) */
+  int32_t kernel_variant;
+} la_tree_args;
+#define LA_TREE_MAX_NODES 64
+
+/* Arguments of la_accept_kv. */
+typedef struct la_accept_args {
+  /* latent cache, laid out as for la_append_args; seq_lens holds the rows with
+   * the tree's among them and gets those that stay */
+  void* kv_cache;
+  int32_t kv_dtype;
+  int64_t total_rows;
+  int32_t num_seqs;
+  int32_t seq_capacity;
+  const int32_t* seq_offsets;
+  int32_t* seq_lens;
+  const int32_t* block_table;
+  int32_t block_size;
+  int32_t blocks_per_seq;
+  /* the last `nodes` rows (1 .. LA_TREE_MAX_NODES) are a tree's; path (DEVICE
+   * int32, num_seqs * nodes) lists the accepted nodes from the top down, each
+   * larger than the one before it; the first entry that is not, or is no node,
+   * ends it. Node path[i]'s row moves to row L - nodes + i and the length
+   * becomes L - nodes + (nodes listed). A sequence with fewer rows than nodes
+   * is left unchanged. */
+  int32_t nodes;
+  const int32_t* path;
+  la_mla_config cfg;
+} la_accept_args;
+
+/* Arguments of la_weigh_kv. */
+typedef struct la_weigh_args {
+  /* latent cache, as in la_prefill_args */
+  const void* kv_cache;
+  int32_t kv_dtype;
+  int64_t total_rows;
+  int32_t num_seqs;
+  int32_t seq_len;
+  const int32_t* seq_offsets;
+  const int32_t* seq_lens;
+  const int32_t* block_table;
+  int32_t block_size;
+  int32_t blocks_per_seq;
+  /* queries of every sequence's last tokens_per_seq rows (num_seqs *
+   * tokens_per_seq, num_heads, .), as in la_prefill_args: token j of n of a
+   * sequence with L rows is at position L - n + j and sees the rows up to its own */
+  int32_t tokens_per_seq;
+  const void* q_nope;
+  const void* q_rope;
+  int32_t q_dtype;
+  int64_t q_nope_token_stride, q_nope_head_stride;
+  int64_t q_rope_token_stride, q_rope_head_stride;
+  int32_t rotate_q;
+  const void* W_UK;
+  int32_t w_uk_dtype;
+  const float* rope_cos;
+  const float* rope_sin;
+  int64_t rope_rows;
+  /* fp32, one per row of the sequences' regions: position p of sequence s at
+   * s * seq_len + p (equal regions), seq_offsets[s] + p, or s *
+   * blocks_per_seq * block_size + p (paged). Entries past a sequence's rows
+   * are left as they are. */
+  float* weights;
+  la_mla_config cfg;
+  void* workspace; /* la_weigh_kv_workspace_size bytes; NULL: taken stream-ordered (not under capture) */
+  size_t workspace_bytes;
+  int32_t kernel_variant; /* 0 = automatic; 1 = plain kernels (any type and head shape); 2 = matrix cores */
+} la_weigh_args;
+
+/* Arguments of la_evict_kv. */
+typedef struct la_evict_args {
+  /* latent cache, laid out as for la_append_args; seq_lens is changed */
+  void* kv_cache;
+  int32_t kv_dtype;
+  int64_t total_rows;
+  int32_t num_seqs;
+  int32_t seq_capacity;
+  const int32_t* seq_offsets;
+  int32_t* seq_lens;
+  const int32_t* block_table;
+  int32_t block_size;
+  int32_t blocks_per_seq;
+  float* weights; /* as in la_weigh_args (seq_capacity for seq_len); moved along */
+  /* a sequence with more than `keep` rows keeps its first `first` ones, its
+   * last `last` ones and of the rows between the keep - first - last with the
+   * largest weights (of equal ones the earlier; NaN counts as the smallest):
+   * rows and weights move down to [0, keep) in their order, the weights behind
+   * are zeroed (the rows are left as they are), the length becomes keep.
+   * Positions are a row's place in the cache, here as everywhere. Shorter
+   * sequences are left unchanged. first + last <= keep. */
+  int32_t keep;
+  int32_t first;
+  int32_t last;
+  /* optional (DEVICE int32, num_seqs * keep): every row's position before the
+   * call, -1 past the sequence's rows */
+  int32_t* kept;
+  la_mla_config cfg;
+  void* workspace; /* la_evict_kv_workspace_size bytes; NULL: taken stream-ordered (not under capture) */
+  size_t workspace_bytes;
+} la_evict_args;
+
 /* Human-readable name of an la_status value. */
 const char* la_status_string(int status);
 
@@ -497,6 +650,22 @@ size_t la_expanded_size(int32_t rows, const la_mla_config* cfg);
  * part is computed for all queries at once. */
 int la_mla_decode_shared(const la_shared_args* args, void* stream);
 size_t la_mla_decode_shared_workspace_size(const la_shared_args* args);
+
+/* out[j,h] as in la_mla_prefill, over the keys that node j sees. */
+int la_mla_decode_tree(const la_tree_args* args, void* stream);
+size_t la_mla_decode_tree_workspace_size(const la_tree_args* args);
+
+/* Keeps an accepted path's rows of a tree and sets the lengths. */
+int la_accept_kv(const la_accept_args* args, void* stream);
+
+/* weights[s,p] += sum over the sequence's tokens t that see p, and heads h, of
+ * softmax_p(scale * (q_nope[t,h] . K[p,h] + q_rope[t,h] . RoPE(k_rope[p], p))), in fp32. */
+int la_weigh_kv(const la_weigh_args* args, void* stream);
+size_t la_weigh_kv_workspace_size(const la_weigh_args* args);
+
+/* Cuts every sequence back to its heaviest rows, in place. */
+int la_evict_kv(const la_evict_args* args, void* stream);
+size_t la_evict_kv_workspace_size(const la_evict_args* args);
 
 #ifdef __cplusplus
 } /* extern "C" */

@@ -35,8 +35,8 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 
 LIB_NAME = "liblatent_attn_hip.so"
-HIP_SOURCES = ["la_append.hip", "la_capi.hip", "la_expand.hip", "la_f32.hip", "la_generic.hip", "la_join.hip", "la_mfma.hip",
-               "la_mfma16.hip", "la_naive.hip", "la_proj.hip", "la_prompt.hip"]
+HIP_SOURCES = ["la_append.hip", "la_capi.hip", "la_evict.hip", "la_expand.hip", "la_f32.hip", "la_generic.hip", "la_join.hip",
+               "la_mfma.hip", "la_mfma16.hip", "la_naive.hip", "la_proj.hip", "la_prompt.hip", "la_tree.hip", "la_weigh.hip"]
 
 # -packed-fp32-ops: keep hipcc from emitting v_pk_{add,mul,fma}_f32.
 HIP_FLAGS = [

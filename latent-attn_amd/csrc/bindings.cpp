@@ -8,8 +8,9 @@
 // contract) or bfloat16, float32 caches/weights select the fp32 path, a
 // device guard is taken, and functions are added (mla_decode_forward,
 // mla_decode_absorbed_forward, append_kv_forward, absorb_q_forward,
-// mla_prefill_forward, expand_prefix_forward, mla_decode_shared_forward). No tensor math happens here; all compute is in the HIP
-// library.
+// mla_prefill_forward, expand_prefix_forward, mla_decode_shared_forward,
+// mla_decode_tree_forward, accept_kv_forward, weigh_kv_forward, evict_kv_forward). No tensor math happens here; all
+// compute is in the HIP library.
 #include <torch/extension.h>
 #include <c10/hip/HIPStream.h>
 
@@ -810,6 +811,241 @@ torch::Tensor mla_decode_shared_forward(torch::Tensor prefix, c10::optional<torc
   return output;
 }
 
+namespace {
+
+// Sequences of a cache: as block_table, seq_offsets or the cache's first dimension tell.
+int64_t batch_of(const torch::Tensor& kv_cache, const c10::optional<torch::Tensor>& seq_offsets,
+                 const c10::optional<torch::Tensor>& block_table, int64_t row) {
+  int64_t batch;
+  if (block_table.has_value() && block_table->defined()) {
+    TORCH_CHECK(block_table->dim() == 2, "block_table must be a contiguous int32 CUDA tensor (batch, blocks_per_seq)");
+    batch = block_table->size(0);
+  } else if (seq_offsets.has_value() && seq_offsets->defined()) {
+    TORCH_CHECK(seq_offsets->dim() == 1 && seq_offsets->size(0) > 0, "seq_offsets must have batch + 1 entries");
+    batch = seq_offsets->size(0) - 1;
+  } else {
+    TORCH_CHECK(kv_cache.dim() == 3, "kv_cache must be (batch, seq_len, ", row, ") when seq_offsets is None");
+    batch = kv_cache.size(0);
+  }
+  TORCH_CHECK(batch < INT32_MAX, "batch too large");
+  return batch;
+}
+
+// Queries (batch * n, num_heads, .) of any type and strides, as mla_prefill_forward takes them. Returns n.
+template <typename Args>
+int64_t fill_queries(Args& a, const torch::Tensor& kv_cache, torch::Tensor& q_nope, torch::Tensor& q_rope, bool rotate_q,
+                     int64_t batch, const la_mla_config& c) {
+  TORCH_CHECK(q_nope.dim() == 3 && q_nope.size(1) == c.num_heads && q_nope.size(2) == c.qk_nope_head_dim,
+              "q_nope must be (tokens, num_heads, qk_nope_head_dim)");
+  const int64_t tokens = q_nope.size(0);
+  TORCH_CHECK(q_rope.dim() == 3 && q_rope.size(0) == tokens && q_rope.size(1) == c.num_heads &&
+                  q_rope.size(2) == c.qk_rope_head_dim,
+              "q_rope must be (tokens, num_heads, qk_rope_head_dim)");
+  TORCH_CHECK(dtype_tag(q_nope) >= 0 && dtype_tag(q_nope) != LA_DTYPE_FP8_E4M3,
+              "q_nope must be float16, bfloat16 or float32, got ", q_nope.dtype());
+  TORCH_CHECK(q_rope.dtype() == q_nope.dtype(), "q_nope and q_rope must have the same dtype");
+  TORCH_CHECK(batch > 0 ? tokens % batch == 0 : tokens == 0, "tokens must be a multiple of the batch");
+  TORCH_CHECK(tokens <= INT32_MAX / c.num_heads, "too many tokens");
+  for (auto* t : {&q_nope, &q_rope}) {
+    TORCH_CHECK(t->is_cuda(), "queries must be on CUDA");
+    TORCH_CHECK(t->stride(2) == 1 && t->stride(0) >= 0 && t->stride(1) >= 0,
+                "queries must be contiguous in their last dimension");
+    check_same_device(kv_cache, *t, "queries");
+    // one row broadcast to all tokens and heads: strides of 0, which mean packed below
+    if (t->stride(0) == 0 && t->stride(1) == 0) *t = t->contiguous();
+  }
+  a.q_nope = q_nope.data_ptr();
+  a.q_rope = q_rope.data_ptr();
+  a.q_dtype = dtype_tag(q_nope);
+  if (!q_nope.is_contiguous()) a.q_nope_token_stride = q_nope.stride(0), a.q_nope_head_stride = q_nope.stride(1);
+  if (!q_rope.is_contiguous()) a.q_rope_token_stride = q_rope.stride(0), a.q_rope_head_stride = q_rope.stride(1);
+  a.rotate_q = rotate_q;
+  return batch > 0 ? tokens / batch : 0;
+}
+
+template <typename Args>
+void fill_tables(Args& a, const torch::Tensor& kv_cache, const torch::Tensor& rope_cos, const torch::Tensor& rope_sin,
+                 int64_t longest, const la_mla_config& c) {
+  check_fp32_contiguous(rope_cos, "rope_cos");
+  check_fp32_contiguous(rope_sin, "rope_sin");
+  check_rope(rope_cos, rope_sin, std::max<int64_t>(longest, 1), c);
+  for (auto* t : {&rope_cos, &rope_sin}) check_same_device(kv_cache, *t, "inputs");
+  a.rope_cos = rope_cos.data_ptr<float>();
+  a.rope_sin = rope_sin.data_ptr<float>();
+  a.rope_rows = std::min(rope_cos.size(0), rope_sin.size(0));
+}
+
+// One int32 per sequence and `n`, on the cache's device.
+void check_ints(const torch::Tensor& kv_cache, const torch::Tensor& t, int64_t batch, int64_t n, const char* name,
+                const char* shape) {
+  TORCH_CHECK(t.dtype() == torch::kInt32 && t.is_contiguous() && t.is_cuda() && t.dim() == 2 && t.size(0) == batch &&
+                  t.size(1) == n,
+              name, " must be a contiguous int32 CUDA tensor ", shape);
+  check_same_device(kv_cache, t, name);
+}
+
+// Row weights over the sequences' regions.
+template <typename Args>
+void check_row_weights(const Args& a, const torch::Tensor& kv_cache, const torch::Tensor& weights, int64_t capacity) {
+  check_fp32_contiguous(weights, "weights");
+  check_same_device(kv_cache, weights, "weights");
+  if (a.seq_offsets) {
+    TORCH_CHECK(weights.dim() == 1 && weights.size(0) == a.total_rows, "weights must be (total_rows,) for a packed cache");
+  } else {
+    TORCH_CHECK(weights.dim() == 2 && weights.size(0) == a.num_seqs && weights.size(1) == capacity,
+                "weights must be (batch, ", capacity, "), one per row of the sequences' regions");
+  }
+}
+
+// Cache whose rows move and whose lengths change: as append_kv_forward's.
+template <typename Args>
+void fill_moved(Args& a, const torch::Tensor& kv_cache, const torch::Tensor& seq_lens,
+                const c10::optional<torch::Tensor>& seq_offsets, const c10::optional<torch::Tensor>& block_table,
+                int block_size, const la_mla_config& c) {
+  check_storage(kv_cache, "kv_cache");
+  TORCH_CHECK(seq_lens.dtype() == torch::kInt32 && seq_lens.is_contiguous() && seq_lens.is_cuda() && seq_lens.dim() == 1,
+              "seq_lens must be a contiguous 1D int32 CUDA tensor");
+  la_prefill_args f{};  // the checks of the caches that are read
+  const int64_t row = (int64_t)c.kv_lora_rank + c.qk_rope_head_dim;
+  const int64_t batch = batch_of(kv_cache, seq_offsets, block_table, row);
+  fill_cache(f, kv_cache, seq_offsets, seq_lens, block_table, block_size, batch, row);
+  a.kv_cache = kv_cache.data_ptr();
+  a.kv_dtype = f.kv_dtype;
+  a.total_rows = f.total_rows;
+  a.num_seqs = f.num_seqs;
+  a.seq_capacity = f.seq_len;
+  a.seq_offsets = f.seq_offsets;
+  a.seq_lens = seq_lens.data_ptr<int32_t>();
+  a.block_table = f.block_table;
+  a.block_size = f.block_size;
+  a.blocks_per_seq = f.blocks_per_seq;
+  a.cfg = c;
+}
+
+}  // namespace
+
+// mla_decode_tree_forward -- trees of drafted tokens (la_mla_decode_tree):
+//   q_nope (B*n, nh, dn), q_rope (B*n, nh, dR), parents int32 (B, n); returns
+//   (B*n, nh, dv) in out_dtype.
+torch::Tensor mla_decode_tree_forward(torch::Tensor kv_cache, torch::Tensor q_nope, torch::Tensor q_rope,
+                                      torch::Tensor W_UK, torch::Tensor W_UV, torch::Tensor rope_cos,
+                                      torch::Tensor rope_sin, torch::Tensor parents,
+                                      c10::optional<torch::Tensor> seq_offsets, int d_model, int kv_lora_rank,
+                                      int qk_nope_head_dim, int qk_rope_head_dim, int num_heads, int v_head_dim,
+                                      c10::optional<torch::Tensor> seq_lens, c10::optional<torch::Tensor> block_table,
+                                      int block_size, bool rotate_q, c10::ScalarType out_dtype, int kernel_variant) {
+  check_storage(kv_cache, "kv_cache");
+  const la_mla_config cfg =
+      config_from_args(d_model, kv_lora_rank, qk_nope_head_dim, qk_rope_head_dim, num_heads, v_head_dim);
+  const int64_t row = (int64_t)kv_lora_rank + qk_rope_head_dim;
+  const int64_t batch = batch_of(kv_cache, seq_offsets, block_table, row);
+  la_tree_args a{};
+  const int64_t longest = fill_cache(a, kv_cache, seq_offsets, seq_lens, block_table, block_size, batch, row);
+  const int64_t nodes = fill_queries(a, kv_cache, q_nope, q_rope, rotate_q, batch, cfg);
+  TORCH_CHECK(batch == 0 || (nodes >= 1 && nodes <= LA_TREE_MAX_NODES), "a tree has 1 to ", LA_TREE_MAX_NODES, " nodes");
+  check_ints(kv_cache, parents, batch, batch > 0 ? nodes : parents.size(-1), "parents", "(batch, nodes)");
+  check_weights(kv_cache, W_UK, W_UV, cfg);
+  fill_tables(a, kv_cache, rope_cos, rope_sin, longest, cfg);
+  a.nodes = (int32_t)std::max<int64_t>(nodes, 1);
+  a.parents = parents.data_ptr<int32_t>();
+  a.W_UK = W_UK.data_ptr();
+  a.w_uk_dtype = dtype_tag(W_UK);
+  a.W_UV = W_UV.data_ptr();
+  a.w_uv_dtype = dtype_tag(W_UV);
+  a.out_dtype = out_tag(out_dtype);
+  a.cfg = cfg;
+  a.kernel_variant = kernel_variant;
+  const at::DeviceGuard guard(kv_cache.device());
+  auto output = torch::empty({q_nope.size(0), num_heads, v_head_dim}, kv_cache.options().dtype(out_dtype));
+  if (batch == 0) return output;
+  a.output = output.data_ptr();
+  a.workspace_bytes = la_mla_decode_tree_workspace_size(&a);
+  auto ws = workspace(kv_cache, a.workspace_bytes);
+  a.workspace = ws.data_ptr();
+  check_status(la_mla_decode_tree(&a, current_stream()), "la_mla_decode_tree");
+  return output;
+}
+
+// accept_kv_forward -- keeps an accepted path's rows (la_accept_kv); path int32 (B, nodes).
+void accept_kv_forward(torch::Tensor kv_cache, torch::Tensor seq_lens, int64_t nodes, torch::Tensor path,
+                       c10::optional<torch::Tensor> seq_offsets, int d_model, int kv_lora_rank, int qk_nope_head_dim,
+                       int qk_rope_head_dim, int num_heads, int v_head_dim, c10::optional<torch::Tensor> block_table,
+                       int block_size) {
+  const la_mla_config cfg =
+      config_from_args(d_model, kv_lora_rank, qk_nope_head_dim, qk_rope_head_dim, num_heads, v_head_dim);
+  la_accept_args a{};
+  fill_moved(a, kv_cache, seq_lens, seq_offsets, block_table, block_size, cfg);
+  TORCH_CHECK(nodes >= 1 && nodes <= LA_TREE_MAX_NODES, "a tree has 1 to ", LA_TREE_MAX_NODES, " nodes");
+  check_ints(kv_cache, path, a.num_seqs, nodes, "path", "(batch, nodes)");
+  a.nodes = (int32_t)nodes;
+  a.path = path.data_ptr<int32_t>();
+  const at::DeviceGuard guard(kv_cache.device());
+  check_status(la_accept_kv(&a, current_stream()), "la_accept_kv");
+}
+
+// weigh_kv_forward -- adds the weight that the last tokens give every row (la_weigh_kv).
+void weigh_kv_forward(torch::Tensor weights, torch::Tensor kv_cache, torch::Tensor q_nope, torch::Tensor q_rope,
+                      torch::Tensor W_UK, torch::Tensor rope_cos, torch::Tensor rope_sin,
+                      c10::optional<torch::Tensor> seq_offsets, int d_model, int kv_lora_rank, int qk_nope_head_dim,
+                      int qk_rope_head_dim, int num_heads, int v_head_dim, c10::optional<torch::Tensor> seq_lens,
+                      c10::optional<torch::Tensor> block_table, int block_size, bool rotate_q, int kernel_variant) {
+  check_storage(kv_cache, "kv_cache");
+  const la_mla_config cfg =
+      config_from_args(d_model, kv_lora_rank, qk_nope_head_dim, qk_rope_head_dim, num_heads, v_head_dim);
+  const int64_t row = (int64_t)kv_lora_rank + qk_rope_head_dim;
+  const int64_t batch = batch_of(kv_cache, seq_offsets, block_table, row);
+  la_weigh_args a{};
+  const int64_t longest = fill_cache(a, kv_cache, seq_offsets, seq_lens, block_table, block_size, batch, row);
+  const int64_t n = fill_queries(a, kv_cache, q_nope, q_rope, rotate_q, batch, cfg);
+  check_weight(W_UK, "W_UK");
+  TORCH_CHECK(W_UK.dim() == 2 && W_UK.size(0) == (int64_t)num_heads * qk_nope_head_dim && W_UK.size(1) == kv_lora_rank,
+              "W_UK shape mismatch");
+  check_same_device(kv_cache, W_UK, "W_UK");
+  fill_tables(a, kv_cache, rope_cos, rope_sin, longest, cfg);
+  check_row_weights(a, kv_cache, weights, a.block_table ? (int64_t)a.blocks_per_seq * a.block_size : (int64_t)a.seq_len);
+  a.tokens_per_seq = (int32_t)n;
+  a.W_UK = W_UK.data_ptr();
+  a.w_uk_dtype = dtype_tag(W_UK);
+  a.weights = weights.data_ptr<float>();
+  a.cfg = cfg;
+  a.kernel_variant = kernel_variant;
+  if (batch == 0 || n == 0 || weights.numel() == 0) return;
+  const at::DeviceGuard guard(kv_cache.device());
+  a.workspace_bytes = la_weigh_kv_workspace_size(&a);
+  auto ws = workspace(kv_cache, a.workspace_bytes);
+  a.workspace = ws.data_ptr();
+  check_status(la_weigh_kv(&a, current_stream()), "la_weigh_kv");
+}
+
+// evict_kv_forward -- cuts every sequence back to its heaviest rows (la_evict_kv); returns the kept rows' positions
+// before the call, int32 (B, keep).
+torch::Tensor evict_kv_forward(torch::Tensor kv_cache, torch::Tensor seq_lens, torch::Tensor weights, int64_t keep,
+                               int64_t first, int64_t last, c10::optional<torch::Tensor> seq_offsets, int d_model,
+                               int kv_lora_rank, int qk_nope_head_dim, int qk_rope_head_dim, int num_heads,
+                               int v_head_dim, c10::optional<torch::Tensor> block_table, int block_size) {
+  const la_mla_config cfg =
+      config_from_args(d_model, kv_lora_rank, qk_nope_head_dim, qk_rope_head_dim, num_heads, v_head_dim);
+  la_evict_args a{};
+  fill_moved(a, kv_cache, seq_lens, seq_offsets, block_table, block_size, cfg);
+  TORCH_CHECK(keep >= 0 && keep <= INT32_MAX && first >= 0 && last >= 0 && first <= keep && last <= keep - first,
+              "keep must be at least first + last, and none negative");
+  check_row_weights(a, kv_cache, weights, a.block_table ? (int64_t)a.blocks_per_seq * a.block_size : (int64_t)a.seq_capacity);
+  a.weights = weights.data_ptr<float>();
+  a.keep = (int32_t)keep;
+  a.first = (int32_t)first;
+  a.last = (int32_t)last;
+  const at::DeviceGuard guard(kv_cache.device());
+  auto kept = torch::empty({a.num_seqs, keep}, seq_lens.options());
+  if (a.num_seqs == 0) return kept;
+  if (weights.numel() == 0) return kept.fill_(-1);  // no row anywhere
+  a.kept = keep > 0 ? kept.data_ptr<int32_t>() : nullptr;
+  a.workspace_bytes = la_evict_kv_workspace_size(&a);
+  auto ws = workspace(kv_cache, a.workspace_bytes);
+  a.workspace = ws.data_ptr();
+  check_status(la_evict_kv(&a, current_stream()), "la_evict_kv");
+  return kept;
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("naive_mla_forward", &naive_mla_forward, "MLA forward from q_nope and W_UK (decompress-then-attend result)");
   m.def("fused_mla_forward", &fused_mla_forward,
@@ -842,4 +1078,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("expand_prefix_forward", &expand_prefix_forward, "Per-head keys and values of a prefix's latent rows");
   m.def("mla_decode_shared_forward", &mla_decode_shared_forward,
         "Decode step over a shared prefix and every sequence's own rows");
+  m.def("mla_decode_tree_forward", &mla_decode_tree_forward, "Attention of trees of drafted tokens over latent caches");
+  m.def("accept_kv_forward", &accept_kv_forward, "Keeps the rows of trees' accepted paths");
+  m.def("weigh_kv_forward", &weigh_kv_forward, "Adds the attention weight that cache rows get");
+  m.def("evict_kv_forward", &evict_kv_forward, "Cuts sequences back to their heaviest rows");
 }

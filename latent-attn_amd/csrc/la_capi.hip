@@ -7,6 +7,7 @@
 // the other absorption in la_f32.hip and la_generic.hip, la_append.hip,
 // la_naive.hip.
 #include "la_internal.hpp"
+#include "la_draft.hpp"
 #include "la_prompt.hpp"
 
 #include <algorithm>
@@ -312,6 +313,7 @@ struct StepTail {
   DecodeProblem p;               // out: the problem with its slots' addresses
   bool merge = true;             // false: the slots stay as they are, nothing is written to the output
   const void* q_prep = nullptr;  // the same queries' 16-bit rows in a layout that is this step's too
+  TreeStep tree{};               // the queries are trees' nodes (MFMA kernels only)
 };
 int run(const la_decode_args* a, hipStream_t stream, hipEvent_t ev_b = nullptr, hipEvent_t ev_e = nullptr,
         int repeat = 1, bool coarse = false, StepTail* tail = nullptr) {
@@ -1219,6 +1221,333 @@ int decode_shared(const la_shared_args* a, hipStream_t stream, bool run_it, size
   return scratch.finish(st);
 }
 
+// ---- trees of drafted tokens, eviction --------------------------------------------------------------
+
+// Cache and sequences of la_tree_args and la_weigh_args: checked as prepare() and prepare_prefill() do.
+template <typename Args>
+bool row_source(const Args* a, RowSource* out) {
+  if (a->num_seqs < 0 || a->num_seqs == INT32_MAX || a->total_rows < 0 || a->rope_rows < 0) return false;
+  const bool paged = a->block_table != nullptr;
+  if (paged) {
+    if (a->block_size <= 0 || a->blocks_per_seq <= 0 || a->seq_offsets || !a->seq_lens ||
+        a->total_rows % a->block_size != 0 || (int64_t)a->blocks_per_seq * a->block_size > INT32_MAX ||
+        a->total_rows > (int64_t)UINT32_MAX || (a->num_seqs > 0 && a->total_rows < a->block_size))
+      return false;
+  } else if (a->seq_offsets) {
+    if (a->total_rows > INT32_MAX) return false;
+  } else if (a->seq_len < 0 || (int64_t)a->num_seqs * a->seq_len > a->total_rows) {
+    return false;
+  }
+  RowSource r{};
+  r.kv = a->kv_cache;
+  r.kv_dtype = a->kv_dtype;
+  r.row_elems = a->cfg.kv_lora_rank + a->cfg.qk_rope_head_dim;
+  r.total_rows = a->total_rows;
+  r.num_seqs = a->num_seqs;
+  r.offsets = a->seq_offsets;
+  r.lens = a->seq_lens;
+  r.cos = a->rope_cos;
+  r.sin = a->rope_sin;
+  r.rope_rows = a->rope_rows;
+  if (paged) {
+    r.block_table = a->block_table;
+    r.block_size = a->block_size;
+    r.blocks_per_seq = a->blocks_per_seq;
+    r.pool_blocks = a->total_rows / a->block_size;
+    r.region = a->blocks_per_seq * a->block_size;
+  } else if (!a->seq_offsets) {
+    r.region = r.stride_rows = a->seq_len;
+  }
+  *out = r;
+  return true;
+}
+// Their queries, n tokens per sequence.
+template <typename Args>
+bool query_source(const Args* a, int n, QuerySource* out) {
+  const la_mla_config& c = a->cfg;
+  if (!valid_dtype(a->q_dtype) || (a->rotate_q != 0 && a->rotate_q != 1) || a->q_nope_token_stride < 0 ||
+      a->q_nope_head_stride < 0 || a->q_rope_token_stride < 0 || a->q_rope_head_stride < 0 ||
+      (int64_t)a->num_seqs * n > INT32_MAX / c.num_heads)
+    return false;
+  QuerySource q{};
+  q.q_nope = a->q_nope;
+  q.q_rope = a->q_rope;
+  q.dtype = a->q_dtype;
+  const bool nope_packed = a->q_nope_token_stride == 0 && a->q_nope_head_stride == 0;
+  const bool rope_packed = a->q_rope_token_stride == 0 && a->q_rope_head_stride == 0;
+  q.nope_stride = nope_packed ? (int64_t)c.num_heads * c.qk_nope_head_dim : a->q_nope_token_stride;
+  q.nope_head = nope_packed ? c.qk_nope_head_dim : a->q_nope_head_stride;
+  q.rope_stride = rope_packed ? (int64_t)c.num_heads * c.qk_rope_head_dim : a->q_rope_token_stride;
+  q.rope_head = rope_packed ? c.qk_rope_head_dim : a->q_rope_head_stride;
+  q.rotate = a->rotate_q;
+  q.tokens = (int64_t)a->num_seqs * n;
+  q.num_seqs = a->num_seqs;
+  q.per_seq = n;
+  *out = q;
+  return true;
+}
+// Queries that the absorption and the decode kernels take where they lie.
+bool packed_f32(const void* base, int dtype, int64_t stride, int64_t head, int nh, int dim) {
+  return dtype == LA_DTYPE_F32 && head == dim && stride == (int64_t)nh * dim && (reinterpret_cast<uintptr_t>(base) & 15) == 0;
+}
+bool queries_vec(const QuerySource& q) {
+  return q_vec(q.q_nope, q.dtype, q.nope_stride, q.nope_head) && q_vec(q.q_rope, q.dtype, q.rope_stride, q.rope_head);
+}
+
+constexpr bool tree_kernels() { return false; }
+enum TreeForm { kTreePlain = 1, kTreeMfma = 2 };
+
+int decode_tree(const la_tree_args* a, void* stream_v, bool run_it, size_t* need) {
+  const hipStream_t stream = static_cast<hipStream_t>(stream_v);
+  if (!a || !valid_cfg(&a->cfg) || !valid_cache_dtype(a->kv_dtype) || !valid_dtype(a->w_uk_dtype) ||
+      !valid_dtype(a->w_uv_dtype) || !valid_out(a->out_dtype) || a->nodes < 1 || a->nodes > kTreeNodes ||
+      a->kernel_variant < 0 || a->kernel_variant > kTreeMfma)
+    return LA_ERROR_INVALID_VALUE;
+  const la_mla_config& c = a->cfg;
+  const int nh = c.num_heads, n = a->nodes;
+  TreeQueries t{};
+  if (!row_source(a, &t.src) || !query_source(a, n, &t.q)) return LA_ERROR_INVALID_VALUE;
+  if (need) *need = 0;
+  if (a->num_seqs == 0) return LA_SUCCESS;
+  if (!a->parents || !a->q_nope || !a->q_rope || !a->W_UK || !a->W_UV || !a->rope_cos || !a->rope_sin || !a->output ||
+      (a->total_rows > 0 && !a->kv_cache))
+    return LA_ERROR_INVALID_VALUE;
+  const int64_t tokens = t.q.tokens, rows = tokens * nh;
+  const bool nope_as_is = packed_f32(t.q.q_nope, t.q.dtype, t.q.nope_stride, t.q.nope_head, nh, c.qk_nope_head_dim);
+  const bool rope_as_is = !a->rotate_q && packed_f32(t.q.q_rope, t.q.dtype, t.q.rope_stride, t.q.rope_head, nh, c.qk_rope_head_dim);
+
+  // The step over the trees: every node a query of its sequence. Aligned addresses stand for what lies in the workspace.
+  alignas(256) static const char any[256] = {0};
+  la_decode_args d{};
+  d.kv_cache = a->kv_cache;
+  d.kv_dtype = a->kv_dtype;
+  d.total_rows = a->total_rows;
+  d.num_seqs = a->num_seqs;
+  d.seq_len = a->seq_len;
+  d.seq_offsets = a->seq_offsets;
+  d.seq_lens = reinterpret_cast<const int32_t*>(any);
+  d.block_table = a->block_table;
+  d.block_size = a->block_size;
+  d.blocks_per_seq = a->blocks_per_seq;
+  d.queries_per_seq = n;
+  d.q_nope = nope_as_is ? static_cast<const float*>(a->q_nope) : reinterpret_cast<const float*>(any);
+  d.q_rope = rope_as_is ? static_cast<const float*>(a->q_rope) : reinterpret_cast<const float*>(any);
+  d.W_UK = a->W_UK;
+  d.w_uk_dtype = a->w_uk_dtype;
+  d.W_UV = a->W_UV;
+  d.w_uv_dtype = a->w_uv_dtype;
+  d.rope_cos = a->rope_cos;
+  d.rope_sin = a->rope_sin;
+  d.rope_rows = a->rope_rows;
+  d.output = reinterpret_cast<float*>(const_cast<char*>(any));
+  d.cfg = c;
+  DecodeProblem step;
+  Plan plan;
+  const bool mfma = tree_kernels() && a->kernel_variant != kTreePlain && prepare(&d, &step, &plan) == LA_SUCCESS && plan.mfma;
+  if (!mfma && (a->kernel_variant == kTreeMfma || !generic_prompt_supported(c.kv_lora_rank, c.qk_rope_head_dim)))
+    return LA_ERROR_NOT_SUPPORTED;
+  const bool join = mfma && merge_join_supported(step);
+  const size_t step_bytes = mfma ? la_mla_decode_workspace_size(&d) : 0;
+
+  float *q_abs = nullptr, *out32 = nullptr;
+  void* step_ws = nullptr;
+  auto carve = [&](void* ws) {
+    Carve v(ws);
+    t.lens = static_cast<int32_t*>(v.take((size_t)a->num_seqs * sizeof(int32_t)));
+    t.seen = static_cast<uint64_t*>(v.take((size_t)tokens * sizeof(uint64_t)));
+    t.cos = static_cast<float*>(v.take((size_t)tokens * (c.qk_rope_head_dim / 2) * sizeof(float)));
+    t.sin = static_cast<float*>(v.take((size_t)tokens * (c.qk_rope_head_dim / 2) * sizeof(float)));
+    if (!nope_as_is) t.q_nope = static_cast<float*>(v.take((size_t)rows * c.qk_nope_head_dim * sizeof(float)));
+    if (!rope_as_is) t.q_rope = static_cast<float*>(v.take((size_t)rows * c.qk_rope_head_dim * sizeof(float)));
+    if (mfma) {
+      step_ws = v.take(step_bytes);
+      if (!join && a->out_dtype != LA_DTYPE_F32) out32 = static_cast<float*>(v.take((size_t)rows * c.v_head_dim * sizeof(float)));
+    } else {
+      q_abs = static_cast<float*>(v.take((size_t)rows * c.kv_lora_rank * sizeof(float)));
+    }
+    return v.total();
+  };
+  const size_t total = carve(nullptr);
+  if (need) *need = total;
+  if (!run_it) return LA_SUCCESS;
+  Scratch scratch(a->workspace, a->workspace_bytes, total, stream);
+  if (scratch.status != LA_SUCCESS) return scratch.status;
+  carve(scratch.ws);
+
+  t.parents = a->parents;
+  t.nh = nh;
+  t.dn = c.qk_nope_head_dim;
+  t.dR = c.qk_rope_head_dim;
+  t.vec = queries_vec(t.q);
+  hipError_t e = launch_tree_queries(t, stream);
+  if (e != hipSuccess) return scratch.finish(record_hip(e));
+  const float* const qn = nope_as_is ? static_cast<const float*>(a->q_nope) : t.q_nope;
+  const float* const qr = rope_as_is ? static_cast<const float*>(a->q_rope) : t.q_rope;
+  if (!mfma) {
+    const int st = la_absorb_q(qn, a->W_UK, a->w_uk_dtype, q_abs, (int)tokens, &c, stream_v);
+    if (st != LA_SUCCESS) return scratch.finish(st);
+    PlainTree p{};
+    p.src = t.src;
+    p.src.lens = t.lens;
+    p.seen = t.seen;
+    p.nodes = n;
+    p.q_abs = q_abs;
+    p.q_rope = qr;
+    p.W_UV = a->W_UV;
+    p.wuv_dtype = a->w_uv_dtype;
+    p.nh = nh;
+    p.dc = c.kv_lora_rank;
+    p.dR = c.qk_rope_head_dim;
+    p.dv = c.v_head_dim;
+    p.scale_log2 = (float)(kLog2e / std::sqrt((double)(c.qk_nope_head_dim + c.qk_rope_head_dim)));
+    p.out = a->output;
+    p.out_dtype = a->out_dtype;
+    return scratch.finish(status_of(launch_plain_tree(p, stream)));
+  }
+  d.seq_lens = t.lens;
+  d.q_nope = qn;
+  d.q_rope = qr;
+  d.output = out32 ? out32 : static_cast<float*>(a->output);  // (join: the step leaves it alone)
+  d.workspace = step_ws;
+  d.workspace_bytes = step_bytes;
+  StepTail tail;
+  tail.merge = !join;
+  tail.tree = TreeStep{t.seen, t.cos, t.sin};
+  int st = run(&d, stream, nullptr, nullptr, 1, false, &tail);
+  if (st == LA_SUCCESS && join) {
+    JoinProblem j{};
+    j.rows = rows;
+    j.nh = nh;
+    j.dv = c.v_head_dim;
+    j.step[0] = tail.p;
+    j.out = a->output;
+    j.out_dtype = a->out_dtype;
+    st = status_of(launch_merge_join(j, stream, cu_count()));
+  }
+  if (st == LA_SUCCESS && out32) st = status_of(launch_cast(out32, a->output, a->out_dtype, rows * c.v_head_dim, stream));
+  return scratch.finish(st);
+}
+
+// Cache and sequences of la_accept_args and la_evict_args: as la_append_kv's.
+template <typename Args>
+bool moved_rows(const Args* a, MovedRows* out) {
+  if (!valid_cfg(&a->cfg) || !valid_cache_dtype(a->kv_dtype) || a->num_seqs < 0 || a->total_rows < 0) return false;
+  const bool paged = a->block_table != nullptr;
+  if (paged) {
+    if (a->block_size <= 0 || a->blocks_per_seq <= 0 || a->seq_offsets || a->total_rows % a->block_size != 0 ||
+        (int64_t)a->blocks_per_seq * a->block_size > INT32_MAX || (a->num_seqs > 0 && a->total_rows < a->block_size))
+      return false;
+  } else if (a->seq_offsets) {
+    if (a->total_rows > INT32_MAX) return false;
+  } else if (a->seq_capacity < 0 || (int64_t)a->num_seqs * a->seq_capacity > a->total_rows) {
+    return false;
+  }
+  if (a->num_seqs > 0 && (!a->seq_lens || (a->total_rows > 0 && !a->kv_cache))) return false;
+  const int64_t row = (int64_t)a->cfg.kv_lora_rank + a->cfg.qk_rope_head_dim;
+  if (row > INT32_MAX / 4) return false;
+  MovedRows r{};
+  r.kv = static_cast<char*>(a->kv_cache);
+  r.row_bytes = row * (a->kv_dtype == LA_DTYPE_F32 ? 4 : a->kv_dtype == LA_DTYPE_FP8_E4M3 ? 1 : 2);
+  r.total_rows = a->total_rows;
+  r.num_seqs = a->num_seqs;
+  r.region = paged ? a->blocks_per_seq * a->block_size : a->seq_offsets ? 0 : a->seq_capacity;
+  r.offsets = a->seq_offsets;
+  r.lens = a->seq_lens;
+  if (paged) {
+    r.block_table = a->block_table;
+    r.block_size = a->block_size;
+    r.blocks_per_seq = a->blocks_per_seq;
+    r.pool_blocks = a->total_rows / a->block_size;
+  }
+  *out = r;
+  return true;
+}
+
+int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
+  const hipStream_t stream = static_cast<hipStream_t>(stream_v);
+  if (!a || !valid_cfg(&a->cfg) || !valid_cache_dtype(a->kv_dtype) || !valid_dtype(a->w_uk_dtype) ||
+      a->tokens_per_seq < 0 || a->kernel_variant < 0 || a->kernel_variant > 2)
+    return LA_ERROR_INVALID_VALUE;
+  const la_mla_config& c = a->cfg;
+  const int nh = c.num_heads, n = a->tokens_per_seq;
+  WeighProblem p{};
+  QuerySource q{};
+  if (!row_source(a, &p.src) || !query_source(a, n, &q)) return LA_ERROR_INVALID_VALUE;
+  if (need) *need = 0;
+  if (a->num_seqs == 0 || n == 0) return LA_SUCCESS;
+  if (!a->weights || !a->q_nope || !a->q_rope || !a->W_UK || !a->rope_cos || !a->rope_sin ||
+      (a->total_rows > 0 && !a->kv_cache))
+    return LA_ERROR_INVALID_VALUE;
+  if (a->kernel_variant == 2 || !generic_prompt_supported(c.kv_lora_rank, c.qk_rope_head_dim)) return LA_ERROR_NOT_SUPPORTED;
+  const int64_t rows = q.tokens * nh;
+  const bool nope_as_is = packed_f32(q.q_nope, q.dtype, q.nope_stride, q.nope_head, nh, c.qk_nope_head_dim);
+  const bool rope_as_is = !a->rotate_q && packed_f32(q.q_rope, q.dtype, q.rope_stride, q.rope_head, nh, c.qk_rope_head_dim);
+  TokenProblem t{};
+  float* q_abs = nullptr;
+  auto carve = [&](void* ws) {
+    Carve v(ws);
+    if (!nope_as_is) t.q_nope = static_cast<float*>(v.take((size_t)rows * c.qk_nope_head_dim * sizeof(float)));
+    if (!rope_as_is) t.q_rope = static_cast<float*>(v.take((size_t)rows * c.qk_rope_head_dim * sizeof(float)));
+    q_abs = static_cast<float*>(v.take((size_t)rows * c.kv_lora_rank * sizeof(float)));
+    p.lse = static_cast<float*>(v.take((size_t)rows * sizeof(float)));
+    return v.total();
+  };
+  const size_t total = carve(nullptr);
+  if (need) *need = total;
+  if (!run_it) return LA_SUCCESS;
+  Scratch scratch(a->workspace, a->workspace_bytes, total, stream);
+  if (scratch.status != LA_SUCCESS) return scratch.status;
+  carve(scratch.ws);
+  t.q = q;
+  t.src = p.src;
+  t.nh = nh;
+  t.dn = c.qk_nope_head_dim;
+  t.dR = c.qk_rope_head_dim;
+  t.vec = queries_vec(q);
+  if (t.q_nope || t.q_rope) {
+    const hipError_t e = launch_tokens(t, stream);
+    if (e != hipSuccess) return scratch.finish(record_hip(e));
+  }
+  const int st = la_absorb_q(nope_as_is ? static_cast<const float*>(a->q_nope) : t.q_nope, a->W_UK, a->w_uk_dtype, q_abs,
+                             (int)q.tokens, &c, stream_v);
+  if (st != LA_SUCCESS) return scratch.finish(st);
+  p.tokens = n;
+  p.nh = nh;
+  p.dc = c.kv_lora_rank;
+  p.dR = c.qk_rope_head_dim;
+  p.q_abs = q_abs;
+  p.q_rope = rope_as_is ? static_cast<const float*>(a->q_rope) : t.q_rope;
+  p.scale_log2 = (float)(kLog2e / std::sqrt((double)(c.qk_nope_head_dim + c.qk_rope_head_dim)));
+  p.weights = a->weights;
+  return scratch.finish(status_of(launch_weigh_plain(p, stream)));
+}
+
+int evict(const la_evict_args* a, hipStream_t stream, bool run_it, size_t* need) {
+  EvictProblem p{};
+  if (!a || !moved_rows(a, &p.rows) || a->keep < 0 || a->first < 0 || a->last < 0 ||
+      (int64_t)a->first + a->last > a->keep || (a->num_seqs > 0 && a->total_rows > 0 && !a->weights))
+    return LA_ERROR_INVALID_VALUE;
+  if (need) *need = 0;
+  if (a->num_seqs == 0) return LA_SUCCESS;
+  p.weights = a->weights;
+  p.keep = a->keep;
+  p.first = a->first;
+  p.last = a->last;
+  auto carve = [&](void* ws) {
+    Carve v(ws);
+    p.start = static_cast<int32_t*>(v.take((size_t)a->num_seqs * sizeof(int32_t)));
+    p.kept = a->kept ? a->kept : static_cast<int32_t*>(v.take((size_t)a->num_seqs * a->keep * sizeof(int32_t)));
+    return v.total();
+  };
+  const size_t total = carve(nullptr);
+  if (need) *need = total;
+  if (!run_it) return LA_SUCCESS;
+  Scratch scratch(a->workspace, a->workspace_bytes, total, stream);
+  if (scratch.status != LA_SUCCESS) return scratch.status;
+  carve(scratch.ws);
+  return scratch.finish(status_of(launch_evict(p, stream)));
+}
+
 }  // namespace
 }  // namespace la
 
@@ -1546,6 +1875,39 @@ int la_mla_decode_shared(const la_shared_args* args, void* stream) {
 size_t la_mla_decode_shared_workspace_size(const la_shared_args* args) {
   size_t need = 0;
   return la::decode_shared(args, nullptr, false, &need) == LA_SUCCESS ? need : 0;
+}
+
+int la_mla_decode_tree(const la_tree_args* args, void* stream) { return la::decode_tree(args, stream, true, nullptr); }
+
+size_t la_mla_decode_tree_workspace_size(const la_tree_args* args) {
+  size_t need = 0;
+  return la::decode_tree(args, nullptr, false, &need) == LA_SUCCESS ? need : 0;
+}
+
+int la_accept_kv(const la_accept_args* args, void* stream) {
+  la::AcceptProblem p{};
+  if (!args || !la::moved_rows(args, &p.rows) || args->nodes < 1 || args->nodes > la::kTreeNodes) return LA_ERROR_INVALID_VALUE;
+  if (args->num_seqs == 0) return LA_SUCCESS;
+  if (!args->path) return LA_ERROR_INVALID_VALUE;
+  p.nodes = args->nodes;
+  p.path = args->path;
+  return la::status_of(la::launch_accept(p, static_cast<hipStream_t>(stream)));
+}
+
+int la_weigh_kv(const la_weigh_args* args, void* stream) { return la::weigh(args, stream, true, nullptr); }
+
+size_t la_weigh_kv_workspace_size(const la_weigh_args* args) {
+  size_t need = 0;
+  return la::weigh(args, nullptr, false, &need) == LA_SUCCESS ? need : 0;
+}
+
+int la_evict_kv(const la_evict_args* args, void* stream) {
+  return la::evict(args, static_cast<hipStream_t>(stream), true, nullptr);
+}
+
+size_t la_evict_kv_workspace_size(const la_evict_args* args) {
+  size_t need = 0;
+  return la::evict(args, nullptr, false, &need) == LA_SUCCESS ? need : 0;
 }
 
 }  // extern "C"

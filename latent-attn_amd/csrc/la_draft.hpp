@@ -1,0 +1,116 @@
+// Types shared by the draft-tree and cache-cutting kernels (la_tree.hip,
+// la_weigh.hip, la_evict.hip) and the C-ABI layer. Not installed.
+#pragma once
+
+#include "la_prompt.hpp"
+
+namespace la {
+
+constexpr int kTreeNodes = LA_TREE_MAX_NODES;
+static_assert(kTreeNodes == 64, "a node's ancestors are the bits of one word, a tree's nodes the lanes of one wave");
+
+// Trees as the attention kernels take them, and packed fp32 queries, rotated by
+// their nodes' positions if asked (launch_tree_queries).
+struct TreeQueries {
+  QuerySource q;  // offsets nullptr, per_seq nodes
+  RowSource src;
+  const int32_t* parents;  // (num_seqs, nodes)
+  int nh, dn, dR;
+  float* q_nope;   // (tokens, nh, dn), or nullptr
+  float* q_rope;   // (tokens, nh, dR), or nullptr
+  int32_t* lens;   // (num_seqs): rows, 0 where they are fewer than the nodes
+  uint64_t* seen;  // TreeStep
+  float* cos;
+  float* sin;
+  int vec;  // queries are whole-vector aligned
+};
+hipError_t launch_tree_queries(const TreeQueries& p, hipStream_t stream);
+
+// Any type and head shape: absorbed fp32 queries, one workgroup per (token, head).
+struct PlainTree {
+  RowSource src;  // with TreeQueries' lens
+  const uint64_t* seen;
+  int nodes;
+  const float* q_abs;
+  const float* q_rope;  // rotated
+  const void* W_UV;
+  int wuv_dtype;
+  int nh, dc, dR, dv;
+  float scale_log2;
+  void* out;
+  int out_dtype;
+};
+hipError_t launch_plain_tree(const PlainTree& p, hipStream_t stream);
+
+// A cache whose rows move within their sequences.
+struct MovedRows {
+  char* kv;
+  int64_t row_bytes;
+  int64_t total_rows;
+  int num_seqs;
+  int region;              // rows of a sequence at most (offsets == nullptr)
+  const int32_t* offsets;  // device, num_seqs + 1, or nullptr
+  int32_t* lens;           // device, num_seqs
+  const int32_t* block_table;
+  int block_size;
+  int blocks_per_seq;
+  int64_t pool_blocks;
+};
+// First row of sequence s in the row space of the sequences, and the rows it has room for.
+__device__ inline int64_t moved_begin(const MovedRows& r, int s) {
+  return r.offsets ? clamp64(r.offsets[s], 0, r.total_rows) : (int64_t)s * r.region;
+}
+__device__ inline int moved_room(const MovedRows& r, int s) {
+  if (!r.offsets) return r.region;
+  return (int)max(clamp64(r.offsets[s + 1], 0, r.total_rows) - moved_begin(r, s), (int64_t)0);
+}
+// Row of position pos, which lies in the sequence's room (block ids are clamped into the pool).
+__device__ inline char* moved_row(const MovedRows& r, int s, int64_t begin, int pos) {
+  int64_t row = begin + pos;
+  if (r.block_table) {
+    const int64_t b = clamp64(r.block_table[(int64_t)s * r.blocks_per_seq + pos / r.block_size], 0, r.pool_blocks - 1);
+    row = b * r.block_size + pos % r.block_size;
+  }
+  return r.kv + row * r.row_bytes;
+}
+// Between the reads of rows that move and the barrier after which others write there: the
+// barrier alone does not wait for loads.
+__device__ inline void rows_read() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// The widest accesses that rows and the cache's address allow: 16, 8, 4, 2 or 1 bytes.
+inline int moved_unit(const MovedRows& r) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(r.kv) | (uintptr_t)r.row_bytes | 16;
+  return (int)(a & -a);
+}
+
+// la_accept_kv.
+struct AcceptProblem {
+  MovedRows rows;
+  int nodes;
+  const int32_t* path;  // (num_seqs, nodes)
+};
+hipError_t launch_accept(const AcceptProblem& p, hipStream_t stream);
+
+// la_weigh_kv: packed fp32 queries (q_rope rotated), q.per_seq tokens each.
+struct WeighProblem {
+  RowSource src;
+  int tokens;  // of every sequence
+  int nh, dc, dR;
+  const float* q_abs;   // (num_seqs * tokens, nh, dc)
+  const float* q_rope;  // (num_seqs * tokens, nh, dR)
+  float scale_log2;
+  float* weights;
+  float* lse;  // (num_seqs * tokens, nh), base 2
+};
+hipError_t launch_weigh_plain(const WeighProblem& p, hipStream_t stream);
+
+// la_evict_kv.
+struct EvictProblem {
+  MovedRows rows;
+  float* weights;
+  int keep, first, last;
+  int32_t* kept;   // (num_seqs, keep)
+  int32_t* start;  // (num_seqs): the first position that changes rows, keep if none does
+};
+hipError_t launch_evict(const EvictProblem& p, hipStream_t stream);
+
+}  // namespace la

@@ -584,6 +584,15 @@ bool absorb_f32_supported(const void* q_nope, const void* W_UK, int w_dtype, con
 hipError_t launch_absorb_f32(const float* q_nope, const void* W_UK, float* q_abs, int tokens, int nh, int dn, int dc,
                              hipStream_t stream);
 
+// A decode step over trees of drafted tokens (la_mla_decode_tree): query token j
+// of a sequence (qps of them) is node j, the sequence's last qps rows are the
+// nodes' own.
+struct TreeStep {
+  const uint64_t* seen;  // (num_seqs, qps): bit i of node j: node i is j or an ancestor; nullptr: no trees
+  const float* cos;      // (num_seqs, qps, dR / 2): the tables' rows of the nodes' positions
+  const float* sin;
+};
+
 // MFMA split-KV decode for 16-bit and FP8 E4M3 caches with kv_lora_rank 512,
 // qk_rope_head_dim 64.
 // ev_begin / ev_end (optional) are recorded at the kernel's start and end.

@@ -159,6 +159,119 @@ class SharedArgs(ctypes.Structure):
     ]
 
 
+class TreeArgs(ctypes.Structure):
+    _fields_ = [
+        ("kv_cache", ctypes.c_void_p),
+        ("kv_dtype", ctypes.c_int32),
+        ("total_rows", ctypes.c_int64),
+        ("num_seqs", ctypes.c_int32),
+        ("seq_len", ctypes.c_int32),
+        ("seq_offsets", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("block_size", ctypes.c_int32),
+        ("blocks_per_seq", ctypes.c_int32),
+        ("nodes", ctypes.c_int32),
+        ("parents", ctypes.c_void_p),
+        ("q_nope", ctypes.c_void_p),
+        ("q_rope", ctypes.c_void_p),
+        ("q_dtype", ctypes.c_int32),
+        ("q_nope_token_stride", ctypes.c_int64),
+        ("q_nope_head_stride", ctypes.c_int64),
+        ("q_rope_token_stride", ctypes.c_int64),
+        ("q_rope_head_stride", ctypes.c_int64),
+        ("rotate_q", ctypes.c_int32),
+        ("W_UK", ctypes.c_void_p),
+        ("w_uk_dtype", ctypes.c_int32),
+        ("W_UV", ctypes.c_void_p),
+        ("w_uv_dtype", ctypes.c_int32),
+        ("rope_cos", ctypes.c_void_p),
+        ("rope_sin", ctypes.c_void_p),
+        ("rope_rows", ctypes.c_int64),
+        ("output", ctypes.c_void_p),
+        ("out_dtype", ctypes.c_int32),
+        ("cfg", MlaConfig),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("kernel_variant", ctypes.c_int32),
+    ]
+
+
+class AcceptArgs(ctypes.Structure):
+    _fields_ = [
+        ("kv_cache", ctypes.c_void_p),
+        ("kv_dtype", ctypes.c_int32),
+        ("total_rows", ctypes.c_int64),
+        ("num_seqs", ctypes.c_int32),
+        ("seq_capacity", ctypes.c_int32),
+        ("seq_offsets", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("block_size", ctypes.c_int32),
+        ("blocks_per_seq", ctypes.c_int32),
+        ("nodes", ctypes.c_int32),
+        ("path", ctypes.c_void_p),
+        ("cfg", MlaConfig),
+    ]
+
+
+class WeighArgs(ctypes.Structure):
+    _fields_ = [
+        ("kv_cache", ctypes.c_void_p),
+        ("kv_dtype", ctypes.c_int32),
+        ("total_rows", ctypes.c_int64),
+        ("num_seqs", ctypes.c_int32),
+        ("seq_len", ctypes.c_int32),
+        ("seq_offsets", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("block_size", ctypes.c_int32),
+        ("blocks_per_seq", ctypes.c_int32),
+        ("tokens_per_seq", ctypes.c_int32),
+        ("q_nope", ctypes.c_void_p),
+        ("q_rope", ctypes.c_void_p),
+        ("q_dtype", ctypes.c_int32),
+        ("q_nope_token_stride", ctypes.c_int64),
+        ("q_nope_head_stride", ctypes.c_int64),
+        ("q_rope_token_stride", ctypes.c_int64),
+        ("q_rope_head_stride", ctypes.c_int64),
+        ("rotate_q", ctypes.c_int32),
+        ("W_UK", ctypes.c_void_p),
+        ("w_uk_dtype", ctypes.c_int32),
+        ("rope_cos", ctypes.c_void_p),
+        ("rope_sin", ctypes.c_void_p),
+        ("rope_rows", ctypes.c_int64),
+        ("weights", ctypes.c_void_p),
+        ("cfg", MlaConfig),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("kernel_variant", ctypes.c_int32),
+    ]
+
+
+class EvictArgs(ctypes.Structure):
+    _fields_ = [
+        ("kv_cache", ctypes.c_void_p),
+        ("kv_dtype", ctypes.c_int32),
+        ("total_rows", ctypes.c_int64),
+        ("num_seqs", ctypes.c_int32),
+        ("seq_capacity", ctypes.c_int32),
+        ("seq_offsets", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("block_size", ctypes.c_int32),
+        ("blocks_per_seq", ctypes.c_int32),
+        ("weights", ctypes.c_void_p),
+        ("keep", ctypes.c_int32),
+        ("first", ctypes.c_int32),
+        ("last", ctypes.c_int32),
+        ("kept", ctypes.c_void_p),
+        ("cfg", MlaConfig),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class PlanInfo(ctypes.Structure):
     _fields_ = [
         ("attention", ctypes.c_int32),
@@ -229,11 +342,14 @@ def load() -> ctypes.CDLL:
     lib.la_naive_mla_workspace_size.argtypes = [i32, cfgp]
     lib.la_append_kv.restype = i32
     lib.la_append_kv.argtypes = [ctypes.POINTER(AppendArgs), vp]
-    for name, args in (("la_mla_prefill", PrefillArgs), ("la_expand_prefix", ExpandArgs), ("la_mla_decode_shared", SharedArgs)):
+    for name, args in (("la_mla_prefill", PrefillArgs), ("la_expand_prefix", ExpandArgs), ("la_mla_decode_shared", SharedArgs),
+                       ("la_mla_decode_tree", TreeArgs), ("la_weigh_kv", WeighArgs), ("la_evict_kv", EvictArgs)):
         getattr(lib, name).restype = i32
         getattr(lib, name).argtypes = [ctypes.POINTER(args), vp]
         getattr(lib, name + "_workspace_size").restype = sz
         getattr(lib, name + "_workspace_size").argtypes = [ctypes.POINTER(args)]
+    lib.la_accept_kv.restype = i32
+    lib.la_accept_kv.argtypes = [ctypes.POINTER(AcceptArgs), vp]
     lib.la_expanded_size.restype = sz
     lib.la_expanded_size.argtypes = [ctypes.c_int32, cfgp]
     _lib = lib

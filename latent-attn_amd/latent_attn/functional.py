@@ -6,7 +6,9 @@ Same entry points and argument order as the reference
 ragged caches with query absorption, split-KV and the W_UV projection in one
 call) and ``absorb_q``; ``append_kv``; ``mla_prefill`` (several new tokens per
 sequence: prompts, chunks, drafted tokens), ``expand_prefix`` and
-``mla_decode_shared`` (decode behind one prefix of the whole batch). All compute runs in the HIP library; nothing here
+``mla_decode_shared`` (decode behind one prefix of the whole batch);
+``mla_decode_tree`` (trees of drafted tokens) and ``accept_kv``; ``weigh_kv`` and
+``evict_kv`` (caches cut back to the rows that attention uses). All compute runs in the HIP library; nothing here
 falls back to PyTorch math -- if the extension is missing, the call raises.
 """
 
@@ -385,3 +387,154 @@ def mla_decode_shared(
     return _C.mla_decode_shared_forward(prefix, expanded, kv_cache, q_nope, q_rope, W_UK, W_UV, rope_cos, rope_sin,
                                         seq_offsets, *_cfg_args(cfg), seq_lens, block_table, block_size, out_dtype,
                                         kernel_variant)
+
+
+def mla_decode_tree(
+    kv_cache: torch.Tensor,
+    q_nope: torch.Tensor,
+    q_rope: torch.Tensor,
+    W_UK: torch.Tensor,
+    W_UV: torch.Tensor,
+    rope_cos: torch.Tensor,
+    rope_sin: torch.Tensor,
+    cfg: "MLAConfig",
+    parents: torch.Tensor,
+    seq_offsets: Optional[torch.Tensor] = None,
+    seq_lens: Optional[torch.Tensor] = None,
+    block_table: Optional[torch.Tensor] = None,
+    block_size: int = 0,
+    rotate_q: bool = False,
+    out_dtype: Optional[torch.dtype] = None,
+    kernel_variant: int = 0,
+) -> torch.Tensor:
+    """Attention of a tree of drafted tokens per sequence, to check many
+    continuations at once.
+
+    The nodes' rows are in the cache (``append_kv`` with as many tokens) and
+    are each sequence's last, in the nodes' order. Node j of n of a sequence
+    with L rows is at position L - n + its depth, and so is its key; it sees the
+    first L - n rows, its ancestors and itself. ``accept_kv`` afterwards keeps
+    the rows of the path that was accepted.
+
+    Args:
+        kv_cache, seq_offsets, seq_lens, block_table, block_size: as in
+                     ``mla_prefill``
+        q_nope, q_rope: (batch * nodes, num_heads, .), as in ``mla_prefill``:
+                     any type, strided views; up to 64 nodes per sequence
+        parents:     int32 (batch, nodes) device tensor: every node's parent, a
+                     node before it, or -1 (as anything else counts): it follows
+                     the last row before the nodes'. Sequences that draft fewer
+                     nodes pad theirs with any: nothing sees a node but its
+                     descendants. A sequence with fewer rows than nodes has no
+                     tree: its tokens get zeros.
+        rotate_q:    q_rope is not rotated yet: rotated on the way by its
+                     node's position (the tensor is left as it is)
+        out_dtype:   fp32 / fp16 / bf16; None: the queries' type
+        kernel_variant: 0 = automatic, 1 = plain kernel, 2 = matrix cores
+
+    Returns:
+        (batch * nodes, num_heads, v_head_dim) in out_dtype
+    """
+    _C = _load_ext()
+    return _C.mla_decode_tree_forward(kv_cache, q_nope, q_rope, W_UK, W_UV, rope_cos, rope_sin, parents, seq_offsets,
+                                      *_cfg_args(cfg), seq_lens, block_table, block_size, rotate_q,
+                                      q_nope.dtype if out_dtype is None else out_dtype, kernel_variant)
+
+
+def accept_kv(
+    kv_cache: torch.Tensor,
+    seq_lens: torch.Tensor,
+    nodes: int,
+    path: torch.Tensor,
+    cfg: "MLAConfig",
+    seq_offsets: Optional[torch.Tensor] = None,
+    block_table: Optional[torch.Tensor] = None,
+    block_size: int = 0,
+) -> None:
+    """Keeps the rows of a tree's accepted path: they become the sequence's
+    last ones, the tree's others are dropped.
+
+    Args:
+        kv_cache, seq_offsets, block_table, block_size: as in ``append_kv``
+        seq_lens:    int32 (batch,) device tensor: the rows with the trees'
+                     among them; set in place to those that stay. A sequence with
+                     fewer than ``nodes`` is left unchanged.
+        nodes:       rows of each tree, 1 to 64
+        path:        int32 (batch, nodes) device tensor: the accepted nodes from
+                     the top down, ended by -1 (or anything that is not a later
+                     node than the one before it)
+    """
+    _C = _load_ext()
+    _C.accept_kv_forward(kv_cache, seq_lens, nodes, path, seq_offsets, *_cfg_args(cfg), block_table, block_size)
+
+
+def weigh_kv(
+    weights: torch.Tensor,
+    kv_cache: torch.Tensor,
+    q_nope: torch.Tensor,
+    q_rope: torch.Tensor,
+    W_UK: torch.Tensor,
+    rope_cos: torch.Tensor,
+    rope_sin: torch.Tensor,
+    cfg: "MLAConfig",
+    seq_offsets: Optional[torch.Tensor] = None,
+    seq_lens: Optional[torch.Tensor] = None,
+    block_table: Optional[torch.Tensor] = None,
+    block_size: int = 0,
+    rotate_q: bool = False,
+    kernel_variant: int = 0,
+) -> None:
+    """Adds to every cache row's weight the attention that the newest tokens
+    pay it, summed over them and all heads: what ``evict_kv`` goes by. Called
+    with every decode step's queries, or with those of a prompt's last tokens.
+
+    Args:
+        weights:     float32 device tensor, changed in place: (batch, capacity),
+                     (batch, blocks_per_seq * block_size) for a paged cache,
+                     (total_rows,) with ``seq_offsets``. Entries past a
+                     sequence's rows are left as they are (rows appended later
+                     start at what these hold: zeros).
+        kv_cache, seq_offsets, seq_lens, block_table, block_size: as in
+                     ``mla_prefill``
+        q_nope, q_rope: (batch * n, num_heads, .), as in ``mla_prefill``, of the
+                     sequences' last n rows: token j of n of a sequence with L
+                     rows is at position L - n + j and sees the rows up to its own
+        rotate_q:    q_rope is not rotated yet
+        kernel_variant: 0 = automatic, 1 = plain kernels, 2 = matrix cores
+    """
+    _C = _load_ext()
+    _C.weigh_kv_forward(weights, kv_cache, q_nope, q_rope, W_UK, rope_cos, rope_sin, seq_offsets, *_cfg_args(cfg),
+                        seq_lens, block_table, block_size, rotate_q, kernel_variant)
+
+
+def evict_kv(
+    kv_cache: torch.Tensor,
+    seq_lens: torch.Tensor,
+    weights: torch.Tensor,
+    cfg: "MLAConfig",
+    keep: int,
+    first: int = 0,
+    last: int = 0,
+    seq_offsets: Optional[torch.Tensor] = None,
+    block_table: Optional[torch.Tensor] = None,
+    block_size: int = 0,
+) -> torch.Tensor:
+    """Cuts every sequence with more than ``keep`` rows back to that many, in
+    place: its first ``first`` and last ``last`` rows and, of those between, the
+    ones with the largest weights (of equal ones the earlier; NaN counts as the
+    smallest). Rows keep their order and move to the front with their weights;
+    their positions, for RoPE too, are then their places in the cache, as
+    everywhere. In a paged cache the blocks past ``keep`` are free afterwards.
+
+    Args:
+        kv_cache, seq_offsets, block_table, block_size: as in ``append_kv``
+        seq_lens:    int32 (batch,) device tensor, set in place
+        weights:     as in ``weigh_kv``; those behind the kept rows are zeroed
+
+    Returns:
+        int32 (batch, keep): the rows' positions before the call, -1 past a
+        shorter sequence's rows
+    """
+    _C = _load_ext()
+    return _C.evict_kv_forward(kv_cache, seq_lens, weights, keep, first, last, seq_offsets, *_cfg_args(cfg),
+                               block_table, block_size)
