@@ -1463,6 +1463,9 @@ bool moved_rows(const Args* a, MovedRows* out) {
   return true;
 }
 
+// Scores that weigh_kv keeps at once.
+constexpr size_t kMostScores = (size_t)512 << 20;
+
 int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
   const hipStream_t stream = static_cast<hipStream_t>(stream_v);
   if (!a || !valid_cfg(&a->cfg) || !valid_cache_dtype(a->kv_dtype) || !valid_dtype(a->w_uk_dtype) ||
@@ -1478,7 +1481,30 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
   if (!a->weights || !a->q_nope || !a->q_rope || !a->W_UK || !a->rope_cos || !a->rope_sin ||
       (a->total_rows > 0 && !a->kv_cache))
     return LA_ERROR_INVALID_VALUE;
-  if (a->kernel_variant == 2 || !generic_prompt_supported(c.kv_lora_rank, c.qk_rope_head_dim)) return LA_ERROR_NOT_SUPPORTED;
+  p.tokens = n;
+  p.nh = nh;
+  p.dc = c.kv_lora_rank;
+  p.dR = c.qk_rope_head_dim;
+  p.weights = a->weights;
+  p.scale_log2 = (float)(kLog2e / std::sqrt((double)(c.qk_nope_head_dim + c.qk_rope_head_dim)));
+  const int64_t seq_tiles = ((int64_t)p.src.region + kWeighKeys - 1) / kWeighKeys;
+  const int64_t all_tiles = a->seq_offsets ? a->total_rows / kWeighKeys + a->num_seqs : seq_tiles * a->num_seqs;
+  const bool mfma = a->kernel_variant != 1 && weigh_mfma_supported(p) && all_tiles <= INT32_MAX / kWeighKeys;
+  if (!mfma && (a->kernel_variant == 2 || !generic_prompt_supported(c.kv_lora_rank, c.qk_rope_head_dim))) return LA_ERROR_NOT_SUPPORTED;
+  // The matrix form keeps the scores between its two kernels: pieces of the call, tokens and
+  // then sequences at a time (packed ones, whose lengths only the device knows, all together).
+  int64_t most_tiles = 0;
+  if (mfma) {
+    p.count = std::max(1, std::min(n, kWeighRows / nh));
+    p.seqs = a->num_seqs;
+    if (!a->seq_offsets && seq_tiles > 0) {
+      const size_t one = weigh_score_bytes(seq_tiles, p.count * nh);
+      p.seqs = (int)std::max<int64_t>(1, std::min<int64_t>(p.seqs, kMostScores / one));
+    }
+    most_tiles = a->seq_offsets ? all_tiles : seq_tiles * p.seqs;
+    while (p.count > 1 && weigh_score_bytes(most_tiles, p.count * nh) > kMostScores) p.count = (p.count + 1) / 2;
+    p.spans = weigh_spans(p.count * nh, cu_count());
+  }
   const int64_t rows = q.tokens * nh;
   const bool nope_as_is = packed_f32(q.q_nope, q.dtype, q.nope_stride, q.nope_head, nh, c.qk_nope_head_dim);
   const bool rope_as_is = !a->rotate_q && packed_f32(q.q_rope, q.dtype, q.rope_stride, q.rope_head, nh, c.qk_rope_head_dim);
@@ -1489,7 +1515,12 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
     if (!nope_as_is) t.q_nope = static_cast<float*>(v.take((size_t)rows * c.qk_nope_head_dim * sizeof(float)));
     if (!rope_as_is) t.q_rope = static_cast<float*>(v.take((size_t)rows * c.qk_rope_head_dim * sizeof(float)));
     q_abs = static_cast<float*>(v.take((size_t)rows * c.kv_lora_rank * sizeof(float)));
-    p.lse = static_cast<float*>(v.take((size_t)rows * sizeof(float)));
+    if (mfma) {
+      p.scores = static_cast<float*>(v.take(weigh_score_bytes(most_tiles, p.count * nh)));
+      p.part = static_cast<float*>(v.take(weigh_part_bytes(p.spans, p.seqs, p.count * nh)));
+    } else {
+      p.lse = static_cast<float*>(v.take((size_t)rows * sizeof(float)));
+    }
     return v.total();
   };
   const size_t total = carve(nullptr);
@@ -1511,15 +1542,20 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
   const int st = la_absorb_q(nope_as_is ? static_cast<const float*>(a->q_nope) : t.q_nope, a->W_UK, a->w_uk_dtype, q_abs,
                              (int)q.tokens, &c, stream_v);
   if (st != LA_SUCCESS) return scratch.finish(st);
-  p.tokens = n;
-  p.nh = nh;
-  p.dc = c.kv_lora_rank;
-  p.dR = c.qk_rope_head_dim;
   p.q_abs = q_abs;
   p.q_rope = rope_as_is ? static_cast<const float*>(a->q_rope) : t.q_rope;
-  p.scale_log2 = (float)(kLog2e / std::sqrt((double)(c.qk_nope_head_dim + c.qk_rope_head_dim)));
-  p.weights = a->weights;
-  return scratch.finish(status_of(launch_weigh_plain(p, stream)));
+  if (!mfma) return scratch.finish(status_of(launch_weigh_plain(p, stream)));
+  hipError_t e = hipSuccess;
+  const int most_seqs = p.seqs, most_count = p.count;
+  for (int j = 0; j < n && most_tiles > 0; j += most_count)
+    for (int s = 0; s < a->num_seqs && e == hipSuccess; s += most_seqs) {
+      p.token0 = j;
+      p.count = std::min(most_count, n - j);
+      p.seq0 = s;
+      p.seqs = std::min(most_seqs, a->num_seqs - s);
+      e = launch_weigh_mfma(p, a->seq_offsets ? all_tiles : seq_tiles * p.seqs, stream, cu_count());
+    }
+  return scratch.finish(status_of(e));
 }
 
 int evict(const la_evict_args* a, hipStream_t stream, bool run_it, size_t* need) {

@@ -90,7 +90,7 @@ struct AcceptProblem {
 };
 hipError_t launch_accept(const AcceptProblem& p, hipStream_t stream);
 
-// la_weigh_kv: packed fp32 queries (q_rope rotated), q.per_seq tokens each.
+// la_weigh_kv: packed fp32 queries (q_rope rotated), tokens per sequence.
 struct WeighProblem {
   RowSource src;
   int tokens;  // of every sequence
@@ -99,9 +99,25 @@ struct WeighProblem {
   const float* q_rope;  // (num_seqs * tokens, nh, dR)
   float scale_log2;
   float* weights;
-  float* lse;  // (num_seqs * tokens, nh), base 2
+  float* lse;  // plain form: (num_seqs * tokens, nh), base 2
+  // matrix form: one piece of the call, `seqs` sequences from seq0 on and of
+  // each `count` tokens from token0 on
+  int seq0, seqs, token0, count;
+  int spans;       // workgroups that share the tiles of a row group
+  float* scores;   // [tile][32 rows][32 keys] of `row_blocks` blocks per tile
+  float* part;     // [slot][m, l][rows rounded up to 32]
 };
 hipError_t launch_weigh_plain(const WeighProblem& p, hipStream_t stream);
+// The matrix form: 16-bit and FP8 rows of 512 + 64 elements. A piece's workspace goes
+// by the tiles (of 32 rows) that its sequences have room for.
+bool weigh_mfma_supported(const WeighProblem& p);
+constexpr int kWeighKeys = 32, kWeighRows = 4096;  // keys per tile; (token, head) rows of a piece at most
+int weigh_spans(int rows, int ncu);
+inline size_t weigh_score_bytes(int64_t tiles, int rows) { return (size_t)tiles * ((rows + 31) / 32) * 4096; }
+inline size_t weigh_part_bytes(int spans, int seqs, int rows) {
+  return (size_t)(spans + seqs - 1) * 2 * ((rows + 31) / 32 * 32) * sizeof(float);
+}
+hipError_t launch_weigh_mfma(const WeighProblem& p, int64_t most_tiles, hipStream_t stream, int ncu);
 
 // la_evict_kv.
 struct EvictProblem {

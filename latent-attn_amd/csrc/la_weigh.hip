@@ -76,6 +76,436 @@ __global__ __launch_bounds__(256) void plain_weigh_kernel(WeighProblem p, int s,
   if (lane == 0) p.weights[at] += sum;
 }
 
+// ---- the matrix form ----------------------------------------------------------------------------------
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char lchar;
+
+// Two parts of a value in the products' type: hi + lo / kLow.
+template <typename T>
+struct Mm;
+template <>
+struct Mm<__hip_bfloat16> {
+  typedef bf16x8 vec;
+  typedef __bf16 elem;
+  static constexpr float kLow = 1.f;
+  static __device__ inline f32x16 mma(vec a, vec b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mm<__half> {
+  typedef f16x8 vec;
+  typedef _Float16 elem;
+  static constexpr float kLow = 2048.f;  // (what is left of small values would be subnormal)
+  static __device__ inline f32x16 mma(vec a, vec b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <typename T>
+__device__ inline void split(float x, typename Mm<T>::elem& hi, typename Mm<T>::elem& lo) {
+  hi = (typename Mm<T>::elem)x;
+  lo = (typename Mm<T>::elem)((x - (float)hi) * Mm<T>::kLow);
+}
+
+// Tiles of 32 rows of the piece's sequences, counted over them, shared out evenly:
+// span w of W has [w T / W, (w + 1) T / W), one tile at least (W <= T). The lengths are on the device, so
+// every wave sums them itself.
+struct Spans {
+  const WeighProblem& p;
+  __device__ int tiles(int i) const {  // of the piece's sequence i
+    return i < p.seqs ? (source_rows(p.src, p.seq0 + i) + kWeighKeys - 1) / kWeighKeys : 0;
+  }
+  __device__ int total() const {
+    int t = 0;
+    for (int i = wave_lane(); i < p.seqs; i += 64) t += tiles(i);
+    return wave_sum_i(t);
+  }
+  // Sequence of tile t (< total), its first tile and tiles; false only if the lengths change meanwhile.
+  __device__ bool find(int t, int* seq, int* first, int* n) const {
+    int before = 0;
+    for (int i0 = 0; i0 < p.seqs; i0 += 64) {
+      const int mine = tiles(i0 + wave_lane()), end = wave_scan(mine);
+      const uint64_t past = __builtin_amdgcn_ballot_w64(before + end > t);
+      if (past) {
+        const int k = __builtin_ctzll(past);
+        *seq = i0 + k;
+        *n = __builtin_amdgcn_readlane(mine, k);
+        *first = before + __builtin_amdgcn_readlane(end, k) - *n;
+        return true;
+      }
+      before += __builtin_amdgcn_readlane(end, 63);
+    }
+    return false;
+  }
+  // The next one with tiles.
+  __device__ bool next(int* seq, int* first, int* n) const {
+    *first += *n;
+    do {
+      if (++*seq >= p.seqs) return false;
+      *n = tiles(*seq);
+    } while (*n == 0);
+    return true;
+  }
+  static __device__ int begin(int w, int T, int W) { return (int)((int64_t)w * T / W); }
+  static __device__ int of(int t, int T, int W) { return (int)((((int64_t)t + 1) * W - 1) / T); }  // the span that has tile t
+};
+
+// One tile in LDS: 32 rows of 1024 B whose starts are spread over the banks (every
+// read takes one 16-B piece of each row), and the rotated rope keys in two parts,
+// 128-B rows with their 16-B pieces permuted.
+constexpr int kPitch = 1088;
+__host__ __device__ constexpr int row_at(int r) { return r * kPitch + 16 * ((r >> 2) & 3); }
+__device__ inline int rope_piece(int row, int piece) { return row * 128 + 16 * (piece ^ ((row >> 1) & 7)); }
+constexpr int kRopeHi = (row_at(31) + 1024 + 127) / 128 * 128, kRopeLo = kRopeHi + 32 * 128, kTile = kRopeLo + 32 * 128;
+
+// What a wave holds of a tile on its way to LDS: its 8 rows' latent parts, 16 (8-bit
+// rows: 8) B of each row per lane, and the rope part of row lane / 8, pairs 4 (lane % 8) .. + 3.
+template <bool kFp8>
+struct Staged;
+template <>
+struct Staged<false> {
+  u32x4 c[8];
+  u32x2 ka, kb;
+  f32x4 cs, sn;
+};
+template <>
+struct Staged<true> {
+  u32x2 c[8];
+  uint32_t ka, kb;
+  f32x4 cs, sn;
+};
+template <bool kFp8>
+__device__ inline void stage_load(const WeighProblem& p, Staged<kFp8>& x, int s, int t, int last, int wave, int lane) {
+  constexpr int kRowB = kFp8 ? 576 : 1152;
+  typedef decltype(x.c[0] + x.c[0]) cvec;
+  typedef decltype(x.ka) kvec;
+  const int pos = min(kWeighKeys * t + 8 * wave + (lane >> 3), last);
+  const uint64_t at = (uint64_t)(uintptr_t)p.src.kv + (uint64_t)source_row(p.src, s, pos) * kRowB;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint64_t row = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(at >> 32), 8 * i) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, 8 * i);
+    x.c[i] = reinterpret_cast<const cvec*>(row)[lane];
+  }
+  const char* const rope = reinterpret_cast<const char*>(at) + (kFp8 ? 512 : 1024) + sizeof(kvec) * (lane & 7);
+  x.ka = *reinterpret_cast<const kvec*>(rope);
+  x.kb = *reinterpret_cast<const kvec*>(rope + 8 * sizeof(kvec));
+  const int64_t rp = source_rope_row(p.src, pos) * 32 + 4 * (lane & 7);
+  x.cs = *reinterpret_cast<const f32x4*>(p.src.cos + rp);
+  x.sn = *reinterpret_cast<const f32x4*>(p.src.sin + rp);
+}
+template <typename T, bool kFp8>
+__device__ inline void stage_store(const Staged<kFp8>& x, lchar* L, int wave, int lane) {
+  typedef typename Mm<T>::elem elem;
+  auto put = [&](int at, auto v) { *reinterpret_cast<__attribute__((address_space(3))) decltype(v)*>(L + at) = v; };
+  const int row0 = row_at(8 * wave) + 16 * lane;  // row 8 w + i is 1088 i + 16 (i / 4) on
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    u32x4 y;
+    if constexpr (kFp8) {
+      y[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.c[i][0], 1.f, false));
+      y[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.c[i][0], 1.f, true));
+      y[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.c[i][1], 1.f, false));
+      y[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.c[i][1], 1.f, true));
+    } else {
+      y = x.c[i];
+    }
+    put(row0 + kPitch * i + 16 * (i >> 2), y);
+  }
+  const int row = 8 * wave + (lane >> 3), u = lane & 7;
+  typedef elem e4 __attribute__((ext_vector_type(4)));
+  e4 ah, al, bh, bl;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float a, b;
+    if constexpr (kFp8) {
+      const auto va = (e & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8(x.ka, true) : __builtin_amdgcn_cvt_pk_f32_fp8(x.ka, false);
+      const auto vb = (e & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8(x.kb, true) : __builtin_amdgcn_cvt_pk_f32_fp8(x.kb, false);
+      a = va[e & 1];
+      b = vb[e & 1];
+    } else {
+      a = (float)__builtin_bit_cast(elem, (uint16_t)(x.ka[e >> 1] >> (16 * (e & 1))));
+      b = (float)__builtin_bit_cast(elem, (uint16_t)(x.kb[e >> 1] >> (16 * (e & 1))));
+    }
+    elem h, l;
+    split<T>(a * x.cs[e] - b * x.sn[e], h, l);
+    ah[e] = h, al[e] = l;
+    split<T>(a * x.sn[e] + b * x.cs[e], h, l);
+    bh[e] = h, bl[e] = l;
+  }
+  const int pa = rope_piece(row, u >> 1) + 8 * (u & 1), pb = rope_piece(row, 4 + (u >> 1)) + 8 * (u & 1);
+  put(kRopeHi + pa, ah);
+  put(kRopeLo + pa, al);
+  put(kRopeHi + pb, bh);
+  put(kRopeLo + pb, bl);
+}
+
+// Scores of a span's tiles against 128 (32 kWR) rows of queries, and their partial
+// maxima and sums of exponentials.
+//
+// Precision: a score has to hold fp32's worth, since weights are compared with each
+// other; fp32 matrix instructions have a sixteenth of the 16-bit ones' rate.
+// Cache rows are 16-bit numbers (8-bit ones widen exactly), so the queries go in as
+// two 16-bit parts, hi and what is left, whose products with a row are exact and
+// summed in fp32: 2 products for the latent part, 3 for the rope part, whose
+// rotated keys have two parts as well. bf16 leaves 2^-18 of an operand, fp16 less.
+//
+// 4 waves: kWR of them have 32 rows of queries each, with their operands in
+// registers for the whole segment, the 4 / kWR others of a row block take shares of
+// the contraction, summed through LDS (few heads: a wave per row block alone would
+// leave three quarters of the matrix cores idle). Tiles go HBM -> registers -> LDS,
+// the next but one on its way during the products.
+template <typename T, bool kFp8, int kWR>
+__global__ __launch_bounds__(256, 1) void weigh_scores_kernel(WeighProblem p, int row_blocks) {
+  typedef typename Mm<T>::vec vec;
+  typedef typename Mm<T>::elem elem;
+  constexpr int kKD = 4 / kWR;            // shares of the contraction
+  constexpr int kC = 32 / kKD;            // latent steps of 16 of a share
+  constexpr int kR = 4 / kKD;             // rope steps
+  constexpr int kN = 16 / kKD;            // scores of a lane after the sum
+  extern __shared__ __attribute__((aligned(1024))) char weigh_lds[];
+  lchar* const L = (lchar*)weigh_lds;
+  lchar* const sums = L + 2 * kTile;      // kKD > 1: 4 KB per wave
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int wr = wave % kWR, kd = wave / kWR, r32 = lane & 31, g = lane >> 5;
+  // an eighth of the items to each XCD, row groups of a span together
+  const int groups = (row_blocks + kWR - 1) / kWR, items = p.spans * groups, per = (items + 7) / 8;
+  const int item = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || item >= items) return;
+  const int span = item / groups, block = item % groups * kWR + wr;
+  const int rows = p.count * p.nh, row = min(32 * block + r32, rows - 1);
+  const bool valid = 32 * block + r32 < rows;
+  const Spans sp{p};
+  const int T_all = sp.total(), W = min(p.spans, T_all);
+  if (span >= W) return;
+  int t = Spans::begin(span, T_all, W);
+  const int t_end = Spans::begin(span + 1, T_all, W);
+  int i, first, n;
+  if (!sp.find(t, &i, &first, &n)) return;
+  while (true) {
+    const int s = p.seq0 + i, len = source_rows(p.src, s), last = len - 1;
+    const int end = min(t_end, first + n);
+    // ---- the queries' operands: [16 k + 8 g .. + 7] of the row, times the softmax's scale ----
+    vec qh[kC + kR], ql[kC + kR];
+    {
+      const int64_t q = ((int64_t)s * p.tokens + p.token0) * p.nh + row;
+      const float *const qa = p.q_abs + q * 512 + 16 * kC * kd + 8 * g, *const qr = p.q_rope + q * 64 + 16 * kR * kd + 8 * g;
+#pragma unroll
+      for (int k = 0; k < kC + kR; ++k) {
+        const float* const from = k < kC ? qa + 16 * k : qr + 16 * (k - kC);
+        const f32x4 a = *reinterpret_cast<const f32x4*>(from), b = *reinterpret_cast<const f32x4*>(from + 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          elem h, l;
+          split<T>((e < 4 ? a[e & 3] : b[e & 3]) * p.scale_log2, h, l);
+          qh[k][e] = h;
+          ql[k][e] = l;
+        }
+      }
+    }
+    // keys that the row's token sees
+    const int sees = len - p.tokens + p.token0 + row / p.nh + 1;
+    float m = kNoScore, l = 0.f;
+    Staged<kFp8> x;
+    stage_load<kFp8>(p, x, s, t - first, last, wave, lane);
+    lds_barrier();  // every wave is done with the segment before
+    stage_store<T, kFp8>(x, L, wave, lane);
+    if (t + 1 < end) stage_load<kFp8>(p, x, s, t + 1 - first, last, wave, lane);
+    for (int u = t; u < end; ++u) {
+      lds_barrier();  // tile u is there, tile u - 1 is read
+      const lchar* const b = L + ((u - t) & 1) * kTile;
+      if (u + 1 < end) {
+        stage_store<T, kFp8>(x, L + ((u + 1 - t) & 1) * kTile, wave, lane);
+        if (u + 2 < end) stage_load<kFp8>(p, x, s, u + 2 - first, last, wave, lane);
+      }
+      f32x16 hi = {}, lo = {};
+      auto operand = [&](int k) -> vec {  // keys r32, elements [16 k + 8 g .. + 7]
+        const int at = k < kC ? row_at(r32) + 32 * (kC * kd + k) + 16 * g
+                       : k < kC + kR ? kRopeHi + rope_piece(r32, 2 * (kR * kd + k - kC) + g)
+                                     : kRopeLo + rope_piece(r32, 2 * (kR * kd + k - kC - kR) + g);
+        return *reinterpret_cast<const __attribute__((address_space(3))) vec*>(b + at);
+      };
+      constexpr int kSteps = kC + 2 * kR, kAhead = 6;
+      vec a[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) a[k] = operand(k);
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        const vec v = a[k % kAhead];
+        if (k < kC + kR) hi = Mm<T>::mma(v, qh[k], hi);
+        lo = Mm<T>::mma(v, k < kC + kR ? ql[k] : qh[k - kR], lo);
+        if (k + kAhead < kSteps) a[k % kAhead] = operand(k + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      settle(hi);
+      settle(lo);
+      // lane: row r32, keys 8 (e / 4) + 4 g + e % 4
+      float sc[kN];
+      if constexpr (kKD == 1) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[e] = hi[e] + lo[e] * (1.f / Mm<T>::kLow);
+      } else {
+        typedef __attribute__((address_space(3))) f32x4 lvec;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = hi[4 * q + e] + lo[4 * q + e] * (1.f / Mm<T>::kLow);
+          *reinterpret_cast<lvec*>(sums + 4096 * wave + 1024 * q + 16 * lane) = v;
+        }
+        lds_barrier();
+#pragma unroll
+        for (int q = 0; q < kN / 4; ++q) {
+          f32x4 v = {};
+#pragma unroll
+          for (int w = 0; w < kKD; ++w)
+            v += *reinterpret_cast<const lvec*>(sums + 4096 * (wr + kWR * w) + 1024 * (kN / 4 * kd + q) + 16 * lane);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[4 * q + e] = v[e];
+        }
+      }
+      const int key0 = kWeighKeys * (u - first) + 2 * kN * kd + 4 * g;
+      const int most = min(len, sees) - key0;
+      if (kWeighKeys * (u - first + 1) > len - p.tokens + p.token0 + 1) {
+#pragma unroll
+        for (int e = 0; e < kN; ++e)
+          if (8 * (e >> 2) + (e & 3) >= most) sc[e] = -INFINITY;
+      }
+      float top = sc[0];
+#pragma unroll
+      for (int e = 1; e < kN; ++e) top = fmaxf(top, sc[e]);
+      const float up = fmaxf(m, top);
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < kN; ++e) sum += __builtin_amdgcn_exp2f(sc[e] - up);
+      l = l * __builtin_amdgcn_exp2f(m - up) + sum;
+      m = up;
+      if (valid) {
+        float* const to = p.scores + ((int64_t)u * row_blocks + block) * 1024 + 32 * r32 + 2 * kN * kd + 4 * g;
+#pragma unroll
+        for (int q = 0; q < kN / 4; ++q)
+          *reinterpret_cast<f32x4*>(to + 8 * q) = f32x4{sc[4 * q], sc[4 * q + 1], sc[4 * q + 2], sc[4 * q + 3]};
+      }
+    }
+    // ---- the segment's share of the rows' sums ----
+    {
+      auto join = [&](float m2, float l2) {
+        const float up = fmaxf(m, m2);
+        l = l * __builtin_amdgcn_exp2f(m - up) + l2 * __builtin_amdgcn_exp2f(m2 - up);
+        m = up;
+      };
+      const auto sm = __builtin_amdgcn_permlane32_swap(u_of(m), u_of(m), false, false);
+      const auto sl = __builtin_amdgcn_permlane32_swap(u_of(l), u_of(l), false, false);
+      m = f_of(sm[0]), l = f_of(sl[0]);
+      join(f_of(sm[1]), f_of(sl[1]));
+      if constexpr (kKD > 1) {
+        typedef __attribute__((address_space(3))) float lfloat;
+        lds_barrier();  // the sums are read
+        lfloat* const ml = reinterpret_cast<lfloat*>(sums) + 64 * wave;
+        if (g == 0) ml[r32] = m, ml[32 + r32] = l;
+        lds_barrier();
+#pragma unroll
+        for (int w = 1; w < kKD; ++w) {
+          const lfloat* const o = reinterpret_cast<const lfloat*>(sums) + 64 * (wr + kWR * w);
+          if (kd == 0) join(o[r32], o[32 + r32]);
+        }
+      }
+      if (kd == 0 && g == 0 && block < row_blocks) {
+        float* const to = p.part + (int64_t)(span + i) * 2 * 32 * row_blocks + 32 * block + r32;
+        to[0] = m;
+        to[32 * row_blocks] = l;
+      }
+    }
+    t = end;
+    if (t >= t_end || !sp.next(&i, &first, &n)) return;
+  }
+}
+
+// The second kernel: rows' log-sum-exps from their partial sums, then a wave per
+// tile adds the exponentials of its scores over the rows, in their order.
+__global__ __launch_bounds__(256) void weigh_sum_kernel(WeighProblem p, int row_blocks) {
+  __shared__ float lse[kWeighRows];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const Spans sp{p};
+  const int T_all = sp.total(), W = min((int)gridDim.x, T_all), W1 = min(p.spans, T_all), w = blockIdx.x;
+  if (w >= W) return;
+  int t = Spans::begin(w, T_all, W);
+  const int t_end = Spans::begin(w + 1, T_all, W);
+  int i, first, n;
+  if (!sp.find(t, &i, &first, &n)) return;
+  const int rows = p.count * p.nh;
+  while (true) {
+    const int s = p.seq0 + i, len = source_rows(p.src, s), end = min(t_end, first + n);
+    const int c0 = Spans::of(first, T_all, W1), c1 = Spans::of(first + n - 1, T_all, W1);
+    __syncthreads();
+    for (int r = threadIdx.x; r < 32 * row_blocks; r += 256) {
+      float m = kNoScore, l = 0.f;
+      if (r < rows)
+        for (int c = c0; c <= c1; ++c) {
+          const float* const from = p.part + (int64_t)(c + i) * 2 * 32 * row_blocks + r;
+          const float m2 = from[0], l2 = from[32 * row_blocks], up = fmaxf(m, m2);
+          l = l * exp2f(m - up) + l2 * exp2f(m2 - up);
+          m = up;
+        }
+      // rows past the last, and tokens that see nothing, give nothing
+      lse[r] = l == 0.f ? INFINITY : m + log2f(l);
+    }
+    __syncthreads();
+    for (int u = t + wave; u < end; u += 4) {
+      const float* const from = p.scores + (int64_t)u * row_blocks * 1024 + 4 * lane;
+      f32x4 sum = {};
+      for (int b = 0; b < row_blocks; ++b) {
+        f32x4 v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const f32x4*>(from + 1024 * b + 256 * q);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = 32 * b + 8 * q + (lane >> 3);
+          const float e = lse[r];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) sum[k] += r < rows ? exp2f(v[q][k] - e) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int o = 8; o < 64; o <<= 1)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] += __shfl_xor(sum[k], o, 64);
+      const int key = kWeighKeys * (u - first) + 4 * lane;
+      if (lane < 8) {
+        float* const to = p.weights + (p.src.offsets ? source_begin(p.src, s) : (int64_t)s * p.src.region);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (key + k < len) to[key + k] += sum[k];
+      }
+    }
+    t = end;
+    if (t >= t_end || !sp.next(&i, &first, &n)) return;
+  }
+}
+
+template <typename T, bool kFp8, int kWR>
+hipError_t scores_t(const WeighProblem& p, int row_blocks, hipStream_t stream) {
+  constexpr int lds = 2 * kTile + (kWR < 4 ? 4 * 4096 : 0);
+  static OncePerDevice once;
+  const hipError_t e = allow_lds(once, reinterpret_cast<const void*>(&weigh_scores_kernel<T, kFp8, kWR>), lds);
+  if (e != hipSuccess) return e;
+  const int64_t items = (int64_t)p.spans * ((row_blocks + kWR - 1) / kWR);
+  hipLaunchKernelGGL((weigh_scores_kernel<T, kFp8, kWR>), dim3((unsigned)(8 * ((items + 7) / 8))), dim3(256), lds, stream, p, row_blocks);
+  return hipGetLastError();
+}
+template <typename T, bool kFp8>
+hipError_t scores_w(const WeighProblem& p, int row_blocks, hipStream_t stream) {
+  if (row_blocks == 1) return scores_t<T, kFp8, 1>(p, row_blocks, stream);
+  if (row_blocks == 2) return scores_t<T, kFp8, 2>(p, row_blocks, stream);
+  return scores_t<T, kFp8, 4>(p, row_blocks, stream);
+}
+
 }  // namespace
 
 hipError_t launch_weigh_plain(const WeighProblem& p, hipStream_t stream) {
@@ -90,6 +520,30 @@ hipError_t launch_weigh_plain(const WeighProblem& p, hipStream_t stream) {
       hipLaunchKernelGGL(plain_weigh_kernel, dim3(blocks), dim3(256), 0, stream, p, s, first);
     });
   return e;
+}
+
+bool weigh_mfma_supported(const WeighProblem& p) {
+  if (p.src.kv_dtype == LA_DTYPE_F32 || p.dc != 512 || p.dR != 64 || p.nh > kWeighRows) return false;
+  // 16-byte loads of rows and tables
+  if (((reinterpret_cast<uintptr_t>(p.src.kv) | reinterpret_cast<uintptr_t>(p.src.cos) | reinterpret_cast<uintptr_t>(p.src.sin)) & 15) != 0)
+    return false;
+  return device_is_gfx950();
+}
+
+int weigh_spans(int rows, int ncu) {
+  const int blocks = (rows + 31) / 32, groups = blocks <= 4 ? 1 : (blocks + 3) / 4;
+  return groups < ncu ? ncu / groups : 1;
+}
+
+hipError_t launch_weigh_mfma(const WeighProblem& p, int64_t most_tiles, hipStream_t stream, int ncu) {
+  const int row_blocks = (p.count * p.nh + 31) / 32;
+  hipError_t e = p.src.kv_dtype == LA_DTYPE_FP8_E4M3 ? scores_w<__hip_bfloat16, true>(p, row_blocks, stream)
+                 : p.src.kv_dtype == LA_DTYPE_BF16   ? scores_w<__hip_bfloat16, false>(p, row_blocks, stream)
+                                                     : scores_w<__half, false>(p, row_blocks, stream);
+  if (e != hipSuccess) return e;
+  const int64_t blocks = (most_tiles + 3) / 4 < 8LL * ncu ? (most_tiles + 3) / 4 : 8LL * ncu;
+  hipLaunchKernelGGL(weigh_sum_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p, row_blocks);
+  return hipGetLastError();
 }
 
 }  // namespace la

@@ -11,8 +11,14 @@ a score is off by at most e = (2^-16 + (K + 160) 2^-24) A, A = scale times the
 sum of the terms' magnitudes (the absorbed query's own sum has 128 terms), a
 weight by a factor within exp(+-2 e) (its exponent and its log-sum-exp), and an
 exponential, its logarithm and the sum over n tokens, heads and partial sums by
-(n heads + keys + 16) 2^-24 more, all of it relative to the weight. Errors of
-different terms are independent: normwise 1e-5 holds too.
+(n heads + keys + 16) 2^-24 more, all of it relative to the weight.
+Normwise: roundings of different terms are independent and at most 2^-18 of the
+term (hi = x (1 + d), |d| <= 2^-9, of what is left 2^-9 again), so a score's
+error has a standard deviation of at most 2^-18 B, B = scale times the root of
+the sum of the squared terms, and its weight moves by at most twice that
+(exponent and log-sum-exp): 2^-17 B of it. Scores of standard deviation 1 have B
+of about 1, where 2^-17 and the fp32 sums stay below 1e-5; the tests hold
+max(1e-5, 2^-17 B).
 """
 
 from __future__ import annotations
@@ -70,7 +76,8 @@ def weight_places(layout, s, n):
 
 
 def scores(rows, q_nope, q_rope, W_UK, cos, sin, key_at, q_at, rotate_q):
-    """(tokens, heads, rows) natural scores and the sums of their terms' magnitudes in latent space."""
+    """(tokens, heads, rows) natural scores, the sums of their terms' magnitudes in latent space, and the roots of the
+    sums of their squares."""
     heads, dn = q_nope.shape[1:]
     dc = W_UK.shape[1]
     scale = 1.0 / math.sqrt(dn + q_rope.shape[2])
@@ -81,7 +88,8 @@ def scores(rows, q_nope, q_rope, W_UK, cos, sin, key_at, q_at, rotate_q):
     x = scale * (torch.einsum("thc,kc->thk", qa, rows[:, :dc]) + torch.einsum("thr,kr->thk", qr, R))
     size = scale * (torch.einsum("thc,kc->thk", torch.einsum("thi,hic->thc", q_nope.abs(), W.abs()), rows[:, :dc].abs()) +
                     torch.einsum("thr,kr->thk", qr.abs(), rows[:, dc:].abs() * 2))
-    return x, size
+    root = scale * (torch.einsum("thc,kc->thk", qa ** 2, rows[:, :dc] ** 2) + torch.einsum("thr,kr->thk", qr ** 2, R ** 2)).sqrt()
+    return x, size, root
 
 
 def tree_reference(rows, q_nope, q_rope, W_UK, W_UV, cos, sin, parents, rotate_q):
@@ -96,7 +104,7 @@ def tree_reference(rows, q_nope, q_rope, W_UK, W_UV, cos, sin, parents, rotate_q
         depth = torch.tensor([len(a) - 1 for a in sets])
         key_at = torch.cat([torch.arange(L - n), L - n + depth])
         t = slice(s * n, (s + 1) * n)
-        x, _ = scores(r, q_nope[t], q_rope[t], W_UK, cos, sin, key_at, L - n + depth, rotate_q)
+        x, _, _ = scores(r, q_nope[t], q_rope[t], W_UK, cos, sin, key_at, L - n + depth, rotate_q)
         sees = torch.zeros(n, L, dtype=torch.bool)
         sees[:, :L - n] = True
         for j, a in enumerate(sets):
@@ -111,26 +119,28 @@ def tree_reference(rows, q_nope, q_rope, W_UK, W_UV, cos, sin, parents, rotate_q
 
 
 def weigh_reference(rows, q_nope, q_rope, W_UK, cos, sin, n, rotate_q):
-    """Of every sequence the weight that each row gets, and the bound of its error (the module's comment)."""
-    outs, bounds = [], []
+    """Of every sequence the weight that each row gets, the bound of its error, and the normwise one (the module's comment)."""
+    outs, bounds, norms = [], [], []
     K = rows[0].shape[1] if rows else 0
     for s, r in enumerate(rows):
         L = r.shape[0]
         q_at = (torch.arange(n) + L - n).clamp(min=0)
         t = slice(s * n, (s + 1) * n)
-        w, b = torch.zeros(L, dtype=torch.float64), torch.zeros(L, dtype=torch.float64)
+        w, b, norm = torch.zeros(L, dtype=torch.float64), torch.zeros(L, dtype=torch.float64), 1e-5
         if L:
-            x, size = scores(r, q_nope[t], q_rope[t], W_UK, cos, sin, torch.arange(L), q_at, rotate_q)
+            x, size, root = scores(r, q_nope[t], q_rope[t], W_UK, cos, sin, torch.arange(L), q_at, rotate_q)
             for j in range(n):
                 see = L - n + j + 1
                 if see > 0:
                     p = torch.softmax(x[j, :, :see], -1)
                     off = (2.0 ** -16 + (K + 160) * 2.0 ** -24) * size[j, :, :see].amax(-1, keepdim=True)
                     w[:see] += p.sum(0)
+                    norm = max(norm, 2.0 ** -17 * float(root[j, :, :see].max()))
                     b[:see] += (p * (torch.expm1(2 * off) + (n * q_nope.shape[1] + L + 16) * 2.0 ** -24)).sum(0)
         outs.append(w)
         bounds.append(b)
-    return outs, bounds
+        norms.append(norm)
+    return outs, bounds, norms
 
 
 def evict_reference(w, keep, first, last):
