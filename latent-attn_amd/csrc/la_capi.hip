@@ -323,6 +323,9 @@ int run(const la_decode_args* a, hipStream_t stream, hipEvent_t ev_b = nullptr, 
   int st = prepare(a, &p, &plan, coarse);
   if (st != LA_SUCCESS) return st;
   if (a->num_seqs == 0) return LA_SUCCESS;
+  const bool tree = tail && tail->tree.seen;
+  if (tree && !plan.mfma) return LA_ERROR_NOT_SUPPORTED;
+  if (tree) plan.waves16 = 0;
 
   char* ws = static_cast<char*>(a->workspace);
   bool owned = false;
@@ -394,6 +397,7 @@ int run(const la_decode_args* a, hipStream_t stream, hipEvent_t ev_b = nullptr, 
     hipError_t e = hipSuccess;
     const int reps = repeat > 1 ? repeat : 1;
     auto launch_mfma = [&](hipEvent_t b, hipEvent_t en) {
+      if (tree) return launch_decode_mfma_tree(p, tail->tree, stream);
       return plan.waves16 ? launch_decode_mfma16(p, plan.waves16, stream, p.q_prep ? nullptr : zero_out, zero_n, b, en)
                           : launch_decode_mfma(p, stream, b, en);
     };
@@ -1294,7 +1298,6 @@ bool queries_vec(const QuerySource& q) {
   return q_vec(q.q_nope, q.dtype, q.nope_stride, q.nope_head) && q_vec(q.q_rope, q.dtype, q.rope_stride, q.rope_head);
 }
 
-constexpr bool tree_kernels() { return false; }
 enum TreeForm { kTreePlain = 1, kTreeMfma = 2 };
 
 int decode_tree(const la_tree_args* a, void* stream_v, bool run_it, size_t* need) {
@@ -1343,7 +1346,7 @@ int decode_tree(const la_tree_args* a, void* stream_v, bool run_it, size_t* need
   d.cfg = c;
   DecodeProblem step;
   Plan plan;
-  const bool mfma = tree_kernels() && a->kernel_variant != kTreePlain && prepare(&d, &step, &plan) == LA_SUCCESS && plan.mfma;
+  const bool mfma = a->kernel_variant != kTreePlain && prepare(&d, &step, &plan) == LA_SUCCESS && plan.mfma;
   if (!mfma && (a->kernel_variant == kTreeMfma || !generic_prompt_supported(c.kv_lora_rank, c.qk_rope_head_dim)))
     return LA_ERROR_NOT_SUPPORTED;
   const bool join = mfma && merge_join_supported(step);

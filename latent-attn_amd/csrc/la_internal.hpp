@@ -598,6 +598,7 @@ struct TreeStep {
 // ev_begin / ev_end (optional) are recorded at the kernel's start and end.
 hipError_t launch_decode_mfma(const DecodeProblem& p, hipStream_t stream, hipEvent_t ev_begin = nullptr,
                               hipEvent_t ev_end = nullptr);
+hipError_t launch_decode_mfma_tree(const DecodeProblem& p, const TreeStep& tree, hipStream_t stream);
 bool mfma_supported(const DecodeProblem& p);
 // The same with 16 query heads per workgroup (la_mfma16.hip); waves = 4 or 8
 // per workgroup (tiles of 64 or 128 positions).

@@ -221,6 +221,15 @@ static_assert(pv_wait_n(kExpWaitStep - 1, true) == pv_later(kExpWaitStep - 1) + 
 static_assert(kExpWaitStep > kRotStep && kExpWaitStep + 3 < kPvSteps && kExpSlot0 + 7 < 2 * kPvSteps,
               "fp8 expansion slots inside PV");
 static_assert(kLdsBytes <= 160 * 1024, "LDS budget");
+// Trees of drafted tokens (TreeStep): what each query head's node sees, 8 B per
+// head of the group, behind the rest. The rows of a tile with nodes that are not
+// numbers are the bits of a word (a byte per wave) in the buffer's last bytes
+// before its k_rope rows.
+constexpr int kSeenOff = kLdsBytes;
+constexpr int kTreeLdsBytes = kSeenOff + 8 * kHG;
+constexpr int kBadOff = kCtBytes;
+static_assert(kSeenOff % 8 == 0 && kTreeLdsBytes <= 160 * 1024 && kBadOff + 4 <= kRopeOff && kBadOff % 4 == 0, "tree LDS");
+constexpr float kNoScore = -1e30f;  // a tree's running maximum before the first row that its head sees
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -607,6 +616,10 @@ struct SegCtx {
   // the clamp of rope_row in 32 bits (the MFMA kernels' positions and table
   // rows stay below 2^24 + 2^20, mfma_supported)
   int pc, rlim;
+  // trees: the sequence's first node's row, relative to the segment's first, and
+  // the table rows of its nodes
+  int node0;
+  const float *tcos, *tsin;
 };
 
 // Tile k covers segment rows [32k, 32k + 32). The pipeline also copies up to
@@ -693,7 +706,8 @@ __device__ inline TileDma tile_dma(const SegCtx& sg, int k, const char* base, in
 // unswizzled at ct_row_off, so the lane offset is the same for every row. The
 // instruction's immediate offset would move the LDS destination too, so row
 // steps go into the VGPR offset.
-template <int J>
+// kTree: nodes' table rows are those of their depths, gathered per sequence.
+template <int J, bool kTree = false>
 __device__ inline void issue_copy(const DecodeProblem& p, const SegCtx& sg, int k, lchar* L, uint32_t buf, int wave,
                                   int lane, const TileDma& d) {
   const int r_first = 8 * wave;
@@ -709,6 +723,15 @@ __device__ inline void issue_copy(const DecodeProblem& p, const SegCtx& sg, int 
     const int r = min(k * kT + row, sg.last);
     const uint32_t toff = (uint32_t)min(sg.pc + r, sg.rlim) * ((kDr / 2) * 4) + (lane & 7) * 16;
     const float* tab = J == 9 ? p.rope_cos : p.rope_sin;
+    if constexpr (kTree) {
+      if (min(k * kT + r_first + 7, sg.last) >= sg.node0) {  // wave-uniform: a node among the wave's rows
+        const char* from = reinterpret_cast<const char*>(tab) + toff;
+        if (r >= sg.node0)
+          from = reinterpret_cast<const char*>(J == 9 ? sg.tcos : sg.tsin) + (r - sg.node0) * ((kDr / 2) * 4) + (lane & 7) * 16;
+        __builtin_amdgcn_global_load_lds(from, (lds_void*)(L + (J == 9 ? kCosOff : kSinOff) + r_first * 128), 16, 0, 0);
+        return;
+      }
+    }
     __builtin_amdgcn_global_load_lds(reinterpret_cast<const char*>(tab) + toff,
                                      (lds_void*)(L + (J == 9 ? kCosOff : kSinOff) + r_first * 128), 16, 0, 0);
   }
@@ -720,7 +743,7 @@ __device__ inline void issue_copy(const DecodeProblem& p, const SegCtx& sg, int 
 // last row each lane re-reads that chunk of the last row instead (rows past it
 // are masked, and unfilled capacity is never read). J = kFp8RowCopies /
 // + 1: the cos / sin rows, as for a 16-bit cache.
-template <int J>
+template <int J, bool kTree = false>
 __device__ inline void issue_copy_fp8(const DecodeProblem& p, const SegCtx& sg, int k, lchar* L, uint32_t buf,
                                       int wave, int lane, const TileDma& d) {
   if constexpr (J < kFp8RowCopies) {
@@ -739,23 +762,23 @@ __device__ inline void issue_copy_fp8(const DecodeProblem& p, const SegCtx& sg, 
       __builtin_amdgcn_global_load_lds(d.base + off, dst, 16, 0, kStreamPolicy);
     }
   } else {
-    issue_copy<J - kFp8RowCopies + 9>(p, sg, k, L, buf, wave, lane, d);
+    issue_copy<J - kFp8RowCopies + 9, kTree>(p, sg, k, L, buf, wave, lane, d);
   }
 }
 
-template <bool kFp8, int J>
+template <bool kFp8, int J, bool kTree>
 __device__ inline void issue_copy_any(const DecodeProblem& p, const SegCtx& sg, int k, lchar* L, uint32_t buf,
                                       int wave, int lane, const TileDma& d) {
-  if constexpr (kFp8) issue_copy_fp8<J>(p, sg, k, L, buf, wave, lane, d);
-  else issue_copy<J>(p, sg, k, L, buf, wave, lane, d);
+  if constexpr (kFp8) issue_copy_fp8<J, kTree>(p, sg, k, L, buf, wave, lane, d);
+  else issue_copy<J, kTree>(p, sg, k, L, buf, wave, lane, d);
 }
 
 // All copies of tile k (base: tile_base of tile k).
-template <bool kFp8>
+template <bool kFp8, bool kTree = false>
 __device__ inline void issue_tile_dma(const DecodeProblem& p, const SegCtx& sg, int k, const char* base, lchar* L,
                                       uint32_t buf, int wave, int lane) {
   const TileDma d = tile_dma<kFp8>(sg, k, base, wave, lane);
-  static_for<dma_per_wave(kFp8)>([&](auto j) { issue_copy_any<kFp8, decltype(j)::value>(p, sg, k, L, buf, wave, lane, d); });
+  static_for<dma_per_wave(kFp8)>([&](auto j) { issue_copy_any<kFp8, decltype(j)::value, kTree>(p, sg, k, L, buf, wave, lane, d); });
 }
 
 // Rotate-half RoPE of rows 8w..8w+7 of the tile at LDS offset buf, in place
@@ -933,11 +956,39 @@ constexpr bool fp8_half_order_ok() {
 }
 static_assert(fp8_half_order_ok(), "fp8 expansion halves overlap");
 
+// Trees: the wave's 8 rows of a tile that has nodes, once they lie in LDS. A row is
+// seen by its descendants only, but the products weigh every row of the tile for
+// every head, by zero where it is hidden, and zero times an infinity or NaN is
+// NaN. So a row that holds one becomes zeros and is noted: its scores become NaN
+// where it is seen.
+template <typename KT>
+__device__ inline void check_rows(lchar* L, uint32_t buf, int wave, int lane) {
+  constexpr uint32_t kExp = std::is_same<KT, __half>::value ? 0x7C00u : 0x7F80u;
+  uint32_t bad = 0;
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t at = buf + ct_row_off(8 * wave + i) + 16 * lane;
+    const u32x4 x = lds_ld<u32x4>(L, at);
+    bool hit = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) hit |= (x[e] & kExp) == kExp || (x[e] >> 16 & kExp) == kExp;
+    if (__builtin_amdgcn_ballot_w64(hit) != 0) {
+      bad |= 1u << i;
+      lds_st(L, at, u32x4{0, 0, 0, 0});
+    }
+  }
+  if (lane == 0) lds_st(L, buf + kBadOff + wave, (uint8_t)bad);
+}
+
 // kFp8: FP8 E4M3 cache rows (KT = bf16: the tiles are expanded to bf16 in
 // LDS and the MFMAs run on bf16).
 // kFilled: chunks over filled rows (ChunkWalk).
-template <typename KT, bool kPaged, bool kFp8, int kFilled>
-__device__ __forceinline__ void decode_mfma_body(const DecodeProblem& p, int groups) {
+// kTree: the sequences' last p.qps rows are the nodes of a tree, query tokens alike
+// (TreeStep): only the tiles that have nodes take the code for them. A head may
+// see no row of a tile there, even of a whole segment (its slot then weighs
+// nothing: its log-sum-exp is -infinity, its maximum kNoScore).
+template <typename KT, bool kPaged, bool kFp8, int kFilled, bool kTree = false>
+__device__ __forceinline__ void decode_mfma_body(const DecodeProblem& p, int groups, const TreeStep& tree = TreeStep{}) {
   static_assert(!kFp8 || std::is_same<KT, __hip_bfloat16>::value, "fp8 tiles expand to bf16");
   constexpr int kDma = dma_per_wave(kFp8);
   typedef Ops<KT> O_;
@@ -977,6 +1028,11 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeProblem& p, int gro
     sg.tile0 = (uint32_t)(sg.pos0 / kT);
     sg.rlim = p.rope_rows > 0 ? (int)(p.rope_rows - 1) : INT32_MAX;
     sg.pc = (int)min(sg.pos0, (int64_t)sg.rlim);
+    if constexpr (kTree) {  // (the lengths are within the regions, launch_tree_queries)
+      sg.node0 = (int)((int64_t)p.lens[s] - p.qps - sg.pos0);
+      sg.tcos = tree.cos + (int64_t)s * p.qps * (kDr / 2);
+      sg.tsin = tree.sin + (int64_t)s * p.qps * (kDr / 2);
+    }
     const int seg_len = sg.last + 1;
     const int ntiles = (seg_len + kT - 1) / kT;
 
@@ -1002,10 +1058,18 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeProblem& p, int gro
       asm volatile("" : "+v"(blk_cur));
     }
 
+    // what this lane's head sees: on its way before the copies, so it has landed with them
+    uint64_t seen = 0;
+    if constexpr (kTree) {
+      const int wblk = min(32 * wave, (hg_heads - 1) & ~31), r = min(lane_id() & 31, hg_heads - 1 - wblk);
+      const uint64_t* from = tree.seen + (int64_t)s * p.qps + (uint32_t)(group * kHG + wblk + r) / (uint32_t)p.nh;
+      asm volatile("global_load_dwordx2 %0, %1, off" : "=v"(seen) : "v"(from));
+    }
+
     // tile 1 rides along iteration -1; a fresh lane index keeps the per-lane
     // addresses out of the registers (and spill slots) that live across the
     // prologue: a spill reload here would wait on vmcnt and so serialise the copies
-    issue_tile_dma<kFp8>(p, sg, 0, base0, L, 0, wave, lane_id());
+    issue_tile_dma<kFp8, kTree>(p, sg, 0, base0, L, 0, wave, lane_id());
 
     // Q^T as the B operand: lane holds Q[head][16kk + 8*g2 .. +8], pre-scaled.
     // q_prep is stored in operand order (qprep_index): the wave's 32 rows form
@@ -1031,7 +1095,8 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeProblem& p, int gro
     }
     LA_STAMP(3);
 
-    float m_run = -INFINITY, l_run = 0.f;
+    constexpr float kFirst = kTree ? kNoScore : -INFINITY;
+    float m_run = kFirst, l_run = 0.f;
     // O = 0, written by MFMAs of zero operands straight into the AGPRs (a
     // zero vector built by the compiler would be kept in a spill slot)
     f32x16 acc[16];
@@ -1046,6 +1111,12 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeProblem& p, int gro
     LA_STAMP(4);
     rotate_rows<KT, kFp8>(L, 0, wave, lane_id());  // fresh lane index: no spilled addresses
     if constexpr (kFp8) expand_rows(L, 0, wave, lane_id());
+    if constexpr (kTree) {
+      asm volatile("" : "+v"(seen));
+      const int ln = lane_id();
+      if (ln < 32) lds_st(L, kSeenOff + 8 * (32 * wave + ln), seen);
+      if (kT > sg.node0) check_rows<KT>(L, 0, wave, lane_id());
+    }
     LA_STAMP(5);
 
     // Software pipeline over tiles; iteration t (from -1):
@@ -1255,8 +1326,8 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeProblem& p, int gro
         if constexpr (kk + D < 36) a = a_rd(std::integral_constant<int, kk + D>());
         constexpr int cm = (kk - kCopyFirst) / kCopyStride;  // the copy of this step, if any
         if constexpr (kk >= kCopyFirst && (kk - kCopyFirst) % kCopyStride == 0 && cm < kDma) {
-          if constexpr (kFp8) issue_copy_fp8<cm>(p, sg, t + 2, L, dbuf, wave, lane, dm);
-          else issue_copy<dma_order(cm)>(p, sg, t + 2, L, dbuf, wave, lane, dm);
+          if constexpr (kFp8) issue_copy_fp8<cm, kTree>(p, sg, t + 2, L, dbuf, wave, lane, dm);
+          else issue_copy<dma_order(cm), kTree>(p, sg, t + 2, L, dbuf, wave, lane, dm);
         }
         if constexpr (kk >= kTrAt && kk - kTrAt < kPvDepth) b_issue(tr[kk - kTrAt], std::integral_constant<int, kk - kTrAt>());
         qk_setup(kk_c);
@@ -1295,7 +1366,26 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeProblem& p, int gro
         constexpr int step = decltype(step_c)::value;
         if constexpr (step == kSmSettle) {
           settle1(s_next);
-          if (sm && valid < kT) {
+          if constexpr (kTree) {
+            const int at = (t + 1) * kT - sg.node0;  // node of the tile's first row, or less: rows before the nodes
+            if (sm && (valid < kT || at > -kT)) {
+              const uint64_t seen = lds_ld<uint64_t>(L, kSeenOff + 8 * (32 * wave + (lane & 31)));
+              uint32_t see = at >= 0     ? at < 64 ? (uint32_t)(seen >> at) : 0u
+                             : at > -kT ? (uint32_t)(seen << -at) | ((1u << -at) - 1)
+                                        : ~0u;
+              if (valid < kT) see &= (1u << valid) - 1;
+              const uint32_t mine = see >> (4 * g2);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) s_next[i] = mine >> (8 * (i >> 2) + (i & 3)) & 1 ? s_next[i] : -INFINITY;
+              const uint32_t bad = at > -kT ? lds_ld<uint32_t>(L, nxt + kBadOff) : 0u;
+              if (__builtin_amdgcn_readfirstlane((int)bad) != 0) {
+                const uint32_t hit = (bad & see) >> (4 * g2);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                  if (hit >> (8 * (i >> 2) + (i & 3)) & 1) s_next[i] = __builtin_nanf("");
+              }
+            }
+          } else if (sm && valid < kT) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const int pos = 8 * (i >> 2) + 4 * g2 + (i & 3);
@@ -1326,7 +1416,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeProblem& p, int gro
           if (__builtin_amdgcn_ballot_w64(need) != 0) {
             const float tmax = max_halves(lmax);
             const float m_new = fmaxf(m_run, tmax);
-            const bool first = m_run == -INFINITY;
+            const bool first = m_run == kFirst;
             const float alpha = first ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
             m_run = m_new;
             l_run *= alpha;
@@ -1515,6 +1605,9 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeProblem& p, int gro
       LA_TSTAMP(tt3);
 #endif
       wait_vm<0>();  // this wave's copies of tile t+2 (issued in this iteration) have landed
+      if constexpr (kTree) {
+        if (t + 2 < ntiles && (t + 3) * kT > sg.node0) check_rows<KT>(L, dbuf, wave, lane_id());
+      }
       if constexpr (kPaged) tie(blk_cur);  // and the table entry loaded with them
 #ifdef LA_PHASE_STAMPS
       LA_TSTAMP(tt4);
@@ -1678,6 +1771,12 @@ __global__ __launch_bounds__(kThreads) void decode_mfma_filled_kernel(DecodeProb
   decode_mfma_body<KT, false, kFp8, 2>(p, groups);
 }
 
+// Trees of drafted tokens: kFilled 1 (paged), 2 or 0 (contiguous, filled rows or regions).
+template <typename KT, bool kPaged, bool kFp8, int kFilled>
+__global__ __launch_bounds__(kThreads) void decode_mfma_tree_kernel(DecodeProblem p, int groups, TreeStep tree) {
+  decode_mfma_body<KT, kPaged, kFp8, kFilled, true>(p, groups, tree);
+}
+
 // Copies-only variant of the attention kernel, for measuring the streaming
 // ceiling of its copy schedule: the same grid and block mapping
 // (block_coords), the same segment walk, and per tile the same 11 HBM->LDS
@@ -1785,19 +1884,21 @@ __global__ __launch_bounds__(256) void prep_q_kernel(const float* __restrict__ q
   *reinterpret_cast<vec*>(out + qprep_index(qrow, 8 * j)) = v;
 }
 
-hipError_t launch_k(void (*k)(DecodeProblem, int), OncePerDevice& once, const DecodeProblem& p, hipStream_t stream,
-                    hipEvent_t ev_begin, hipEvent_t ev_end) {
+hipError_t allow_whole_lds(OncePerDevice& once, const void* fn, int bytes) {
   int dev = 0;
-  hipError_t e = hipGetDevice(&dev);
+  const hipError_t e = hipGetDevice(&dev);
   if (e != hipSuccess) return e;
-  e = once.run(dev, [&] {
-    const void* fn = reinterpret_cast<const void*>(k);
+  return once.run(dev, [&] {
     hipFuncAttributes fa;
     const hipError_t f = hipFuncGetAttributes(&fa, fn);
     if (f != hipSuccess) return f;
     if (fa.sharedSizeBytes != 0) return hipErrorInvalidKernelFile;  // LDS offsets would not be addresses
-    return hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
+    return hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   });
+}
+hipError_t launch_k(void (*k)(DecodeProblem, int), OncePerDevice& once, const DecodeProblem& p, hipStream_t stream,
+                    hipEvent_t ev_begin, hipEvent_t ev_end) {
+  const hipError_t e = allow_whole_lds(once, reinterpret_cast<const void*>(k), kLdsBytes);
   if (e != hipSuccess) return e;
   const int groups = (p.Hq + kHG - 1) / kHG;
   const dim3 blocks((unsigned)mfma_grid_blocks(p.num_chunks, groups));
@@ -1814,6 +1915,23 @@ hipError_t launch_t(const DecodeProblem& p, hipStream_t stream, hipEvent_t ev_be
   if (p.block_table) return launch_k(decode_mfma_kernel<KT, true, kFp8>, once[0], p, stream, ev_begin, ev_end);
   if (p.chunk_len < 0) return launch_k(decode_mfma_filled_kernel<KT, kFp8>, once[1], p, stream, ev_begin, ev_end);
   return launch_k(decode_mfma_kernel<KT, false, kFp8>, once[2], p, stream, ev_begin, ev_end);
+}
+
+template <typename KT, bool kPaged, bool kFp8, int kFilled>
+hipError_t launch_tree_k(const DecodeProblem& p, const TreeStep& tree, hipStream_t stream) {
+  static OncePerDevice once;
+  const auto k = decode_mfma_tree_kernel<KT, kPaged, kFp8, kFilled>;
+  const hipError_t e = allow_whole_lds(once, reinterpret_cast<const void*>(k), kTreeLdsBytes);
+  if (e != hipSuccess) return e;
+  const int groups = (p.Hq + kHG - 1) / kHG;
+  hipLaunchKernelGGL(k, dim3((unsigned)mfma_grid_blocks(p.num_chunks, groups)), dim3(kThreads), kTreeLdsBytes, stream, p, groups, tree);
+  return hipGetLastError();
+}
+template <typename KT, bool kFp8>
+hipError_t launch_tree_t(const DecodeProblem& p, const TreeStep& tree, hipStream_t stream) {
+  if (p.block_table) return launch_tree_k<KT, true, kFp8, 1>(p, tree, stream);
+  if (p.chunk_len < 0) return launch_tree_k<KT, false, kFp8, 2>(p, tree, stream);
+  return launch_tree_k<KT, false, kFp8, 0>(p, tree, stream);
 }
 
 }  // namespace
@@ -1888,6 +2006,13 @@ hipError_t launch_decode_mfma(const DecodeProblem& p, hipStream_t stream, hipEve
   if (p.kv_dtype == LA_DTYPE_FP8_E4M3) return launch_t<__hip_bfloat16, true>(p, stream, ev_begin, ev_end);
   if (p.kv_dtype == LA_DTYPE_BF16) return launch_t<__hip_bfloat16, false>(p, stream, ev_begin, ev_end);
   return launch_t<__half, false>(p, stream, ev_begin, ev_end);
+}
+
+hipError_t launch_decode_mfma_tree(const DecodeProblem& p, const TreeStep& tree, hipStream_t stream) {
+  if (!p.lens || p.qps < 1 || p.qps > LA_TREE_MAX_NODES) return hipErrorInvalidValue;
+  if (p.kv_dtype == LA_DTYPE_FP8_E4M3) return launch_tree_t<__hip_bfloat16, true>(p, tree, stream);
+  if (p.kv_dtype == LA_DTYPE_BF16) return launch_tree_t<__hip_bfloat16, false>(p, tree, stream);
+  return launch_tree_t<__half, false>(p, tree, stream);
 }
 
 #ifdef LA_PHASE_STAMPS
