@@ -1446,6 +1446,7 @@ bool moved_rows(const Args* a, MovedRows* out) {
     return false;
   }
   if (a->num_seqs > 0 && (!a->seq_lens || (a->total_rows > 0 && !a->kv_cache))) return false;
+  if (a->total_rows > (int64_t)UINT32_MAX) return false;  // rows are 32-bit numbers there
   const int64_t row = (int64_t)a->cfg.kv_lora_rank + a->cfg.qk_rope_head_dim;
   if (row > INT32_MAX / 4) return false;
   MovedRows r{};
@@ -1572,10 +1573,13 @@ int evict(const la_evict_args* a, hipStream_t stream, bool run_it, size_t* need)
   p.keep = a->keep;
   p.first = a->first;
   p.last = a->last;
+  const bool staged = evict_staged(p, cu_count());
   auto carve = [&](void* ws) {
     Carve v(ws);
     p.start = static_cast<int32_t*>(v.take((size_t)a->num_seqs * sizeof(int32_t)));
     p.kept = a->kept ? a->kept : static_cast<int32_t*>(v.take((size_t)a->num_seqs * a->keep * sizeof(int32_t)));
+    p.from = static_cast<uint32_t*>(v.take((size_t)a->num_seqs * a->keep * sizeof(uint32_t)));
+    if (staged) p.staged = static_cast<char*>(v.take((size_t)a->num_seqs * a->keep * p.rows.row_bytes));
     return v.total();
   };
   const size_t total = carve(nullptr);

@@ -65,13 +65,13 @@ __device__ inline int moved_room(const MovedRows& r, int s) {
   return (int)max(clamp64(r.offsets[s + 1], 0, r.total_rows) - moved_begin(r, s), (int64_t)0);
 }
 // Row of position pos, which lies in the sequence's room (block ids are clamped into the pool).
+__device__ inline int64_t moved_index(const MovedRows& r, int s, int64_t begin, int pos) {
+  if (!r.block_table) return begin + pos;
+  const int64_t b = clamp64(r.block_table[(int64_t)s * r.blocks_per_seq + pos / r.block_size], 0, r.pool_blocks - 1);
+  return b * r.block_size + pos % r.block_size;
+}
 __device__ inline char* moved_row(const MovedRows& r, int s, int64_t begin, int pos) {
-  int64_t row = begin + pos;
-  if (r.block_table) {
-    const int64_t b = clamp64(r.block_table[(int64_t)s * r.blocks_per_seq + pos / r.block_size], 0, r.pool_blocks - 1);
-    row = b * r.block_size + pos % r.block_size;
-  }
-  return r.kv + row * r.row_bytes;
+  return r.kv + moved_index(r, s, begin, pos) * r.row_bytes;
 }
 // Between the reads of rows that move and the barrier after which others write there: the
 // barrier alone does not wait for loads.
@@ -124,9 +124,13 @@ struct EvictProblem {
   MovedRows rows;
   float* weights;
   int keep, first, last;
-  int32_t* kept;   // (num_seqs, keep)
-  int32_t* start;  // (num_seqs): the first position that changes rows, keep if none does
+  int32_t* kept;    // (num_seqs, keep)
+  int32_t* start;   // (num_seqs): the first position that gets another row, keep if none does
+  uint32_t* from;   // (num_seqs, keep): the rows that stay, as rows of the cache
+  char* staged;     // evict_staged: (num_seqs, keep) rows; else nullptr
 };
+// Whether the rows go through a copy of them (few sequences: fewer stripes than compute units).
+bool evict_staged(const EvictProblem& p, int ncu);
 hipError_t launch_evict(const EvictProblem& p, hipStream_t stream);
 
 }  // namespace la

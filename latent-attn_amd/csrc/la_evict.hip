@@ -2,23 +2,29 @@
 // rows and the heaviest ones between, in order and in place.
 //
 // Selection, one workgroup per sequence: the weights become keys that order as
-// unsigned numbers, the k-th largest key is found 8 bits at a time from
-// histograms in LDS (radix selection), and one pass in order keeps what is
-// larger and as many of the equal ones as are left, earliest first, moving the
-// weights on its way (position i goes to i or before, and a pass's writes follow
-// its reads).
+// unsigned numbers, the k-th largest key is found 11 bits at a time from
+// histograms in LDS (radix selection: three passes over the keys, which stay in
+// registers up to 16,384 rows), and one pass in order keeps what is larger and as
+// many of the equal ones as are left, earliest first, moving the weights on its
+// way (position i goes to i or before, and a pass's writes follow its reads).
+// Every thread has consecutive rows, so a rank is one scan over the threads.
 //
 // Movement: rows only move down, and the columns of a row are independent of
 // one another. So a workgroup owns a stripe of columns of a sequence and goes
 // through the kept rows in order, a tile of them read before any of it is
 // written: no row is overwritten before its stripe is read, and no workgroup
-// waits for another.
+// waits for another. A few sequences have too few stripes for that; their rows go
+// through a copy, two launches over all compute units.
 #include "la_draft.hpp"
+
+#include <algorithm>
+#include <type_traits>
 
 namespace la {
 namespace {
 
-constexpr int kSelectThreads = 1024;
+constexpr int kSelectThreads = 1024, kItems = 16, kSegment = kItems * kSelectThreads;
+constexpr int kBins = 2048;
 
 // Largest first; NaN below everything, -0 as 0.
 __device__ inline uint32_t key_of(float w) {
@@ -34,138 +40,209 @@ __device__ inline int block_scan(int v, int* sums, int* total) {
   __syncthreads();
   if (lane == 63) sums[wave] = in;
   __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < kSelectThreads / 64; ++w) {
-    before += w < wave ? sums[w] : 0;
-    all += sums[w];
-  }
-  *total = all;
-  return before + in - v;
+  const int mine = lane < kSelectThreads / 64 ? sums[lane] : 0, end = wave_scan(mine);
+  *total = __builtin_amdgcn_readlane(end, 63);
+  return __shfl(end - mine, wave, 64) + in - v;
 }
 
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictProblem p, int64_t first_seq) {
-  __shared__ int hist[256];
+  __shared__ int hist[kBins];
   __shared__ int sums[kSelectThreads / 64];
-  __shared__ uint32_t pick[2];
-  const int s = (int)first_seq + blockIdx.x;
+  __shared__ int pick[2];
+  const int s = (int)first_seq + blockIdx.x, tid = threadIdx.x;
   const int64_t begin = moved_begin(p.rows, s);
   const int L = max(min(p.rows.lens[s], moved_room(p.rows, s)), 0);
   float* const w = p.weights + begin;
   int32_t* const kept = p.kept + (int64_t)s * p.keep;
   if (L <= p.keep) {
-    for (int i = threadIdx.x; i < p.keep; i += kSelectThreads) kept[i] = i < L ? i : -1;
-    if (threadIdx.x == 0) p.start[s] = p.keep;
+    for (int i = tid; i < p.keep; i += kSelectThreads) kept[i] = i < L ? i : -1;
+    if (tid == 0) p.start[s] = p.keep;
     return;
   }
   const int lo = p.first, hi = L - p.last;  // the rows between
   int left = p.keep - p.first - p.last;     // of which so many stay
+  const int segments = (L + kSegment - 1) / kSegment;
+  // of segment g this thread has rows at(g) .. + each(g) - 1
+  auto each = [&](int g) { return (min(L - g * kSegment, kSegment) + kSelectThreads - 1) / kSelectThreads; };
+  auto at = [&](int g) { return g * kSegment + tid * each(g); };
+  float x[kItems];
+  auto load = [&](int g) {
+    const int n = each(g), i0 = at(g);
+#pragma unroll
+    for (int e = 0; e < kItems; ++e) x[e] = e < n && i0 + e < L ? w[i0 + e] : 0.f;
+  };
+  load(0);
   // the left-th largest key between, and how many equal to it stay
-  uint32_t prefix = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += kSelectThreads) hist[i] = 0;
-    __syncthreads();
-    for (int i = lo + threadIdx.x; i < hi; i += kSelectThreads) {
-      const uint32_t k = key_of(w[i]);
-      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
+  uint32_t prefix = left > 0 ? 0 : ~0u;  // (no key is as large: nothing between stays)
+  if (left > 0) {
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+      for (int i = tid; i < kBins; i += kSelectThreads) hist[i] = 0;
+      __syncthreads();
+      for (int g = 0; g < segments; ++g) {
+        if (segments > 1) load(g);
+        const int n = each(g), i0 = at(g);
+#pragma unroll
+        for (int e = 0; e < kItems; ++e) {
+          const uint32_t k = key_of(x[e]);
+          if (e < n && i0 + e >= lo && i0 + e < hi && (pass == 0 || k >> (shift + bits) == prefix >> (shift + bits)))
+            atomicAdd(&hist[k >> shift & ((1 << bits) - 1)], 1);
+        }
+      }
+      __syncthreads();
+      // this thread's two bins, from the largest down
+      const int b = kBins - 1 - 2 * tid, c0 = hist[b], c1 = hist[b - 1];
+      int total;
+      const int more = block_scan(c0 + c1, sums, &total);
+      if (more < left && left <= more + c0 + c1) {
+        const bool second = left > more + c0;
+        pick[0] = second ? b - 1 : b;
+        pick[1] = left - more - (second ? c0 : 0);
+      }
+      __syncthreads();
+      prefix |= (uint32_t)pick[0] << shift;
+      left = pick[1];
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int n = left, b = 255;
-      while (b > 0 && hist[b] < n) n -= hist[b--];
-      pick[0] = (uint32_t)b;
-      pick[1] = (uint32_t)n;
-    }
-    __syncthreads();
-    prefix |= pick[0] << shift;
-    left = (int)pick[1];
-    __syncthreads();
   }
-  // in order: what is larger, the first `left` of the equal ones (none where no row between stays)
-  if (p.keep == p.first + p.last) prefix = ~0u, left = 0;
-  int at = 0, equal = 0;
-  for (int i0 = 0; i0 < L; i0 += kSelectThreads) {
-    const int i = i0 + threadIdx.x;
-    const float x = i < L ? w[i] : 0.f;
-    const uint32_t k = key_of(x);
-    const bool between = i >= lo && i < hi, same = between && k == prefix;
-    int total;
-    const int rank = equal + block_scan(same ? 1 : 0, sums, &total);
+  __syncthreads();
+  if (tid == 0) pick[0] = p.keep;
+  // in order: what is larger, and the first `left` of the equal ones
+  int done = 0, equal = 0;
+  for (int g = 0; g < segments; ++g) {
+    if (segments > 1) load(g);
+    const int n = each(g), i0 = at(g);
+    int same = 0, total;
+#pragma unroll
+    for (int e = 0; e < kItems; ++e) same += e < n && i0 + e >= lo && i0 + e < hi && key_of(x[e]) == prefix;
+    int rank = equal + block_scan(same, sums, &total);
     equal += total;
-    const bool stays = i < L && (!between || (same ? rank < left : k > prefix));
-    const int to = at + block_scan(stays ? 1 : 0, sums, &total);  // (its barriers: every weight of the pass is read)
-    if (stays) {
-      kept[to] = i;
-      if (to != i) w[to] = x;
+    uint32_t stays = 0;
+#pragma unroll
+    for (int e = 0; e < kItems; ++e) {
+      const int i = i0 + e;
+      const uint32_t k = key_of(x[e]);
+      const bool between = i >= lo && i < hi;
+      if (e < n && i < L && (!between || k > prefix || (k == prefix && rank < left))) stays |= 1u << e;
+      rank += e < n && between && k == prefix;
     }
-    at += total;
+    int to = done + block_scan(__popc(stays), sums, &total);  // (its barriers: every weight of the segment is read)
+    done += total;
+    int moves = p.keep;
+#pragma unroll
+    for (int e = 0; e < kItems; ++e)
+      if (stays >> e & 1) {
+        kept[to] = i0 + e;
+        p.from[(int64_t)s * p.keep + to] = (uint32_t)moved_index(p.rows, s, begin, i0 + e);
+        if (to != i0 + e) {
+          w[to] = x[e];
+          moves = min(moves, to);
+        }
+        ++to;
+      }
+    if (moves < p.keep) atomicMin(&pick[0], moves);
   }
   __syncthreads();
-  for (int i = p.keep + threadIdx.x; i < L; i += kSelectThreads) w[i] = 0.f;
-  // the first position that gets another row
-  if (threadIdx.x == 0) pick[0] = (uint32_t)p.keep;
-  __syncthreads();
-  for (int i = threadIdx.x; i < p.keep; i += kSelectThreads)
-    if (kept[i] != i) {
-      atomicMin(&pick[0], (uint32_t)i);
-      break;
-    }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    p.start[s] = (int)pick[0];
+  for (int i = p.keep + tid; i < L; i += kSelectThreads) w[i] = 0.f;
+  if (tid == 0) {
+    p.start[s] = pick[0];
     p.rows.lens[s] = p.keep;
   }
 }
 
-// kRows rows of kLanes units of kU bytes at a time, kDeep of these in flight.
-constexpr int kMoveThreads = 256;
-template <typename U, int kLanes>
+// kLanes units of U per row and workgroup, kRows rows at a time, kDeep of these in
+// flight and as many more on their way behind them.
+constexpr int kMoveThreads = 256, kLanes = 8, kRows = kMoveThreads / kLanes, kDeep = 8;
+template <typename U>
 __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictProblem p, int stripes, int64_t first) {
-  constexpr int kRows = kMoveThreads / kLanes, kDeep = 8;
   const int64_t item = first + blockIdx.x;
-  const int s = (int)(item / stripes), column = (int)(item % stripes) * kLanes + threadIdx.x % kLanes;
-  const int row = threadIdx.x / kLanes;
-  const bool in = column < (int)(p.rows.row_bytes / sizeof(U));
+  const int s = (int)(item / stripes), units = (int)(p.rows.row_bytes / sizeof(U));
+  const int column = (int)(item % stripes) * kLanes + threadIdx.x % kLanes, row = threadIdx.x / kLanes;
+  const bool in = column < units;
   const int64_t begin = moved_begin(p.rows, s);
-  const int32_t* const kept = p.kept + (int64_t)s * p.keep;
-  for (int i0 = p.start[s]; i0 < p.keep; i0 += kRows * kDeep) {
-    U v[kDeep];
+  const uint32_t* const from = p.from + (int64_t)s * p.keep;
+  const U* const base = reinterpret_cast<const U*>(p.rows.kv) + min(column, units - 1);
+  const int start = p.start[s];
+  if (start >= p.keep) return;
+  typedef typename std::conditional<(sizeof(U) < 4), uint32_t, U>::type H;  // (a register each)
+  auto load = [&](int i0, H(&v)[kDeep]) {  // (rows past the last: the last again)
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) v[k] = base[(int64_t)from[min(i0 + k * kRows + row, p.keep - 1)] * units];
+  };
+  auto store = [&](int i0, H(&v)[kDeep]) {
 #pragma unroll
     for (int k = 0; k < kDeep; ++k) {
       const int i = i0 + k * kRows + row;
-      if (in && i < p.keep) v[k] = reinterpret_cast<const U*>(moved_row(p.rows, s, begin, kept[i]))[column];
+      if (in && i < p.keep) reinterpret_cast<U*>(moved_row(p.rows, s, begin, i))[column] = (U)v[k];
     }
-    rows_read();
-    __syncthreads();
+  };
+  // everyone's rows of a tile are read before anyone writes it
+  auto read = [](H(&v)[kDeep]) {
 #pragma unroll
-    for (int k = 0; k < kDeep; ++k) {
-      const int i = i0 + k * kRows + row;
-      if (in && i < p.keep) reinterpret_cast<U*>(moved_row(p.rows, s, begin, i))[column] = v[k];
-    }
+    for (int k = 0; k < kDeep; ++k) asm volatile("" : "+v"(v[k]));
+    lds_barrier();
+  };
+  constexpr int kTile = kRows * kDeep;
+  H a[kDeep], b[kDeep];
+  load(start, a);
+  for (int i0 = start; i0 < p.keep; i0 += 2 * kTile) {
+    load(min(i0 + kTile, p.keep - 1), b);
+    read(a);
+    store(i0, a);
+    if (i0 + kTile >= p.keep) break;
+    load(min(i0 + 2 * kTile, p.keep - 1), a);
+    read(b);
+    store(i0 + kTile, b);
   }
 }
 
-struct alignas(16) Unit16 {
-  uint32_t x[4];
-};
+// Unit by unit, to the copy (kOut) and back.
+template <typename U, bool kOut>
+__global__ __launch_bounds__(256) void evict_copy_kernel(EvictProblem p, int blocks_per) {
+  const int s = blockIdx.x / blocks_per, b = blockIdx.x % blocks_per, units = (int)(p.rows.row_bytes / sizeof(U));
+  const int start = p.start[s];
+  const int64_t begin = moved_begin(p.rows, s), all = (int64_t)(p.keep - start) * units;
+  U* const copy = reinterpret_cast<U*>(p.staged) + ((int64_t)s * p.keep + start) * units;
+  const uint32_t* const from = p.from + (int64_t)s * p.keep;
+  for (int64_t u = (int64_t)b * 256 + threadIdx.x; u < all; u += (int64_t)blocks_per * 256) {
+    const int i = start + (int)(u / units), c = (int)(u % units);
+    if constexpr (kOut) copy[u] = (reinterpret_cast<const U*>(p.rows.kv) + (int64_t)from[i] * units)[c];
+    else reinterpret_cast<U*>(moved_row(p.rows, s, begin, i))[c] = copy[u];
+  }
+}
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 template <typename U>
 hipError_t move_t(const EvictProblem& p, hipStream_t stream) {
-  constexpr int kLanes = 8;
-  const int stripes = (int)((p.rows.row_bytes / sizeof(U) + kLanes - 1) / kLanes);
+  const int64_t units = p.rows.row_bytes / sizeof(U);
+  if (p.staged) {
+    const int64_t each = (p.keep * units + 1023) / 1024, most = std::max<int64_t>(4096 / p.rows.num_seqs, 1);
+    const int blocks = (int)std::max<int64_t>(std::min(each, most), 1);
+    hipLaunchKernelGGL((evict_copy_kernel<U, true>), dim3((unsigned)(p.rows.num_seqs * blocks)), dim3(256), 0, stream, p, blocks);
+    hipLaunchKernelGGL((evict_copy_kernel<U, false>), dim3((unsigned)(p.rows.num_seqs * blocks)), dim3(256), 0, stream, p, blocks);
+    return hipGetLastError();
+  }
+  const int stripes = (int)((units + kLanes - 1) / kLanes);
   return in_grids((int64_t)p.rows.num_seqs * stripes, most_blocks(kMoveThreads), [&](int64_t first, unsigned blocks) {
-    hipLaunchKernelGGL((evict_move_kernel<U, kLanes>), dim3(blocks), dim3(kMoveThreads), 0, stream, p, stripes, first);
+    hipLaunchKernelGGL(evict_move_kernel<U>, dim3(blocks), dim3(kMoveThreads), 0, stream, p, stripes, first);
   });
 }
 
 }  // namespace
 
+bool evict_staged(const EvictProblem& p, int ncu) {
+  const int unit = moved_unit(p.rows);
+  return p.rows.num_seqs * ((p.rows.row_bytes / unit + kLanes - 1) / kLanes) < ncu / 2;
+}
+
 hipError_t launch_evict(const EvictProblem& p, hipStream_t stream) {
   const hipError_t e = in_grids(p.rows.num_seqs, most_blocks(kSelectThreads), [&](int64_t first, unsigned blocks) {
     hipLaunchKernelGGL(evict_select_kernel, dim3(blocks), dim3(kSelectThreads), 0, stream, p, first);
   });
-  if (e != hipSuccess) return e;
+  if (e != hipSuccess || p.keep == 0) return e;
   switch (moved_unit(p.rows)) {
-    case 16: return move_t<Unit16>(p, stream);
+    case 16: return move_t<u32x4>(p, stream);
     case 8: return move_t<uint64_t>(p, stream);
     case 4: return move_t<uint32_t>(p, stream);
     case 2: return move_t<uint16_t>(p, stream);
