@@ -7,7 +7,7 @@
 // registers up to 16,384 rows), and one pass in order keeps what is larger and as
 // many of the equal ones as are left, earliest first, moving the weights on its
 // way (position i goes to i or before, and a pass's writes follow its reads).
-// Every thread has consecutive rows, so a rank is one scan over the threads.
+// Every wave has consecutive rows, so ranks are ballots and one sum over the waves.
 //
 // Movement: rows only move down, and the columns of a row are independent of
 // one another. So a workgroup owns a stripe of columns of a sequence and goes
@@ -23,7 +23,7 @@
 namespace la {
 namespace {
 
-constexpr int kSelectThreads = 1024, kItems = 16, kSegment = kItems * kSelectThreads;
+constexpr int kItems = 16;  // rows of a lane at a time
 constexpr int kBins = 2048;
 
 // Largest first; NaN below everything, -0 as 0.
@@ -33,119 +33,150 @@ __device__ inline uint32_t key_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Exclusive sum over the workgroup's threads in order, and the total.
-__device__ inline int block_scan(int v, int* sums, int* total) {
+// Sum of v over the waves before this one, and over all; one barrier (`sums` is used once).
+template <int kW>
+__device__ inline int wave_rank(int v, int* sums, int* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int in = wave_scan(v);
+  if (lane == 0) sums[wave] = v;
   __syncthreads();
-  if (lane == 63) sums[wave] = in;
-  __syncthreads();
-  const int mine = lane < kSelectThreads / 64 ? sums[lane] : 0, end = wave_scan(mine);
+  const int mine = lane < kW ? sums[lane] : 0, end = wave_scan(mine);
   *total = __builtin_amdgcn_readlane(end, 63);
-  return __shfl(end - mine, wave, 64) + in - v;
+  return __builtin_amdgcn_readlane(end - mine, __builtin_amdgcn_readfirstlane(wave));
 }
 
-__global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictProblem p, int64_t first_seq) {
-  __shared__ int hist[kBins];
-  __shared__ int sums[kSelectThreads / 64];
-  __shared__ int pick[2];
-  const int s = (int)first_seq + blockIdx.x, tid = threadIdx.x;
+template <int kW>
+__global__ __launch_bounds__(64 * kW) void evict_select_kernel(EvictProblem p, int64_t first_seq) {
+  constexpr int kThreads = 64 * kW, kSegment = kItems * kThreads;
+  __shared__ int hist[3][kBins];
+  __shared__ int sums[5][kW];
+  __shared__ int pick[3][2];
+  __shared__ int moved;
+  const int s = (int)first_seq + blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t begin = moved_begin(p.rows, s);
   const int L = max(min(p.rows.lens[s], moved_room(p.rows, s)), 0);
   float* const w = p.weights + begin;
   int32_t* const kept = p.kept + (int64_t)s * p.keep;
+  uint32_t* const from = p.from + (int64_t)s * p.keep;
   if (L <= p.keep) {
-    for (int i = tid; i < p.keep; i += kSelectThreads) kept[i] = i < L ? i : -1;
+    for (int i = tid; i < p.keep; i += kThreads) kept[i] = i < L ? i : -1;
     if (tid == 0) p.start[s] = p.keep;
     return;
   }
   const int lo = p.first, hi = L - p.last;  // the rows between
   int left = p.keep - p.first - p.last;     // of which so many stay
   const int segments = (L + kSegment - 1) / kSegment;
-  // of segment g this thread has rows at(g) .. + each(g) - 1
-  auto each = [&](int g) { return (min(L - g * kSegment, kSegment) + kSelectThreads - 1) / kSelectThreads; };
-  auto at = [&](int g) { return g * kSegment + tid * each(g); };
+  // of segment g a wave has 64 each(g) rows from at(g) on, 64 at a time
+  auto each = [&](int g) { return (min(L - g * kSegment, kSegment) + kThreads - 1) / kThreads; };
+  auto at = [&](int g) { return g * kSegment + wave * 64 * each(g) + lane; };
   float x[kItems];
   auto load = [&](int g) {
     const int n = each(g), i0 = at(g);
 #pragma unroll
-    for (int e = 0; e < kItems; ++e) x[e] = e < n && i0 + e < L ? w[i0 + e] : 0.f;
+    for (int e = 0; e < kItems; ++e) x[e] = e < n && i0 + 64 * e < L ? w[i0 + 64 * e] : 0.f;
   };
   load(0);
+  for (int i = tid; i < 3 * kBins; i += kThreads) hist[0][i] = 0;
+  if (tid == 0) moved = p.keep;
+  __syncthreads();
   // the left-th largest key between, and how many equal to it stay
   uint32_t prefix = left > 0 ? 0 : ~0u;  // (no key is as large: nothing between stays)
   if (left > 0) {
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-      for (int i = tid; i < kBins; i += kSelectThreads) hist[i] = 0;
-      __syncthreads();
       for (int g = 0; g < segments; ++g) {
         if (segments > 1) load(g);
         const int n = each(g), i0 = at(g);
 #pragma unroll
         for (int e = 0; e < kItems; ++e) {
+          if (e >= n) break;
+          const int i = i0 + 64 * e;
           const uint32_t k = key_of(x[e]);
-          if (e < n && i0 + e >= lo && i0 + e < hi && (pass == 0 || k >> (shift + bits) == prefix >> (shift + bits)))
-            atomicAdd(&hist[k >> shift & ((1 << bits) - 1)], 1);
+          if (i >= lo && i < hi && (pass == 0 || k >> (shift + bits) == prefix >> (shift + bits)))
+            atomicAdd(&hist[pass][k >> shift & ((1 << bits) - 1)], 1);
         }
       }
       __syncthreads();
-      // this thread's two bins, from the largest down
-      const int b = kBins - 1 - 2 * tid, c0 = hist[b], c1 = hist[b - 1];
+      // this thread's bins, from the largest down
+      constexpr int kEach = kBins / kThreads;
+      int c[kEach], own = 0;
+#pragma unroll
+      for (int q = 0; q < kEach; ++q) own += c[q] = hist[pass][kBins - 1 - kEach * tid - q];
+      const int in = wave_scan(own);
       int total;
-      const int more = block_scan(c0 + c1, sums, &total);
-      if (more < left && left <= more + c0 + c1) {
-        const bool second = left > more + c0;
-        pick[0] = second ? b - 1 : b;
-        pick[1] = left - more - (second ? c0 : 0);
+      int more = wave_rank<kW>(__builtin_amdgcn_readlane(in, 63), sums[pass], &total) + in - own;
+      if (more < left && left <= more + own) {
+#pragma unroll
+        for (int q = 0; q < kEach; ++q) {
+          if (more < left && left <= more + c[q]) {
+            pick[pass][0] = kBins - 1 - kEach * tid - q;
+            pick[pass][1] = left - more;
+          }
+          more += c[q];
+        }
       }
       __syncthreads();
-      prefix |= (uint32_t)pick[0] << shift;
-      left = pick[1];
+      prefix |= (uint32_t)pick[pass][0] << shift;
+      left = pick[pass][1];
     }
   }
-  __syncthreads();
-  if (tid == 0) pick[0] = p.keep;
   // in order: what is larger, and the first `left` of the equal ones
-  int done = 0, equal = 0;
+  const uint64_t before = (1ull << lane) - 1;
+  int done = 0, equal = 0, moves = p.keep;
   for (int g = 0; g < segments; ++g) {
-    if (segments > 1) load(g);
+    if (segments > 1) {
+      load(g);
+      __syncthreads();  // the sums of the segment before are read
+    }
     const int n = each(g), i0 = at(g);
     int same = 0, total;
 #pragma unroll
-    for (int e = 0; e < kItems; ++e) same += e < n && i0 + e >= lo && i0 + e < hi && key_of(x[e]) == prefix;
-    int rank = equal + block_scan(same, sums, &total);
+    for (int e = 0; e < kItems; ++e) {
+      if (e >= n) break;
+      const int i = i0 + 64 * e;
+      same += __popcll(__builtin_amdgcn_ballot_w64(i >= lo && i < hi && key_of(x[e]) == prefix));
+    }
+    int rank = equal + wave_rank<kW>(same, sums[3], &total);
     equal += total;
     uint32_t stays = 0;
+    int count = 0;
 #pragma unroll
     for (int e = 0; e < kItems; ++e) {
-      const int i = i0 + e;
+      if (e >= n) break;
+      const int i = i0 + 64 * e;
       const uint32_t k = key_of(x[e]);
-      const bool between = i >= lo && i < hi;
-      if (e < n && i < L && (!between || k > prefix || (k == prefix && rank < left))) stays |= 1u << e;
-      rank += e < n && between && k == prefix;
+      const bool between = i >= lo && i < hi, is = between && k == prefix;
+      const uint64_t all = __builtin_amdgcn_ballot_w64(is);
+      const bool stay = i < L && (!between || k > prefix || (is && rank + __popcll(all & before) < left));
+      rank += __popcll(all);
+      stays |= (uint32_t)stay << e;
+      count += __popcll(__builtin_amdgcn_ballot_w64(stay));
     }
-    int to = done + block_scan(__popc(stays), sums, &total);  // (its barriers: every weight of the segment is read)
+    int to = done + wave_rank<kW>(count, sums[4], &total);  // (its barrier: every weight of the segment is read)
     done += total;
-    int moves = p.keep;
 #pragma unroll
-    for (int e = 0; e < kItems; ++e)
-      if (stays >> e & 1) {
-        kept[to] = i0 + e;
-        p.from[(int64_t)s * p.keep + to] = (uint32_t)moved_index(p.rows, s, begin, i0 + e);
-        if (to != i0 + e) {
-          w[to] = x[e];
-          moves = min(moves, to);
+    for (int e = 0; e < kItems; ++e) {
+      if (e >= n) break;
+      const bool stay = stays >> e & 1;
+      const uint64_t all = __builtin_amdgcn_ballot_w64(stay);
+      const int i = i0 + 64 * e, mine = to + __popcll(all & before);
+      to += __popcll(all);
+      if (stay) {
+        kept[mine] = i;
+        from[mine] = (uint32_t)moved_index(p.rows, s, begin, i);
+        if (mine != i) {
+          w[mine] = x[e];
+          moves = min(moves, mine);
         }
-        ++to;
       }
-    if (moves < p.keep) atomicMin(&pick[0], moves);
+    }
   }
+  if (moves < p.keep) atomicMin(&moved, moves);
   __syncthreads();
-  for (int i = p.keep + tid; i < L; i += kSelectThreads) w[i] = 0.f;
+  for (int i = p.keep + tid; i < L; i += kThreads) w[i] = 0.f;
   if (tid == 0) {
-    p.start[s] = pick[0];
+    p.start[s] = moved;
     p.rows.lens[s] = p.keep;
   }
 }
@@ -237,8 +268,11 @@ bool evict_staged(const EvictProblem& p, int ncu) {
 }
 
 hipError_t launch_evict(const EvictProblem& p, hipStream_t stream) {
-  const hipError_t e = in_grids(p.rows.num_seqs, most_blocks(kSelectThreads), [&](int64_t first, unsigned blocks) {
-    hipLaunchKernelGGL(evict_select_kernel, dim3(blocks), dim3(kSelectThreads), 0, stream, p, first);
+  // (short sequences: fewer waves meet sooner at every barrier)
+  const bool few = !p.rows.offsets && p.rows.region <= 4 * 64 * kItems;
+  const hipError_t e = in_grids(p.rows.num_seqs, most_blocks(1024), [&](int64_t first, unsigned blocks) {
+    if (few) hipLaunchKernelGGL(evict_select_kernel<4>, dim3(blocks), dim3(256), 0, stream, p, first);
+    else hipLaunchKernelGGL(evict_select_kernel<16>, dim3(blocks), dim3(1024), 0, stream, p, first);
   });
   if (e != hipSuccess || p.keep == 0) return e;
   switch (moved_unit(p.rows)) {
