@@ -86,14 +86,16 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lchar;
 
-// Two parts of a value in the products' type: hi + lo / kLow.
+// Two parts of a value in the products' type: hi + lo. Queries come times kUp: what
+// is left of an fp16 number's 11 bits would be subnormal in small ones (they may
+// reach 65504 / kUp, as scaled for the softmax).
 template <typename T>
 struct Mm;
 template <>
 struct Mm<__hip_bfloat16> {
   typedef bf16x8 vec;
   typedef __bf16 elem;
-  static constexpr float kLow = 1.f;
+  static constexpr float kUp = 1.f;
   static __device__ inline f32x16 mma(vec a, vec b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -102,7 +104,7 @@ template <>
 struct Mm<__half> {
   typedef f16x8 vec;
   typedef _Float16 elem;
-  static constexpr float kLow = 2048.f;  // (what is left of small values would be subnormal)
+  static constexpr float kUp = 64.f;
   static __device__ inline f32x16 mma(vec a, vec b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -110,7 +112,7 @@ struct Mm<__half> {
 template <typename T>
 __device__ inline void split(float x, typename Mm<T>::elem& hi, typename Mm<T>::elem& lo) {
   hi = (typename Mm<T>::elem)x;
-  lo = (typename Mm<T>::elem)((x - (float)hi) * Mm<T>::kLow);
+  lo = (typename Mm<T>::elem)(x - (float)hi);
 }
 
 // Tiles of 32 rows of the piece's sequences, counted over them, shared out evenly:
@@ -180,13 +182,18 @@ struct Staged<true> {
   uint32_t ka, kb;
   f32x4 cs, sn;
 };
+// The row of tile t (rows past `last`: the last one) that the lane's part is of: looked
+// up a tile before its loads, so that a block table's entry has arrived.
+__device__ inline int64_t stage_row(const WeighProblem& p, int s, int t, int last, int wave, int lane) {
+  return source_row(p.src, s, min(kWeighKeys * t + 8 * wave + (lane >> 3), last));
+}
 template <bool kFp8>
-__device__ inline void stage_load(const WeighProblem& p, Staged<kFp8>& x, int s, int t, int last, int wave, int lane) {
+__device__ inline void stage_load(const WeighProblem& p, Staged<kFp8>& x, int64_t src, int t, int last, int wave, int lane) {
   constexpr int kRowB = kFp8 ? 576 : 1152;
   typedef decltype(x.c[0] + x.c[0]) cvec;
   typedef decltype(x.ka) kvec;
   const int pos = min(kWeighKeys * t + 8 * wave + (lane >> 3), last);
-  const uint64_t at = (uint64_t)(uintptr_t)p.src.kv + (uint64_t)source_row(p.src, s, pos) * kRowB;
+  const uint64_t at = (uint64_t)(uintptr_t)p.src.kv + (uint64_t)src * kRowB;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const uint64_t row = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(at >> 32), 8 * i) << 32 |
@@ -262,7 +269,7 @@ __device__ inline void stage_store(const Staged<kFp8>& x, lchar* L, int wave, in
 // leave three quarters of the matrix cores idle). Tiles go HBM -> registers -> LDS,
 // the next but one on its way during the products.
 template <typename T, bool kFp8, int kWR>
-__global__ __launch_bounds__(256, 1) void weigh_scores_kernel(WeighProblem p, int row_blocks) {
+__global__ __launch_bounds__(256, 2) void weigh_scores_kernel(WeighProblem p, int row_blocks) {
   typedef typename Mm<T>::vec vec;
   typedef typename Mm<T>::elem elem;
   constexpr int kKD = 4 / kWR;            // shares of the contraction
@@ -271,7 +278,7 @@ __global__ __launch_bounds__(256, 1) void weigh_scores_kernel(WeighProblem p, in
   constexpr int kN = 16 / kKD;            // scores of a lane after the sum
   extern __shared__ __attribute__((aligned(1024))) char weigh_lds[];
   lchar* const L = (lchar*)weigh_lds;
-  lchar* const sums = L + 2 * kTile;      // kKD > 1: 4 KB per wave
+  lchar* const sums = L + kTile;          // kKD > 1: 4 KB per wave
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int wr = wave % kWR, kd = wave / kWR, r32 = lane & 31, g = lane >> 5;
   // an eighth of the items to each XCD, row groups of a span together
@@ -292,6 +299,7 @@ __global__ __launch_bounds__(256, 1) void weigh_scores_kernel(WeighProblem p, in
     const int s = p.seq0 + i, len = source_rows(p.src, s), last = len - 1;
     const int end = min(t_end, first + n);
     // ---- the queries' operands: [16 k + 8 g .. + 7] of the row, times the softmax's scale ----
+    const float q_scale = p.scale_log2 * Mm<T>::kUp;
     vec qh[kC + kR], ql[kC + kR];
     {
       const int64_t q = ((int64_t)s * p.tokens + p.token0) * p.nh + row;
@@ -303,7 +311,7 @@ __global__ __launch_bounds__(256, 1) void weigh_scores_kernel(WeighProblem p, in
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           elem h, l;
-          split<T>((e < 4 ? a[e & 3] : b[e & 3]) * p.scale_log2, h, l);
+          split<T>((e < 4 ? a[e & 3] : b[e & 3]) * q_scale, h, l);
           qh[k][e] = h;
           ql[k][e] = l;
         }
@@ -312,51 +320,50 @@ __global__ __launch_bounds__(256, 1) void weigh_scores_kernel(WeighProblem p, in
     // keys that the row's token sees
     const int sees = len - p.tokens + p.token0 + row / p.nh + 1;
     float m = kNoScore, l = 0.f;
-    Staged<kFp8> x;
-    stage_load<kFp8>(p, x, s, t - first, last, wave, lane);
-    lds_barrier();  // every wave is done with the segment before
-    stage_store<T, kFp8>(x, L, wave, lane);
-    if (t + 1 < end) stage_load<kFp8>(p, x, s, t + 1 - first, last, wave, lane);
+    Staged<kFp8> x;  // the next tile, and the rows of the one after it
+    auto tile = [&](int u) { return min(u, end - 1) - first; };
+    stage_load<kFp8>(p, x, stage_row(p, s, tile(t), last, wave, lane), tile(t), last, wave, lane);
+    int64_t src = stage_row(p, s, tile(t + 1), last, wave, lane);
     for (int u = t; u < end; ++u) {
-      lds_barrier();  // tile u is there, tile u - 1 is read
-      const lchar* const b = L + ((u - t) & 1) * kTile;
-      if (u + 1 < end) {
-        stage_store<T, kFp8>(x, L + ((u + 1 - t) & 1) * kTile, wave, lane);
-        if (u + 2 < end) stage_load<kFp8>(p, x, s, u + 2 - first, last, wave, lane);
-      }
-      f32x16 hi = {}, lo = {};
+      // (the waves meet again before the sums, or below: the tile before is read)
+      if (kKD == 1 && u > t) lds_barrier();
+      stage_store<T, kFp8>(x, L, wave, lane);
+      stage_load<kFp8>(p, x, src, tile(u + 1), last, wave, lane);
+      src = stage_row(p, s, tile(u + 2), last, wave, lane);
+      lds_barrier();
+      const lchar* const b = L;
+      f32x16 acc = {};
       auto operand = [&](int k) -> vec {  // keys r32, elements [16 k + 8 g .. + 7]
         const int at = k < kC ? row_at(r32) + 32 * (kC * kd + k) + 16 * g
                        : k < kC + kR ? kRopeHi + rope_piece(r32, 2 * (kR * kd + k - kC) + g)
                                      : kRopeLo + rope_piece(r32, 2 * (kR * kd + k - kC - kR) + g);
         return *reinterpret_cast<const __attribute__((address_space(3))) vec*>(b + at);
       };
-      constexpr int kSteps = kC + 2 * kR, kAhead = 6;
+      constexpr int kSteps = kC + 2 * kR, kAhead = 3;
       vec a[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) a[k] = operand(k);
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) {
         const vec v = a[k % kAhead];
-        if (k < kC + kR) hi = Mm<T>::mma(v, qh[k], hi);
-        lo = Mm<T>::mma(v, k < kC + kR ? ql[k] : qh[k - kR], lo);
+        if (k < kC + kR) acc = Mm<T>::mma(v, ql[k], acc);
+        acc = Mm<T>::mma(v, qh[k < kC + kR ? k : k - kR], acc);
         if (k + kAhead < kSteps) a[k % kAhead] = operand(k + kAhead);
         __builtin_amdgcn_sched_barrier(0);
       }
-      settle(hi);
-      settle(lo);
+      settle(acc);
       // lane: row r32, keys 8 (e / 4) + 4 g + e % 4
       float sc[kN];
       if constexpr (kKD == 1) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sc[e] = hi[e] + lo[e] * (1.f / Mm<T>::kLow);
+        for (int e = 0; e < 16; ++e) sc[e] = acc[e] * (1.f / Mm<T>::kUp);
       } else {
         typedef __attribute__((address_space(3))) f32x4 lvec;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           f32x4 v;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = hi[4 * q + e] + lo[4 * q + e] * (1.f / Mm<T>::kLow);
+          for (int e = 0; e < 4; ++e) v[e] = acc[4 * q + e] * (1.f / Mm<T>::kUp);
           *reinterpret_cast<lvec*>(sums + 4096 * wave + 1024 * q + 16 * lane) = v;
         }
         lds_barrier();
@@ -393,6 +400,7 @@ __global__ __launch_bounds__(256, 1) void weigh_scores_kernel(WeighProblem p, in
           *reinterpret_cast<f32x4*>(to + 8 * q) = f32x4{sc[4 * q], sc[4 * q + 1], sc[4 * q + 2], sc[4 * q + 3]};
       }
     }
+    lds_barrier();  // every wave is done with the segment
     // ---- the segment's share of the rows' sums ----
     {
       auto join = [&](float m2, float l2) {
@@ -406,7 +414,6 @@ __global__ __launch_bounds__(256, 1) void weigh_scores_kernel(WeighProblem p, in
       join(f_of(sm[1]), f_of(sl[1]));
       if constexpr (kKD > 1) {
         typedef __attribute__((address_space(3))) float lfloat;
-        lds_barrier();  // the sums are read
         lfloat* const ml = reinterpret_cast<lfloat*>(sums) + 64 * wave;
         if (g == 0) ml[r32] = m, ml[32 + r32] = l;
         lds_barrier();
@@ -431,6 +438,7 @@ __global__ __launch_bounds__(256, 1) void weigh_scores_kernel(WeighProblem p, in
 // tile adds the exponentials of its scores over the rows, in their order.
 __global__ __launch_bounds__(256) void weigh_sum_kernel(WeighProblem p, int row_blocks) {
   __shared__ float lse[kWeighRows];
+  __shared__ f32x4 part[4][8];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const Spans sp{p};
   const int T_all = sp.total(), W = min((int)gridDim.x, T_all), W1 = min(p.spans, T_all), w = blockIdx.x;
@@ -446,21 +454,35 @@ __global__ __launch_bounds__(256) void weigh_sum_kernel(WeighProblem p, int row_
     __syncthreads();
     for (int r = threadIdx.x; r < 32 * row_blocks; r += 256) {
       float m = kNoScore, l = 0.f;
+      constexpr int kOnce = 8;  // partial sums whose loads go out together
       if (r < rows)
-        for (int c = c0; c <= c1; ++c) {
-          const float* const from = p.part + (int64_t)(c + i) * 2 * 32 * row_blocks + r;
-          const float m2 = from[0], l2 = from[32 * row_blocks], up = fmaxf(m, m2);
-          l = l * exp2f(m - up) + l2 * exp2f(m2 - up);
+        for (int c = c0; c <= c1; c += kOnce) {
+          float m2[kOnce], l2[kOnce], up = m;
+#pragma unroll
+          for (int k = 0; k < kOnce; ++k) {
+            const float* const from = p.part + (int64_t)(min(c + k, c1) + i) * 2 * 32 * row_blocks + r;
+            m2[k] = from[0];
+            l2[k] = c + k <= c1 ? from[32 * row_blocks] : 0.f;
+          }
+#pragma unroll
+          for (int k = 0; k < kOnce; ++k) up = fmaxf(up, m2[k]);
+          l *= exp2f(m - up);
+#pragma unroll
+          for (int k = 0; k < kOnce; ++k) l += l2[k] * exp2f(m2[k] - up);
           m = up;
         }
       // rows past the last, and tokens that see nothing, give nothing
       lse[r] = l == 0.f ? INFINITY : m + log2f(l);
     }
     __syncthreads();
-    for (int u = t + wave; u < end; u += 4) {
+    // a tile per wave, or (many rows) a quarter of a tile's row blocks
+    const bool shared = row_blocks >= 8;
+    const int b0 = shared ? wave : 0, db = shared ? 4 : 1;
+    for (int u = shared ? t : t + wave; u < end; u += shared ? 1 : 4) {
       const float* const from = p.scores + (int64_t)u * row_blocks * 1024 + 4 * lane;
       f32x4 sum = {};
-      for (int b = 0; b < row_blocks; ++b) {
+#pragma unroll 4
+      for (int b = b0; b < row_blocks; b += db) {
         f32x4 v[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const f32x4*>(from + 1024 * b + 256 * q);
@@ -469,13 +491,20 @@ __global__ __launch_bounds__(256) void weigh_sum_kernel(WeighProblem p, int row_
           const int r = 32 * b + 8 * q + (lane >> 3);
           const float e = lse[r];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) sum[k] += r < rows ? exp2f(v[q][k] - e) : 0.f;
+          for (int k = 0; k < 4; ++k) sum[k] += r < rows ? __builtin_amdgcn_exp2f(v[q][k] - e) : 0.f;
         }
       }
 #pragma unroll
       for (int o = 8; o < 64; o <<= 1)
 #pragma unroll
         for (int k = 0; k < 4; ++k) sum[k] += __shfl_xor(sum[k], o, 64);
+      if (shared) {
+        __syncthreads();  // (the sums of the tile before are read)
+        if (lane < 8) part[wave][lane] = sum;
+        __syncthreads();
+        if (wave > 0) continue;
+        if (lane < 8) sum = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+      }
       const int key = kWeighKeys * (u - first) + 4 * lane;
       if (lane < 8) {
         float* const to = p.weights + (p.src.offsets ? source_begin(p.src, s) : (int64_t)s * p.src.region);
@@ -491,7 +520,7 @@ __global__ __launch_bounds__(256) void weigh_sum_kernel(WeighProblem p, int row_
 
 template <typename T, bool kFp8, int kWR>
 hipError_t scores_t(const WeighProblem& p, int row_blocks, hipStream_t stream) {
-  constexpr int lds = 2 * kTile + (kWR < 4 ? 4 * 4096 : 0);
+  constexpr int lds = kTile + (kWR < 4 ? 4 * 4096 : 0);
   static OncePerDevice once;
   const hipError_t e = allow_lds(once, reinterpret_cast<const void*>(&weigh_scores_kernel<T, kFp8, kWR>), lds);
   if (e != hipSuccess) return e;
@@ -502,8 +531,7 @@ hipError_t scores_t(const WeighProblem& p, int row_blocks, hipStream_t stream) {
 template <typename T, bool kFp8>
 hipError_t scores_w(const WeighProblem& p, int row_blocks, hipStream_t stream) {
   if (row_blocks == 1) return scores_t<T, kFp8, 1>(p, row_blocks, stream);
-  if (row_blocks == 2) return scores_t<T, kFp8, 2>(p, row_blocks, stream);
-  return scores_t<T, kFp8, 4>(p, row_blocks, stream);
+  return scores_t<T, kFp8, 2>(p, row_blocks, stream);
 }
 
 }  // namespace
@@ -531,8 +559,8 @@ bool weigh_mfma_supported(const WeighProblem& p) {
 }
 
 int weigh_spans(int rows, int ncu) {
-  const int blocks = (rows + 31) / 32, groups = blocks <= 4 ? 1 : (blocks + 3) / 4;
-  return groups < ncu ? ncu / groups : 1;
+  const int blocks = (rows + 31) / 32, groups = (blocks + 1) / 2;
+  return groups < 2 * ncu ? 2 * ncu / groups : 1;
 }
 
 hipError_t launch_weigh_mfma(const WeighProblem& p, int64_t most_tiles, hipStream_t stream, int ncu) {
@@ -541,7 +569,7 @@ hipError_t launch_weigh_mfma(const WeighProblem& p, int64_t most_tiles, hipStrea
                  : p.src.kv_dtype == LA_DTYPE_BF16   ? scores_w<__hip_bfloat16, false>(p, row_blocks, stream)
                                                      : scores_w<__half, false>(p, row_blocks, stream);
   if (e != hipSuccess) return e;
-  const int64_t blocks = (most_tiles + 3) / 4 < 8LL * ncu ? (most_tiles + 3) / 4 : 8LL * ncu;
+  const int64_t items = row_blocks >= 8 ? most_tiles : (most_tiles + 3) / 4, blocks = items < 8LL * ncu ? items : 8LL * ncu;
   hipLaunchKernelGGL(weigh_sum_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p, row_blocks);
   return hipGetLastError();
 }
