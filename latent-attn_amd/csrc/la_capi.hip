@@ -314,6 +314,7 @@ struct StepTail {
   bool merge = true;             // false: the slots stay as they are, nothing is written to the output
   const void* q_prep = nullptr;  // the same queries' 16-bit rows in a layout that is this step's too
   TreeStep tree{};               // the queries are trees' nodes (MFMA kernels only)
+  const AbsorbQueries* queries = nullptr;  // absorbed in place of the arguments' where those would be into 16-bit rows
 };
 int run(const la_decode_args* a, hipStream_t stream, hipEvent_t ev_b = nullptr, hipEvent_t ev_e = nullptr,
         int repeat = 1, bool coarse = false, StepTail* tail = nullptr) {
@@ -365,9 +366,13 @@ int run(const la_decode_args* a, hipStream_t stream, hipEvent_t ev_b = nullptr, 
     if (plan.absorb_prep) {
       // absorbed, scaled 16-bit Q rows for the attention kernel in one pass
       // q_prep in the MFMAs' 16-bit type: fp16 for an fp16 cache, bf16 otherwise
-      e = launch_absorb_mfma(a->q_nope, a->W_UK, a->w_uk_dtype, p.q_prep, p.kv_dtype == LA_DTYPE_F16 ? 2 : 1,
-                             a->q_rope, p.scale_log2, c.qk_rope_head_dim, (int)tokens, c.num_heads,
-                             c.qk_nope_head_dim, c.kv_lora_rank, a->queries_per_seq, stream, zero_out, zero_n);
+      if (tail && tail->queries)
+        e = launch_absorb_any(*tail->queries, a->W_UK, a->w_uk_dtype, p.q_prep, p.kv_dtype == LA_DTYPE_F16 ? 2 : 1,
+                              p.scale_log2, c.num_heads, stream, zero_out, zero_n);
+      else
+        e = launch_absorb_mfma(a->q_nope, a->W_UK, a->w_uk_dtype, p.q_prep, p.kv_dtype == LA_DTYPE_F16 ? 2 : 1,
+                               a->q_rope, p.scale_log2, c.qk_rope_head_dim, (int)tokens, c.num_heads,
+                               c.qk_nope_head_dim, c.kv_lora_rank, a->queries_per_seq, stream, zero_out, zero_n);
     } else {
       float* qa = reinterpret_cast<float*>(ws + plan.q_abs_off);
       if (plan.absorb_f32)
@@ -1316,8 +1321,8 @@ int decode_tree(const la_tree_args* a, void* stream_v, bool run_it, size_t* need
       (a->total_rows > 0 && !a->kv_cache))
     return LA_ERROR_INVALID_VALUE;
   const int64_t tokens = t.q.tokens, rows = tokens * nh;
-  const bool nope_as_is = packed_f32(t.q.q_nope, t.q.dtype, t.q.nope_stride, t.q.nope_head, nh, c.qk_nope_head_dim);
-  const bool rope_as_is = !a->rotate_q && packed_f32(t.q.q_rope, t.q.dtype, t.q.rope_stride, t.q.rope_head, nh, c.qk_rope_head_dim);
+  bool nope_as_is = packed_f32(t.q.q_nope, t.q.dtype, t.q.nope_stride, t.q.nope_head, nh, c.qk_nope_head_dim);
+  bool rope_as_is = !a->rotate_q && packed_f32(t.q.q_rope, t.q.dtype, t.q.rope_stride, t.q.rope_head, nh, c.qk_rope_head_dim);
 
   // The step over the trees: every node a query of its sequence. Aligned addresses stand for what lies in the workspace.
   alignas(256) static const char any[256] = {0};
@@ -1350,6 +1355,9 @@ int decode_tree(const la_tree_args* a, void* stream_v, bool run_it, size_t* need
   if (!mfma && (a->kernel_variant == kTreeMfma || !generic_prompt_supported(c.kv_lora_rank, c.qk_rope_head_dim)))
     return LA_ERROR_NOT_SUPPORTED;
   const bool join = mfma && merge_join_supported(step);
+  // queries that the absorption reads as they are: no copies
+  const bool direct = mfma && plan.absorb_prep && absorb_any_supported(t.q, t.src, a->W_UK, a->w_uk_dtype, c);
+  if (direct) nope_as_is = rope_as_is = true;
   const size_t step_bytes = mfma ? la_mla_decode_workspace_size(&d) : 0;
 
   float *q_abs = nullptr, *out32 = nullptr;
@@ -1360,6 +1368,7 @@ int decode_tree(const la_tree_args* a, void* stream_v, bool run_it, size_t* need
     t.seen = static_cast<uint64_t*>(v.take((size_t)tokens * sizeof(uint64_t)));
     t.cos = static_cast<float*>(v.take((size_t)tokens * (c.qk_rope_head_dim / 2) * sizeof(float)));
     t.sin = static_cast<float*>(v.take((size_t)tokens * (c.qk_rope_head_dim / 2) * sizeof(float)));
+    if (direct) t.pos = static_cast<int32_t*>(v.take((size_t)tokens * sizeof(int32_t)));
     if (!nope_as_is) t.q_nope = static_cast<float*>(v.take((size_t)rows * c.qk_nope_head_dim * sizeof(float)));
     if (!rope_as_is) t.q_rope = static_cast<float*>(v.take((size_t)rows * c.qk_rope_head_dim * sizeof(float)));
     if (mfma) {
@@ -1408,14 +1417,15 @@ int decode_tree(const la_tree_args* a, void* stream_v, bool run_it, size_t* need
     return scratch.finish(status_of(launch_plain_tree(p, stream)));
   }
   d.seq_lens = t.lens;
-  d.q_nope = qn;
-  d.q_rope = qr;
+  if (!direct) d.q_nope = qn, d.q_rope = qr;  // (else the addresses that the plan was made with, which nothing reads)
   d.output = out32 ? out32 : static_cast<float*>(a->output);  // (join: the step leaves it alone)
   d.workspace = step_ws;
   d.workspace_bytes = step_bytes;
   StepTail tail;
   tail.merge = !join;
   tail.tree = TreeStep{t.seen, t.cos, t.sin};
+  const AbsorbQueries x{t.q, t.src, t.pos, 0};
+  if (direct) tail.queries = &x;
   int st = run(&d, stream, nullptr, nullptr, 1, false, &tail);
   if (st == LA_SUCCESS && join) {
     JoinProblem j{};
@@ -1499,14 +1509,14 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
   // then sequences at a time (packed ones, whose lengths only the device knows, all together).
   int64_t most_tiles = 0;
   if (mfma) {
-    p.count = std::max(1, std::min(n, kWeighRows / nh));
+    p.count = weigh_count(n, nh);
     p.seqs = a->num_seqs;
     if (!a->seq_offsets && seq_tiles > 0) {
       const size_t one = weigh_score_bytes(seq_tiles, p.count * nh);
       p.seqs = (int)std::max<int64_t>(1, std::min<int64_t>(p.seqs, kMostScores / one));
     }
     most_tiles = a->seq_offsets ? all_tiles : seq_tiles * p.seqs;
-    while (p.count > 1 && weigh_score_bytes(most_tiles, p.count * nh) > kMostScores) p.count = (p.count + 1) / 2;
+    while (p.count % 2 == 0 && p.count / 2 * nh % 32 == 0 && weigh_score_bytes(most_tiles, p.count * nh) > kMostScores) p.count /= 2;
     p.spans = weigh_spans(p.count * nh, cu_count());
   }
   const int64_t rows = q.tokens * nh;
@@ -1514,12 +1524,18 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
   const bool rope_as_is = !a->rotate_q && packed_f32(q.q_rope, q.dtype, q.rope_stride, q.rope_head, nh, c.qk_rope_head_dim);
   TokenProblem t{};
   float* q_abs = nullptr;
+  void* q_prep = nullptr;
+  const bool direct = mfma && absorb_any_supported(q, p.src, a->W_UK, a->w_uk_dtype, c);
+  const size_t prep_elems = (size_t)a->num_seqs * qprep_rows_per_seq(n * nh) * kQPrepRow;
   auto carve = [&](void* ws) {
     Carve v(ws);
-    if (!nope_as_is) t.q_nope = static_cast<float*>(v.take((size_t)rows * c.qk_nope_head_dim * sizeof(float)));
-    if (!rope_as_is) t.q_rope = static_cast<float*>(v.take((size_t)rows * c.qk_rope_head_dim * sizeof(float)));
-    q_abs = static_cast<float*>(v.take((size_t)rows * c.kv_lora_rank * sizeof(float)));
+    if (!direct) {
+      if (!nope_as_is) t.q_nope = static_cast<float*>(v.take((size_t)rows * c.qk_nope_head_dim * sizeof(float)));
+      if (!rope_as_is) t.q_rope = static_cast<float*>(v.take((size_t)rows * c.qk_rope_head_dim * sizeof(float)));
+      q_abs = static_cast<float*>(v.take((size_t)rows * c.kv_lora_rank * sizeof(float)));
+    }
     if (mfma) {
+      q_prep = v.take(2 * prep_elems * 2);
       p.scores = static_cast<float*>(v.take(weigh_score_bytes(most_tiles, p.count * nh)));
       p.part = static_cast<float*>(v.take(weigh_part_bytes(p.spans, p.seqs, p.count * nh)));
     } else {
@@ -1533,25 +1549,31 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
   Scratch scratch(a->workspace, a->workspace_bytes, total, stream);
   if (scratch.status != LA_SUCCESS) return scratch.status;
   carve(scratch.ws);
-  t.q = q;
-  t.src = p.src;
-  t.nh = nh;
-  t.dn = c.qk_nope_head_dim;
-  t.dR = c.qk_rope_head_dim;
-  t.vec = queries_vec(q);
-  if (t.q_nope || t.q_rope) {
-    const hipError_t e = launch_tokens(t, stream);
-    if (e != hipSuccess) return scratch.finish(record_hip(e));
-  }
-  const int st = la_absorb_q(nope_as_is ? static_cast<const float*>(a->q_nope) : t.q_nope, a->W_UK, a->w_uk_dtype, q_abs,
-                             (int)q.tokens, &c, stream_v);
-  if (st != LA_SUCCESS) return scratch.finish(st);
-  p.q_abs = q_abs;
-  p.q_rope = rope_as_is ? static_cast<const float*>(a->q_rope) : t.q_rope;
-  if (!mfma) return scratch.finish(status_of(launch_weigh_plain(p, stream)));
+  p.q_prep = q_prep;
+  p.low = (int64_t)prep_elems;
   hipError_t e = hipSuccess;
+  if (direct) {
+    const AbsorbQueries x{q, p.src, nullptr, p.low};
+    e = launch_absorb_any(x, a->W_UK, a->w_uk_dtype, q_prep, a->kv_dtype == LA_DTYPE_F16 ? 2 : 1, weigh_query_scale(p), nh, stream);
+  } else {
+    t.q = q;
+    t.src = p.src;
+    t.nh = nh;
+    t.dn = c.qk_nope_head_dim;
+    t.dR = c.qk_rope_head_dim;
+    t.vec = queries_vec(q);
+    if (t.q_nope || t.q_rope) e = launch_tokens(t, stream);
+    if (e != hipSuccess) return scratch.finish(record_hip(e));
+    const int st = la_absorb_q(nope_as_is ? static_cast<const float*>(a->q_nope) : t.q_nope, a->W_UK, a->w_uk_dtype, q_abs,
+                               (int)q.tokens, &c, stream_v);
+    if (st != LA_SUCCESS) return scratch.finish(st);
+    p.q_abs = q_abs;
+    p.q_rope = rope_as_is ? static_cast<const float*>(a->q_rope) : t.q_rope;
+    if (!mfma) return scratch.finish(status_of(launch_weigh_plain(p, stream)));
+    e = launch_weigh_queries(p, stream);
+  }
   const int most_seqs = p.seqs, most_count = p.count;
-  for (int j = 0; j < n && most_tiles > 0; j += most_count)
+  for (int j = 0; j < n && most_tiles > 0 && e == hipSuccess; j += most_count)
     for (int s = 0; s < a->num_seqs && e == hipSuccess; s += most_seqs) {
       p.token0 = j;
       p.count = std::min(most_count, n - j);

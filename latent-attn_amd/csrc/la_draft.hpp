@@ -22,6 +22,7 @@ struct TreeQueries {
   uint64_t* seen;  // TreeStep
   float* cos;
   float* sin;
+  int32_t* pos;    // (tokens): the nodes' positions, or nullptr
   int vec;  // queries are whole-vector aligned
 };
 hipError_t launch_tree_queries(const TreeQueries& p, hipStream_t stream);
@@ -100,9 +101,12 @@ struct WeighProblem {
   float scale_log2;
   float* weights;
   float* lse;  // plain form: (num_seqs * tokens, nh), base 2
-  // matrix form: one piece of the call, `seqs` sequences from seq0 on and of
+  // matrix form: the queries' operands (qprep_index, weigh_query_scale), what their
+  // rounding left `low` elements on, and one piece of the call, `seqs` sequences from seq0 on and of
   // each `count` tokens from token0 on
   int seq0, seqs, token0, count;
+  const void* q_prep;
+  int64_t low;
   int spans;       // workgroups that share the tiles of a row group
   float* scores;   // [tile][32 rows][32 keys] of `row_blocks` blocks per tile
   float* part;     // [slot][m, l][rows rounded up to 32]
@@ -112,6 +116,9 @@ hipError_t launch_weigh_plain(const WeighProblem& p, hipStream_t stream);
 // by the tiles (of 32 rows) that its sequences have room for.
 bool weigh_mfma_supported(const WeighProblem& p);
 constexpr int kWeighKeys = 32, kWeighRows = 4096;  // keys per tile; (token, head) rows of a piece at most
+int weigh_count(int tokens, int nh);  // tokens of a piece at most: in whole blocks of 32 rows if they are not all; 0: too many heads
+float weigh_query_scale(const WeighProblem& p);
+hipError_t launch_weigh_queries(const WeighProblem& p, hipStream_t stream);  // q_prep from q_abs and q_rope
 int weigh_spans(int rows, int ncu);
 inline size_t weigh_score_bytes(int64_t tiles, int rows) { return (size_t)tiles * ((rows + 31) / 32) * 4096; }
 inline size_t weigh_part_bytes(int spans, int seqs, int rows) {

@@ -128,12 +128,14 @@ constexpr int kAbsThreads = 512;
 // the first wait, spread over the block's 8 waves.
 // NKS = dn / 16 when known at compile time (8 for dn = 128: no guards, every
 // load unconditional), 0 for any dn <= 128 that is a multiple of 16.
-template <typename WT, int NKS>
-__global__ __launch_bounds__(kAbsThreads) void absorb_mfma_kernel(const float* __restrict__ q_nope, const WT* __restrict__ W,
-                                                          void* __restrict__ out, int out_mode,
-                                                          const float* __restrict__ q_rope, float scale, int dR,
-                                                          int tokens, int nh, int dn, int dc, int qps,
-                                                          float* __restrict__ zero_out, int64_t zero_n) {
+// kAny: the queries are x's, of any type and strides and with q_rope not rotated
+// yet, and the rows' second parts may be wanted too (AbsorbQueries; modes 1, 2).
+template <typename WT, int NKS, bool kAny>
+__device__ __forceinline__ void absorb_body(const float* __restrict__ q_nope, const WT* __restrict__ W,
+                                            void* __restrict__ out, int out_mode,
+                                            const float* __restrict__ q_rope, float scale, int dR,
+                                            int tokens, int nh, int dn, int dc, int qps,
+                                            float* __restrict__ zero_out, int64_t zero_n, const AbsorbQueries& any) {
   typedef Mma<WT> M;
   typedef typename M::vec vec;
   LA_RSTAMP_DECL;
@@ -170,14 +172,21 @@ __global__ __launch_bounds__(kAbsThreads) void absorb_mfma_kernel(const float* _
   // LDS for the MFMA waves (each wave issues 2 q loads, not 16)
   const int t = t0 + (lane & 31);
   const bool tvalid = t < tokens;
-  const float* qrow = q_nope + ((int64_t)(tvalid ? t : 0) * nh + h) * dn + 8 * (lane >> 5);
+  const float* qrow = kAny ? nullptr : q_nope + ((int64_t)(tvalid ? t : 0) * nh + h) * dn + 8 * (lane >> 5);
   // (with NKS > 0 every wave's k-step exists: the loads go out
   // unconditionally, since a load under a branch gets its result copied at
   // the branch's end, which waits for it before the W_UK loads below issue)
   static_assert(kAbsThreads / 64 == 8, "one q k-step per wave");
   const int ks_w = wave;
   f32x4 qa, qb;
-  if (NKS > 0 || ks_w < nks) {
+  if constexpr (kAny) {
+    const int64_t at = (tvalid ? t : 0) * any.q.nope_stride + h * any.q.nope_head + 16 * ks_w + 8 * (lane >> 5);
+    float x[4], y[4];
+    load_q4(any.q.q_nope, any.q.dtype, at, x);
+    load_q4(any.q.q_nope, any.q.dtype, at + 4, y);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) qa[e] = x[e], qb[e] = y[e];
+  } else if (NKS > 0 || ks_w < nks) {
     qa = *reinterpret_cast<const f32x4*>(qrow + 16 * ks_w);
     qb = *reinterpret_cast<const f32x4*>(qrow + 16 * ks_w + 4);
   }
@@ -201,9 +210,12 @@ __global__ __launch_bounds__(kAbsThreads) void absorb_mfma_kernel(const float* _
   // branch's end, which would wait for every load before it.
   const int rt = tid & 255;
   const int rtr = min(t0 + (rt >> 3), tokens - 1);
-  const float* rsrc = out_mode != 0 ? q_rope + ((int64_t)rtr * nh + h) * dR + 8 * (rt & 7) : q_nope;
-  const f32x4 ra = *reinterpret_cast<const f32x4*>(rsrc);
-  const f32x4 rb = *reinterpret_cast<const f32x4*>(rsrc + 4);
+  f32x4 ra, rb;
+  if constexpr (!kAny) {
+    const float* rsrc = out_mode != 0 ? q_rope + ((int64_t)rtr * nh + h) * dR + 8 * (rt & 7) : q_nope;
+    ra = *reinterpret_cast<const f32x4*>(rsrc);
+    rb = *reinterpret_cast<const f32x4*>(rsrc + 4);
+  }
   LA_RSTAMP(1);
 #pragma unroll
   for (int k = 0; k < kWLoads; ++k) {
@@ -272,11 +284,25 @@ __global__ __launch_bounds__(kAbsThreads) void absorb_mfma_kernel(const float* _
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r] = (__bf16)(v[r] * scale);
         *reinterpret_cast<bf16x4*>(reinterpret_cast<__bf16*>(out) + qprep_index(qrow, col)) = o;
+        if constexpr (kAny) {
+          if (any.low) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = (__bf16)(v[r] * scale - (float)o[r]);
+            *reinterpret_cast<bf16x4*>(reinterpret_cast<__bf16*>(out) + any.low + qprep_index(qrow, col)) = o;
+          }
+        }
       } else {
         f16x4 o;
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r] = (_Float16)(v[r] * scale);
         *reinterpret_cast<f16x4*>(reinterpret_cast<_Float16*>(out) + qprep_index(qrow, col)) = o;
+        if constexpr (kAny) {
+          if (any.low) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = (_Float16)(v[r] * scale - (float)o[r]);
+            *reinterpret_cast<f16x4*>(reinterpret_cast<_Float16*>(out) + any.low + qprep_index(qrow, col)) = o;
+          }
+        }
       }
     }
   }
@@ -284,6 +310,26 @@ __global__ __launch_bounds__(kAbsThreads) void absorb_mfma_kernel(const float* _
     // the q_rope part of the same rows (loaded with the operands above): one
     // 16-B slot of q_prep per thread
     const int tr = t0 + (tid >> 3), j = 8 * (tid & 7);
+    if constexpr (kAny) {
+      // element j + e with its partner of the rotation, j + e + 32 or - 32
+      const int tc = min(tr, tokens - 1), i = j & 31, s = tc / qps;
+      const int64_t at = tc * any.q.rope_stride + h * any.q.rope_head;
+      const int64_t pos = any.pos ? any.pos[tc] : max(source_rows(any.src, s) - qps + tc % qps, 0);
+      float own[8], other[8];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        load_q4(any.q.q_rope, any.q.dtype, at + j + 4 * k, *reinterpret_cast<float(*)[4]>(own + 4 * k));
+        load_q4(any.q.q_rope, any.q.dtype, at + (j ^ 32) + 4 * k, *reinterpret_cast<float(*)[4]>(other + 4 * k));
+      }
+      const float sign = j < 32 ? -1.f : 1.f;
+      const f32x4 *const cs = reinterpret_cast<const f32x4*>(any.src.cos + source_rope_row(any.src, pos) * 32 + i),
+                  *const sn = reinterpret_cast<const f32x4*>(any.src.sin + source_rope_row(any.src, pos) * 32 + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        ra[e] = any.q.rotate ? own[e] * cs[0][e] + sign * other[e] * sn[0][e] : own[e];
+        rb[e] = any.q.rotate ? own[4 + e] * cs[1][e] + sign * other[4 + e] * sn[1][e] : own[4 + e];
+      }
+    }
     if (tr < tokens) {
       const int64_t qr = (int64_t)(tr / qps) * qprep_rows_per_seq(qps * nh) + (int64_t)(tr % qps) * nh + h;
       const int64_t dst = qprep_index(qr, dc + j);
@@ -295,6 +341,13 @@ __global__ __launch_bounds__(kAbsThreads) void absorb_mfma_kernel(const float* _
           v[4 + e] = (__bf16)(rb[e] * scale);
         }
         *reinterpret_cast<bf16x8*>(reinterpret_cast<__bf16*>(out) + dst) = v;
+        if constexpr (kAny) {
+          if (any.low) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (__bf16)((e < 4 ? ra : rb)[e & 3] * scale - (float)v[e]);
+            *reinterpret_cast<bf16x8*>(reinterpret_cast<__bf16*>(out) + any.low + dst) = v;
+          }
+        }
       } else {
         f16x8 v;
 #pragma unroll
@@ -303,10 +356,33 @@ __global__ __launch_bounds__(kAbsThreads) void absorb_mfma_kernel(const float* _
           v[4 + e] = (_Float16)(rb[e] * scale);
         }
         *reinterpret_cast<f16x8*>(reinterpret_cast<_Float16*>(out) + dst) = v;
+        if constexpr (kAny) {
+          if (any.low) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (_Float16)((e < 4 ? ra : rb)[e & 3] * scale - (float)v[e]);
+            *reinterpret_cast<f16x8*>(reinterpret_cast<_Float16*>(out) + any.low + dst) = v;
+          }
+        }
       }
     }
   }
   LA_RSTAMP_WRITE(0);
+}
+template <typename WT, int NKS>
+__global__ __launch_bounds__(kAbsThreads) void absorb_mfma_kernel(const float* __restrict__ q_nope, const WT* __restrict__ W,
+                                                          void* __restrict__ out, int out_mode,
+                                                          const float* __restrict__ q_rope, float scale, int dR,
+                                                          int tokens, int nh, int dn, int dc, int qps,
+                                                          float* __restrict__ zero_out, int64_t zero_n) {
+  absorb_body<WT, NKS, false>(q_nope, W, out, out_mode, q_rope, scale, dR, tokens, nh, dn, dc, qps, zero_out, zero_n,
+                              AbsorbQueries{});
+}
+template <typename WT>
+__global__ __launch_bounds__(kAbsThreads) void absorb_any_kernel(AbsorbQueries any, const WT* __restrict__ W,
+                                                                 void* __restrict__ out, int out_mode, float scale,
+                                                                 int tokens, int nh, int qps, float* __restrict__ zero_out,
+                                                                 int64_t zero_n) {
+  absorb_body<WT, 8, true>(nullptr, W, out, out_mode, nullptr, scale, 64, tokens, nh, 128, 512, qps, zero_out, zero_n, any);
 }
 
 // ---------------------------------------------------------------------------
@@ -1058,6 +1134,27 @@ hipError_t launch_absorb_mfma(const float* q_nope, const void* W_UK, int w_dtype
     hipLaunchKernelGGL(k, grid, dim3(kAbsThreads), 0, stream, q_nope, reinterpret_cast<const __half*>(W_UK), out, out_mode,
                        q_rope, scale, dR, tokens, nh, dn, dc, qps, zero_out, zero_n);
   }
+  return hipGetLastError();
+}
+
+bool absorb_any_supported(const QuerySource& q, const RowSource& r, const void* W_UK, int w_dtype, const la_mla_config& c) {
+  return (w_dtype == LA_DTYPE_BF16 || w_dtype == LA_DTYPE_F16) && (reinterpret_cast<uintptr_t>(W_UK) & 15) == 0 &&
+         c.qk_nope_head_dim == 128 && c.kv_lora_rank == 512 && c.qk_rope_head_dim == 64 &&
+         q_vec(q.q_nope, q.dtype, q.nope_stride, q.nope_head) && q_vec(q.q_rope, q.dtype, q.rope_stride, q.rope_head) &&
+         ((reinterpret_cast<uintptr_t>(r.cos) | reinterpret_cast<uintptr_t>(r.sin)) & 15) == 0 && 64 * 4 * (((q.tokens + 31) / 32 * ((c.num_heads + 7) / 8) + 7) / 8) <= most_blocks(kAbsThreads) && device_is_gfx950();
+}
+
+hipError_t launch_absorb_any(const AbsorbQueries& x, const void* W_UK, int w_dtype, void* out, int out_mode, float scale,
+                             int nh, hipStream_t stream, float* zero_out, int64_t zero_n) {
+  const int tokens = (int)x.q.tokens;
+  const int64_t groups = (int64_t)((tokens + 31) / 32) * ((nh + 7) / 8);
+  const dim3 grid((unsigned)(64 * 4 * ((groups + 7) / 8)));
+  if (w_dtype == LA_DTYPE_BF16)
+    hipLaunchKernelGGL(absorb_any_kernel<__hip_bfloat16>, grid, dim3(kAbsThreads), 0, stream, x,
+                       static_cast<const __hip_bfloat16*>(W_UK), out, out_mode, scale, tokens, nh, x.q.per_seq, zero_out, zero_n);
+  else
+    hipLaunchKernelGGL(absorb_any_kernel<__half>, grid, dim3(kAbsThreads), 0, stream, x, static_cast<const __half*>(W_UK), out,
+                       out_mode, scale, tokens, nh, x.q.per_seq, zero_out, zero_n);
   return hipGetLastError();
 }
 

@@ -312,6 +312,19 @@ struct TokenProblem {
   int vec;  // queries are whole-vector aligned
 };
 hipError_t launch_tokens(const TokenProblem& p, hipStream_t stream);
+// Absorption straight from queries of any type and strides (q.per_seq per
+// sequence) into the matrix kernels' operand order (qprep_index), as
+// launch_absorb_mfma writes it from packed, rotated fp32 ones.
+struct AbsorbQueries {
+  QuerySource q;
+  RowSource src;       // positions: token j of n of a sequence with L rows is at L - n + j
+  const int32_t* pos;  // or given (device, one per token)
+  int64_t low;         // > 0: also what the rounded rows leave, in a second array so many elements on
+};
+bool absorb_any_supported(const QuerySource& q, const RowSource& r, const void* W_UK, int w_dtype, const la_mla_config& c);
+// out_mode 1: bf16, 2: fp16; zero_out as for launch_absorb_mfma.
+hipError_t launch_absorb_any(const AbsorbQueries& x, const void* W_UK, int w_dtype, void* out, int out_mode, float scale,
+                             int nh, hipStream_t stream, float* zero_out = nullptr, int64_t zero_n = 0);
 // fp32 -> out_dtype
 hipError_t launch_cast(const float* src, void* dst, int out_dtype, int64_t n, hipStream_t stream);
 

@@ -49,7 +49,8 @@ __global__ __launch_bounds__(256) void tree_queries_kernel(TreeQueries p, int64_
   const int n = p.q.per_seq, s = (int)(token / n), j = (int)(token % n);
   const int rows = source_rows(p.src, s), L = rows < n ? 0 : rows, half = p.dR / 2;
   const uint64_t seen = shfl64(tree_seen(p.parents, s, n), j);
-  const int64_t pos = source_rope_row(p.src, max(L - n + __popcll(seen) - 1, 0));
+  const int at = max(L - n + __popcll(seen) - 1, 0);
+  const int64_t pos = source_rope_row(p.src, at);
   const float *const cos = p.src.cos + pos * half, *const sin = p.src.sin + pos * half;
   if (blockIdx.y == 0) {
     for (int i = threadIdx.x; i < half; i += 256) {
@@ -58,6 +59,7 @@ __global__ __launch_bounds__(256) void tree_queries_kernel(TreeQueries p, int64_
     }
     if (threadIdx.x == 0) {
       p.seen[token] = seen;
+      if (p.pos) p.pos[token] = at;
       if (j == 0) p.lens[s] = L;
     }
   }
@@ -73,10 +75,10 @@ __global__ __launch_bounds__(256) void tree_queries_kernel(TreeQueries p, int64_
   if (p.q_rope)
     for (int i = first; i < min(last, p.nh * half); i += kN * 256) {
       const int h = i / half, d = i - h * half;
-      const int64_t at = token * p.q.rope_stride + h * p.q.rope_head + d;
+      const int64_t from = token * p.q.rope_stride + h * p.q.rope_head + d;
       float a[kN], b[kN];
-      load_n<kN>(p.q.q_rope, p.q.dtype, at, a);
-      load_n<kN>(p.q.q_rope, p.q.dtype, at + half, b);
+      load_n<kN>(p.q.q_rope, p.q.dtype, from, a);
+      load_n<kN>(p.q.q_rope, p.q.dtype, from + half, b);
       float* const to = p.q_rope + (token * p.nh + h) * p.dR + d;
 #pragma unroll
       for (int e = 0; e < kN; ++e) {

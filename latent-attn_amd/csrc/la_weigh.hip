@@ -182,25 +182,37 @@ struct Staged<true> {
   uint32_t ka, kb;
   f32x4 cs, sn;
 };
-// The row of tile t (rows past `last`: the last one) that the lane's part is of: looked
-// up a tile before its loads, so that a block table's entry has arrived.
-__device__ inline int64_t stage_row(const WeighProblem& p, int s, int t, int last, int wave, int lane) {
-  return source_row(p.src, s, min(kWeighKeys * t + 8 * wave + (lane >> 3), last));
+// A sequence's rows: the first (contiguous caches) and the last, and its block table.
+struct Rows {
+  int64_t begin;
+  const int32_t* table;
+  int last;
+};
+// Position of the lane's part of tile t (past the last row: that one), and its block
+// table's entry: looked up a tile before its loads, so that it has arrived by then.
+__device__ inline int stage_pos(const Rows& r, int t, int wave, int lane) {
+  return min(kWeighKeys * t + 8 * wave + (lane >> 3), r.last);
+}
+__device__ inline int stage_entry(const WeighProblem& p, const Rows& r, int t, int wave, int lane) {
+  return r.table ? r.table[stage_pos(r, t, wave, lane) / p.src.block_size] : 0;
 }
 template <bool kFp8>
-__device__ inline void stage_load(const WeighProblem& p, Staged<kFp8>& x, int64_t src, int t, int last, int wave, int lane) {
+__device__ inline void stage_load(const WeighProblem& p, const Rows& r, Staged<kFp8>& x, int entry, int t, int wave, int lane) {
   constexpr int kRowB = kFp8 ? 576 : 1152;
   typedef decltype(x.c[0] + x.c[0]) cvec;
   typedef decltype(x.ka) kvec;
-  const int pos = min(kWeighKeys * t + 8 * wave + (lane >> 3), last);
-  const uint64_t at = (uint64_t)(uintptr_t)p.src.kv + (uint64_t)src * kRowB;
+  const int pos = stage_pos(r, t, wave, lane);
+  int64_t src = r.begin + pos;
+  if (r.table) src = clamp64(entry, 0, p.src.pool_blocks - 1) * p.src.block_size + pos % p.src.block_size;
+  const int64_t at = src * kRowB;
+  const char* const kv = static_cast<const char*>(p.src.kv);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint64_t row = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(at >> 32), 8 * i) << 32 |
-                         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, 8 * i);
-    x.c[i] = reinterpret_cast<const cvec*>(row)[lane];
+    const int64_t row = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(at >> 32), 8 * i) << 32 |
+                        (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, 8 * i);
+    x.c[i] = reinterpret_cast<const cvec*>(kv + row)[lane];
   }
-  const char* const rope = reinterpret_cast<const char*>(at) + (kFp8 ? 512 : 1024) + sizeof(kvec) * (lane & 7);
+  const char* const rope = kv + at + (kFp8 ? 512 : 1024) + sizeof(kvec) * (lane & 7);
   x.ka = *reinterpret_cast<const kvec*>(rope);
   x.kb = *reinterpret_cast<const kvec*>(rope + 8 * sizeof(kvec));
   const int64_t rp = source_rope_row(p.src, pos) * 32 + 4 * (lane & 7);
@@ -286,8 +298,8 @@ __global__ __launch_bounds__(256, 2) void weigh_scores_kernel(WeighProblem p, in
   const int item = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= per || item >= items) return;
   const int span = item / groups, block = item % groups * kWR + wr;
-  const int rows = p.count * p.nh, row = min(32 * block + r32, rows - 1);
-  const bool valid = 32 * block + r32 < rows;
+  const int row = 32 * block + r32;
+  const bool valid = row < p.count * p.nh;
   const Spans sp{p};
   const int T_all = sp.total(), W = min(p.spans, T_all);
   if (span >= W) return;
@@ -296,40 +308,34 @@ __global__ __launch_bounds__(256, 2) void weigh_scores_kernel(WeighProblem p, in
   int i, first, n;
   if (!sp.find(t, &i, &first, &n)) return;
   while (true) {
-    const int s = p.seq0 + i, len = source_rows(p.src, s), last = len - 1;
-    const int end = min(t_end, first + n);
-    // ---- the queries' operands: [16 k + 8 g .. + 7] of the row, times the softmax's scale ----
-    const float q_scale = p.scale_log2 * Mm<T>::kUp;
+    const int s = p.seq0 + i, len = source_rows(p.src, s), end = min(t_end, first + n);
+    // ---- the queries' operands: [16 k + 8 g .. + 7] of the row, 1 KB per step ----
     vec qh[kC + kR], ql[kC + kR];
     {
-      const int64_t q = ((int64_t)s * p.tokens + p.token0) * p.nh + row;
-      const float *const qa = p.q_abs + q * 512 + 16 * kC * kd + 8 * g, *const qr = p.q_rope + q * 64 + 16 * kR * kd + 8 * g;
+      const int64_t at = (((int64_t)s * qprep_rows_per_seq(p.tokens * p.nh) + p.token0 * p.nh) / 32 + min(block, row_blocks - 1)) * (32 * kQPrepRow);
+      const elem *const q = static_cast<const elem*>(p.q_prep) + at + 8 * lane, *const low = q + p.low;
 #pragma unroll
       for (int k = 0; k < kC + kR; ++k) {
-        const float* const from = k < kC ? qa + 16 * k : qr + 16 * (k - kC);
-        const f32x4 a = *reinterpret_cast<const f32x4*>(from), b = *reinterpret_cast<const f32x4*>(from + 4);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          elem h, l;
-          split<T>((e < 4 ? a[e & 3] : b[e & 3]) * q_scale, h, l);
-          qh[k][e] = h;
-          ql[k][e] = l;
-        }
+        const int step = 512 * (k < kC ? kC * kd + k : 32 + kR * kd + k - kC);
+        qh[k] = *reinterpret_cast<const vec*>(q + step);
+        ql[k] = *reinterpret_cast<const vec*>(low + step);
       }
     }
     // keys that the row's token sees
     const int sees = len - p.tokens + p.token0 + row / p.nh + 1;
     float m = kNoScore, l = 0.f;
-    Staged<kFp8> x;  // the next tile, and the rows of the one after it
+    Staged<kFp8> x;  // the next tile, and the table's entry of the one after it
     auto tile = [&](int u) { return min(u, end - 1) - first; };
-    stage_load<kFp8>(p, x, stage_row(p, s, tile(t), last, wave, lane), tile(t), last, wave, lane);
-    int64_t src = stage_row(p, s, tile(t + 1), last, wave, lane);
+    const Rows from{p.src.block_table ? 0 : source_begin(p.src, s),
+                    p.src.block_table ? p.src.block_table + (int64_t)s * p.src.blocks_per_seq : nullptr, len - 1};
+    stage_load<kFp8>(p, from, x, stage_entry(p, from, tile(t), wave, lane), tile(t), wave, lane);
+    int entry = stage_entry(p, from, tile(t + 1), wave, lane);
     for (int u = t; u < end; ++u) {
       // (the waves meet again before the sums, or below: the tile before is read)
       if (kKD == 1 && u > t) lds_barrier();
       stage_store<T, kFp8>(x, L, wave, lane);
-      stage_load<kFp8>(p, x, src, tile(u + 1), last, wave, lane);
-      src = stage_row(p, s, tile(u + 2), last, wave, lane);
+      stage_load<kFp8>(p, from, x, entry, tile(u + 1), wave, lane);
+      entry = stage_entry(p, from, tile(u + 2), wave, lane);
       lds_barrier();
       const lchar* const b = L;
       f32x16 acc = {};
@@ -534,7 +540,39 @@ hipError_t scores_w(const WeighProblem& p, int row_blocks, hipStream_t stream) {
   return scores_t<T, kFp8, 2>(p, row_blocks, stream);
 }
 
+// Queries' operands from absorbed fp32 ones, where the absorption does not write them: 8 elements of a row per thread.
+template <typename T>
+__global__ __launch_bounds__(256) void weigh_queries_kernel(WeighProblem p, int64_t first) {
+  typedef typename Mm<T>::elem elem;
+  const int64_t n = (int64_t)p.src.num_seqs * p.tokens * p.nh * (kQPrepRow / 8), i = (first + blockIdx.x) * 256 + threadIdx.x;
+  if (i >= n) return;
+  const int64_t row = i / (kQPrepRow / 8);
+  const int j = 8 * (int)(i % (kQPrepRow / 8)), each = p.tokens * p.nh;
+  const float* const from = j < 512 ? p.q_abs + row * 512 + j : p.q_rope + row * 64 + j - 512;
+  const int64_t at = qprep_index(row / each * qprep_rows_per_seq(each) + row % each, j);
+  elem* const to = static_cast<elem*>(const_cast<void*>(p.q_prep)) + at;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    elem h, l;
+    split<T>(from[e] * (p.scale_log2 * Mm<T>::kUp), h, l);
+    to[e] = h;
+    to[p.low + e] = l;
+  }
+}
+
 }  // namespace
+
+float weigh_query_scale(const WeighProblem& p) {
+  return p.scale_log2 * (p.src.kv_dtype == LA_DTYPE_F16 ? Mm<__half>::kUp : Mm<__hip_bfloat16>::kUp);
+}
+
+hipError_t launch_weigh_queries(const WeighProblem& p, hipStream_t stream) {
+  const int64_t n = (int64_t)p.src.num_seqs * p.tokens * p.nh * (kQPrepRow / 8);
+  const auto k = p.src.kv_dtype == LA_DTYPE_F16 ? weigh_queries_kernel<__half> : weigh_queries_kernel<__hip_bfloat16>;
+  return in_grids((n + 255) / 256, most_blocks(256), [&](int64_t first, unsigned blocks) {
+    hipLaunchKernelGGL(k, dim3(blocks), dim3(256), 0, stream, p, first);
+  });
+}
 
 hipError_t launch_weigh_plain(const WeighProblem& p, hipStream_t stream) {
   const int64_t items = (int64_t)p.src.num_seqs * p.tokens * p.nh;
@@ -550,8 +588,15 @@ hipError_t launch_weigh_plain(const WeighProblem& p, hipStream_t stream) {
   return e;
 }
 
+int weigh_count(int tokens, int nh) {
+  if ((int64_t)tokens * nh <= kWeighRows) return tokens;
+  int whole = 1;  // tokens of whole blocks of 32 rows
+  while (whole * nh % 32 != 0) whole *= 2;
+  return kWeighRows / nh / whole * whole;
+}
+
 bool weigh_mfma_supported(const WeighProblem& p) {
-  if (p.src.kv_dtype == LA_DTYPE_F32 || p.dc != 512 || p.dR != 64 || p.nh > kWeighRows) return false;
+  if (p.src.kv_dtype == LA_DTYPE_F32 || p.dc != 512 || p.dR != 64 || weigh_count(p.tokens, p.nh) < 1) return false;
   // 16-byte loads of rows and tables
   if (((reinterpret_cast<uintptr_t>(p.src.kv) | reinterpret_cast<uintptr_t>(p.src.cos) | reinterpret_cast<uintptr_t>(p.src.sin)) & 15) != 0)
     return false;
