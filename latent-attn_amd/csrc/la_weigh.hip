@@ -5,6 +5,8 @@
 // against each other, so they and the scores are kept to fp32.
 #include "la_draft.hpp"
 
+#include <type_traits>
+
 namespace la {
 namespace {
 
@@ -166,21 +168,18 @@ __host__ __device__ constexpr int row_at(int r) { return r * kPitch + 16 * ((r >
 __device__ inline int rope_piece(int row, int piece) { return row * 128 + 16 * (piece ^ ((row >> 1) & 7)); }
 constexpr int kRopeHi = (row_at(31) + 1024 + 127) / 128 * 128, kRopeLo = kRopeHi + 32 * 128, kTile = kRopeLo + 32 * 128;
 
-// What a wave holds of a tile on its way to LDS: its 8 rows' latent parts, 16 (8-bit
-// rows: 8) B of each row per lane, and the rope part of row lane / 8, pairs 4 (lane % 8) .. + 3.
-template <bool kFp8>
-struct Staged;
-template <>
-struct Staged<false> {
-  u32x4 c[8];
-  u32x2 ka, kb;
-  f32x4 cs, sn;
-};
-template <>
-struct Staged<true> {
-  u32x2 c[8];
-  uint32_t ka, kb;
-  f32x4 cs, sn;
+// What a wave of kW holds of a tile on its way to LDS: the latent parts of its kS = 32 / kW rows,
+// 16 (8-bit rows: 8) B of each per lane, and kP pairs of the rope part of row lane / kLR.
+template <bool kFp8, int kW>
+struct Staged {
+  static constexpr int kS = 32 / kW, kLR = 64 / kS, kP = 32 / kLR;
+  typedef typename std::conditional<kFp8, u32x2, u32x4>::type cvec;
+  typedef typename std::conditional<(kFp8 ? kP : 2 * kP) == 8, u32x2,
+                                    typename std::conditional<(kFp8 ? kP : 2 * kP) == 4, uint32_t, uint16_t>::type>::type kvec;
+  typedef float pvec __attribute__((ext_vector_type(kP)));
+  cvec c[kS];
+  kvec ka, kb;
+  pvec cs, sn;
 };
 // A sequence's rows: the first (contiguous caches) and the last, and its block table.
 struct Rows {
@@ -190,42 +189,44 @@ struct Rows {
 };
 // Position of the lane's part of tile t (past the last row: that one), and its block
 // table's entry: looked up a tile before its loads, so that it has arrived by then.
+template <int kW>
 __device__ inline int stage_pos(const Rows& r, int t, int wave, int lane) {
-  return min(kWeighKeys * t + 8 * wave + (lane >> 3), r.last);
+  return min(kWeighKeys * t + 32 / kW * wave + lane / (2 * kW), r.last);
 }
+template <int kW>
 __device__ inline int stage_entry(const WeighProblem& p, const Rows& r, int t, int wave, int lane) {
-  return r.table ? r.table[stage_pos(r, t, wave, lane) / p.src.block_size] : 0;
+  return r.table ? r.table[stage_pos<kW>(r, t, wave, lane) / p.src.block_size] : 0;
 }
-template <bool kFp8>
-__device__ inline void stage_load(const WeighProblem& p, const Rows& r, Staged<kFp8>& x, int entry, int t, int wave, int lane) {
+template <bool kFp8, int kW>
+__device__ inline void stage_load(const WeighProblem& p, const Rows& r, Staged<kFp8, kW>& x, int entry, int t, int wave, int lane) {
+  typedef Staged<kFp8, kW> S;
   constexpr int kRowB = kFp8 ? 576 : 1152;
-  typedef decltype(x.c[0] + x.c[0]) cvec;
-  typedef decltype(x.ka) kvec;
-  const int pos = stage_pos(r, t, wave, lane);
+  const int pos = stage_pos<kW>(r, t, wave, lane);
   int64_t src = r.begin + pos;
   if (r.table) src = clamp64(entry, 0, p.src.pool_blocks - 1) * p.src.block_size + pos % p.src.block_size;
   const int64_t at = src * kRowB;
   const char* const kv = static_cast<const char*>(p.src.kv);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t row = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(at >> 32), 8 * i) << 32 |
-                        (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, 8 * i);
-    x.c[i] = reinterpret_cast<const cvec*>(kv + row)[lane];
+  for (int i = 0; i < S::kS; ++i) {
+    const int64_t row = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(at >> 32), S::kLR * i) << 32 |
+                        (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, S::kLR * i);
+    x.c[i] = reinterpret_cast<const typename S::cvec*>(kv + row)[lane];
   }
-  const char* const rope = kv + at + (kFp8 ? 512 : 1024) + sizeof(kvec) * (lane & 7);
-  x.ka = *reinterpret_cast<const kvec*>(rope);
-  x.kb = *reinterpret_cast<const kvec*>(rope + 8 * sizeof(kvec));
-  const int64_t rp = source_rope_row(p.src, pos) * 32 + 4 * (lane & 7);
-  x.cs = *reinterpret_cast<const f32x4*>(p.src.cos + rp);
-  x.sn = *reinterpret_cast<const f32x4*>(p.src.sin + rp);
+  const char* const rope = kv + at + (kFp8 ? 512 : 1024) + sizeof(typename S::kvec) * (lane % S::kLR);
+  x.ka = *reinterpret_cast<const typename S::kvec*>(rope);
+  x.kb = *reinterpret_cast<const typename S::kvec*>(rope + (kFp8 ? 32 : 64));
+  const int64_t rp = source_rope_row(p.src, pos) * 32 + S::kP * (lane % S::kLR);
+  x.cs = *reinterpret_cast<const typename S::pvec*>(p.src.cos + rp);
+  x.sn = *reinterpret_cast<const typename S::pvec*>(p.src.sin + rp);
 }
-template <typename T, bool kFp8>
-__device__ inline void stage_store(const Staged<kFp8>& x, lchar* L, int wave, int lane) {
+template <typename T, bool kFp8, int kW>
+__device__ inline void stage_store(const Staged<kFp8, kW>& x, lchar* L, int wave, int lane) {
+  typedef Staged<kFp8, kW> S;
   typedef typename Mm<T>::elem elem;
   auto put = [&](int at, auto v) { *reinterpret_cast<__attribute__((address_space(3))) decltype(v)*>(L + at) = v; };
-  const int row0 = row_at(8 * wave) + 16 * lane;  // row 8 w + i is 1088 i + 16 (i / 4) on
+  const int row0 = row_at(S::kS * wave) + 16 * lane;  // row i of the wave is 1088 i + 16 (i / 4) on
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < S::kS; ++i) {
     u32x4 y;
     if constexpr (kFp8) {
       y[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.c[i][0], 1.f, false));
@@ -237,28 +238,33 @@ __device__ inline void stage_store(const Staged<kFp8>& x, lchar* L, int wave, in
     }
     put(row0 + kPitch * i + 16 * (i >> 2), y);
   }
-  const int row = 8 * wave + (lane >> 3), u = lane & 7;
-  typedef elem e4 __attribute__((ext_vector_type(4)));
-  e4 ah, al, bh, bl;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float a, b;
+  // element e of a lane's share
+  auto word = [](const typename S::kvec& v, int i) -> uint32_t {
+    if constexpr (sizeof(v) == 8) return v[i];
+    else return (uint32_t)v;
+  };
+  auto value = [&](const typename S::kvec& v, int e) -> float {
     if constexpr (kFp8) {
-      const auto va = (e & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8(x.ka, true) : __builtin_amdgcn_cvt_pk_f32_fp8(x.ka, false);
-      const auto vb = (e & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8(x.kb, true) : __builtin_amdgcn_cvt_pk_f32_fp8(x.kb, false);
-      a = va[e & 1];
-      b = vb[e & 1];
+      const uint32_t w = word(v, 0);
+      const auto two = (e & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8(w, true) : __builtin_amdgcn_cvt_pk_f32_fp8(w, false);
+      return two[e & 1];
     } else {
-      a = (float)__builtin_bit_cast(elem, (uint16_t)(x.ka[e >> 1] >> (16 * (e & 1))));
-      b = (float)__builtin_bit_cast(elem, (uint16_t)(x.kb[e >> 1] >> (16 * (e & 1))));
+      return (float)__builtin_bit_cast(elem, (uint16_t)(word(v, e >> 1) >> (16 * (e & 1))));
     }
+  };
+  typedef elem evec __attribute__((ext_vector_type(S::kP)));
+  evec ah, al, bh, bl;
+#pragma unroll
+  for (int e = 0; e < S::kP; ++e) {
+    const float a = value(x.ka, e), b = value(x.kb, e);
     elem h, l;
     split<T>(a * x.cs[e] - b * x.sn[e], h, l);
     ah[e] = h, al[e] = l;
     split<T>(a * x.sn[e] + b * x.cs[e], h, l);
     bh[e] = h, bl[e] = l;
   }
-  const int pa = rope_piece(row, u >> 1) + 8 * (u & 1), pb = rope_piece(row, 4 + (u >> 1)) + 8 * (u & 1);
+  const int row = S::kS * wave + lane / S::kLR, i0 = S::kP * (lane % S::kLR);
+  const int pa = rope_piece(row, i0 >> 3) + 2 * (i0 & 7), pb = rope_piece(row, 4 + (i0 >> 3)) + 2 * (i0 & 7);
   put(kRopeHi + pa, ah);
   put(kRopeLo + pa, al);
   put(kRopeHi + pb, bh);
@@ -275,22 +281,29 @@ __device__ inline void stage_store(const Staged<kFp8>& x, lchar* L, int wave, in
 // summed in fp32: 2 products for the latent part, 3 for the rope part, whose
 // rotated keys have two parts as well. bf16 leaves 2^-18 of an operand, fp16 less.
 //
-// 4 waves: kWR of them have 32 rows of queries each, with their operands in
-// registers for the whole segment, the 4 / kWR others of a row block take shares of
-// the contraction, summed through LDS (few heads: a wave per row block alone would
-// leave three quarters of the matrix cores idle). Tiles go HBM -> registers -> LDS,
-// the next but one on its way during the products.
-template <typename T, bool kFp8, int kWR>
-__global__ __launch_bounds__(256, 2) void weigh_scores_kernel(WeighProblem p, int row_blocks) {
+// kWR of the kW waves have 32 rows of queries each, with their operands in registers
+// for the whole segment; the kKD = kW / kWR others of a row block take shares of the
+// contraction, summed through LDS. So all matrix cores work whatever the rows, and
+// a SIMD has two waves (256 registers each), one's other work under the other's
+// products: up to 64 rows in two workgroups of 4 waves per CU, more in one of 8, whose
+// tiles serve 128 rows. Tiles go HBM -> registers -> LDS, the next one on its way
+// during the products.
+constexpr int weigh_sums(int kWR, int kW) { return (kW / kWR == 2 ? 2048 : 4096) * kW; }
+template <typename T, bool kFp8, int kWR, int kW>
+__global__ __launch_bounds__(64 * kW, 2) void weigh_scores_kernel(WeighProblem p, int row_blocks) {
   typedef typename Mm<T>::vec vec;
   typedef typename Mm<T>::elem elem;
-  constexpr int kKD = 4 / kWR;            // shares of the contraction
+  typedef __attribute__((address_space(3))) f32x4 lvec;
+  constexpr int kKD = kW / kWR;           // shares of the contraction
   constexpr int kC = 32 / kKD;            // latent steps of 16 of a share
   constexpr int kR = 4 / kKD;             // rope steps
   constexpr int kN = 16 / kKD;            // scores of a lane after the sum
+  constexpr bool kTwo = kW == 8;          // two buffers of a tile and of its sums: one barrier a tile
+  constexpr int kSums = weigh_sums(kWR, kW);
+  static_assert(kKD == 2 || kKD == 4, "the waves meet at the sums, behind a tile's last read");
   extern __shared__ __attribute__((aligned(1024))) char weigh_lds[];
   lchar* const L = (lchar*)weigh_lds;
-  lchar* const sums = L + kTile;          // kKD > 1: 4 KB per wave
+  lchar* const sums0 = L + (kTwo ? 2 : 1) * kTile;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int wr = wave % kWR, kd = wave / kWR, r32 = lane & 31, g = lane >> 5;
   // an eighth of the items to each XCD, row groups of a span together
@@ -309,6 +322,12 @@ __global__ __launch_bounds__(256, 2) void weigh_scores_kernel(WeighProblem p, in
   if (!sp.find(t, &i, &first, &n)) return;
   while (true) {
     const int s = p.seq0 + i, len = source_rows(p.src, s), end = min(t_end, first + n);
+    Staged<kFp8, kW> x;  // the next tile, and the table's entry of the one after it
+    auto tile = [&](int u) { return min(u, end - 1) - first; };
+    const Rows from{p.src.block_table ? 0 : source_begin(p.src, s),
+                    p.src.block_table ? p.src.block_table + (int64_t)s * p.src.blocks_per_seq : nullptr, len - 1};
+    stage_load(p, from, x, stage_entry<kW>(p, from, tile(t), wave, lane), tile(t), wave, lane);
+    int entry = stage_entry<kW>(p, from, tile(t + 1), wave, lane);
     // ---- the queries' operands: [16 k + 8 g .. + 7] of the row, 1 KB per step ----
     vec qh[kC + kR], ql[kC + kR];
     {
@@ -324,20 +343,20 @@ __global__ __launch_bounds__(256, 2) void weigh_scores_kernel(WeighProblem p, in
     // keys that the row's token sees
     const int sees = len - p.tokens + p.token0 + row / p.nh + 1;
     float m = kNoScore, l = 0.f;
-    Staged<kFp8> x;  // the next tile, and the table's entry of the one after it
-    auto tile = [&](int u) { return min(u, end - 1) - first; };
-    const Rows from{p.src.block_table ? 0 : source_begin(p.src, s),
-                    p.src.block_table ? p.src.block_table + (int64_t)s * p.src.blocks_per_seq : nullptr, len - 1};
-    stage_load<kFp8>(p, from, x, stage_entry(p, from, tile(t), wave, lane), tile(t), wave, lane);
-    int entry = stage_entry(p, from, tile(t + 1), wave, lane);
-    for (int u = t; u < end; ++u) {
-      // (the waves meet again before the sums, or below: the tile before is read)
-      if (kKD == 1 && u > t) lds_barrier();
-      stage_store<T, kFp8>(x, L, wave, lane);
-      stage_load<kFp8>(p, from, x, entry, tile(u + 1), wave, lane);
-      entry = stage_entry(p, from, tile(u + 2), wave, lane);
+    if constexpr (kTwo) {
+      stage_store<T>(x, L, wave, lane);
+      stage_load(p, from, x, entry, tile(t + 1), wave, lane);
+      entry = stage_entry<kW>(p, from, tile(t + 2), wave, lane);
       lds_barrier();
-      const lchar* const b = L;
+    }
+    for (int u = t; u < end; ++u) {
+      // (the waves have met behind the last read of the tile before, at its sums)
+      stage_store<T>(x, L + (kTwo ? (u + 1 - t) & 1 : 0) * kTile, wave, lane);
+      stage_load(p, from, x, entry, tile(u + (kTwo ? 2 : 1)), wave, lane);
+      entry = stage_entry<kW>(p, from, tile(u + (kTwo ? 3 : 2)), wave, lane);
+      if constexpr (!kTwo) lds_barrier();
+      const lchar* const b = L + (kTwo ? (u - t) & 1 : 0) * kTile;
+      lchar* const sums = sums0 + (kTwo ? (u - t) & 1 : 0) * kSums;
       f32x16 acc = {};
       auto operand = [&](int k) -> vec {  // keys r32, elements [16 k + 8 g .. + 7]
         const int at = k < kC ? row_at(r32) + 32 * (kC * kd + k) + 16 * g
@@ -358,20 +377,26 @@ __global__ __launch_bounds__(256, 2) void weigh_scores_kernel(WeighProblem p, in
         __builtin_amdgcn_sched_barrier(0);
       }
       settle(acc);
-      // lane: row r32, keys 8 (e / 4) + 4 g + e % 4
+      // lane: row r32, keys 8 (e / 4) + 4 g + e % 4; this share's are quads kN / 4 kd and on
       float sc[kN];
-      if constexpr (kKD == 1) {
+      auto quad = [&](int q) {
+        return f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+      };
+      if constexpr (kKD == 2) {  // the other's quads to it, its for this wave back
+        lchar* const mine = sums + 2048 * wave + 16 * lane;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sc[e] = acc[e] * (1.f / Mm<T>::kUp);
-      } else {
-        typedef __attribute__((address_space(3))) f32x4 lvec;
+        for (int q = 0; q < 2; ++q) *reinterpret_cast<lvec*>(mine + 1024 * q) = kd == 0 ? quad(2 + q) : quad(q);
+        lds_barrier();
+        const lchar* const its = sums + 2048 * (wr + kWR * (1 - kd)) + 16 * lane;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          f32x4 v;
+        for (int q = 0; q < 2; ++q) {
+          const f32x4 v = *reinterpret_cast<const lvec*>(its + 1024 * q), own = kd == 0 ? quad(q) : quad(2 + q);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = acc[4 * q + e] * (1.f / Mm<T>::kUp);
-          *reinterpret_cast<lvec*>(sums + 4096 * wave + 1024 * q + 16 * lane) = v;
+          for (int e = 0; e < 4; ++e) sc[4 * q + e] = (own[e] + v[e]) * (1.f / Mm<T>::kUp);
         }
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *reinterpret_cast<lvec*>(sums + 4096 * wave + 1024 * q + 16 * lane) = quad(q);
         lds_barrier();
 #pragma unroll
         for (int q = 0; q < kN / 4; ++q) {
@@ -380,7 +405,7 @@ __global__ __launch_bounds__(256, 2) void weigh_scores_kernel(WeighProblem p, in
           for (int w = 0; w < kKD; ++w)
             v += *reinterpret_cast<const lvec*>(sums + 4096 * (wr + kWR * w) + 1024 * (kN / 4 * kd + q) + 16 * lane);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[4 * q + e] = v[e];
+          for (int e = 0; e < 4; ++e) sc[4 * q + e] = v[e] * (1.f / Mm<T>::kUp);
         }
       }
       const int key0 = kWeighKeys * (u - first) + 2 * kN * kd + 4 * g;
@@ -418,16 +443,14 @@ __global__ __launch_bounds__(256, 2) void weigh_scores_kernel(WeighProblem p, in
       const auto sl = __builtin_amdgcn_permlane32_swap(u_of(l), u_of(l), false, false);
       m = f_of(sm[0]), l = f_of(sl[0]);
       join(f_of(sm[1]), f_of(sl[1]));
-      if constexpr (kKD > 1) {
-        typedef __attribute__((address_space(3))) float lfloat;
-        lfloat* const ml = reinterpret_cast<lfloat*>(sums) + 64 * wave;
-        if (g == 0) ml[r32] = m, ml[32 + r32] = l;
-        lds_barrier();
+      typedef __attribute__((address_space(3))) float lfloat;
+      lfloat* const ml = reinterpret_cast<lfloat*>(sums0) + 64 * wave;
+      if (g == 0) ml[r32] = m, ml[32 + r32] = l;
+      lds_barrier();
 #pragma unroll
-        for (int w = 1; w < kKD; ++w) {
-          const lfloat* const o = reinterpret_cast<const lfloat*>(sums) + 64 * (wr + kWR * w);
-          if (kd == 0) join(o[r32], o[32 + r32]);
-        }
+      for (int w = 1; w < kKD; ++w) {
+        const lfloat* const o = reinterpret_cast<const lfloat*>(sums0) + 64 * (wr + kWR * w);
+        if (kd == 0) join(o[r32], o[32 + r32]);
       }
       if (kd == 0 && g == 0 && block < row_blocks) {
         float* const to = p.part + (int64_t)(span + i) * 2 * 32 * row_blocks + 32 * block + r32;
@@ -524,20 +547,22 @@ __global__ __launch_bounds__(256) void weigh_sum_kernel(WeighProblem p, int row_
   }
 }
 
-template <typename T, bool kFp8, int kWR>
+template <typename T, bool kFp8, int kWR, int kW>
 hipError_t scores_t(const WeighProblem& p, int row_blocks, hipStream_t stream) {
-  constexpr int lds = kTile + (kWR < 4 ? 4 * 4096 : 0);
+  constexpr int lds = (kW == 8 ? 2 : 1) * (kTile + weigh_sums(kWR, kW));
   static OncePerDevice once;
-  const hipError_t e = allow_lds(once, reinterpret_cast<const void*>(&weigh_scores_kernel<T, kFp8, kWR>), lds);
+  const auto k = weigh_scores_kernel<T, kFp8, kWR, kW>;
+  const hipError_t e = allow_lds(once, reinterpret_cast<const void*>(k), lds);
   if (e != hipSuccess) return e;
   const int64_t items = (int64_t)p.spans * ((row_blocks + kWR - 1) / kWR);
-  hipLaunchKernelGGL((weigh_scores_kernel<T, kFp8, kWR>), dim3((unsigned)(8 * ((items + 7) / 8))), dim3(256), lds, stream, p, row_blocks);
+  hipLaunchKernelGGL(k, dim3((unsigned)(8 * ((items + 7) / 8))), dim3(64 * kW), lds, stream, p, row_blocks);
   return hipGetLastError();
 }
 template <typename T, bool kFp8>
 hipError_t scores_w(const WeighProblem& p, int row_blocks, hipStream_t stream) {
-  if (row_blocks == 1) return scores_t<T, kFp8, 1>(p, row_blocks, stream);
-  return scores_t<T, kFp8, 2>(p, row_blocks, stream);
+  if (row_blocks == 1) return scores_t<T, kFp8, 1, 4>(p, row_blocks, stream);
+  if (row_blocks == 2) return scores_t<T, kFp8, 2, 4>(p, row_blocks, stream);
+  return scores_t<T, kFp8, 4, 8>(p, row_blocks, stream);
 }
 
 // Queries' operands from absorbed fp32 ones, where the absorption does not write them: 8 elements of a row per thread.
@@ -603,9 +628,9 @@ bool weigh_mfma_supported(const WeighProblem& p) {
   return device_is_gfx950();
 }
 
-int weigh_spans(int rows, int ncu) {
-  const int blocks = (rows + 31) / 32, groups = (blocks + 1) / 2;
-  return groups < 2 * ncu ? 2 * ncu / groups : 1;
+int weigh_spans(int rows, int ncu) {  // as many workgroups as run at once
+  const int blocks = (rows + 31) / 32, groups = blocks <= 2 ? 1 : (blocks + 3) / 4, most = blocks <= 2 ? 2 * ncu : ncu;
+  return groups < most ? most / groups : 1;
 }
 
 hipError_t launch_weigh_mfma(const WeighProblem& p, int64_t most_tiles, hipStream_t stream, int ncu) {
