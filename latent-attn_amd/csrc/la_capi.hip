@@ -63,6 +63,7 @@ struct Plan {
   bool f32 = false;  // decode_f32_kernel
   int waves16 = 0;  // 4 / 8: decode_mfma16_kernel with that many waves; 0: decode_mfma_kernel
   int chunk_len = 0;
+  int shortest = 0;  // tiles of a span at least
   int num_chunks = 0;
   int num_slots = 0;
   bool proj_mfma = false;
@@ -79,7 +80,7 @@ struct Plan {
 // coarse: the chunks of one 128-head (or VALU) workgroup per target block, also
 // for the kernels with 16 heads per workgroup: fewer partial slots, for a caller
 // whose scratch does not hold the others.
-int prepare(const la_decode_args* a, DecodeProblem* p, Plan* plan, bool coarse = false) {
+int prepare(const la_decode_args* a, DecodeProblem* p, Plan* plan, bool coarse = false, bool tree = false) {
   if (!a || !valid_cfg(&a->cfg)) return LA_ERROR_INVALID_VALUE;
   const int chunk_rows = a->chunk_rows;
   const int variant = a->kernel_variant;
@@ -177,7 +178,7 @@ int prepare(const la_decode_args* a, DecodeProblem* p, Plan* plan, bool coarse =
   const int heads16 = pl.mfma ? p->Hq / 16 : 0;
   const bool by_fill = a->seq_lens && chunk_rows == 0 && 4LL * a->num_seqs <= ncu;
   const int64_t most16 = a->num_seqs == 1 ? 200000 : 240000;
-  const bool few_heads = pl.mfma && (heads16 == 1 || (heads16 == 2 && (a->kv_dtype == LA_DTYPE_FP8_E4M3 || by_fill ||
+  const bool few_heads = pl.mfma && !tree && (heads16 == 1 || (heads16 == 2 && (a->kv_dtype == LA_DTYPE_FP8_E4M3 || by_fill ||
                                                                        total <= most16)));
   int64_t L, min_rows = 64;
   if (chunk_rows > 0) {
@@ -230,7 +231,12 @@ int prepare(const la_decode_args* a, DecodeProblem* p, Plan* plan, bool coarse =
   if (L > (int64_t)1 << 30) L = (int64_t)1 << 30;
   if ((pl.mfma || pl.f32) && L > kMaxChunkRows) L = kMaxChunkRows;
   if (paged && (pl.mfma || pl.f32)) L = (L + 63) / 64 * 64;  // MFMA tiles start block-aligned
-  const int64_t nchunks = total > 0 ? (total + L - 1) / L : 0;
+  int64_t nchunks = total > 0 ? (total + L - 1) / L : 0;
+  if (tree && total > 0) {  // spans, their length found on the device: as many as there is room for
+    const int64_t rows = total + (int64_t)a->num_seqs * (kSpanRows - 1), groups = (p->Hq + mfma_heads_per_group() - 1) / mfma_heads_per_group();
+    nchunks = std::max(std::min(std::max<int64_t>(ncu / groups, 1), (rows + min_rows - 1) / min_rows),
+                       (rows + kMaxChunkRows - 1) / kMaxChunkRows);
+  }
   if (nchunks > (int64_t)1 << 30) return LA_ERROR_INVALID_VALUE;
   pl.chunk_len = (int)L;
   pl.num_chunks = (int)nchunks;
@@ -239,7 +245,7 @@ int prepare(const la_decode_args* a, DecodeProblem* p, Plan* plan, bool coarse =
   // 128 heads 16.2 us on the 128-head kernel, 7.9 here; 1 x 8192 17.0 / 11.6;
   // four times that (16 queries over 2048 rows) 21.7 / 36.3. With at most one
   // workgroup per CU, 8 waves take 128 positions per round trip.
-  if (pl.mfma && (few_heads || (heads16 > 2 && nchunks * heads16 <= 2 * ncu)))
+  if (pl.mfma && !tree && (few_heads || (heads16 > 2 && nchunks * heads16 <= 2 * ncu)))
     pl.waves16 = nchunks * heads16 <= ncu && L >= 128 ? 8 : 4;
   pl.num_slots = nchunks > 0 ? (int)(nchunks + a->num_seqs - 1) : 0;
 
@@ -288,6 +294,7 @@ int prepare(const la_decode_args* a, DecodeProblem* p, Plan* plan, bool coarse =
   // the device (32 of 100 to 500 rows in 512-row regions, 128 heads: 36.4 against
   // 35.5, fp8 38.5 against 37.1).
   if (filled) p->chunk_len = -piece;
+  if (tree) p->chunk_len = kSpans, pl.shortest = (int)((min_rows + kSpanRows - 1) / kSpanRows);
   p->num_chunks = pl.num_chunks;
   p->num_slots = pl.num_slots;
   *plan = pl;
@@ -321,12 +328,11 @@ int run(const la_decode_args* a, hipStream_t stream, hipEvent_t ev_b = nullptr, 
   if (repeat < 0) return LA_ERROR_INVALID_VALUE;
   DecodeProblem p;
   Plan plan;
-  int st = prepare(a, &p, &plan, coarse);
+  const bool tree = tail && tail->tree.seen;
+  int st = prepare(a, &p, &plan, coarse, tree);
   if (st != LA_SUCCESS) return st;
   if (a->num_seqs == 0) return LA_SUCCESS;
-  const bool tree = tail && tail->tree.seen;
   if (tree && !plan.mfma) return LA_ERROR_NOT_SUPPORTED;
-  if (tree) plan.waves16 = 0;
 
   char* ws = static_cast<char*>(a->workspace);
   bool owned = false;
@@ -1351,20 +1357,20 @@ int decode_tree(const la_tree_args* a, void* stream_v, bool run_it, size_t* need
   d.cfg = c;
   DecodeProblem step;
   Plan plan;
-  const bool mfma = a->kernel_variant != kTreePlain && prepare(&d, &step, &plan) == LA_SUCCESS && plan.mfma;
+  const bool mfma = a->kernel_variant != kTreePlain && prepare(&d, &step, &plan, false, true) == LA_SUCCESS && plan.mfma;
   if (!mfma && (a->kernel_variant == kTreeMfma || !generic_prompt_supported(c.kv_lora_rank, c.qk_rope_head_dim)))
     return LA_ERROR_NOT_SUPPORTED;
   const bool join = mfma && merge_join_supported(step);
   // queries that the absorption reads as they are: no copies
   const bool direct = mfma && plan.absorb_prep && absorb_any_supported(t.q, t.src, a->W_UK, a->w_uk_dtype, c);
   if (direct) nope_as_is = rope_as_is = true;
-  const size_t step_bytes = mfma ? la_mla_decode_workspace_size(&d) : 0;
+  const size_t step_bytes = mfma ? plan.total : 0;
 
   float *q_abs = nullptr, *out32 = nullptr;
   void* step_ws = nullptr;
   auto carve = [&](void* ws) {
     Carve v(ws);
-    t.lens = static_cast<int32_t*>(v.take((size_t)a->num_seqs * sizeof(int32_t)));
+    t.lens = static_cast<int32_t*>(v.take(2 * ((size_t)a->num_seqs + 1) * sizeof(int32_t)));
     t.seen = static_cast<uint64_t*>(v.take((size_t)tokens * sizeof(uint64_t)));
     t.cos = static_cast<float*>(v.take((size_t)tokens * (c.qk_rope_head_dim / 2) * sizeof(float)));
     t.sin = static_cast<float*>(v.take((size_t)tokens * (c.qk_rope_head_dim / 2) * sizeof(float)));
@@ -1391,6 +1397,8 @@ int decode_tree(const la_tree_args* a, void* stream_v, bool run_it, size_t* need
   t.dn = c.qk_nope_head_dim;
   t.dR = c.qk_rope_head_dim;
   t.vec = queries_vec(t.q);
+  t.chunks = mfma ? plan.num_chunks : 0;
+  t.shortest = plan.shortest;
   hipError_t e = launch_tree_queries(t, stream);
   if (e != hipSuccess) return scratch.finish(record_hip(e));
   const float* const qn = nope_as_is ? static_cast<const float*>(a->q_nope) : t.q_nope;

@@ -18,7 +18,8 @@ struct TreeQueries {
   int nh, dn, dR;
   float* q_nope;   // (tokens, nh, dn), or nullptr
   float* q_rope;   // (tokens, nh, dR), or nullptr
-  int32_t* lens;   // (num_seqs): rows, 0 where they are fewer than the nodes
+  int32_t* lens;   // (num_seqs): rows, 0 where they are fewer than the nodes; with chunks, the plan of the spans behind them (num_seqs + 2)
+  int chunks, shortest;  // of spans, and the fewest tiles of one (DecodeProblem); 0: none
   uint64_t* seen;  // TreeStep
   float* cos;
   float* sin;

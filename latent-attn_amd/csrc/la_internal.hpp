@@ -320,13 +320,26 @@ __device__ inline int32_t* filled_notes(const DecodeProblem& p) {
   return reinterpret_cast<int32_t*>(reinterpret_cast<char*>(p.part_o) +
                                     (int64_t)p.num_chunks * p.Hq * p.dc * (p.part_f16 ? 2 : 4));
 }
+// Spans (chunk_len == kSpans; the kernels for trees of drafted tokens): chunks of equal
+// length in a row space where every sequence has whole tiles of kSpanRows rows. The
+// kernel that runs before them plans it: behind the num_seqs lengths it leaves every
+// sequence's first tile, the tiles of all, and the tiles of a chunk.
+constexpr int kSpans = INT32_MIN, kSpanRows = 32;
+__device__ inline const int32_t* span_tiles(const DecodeProblem& p) { return p.lens + p.num_seqs; }
+__device__ inline int span_rows(const DecodeProblem& p) { return kSpanRows * span_tiles(p)[p.num_seqs + 1]; }
+__device__ inline int64_t span_begin(const DecodeProblem& p, int s) { return (int64_t)kSpanRows * span_tiles(p)[s]; }
+__device__ inline int64_t span_end(const DecodeProblem& p, int s) {
+  return min(span_begin(p, s) + filled_rows(p, s), span_begin(p, s + 1));
+}
 // Partial slot of the piece of chunk c inside sequence s.
-__device__ inline int64_t slot_of(const DecodeProblem& p, int64_t c, int s) { return c + (p.chunk_len < 0 ? 0 : s); }
+__device__ inline int64_t slot_of(const DecodeProblem& p, int64_t c, int s) {
+  return c + (p.chunk_len < 0 && p.chunk_len != kSpans ? 0 : s);
+}
 // A walk over the segments of one chunk (pieces of it inside one sequence).
 // kFilled: 0, chunks of the regions only (such a kernel keeps the other code,
 // and the registers it holds for later segments, out of its way to the first
 // copy); 1, chunk_len may be < 0; 2, it is (one segment: with the code of the
-// others beside it the 128-head kernel's body spilled two registers).
+// others beside it the 128-head kernel's body spilled two registers); 3, spans.
 template <int kFilled>
 struct ChunkWalk {
   int64_t lo, hi;  // what is left of the chunk, in the plan's row space
@@ -337,7 +350,7 @@ struct ChunkWalk {
 };
 template <int kFilled>
 __device__ inline bool walk_begin(const DecodeProblem& p, int chunk, int group, ChunkWalk<kFilled>& w) {
-  if (kFilled == 2 || (kFilled && p.chunk_len < 0)) {
+  if (kFilled == 2 || (kFilled == 1 && p.chunk_len < 0)) {
     const FilledPiece f = filled_piece(p, chunk);
     // the last two: malformed offsets, whose sums wrap
     if (f.s >= p.num_seqs || chunk < f.first || (int64_t)(chunk - f.first) * f.len >= f.rows) return false;
@@ -352,6 +365,22 @@ __device__ inline bool walk_begin(const DecodeProblem& p, int chunk, int group, 
     }
     return true;
   }
+  if constexpr (kFilled == 3) {
+    const int32_t* const first = span_tiles(p);
+    const int len = span_rows(p);
+    w.lo = (int64_t)chunk * len;
+    w.hi = min(w.lo + len, span_begin(p, p.num_seqs));
+    if (w.lo >= w.hi) return false;
+    w.s = -1;  // the last sequence that begins no later: it has tiles
+    const int lane = wave_lane(), tile = (int)(w.lo / kSpanRows);
+    for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
+      const uint64_t before = __builtin_amdgcn_ballot_w64(s0 + lane < p.num_seqs && first[min(s0 + lane, p.num_seqs)] <= tile);
+      w.s += __builtin_popcountll(before);
+      if (~before) break;
+    }
+    w.s = max(w.s, 0);
+    return true;
+  }
   const int64_t end_all = seq_begin(p, p.num_seqs);
   w.lo = (int64_t)chunk * p.chunk_len;
   w.hi = min(w.lo + (int64_t)p.chunk_len, end_all);
@@ -362,9 +391,22 @@ __device__ inline bool walk_begin(const DecodeProblem& p, int chunk, int group, 
 }
 // The next segment [lo, seg_hi) of sequence s; after it the caller sets lo = seg_hi and ++s.
 template <int kFilled>
-__device__ inline bool walk_next(const DecodeProblem& p, ChunkWalk<kFilled>& w) {
+__device__ inline bool walk_next(const DecodeProblem& p, ChunkWalk<kFilled>& w, int chunk = 0) {
+  if constexpr (kFilled == 3) {  // from the sequence alone: nothing else is held through a segment
+    const int64_t len = span_rows(p), hi = min((chunk + 1) * len, span_begin(p, p.num_seqs));
+    for (; w.s < p.num_seqs; ++w.s) {
+      w.s_lo = span_begin(p, w.s);
+      w.lo = max(chunk * len, w.s_lo);
+      if (w.lo >= hi) return false;
+      w.seg_hi = min(hi, span_end(p, w.s));
+      if (w.lo < w.seg_hi) break;
+    }
+    const int64_t row0 = seq_begin(p, min(w.s, p.num_seqs - 1));
+    w.row0 = (int64_t)__builtin_amdgcn_readfirstlane((int)(row0 >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)row0);  // (else held in vector registers)
+    return w.s < p.num_seqs;
+  }
   while (w.lo < w.hi) {
-    if (kFilled == 2 || (kFilled && p.chunk_len < 0)) return true;  // the one segment, set by walk_begin
+    if (kFilled == 2 || (kFilled == 1 && p.chunk_len < 0)) return true;  // the one segment, set by walk_begin
     w.s_lo = w.row0 = seq_begin(p, w.s);
     w.lo = max(w.lo, w.s_lo);  // past the unfilled rows of the previous region
     if (w.lo >= w.hi) return false;
@@ -381,6 +423,11 @@ __device__ inline bool walk_next(const DecodeProblem& p, ChunkWalk<kFilled>& w) 
 
 // Rows [lo, hi) of sequence s in the plan's row space, and the rows per chunk.
 __device__ inline int seq_in_plan(const DecodeProblem& p, int s, int64_t* lo, int64_t* hi) {
+  if (p.chunk_len == kSpans) {
+    *lo = span_begin(p, s);
+    *hi = span_end(p, s);
+    return span_rows(p);
+  }
   if (p.chunk_len < 0) {
     *hi = *lo = 0;
     const int rows = filled_rows(p, s);

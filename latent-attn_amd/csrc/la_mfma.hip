@@ -1017,7 +1017,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeProblem& p, int gro
   ChunkWalk<kFilled> w;
   if (!walk_begin(p, chunk, group, w)) return;
 
-  while (walk_next(p, w)) {
+  while (walk_next(p, w, chunk)) {
     const int s = w.s;
     SegCtx sg;
     sg.base = reinterpret_cast<const char*>(p.kv) + (kPaged ? 0 : (w.row0 + (w.lo - w.s_lo)) * cache_row_bytes<kFp8>());
@@ -1638,7 +1638,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeProblem& p, int gro
     const int le = lane_id();  // fresh: the prologue's lane index would come back from a spill slot
     const int g2 = le >> 5;
     const float l_tot = sum_halves(l_run);
-    const int64_t slot = kFilled == 2 ? (int64_t)chunk : kFilled ? slot_of(p, chunk, s) : (int64_t)chunk + s;
+    const int64_t slot = kFilled == 2 ? (int64_t)chunk : kFilled == 1 ? slot_of(p, chunk, s) : (int64_t)chunk + s;
     const int64_t hqg = slot * p.Hq + group * kHG;  // slot row of head 0 of the group
     if (le < 32 && 32 * wave + le < hg_heads) {
       p.part_lse[hqg + 32 * wave + le] = m_run + log2f(l_tot);
@@ -1771,10 +1771,10 @@ __global__ __launch_bounds__(kThreads) void decode_mfma_filled_kernel(DecodeProb
   decode_mfma_body<KT, false, kFp8, 2>(p, groups);
 }
 
-// Trees of drafted tokens: kFilled 1 (paged), 2 or 0 (contiguous, filled rows or regions).
-template <typename KT, bool kPaged, bool kFp8, int kFilled>
+// Trees of drafted tokens (spans).
+template <typename KT, bool kPaged, bool kFp8>
 __global__ __launch_bounds__(kThreads) void decode_mfma_tree_kernel(DecodeProblem p, int groups, TreeStep tree) {
-  decode_mfma_body<KT, kPaged, kFp8, kFilled, true>(p, groups, tree);
+  decode_mfma_body<KT, kPaged, kFp8, 3, true>(p, groups, tree);
 }
 
 // Copies-only variant of the attention kernel, for measuring the streaming
@@ -1917,10 +1917,10 @@ hipError_t launch_t(const DecodeProblem& p, hipStream_t stream, hipEvent_t ev_be
   return launch_k(decode_mfma_kernel<KT, false, kFp8>, once[2], p, stream, ev_begin, ev_end);
 }
 
-template <typename KT, bool kPaged, bool kFp8, int kFilled>
+template <typename KT, bool kPaged, bool kFp8>
 hipError_t launch_tree_k(const DecodeProblem& p, const TreeStep& tree, hipStream_t stream) {
   static OncePerDevice once;
-  const auto k = decode_mfma_tree_kernel<KT, kPaged, kFp8, kFilled>;
+  const auto k = decode_mfma_tree_kernel<KT, kPaged, kFp8>;
   const hipError_t e = allow_whole_lds(once, reinterpret_cast<const void*>(k), kTreeLdsBytes);
   if (e != hipSuccess) return e;
   const int groups = (p.Hq + kHG - 1) / kHG;
@@ -1929,9 +1929,7 @@ hipError_t launch_tree_k(const DecodeProblem& p, const TreeStep& tree, hipStream
 }
 template <typename KT, bool kFp8>
 hipError_t launch_tree_t(const DecodeProblem& p, const TreeStep& tree, hipStream_t stream) {
-  if (p.block_table) return launch_tree_k<KT, true, kFp8, 1>(p, tree, stream);
-  if (p.chunk_len < 0) return launch_tree_k<KT, false, kFp8, 2>(p, tree, stream);
-  return launch_tree_k<KT, false, kFp8, 0>(p, tree, stream);
+  return p.block_table ? launch_tree_k<KT, true, kFp8>(p, tree, stream) : launch_tree_k<KT, false, kFp8>(p, tree, stream);
 }
 
 }  // namespace

@@ -34,6 +34,66 @@ __device__ inline uint64_t tree_seen(const int32_t* parents, int s, int n) {
   return seen;
 }
 
+// Rows of sequence s that its tree's attention reads.
+__device__ inline int tree_rows(const TreeQueries& p, int s) {
+  const int rows = source_rows(p.src, s);
+  return rows < p.q.per_seq ? 0 : rows;
+}
+// The spans' plan (kSpans) of one wave. Either the tiles of all sequences are divided
+// evenly, or every sequence starts a chunk of its own, at the fewest tiles a chunk that
+// suffice. A chunk over several sequences pays kSegment tiles for each after the first
+// (a segment's fixed part: its queries, its first tiles' way, its partial rows), own
+// chunks for the shorter last ones: the smaller estimate of the longest chunk is taken.
+constexpr int kSegment = 8;
+__device__ inline void plan_spans(const TreeQueries& p) {
+  const int lane = wave_lane(), seqs = p.q.num_seqs;
+  // 2^24 tiles: more than the memory holds; their sums stay below 2^31 (malformed offsets may overlap)
+  auto tiles = [&](int s) { return s < seqs ? (int)min(((uint32_t)tree_rows(p, s) + kSpanRows - 1) / kSpanRows, 1u << 24) : 0; };
+  const int mine = tiles(lane);
+  int64_t total = 0;
+  int filled = 0, most = 0;
+  for (int s0 = 0; s0 < seqs; s0 += 64) {
+    const int n = s0 == 0 ? mine : tiles(s0 + lane);
+    total += wave_sum_i(n);
+    filled += wave_sum_i(n > 0);
+    most = max(most, n);
+  }
+  for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+  constexpr int kMost = kMaxChunkRows / kSpanRows;
+  const int even = (int)min(max((total + p.chunks - 1) / p.chunks, (int64_t)p.shortest), (int64_t)kMost);
+  int len = even;
+  bool own = false;
+  if (filled <= p.chunks) {
+    auto fits = [&](int n) {
+      int64_t sum = 0;
+      for (int s0 = 0; s0 < seqs; s0 += 64) sum += wave_sum_i(pieces(s0 == 0 ? mine : tiles(s0 + lane), n));
+      return sum <= p.chunks;
+    };
+    int lo = even, hi = max(even, min(most, kMost));
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (fits(mid)) hi = mid;
+      else lo = mid + 1;
+    }
+    own = lo <= even + kSegment * ((filled - 1 + p.chunks - 1) / p.chunks);
+    if (own) len = lo;
+  }
+  int32_t* const first = p.lens + seqs;
+  const int64_t limit = (int64_t)p.chunks * len;
+  int64_t at = 0;
+  for (int s0 = 0; s0 < seqs; s0 += 64) {
+    int n = s0 == 0 ? mine : tiles(s0 + lane);
+    if (own) n = pieces(n, len) * len;
+    const int end = wave_scan(n);
+    if (s0 + lane < seqs) first[s0 + lane] = (int)min(at + end - n, limit);
+    at += __builtin_amdgcn_readlane(end, 63);
+  }
+  if (lane == 0) {
+    first[seqs] = (int)min(at, limit);
+    first[seqs + 1] = len;
+  }
+}
+
 // As tokens_kernel: kElems elements of a token's nope queries, and as many pairs of
 // rope ones, per workgroup (x: token, y: share), kN at a time; the first also
 // writes what the tree's kernels take of its node.
@@ -47,7 +107,7 @@ template <int kN>
 __global__ __launch_bounds__(256) void tree_queries_kernel(TreeQueries p, int64_t token0) {
   const int64_t token = token0 + blockIdx.x;
   const int n = p.q.per_seq, s = (int)(token / n), j = (int)(token % n);
-  const int rows = source_rows(p.src, s), L = rows < n ? 0 : rows, half = p.dR / 2;
+  const int L = tree_rows(p, s), half = p.dR / 2;
   const uint64_t seen = shfl64(tree_seen(p.parents, s, n), j);
   const int at = max(L - n + __popcll(seen) - 1, 0);
   const int64_t pos = source_rope_row(p.src, at);
@@ -62,6 +122,7 @@ __global__ __launch_bounds__(256) void tree_queries_kernel(TreeQueries p, int64_
       if (p.pos) p.pos[token] = at;
       if (j == 0) p.lens[s] = L;
     }
+    if (token == 0 && p.chunks > 0 && threadIdx.x >= 192) plan_spans(p);
   }
   const int first = blockIdx.y * kElems + kN * threadIdx.x, last = (blockIdx.y + 1) * kElems;
   if (p.q_nope)

@@ -103,6 +103,24 @@ def test_other_head_shapes(cuda, dims, heads):
     c.check(c.run(), True, str(dims))
 
 
+# 64 nodes x 128 heads leave a chip of 256 compute units four chunks: several
+# sequences in one, a sequence over several, none in a sequence without rows, and, with
+# sequences of about one length, a chunk each
+@pytest.mark.parametrize("layout", ["capacity", "packed_capacity", "packed", "paged"])
+@pytest.mark.parametrize("rows", [[70, 900, 64, 65, 300, 96, 128], [1200], [64, 64, 64, 64], [63, 700, 1, 690, 64, 10],
+                                  [10, 20, 300]])
+def test_chunks_across_sequences(cuda, layout, rows):
+    case = Case(cuda, layout, rows, 64, heads=128, seed=len(rows))
+    case.check(case.run(), False, (layout, rows))
+
+
+@pytest.mark.parametrize("count,n,heads", [(150, 3, 16), (70, 16, 64), (65, 1, 16)])
+def test_more_sequences_than_lanes(cuda, count, n, heads):
+    rows = [(37 * i * i + 11 * i) % 190 for i in range(count)]
+    case = Case(cuda, "capacity", rows, n, heads=heads)
+    case.check(case.run(), False, (count, n, heads))
+
+
 def test_parents_outside_their_range_are_none(cuda):
     parents = [[5, -7, 0, 3, 2 ** 30, 1, 4], [-1, 0, 1, -2 ** 31, 3, 6, 5]]
     c = Case(cuda, "paged", [50, 90], 7, parents=parents)
