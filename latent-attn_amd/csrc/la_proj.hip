@@ -1002,6 +1002,178 @@ __global__ __launch_bounds__(kMPWaves * 64, 4) void merge_join_kernel(JoinProble
     }
 }
 
+// merge_join_kernel for a step over spans alone, where there is work for several
+// rounds of workgroups: share `first` of `shares` of a head's blocks of 16 query rows,
+// with W_UV in registers for all of them, the next block's slots (two rows a wave,
+// kMSSlots of each and the weights' inputs) on their way during one, and the sequences'
+// places those of the block after it: no load is waited for from a cold start. Of up to
+// four slots the weights are made in the lanes that loaded their inputs, by swaps in
+// groups of four. 16 trees of 16 tokens, 128 heads, 63 MB of slots: 35 us, merge_join_kernel
+// 65; 4 of 64 32 us and 58; 8 of 25, 32 heads, less than two rounds: 27 and 22.
+constexpr int kMSSlots = 4;
+template <int kCtrl>
+__device__ inline float quad_swap(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, 0xF, 0xF, true));
+}
+// Maximum and sum of a lane's group of four.
+__device__ inline float quad_max(float v) {
+  v = fmaxf(v, quad_swap<0xB1>(v));    // quad_perm 1 0 3 2
+  return fmaxf(v, quad_swap<0x4E>(v));  // quad_perm 2 3 0 1
+}
+__device__ inline float quad_sum(float v) {
+  v += quad_swap<0xB1>(v);
+  return v + quad_swap<0x4E>(v);
+}
+template <typename WT>
+__global__ __launch_bounds__(kMPWaves * 64, 2) void merge_spans_kernel(JoinProblem j, int shares) {
+  const DecodeProblem& p = j.step[0];
+  typedef Mma16<WT> M;
+  typedef typename M::vec vec;
+  constexpr float kLoScale = Mma<WT>::kLoScale;
+  __shared__ __attribute__((aligned(16))) short oh[2][kMPRows * kMPOPitch];  // merged O rows, high parts
+  __shared__ __attribute__((aligned(16))) short ol[2][kMPRows * kMPOPitch];  // and residuals
+  const int R = p.num_seqs * p.qps, blocks = (R + kMPRows - 1) / kMPRows;
+  const int x = blockIdx.x & 7, k = blockIdx.x >> 3, h = k / shares * 8 + x, first = k % shares;
+  if (h >= p.nh || first >= blocks) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int32_t* const tiles = span_tiles(p);
+  const uint32_t len = (uint32_t)tiles[p.num_seqs + 1];
+  const int64_t stride = (int64_t)p.Hq * kDcP;
+
+  struct Place {  // of a query row: its sequence's tiles, and its length, which is within the region (as loaded: nothing waits here)
+    int s, begin, end, rows;
+  };
+  struct Slots {
+    int n;
+    int64_t row0;
+    SlotRow<true> d[kMSSlots];
+    float lse, m, a, b;
+  };
+  auto place = [&](int block, int q) {
+    const int t = block * kMPRows + wave + kMPWaves * q;
+    Place y{t < R ? t / p.qps : -1, 0, 0, 0};
+    if (y.s >= 0) y.begin = tiles[y.s], y.end = tiles[y.s + 1], y.rows = p.lens[y.s];
+    return y;
+  };
+  const _Float16* const part = reinterpret_cast<const _Float16*>(p.part_o) + 8 * lane;
+  auto load = [&](const Place& y, int block, int q) {
+    Slots z;
+    z.n = 0;
+    z.row0 = 0;
+    const int s = __builtin_amdgcn_readfirstlane(y.s), begin = __builtin_amdgcn_readfirstlane(y.begin);
+    const int end = __builtin_amdgcn_readfirstlane(min(y.end, y.begin + (int)(((uint32_t)y.rows + kSpanRows - 1) / kSpanRows)));
+    if (s >= 0 && end > begin) {
+      const int c = (int)((uint32_t)begin / len), t = block * kMPRows + wave + kMPWaves * q;
+      z.n = (int)((uint32_t)(end - 1) / len) - c + 1;
+      z.row0 = (int64_t)(c + s) * p.Hq + (int64_t)(t - s * p.qps) * p.nh + h;
+    }
+#pragma unroll
+    for (int u = 0; u < kMSSlots; ++u)
+      if (u < z.n) z.d[u].load(part + z.row0 * kDcP + u * stride);
+    const bool own = lane < z.n;
+    const int64_t at = z.row0 + (own ? (int64_t)lane * p.Hq : 0);
+    z.lse = own ? p.part_lse[at] : -INFINITY;
+    z.m = own ? p.part_m[at] : -INFINITY;
+    z.a = own ? p.part_scale[2 * at] : 0.f;
+    z.b = own ? p.part_scale[2 * at + 1] : 0.f;
+    return z;
+  };
+  auto lane_of = [](float v, int u) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), u));
+  };
+  // more slots than are on their way: from memory, in rounds of 64
+  auto merge_many = [&](const Slots& z, f32x4 (&o)[2]) {
+    float mx = -INFINITY, den = 0.f;
+    for (int i = lane; i < z.n; i += 64) mx = fmaxf(mx, p.part_lse[z.row0 + (int64_t)i * p.Hq]);
+    mx = wave_max(mx);
+    for (int i = lane; i < z.n; i += 64) den += exp2f(p.part_lse[z.row0 + (int64_t)i * p.Hq] - mx);
+    const float inv = 1.f / wave_sum(den);
+    for (int i0 = 0; i0 < z.n; i0 += 64) {
+      const bool own = i0 + lane < z.n;
+      const int64_t at = z.row0 + (own ? (int64_t)(i0 + lane) * p.Hq : 0);
+      const float e = own ? exp2f(p.part_m[at] - mx) * inv : 0.f, lo = e * p.part_scale[2 * at], hi = e * p.part_scale[2 * at + 1];
+      for (int u = 0; u < min(z.n - i0, 64); ++u) {
+        SlotRow<true> d;
+        d.load(part + z.row0 * kDcP + (i0 + u) * stride);
+        d.fma(lane < 32 ? lane_of(lo, u) : lane_of(hi, u), o[0], o[1]);
+      }
+    }
+  };
+  auto merge = [&](const Slots& z, f32x4 (&o)[2]) {
+    o[0] = o[1] = f32x4{};
+    if (z.n == 0) return;
+    if (z.n > kMSSlots) return merge_many(z, o);
+    // lanes 0 to 3 have the slots' values
+    const float mx = quad_max(z.lse), e = exp2f(z.m - mx) / quad_sum(lane < z.n ? exp2f(z.lse - mx) : 0.f);
+    const float lo = e * z.a, hi = e * z.b;
+#pragma unroll
+    for (int u = 0; u < kMSSlots; ++u)
+      if (u < z.n) {
+        const float w0 = lane_of(lo, u), w1 = lane_of(hi, u);
+        z.d[u].fma(lane < 32 ? w0 : w1, o[0], o[1]);
+      }
+  };
+  auto put8 = [&](int at, const f32x4 (&o)[2], short* high, short* low) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = o[0][e], v[4 + e] = o[1][e];
+    vec hi, lo;
+    split8<WT>(v, hi, lo);
+    *reinterpret_cast<vec*>(&high[at]) = hi;
+    *reinterpret_cast<vec*>(&low[at]) = lo;
+  };
+
+  Place pa = place(first, 0), pb = place(first, 1);
+  Slots za = load(pa, first, 0), zb = load(pb, first, 1);
+  pa = place(first + shares, 0), pb = place(first + shares, 1);
+  // W_UV operands: A[m = lane % 16][k = 32 ks + 8 (lane / 16) + j]
+  const WT* const wrow = reinterpret_cast<const WT*>(p.W_UV) + ((int64_t)h * p.dv + 16 * wave + (lane & 15)) * kDcP +
+                         8 * (lane >> 4);
+  vec bw[16];
+#pragma unroll
+  for (int ks = 0; ks < 16; ++ks) bw[ks] = __builtin_bit_cast(vec, *reinterpret_cast<const i16x8*>(wrow + 32 * ks));
+#pragma unroll
+  for (int ks = 0; ks < 16; ++ks) asm volatile("" : "+v"(bw[ks]));  // here: no wait for them is left in the loop
+  int buf = 0;
+  for (int block = first; block < blocks; block += shares, buf ^= 1) {
+    const Slots ya = za, yb = zb;
+    za = load(pa, block + shares, 0), zb = load(pb, block + shares, 1);
+    pa = place(block + 2 * shares, 0), pb = place(block + 2 * shares, 1);
+    f32x4 o[2];
+    merge(ya, o);
+    put8(wave * kMPOPitch + 8 * lane, o, oh[buf], ol[buf]);
+    merge(yb, o);
+    put8((wave + kMPWaves) * kMPOPitch + 8 * lane, o, oh[buf], ol[buf]);
+    lds_barrier();  // the loads stay on their way; the other buffer's readers are past the barrier before
+    // W_UV's rows as A, O[n = lane % 16][k = 32 ks + 8 (lane / 16) + j] (high, low) as B
+    f32x4 acc_hi = {}, acc_lo = {};
+    const int a0 = (lane & 15) * kMPOPitch + 8 * (lane >> 4);
+    constexpr int kAhead = 5;
+    vec hi[kAhead], lo[kAhead];
+#pragma unroll
+    for (int ks = 0; ks < 16 + kAhead; ++ks) {
+      if (ks >= kAhead) {
+        acc_hi = M::mma(bw[ks - kAhead], hi[ks % kAhead], acc_hi);
+        acc_lo = M::mma(bw[ks - kAhead], lo[ks % kAhead], acc_lo);
+      }
+      if (ks < 16) {
+        hi[ks % kAhead] = *reinterpret_cast<const vec*>(&oh[buf][a0 + 32 * ks]);
+        lo[ks % kAhead] = *reinterpret_cast<const vec*>(&ol[buf][a0 + 32 * ks]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // D[column 4 (lane / 16) + i][row lane % 16]: four columns of a row
+    const int r = block * kMPRows + (lane & 15);
+    if (r >= R) continue;
+    const int64_t at = ((int64_t)r * p.nh + h) * p.dv + 16 * wave + 4 * (lane >> 4);
+    const f32x4 v = acc_hi + acc_lo * (1.f / kLoScale);
+    typedef __bf16 b16x4 __attribute__((ext_vector_type(4)));
+    if (j.out_dtype == LA_DTYPE_F32) *reinterpret_cast<f32x4*>(static_cast<float*>(j.out) + at) = v;
+    else if (j.out_dtype == LA_DTYPE_BF16) *reinterpret_cast<b16x4*>(static_cast<__bf16*>(j.out) + at) = __builtin_convertvector(v, b16x4);
+    else *reinterpret_cast<f16x4*>(static_cast<_Float16*>(j.out) + at) = __builtin_convertvector(v, f16x4);
+  }
+}
+
 // The same for float32 weights, all in fp32 (v_mfma_f32_16x16x4_f32): one
 // workgroup of 8 waves per (head h, 16 query rows), or, with kHalf and an
 // output zeroed earlier in the call, per latent half of it, the halves added
@@ -1267,6 +1439,14 @@ hipError_t launch_merge_join(const JoinProblem& j, hipStream_t stream, int ncu) 
   while (rpb_log2 > 0 && (int64_t)hb * ((R + (1 << rpb_log2) - 1) >> rpb_log2) < ncu) --rpb_log2;
   const int64_t blocks = (int64_t)hb * ((R + (1 << rpb_log2) - 1) >> rpb_log2);
   if (blocks > most_blocks(kMPWaves * 64)) return hipErrorInvalidValue;
+  // a round of merge_join_kernel's workgroups or more, and an output that takes four columns at once
+  if (p.chunk_len == kSpans && j.splits == 0 && j.step[1].num_seqs == 0 && blocks >= 2 * ncu &&
+      (reinterpret_cast<uintptr_t>(j.out) & 15) == 0) {
+    const int shares = std::max(ncu / hb, 1);
+    const auto k = p.wuv_dtype == LA_DTYPE_BF16 ? merge_spans_kernel<__hip_bfloat16> : merge_spans_kernel<__half>;
+    hipLaunchKernelGGL(k, dim3((unsigned)(hb * shares)), dim3(kMPWaves * 64), 0, stream, j, shares);
+    return hipGetLastError();
+  }
   if (p.wuv_dtype == LA_DTYPE_BF16)
     hipLaunchKernelGGL(merge_join_kernel<__hip_bfloat16>, dim3((unsigned)blocks), dim3(kMPWaves * 64), 0, stream, j, rpb_log2);
   else
