@@ -374,7 +374,7 @@ int run(const la_decode_args* a, hipStream_t stream, hipEvent_t ev_b = nullptr, 
       // q_prep in the MFMAs' 16-bit type: fp16 for an fp16 cache, bf16 otherwise
       if (tail && tail->queries)
         e = launch_absorb_any(*tail->queries, a->W_UK, a->w_uk_dtype, p.q_prep, p.kv_dtype == LA_DTYPE_F16 ? 2 : 1,
-                              p.scale_log2, c.num_heads, stream, zero_out, zero_n);
+                              p.scale_log2, c.num_heads, stream, cu_count(), zero_out, zero_n);
       else
         e = launch_absorb_mfma(a->q_nope, a->W_UK, a->w_uk_dtype, p.q_prep, p.kv_dtype == LA_DTYPE_F16 ? 2 : 1,
                                a->q_rope, p.scale_log2, c.qk_rope_head_dim, (int)tokens, c.num_heads,
@@ -1562,7 +1562,7 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
   hipError_t e = hipSuccess;
   if (direct) {
     const AbsorbQueries x{q, p.src, nullptr, p.low};
-    e = launch_absorb_any(x, a->W_UK, a->w_uk_dtype, q_prep, a->kv_dtype == LA_DTYPE_F16 ? 2 : 1, weigh_query_scale(p), nh, stream);
+    e = launch_absorb_any(x, a->W_UK, a->w_uk_dtype, q_prep, a->kv_dtype == LA_DTYPE_F16 ? 2 : 1, weigh_query_scale(p), nh, stream, cu_count());
   } else {
     t.q = q;
     t.src = p.src;

@@ -128,14 +128,12 @@ constexpr int kAbsThreads = 512;
 // the first wait, spread over the block's 8 waves.
 // NKS = dn / 16 when known at compile time (8 for dn = 128: no guards, every
 // load unconditional), 0 for any dn <= 128 that is a multiple of 16.
-// kAny: the queries are x's, of any type and strides and with q_rope not rotated
-// yet, and the rows' second parts may be wanted too (AbsorbQueries; modes 1, 2).
-template <typename WT, int NKS, bool kAny>
-__device__ __forceinline__ void absorb_body(const float* __restrict__ q_nope, const WT* __restrict__ W,
-                                            void* __restrict__ out, int out_mode,
-                                            const float* __restrict__ q_rope, float scale, int dR,
-                                            int tokens, int nh, int dn, int dc, int qps,
-                                            float* __restrict__ zero_out, int64_t zero_n, const AbsorbQueries& any) {
+template <typename WT, int NKS>
+__global__ __launch_bounds__(kAbsThreads) void absorb_mfma_kernel(const float* __restrict__ q_nope, const WT* __restrict__ W,
+                                                          void* __restrict__ out, int out_mode,
+                                                          const float* __restrict__ q_rope, float scale, int dR,
+                                                          int tokens, int nh, int dn, int dc, int qps,
+                                                          float* __restrict__ zero_out, int64_t zero_n) {
   typedef Mma<WT> M;
   typedef typename M::vec vec;
   LA_RSTAMP_DECL;
@@ -172,21 +170,14 @@ __device__ __forceinline__ void absorb_body(const float* __restrict__ q_nope, co
   // LDS for the MFMA waves (each wave issues 2 q loads, not 16)
   const int t = t0 + (lane & 31);
   const bool tvalid = t < tokens;
-  const float* qrow = kAny ? nullptr : q_nope + ((int64_t)(tvalid ? t : 0) * nh + h) * dn + 8 * (lane >> 5);
+  const float* qrow = q_nope + ((int64_t)(tvalid ? t : 0) * nh + h) * dn + 8 * (lane >> 5);
   // (with NKS > 0 every wave's k-step exists: the loads go out
   // unconditionally, since a load under a branch gets its result copied at
   // the branch's end, which waits for it before the W_UK loads below issue)
   static_assert(kAbsThreads / 64 == 8, "one q k-step per wave");
   const int ks_w = wave;
   f32x4 qa, qb;
-  if constexpr (kAny) {
-    const int64_t at = (tvalid ? t : 0) * any.q.nope_stride + h * any.q.nope_head + 16 * ks_w + 8 * (lane >> 5);
-    float x[4], y[4];
-    load_q4(any.q.q_nope, any.q.dtype, at, x);
-    load_q4(any.q.q_nope, any.q.dtype, at + 4, y);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) qa[e] = x[e], qb[e] = y[e];
-  } else if (NKS > 0 || ks_w < nks) {
+  if (NKS > 0 || ks_w < nks) {
     qa = *reinterpret_cast<const f32x4*>(qrow + 16 * ks_w);
     qb = *reinterpret_cast<const f32x4*>(qrow + 16 * ks_w + 4);
   }
@@ -210,12 +201,9 @@ __device__ __forceinline__ void absorb_body(const float* __restrict__ q_nope, co
   // branch's end, which would wait for every load before it.
   const int rt = tid & 255;
   const int rtr = min(t0 + (rt >> 3), tokens - 1);
-  f32x4 ra, rb;
-  if constexpr (!kAny) {
-    const float* rsrc = out_mode != 0 ? q_rope + ((int64_t)rtr * nh + h) * dR + 8 * (rt & 7) : q_nope;
-    ra = *reinterpret_cast<const f32x4*>(rsrc);
-    rb = *reinterpret_cast<const f32x4*>(rsrc + 4);
-  }
+  const float* rsrc = out_mode != 0 ? q_rope + ((int64_t)rtr * nh + h) * dR + 8 * (rt & 7) : q_nope;
+  const f32x4 ra = *reinterpret_cast<const f32x4*>(rsrc);
+  const f32x4 rb = *reinterpret_cast<const f32x4*>(rsrc + 4);
   LA_RSTAMP(1);
 #pragma unroll
   for (int k = 0; k < kWLoads; ++k) {
@@ -284,25 +272,11 @@ __device__ __forceinline__ void absorb_body(const float* __restrict__ q_nope, co
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r] = (__bf16)(v[r] * scale);
         *reinterpret_cast<bf16x4*>(reinterpret_cast<__bf16*>(out) + qprep_index(qrow, col)) = o;
-        if constexpr (kAny) {
-          if (any.low) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = (__bf16)(v[r] * scale - (float)o[r]);
-            *reinterpret_cast<bf16x4*>(reinterpret_cast<__bf16*>(out) + any.low + qprep_index(qrow, col)) = o;
-          }
-        }
       } else {
         f16x4 o;
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r] = (_Float16)(v[r] * scale);
         *reinterpret_cast<f16x4*>(reinterpret_cast<_Float16*>(out) + qprep_index(qrow, col)) = o;
-        if constexpr (kAny) {
-          if (any.low) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = (_Float16)(v[r] * scale - (float)o[r]);
-            *reinterpret_cast<f16x4*>(reinterpret_cast<_Float16*>(out) + any.low + qprep_index(qrow, col)) = o;
-          }
-        }
       }
     }
   }
@@ -310,26 +284,6 @@ __device__ __forceinline__ void absorb_body(const float* __restrict__ q_nope, co
     // the q_rope part of the same rows (loaded with the operands above): one
     // 16-B slot of q_prep per thread
     const int tr = t0 + (tid >> 3), j = 8 * (tid & 7);
-    if constexpr (kAny) {
-      // element j + e with its partner of the rotation, j + e + 32 or - 32
-      const int tc = min(tr, tokens - 1), i = j & 31, s = tc / qps;
-      const int64_t at = tc * any.q.rope_stride + h * any.q.rope_head;
-      const int64_t pos = any.pos ? any.pos[tc] : max(source_rows(any.src, s) - qps + tc % qps, 0);
-      float own[8], other[8];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        load_q4(any.q.q_rope, any.q.dtype, at + j + 4 * k, *reinterpret_cast<float(*)[4]>(own + 4 * k));
-        load_q4(any.q.q_rope, any.q.dtype, at + (j ^ 32) + 4 * k, *reinterpret_cast<float(*)[4]>(other + 4 * k));
-      }
-      const float sign = j < 32 ? -1.f : 1.f;
-      const f32x4 *const cs = reinterpret_cast<const f32x4*>(any.src.cos + source_rope_row(any.src, pos) * 32 + i),
-                  *const sn = reinterpret_cast<const f32x4*>(any.src.sin + source_rope_row(any.src, pos) * 32 + i);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        ra[e] = any.q.rotate ? own[e] * cs[0][e] + sign * other[e] * sn[0][e] : own[e];
-        rb[e] = any.q.rotate ? own[4 + e] * cs[1][e] + sign * other[4 + e] * sn[1][e] : own[4 + e];
-      }
-    }
     if (tr < tokens) {
       const int64_t qr = (int64_t)(tr / qps) * qprep_rows_per_seq(qps * nh) + (int64_t)(tr % qps) * nh + h;
       const int64_t dst = qprep_index(qr, dc + j);
@@ -341,13 +295,6 @@ __device__ __forceinline__ void absorb_body(const float* __restrict__ q_nope, co
           v[4 + e] = (__bf16)(rb[e] * scale);
         }
         *reinterpret_cast<bf16x8*>(reinterpret_cast<__bf16*>(out) + dst) = v;
-        if constexpr (kAny) {
-          if (any.low) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = (__bf16)((e < 4 ? ra : rb)[e & 3] * scale - (float)v[e]);
-            *reinterpret_cast<bf16x8*>(reinterpret_cast<__bf16*>(out) + any.low + dst) = v;
-          }
-        }
       } else {
         f16x8 v;
 #pragma unroll
@@ -356,33 +303,199 @@ __device__ __forceinline__ void absorb_body(const float* __restrict__ q_nope, co
           v[4 + e] = (_Float16)(rb[e] * scale);
         }
         *reinterpret_cast<f16x8*>(reinterpret_cast<_Float16*>(out) + dst) = v;
-        if constexpr (kAny) {
-          if (any.low) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = (_Float16)((e < 4 ? ra : rb)[e & 3] * scale - (float)v[e]);
-            *reinterpret_cast<f16x8*>(reinterpret_cast<_Float16*>(out) + any.low + dst) = v;
-          }
-        }
       }
     }
   }
   LA_RSTAMP_WRITE(0);
 }
-template <typename WT, int NKS>
-__global__ __launch_bounds__(kAbsThreads) void absorb_mfma_kernel(const float* __restrict__ q_nope, const WT* __restrict__ W,
-                                                          void* __restrict__ out, int out_mode,
-                                                          const float* __restrict__ q_rope, float scale, int dR,
-                                                          int tokens, int nh, int dn, int dc, int qps,
-                                                          float* __restrict__ zero_out, int64_t zero_n) {
-  absorb_body<WT, NKS, false>(q_nope, W, out, out_mode, q_rope, scale, dR, tokens, nh, dn, dc, qps, zero_out, zero_n,
-                              AbsorbQueries{});
+
+// Absorption straight from queries of any type and strides (AbsorbQueries), rotated on the
+// way: q_prep rows (hi, and lo if asked) of a head's 128 latent columns. A workgroup of
+// 8 waves has W_UK's tile once, as operands in registers (wave: 32 columns), and goes
+// through share `share` of `shares` of the tokens, 64 at a time (wave: 32 of them), the
+// next ones' loads on their way during the products. The queries' split operands go through
+// LDS; the rope part (one 16-byte slot per thread) is the workgroups' of columns 0.
+// Of two runs of 8 columns, lanes 0 to 31 take the first's second half from the lanes
+// 32 on, which take the second's first half: whole 16-byte slots go out.
+constexpr int kAnyTokens = 64;
+// A barrier for __shared__ arrays that leaves global loads on their way (a memory clobber
+// alone does not cover arrays whose address no one else has).
+__device__ inline void shared_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
-template <typename WT>
-__global__ __launch_bounds__(kAbsThreads) void absorb_any_kernel(AbsorbQueries any, const WT* __restrict__ W,
-                                                                 void* __restrict__ out, int out_mode, float scale,
-                                                                 int tokens, int nh, int qps, float* __restrict__ zero_out,
-                                                                 int64_t zero_n) {
-  absorb_body<WT, 8, true>(nullptr, W, out, out_mode, nullptr, scale, 64, tokens, nh, 128, 512, qps, zero_out, zero_n, any);
+// Eight elements as loaded (in two halves: 16-bit ones are aligned to four), and as values.
+template <typename QT>
+struct Eight {
+  typedef QT half __attribute__((ext_vector_type(4)));
+  half v[2];
+  __device__ void load(const QT* from) {
+    v[0] = *reinterpret_cast<const half*>(from);
+    v[1] = *reinterpret_cast<const half*>(from + 4);
+  }
+  __device__ float at(int e) const { return (float)v[e >> 2][e & 3]; }
+};
+template <typename WT, typename QT>
+__global__ __launch_bounds__(kAbsThreads, 4) void absorb_any_kernel(AbsorbQueries any, const WT* __restrict__ W,
+                                                                    void* __restrict__ out, int out_mode, float scale,
+                                                                    int tokens, int nh, int qps, int shares,
+                                                                    float* __restrict__ zero_out, int64_t zero_n) {
+  typedef Mma<WT> M;
+  typedef typename M::vec vec;
+  __shared__ __attribute__((aligned(16))) char wt[128 * kAbsRowBytes];
+  __shared__ __attribute__((aligned(16))) char qs[2 * 8 * 2 * 64 * 16];  // [token half][k-step][hi|lo][lane] 16 B
+  // (share, 8 heads) groups of 32 workgroups on one XCD each: a 128-B line of q_prep has
+  // 8 heads' slots, and the column blocks of a head read the same queries
+  constexpr int ncb = 512 / kAbsCols, gb = 8 * ncb;
+  const int nh8 = (nh + 7) / 8;
+  const int x = blockIdx.x & 7, k = blockIdx.x >> 3, grp = x + 8 * (k / gb), j = k % gb;
+  const int share = grp / nh8, h = 8 * (grp - share * nh8) + (j & 7), cb = j >> 3;
+  if (zero_out)
+    for (int64_t i = (int64_t)blockIdx.x * kAbsThreads + threadIdx.x; i < zero_n; i += (int64_t)gridDim.x * kAbsThreads)
+      zero_out[i] = 0.f;
+  if (share >= shares || h >= nh) return;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+
+  // queries of tokens t0 + 32 i + lane % 32, elements 16 wave + 8 (lane / 32) .. + 8
+  const QT *const nope = static_cast<const QT*>(any.q.q_nope) + h * any.q.nope_head + 16 * wave + 8 * (lane >> 5),
+           *const rope = static_cast<const QT*>(any.q.q_rope) + h * any.q.rope_head;
+  Eight<QT> q[2];
+  auto load_q = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      q[i].load(nope + min(t0 + 32 * i + (lane & 31), tokens - 1) * any.q.nope_stride);
+    }
+  };
+  auto put_q = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = q[i].at(e);
+      vec hi, lo;
+      split8<WT>(v, hi, lo);
+      *reinterpret_cast<vec*>(qs + 16384 * i + 2 * wave * 1024 + 16 * lane) = hi;
+      *reinterpret_cast<vec*>(qs + 16384 * i + (2 * wave + 1) * 1024 + 16 * lane) = lo;
+    }
+  };
+  int t0 = kAnyTokens * share;
+  load_q(t0);
+  constexpr int kWLoads = 128 * 16 / kAbsThreads;
+  i16x8 wv[kWLoads];
+#pragma unroll
+  for (int i = 0; i < kWLoads; ++i) {
+    const int e = tid + kAbsThreads * i;
+    wv[i] = *reinterpret_cast<const i16x8*>(W + ((int64_t)h * 128 + (e >> 4)) * 512 + cb * kAbsCols + (e & 15) * 8);
+  }
+  // the rope part of a token: elements 8 (tid % 8) .. + 8 and their partners in the rotation
+  const int rj = 8 * (tid & 7);
+  Eight<QT> own, other;
+  int32_t pos = 0;
+  auto load_rope = [&](int t0) {
+    const int tc = min(t0 + (tid >> 3), tokens - 1), s = tc / qps;
+    const QT* const from = rope + tc * any.q.rope_stride;
+    pos = any.pos ? any.pos[tc] : max(source_rows(any.src, s) - qps + tc % qps, 0);
+    own.load(from + rj);
+    other.load(from + (rj ^ 32));
+  };
+  if (cb == 0) load_rope(t0);
+#pragma unroll
+  for (int i = 0; i < kWLoads; ++i) {
+    const int e = tid + kAbsThreads * i;
+    *reinterpret_cast<i16x8*>(wt + (e >> 4) * kAbsRowBytes + (e & 15) * 16) = wv[i];
+  }
+  __syncthreads();
+  // W[i][c] as A[m = c][k = i]: rows 16 ks + 8 (g / 2) + 4 hf + s / 4, columns 32 (wave % 4) + 16 (g % 2) + 4 (s % 4)
+  const int g = lane >> 4, s = lane & 15;
+  vec w[8];
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) {
+    i16x8 v;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int row = 16 * ks + 8 * (g >> 1) + 4 * hf + (s >> 2), col = 32 * (wave & 3) + 16 * (g & 1) + 4 * (s & 3);
+      const i16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) i16x4*)(lds_void*)(wt + row * kAbsRowBytes + col * 2));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * hf + e] = r[e];
+    }
+    w[ks] = __builtin_bit_cast(vec, v);
+  }
+  auto slot = [&](auto elem, const float (&v)[8], int64_t at) {
+    typedef decltype(elem) E;
+    typedef E e8 __attribute__((ext_vector_type(8)));
+    e8 o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = (E)v[e];
+    *reinterpret_cast<e8*>(reinterpret_cast<E*>(out) + at) = o;
+    if (any.low) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = (E)(v[e] - (float)o[e]);
+      *reinterpret_cast<e8*>(reinterpret_cast<E*>(out) + any.low + at) = o;
+    }
+  };
+  auto row_of = [&](int t) { return (int64_t)(t / qps) * qprep_rows_per_seq(qps * nh) + (int64_t)(t % qps) * nh + h; };
+  for (; t0 < tokens; t0 += kAnyTokens * shares) {
+    put_q(t0);
+    shared_barrier();
+    const int next = t0 + kAnyTokens * shares;
+    if (next < tokens) load_q(next);
+    const char* const mine = qs + 16384 * (wave >> 2) + 16 * lane;
+    f32x16 acc_hi = {}, acc_lo = {};
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+      acc_hi = M::mma(w[ks], *reinterpret_cast<const vec*>(mine + 2 * ks * 1024), acc_hi);
+      acc_lo = M::mma(w[ks], *reinterpret_cast<const vec*>(mine + (2 * ks + 1) * 1024), acc_lo);
+    }
+    // register 4 q + r: column 32 (wave % 4) + 8 q + 4 (lane / 32) + r of token lane % 32
+    const int tt = t0 + 32 * (wave >> 2) + (lane & 31);
+    const int64_t to = row_of(tt);
+#pragma unroll
+    for (int q2 = 0; q2 < 4; q2 += 2) {
+      float v[8];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float a = (acc_hi[4 * q2 + r] + acc_lo[4 * q2 + r] * (1.f / M::kLoScale)) * scale;
+        const float b = (acc_hi[4 * q2 + 4 + r] + acc_lo[4 * q2 + 4 + r] * (1.f / M::kLoScale)) * scale;
+        const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
+        v[r] = f_of(both[0]), v[4 + r] = f_of(both[1]);
+      }
+      const int64_t at = qprep_index(to, cb * kAbsCols + 32 * (wave & 3) + 8 * q2 + 8 * (lane >> 5));
+      if (tt < tokens) {
+        if (out_mode == 1) slot(__bf16(), v, at);
+        else slot(_Float16(), v, at);
+      }
+    }
+    if (cb == 0) {
+      const int tr = t0 + (tid >> 3);
+      f32x4 cs[2], sn[2];
+      if (any.q.rotate) {
+        const int64_t at = source_rope_row(any.src, pos) * 32 + (rj & 31);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          cs[i] = *reinterpret_cast<const f32x4*>(any.src.cos + at + 4 * i);
+          sn[i] = *reinterpret_cast<const f32x4*>(any.src.sin + at + 4 * i);
+        }
+      }
+      const float sign = rj < 32 ? -1.f : 1.f;
+      float v[8];
+      if (any.q.rotate) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (own.at(e) * cs[e >> 2][e & 3] + sign * other.at(e) * sn[e >> 2][e & 3]) * scale;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = own.at(e) * scale;
+      }
+      if (tr < tokens) {
+        const int64_t at = qprep_index(row_of(tr), 512 + rj);
+        if (out_mode == 1) slot(__bf16(), v, at);
+        else slot(_Float16(), v, at);
+      }
+      if (next < tokens) load_rope(next);
+    }
+    shared_barrier();  // the operands have been read
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1144,7 +1257,7 @@ __global__ __launch_bounds__(kMPWaves * 64, 2) void merge_spans_kernel(JoinProbl
     put8(wave * kMPOPitch + 8 * lane, o, oh[buf], ol[buf]);
     merge(yb, o);
     put8((wave + kMPWaves) * kMPOPitch + 8 * lane, o, oh[buf], ol[buf]);
-    lds_barrier();  // the loads stay on their way; the other buffer's readers are past the barrier before
+    shared_barrier();  // the loads stay on their way; the other buffer's readers are past the barrier before
     // W_UV's rows as A, O[n = lane % 16][k = 32 ks + 8 (lane / 16) + j] (high, low) as B
     f32x4 acc_hi = {}, acc_lo = {};
     const int a0 = (lane & 15) * kMPOPitch + 8 * (lane >> 4);
@@ -1317,16 +1430,23 @@ bool absorb_any_supported(const QuerySource& q, const RowSource& r, const void* 
 }
 
 hipError_t launch_absorb_any(const AbsorbQueries& x, const void* W_UK, int w_dtype, void* out, int out_mode, float scale,
-                             int nh, hipStream_t stream, float* zero_out, int64_t zero_n) {
-  const int tokens = (int)x.q.tokens;
-  const int64_t groups = (int64_t)((tokens + 31) / 32) * ((nh + 7) / 8);
-  const dim3 grid((unsigned)(64 * 4 * ((groups + 7) / 8)));
-  if (w_dtype == LA_DTYPE_BF16)
-    hipLaunchKernelGGL(absorb_any_kernel<__hip_bfloat16>, grid, dim3(kAbsThreads), 0, stream, x,
-                       static_cast<const __hip_bfloat16*>(W_UK), out, out_mode, scale, tokens, nh, x.q.per_seq, zero_out, zero_n);
-  else
-    hipLaunchKernelGGL(absorb_any_kernel<__half>, grid, dim3(kAbsThreads), 0, stream, x, static_cast<const __half*>(W_UK), out,
-                       out_mode, scale, tokens, nh, x.q.per_seq, zero_out, zero_n);
+                             int nh, hipStream_t stream, int ncu, float* zero_out, int64_t zero_n) {
+  const int tokens = (int)x.q.tokens, blocks = (tokens + kAnyTokens - 1) / kAnyTokens, nh8 = (nh + 7) / 8;
+  // two workgroups per CU
+  const int shares = std::max(1, std::min(blocks, 2 * ncu / (8 * nh8 * 512 / kAbsCols)));
+  const dim3 grid((unsigned)(64 * (512 / kAbsCols) * ((shares * nh8 + 7) / 8)));
+  auto launch = [&](auto w, auto qt) {
+    typedef decltype(w) WT;
+    hipLaunchKernelGGL((absorb_any_kernel<WT, decltype(qt)>), grid, dim3(kAbsThreads), 0, stream, x, static_cast<const WT*>(W_UK),
+                       out, out_mode, scale, tokens, nh, x.q.per_seq, shares, zero_out, zero_n);
+  };
+  auto by_query = [&](auto w) {
+    if (x.q.dtype == LA_DTYPE_F32) launch(w, float());
+    else if (x.q.dtype == LA_DTYPE_BF16) launch(w, __bf16());
+    else launch(w, _Float16());
+  };
+  if (w_dtype == LA_DTYPE_BF16) by_query(__hip_bfloat16());
+  else by_query(__half());
   return hipGetLastError();
 }
 

@@ -324,7 +324,7 @@ struct AbsorbQueries {
 bool absorb_any_supported(const QuerySource& q, const RowSource& r, const void* W_UK, int w_dtype, const la_mla_config& c);
 // out_mode 1: bf16, 2: fp16; zero_out as for launch_absorb_mfma.
 hipError_t launch_absorb_any(const AbsorbQueries& x, const void* W_UK, int w_dtype, void* out, int out_mode, float scale,
-                             int nh, hipStream_t stream, float* zero_out = nullptr, int64_t zero_n = 0);
+                             int nh, hipStream_t stream, int ncu, float* zero_out = nullptr, int64_t zero_n = 0);
 // fp32 -> out_dtype
 hipError_t launch_cast(const float* src, void* dst, int out_dtype, int64_t n, hipStream_t stream);
 
