@@ -232,9 +232,14 @@ int prepare(const la_decode_args* a, DecodeProblem* p, Plan* plan, bool coarse =
   if ((pl.mfma || pl.f32) && L > kMaxChunkRows) L = kMaxChunkRows;
   if (paged && (pl.mfma || pl.f32)) L = (L + 63) / 64 * 64;  // MFMA tiles start block-aligned
   int64_t nchunks = total > 0 ? (total + L - 1) / L : 0;
-  if (tree && total > 0) {  // spans, their length found on the device: as many as there is room for
+  if (tree && pl.mfma && total > 0) {  // spans, their length found on the device: as many as there is room for
     const int64_t rows = total + (int64_t)a->num_seqs * (kSpanRows - 1), groups = (p->Hq + mfma_heads_per_group() - 1) / mfma_heads_per_group();
-    nchunks = std::max(std::min(std::max<int64_t>(ncu / groups, 1), (rows + min_rows - 1) / min_rows),
+    // 16 heads per workgroup while that leaves each two tiles of 128 rows at most
+    if (rows * (p->Hq / 16) <= 256LL * ncu) {
+      pl.waves16 = 8;
+      min_rows = 128;
+    }
+    nchunks = std::max(std::min(std::max<int64_t>(ncu / (pl.waves16 ? p->Hq / 16 : groups), 1), (rows + min_rows - 1) / min_rows),
                        (rows + kMaxChunkRows - 1) / kMaxChunkRows);
   }
   if (nchunks > (int64_t)1 << 30) return LA_ERROR_INVALID_VALUE;
@@ -294,7 +299,7 @@ int prepare(const la_decode_args* a, DecodeProblem* p, Plan* plan, bool coarse =
   // the device (32 of 100 to 500 rows in 512-row regions, 128 heads: 36.4 against
   // 35.5, fp8 38.5 against 37.1).
   if (filled) p->chunk_len = -piece;
-  if (tree) p->chunk_len = kSpans, pl.shortest = (int)((min_rows + kSpanRows - 1) / kSpanRows);
+  if (tree && pl.mfma) p->chunk_len = kSpans, pl.shortest = (int)((min_rows + kSpanRows - 1) / kSpanRows);
   p->num_chunks = pl.num_chunks;
   p->num_slots = pl.num_slots;
   *plan = pl;
@@ -398,7 +403,7 @@ int run(const la_decode_args* a, hipStream_t stream, hipEvent_t ev_b = nullptr, 
   p.part_scale = plan.mfma ? reinterpret_cast<float*>(ws + plan.part_scale_off) : nullptr;
   p.part_m = plan.mfma ? p.part_scale + (size_t)plan.num_slots * p.Hq * 2 : nullptr;
   if (plan.num_chunks > 0) {
-    if (plan.waves16 == 8 && !plan.absorb_prep) {
+    if (plan.waves16 == 8 && !plan.absorb_prep && !tree) {
       p.q_prep = nullptr;  // decode_mfma16_kernel takes the fp32 queries and zeroes the output
     } else if (plan.mfma && !plan.absorb_prep) {
       hipError_t e = launch_prep_q(p, stream, zero_out, zero_n);
@@ -408,7 +413,8 @@ int run(const la_decode_args* a, hipStream_t stream, hipEvent_t ev_b = nullptr, 
     hipError_t e = hipSuccess;
     const int reps = repeat > 1 ? repeat : 1;
     auto launch_mfma = [&](hipEvent_t b, hipEvent_t en) {
-      if (tree) return launch_decode_mfma_tree(p, tail->tree, stream);
+      if (tree)
+        return plan.waves16 ? launch_decode_mfma16_tree(p, tail->tree, stream) : launch_decode_mfma_tree(p, tail->tree, stream);
       return plan.waves16 ? launch_decode_mfma16(p, plan.waves16, stream, p.q_prep ? nullptr : zero_out, zero_n, b, en)
                           : launch_decode_mfma(p, stream, b, en);
     };
@@ -1399,6 +1405,7 @@ int decode_tree(const la_tree_args* a, void* stream_v, bool run_it, size_t* need
   t.vec = queries_vec(t.q);
   t.chunks = mfma ? plan.num_chunks : 0;
   t.shortest = plan.shortest;
+  t.step = plan.waves16 ? 128 / kSpanRows : 1;
   hipError_t e = launch_tree_queries(t, stream);
   if (e != hipSuccess) return scratch.finish(record_hip(e));
   const float* const qn = nope_as_is ? static_cast<const float*>(a->q_nope) : t.q_nope;

@@ -20,6 +20,7 @@ struct TreeQueries {
   float* q_rope;   // (tokens, nh, dR), or nullptr
   int32_t* lens;   // (num_seqs): rows, 0 where they are fewer than the nodes; with chunks, the plan of the spans behind them (num_seqs + 2)
   int chunks, shortest;  // of spans, and the fewest tiles of one (DecodeProblem); 0: none
+  int step;              // tiles that the attention kernel takes at a time: a span has whole ones
   uint64_t* seen;  // TreeStep
   float* cos;
   float* sin;

@@ -647,6 +647,8 @@ hipError_t launch_decode_mfma(const DecodeProblem& p, hipStream_t stream, hipEve
                               hipEvent_t ev_end = nullptr);
 hipError_t launch_decode_mfma_tree(const DecodeProblem& p, const TreeStep& tree, hipStream_t stream);
 bool mfma_supported(const DecodeProblem& p);
+// and with 16 query heads and 8 waves per workgroup
+hipError_t launch_decode_mfma16_tree(const DecodeProblem& p, const TreeStep& tree, hipStream_t stream);
 // The same with 16 query heads per workgroup (la_mfma16.hip); waves = 4 or 8
 // per workgroup (tiles of 64 or 128 positions).
 // With 8 waves and no q_prep it takes the fp32 queries; zero_out (optional): zero_n floats

@@ -43,9 +43,12 @@
 
 #include <hip/hip_ext.h>
 
+#include <type_traits>
+
 namespace la {
 namespace {
 
+constexpr float kNoScore = -1e30f;  // trees: a head may see no row of a tile
 constexpr int kDc = 512;
 constexpr int kDr = 64;
 constexpr int kRowElems = kDc + kDr;
@@ -151,9 +154,11 @@ __device__ inline float sum_groups(float x) {
 // slower than with the launch.) kW = 4 has no room for it (its k_rope and P rows
 // are smaller than the queries). zero_out (optional): zero_n floats zeroed for
 // a half-row merge.
-template <typename KT, int kW, bool kPaged, bool kFp8, bool kFilled>
-__global__ __launch_bounds__(64 * kW, 2) void decode_mfma16_kernel(DecodeProblem p, int groups, float* zero_out,
-                                                                  int zero_n) {
+// kFilled: ChunkWalk's. kTree: the sequences' last p.qps rows are the nodes of a tree,
+// as in decode_mfma_kernel's form for it.
+template <typename KT, int kW, bool kPaged, bool kFp8, int kFilled, bool kTree = false>
+__device__ __forceinline__ void decode16_body(const DecodeProblem& p, int groups, float* zero_out, int zero_n,
+                                              const TreeStep& tree = TreeStep{}) {
   typedef Ops16<KT> O_;
   typedef typename O_::vec vec;
   typedef typename O_::elem E;
@@ -182,13 +187,20 @@ __global__ __launch_bounds__(64 * kW, 2) void decode_mfma16_kernel(DecodeProblem
   ChunkWalk<kFilled> w;
   if (!walk_begin(p, chunk, group, w)) return;
 
-  while (walk_next(p, w)) {
+  while (walk_next(p, w, chunk)) {
     const int s = w.s;
     const char* const seg_base = reinterpret_cast<const char*>(p.kv) + (kPaged ? 0 : (w.row0 + (w.lo - w.s_lo)) * kRowB);
     const uint32_t pos0 = (uint32_t)(w.lo - w.s_lo);
     const int last = (int)(w.seg_hi - w.lo - 1);
     const int ntiles = last / kT + 1;
     const int rlim = p.rope_rows > 0 ? (int)(p.rope_rows - 1) : INT32_MAX;
+    // the segment's row of node 0 (or less: the rows before it), and the nodes that the lane's head sees
+    int node0 = 0;
+    uint64_t seen = 0;
+    if constexpr (kTree) {
+      node0 = p.lens[s] - p.qps - (int)pos0;
+      seen = tree.seen[(int64_t)s * p.qps + (uint32_t)(head0 + (wave_lane() & 15)) / (uint32_t)p.nh];
+    }
 
     // Q^T as the B operand: lane holds Q[head0 + n16][32kk + 8g .. +8], from
     // q_prep (in operand order, qprep_index), or from the fp32 queries' slots
@@ -218,7 +230,7 @@ __global__ __launch_bounds__(64 * kW, 2) void decode_mfma16_kernel(DecodeProblem
       }
     }
     f32x4 o[kCB];
-    float m = -INFINITY, l = 0.f;
+    float m = kTree ? kNoScore : -INFINITY, l = 0.f;
 #pragma unroll
     for (int cb = 0; cb < kCB; ++cb) o[cb] = f32x4{0.f, 0.f, 0.f, 0.f};
 
@@ -246,6 +258,13 @@ __global__ __launch_bounds__(64 * kW, 2) void decode_mfma16_kernel(DecodeProblem
       const char* ksrc = base + rrow * kRowB + (kFp8 ? kDc : 2 * kDc);
       const f32x4* cs = reinterpret_cast<const f32x4*>(p.rope_cos + (int64_t)rpos * (kDr / 2) + 8 * u);
       const f32x4* sn = reinterpret_cast<const f32x4*>(p.rope_sin + (int64_t)rpos * (kDr / 2) + 8 * u);
+      if constexpr (kTree) {
+        const int node = pb + rrow - node0;
+        if (node >= 0) {
+          cs = reinterpret_cast<const f32x4*>(tree.cos + ((int64_t)s * p.qps + node) * (kDr / 2) + 8 * u);
+          sn = reinterpret_cast<const f32x4*>(tree.sin + ((int64_t)s * p.qps + node) * (kDr / 2) + 8 * u);
+        }
+      }
       i16x8 ka, kb;
       u32x2 k8a, k8b;
       if constexpr (kFp8) {
@@ -328,6 +347,28 @@ __global__ __launch_bounds__(64 * kW, 2) void decode_mfma16_kernel(DecodeProblem
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       const int n16 = ln & 15, g = ln >> 4;
       const int row_l = 16 * wave + n16;
+      // the wave's rows of nodes that are not numbers: zeros (hidden ones weigh nothing, and zero times an
+      // infinity is NaN), and NaN scores where they are seen
+      uint32_t bad = 0;
+      const bool nodes = kTree && kT * (t + 1) > node0;
+      if constexpr (kTree) {
+        if (kT * t + 16 * wave + 16 > node0) {
+          constexpr uint32_t kExp = std::is_same<KT, __half>::value ? 0x7C007C00u : 0x7F807F80u;
+          constexpr uint32_t kOne = std::is_same<KT, __half>::value ? 0x04000400u : 0x00800080u;
+#pragma unroll 4
+          for (int j = 0; j < 16; ++j) {
+            const int at = (16 * wave + j) * kCtPitch + 16 * ln;
+            const u32x4 x = lds_ld<u32x4>(L, at);
+            uint32_t hit = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hit |= (x[e] & kExp) + kOne;  // (an exponent of ones carries)
+            if (__builtin_amdgcn_ballot_w64((hit & 0x80008000u) != 0) != 0) {
+              bad |= 1u << j;
+              lds_st(L, at, u32x4{0, 0, 0, 0});
+            }
+          }
+        }
+      }
       const int ct0 = row_l * kCtPitch + 16 * (g ^ cf(n16));  // k-step 0; 64 (kk % 4) is an exclusive or
       f32x4 sc = {0.f, 0.f, 0.f, 0.f};
       // operands kAhead k-steps ahead (the scheduling barriers keep the compiler from reading all 18 at once)
@@ -351,6 +392,14 @@ __global__ __launch_bounds__(64 * kW, 2) void decode_mfma16_kernel(DecodeProblem
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (16 * wave + 4 * g + i >= valid) sc[i] = -INFINITY;
+      }
+      if (nodes) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = 16 * wave + 4 * g + i, node = kT * t + row - node0;
+          if (row < valid && bad >> (4 * g + i) & 1) sc[i] = __builtin_nanf("");
+          if (node >= 0 && (node >= 64 || !(seen >> node & 1))) sc[i] = -INFINITY;
+        }
       }
       const float mx = max_groups(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])));
       if (g == 0) lds_st(L, D::kMax + 4 * kW * n16 + 4 * wave, mx);
@@ -416,7 +465,7 @@ __global__ __launch_bounds__(64 * kW, 2) void decode_mfma16_kernel(DecodeProblem
     lds_barrier();  // every wave is done with the tile
     const int lane = wave_lane();
     const int n16 = lane & 15, g = lane >> 4;
-    const int64_t hq0 = (kFilled ? slot_of(p, chunk, s) : (int64_t)chunk + s) * p.Hq + head0;
+    const int64_t hq0 = (kFilled == 1 ? slot_of(p, chunk, s) : (int64_t)chunk + s) * p.Hq + head0;
     float rmax = 0.f;
 #pragma unroll
     for (int cb = 0; cb < kCB; ++cb) settle(o[cb]);
@@ -469,6 +518,17 @@ __global__ __launch_bounds__(64 * kW, 2) void decode_mfma16_kernel(DecodeProblem
 }
 
 template <typename KT, int kW, bool kPaged, bool kFp8, bool kFilled>
+__global__ __launch_bounds__(64 * kW, 2) void decode_mfma16_kernel(DecodeProblem p, int groups, float* zero_out,
+                                                                  int zero_n) {
+  decode16_body<KT, kW, kPaged, kFp8, kFilled>(p, groups, zero_out, zero_n);
+}
+// Trees of drafted tokens (spans; 8 waves: it runs where a workgroup has a tile or two).
+template <typename KT, bool kPaged, bool kFp8>
+__global__ __launch_bounds__(512, 2) void decode_mfma16_tree_kernel(DecodeProblem p, int groups, TreeStep tree) {
+  decode16_body<KT, 8, kPaged, kFp8, 3, true>(p, groups, nullptr, 0, tree);
+}
+
+template <typename KT, int kW, bool kPaged, bool kFp8, bool kFilled>
 hipError_t launch16_t(const DecodeProblem& p, hipStream_t stream, float* zero_out, int zero_n, hipEvent_t ev_begin,
                       hipEvent_t ev_end) {
   constexpr int lds = Lds<kW>::kBytes;
@@ -505,7 +565,29 @@ hipError_t launch16_k(const DecodeProblem& p, hipStream_t stream, float* zero_ou
   return launch16_w<kW, false, false>(p, stream, zero_out, zero_n, ev_begin, ev_end);
 }
 
+template <typename KT, bool kPaged, bool kFp8>
+hipError_t launch16_tree_k(const DecodeProblem& p, const TreeStep& tree, hipStream_t stream) {
+  constexpr int lds = Lds<8>::kBytes;
+  static OncePerDevice once;
+  const auto k = decode_mfma16_tree_kernel<KT, kPaged, kFp8>;
+  const hipError_t e = allow_lds(once, reinterpret_cast<const void*>(k), lds);
+  if (e != hipSuccess) return e;
+  const int groups = p.Hq / 16;
+  hipLaunchKernelGGL(k, dim3((unsigned)mfma_grid_blocks(p.num_chunks, groups)), dim3(512), lds, stream, p, groups, tree);
+  return hipGetLastError();
+}
+template <typename KT, bool kFp8>
+hipError_t launch16_tree(const DecodeProblem& p, const TreeStep& tree, hipStream_t stream) {
+  return p.block_table ? launch16_tree_k<KT, true, kFp8>(p, tree, stream) : launch16_tree_k<KT, false, kFp8>(p, tree, stream);
+}
+
 }  // namespace
+
+hipError_t launch_decode_mfma16_tree(const DecodeProblem& p, const TreeStep& tree, hipStream_t stream) {
+  if (p.kv_dtype == LA_DTYPE_FP8_E4M3) return launch16_tree<__hip_bfloat16, true>(p, tree, stream);
+  if (p.kv_dtype == LA_DTYPE_BF16) return launch16_tree<__hip_bfloat16, false>(p, tree, stream);
+  return launch16_tree<__half, false>(p, tree, stream);
+}
 
 hipError_t launch_decode_mfma16(const DecodeProblem& p, int waves, hipStream_t stream, float* zero_out, int64_t zero_n,
                                 hipEvent_t ev_begin, hipEvent_t ev_end) {

@@ -78,6 +78,7 @@ __device__ inline void plan_spans(const TreeQueries& p) {
     own = lo <= even + kSegment * ((filled - 1 + p.chunks - 1) / p.chunks);
     if (own) len = lo;
   }
+  len = min((len + p.step - 1) / p.step * p.step, kMost);
   int32_t* const first = p.lens + seqs;
   const int64_t limit = (int64_t)p.chunks * len;
   int64_t at = 0;

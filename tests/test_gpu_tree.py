@@ -167,6 +167,36 @@ def test_rows_that_are_not_finite_reach_only_those_that_see_them(cuda, kv, bad, 
             assert got[sees].isnan().all()
 
 
+# 64 nodes x 128 heads: the kernel of 128 heads per workgroup (fewer take the one of 16)
+@pytest.mark.parametrize("kv", [torch.bfloat16, torch.float16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("bad,part", [(float("nan"), "latent"), (float("inf"), "latent"), (float("nan"), "rope")])
+def test_rows_that_are_not_finite_with_many_heads(cuda, kv, bad, part):
+    if kv == torch.float8_e4m3fn and bad == bad:
+        pytest.skip("e4m3 has no infinities")
+    n = 64
+    for L, node in ((150, 5), (224, 11), (700, 63)):
+        g = torch.Generator().manual_seed(L + node)
+        data = [torch.randn(L, 576, generator=g).to(kv).float()]
+        c = Case(cuda, "paged", [L], n, heads=128, kv=kv, data=data, seed=node)
+        clean = c.reference()
+        data[0][L - n + node, 100 if part == "latent" else 530] = bad
+        c.layout = Layout("paged", data, kv, cuda, block=64, seed=node)
+        got = c.run(kernel_variant=MFMA, out_dtype=torch.float32).double().cpu()
+        sees = torch.tensor([node in a for a in ancestors(c.parents[0])])
+        assert sees.any() and not sees.all()
+        assert_close(got[~sees].numpy(), clean[~sees].numpy(), "bf16")
+        assert got[sees].isnan().all()
+
+
+# the 16-head kernel's largest launches and the 128-head kernel's smallest (256 compute units x 256 rows x 16 heads)
+@pytest.mark.parametrize("rows,n,heads", [([2000, 40], 1, 128), ([2100, 40, 700], 3, 128), ([9000], 7, 16), ([17000], 5, 16),
+                                          ([300, 800, 129], 17, 16)])
+@pytest.mark.parametrize("kv", [torch.bfloat16, torch.float8_e4m3fn])
+def test_around_the_smaller_kernels_range(cuda, rows, n, heads, kv):
+    case = Case(cuda, "packed_capacity", rows, n, heads=heads, kv=kv)
+    case.check(case.run(), False, (rows, n, heads))
+
+
 def test_scores_far_apart(cuda):
     """Rows scaled so that scores jump by hundreds between context and nodes, either way."""
     for scale in (6.0, 1 / 6.0):
