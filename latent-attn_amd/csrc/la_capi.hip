@@ -234,12 +234,18 @@ int prepare(const la_decode_args* a, DecodeProblem* p, Plan* plan, bool coarse =
   int64_t nchunks = total > 0 ? (total + L - 1) / L : 0;
   if (tree && pl.mfma && total > 0) {  // spans, their length found on the device: as many as there is room for
     const int64_t rows = total + (int64_t)a->num_seqs * (kSpanRows - 1), groups = (p->Hq + mfma_heads_per_group() - 1) / mfma_heads_per_group();
-    // 16 heads per workgroup while that leaves each two tiles of 128 rows at most
-    if (rows * (p->Hq / 16) <= 256LL * ncu) {
+    // 16 heads per workgroup where a sequence has no more, or that leaves each few tiles of
+    // 128 rows: eight where the 128-head kernel has under 128 heads to a sequence, else
+    // four. A call, us, 128-head kernel / this one: 1 x 500 rows, 7 x 16 heads 36.2 / 28.6;
+    // 1 x 16,000 45.5 / 40.8; 1 x 30,000 55.9 / 53.3; 1 x 60,000 60.3 / 72.9; 4 x 2000,
+    // 16 x 16 heads 47.2 / 42.4; 4 x 3900 53.3 / 56.5; 1 x 16,000, 128 heads 47.6 / 42.6;
+    // 2 x 2000, 7 x 128 48.4 / 56.4; 32 x 1000, 16 heads 38.6 / 34.9; 32 x 30,000 296 / 223.
+    const int64_t heads16 = p->Hq / 16, most = heads16 == 1 ? rows : heads16 < 8 ? 1024LL * ncu : 512LL * ncu;
+    if (rows * heads16 <= most) {
       pl.waves16 = 8;
       min_rows = 128;
     }
-    nchunks = std::max(std::min(std::max<int64_t>(ncu / (pl.waves16 ? p->Hq / 16 : groups), 1), (rows + min_rows - 1) / min_rows),
+    nchunks = std::max(std::min(std::max<int64_t>(ncu / (pl.waves16 ? heads16 : groups), 1), (rows + min_rows - 1) / min_rows),
                        (rows + kMaxChunkRows - 1) / kMaxChunkRows);
   }
   if (nchunks > (int64_t)1 << 30) return LA_ERROR_INVALID_VALUE;

@@ -188,9 +188,10 @@ def test_rows_that_are_not_finite_with_many_heads(cuda, kv, bad, part):
         assert got[sees].isnan().all()
 
 
-# the 16-head kernel's largest launches and the 128-head kernel's smallest (256 compute units x 256 rows x 16 heads)
-@pytest.mark.parametrize("rows,n,heads", [([2000, 40], 1, 128), ([2100, 40, 700], 3, 128), ([9000], 7, 16), ([17000], 5, 16),
-                                          ([300, 800, 129], 17, 16)])
+# the 16-head kernel's largest launches and the 128-head kernel's smallest: 512 (under 128 heads to a sequence: 1024)
+# rows per 16 heads and compute unit, of 256
+@pytest.mark.parametrize("rows,n,heads", [([8000, 40], 1, 128), ([4700, 40, 700], 3, 128), ([36000], 7, 16), ([38000], 7, 16),
+                                          ([9000, 300, 129], 1, 16)])
 @pytest.mark.parametrize("kv", [torch.bfloat16, torch.float8_e4m3fn])
 def test_around_the_smaller_kernels_range(cuda, rows, n, heads, kv):
     case = Case(cuda, "packed_capacity", rows, n, heads=heads, kv=kv)
