@@ -1616,12 +1616,15 @@ int evict(const la_evict_args* a, hipStream_t stream, bool run_it, size_t* need)
   p.keep = a->keep;
   p.first = a->first;
   p.last = a->last;
-  const bool staged = evict_staged(p, cu_count());
+  // no sequence has more rows than it has room for: nothing moves, and a list is all that can be asked for
+  const bool moves = a->keep < (a->seq_offsets ? a->total_rows : (int64_t)p.rows.region);
+  if (!moves && !a->kept) return LA_SUCCESS;
+  const bool staged = moves && evict_staged(p, cu_count());
   auto carve = [&](void* ws) {
     Carve v(ws);
     p.start = static_cast<int32_t*>(v.take((size_t)a->num_seqs * sizeof(int32_t)));
     p.kept = a->kept ? a->kept : static_cast<int32_t*>(v.take((size_t)a->num_seqs * a->keep * sizeof(int32_t)));
-    p.from = static_cast<uint32_t*>(v.take((size_t)a->num_seqs * a->keep * sizeof(uint32_t)));
+    if (moves) p.from = static_cast<uint32_t*>(v.take((size_t)a->num_seqs * a->keep * sizeof(uint32_t)));
     if (staged) p.staged = static_cast<char*>(v.take((size_t)a->num_seqs * a->keep * p.rows.row_bytes));
     return v.total();
   };

@@ -129,7 +129,7 @@ inline size_t weigh_part_bytes(int spans, int seqs, int rows) {
 hipError_t launch_weigh_mfma(const WeighProblem& p, int64_t most_tiles, hipStream_t stream, int ncu);
 
 // la_evict_kv.
-struct EvictProblem {
+struct EvictProblem {  // from: nullptr where no sequence can have more than `keep` rows
   MovedRows rows;
   float* weights;
   int keep, first, last;

@@ -57,12 +57,12 @@ __global__ __launch_bounds__(64 * kW) void evict_select_kernel(EvictProblem p, i
   const int L = max(min(p.rows.lens[s], moved_room(p.rows, s)), 0);
   float* const w = p.weights + begin;
   int32_t* const kept = p.kept + (int64_t)s * p.keep;
-  uint32_t* const from = p.from + (int64_t)s * p.keep;
   if (L <= p.keep) {
     for (int i = tid; i < p.keep; i += kThreads) kept[i] = i < L ? i : -1;
     if (tid == 0) p.start[s] = p.keep;
     return;
   }
+  uint32_t* const from = p.from + (int64_t)s * p.keep;
   const int lo = p.first, hi = L - p.last;  // the rows between
   int left = p.keep - p.first - p.last;     // of which so many stay
   const int segments = (L + kSegment - 1) / kSegment;
@@ -274,7 +274,7 @@ hipError_t launch_evict(const EvictProblem& p, hipStream_t stream) {
     if (few) hipLaunchKernelGGL(evict_select_kernel<4>, dim3(blocks), dim3(256), 0, stream, p, first);
     else hipLaunchKernelGGL(evict_select_kernel<16>, dim3(blocks), dim3(1024), 0, stream, p, first);
   });
-  if (e != hipSuccess || p.keep == 0) return e;
+  if (e != hipSuccess || p.keep == 0 || !p.from) return e;
   switch (moved_unit(p.rows)) {
     case 16: return move_t<u32x4>(p, stream);
     case 8: return move_t<uint64_t>(p, stream);

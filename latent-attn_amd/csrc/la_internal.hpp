@@ -322,14 +322,15 @@ __device__ inline int32_t* filled_notes(const DecodeProblem& p) {
 }
 // Spans (chunk_len == kSpans; the kernels for trees of drafted tokens): chunks of equal
 // length in a row space where every sequence has whole tiles of kSpanRows rows. The
-// kernel that runs before them plans it: behind the num_seqs lengths it leaves every
-// sequence's first tile, the tiles of all, and the tiles of a chunk.
+// kernel that runs before them plans it: behind the num_seqs lengths, which it has kept
+// within their regions, it leaves every sequence's first tile, the tiles of all, and the
+// tiles of a chunk.
 constexpr int kSpans = INT32_MIN, kSpanRows = 32;
 __device__ inline const int32_t* span_tiles(const DecodeProblem& p) { return p.lens + p.num_seqs; }
 __device__ inline int span_rows(const DecodeProblem& p) { return kSpanRows * span_tiles(p)[p.num_seqs + 1]; }
 __device__ inline int64_t span_begin(const DecodeProblem& p, int s) { return (int64_t)kSpanRows * span_tiles(p)[s]; }
 __device__ inline int64_t span_end(const DecodeProblem& p, int s) {
-  return min(span_begin(p, s) + filled_rows(p, s), span_begin(p, s + 1));
+  return min(span_begin(p, s) + p.lens[s], span_begin(p, s + 1));
 }
 // Partial slot of the piece of chunk c inside sequence s.
 __device__ inline int64_t slot_of(const DecodeProblem& p, int64_t c, int s) {

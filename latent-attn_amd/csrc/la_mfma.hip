@@ -1062,7 +1062,9 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeProblem& p, int gro
     uint64_t seen = 0;
     if constexpr (kTree) {
       const int wblk = min(32 * wave, (hg_heads - 1) & ~31), r = min(lane_id() & 31, hg_heads - 1 - wblk);
-      const uint64_t* from = tree.seen + (int64_t)s * p.qps + (uint32_t)(group * kHG + wblk + r) / (uint32_t)p.nh;
+      uint32_t nh = (uint32_t)p.nh;
+      asm volatile("" : "+s"(nh));  // (its reciprocal, made before the loop, was spilled)
+      const uint64_t* from = tree.seen + (int64_t)s * p.qps + (uint32_t)(group * kHG + wblk + r) / nh;
       asm volatile("global_load_dwordx2 %0, %1, off" : "=v"(seen) : "v"(from));
     }
 

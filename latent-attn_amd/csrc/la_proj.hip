@@ -1426,7 +1426,7 @@ bool absorb_any_supported(const QuerySource& q, const RowSource& r, const void* 
   return (w_dtype == LA_DTYPE_BF16 || w_dtype == LA_DTYPE_F16) && (reinterpret_cast<uintptr_t>(W_UK) & 15) == 0 &&
          c.qk_nope_head_dim == 128 && c.kv_lora_rank == 512 && c.qk_rope_head_dim == 64 &&
          q_vec(q.q_nope, q.dtype, q.nope_stride, q.nope_head) && q_vec(q.q_rope, q.dtype, q.rope_stride, q.rope_head) &&
-         ((reinterpret_cast<uintptr_t>(r.cos) | reinterpret_cast<uintptr_t>(r.sin)) & 15) == 0 && 64 * 4 * (((q.tokens + 31) / 32 * ((c.num_heads + 7) / 8) + 7) / 8) <= most_blocks(kAbsThreads) && device_is_gfx950();
+         ((reinterpret_cast<uintptr_t>(r.cos) | reinterpret_cast<uintptr_t>(r.sin)) & 15) == 0 && device_is_gfx950();
 }
 
 hipError_t launch_absorb_any(const AbsorbQueries& x, const void* W_UK, int w_dtype, void* out, int out_mode, float scale,

@@ -49,41 +49,50 @@ __device__ inline void plan_spans(const TreeQueries& p) {
   const int lane = wave_lane(), seqs = p.q.num_seqs;
   // 2^24 tiles: more than the memory holds; their sums stay below 2^31 (malformed offsets may overlap)
   auto tiles = [&](int s) { return s < seqs ? (int)min(((uint32_t)tree_rows(p, s) + kSpanRows - 1) / kSpanRows, 1u << 24) : 0; };
-  const int mine = tiles(lane);
-  int64_t total = 0;
-  int filled = 0, most = 0;
-  for (int s0 = 0; s0 < seqs; s0 += 64) {
-    const int n = s0 == 0 ? mine : tiles(s0 + lane);
-    total += wave_sum_i(n);
-    filled += wave_sum_i(n > 0);
-    most = max(most, n);
+  constexpr int kHeld = 4;  // of the first 256 sequences, in registers
+  int held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) held[i] = tiles(lane + 64 * i);
+  int64_t sum = 0;
+  int have = 0;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) sum += held[i], have += held[i] > 0;
+#pragma unroll 4
+  for (int s = lane + 64 * kHeld; s < seqs; s += 64) {
+    const int n = tiles(s);
+    sum += n, have += n > 0;
   }
-  for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  const int64_t total = sum;
+  const int filled = wave_sum_i(have);
   constexpr int kMost = kMaxChunkRows / kSpanRows;
   const int even = (int)min(max((total + p.chunks - 1) / p.chunks, (int64_t)p.shortest), (int64_t)kMost);
   int len = even;
   bool own = false;
   if (filled <= p.chunks) {
     auto fits = [&](int n) {
-      int64_t sum = 0;
-      for (int s0 = 0; s0 < seqs; s0 += 64) sum += wave_sum_i(pieces(s0 == 0 ? mine : tiles(s0 + lane), n));
-      return sum <= p.chunks;
+      int64_t count = 0;
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) count += pieces(held[i], n);
+      for (int s = lane + 64 * kHeld; s < seqs; s += 64) count += pieces(tiles(s), n);
+      for (int o = 32; o > 0; o >>= 1) count += __shfl_xor(count, o, 64);
+      return count <= p.chunks;
     };
-    int lo = even, hi = max(even, min(most, kMost));
-    while (lo < hi) {
+    int lo = even, hi = min(even + kSegment * ((filled - 1 + p.chunks - 1) / p.chunks), kMost);
+    own = fits(hi);
+    while (own && lo < hi) {
       const int mid = (lo + hi) / 2;
       if (fits(mid)) hi = mid;
       else lo = mid + 1;
     }
-    own = lo <= even + kSegment * ((filled - 1 + p.chunks - 1) / p.chunks);
-    if (own) len = lo;
+    if (own) len = hi;
   }
   len = min((len + p.step - 1) / p.step * p.step, kMost);
   int32_t* const first = p.lens + seqs;
   const int64_t limit = (int64_t)p.chunks * len;
   int64_t at = 0;
   for (int s0 = 0; s0 < seqs; s0 += 64) {
-    int n = s0 == 0 ? mine : tiles(s0 + lane);
+    int n = tiles(s0 + lane);
     if (own) n = pieces(n, len) * len;
     const int end = wave_scan(n);
     if (s0 + lane < seqs) first[s0 + lane] = (int)min(at + end - n, limit);
@@ -279,9 +288,7 @@ __global__ __launch_bounds__(kAcceptThreads) void accept_kernel(AcceptProblem p,
   if (threadIdx.x == 0) p.rows.lens[s] = L - n + rows;
 }
 
-struct alignas(16) Unit16 {
-  uint32_t x[4];
-};
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 }  // namespace
 
@@ -305,7 +312,7 @@ hipError_t launch_plain_tree(const PlainTree& p, hipStream_t stream) {
 
 hipError_t launch_accept(const AcceptProblem& p, hipStream_t stream) {
   const int unit = moved_unit(p.rows);
-  const auto k = unit == 16  ? accept_kernel<Unit16>
+  const auto k = unit == 16  ? accept_kernel<u32x4>
                  : unit == 8 ? accept_kernel<uint64_t>
                  : unit == 4 ? accept_kernel<uint32_t>
                  : unit == 2 ? accept_kernel<uint16_t>

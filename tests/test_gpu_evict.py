@@ -226,3 +226,37 @@ def test_kept_is_optional_and_the_workspace_the_callers(cuda):
         torch.cuda.synchronize()
         assert torch.equal(x, kv) and torch.equal(y, w) and torch.equal(z, lens)
         assert (ws[need + 8:] == 0xFF).all() and (ws[:8] == 0xFF).all()
+
+
+@pytest.mark.parametrize("keep", [300, 1 << 30])
+def test_more_than_a_region_holds(cuda, keep):
+    """Nothing can move: no workspace for it, whatever the number asked for."""
+    lib = capi.load()
+    g = torch.Generator().manual_seed(4)
+    kv, w = torch.randn(3, 300, 576, generator=g).bfloat16().to(cuda), torch.rand(3, 300, generator=g).to(cuda)
+    lens = torch.tensor([300, 20, 900], dtype=torch.int32, device=cuda)
+    old = kv.clone(), w.clone(), lens.clone()
+    a = capi.EvictArgs(kv_cache=kv.data_ptr(), kv_dtype=capi.LA_DTYPE_BF16, total_rows=900, num_seqs=3, seq_capacity=300,
+                       seq_lens=lens.data_ptr(), weights=w.data_ptr(), keep=keep, cfg=capi.config(MLAConfig.deepseek_v2()))
+    assert lib.la_evict_kv_workspace_size(ctypes.byref(a)) <= 4096
+    assert lib.la_evict_kv(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == capi.LA_SUCCESS
+    if keep == 300:
+        kept = F.evict_kv(kv, lens, w, MLAConfig.deepseek_v2(), keep).cpu()
+        for s, n in enumerate((300, 20, 300)):
+            assert kept[s].tolist() == list(range(n)) + [-1] * (keep - n)
+    assert torch.equal(kv, old[0]) and torch.equal(w, old[1]) and torch.equal(lens, old[2])
+
+
+def test_few_and_many_sequences_agree(cuda):
+    """A few sequences' rows go through a copy, many are moved where they lie: the same rows either way."""
+    g = torch.Generator().manual_seed(6)
+    cfg = MLAConfig.deepseek_v2()
+    kv, w = torch.randn(64, 500, 576, generator=g).bfloat16().to(cuda), torch.rand(64, 500, generator=g).to(cuda)
+    lens = torch.randint(300, 501, (64,), generator=g, dtype=torch.int32).to(cuda)
+    one = [x.clone() for x in (kv, w, lens)]
+    kept = F.evict_kv(kv, lens, w, cfg, 250, first=4, last=16)
+    for s in (0, 31, 63):
+        a, b, n = (x[s:s + 1].clone() for x in one)
+        k = F.evict_kv(a, n, b, cfg, 250, first=4, last=16)
+        assert torch.equal(k[0], kept[s]) and torch.equal(n[0], lens[s]) and torch.equal(b[0], w[s])
+        assert torch.equal(a[0, :250], kv[s, :250])

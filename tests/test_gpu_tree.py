@@ -114,11 +114,30 @@ def test_chunks_across_sequences(cuda, layout, rows):
     case.check(case.run(), False, (layout, rows))
 
 
-@pytest.mark.parametrize("count,n,heads", [(150, 3, 16), (70, 16, 64), (65, 1, 16)])
+@pytest.mark.parametrize("count,n,heads", [(150, 3, 16), (70, 16, 64), (65, 1, 16), (300, 2, 16), (600, 8, 16)])
 def test_more_sequences_than_lanes(cuda, count, n, heads):
     rows = [(37 * i * i + 11 * i) % 190 for i in range(count)]
     case = Case(cuda, "capacity", rows, n, heads=heads)
     case.check(case.run(), False, (count, n, heads))
+
+
+@pytest.mark.parametrize("block", [7, 16, 48, 96])
+def test_block_sizes(cuda, block):
+    """A tile of 32 rows lies in one block, or the plain kernel runs."""
+    case = Case(cuda, "paged", [200, 20, 97], 9, block=block)
+    case.check(case.run(), False, block)
+
+
+@pytest.mark.parametrize("variant", [AUTO, PLAIN])
+@pytest.mark.parametrize("q", [torch.float32, torch.bfloat16])
+def test_queries_out_of_line(cuda, variant, q):
+    """Views whose elements are not aligned to whole vectors, by token, head or address."""
+    for pad, skip in ((1, 0), (4, 1), (3, 2)):
+        c = Case(cuda, "capacity", [150, 64, 300], 6, q=q, seed=pad)
+        wide = torch.zeros(*c.q.shape[:2], c.q.shape[2] + pad, dtype=q, device=cuda)
+        wide[..., skip:skip + c.q.shape[2]] = c.q
+        c.q = wide[..., skip:skip + c.q.shape[2]]
+        c.check(c.run(kernel_variant=variant, out_dtype=torch.float32), variant == PLAIN, (pad, skip))
 
 
 def test_parents_outside_their_range_are_none(cuda):

@@ -46,8 +46,9 @@ class Case:
         return weigh_reference(self.rows, q[..., :self.dn], q[..., self.dn:], as_double(self.W_UK), as_double(self.cos),
                                as_double(self.sin), self.n, self.rotate_q)
 
-    def check(self, variant=AUTO, what=""):
-        """From zeros, within the bound; on top of other weights, the same sum; nothing outside the sequences' rows."""
+    def check(self, variant=AUTO, what="", pieces=1):
+        """From zeros, within the bound; on top of other weights, the same sum; nothing outside the sequences' rows.
+        pieces: sums that the call adds to a weight one after another (4096 rows of tokens and heads at most in each)."""
         zero = torch.full_like(self.weights, 7.0)
         places = [weight_places(self.layout, s, r.shape[0]) for s, r in enumerate(self.rows)]
         inside = torch.cat(places) if places else torch.zeros(0, dtype=torch.long)
@@ -67,9 +68,11 @@ class Case:
         assert (got[outside] == 7).all()
         first = start.cpu().view(-1)
         assert torch.equal(more[outside], first[outside])
-        # one fp32 sum more
+        # The weights are positive, so every partial sum is below the whole and its rounding below 2^-24 of that
+        # (1 + 2^-20 for the roundings before it). P pieces make P such sums on top of other weights and P - 1 from
+        # zero (the first is exact): 2 P - 1 together, and one piece is given 2.
         want = first[inside].double() + got[inside]
-        assert ((more[inside].double() - want).abs() <= 2.0 ** -23 * want).all()
+        assert ((more[inside].double() - want).abs() <= max(2, 2 * pieces - 1) * (1 + 2.0 ** -20) * 2.0 ** -24 * want).all()
 
 
 @pytest.mark.parametrize("layout", ["uniform", "capacity", "packed", "packed_capacity", "paged"])
@@ -111,6 +114,67 @@ def test_other_head_shapes(cuda, dims, heads):
 def test_scores_far_apart_and_all_alike(cuda, scale, variant):
     c = Case(cuda, "capacity", [400, 100], 2, q=torch.float32, scale=scale)
     c.check(variant, str(scale))
+
+
+@pytest.mark.parametrize("block", [1, 7, 16, 48])
+@pytest.mark.parametrize("heads", [16, 128])
+def test_block_sizes(cuda, block, heads):
+    Case(cuda, "paged", [100, 33, 64, 31, 5], 2, heads=heads, block=block).check(MFMA, block)
+
+
+@pytest.mark.parametrize("variant", [AUTO, PLAIN])
+@pytest.mark.parametrize("q", [torch.float32, torch.bfloat16])
+def test_queries_out_of_line(cuda, variant, q):
+    """Views whose elements are not aligned to whole vectors, by token, head or address."""
+    for pad, skip in ((1, 0), (4, 1), (3, 2)):
+        c = Case(cuda, "capacity", [150, 64, 300], 6, q=q, seed=pad)
+        wide = torch.zeros(*c.q.shape[:2], c.q.shape[2] + pad, dtype=q, device=cuda)
+        wide[..., skip:skip + c.q.shape[2]] = c.q
+        c.q = wide[..., skip:skip + c.q.shape[2]]
+        c.check(variant, (pad, skip))
+
+
+# more (token, head) rows than one piece of the call takes
+@pytest.mark.parametrize("n,heads,pieces", [(50, 128, 2), (300, 40, 3), (129, 33, 2)])
+def test_pieces_of_tokens(cuda, n, heads, pieces):
+    Case(cuda, "capacity", [n + 37, n, 20], n, heads=heads, kv=torch.float16).check(MFMA, (n, heads), pieces)
+
+
+def test_pieces_of_sequences(cuda):
+    """More room for scores than the call takes at once: in pieces of 128 sequences; each as on its own."""
+    count, region, heads = 200, 8192, 128
+    g = torch.Generator(device=cuda).manual_seed(3)
+    cfg = MLAConfig(5120, 512, 128, 64, heads, 128)
+    kv = torch.zeros(count, region, 576, dtype=torch.float8_e4m3fn, device=cuda)
+    kv[:, :120] = torch.randn(count, 120, 576, generator=g, device=cuda).to(torch.float8_e4m3fn)
+    lens = torch.randint(1, 121, (count,), generator=g, device=cuda, dtype=torch.int32)
+    q = torch.randn(count, heads, 192, generator=g, device=cuda).bfloat16()
+    W_UK = weights(heads, torch.bfloat16, 5, 512, 128, 128)[0].to(cuda)
+    cos, sin = (x.to(cuda) for x in tables(region, 64))
+    w = torch.zeros(count, region, device=cuda)
+    F.weigh_kv(w, kv, q[..., :128], q[..., 128:], W_UK, cos, sin, cfg, seq_lens=lens, rotate_q=True)
+    for s in (0, 1, 127, 128, 129, 199):
+        n = int(lens[s])
+        alone = torch.zeros(1, region, device=cuda)
+        F.weigh_kv(alone, kv[s:s + 1], q[s:s + 1, :, :128], q[s:s + 1, :, 128:], W_UK, cos, sin, cfg, seq_lens=lens[s:s + 1],
+                   rotate_q=True)
+        # two orders of the same fp32 sums of 128 terms: 128 half steps each
+        assert ((alone[0, :n] - w[s, :n]).abs() <= 256 * 2.0 ** -24 * w[s, :n]).all()
+        assert abs(float(w[s, :n].double().sum()) - heads) <= 1e-5 * heads
+        assert (w[s, n:] == 0).all()
+
+
+def test_on_another_stream(cuda):
+    """weigh_kv behind its inputs on a stream of the caller's, beside the current one's work."""
+    c = Case(cuda, "paged", [900, 33, 64], 2, heads=128)
+    want, got = torch.zeros_like(c.weights), torch.zeros_like(c.weights)
+    c.run(want)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        c.run(got)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
 
 
 def test_long_rows_of_one_sequence(cuda):
