@@ -442,7 +442,10 @@ typedef struct la_weigh_args {
   /* fp32, one per row of the sequences' regions: position p of sequence s at
    * s * seq_len + p (equal regions), seq_offsets[s] + p, or s *
    * blocks_per_seq * block_size + p (paged). Entries past a sequence's rows
-   * are left as they are. */
+   * are left as they are. A row that is not finite makes its own sequence's
+   * weights NaN. On the matrix cores an fp16 cache takes absorbed queries whose
+   * elements, times log2(e) / sqrt(qk_nope_head_dim + qk_rope_head_dim), stay
+   * within 65504 / 64. */
   float* weights;
   la_mla_config cfg;
   void* workspace; /* la_weigh_kv_workspace_size bytes; NULL: taken stream-ordered (not under capture) */
@@ -470,7 +473,8 @@ typedef struct la_evict_args {
    * rows and weights move down to [0, keep) in their order, the weights behind
    * are zeroed (the rows are left as they are), the length becomes keep.
    * Positions are a row's place in the cache, here as everywhere. Shorter
-   * sequences are left unchanged. first + last <= keep. */
+   * sequences are left unchanged. first + last <= keep. Sequences that are cut
+   * back must not share blocks of a pool. */
   int32_t keep;
   int32_t first;
   int32_t last;

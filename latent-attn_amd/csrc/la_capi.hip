@@ -5,7 +5,10 @@
 // la_f32.hip (float32) and la_generic.hip (any shape), absorption and merge +
 // projection for 16-bit weights and the merge for float32 ones in la_proj.hip,
 // the other absorption in la_f32.hip and la_generic.hip, la_append.hip,
-// la_naive.hip.
+// la_naive.hip; prompts and prefixes in la_prompt.hip, la_expand.hip and
+// la_join.hip; drafted trees and accepted paths in la_tree.hip, with attention
+// kernels of their own in la_mfma.hip and la_mfma16.hip; row weights and
+// evictions in la_weigh.hip and la_evict.hip.
 #include "la_internal.hpp"
 #include "la_draft.hpp"
 #include "la_prompt.hpp"

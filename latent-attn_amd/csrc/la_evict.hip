@@ -15,6 +15,11 @@
 // written: no row is overwritten before its stripe is read, and no workgroup
 // waits for another. A few sequences have too few stripes for that; their rows go
 // through a copy, two launches over all compute units.
+//
+// What bounds it (bf16): 32 sequences of 8192 rows cut to 2048, 48 us: selection 18, five
+// rounds of barriers over registers on 32 compute units; movement 30 to 49 (from the
+// caches or HBM), 147 MB. One of 32,768 to 16,384: 66 us through the copy, 529 in stripes;
+// 1001 to 512: 21, latency.
 #include "la_draft.hpp"
 
 #include <algorithm>

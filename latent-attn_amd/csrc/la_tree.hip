@@ -44,6 +44,8 @@ __device__ inline int tree_rows(const TreeQueries& p, int s) {
 // suffice. A chunk over several sequences pays kSegment tiles for each after the first
 // (a segment's fixed part: its queries, its first tiles' way, its partial rows), own
 // chunks for the shorter last ones: the smaller estimate of the longest chunk is taken.
+// (16 trees of 16 behind 500 to 6000 rows, 128 heads, 16 chunks: own chunks 404 us a call, even
+// ones 328.)
 constexpr int kSegment = 8;
 __device__ inline void plan_spans(const TreeQueries& p) {
   const int lane = wave_lane(), seqs = p.q.num_seqs;
@@ -246,7 +248,7 @@ __global__ __launch_bounds__(256) void plain_tree_kernel(PlainTree p, int64_t fi
 // path's rows move down over rows that may be on it), columns of the rows being
 // independent of one another. 16-bit rows of 576 elements and 64 nodes at most
 // are one such step, so the kernel is three dependent loads (length, path,
-// row) and the stores: latency is all there is.
+// row) and the stores: latency is all there is (64 trees of 25 4.3 us, one of 64 3.5).
 constexpr int kAcceptThreads = 1024, kAcceptPieces = 5;
 template <typename U>
 __global__ __launch_bounds__(kAcceptThreads) void accept_kernel(AcceptProblem p, int64_t first) {

@@ -501,6 +501,10 @@ def weigh_kv(
                      rows is at position L - n + j and sees the rows up to its own
         rotate_q:    q_rope is not rotated yet
         kernel_variant: 0 = automatic, 1 = plain kernels, 2 = matrix cores
+                     (an fp16 cache: absorbed queries, times
+                     log2(e) / sqrt(qk_nope_head_dim + qk_rope_head_dim), up to 65504 / 64)
+
+    A row that is not finite makes its own sequence's weights NaN.
     """
     _C = _load_ext()
     _C.weigh_kv_forward(weights, kv_cache, q_nope, q_rope, W_UK, rope_cos, rope_sin, seq_offsets, *_cfg_args(cfg),
@@ -524,7 +528,8 @@ def evict_kv(
     ones with the largest weights (of equal ones the earlier; NaN counts as the
     smallest). Rows keep their order and move to the front with their weights;
     their positions, for RoPE too, are then their places in the cache, as
-    everywhere. In a paged cache the blocks past ``keep`` are free afterwards.
+    everywhere. In a paged cache the blocks past ``keep`` are free afterwards;
+    sequences that are cut back must not share blocks.
 
     Args:
         kv_cache, seq_offsets, block_table, block_size: as in ``append_kv``
