@@ -114,6 +114,69 @@ def test_chunks_across_sequences(cuda, layout, rows):
     case.check(case.run(), False, (layout, rows))
 
 
+@pytest.mark.parametrize("rows,n,heads", [([40, 100], 7, 16), ([700, 64, 130], 64, 128)])
+@pytest.mark.parametrize("w", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("kv", [torch.bfloat16, torch.float16])
+def test_weights_and_outputs_of_every_type(cuda, rows, n, heads, w, kv):
+    c = Case(cuda, "capacity", rows, n, heads=heads, kv=kv, w=w)
+    ref = c.reference().numpy()
+    for out in (torch.float32, torch.float16, torch.bfloat16):
+        got = c.run(kernel_variant=MFMA, out_dtype=out)
+        assert got.dtype == out
+        assert_close(got.double().cpu().numpy(), ref, "bf16", f"{w} {out}")
+
+
+@pytest.mark.parametrize("dims", [(512, 64, 64, 128), (512, 128, 64, 96), (512, 48, 64, 40), (512, 192, 64, 128)])
+@pytest.mark.parametrize("rows,n,heads", [([40, 100], 7, 16), ([500, 64], 32, 64)])
+def test_other_heads_over_the_same_rows(cuda, dims, rows, n, heads):
+    """The matrix cores' attention with absorption and projection of other widths."""
+    c = Case(cuda, "paged", rows, n, heads=heads, dims=dims)
+    c.check(c.run(kernel_variant=MFMA), False, dims)
+
+
+def test_an_output_out_of_line(cuda):
+    """An output that is not aligned to 16 bytes, and nothing written beside it."""
+    lib = capi.load()
+    c = Case(cuda, "capacity", [700, 64, 130], 64, heads=128)
+    want = c.run(out_dtype=torch.bfloat16)
+    room = torch.full((want.numel() + 64,), 7.0, dtype=torch.bfloat16, device=cuda)
+    kv = c.layout.kv
+    a = capi.TreeArgs(kv_cache=kv.data_ptr(), kv_dtype=capi.LA_DTYPE_BF16, total_rows=kv.shape[0] * kv.shape[1], num_seqs=3,
+                      seq_len=kv.shape[1], seq_lens=c.layout.kw["seq_lens"].data_ptr(), nodes=64, parents=c.par.data_ptr(),
+                      q_nope=c.q.data_ptr(), q_rope=c.q.data_ptr() + 2 * 128, q_dtype=capi.LA_DTYPE_BF16,
+                      q_nope_token_stride=128 * 192, q_nope_head_stride=192, q_rope_token_stride=128 * 192,
+                      q_rope_head_stride=192, rotate_q=1, W_UK=c.W_UK.data_ptr(), w_uk_dtype=capi.LA_DTYPE_BF16,
+                      W_UV=c.W_UV.data_ptr(), w_uv_dtype=capi.LA_DTYPE_BF16, rope_cos=c.cos.data_ptr(),
+                      rope_sin=c.sin.data_ptr(), rope_rows=c.cos.shape[0], output=room.data_ptr() + 2 * 3,
+                      out_dtype=capi.LA_DTYPE_BF16, cfg=capi.config(c.cfg))
+    assert lib.la_mla_decode_tree(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == capi.LA_SUCCESS
+    torch.cuda.synchronize()
+    got = room[3:3 + want.numel()].view_as(want)
+    assert_close(got.double().cpu().numpy(), want.double().cpu().numpy(), "bf16")
+    assert (room[:3] == 7).all() and (room[3 + want.numel():] == 7).all()
+
+
+def test_captured_with_many_heads(cuda):
+    """The chunks follow the lengths at every replay: of one long sequence, of equal ones, of none."""
+    c = Case(cuda, "paged", [900, 800, 700, 64], 64, heads=128)
+    par0, lens = c.par.clone(), c.layout.kw["seq_lens"]
+    graph, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    c.run()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=s):
+        got = c.run()
+    for rows in ([900, 800, 700, 64], [900, 0, 0, 0], [100, 100, 100, 64], [0, 0, 0, 0], [70, 800, 63, 64], [900, 800, 700, 64]):
+        lens.copy_(torch.tensor(rows, dtype=torch.int32))
+        graph.replay()
+        eager = c.run()
+        torch.cuda.synchronize()
+        assert torch.equal(got.view(torch.int16), eager.view(torch.int16)), rows
+        short = torch.tensor([n < 64 for n in rows], device=cuda).repeat_interleave(64)
+        assert (got[short] == 0).all() and got.isfinite().all()
+    c.check(got, False)
+    assert torch.equal(c.par, par0)
+
+
 @pytest.mark.parametrize("count,n,heads", [(150, 3, 16), (70, 16, 64), (65, 1, 16), (300, 2, 16), (600, 8, 16)])
 def test_more_sequences_than_lanes(cuda, count, n, heads):
     rows = [(37 * i * i + 11 * i) % 190 for i in range(count)]
