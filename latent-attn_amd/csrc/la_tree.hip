@@ -64,8 +64,8 @@ __device__ inline void plan_spans(const TreeQueries& p) {
     const int n = tiles(s);
     sum += n, have += n > 0;
   }
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-  const int64_t total = sum;
+  // (in two parts: a lane's below 2^40 and so the 64 sums below 2^30)
+  const int64_t total = (int64_t)wave_sum_i((int)min(sum >> 16, (int64_t)1 << 24)) * 65536 + wave_sum_i((int)(sum & 0xFFFF));
   const int filled = wave_sum_i(have);
   constexpr int kMost = kMaxChunkRows / kSpanRows;
   const int even = (int)min(max((total + p.chunks - 1) / p.chunks, (int64_t)p.shortest), (int64_t)kMost);
@@ -77,8 +77,7 @@ __device__ inline void plan_spans(const TreeQueries& p) {
 #pragma unroll
       for (int i = 0; i < kHeld; ++i) count += pieces(held[i], n);
       for (int s = lane + 64 * kHeld; s < seqs; s += 64) count += pieces(tiles(s), n);
-      for (int o = 32; o > 0; o >>= 1) count += __shfl_xor(count, o, 64);
-      return count <= p.chunks;
+      return wave_sum_i((int)min(count, (int64_t)1 << 24)) <= p.chunks;
     };
     int lo = even, hi = min(even + kSegment * ((filled - 1 + p.chunks - 1) / p.chunks), kMost);
     own = fits(hi);
