@@ -1124,8 +1124,10 @@ __global__ __launch_bounds__(kMPWaves * 64, 4) void merge_join_kernel(JoinProble
 // kMSSlots of each and the weights' inputs) on their way during one, and the sequences'
 // places those of the block after it: no load is waited for from a cold start. Of up to
 // four slots the weights are made in the lanes that loaded their inputs, by swaps in
-// groups of four. 16 trees of 16 tokens, 128 heads, 63 MB of slots: 35 us, merge_join_kernel
-// 65; 4 of 64 32 us and 58; 8 of 25, 32 heads, less than two rounds: 27 and 22.
+// groups of four; more are loaded eight at a time. 16 trees of 16 tokens, 128 heads, 63 MB of
+// slots: 35 us, merge_join_kernel 65; 4 of 64 32 us and 58; 8 of 25, 32 heads, 22 and 21. A
+// call over one sequence of 30,000 rows and 15 of 300, 16 x 128 heads 293 and 319 us, 4 x 64
+// heads 67 and 84; 16 of 500, 2 x 128 heads 45 and 47; 2 of 2000, 25 x 64 heads 57 and 56.
 constexpr int kMSSlots = 4;
 template <int kCtrl>
 __device__ inline float quad_swap(float v) {
@@ -1208,10 +1210,17 @@ __global__ __launch_bounds__(kMPWaves * 64, 2) void merge_spans_kernel(JoinProbl
       const bool own = i0 + lane < z.n;
       const int64_t at = z.row0 + (own ? (int64_t)(i0 + lane) * p.Hq : 0);
       const float e = own ? exp2f(p.part_m[at] - mx) * inv : 0.f, lo = e * p.part_scale[2 * at], hi = e * p.part_scale[2 * at + 1];
-      for (int u = 0; u < min(z.n - i0, 64); ++u) {
-        SlotRow<true> d;
-        d.load(part + z.row0 * kDcP + (i0 + u) * stride);
-        d.fma(lane < 32 ? lane_of(lo, u) : lane_of(hi, u), o[0], o[1]);
+      const int n = min(z.n - i0, 64);
+      constexpr int kOnce = 8;  // slots whose loads go out together
+      for (int u0 = 0; u0 < n; u0 += kOnce) {
+        SlotRow<true> d[kOnce];
+#pragma unroll
+        for (int k = 0; k < kOnce; ++k) d[k].load(part + z.row0 * kDcP + (i0 + min(u0 + k, n - 1)) * stride);
+#pragma unroll
+        for (int k = 0; k < kOnce; ++k) {
+          const float w0 = lane_of(lo, min(u0 + k, n - 1)), w1 = lane_of(hi, min(u0 + k, n - 1));
+          if (u0 + k < n) d[k].fma(lane < 32 ? w0 : w1, o[0], o[1]);
+        }
       }
     }
   };
@@ -1562,8 +1571,8 @@ hipError_t launch_merge_join(const JoinProblem& j, hipStream_t stream, int ncu) 
   while (rpb_log2 > 0 && (int64_t)hb * ((R + (1 << rpb_log2) - 1) >> rpb_log2) < ncu) --rpb_log2;
   const int64_t blocks = (int64_t)hb * ((R + (1 << rpb_log2) - 1) >> rpb_log2);
   if (blocks > most_blocks(kMPWaves * 64)) return hipErrorInvalidValue;
-  // a round of merge_join_kernel's workgroups or more, and an output that takes four columns at once
-  if (p.chunk_len == kSpans && j.splits == 0 && j.step[1].num_seqs == 0 && blocks >= 2 * ncu &&
+  // a block of 16 rows for every CU, and an output that takes four columns at once
+  if (p.chunk_len == kSpans && j.splits == 0 && j.step[1].num_seqs == 0 && (int64_t)hb * ((R + kMPRows - 1) / kMPRows) >= ncu &&
       (reinterpret_cast<uintptr_t>(j.out) & 15) == 0) {
     const int shares = std::max(ncu / hb, 1);
     const auto k = p.wuv_dtype == LA_DTYPE_BF16 ? merge_spans_kernel<__hip_bfloat16> : merge_spans_kernel<__half>;
