@@ -372,14 +372,16 @@ __device__ inline bool walk_begin(const DecodeProblem& p, int chunk, int group, 
     w.lo = (int64_t)chunk * len;
     w.hi = min(w.lo + len, span_begin(p, p.num_seqs));
     if (w.lo >= w.hi) return false;
-    w.s = -1;  // the last sequence that begins no later: it has tiles
+    // the last sequence that begins no later, 64 of them tried at a time: it has tiles
     const int lane = wave_lane(), tile = (int)(w.lo / kSpanRows);
-    for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
-      const uint64_t before = __builtin_amdgcn_ballot_w64(s0 + lane < p.num_seqs && first[min(s0 + lane, p.num_seqs)] <= tile);
-      w.s += __builtin_popcountll(before);
-      if (~before) break;
+    w.s = 0;
+    for (int n = p.num_seqs; n > 1;) {
+      const int each = (n + 63) >> 6;
+      const uint64_t before = __builtin_amdgcn_ballot_w64(lane * each < n && first[w.s + min(lane * each, n - 1)] <= tile);
+      const int k = max(__builtin_popcountll(before) - 1, 0) * each;
+      w.s += k;
+      n = min(each, n - k);
     }
-    w.s = max(w.s, 0);
     return true;
   }
   const int64_t end_all = seq_begin(p, p.num_seqs);
