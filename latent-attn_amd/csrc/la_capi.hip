@@ -1603,7 +1603,8 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
       p.count = std::min(most_count, n - j);
       p.seq0 = s;
       p.seqs = std::min(most_seqs, a->num_seqs - s);
-      e = launch_weigh_mfma(p, a->seq_offsets ? all_tiles : seq_tiles * p.seqs, stream, cu_count());
+      p.tiles = (int)(a->seq_offsets ? all_tiles : seq_tiles * p.seqs);
+      e = launch_weigh_mfma(p, stream, cu_count());
     }
   return scratch.finish(status_of(e));
 }

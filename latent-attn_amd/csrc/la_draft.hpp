@@ -110,6 +110,7 @@ struct WeighProblem {
   const void* q_prep;
   int64_t low;
   int spans;       // workgroups that share the tiles of a row group
+  int tiles;       // the piece's at most: `scores` has room for so many (offsets that overlap add up to more rows than there are)
   float* scores;   // [tile][32 rows][32 keys] of `row_blocks` blocks per tile
   float* part;     // [slot][m, l][rows rounded up to 32]
 };
@@ -126,7 +127,7 @@ inline size_t weigh_score_bytes(int64_t tiles, int rows) { return (size_t)tiles 
 inline size_t weigh_part_bytes(int spans, int seqs, int rows) {
   return (size_t)(spans + seqs - 1) * 2 * ((rows + 31) / 32 * 32) * sizeof(float);
 }
-hipError_t launch_weigh_mfma(const WeighProblem& p, int64_t most_tiles, hipStream_t stream, int ncu);
+hipError_t launch_weigh_mfma(const WeighProblem& p, hipStream_t stream, int ncu);
 
 // la_evict_kv.
 struct EvictProblem {  // from: nullptr where no sequence can have more than `keep` rows

@@ -119,7 +119,8 @@ __device__ inline void split(float x, typename Mm<T>::elem& hi, typename Mm<T>::
 
 // Tiles of 32 rows of the piece's sequences, counted over them, shared out evenly:
 // span w of W has [w T / W, (w + 1) T / W), one tile at least (W <= T). The lengths are on the device, so
-// every wave sums them itself.
+// every wave sums them itself. Tiles past p.tiles (of packed sequences whose offsets are not in order) are left out:
+// every index below is below that then.
 struct Spans {
   const WeighProblem& p;
   __device__ int tiles(int i) const {  // of the piece's sequence i
@@ -127,10 +128,11 @@ struct Spans {
   }
   __device__ int total() const {
     int t = 0;
-    for (int i = wave_lane(); i < p.seqs; i += 64) t += tiles(i);
-    return wave_sum_i(t);
+    for (int i = wave_lane(); i < p.seqs; i += 64) t = min(t + tiles(i), p.tiles);
+    return (int)min((uint32_t)wave_sum_i(t), (uint32_t)p.tiles);  // (64 numbers below 2^26)
   }
-  // Sequence of tile t (< total), its first tile and tiles; false only if the lengths change meanwhile.
+  // Sequence of tile t (< total), its first tile and tiles; false only if the lengths change meanwhile. (The sums up to
+  // the first that passes t stay below 2^27.)
   __device__ bool find(int t, int* seq, int* first, int* n) const {
     int before = 0;
     for (int i0 = 0; i0 < p.seqs; i0 += 64) {
@@ -486,7 +488,7 @@ __global__ __launch_bounds__(256) void weigh_sum_kernel(WeighProblem p, int row_
   const int rows = p.count * p.nh;
   while (true) {
     const int s = p.seq0 + i, len = source_rows(p.src, s), end = min(t_end, first + n);
-    const int c0 = Spans::of(first, T_all, W1), c1 = Spans::of(first + n - 1, T_all, W1);
+    const int c0 = Spans::of(first, T_all, W1), c1 = Spans::of(min(first + n, T_all) - 1, T_all, W1);
     __syncthreads();
     for (int r = threadIdx.x; r < 32 * row_blocks; r += 256) {
       float m = kNoScore, l = 0.f;
@@ -640,13 +642,13 @@ int weigh_spans(int rows, int ncu) {  // as many workgroups as run at once
   return groups < most ? most / groups : 1;
 }
 
-hipError_t launch_weigh_mfma(const WeighProblem& p, int64_t most_tiles, hipStream_t stream, int ncu) {
+hipError_t launch_weigh_mfma(const WeighProblem& p, hipStream_t stream, int ncu) {
   const int row_blocks = (p.count * p.nh + 31) / 32;
   hipError_t e = p.src.kv_dtype == LA_DTYPE_FP8_E4M3 ? scores_w<__hip_bfloat16, true>(p, row_blocks, stream)
                  : p.src.kv_dtype == LA_DTYPE_BF16   ? scores_w<__hip_bfloat16, false>(p, row_blocks, stream)
                                                      : scores_w<__half, false>(p, row_blocks, stream);
   if (e != hipSuccess) return e;
-  const int64_t items = row_blocks >= 8 ? most_tiles : (most_tiles + 3) / 4, blocks = items < 8LL * ncu ? items : 8LL * ncu;
+  const int64_t items = row_blocks >= 8 ? p.tiles : ((int64_t)p.tiles + 3) / 4, blocks = items < 8LL * ncu ? items : 8LL * ncu;
   hipLaunchKernelGGL(weigh_sum_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p, row_blocks);
   return hipGetLastError();
 }
