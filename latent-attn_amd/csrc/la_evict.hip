@@ -7,6 +7,7 @@
 // registers up to 16,384 rows), and one pass in order keeps what is larger and as
 // many of the equal ones as are left, earliest first, moving the weights on its
 // way (position i goes to i or before, and a pass's writes follow its reads).
+// Rows are counted in unsigned numbers: up to 2^31 - 1 of them, and as many asked for, the last step passes 2^31.
 // Every wave has consecutive rows, so ranks are ballots and one sum over the waves.
 //
 // Movement: rows only move down, and the columns of a row are independent of
@@ -59,24 +60,25 @@ __global__ __launch_bounds__(64 * kW) void evict_select_kernel(EvictProblem p, i
   const int s = (int)first_seq + blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t begin = moved_begin(p.rows, s);
-  const int L = max(min(p.rows.lens[s], moved_room(p.rows, s)), 0);
+  const uint32_t L = (uint32_t)max(min(p.rows.lens[s], moved_room(p.rows, s)), 0), keep = (uint32_t)p.keep;
   float* const w = p.weights + begin;
   int32_t* const kept = p.kept + (int64_t)s * p.keep;
-  if (L <= p.keep) {
-    for (int i = tid; i < p.keep; i += kThreads) kept[i] = i < L ? i : -1;
+  if (L <= keep) {
+    for (uint32_t i = tid; i < keep; i += kThreads) kept[i] = i < L ? (int32_t)i : -1;
     if (tid == 0) p.start[s] = p.keep;
     return;
   }
   uint32_t* const from = p.from + (int64_t)s * p.keep;
-  const int lo = p.first, hi = L - p.last;  // the rows between
+  const uint32_t lo = p.first, hi = L - p.last;  // the rows between
   int left = p.keep - p.first - p.last;     // of which so many stay
-  const int segments = (L + kSegment - 1) / kSegment;
+  const int segments = (int)((L + kSegment - 1) / kSegment);
   // of segment g a wave has 64 each(g) rows from at(g) on, 64 at a time
-  auto each = [&](int g) { return (min(L - g * kSegment, kSegment) + kThreads - 1) / kThreads; };
-  auto at = [&](int g) { return g * kSegment + wave * 64 * each(g) + lane; };
+  auto each = [&](int g) { return (int)((min(L - g * (uint32_t)kSegment, (uint32_t)kSegment) + kThreads - 1) / kThreads); };
+  auto at = [&](int g) { return g * (uint32_t)kSegment + wave * 64 * each(g) + lane; };
   float x[kItems];
   auto load = [&](int g) {
-    const int n = each(g), i0 = at(g);
+    const int n = each(g);
+    const uint32_t i0 = at(g);
 #pragma unroll
     for (int e = 0; e < kItems; ++e) x[e] = e < n && i0 + 64 * e < L ? w[i0 + 64 * e] : 0.f;
   };
@@ -92,11 +94,12 @@ __global__ __launch_bounds__(64 * kW) void evict_select_kernel(EvictProblem p, i
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
       for (int g = 0; g < segments; ++g) {
         if (segments > 1) load(g);
-        const int n = each(g), i0 = at(g);
+        const int n = each(g);
+        const uint32_t i0 = at(g);
 #pragma unroll
         for (int e = 0; e < kItems; ++e) {
           if (e >= n) break;
-          const int i = i0 + 64 * e;
+          const uint32_t i = i0 + 64 * e;
           const uint32_t k = key_of(x[e]);
           if (i >= lo && i < hi && (pass == 0 || k >> (shift + bits) == prefix >> (shift + bits)))
             atomicAdd(&hist[pass][k >> shift & ((1 << bits) - 1)], 1);
@@ -134,12 +137,13 @@ __global__ __launch_bounds__(64 * kW) void evict_select_kernel(EvictProblem p, i
       load(g);
       __syncthreads();  // the sums of the segment before are read
     }
-    const int n = each(g), i0 = at(g);
+    const int n = each(g);
+    const uint32_t i0 = at(g);
     int same = 0, total;
 #pragma unroll
     for (int e = 0; e < kItems; ++e) {
       if (e >= n) break;
-      const int i = i0 + 64 * e;
+      const uint32_t i = i0 + 64 * e;
       same += __popcll(__builtin_amdgcn_ballot_w64(i >= lo && i < hi && key_of(x[e]) == prefix));
     }
     int rank = equal + wave_rank<kW>(same, sums[3], &total);
@@ -149,7 +153,7 @@ __global__ __launch_bounds__(64 * kW) void evict_select_kernel(EvictProblem p, i
 #pragma unroll
     for (int e = 0; e < kItems; ++e) {
       if (e >= n) break;
-      const int i = i0 + 64 * e;
+      const uint32_t i = i0 + 64 * e;
       const uint32_t k = key_of(x[e]);
       const bool between = i >= lo && i < hi, is = between && k == prefix;
       const uint64_t all = __builtin_amdgcn_ballot_w64(is);
@@ -165,21 +169,21 @@ __global__ __launch_bounds__(64 * kW) void evict_select_kernel(EvictProblem p, i
       if (e >= n) break;
       const bool stay = stays >> e & 1;
       const uint64_t all = __builtin_amdgcn_ballot_w64(stay);
-      const int i = i0 + 64 * e, mine = to + __popcll(all & before);
+      const uint32_t i = i0 + 64 * e, mine = to + __popcll(all & before);
       to += __popcll(all);
       if (stay) {
-        kept[mine] = i;
-        from[mine] = (uint32_t)moved_index(p.rows, s, begin, i);
+        kept[mine] = (int32_t)i;
+        from[mine] = (uint32_t)moved_index(p.rows, s, begin, (int)i);
         if (mine != i) {
           w[mine] = x[e];
-          moves = min(moves, mine);
+          moves = min(moves, (int)mine);
         }
       }
     }
   }
   if (moves < p.keep) atomicMin(&moved, moves);
   __syncthreads();
-  for (int i = p.keep + tid; i < L; i += kThreads) w[i] = 0.f;
+  for (uint32_t i = keep + tid; i < L; i += kThreads) w[i] = 0.f;
   if (tid == 0) {
     p.start[s] = moved;
     p.rows.lens[s] = p.keep;
@@ -198,18 +202,18 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictProblem p
   const int64_t begin = moved_begin(p.rows, s);
   const uint32_t* const from = p.from + (int64_t)s * p.keep;
   const U* const base = reinterpret_cast<const U*>(p.rows.kv) + min(column, units - 1);
-  const int start = p.start[s];
-  if (start >= p.keep) return;
+  const uint32_t start = p.start[s], keep = (uint32_t)p.keep;
+  if (start >= keep) return;
   typedef typename std::conditional<(sizeof(U) < 4), uint32_t, U>::type H;  // (a register each)
-  auto load = [&](int i0, H(&v)[kDeep]) {  // (rows past the last: the last again)
+  auto load = [&](uint32_t i0, H(&v)[kDeep]) {  // (rows past the last: the last again)
 #pragma unroll
-    for (int k = 0; k < kDeep; ++k) v[k] = base[(int64_t)from[min(i0 + k * kRows + row, p.keep - 1)] * units];
+    for (int k = 0; k < kDeep; ++k) v[k] = base[(int64_t)from[min(i0 + k * kRows + row, keep - 1)] * units];
   };
-  auto store = [&](int i0, H(&v)[kDeep]) {
+  auto store = [&](uint32_t i0, H(&v)[kDeep]) {
 #pragma unroll
     for (int k = 0; k < kDeep; ++k) {
-      const int i = i0 + k * kRows + row;
-      if (in && i < p.keep) reinterpret_cast<U*>(moved_row(p.rows, s, begin, i))[column] = (U)v[k];
+      const uint32_t i = i0 + k * kRows + row;
+      if (in && i < keep) reinterpret_cast<U*>(moved_row(p.rows, s, begin, (int)i))[column] = (U)v[k];
     }
   };
   // everyone's rows of a tile are read before anyone writes it
@@ -218,15 +222,15 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictProblem p
     for (int k = 0; k < kDeep; ++k) asm volatile("" : "+v"(v[k]));
     lds_barrier();
   };
-  constexpr int kTile = kRows * kDeep;
+  constexpr uint32_t kTile = kRows * kDeep;
   H a[kDeep], b[kDeep];
   load(start, a);
-  for (int i0 = start; i0 < p.keep; i0 += 2 * kTile) {
-    load(min(i0 + kTile, p.keep - 1), b);
+  for (uint32_t i0 = start; i0 < keep; i0 += 2 * kTile) {
+    load(min(i0 + kTile, keep - 1), b);
     read(a);
     store(i0, a);
-    if (i0 + kTile >= p.keep) break;
-    load(min(i0 + 2 * kTile, p.keep - 1), a);
+    if (i0 + kTile >= keep) break;
+    load(min(i0 + 2 * kTile, keep - 1), a);
     read(b);
     store(i0 + kTile, b);
   }
