@@ -1529,19 +1529,24 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
   const int64_t all_tiles = a->seq_offsets ? a->total_rows / kWeighKeys + a->num_seqs : seq_tiles * a->num_seqs;
   const bool mfma = a->kernel_variant != 1 && weigh_mfma_supported(p) && all_tiles <= INT32_MAX / kWeighKeys;
   if (!mfma && (a->kernel_variant == 2 || !generic_prompt_supported(c.kv_lora_rank, c.qk_rope_head_dim))) return LA_ERROR_NOT_SUPPORTED;
-  // The matrix form keeps the scores between its two kernels: pieces of the call, tokens and
-  // then sequences at a time (packed ones, whose lengths only the device knows, all together).
+  // The matrix form keeps the scores between its two kernels: pieces of the call, some of every
+  // sequence's (token, head) rows and then sequences at a time (packed ones, whose lengths only the
+  // device knows, all together): those of 32 rows at least, of four times as many (the scores'
+  // workgroups) where they fit.
   int64_t most_tiles = 0;
   if (mfma) {
-    p.count = weigh_count(n, nh);
+    p.count = (int)std::min<int64_t>((int64_t)n * nh, kWeighRows);
     p.seqs = a->num_seqs;
     if (!a->seq_offsets && seq_tiles > 0) {
-      const size_t one = weigh_score_bytes(seq_tiles, p.count * nh);
+      const size_t one = weigh_score_bytes(seq_tiles, p.count);
       p.seqs = (int)std::max<int64_t>(1, std::min<int64_t>(p.seqs, kMostScores / one));
     }
     most_tiles = a->seq_offsets ? all_tiles : seq_tiles * p.seqs;
-    while (p.count % 2 == 0 && p.count / 2 * nh % 32 == 0 && weigh_score_bytes(most_tiles, p.count * nh) > kMostScores) p.count /= 2;
-    p.spans = weigh_spans(p.count * nh, cu_count());
+    if (weigh_score_bytes(most_tiles, p.count) > kMostScores) {
+      const size_t blocks = kMostScores / weigh_score_bytes(most_tiles, 32);
+      p.count = 32 * (int)(blocks < 4 ? std::max<size_t>(blocks, 1) : blocks / 4 * 4);
+    }
+    p.spans = weigh_spans(p.count, cu_count());
   }
   const int64_t rows = q.tokens * nh;
   const bool nope_as_is = packed_f32(q.q_nope, q.dtype, q.nope_stride, q.nope_head, nh, c.qk_nope_head_dim);
@@ -1560,8 +1565,8 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
     }
     if (mfma) {
       q_prep = v.take(2 * prep_elems * 2);
-      p.scores = static_cast<float*>(v.take(weigh_score_bytes(most_tiles, p.count * nh)));
-      p.part = static_cast<float*>(v.take(weigh_part_bytes(p.spans, p.seqs, p.count * nh)));
+      p.scores = static_cast<float*>(v.take(weigh_score_bytes(most_tiles, p.count)));
+      p.part = static_cast<float*>(v.take(weigh_part_bytes(p.spans, p.seqs, p.count)));
     } else {
       p.lse = static_cast<float*>(v.take((size_t)rows * sizeof(float)));
     }
@@ -1597,10 +1602,11 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
     e = launch_weigh_queries(p, stream);
   }
   const int most_seqs = p.seqs, most_count = p.count;
-  for (int j = 0; j < n && most_tiles > 0 && e == hipSuccess; j += most_count)
+  const int64_t each = (int64_t)n * nh;
+  for (int64_t j = 0; j < each && most_tiles > 0 && e == hipSuccess; j += most_count)
     for (int s = 0; s < a->num_seqs && e == hipSuccess; s += most_seqs) {
-      p.token0 = j;
-      p.count = std::min(most_count, n - j);
+      p.row0 = (int)j;
+      p.count = (int)std::min<int64_t>(most_count, each - j);
       p.seq0 = s;
       p.seqs = std::min(most_seqs, a->num_seqs - s);
       p.tiles = (int)(a->seq_offsets ? all_tiles : seq_tiles * p.seqs);

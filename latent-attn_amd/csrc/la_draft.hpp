@@ -105,8 +105,8 @@ struct WeighProblem {
   float* lse;  // plain form: (num_seqs * tokens, nh), base 2
   // matrix form: the queries' operands (qprep_index, weigh_query_scale), what their
   // rounding left `low` elements on, and one piece of the call, `seqs` sequences from seq0 on and of
-  // each `count` tokens from token0 on
-  int seq0, seqs, token0, count;
+  // each `count` of its (token, head) rows from row0 on (a multiple of 32)
+  int seq0, seqs, row0, count;
   const void* q_prep;
   int64_t low;
   int spans;       // workgroups that share the tiles of a row group
@@ -119,7 +119,6 @@ hipError_t launch_weigh_plain(const WeighProblem& p, hipStream_t stream);
 // by the tiles (of 32 rows) that its sequences have room for.
 bool weigh_mfma_supported(const WeighProblem& p);
 constexpr int kWeighKeys = 32, kWeighRows = 4096;  // keys per tile; (token, head) rows of a piece at most
-int weigh_count(int tokens, int nh);  // tokens of a piece at most: in whole blocks of 32 rows if they are not all; 0: too many heads
 float weigh_query_scale(const WeighProblem& p);
 hipError_t launch_weigh_queries(const WeighProblem& p, hipStream_t stream);  // q_prep from q_abs and q_rope
 int weigh_spans(int rows, int ncu);

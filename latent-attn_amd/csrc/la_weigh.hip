@@ -320,7 +320,7 @@ __global__ __launch_bounds__(64 * kW, 2) void weigh_scores_kernel(WeighProblem p
   if ((int)(blockIdx.x >> 3) >= per || item >= items) return;
   const int span = item / groups, block = item % groups * kWR + wr;
   const int row = 32 * block + r32;
-  const bool valid = row < p.count * p.nh;
+  const bool valid = row < p.count;
   const Spans sp{p};
   const int T_all = sp.total(), W = min(p.spans, T_all);
   if (span >= W) return;
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(64 * kW, 2) void weigh_scores_kernel(WeighProblem p
     // ---- the queries' operands: [16 k + 8 g .. + 7] of the row, 1 KB per step ----
     vec qh[kC + kR], ql[kC + kR];
     {
-      const int64_t at = (((int64_t)s * qprep_rows_per_seq(p.tokens * p.nh) + p.token0 * p.nh) / 32 + min(block, row_blocks - 1)) * (32 * kQPrepRow);
+      const int64_t at = (((int64_t)s * qprep_rows_per_seq(p.tokens * p.nh) + p.row0) / 32 + min(block, row_blocks - 1)) * (32 * kQPrepRow);
       const elem *const q = static_cast<const elem*>(p.q_prep) + at + 8 * lane, *const low = q + p.low;
 #pragma unroll
       for (int k = 0; k < kC + kR; ++k) {
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(64 * kW, 2) void weigh_scores_kernel(WeighProblem p
       }
     }
     // keys that the row's token sees
-    const int sees = len - p.tokens + p.token0 + row / p.nh + 1;
+    const int sees = len - p.tokens + (int)((uint32_t)(p.row0 + row) / (uint32_t)p.nh) + 1;
     float m = kNoScore, l = 0.f;
     if constexpr (kTwo) {
       stage_store<T>(x, L, wave, lane);
@@ -418,7 +418,7 @@ __global__ __launch_bounds__(64 * kW, 2) void weigh_scores_kernel(WeighProblem p
       }
       const int key0 = kWeighKeys * (u - first) + 2 * kN * kd + 4 * g;
       const int most = min(len, sees) - key0;
-      if (kWeighKeys * (u - first + 1) > len - p.tokens + p.token0 + 1) {
+      if (kWeighKeys * (u - first + 1) > len - p.tokens + p.row0 / p.nh + 1) {
 #pragma unroll
         for (int e = 0; e < kN; ++e)
           if (8 * (e >> 2) + (e & 3) >= most) sc[e] = -INFINITY;
@@ -485,7 +485,7 @@ __global__ __launch_bounds__(256) void weigh_sum_kernel(WeighProblem p, int row_
   const int t_end = Spans::begin(w + 1, T_all, W);
   int i, first, n;
   if (!sp.find(t, &i, &first, &n)) return;
-  const int rows = p.count * p.nh;
+  const int rows = p.count;
   while (true) {
     const int s = p.seq0 + i, len = source_rows(p.src, s), end = min(t_end, first + n);
     const int c0 = Spans::of(first, T_all, W1), c1 = Spans::of(min(first + n, T_all) - 1, T_all, W1);
@@ -622,15 +622,8 @@ hipError_t launch_weigh_plain(const WeighProblem& p, hipStream_t stream) {
   return e;
 }
 
-int weigh_count(int tokens, int nh) {
-  if ((int64_t)tokens * nh <= kWeighRows) return tokens;
-  int whole = 1;  // tokens of whole blocks of 32 rows
-  while (whole * nh % 32 != 0) whole *= 2;
-  return kWeighRows / nh / whole * whole;
-}
-
 bool weigh_mfma_supported(const WeighProblem& p) {
-  if (p.src.kv_dtype == LA_DTYPE_F32 || p.dc != 512 || p.dR != 64 || weigh_count(p.tokens, p.nh) < 1) return false;
+  if (p.src.kv_dtype == LA_DTYPE_F32 || p.dc != 512 || p.dR != 64) return false;
   // 16-byte loads of rows and tables
   if (((reinterpret_cast<uintptr_t>(p.src.kv) | reinterpret_cast<uintptr_t>(p.src.cos) | reinterpret_cast<uintptr_t>(p.src.sin)) & 15) != 0)
     return false;
@@ -643,7 +636,7 @@ int weigh_spans(int rows, int ncu) {  // as many workgroups as run at once
 }
 
 hipError_t launch_weigh_mfma(const WeighProblem& p, hipStream_t stream, int ncu) {
-  const int row_blocks = (p.count * p.nh + 31) / 32;
+  const int row_blocks = (p.count + 31) / 32;
   hipError_t e = p.src.kv_dtype == LA_DTYPE_FP8_E4M3 ? scores_w<__hip_bfloat16, true>(p, row_blocks, stream)
                  : p.src.kv_dtype == LA_DTYPE_BF16   ? scores_w<__hip_bfloat16, false>(p, row_blocks, stream)
                                                      : scores_w<__half, false>(p, row_blocks, stream);

@@ -1,4 +1,4 @@
-"""weigh_kv at the edges of its arguments' ranges: offsets that are not in order."""
+"""weigh_kv at the edges of its arguments' ranges: offsets that are not in order, rooms far wider than their rows."""
 
 from __future__ import annotations
 
@@ -8,10 +8,13 @@ import pytest
 import torch
 
 from prompt_cases import tables, weights
+from test_gpu_weigh import Case
 
 from latent_attn import MLAConfig, capi
 
 pytestmark = pytest.mark.gpu
+
+MiB = 1 << 20
 
 
 @pytest.mark.parametrize("tokens,heads", [(1, 16), (4, 128)])
@@ -43,3 +46,46 @@ def test_packed_offsets_that_are_not_in_order(cuda, tokens, heads, variant, orde
         assert lib.la_weigh_kv(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == capi.LA_SUCCESS
     torch.cuda.synchronize()
     assert (ws[need:] == 0xFF).all() and (w[rows:] == 0).all()
+
+
+def in_room(c, room, packed):
+    """The case's sequences at the front of regions of `room` rows (packed: of one cache with offsets that far apart)."""
+    count, device = len(c.rows), c.q.device
+    kv = torch.zeros(count, room, 576, dtype=c.layout.kv.dtype, device=device)
+    kv[:, :c.layout.kv.shape[1]] = c.layout.kv
+    c.layout.kv = kv
+    if packed:
+        c.layout.kv = kv.view(-1, 576)
+        c.layout.kw["seq_offsets"] = torch.arange(count + 1, dtype=torch.int32, device=device) * room
+    c.weights = torch.rand(*(c.layout.kv.shape[:1] if packed else (count, room)), device=device)
+    c.cos, c.sin = (x.to(device) for x in tables(room))
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("tokens,heads,room,pieces", [(31, 128, 131072, 8), (5, 128, 1 << 20, 10), (7, 127, 400000, 7), (3, 129, 131072, 1)])
+def test_windows_in_wide_rooms(cuda, packed, tokens, heads, room, pieces):
+    """Windows of any number of tokens in several pieces, which may end between a token's heads."""
+    c = Case(cuda, "capacity", [tokens + 90, 200], tokens, heads=heads, kv=torch.float8_e4m3fn, seed=tokens)
+    in_room(c, room, packed)
+    c.check(2, (tokens, heads, room, packed), pieces)
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 7, 8, 31, 32, 33, 100])
+@pytest.mark.parametrize("heads", [1, 16, 65, 127, 128, 129, 5000])
+@pytest.mark.parametrize("room", [131072, 1 << 20, 40 << 20])
+@pytest.mark.parametrize("packed", [False, True])
+def test_scores_take_no_more_than_they_may(cuda, tokens, heads, room, packed):
+    """512 MiB of scores at a time, or those of 32 (token, head) rows: 128 B per row of room (packed: and 4 KiB per
+    sequence). The rest: two 16-bit parts of 576 elements per query row, their rows in whole 32 per sequence, and for up to
+    512 workgroups and 4 sequences partial sums of 8 B for 4096 rows at most."""
+    lib, seqs, fake = capi.load(), 4, 1 << 12
+    a = capi.WeighArgs(kv_cache=fake, kv_dtype=capi.LA_DTYPE_BF16, total_rows=seqs * room, num_seqs=seqs, seq_len=room, seq_lens=fake,
+                       tokens_per_seq=tokens, q_nope=fake, q_rope=fake, q_dtype=capi.LA_DTYPE_BF16, rotate_q=1, W_UK=fake,
+                       w_uk_dtype=capi.LA_DTYPE_BF16, rope_cos=fake, rope_sin=fake, rope_rows=room, weights=fake,
+                       cfg=capi.config(MLAConfig(5120, 512, 128, 64, heads, 128)), kernel_variant=2)
+    if packed:
+        a.seq_len, a.seq_offsets = 0, fake
+    need = lib.la_weigh_kv_workspace_size(ctypes.byref(a))
+    queries = seqs * -(-tokens * heads // 32) * 32 * 2 * 576 * 2
+    least = 128 * seqs * room + 4096 * seqs if packed else 128 * room
+    assert 0 < need <= max(512 * MiB, least) + queries + 516 * 4096 * 8 + 4096
