@@ -443,9 +443,7 @@ typedef struct la_weigh_args {
    * s * seq_len + p (equal regions), seq_offsets[s] + p, or s *
    * blocks_per_seq * block_size + p (paged). Entries past a sequence's rows
    * are left as they are. A row that is not finite makes its own sequence's
-   * weights NaN. On the matrix cores an fp16 cache takes absorbed queries whose
-   * elements, times log2(e) / sqrt(qk_nope_head_dim + qk_rope_head_dim), stay
-   * within 65504 / 64. */
+   * weights NaN. */
   float* weights;
   la_mla_config cfg;
   void* workspace; /* la_weigh_kv_workspace_size bytes; NULL: taken stream-ordered (not under capture) */

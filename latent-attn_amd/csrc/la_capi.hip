@@ -1448,7 +1448,7 @@ int decode_tree(const la_tree_args* a, void* stream_v, bool run_it, size_t* need
   StepTail tail;
   tail.merge = !join;
   tail.tree = TreeStep{t.seen, t.cos, t.sin};
-  const AbsorbQueries x{t.q, t.src, t.pos, 0};
+  const AbsorbQueries x{t.q, t.src, t.pos, 0, nullptr};
   if (direct) tail.queries = &x;
   int st = run(&d, stream, nullptr, nullptr, 1, false, &tail);
   if (st == LA_SUCCESS && join) {
@@ -1555,7 +1555,7 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
   float* q_abs = nullptr;
   void* q_prep = nullptr;
   const bool direct = mfma && absorb_any_supported(q, p.src, a->W_UK, a->w_uk_dtype, c);
-  const size_t prep_elems = (size_t)a->num_seqs * qprep_rows_per_seq(n * nh) * kQPrepRow;
+  const size_t prep_rows = (size_t)a->num_seqs * qprep_rows_per_seq(n * nh), prep_elems = prep_rows * kQPrepRow;
   auto carve = [&](void* ws) {
     Carve v(ws);
     if (!direct) {
@@ -1565,6 +1565,7 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
     }
     if (mfma) {
       q_prep = v.take(2 * prep_elems * 2);
+      if (a->kv_dtype == LA_DTYPE_F16) p.most = static_cast<uint8_t*>(v.take(kMostRow * prep_rows));
       p.scores = static_cast<float*>(v.take(weigh_score_bytes(most_tiles, p.count)));
       p.part = static_cast<float*>(v.take(weigh_part_bytes(p.spans, p.seqs, p.count)));
     } else {
@@ -1582,7 +1583,7 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
   p.low = (int64_t)prep_elems;
   hipError_t e = hipSuccess;
   if (direct) {
-    const AbsorbQueries x{q, p.src, nullptr, p.low};
+    const AbsorbQueries x{q, p.src, nullptr, p.low, p.most};
     e = launch_absorb_any(x, a->W_UK, a->w_uk_dtype, q_prep, a->kv_dtype == LA_DTYPE_F16 ? 2 : 1, weigh_query_scale(p), nh, stream, cu_count());
   } else {
     t.q = q;

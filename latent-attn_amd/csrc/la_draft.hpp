@@ -109,6 +109,7 @@ struct WeighProblem {
   int seq0, seqs, row0, count;
   const void* q_prep;
   int64_t low;
+  uint8_t* most;  // fp16: the exponents of the operands' pieces (AbsorbQueries)
   int spans;       // workgroups that share the tiles of a row group
   int tiles;       // the piece's at most: `scores` has room for so many (offsets that overlap add up to more rows than there are)
   float* scores;   // [tile][32 rows][32 keys] of `row_blocks` blocks per tile

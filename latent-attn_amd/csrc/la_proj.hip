@@ -339,7 +339,8 @@ struct Eight {
   }
   __device__ float at(int e) const { return (float)v[e >> 2][e & 3]; }
 };
-template <typename WT, typename QT>
+// kFit: any.most.
+template <typename WT, typename QT, bool kFit>
 __global__ __launch_bounds__(kAbsThreads, 4) void absorb_any_kernel(AbsorbQueries any, const WT* __restrict__ W,
                                                                     void* __restrict__ out, int out_mode, float scale,
                                                                     int tokens, int nh, int qps, int shares,
@@ -454,13 +455,23 @@ __global__ __launch_bounds__(kAbsThreads, 4) void absorb_any_kernel(AbsorbQuerie
     // register 4 q + r: column 32 (wave % 4) + 8 q + 4 (lane / 32) + r of token lane % 32
     const int tt = t0 + 32 * (wave >> 2) + (lane & 31);
     const int64_t to = row_of(tt);
+    float fit = 1.f;
+    if constexpr (kFit) {  // of the wave's 32 columns, by both halves' lanes
+      float m = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf((acc_hi[r] + acc_lo[r] * (1.f / M::kLoScale)) * scale));
+      const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, m), __builtin_bit_cast(uint32_t, m), false, false);
+      const int e = exponent_of(fmaxf(f_of(both[0]), f_of(both[1])));
+      if (tt < tokens && lane < 32) any.most[to * kMostRow + 4 * cb + (wave & 3)] = (uint8_t)e;
+      fit = power_of_2(-fit_f16(e));
+    }
 #pragma unroll
     for (int q2 = 0; q2 < 4; q2 += 2) {
       float v[8];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float a = (acc_hi[4 * q2 + r] + acc_lo[4 * q2 + r] * (1.f / M::kLoScale)) * scale;
-        const float b = (acc_hi[4 * q2 + 4 + r] + acc_lo[4 * q2 + 4 + r] * (1.f / M::kLoScale)) * scale;
+        const float a = (acc_hi[4 * q2 + r] + acc_lo[4 * q2 + r] * (1.f / M::kLoScale)) * scale * fit;
+        const float b = (acc_hi[4 * q2 + 4 + r] + acc_lo[4 * q2 + 4 + r] * (1.f / M::kLoScale)) * scale * fit;
         const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
         v[r] = f_of(both[0]), v[4 + r] = f_of(both[1]);
       }
@@ -489,6 +500,17 @@ __global__ __launch_bounds__(kAbsThreads, 4) void absorb_any_kernel(AbsorbQuerie
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = own.at(e) * scale;
+      }
+      if constexpr (kFit) {  // of the eight lanes that have the token's rope part
+        float m = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[e] *= kUpRope));
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        if (tr < tokens && rj == 0) any.most[row_of(tr) * kMostRow + kMostPieces - 1] = (uint8_t)exponent_of(m);
+        const float fit = power_of_2(-fit_f16(exponent_of(m)));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= fit;
       }
       if (tr < tokens) {
         const int64_t at = qprep_index(row_of(tr), 512 + rj);
@@ -1449,8 +1471,9 @@ hipError_t launch_absorb_any(const AbsorbQueries& x, const void* W_UK, int w_dty
   const dim3 grid((unsigned)(64 * (512 / kAbsCols) * ((shares * nh8 + 7) / 8)));
   auto launch = [&](auto w, auto qt) {
     typedef decltype(w) WT;
-    hipLaunchKernelGGL((absorb_any_kernel<WT, decltype(qt)>), grid, dim3(kAbsThreads), 0, stream, x, static_cast<const WT*>(W_UK),
-                       out, out_mode, scale, tokens, nh, x.q.per_seq, shares, zero_out, zero_n);
+    const auto kernel = x.most ? absorb_any_kernel<WT, decltype(qt), true> : absorb_any_kernel<WT, decltype(qt), false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(kAbsThreads), 0, stream, x, static_cast<const WT*>(W_UK), out, out_mode, scale, tokens,
+                       nh, x.q.per_seq, shares, zero_out, zero_n);
   };
   auto by_query = [&](auto w) {
     if (x.q.dtype == LA_DTYPE_F32) launch(w, float());

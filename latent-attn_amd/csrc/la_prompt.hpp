@@ -320,7 +320,18 @@ struct AbsorbQueries {
   RowSource src;       // positions: token j of n of a sequence with L rows is at L - n + j
   const int32_t* pos;  // or given (device, one per token)
   int64_t low;         // > 0: also what the rounded rows leave, in a second array so many elements on
+  uint8_t* most;       // fp16 parts of any queries: (rows, kMostRow), exponents of the pieces' largest numbers (fit_f16); or nullptr
 };
+// Two fp16 parts of a row of queries. Its pieces of 32 latent columns, and its rope part (which comes doubled, for keys in
+// halves), are each divided by a power of two that goes by their largest number m (as exponent_of has it): 1 for m from
+// 2^-6 on below 2^15, where two parts hold it to 2^-19 or better (and where it is not finite), else the one that brings it to
+// 2^14. top_f16 and fit_f16 are those powers' exponents without and with the first case.
+constexpr int kMostPieces = 17, kMostRow = 20;
+constexpr float kUpRope = 2.f;
+__device__ inline int exponent_of(float m) { return (int)(__builtin_bit_cast(uint32_t, m) >> 23); }  // m >= 0
+__device__ inline float power_of_2(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
+__device__ inline int top_f16(int e) { return e == 255 ? 0 : max(e, 27) - 127 - 14; }
+__device__ inline int fit_f16(int e) { return e >= 127 - 6 && e < 127 + 15 ? 0 : top_f16(e); }
 bool absorb_any_supported(const QuerySource& q, const RowSource& r, const void* W_UK, int w_dtype, const la_mla_config& c);
 // out_mode 1: bf16, 2: fp16; zero_out as for launch_absorb_mfma.
 hipError_t launch_absorb_any(const AbsorbQueries& x, const void* W_UK, int w_dtype, void* out, int out_mode, float scale,

@@ -88,16 +88,23 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lchar;
 
-// Two parts of a value in the products' type: hi + lo. Queries come times kUp: what
-// is left of an fp16 number's 11 bits would be subnormal in small ones (they may
-// reach 65504 / kUp, as scaled for the softmax).
+// Two parts of a value in the products' type: hi + lo. fp16 has more bits than bf16 and a
+// narrow range, so there
+// - queries come times kUp, and the pieces of a row (32 latent columns, the rope part) that are
+//   too large or too small then are divided by powers of two (fit_f16). When the products' operands of
+//   such a row are loaded they are brought to one divisor, which leaves the row's largest element near
+//   fp16's and is taken off the scores: any queries that fp32 holds will do (elements below 2^-22 of a
+//   row's largest lose bits of 2^-18 of them);
+// - rotated keys come in halves (they reach sqrt(2) times the largest fp16 number) and what is
+//   left of them times kLow, against queries divided by it: it would be subnormal, or nothing, in
+//   small keys.
 template <typename T>
 struct Mm;
 template <>
 struct Mm<__hip_bfloat16> {
   typedef bf16x8 vec;
   typedef __bf16 elem;
-  static constexpr float kUp = 1.f;
+  static constexpr float kUp = 1.f, kKey = 1.f, kLow = 1.f;
   static __device__ inline f32x16 mma(vec a, vec b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -106,15 +113,15 @@ template <>
 struct Mm<__half> {
   typedef f16x8 vec;
   typedef _Float16 elem;
-  static constexpr float kUp = 64.f;
+  static constexpr float kUp = 64.f, kKey = 1.f / kUpRope, kLow = 2048.f;
   static __device__ inline f32x16 mma(vec a, vec b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
 };
 template <typename T>
-__device__ inline void split(float x, typename Mm<T>::elem& hi, typename Mm<T>::elem& lo) {
+__device__ inline void split(float x, typename Mm<T>::elem& hi, typename Mm<T>::elem& lo, float low = 1.f) {
   hi = (typename Mm<T>::elem)x;
-  lo = (typename Mm<T>::elem)(x - (float)hi);
+  lo = (typename Mm<T>::elem)((x - (float)hi) * low);
 }
 
 // Tiles of 32 rows of the piece's sequences, counted over them, shared out evenly:
@@ -214,7 +221,9 @@ __device__ inline void stage_load(const WeighProblem& p, const Rows& r, Staged<k
                         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, S::kLR * i);
     x.c[i] = reinterpret_cast<const typename S::cvec*>(kv + row)[lane];
   }
-  const char* const rope = kv + at + (kFp8 ? 512 : 1024) + sizeof(typename S::kvec) * (lane % S::kLR);
+  int part = lane;
+  asm volatile("" : "+v"(part));  // (the address with it, held through the tiles' loop, was spilled)
+  const char* const rope = kv + at + (kFp8 ? 512 : 1024) + sizeof(typename S::kvec) * (part % S::kLR);
   x.ka = *reinterpret_cast<const typename S::kvec*>(rope);
   x.kb = *reinterpret_cast<const typename S::kvec*>(rope + (kFp8 ? 32 : 64));
   const int64_t rp = source_rope_row(p.src, pos) * 32 + S::kP * (lane % S::kLR);
@@ -260,9 +269,9 @@ __device__ inline void stage_store(const Staged<kFp8, kW>& x, lchar* L, int wave
   for (int e = 0; e < S::kP; ++e) {
     const float a = value(x.ka, e), b = value(x.kb, e);
     elem h, l;
-    split<T>(a * x.cs[e] - b * x.sn[e], h, l);
+    split<T>((a * x.cs[e] - b * x.sn[e]) * Mm<T>::kKey, h, l, Mm<T>::kLow);
     ah[e] = h, al[e] = l;
-    split<T>(a * x.sn[e] + b * x.cs[e], h, l);
+    split<T>((a * x.sn[e] + b * x.cs[e]) * Mm<T>::kKey, h, l, Mm<T>::kLow);
     bh[e] = h, bl[e] = l;
   }
   const int row = S::kS * wave + lane / S::kLR, i0 = S::kP * (lane % S::kLR);
@@ -308,11 +317,15 @@ __global__ __launch_bounds__(64 * kW, 2) void weigh_scores_kernel(WeighProblem p
   constexpr int kN = 16 / kKD;            // scores of a lane after the sum
   constexpr bool kTwo = kW == 8;          // two buffers of a tile and of its sums: one barrier a tile
   constexpr int kSums = weigh_sums(kWR, kW);
+  constexpr bool kFit = Mm<T>::kUp != 1.f;
   static_assert(kKD == 2 || kKD == 4, "the waves meet at the sums, behind a tile's last read");
   extern __shared__ __attribute__((aligned(1024))) char weigh_lds[];
   lchar* const L = (lchar*)weigh_lds;
   lchar* const sums0 = L + (kTwo ? 2 : 1) * kTile;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  // what a row's products are multiplied by (in LDS, a word per row and wave: a register more is spilled)
+  typedef __attribute__((address_space(3))) float lfloat;
+  lfloat* const back = reinterpret_cast<lfloat*>(sums0 + (kTwo ? 2 : 1) * kSums) + 32 * wave + (lane & 31);
   const int wr = wave % kWR, kd = wave / kWR, r32 = lane & 31, g = lane >> 5;
   // an eighth of the items to each XCD, row groups of a span together
   const int groups = (row_blocks + kWR - 1) / kWR, items = p.spans * groups, per = (items + 7) / 8;
@@ -348,6 +361,35 @@ __global__ __launch_bounds__(64 * kW, 2) void weigh_scores_kernel(WeighProblem p
         ql[k] = *reinterpret_cast<const vec*>(low + step);
       }
     }
+    if constexpr (kFit) {
+      typedef uint32_t words __attribute__((ext_vector_type(4), aligned(4)));
+      const uint8_t* const pieces = p.most + ((int64_t)s * qprep_rows_per_seq(p.tokens * p.nh) + p.row0 + min(row, p.count - 1)) * kMostRow;
+      const words first = *reinterpret_cast<const words*>(pieces);
+      const uint32_t last = pieces[16];
+      auto piece = [&](int k) { return k < 16 ? (int)(first[k >> 2] >> (8 * (k & 3)) & 255) : (int)last; };
+      int most = 0;
+      bool fits = true;
+#pragma unroll
+      for (int k = 0; k < kMostPieces; ++k) {
+        most = max(most, piece(k));
+        fits = fits && fit_f16(piece(k)) == 0;
+      }
+      const int by = fits ? 0 : top_f16(most);
+      *back = power_of_2(by) * (1.f / Mm<T>::kUp);  // (the same from both halves' lanes)
+      if (__builtin_amdgcn_ballot_w64(!fits) != 0) {
+        const uint32_t* const own = reinterpret_cast<const uint32_t*>(pieces + kC / 2 * kd);
+#pragma unroll
+        for (int k = 0; k < kC + kR; ++k) {
+          const int e = fit_f16(k < kC ? (int)(own[k / 8] >> (8 * (k / 2 & 3)) & 255) : (int)last) - by;
+          const int e1 = min(max(e, -14), 14);  // in two steps, each a power of two that fp16 holds (or what is left is nothing)
+          const elem f1 = (elem)power_of_2(e1), f2 = (elem)power_of_2(max(e - e1, -100));
+          qh[k] = qh[k] * f1 * f2;
+          ql[k] = ql[k] * f1 * f2;
+        }
+      }
+    }
+    int own_score = 32 * r32 + 2 * kN * kd + 4 * g;  // of a tile's
+    asm volatile("" : "+v"(own_score));  // (the address with it, made before the operands, was spilled)
     // keys that the row's token sees
     const int sees = len - p.tokens + (int)((uint32_t)(p.row0 + row) / (uint32_t)p.nh) + 1;
     float m = kNoScore, l = 0.f;
@@ -366,6 +408,8 @@ __global__ __launch_bounds__(64 * kW, 2) void weigh_scores_kernel(WeighProblem p
       const lchar* const b = L + (kTwo ? (u - t) & 1 : 0) * kTile;
       lchar* const sums = sums0 + (kTwo ? (u - t) & 1 : 0) * kSums;
       f32x16 acc = {};
+      uint32_t below = __builtin_bit_cast(uint16_t, (elem)(1.f / Mm<T>::kLow));
+      asm volatile("" : "+s"(below));  // (the products with it, made before the loop, were spilled)
       auto operand = [&](int k) -> vec {  // keys r32, elements [16 k + 8 g .. + 7]
         const int at = k < kC ? row_at(r32) + 32 * (kC * kd + k) + 16 * g
                        : k < kC + kR ? kRopeHi + rope_piece(r32, 2 * (kR * kd + k - kC) + g)
@@ -380,13 +424,15 @@ __global__ __launch_bounds__(64 * kW, 2) void weigh_scores_kernel(WeighProblem p
       for (int k = 0; k < kSteps; ++k) {
         const vec v = a[k % kAhead];
         if (k < kC + kR) acc = Mm<T>::mma(v, ql[k], acc);
-        acc = Mm<T>::mma(v, qh[k < kC + kR ? k : k - kR], acc);
+        if (k < kC + kR) acc = Mm<T>::mma(v, qh[k], acc);
+        else acc = Mm<T>::mma(v, kFit ? qh[k - kR] * __builtin_bit_cast(elem, (uint16_t)below) : qh[k - kR], acc);
         if (k + kAhead < kSteps) a[k % kAhead] = operand(k + kAhead);
         __builtin_amdgcn_sched_barrier(0);
       }
       settle(acc);
       // lane: row r32, keys 8 (e / 4) + 4 g + e % 4; this share's are quads kN / 4 kd and on
       float sc[kN];
+      const float to_score = kFit ? *back : 1.f;
       auto quad = [&](int q) {
         return f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
       };
@@ -400,7 +446,7 @@ __global__ __launch_bounds__(64 * kW, 2) void weigh_scores_kernel(WeighProblem p
         for (int q = 0; q < 2; ++q) {
           const f32x4 v = *reinterpret_cast<const lvec*>(its + 1024 * q), own = kd == 0 ? quad(q) : quad(2 + q);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[4 * q + e] = (own[e] + v[e]) * (1.f / Mm<T>::kUp);
+          for (int e = 0; e < 4; ++e) sc[4 * q + e] = (own[e] + v[e]) * to_score;
         }
       } else {
 #pragma unroll
@@ -413,7 +459,7 @@ __global__ __launch_bounds__(64 * kW, 2) void weigh_scores_kernel(WeighProblem p
           for (int w = 0; w < kKD; ++w)
             v += *reinterpret_cast<const lvec*>(sums + 4096 * (wr + kWR * w) + 1024 * (kN / 4 * kd + q) + 16 * lane);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[4 * q + e] = v[e] * (1.f / Mm<T>::kUp);
+          for (int e = 0; e < 4; ++e) sc[4 * q + e] = v[e] * to_score;
         }
       }
       const int key0 = kWeighKeys * (u - first) + 2 * kN * kd + 4 * g;
@@ -433,7 +479,7 @@ __global__ __launch_bounds__(64 * kW, 2) void weigh_scores_kernel(WeighProblem p
       l = l * __builtin_amdgcn_exp2f(m - up) + sum;
       m = up;
       if (valid) {
-        float* const to = p.scores + ((int64_t)u * row_blocks + block) * 1024 + 32 * r32 + 2 * kN * kd + 4 * g;
+        float* const to = p.scores + ((int64_t)u * row_blocks + block) * 1024 + own_score;
 #pragma unroll
         for (int q = 0; q < kN / 4; ++q)
           *reinterpret_cast<f32x4*>(to + 8 * q) = f32x4{sc[4 * q], sc[4 * q + 1], sc[4 * q + 2], sc[4 * q + 3]};
@@ -451,7 +497,6 @@ __global__ __launch_bounds__(64 * kW, 2) void weigh_scores_kernel(WeighProblem p
       const auto sl = __builtin_amdgcn_permlane32_swap(u_of(l), u_of(l), false, false);
       m = f_of(sm[0]), l = f_of(sl[0]);
       join(f_of(sm[1]), f_of(sl[1]));
-      typedef __attribute__((address_space(3))) float lfloat;
       lfloat* const ml = reinterpret_cast<lfloat*>(sums0) + 64 * wave;
       if (g == 0) ml[r32] = m, ml[32 + r32] = l;
       lds_barrier();
@@ -461,7 +506,9 @@ __global__ __launch_bounds__(64 * kW, 2) void weigh_scores_kernel(WeighProblem p
         if (kd == 0) join(o[r32], o[32 + r32]);
       }
       if (kd == 0 && g == 0 && block < row_blocks) {
-        float* const to = p.part + (int64_t)(span + i) * 2 * 32 * row_blocks + 32 * block + r32;
+        int r = r32;
+        asm volatile("" : "+v"(r));  // (the address, made before the loop, was spilled)
+        float* const to = p.part + (int64_t)(span + i) * 2 * 32 * row_blocks + 32 * block + r;
         to[0] = m;
         to[32 * row_blocks] = l;
       }
@@ -558,7 +605,7 @@ __global__ __launch_bounds__(256) void weigh_sum_kernel(WeighProblem p, int row_
 
 template <typename T, bool kFp8, int kWR, int kW>
 hipError_t scores_t(const WeighProblem& p, int row_blocks, hipStream_t stream) {
-  constexpr int lds = (kW == 8 ? 2 : 1) * (kTile + weigh_sums(kWR, kW));
+  constexpr int lds = (kW == 8 ? 2 : 1) * (kTile + weigh_sums(kWR, kW)) + (Mm<T>::kUp != 1.f ? 128 * kW : 0);
   static OncePerDevice once;
   const auto k = weigh_scores_kernel<T, kFp8, kWR, kW>;
   const hipError_t e = allow_lds(once, reinterpret_cast<const void*>(k), lds);
@@ -574,21 +621,39 @@ hipError_t scores_w(const WeighProblem& p, int row_blocks, hipStream_t stream) {
   return scores_t<T, kFp8, 4, 8>(p, row_blocks, stream);
 }
 
-// Queries' operands from absorbed fp32 ones, where the absorption does not write them: 8 elements of a row per thread.
+// Queries' operands from absorbed fp32 ones, where the absorption does not write them: 8 elements of a row per thread, the
+// 4 of a piece (8 of the rope part) next to one another in a wave.
 template <typename T>
 __global__ __launch_bounds__(256) void weigh_queries_kernel(WeighProblem p, int64_t first) {
   typedef typename Mm<T>::elem elem;
   const int64_t n = (int64_t)p.src.num_seqs * p.tokens * p.nh * (kQPrepRow / 8), i = (first + blockIdx.x) * 256 + threadIdx.x;
-  if (i >= n) return;
+  if (i >= n) return;  // (whole rows)
   const int64_t row = i / (kQPrepRow / 8);
   const int j = 8 * (int)(i % (kQPrepRow / 8)), each = p.tokens * p.nh;
   const float* const from = j < 512 ? p.q_abs + row * 512 + j : p.q_rope + row * 64 + j - 512;
   const int64_t at = qprep_index(row / each * qprep_rows_per_seq(each) + row % each, j);
   elem* const to = static_cast<elem*>(const_cast<void*>(p.q_prep)) + at;
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = from[e] * (p.scale_log2 * Mm<T>::kUp) * (j < 512 ? 1.f : 1.f / Mm<T>::kKey);
+  if constexpr (Mm<T>::kUp != 1.f) {
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[e]));
+    m = fmaxf(m, __shfl_xor(m, 1, 64));
+    m = fmaxf(m, __shfl_xor(m, 2, 64));
+    const float wide = __shfl_xor(m, 4, 64);
+    if (j >= 512) m = fmaxf(m, wide);
+    if (j < 512 ? j % 32 == 0 : j == 512)
+      p.most[(row / each * qprep_rows_per_seq(each) + row % each) * kMostRow + j / 32] = (uint8_t)exponent_of(m);
+    const float fit = power_of_2(-fit_f16(exponent_of(m)));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= fit;
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     elem h, l;
-    split<T>(from[e] * (p.scale_log2 * Mm<T>::kUp), h, l);
+    split<T>(v[e], h, l);
     to[e] = h;
     to[p.low + e] = l;
   }

@@ -501,8 +501,6 @@ def weigh_kv(
                      rows is at position L - n + j and sees the rows up to its own
         rotate_q:    q_rope is not rotated yet
         kernel_variant: 0 = automatic, 1 = plain kernels, 2 = matrix cores
-                     (an fp16 cache: absorbed queries, times
-                     log2(e) / sqrt(qk_nope_head_dim + qk_rope_head_dim), up to 65504 / 64)
 
     A row that is not finite makes its own sequence's weights NaN.
     """

@@ -1,4 +1,5 @@
-"""weigh_kv at the edges of its arguments' ranges: offsets that are not in order, rooms far wider than their rows."""
+"""weigh_kv at the edges of its arguments' ranges: offsets that are not in order, rooms far wider than their rows,
+queries outside fp16's range over an fp16 cache."""
 
 from __future__ import annotations
 
@@ -7,6 +8,7 @@ import ctypes
 import pytest
 import torch
 
+from draft_cases import places
 from prompt_cases import tables, weights
 from test_gpu_weigh import Case
 
@@ -89,3 +91,38 @@ def test_scores_take_no_more_than_they_may(cuda, tokens, heads, room, packed):
     queries = seqs * -(-tokens * heads // 32) * 32 * 2 * 576 * 2
     least = 128 * seqs * room + 4096 * seqs if packed else 128 * room
     assert 0 < need <= max(512 * MiB, least) + queries + 516 * 4096 * 8 + 4096
+
+
+def large(c, what, up):
+    """Queries far past fp16's range (or far below one) over rows that are as much smaller (larger), so that scores stay where
+    they were: all of them, one latent column in every head, the rope part, or a few heads' (whose scores move then)."""
+    q, kv = c.q.clone(), c.layout.kv.float()
+    if what == "all":
+        q, kv = q * up, kv / up
+    elif what == "column":
+        c.W_UK[:, 100] *= up
+        kv[..., 100] /= up
+    elif what == "rope":
+        q[..., 128:] *= up
+        kv[..., 512:] /= up
+    elif what == "edge":  # keys that pass fp16's range when they are rotated
+        q[..., 128:] /= up
+        kv[..., 512:] = (kv[..., 512:] * 2 * up).clamp(-65504, 65504)
+    else:
+        q[::2, ::5] *= up
+    c.q, c.layout.kv = q, kv.to(c.layout.kv.dtype)
+    flat = c.layout.kv.view(-1, 576).cpu().double()
+    c.rows = [flat[places(c.layout, s, len(r))] for s, r in enumerate(c.rows)]
+
+
+@pytest.mark.parametrize("what,up", [(x, y) for x in ("all", "column", "rope", "some") for y in (2.0 ** 10, 2.0 ** 14, 2.0 ** -12)] +
+                         [("edge", 2.0 ** 15)])
+@pytest.mark.parametrize("tokens,heads", [(1, 16), (3, 16), (3, 128), (2, 3)])
+@pytest.mark.parametrize("w", [torch.bfloat16, torch.float32])
+def test_large_queries_over_an_fp16_cache(cuda, what, up, tokens, heads, w):
+    """Absorbed and scaled, elements of up to some 10^4 (q 2^14, scale log2(e) 0.1): fp16 holds 64 times them up to 1023. With
+    float32 weights the operands come from another kernel."""
+    c = Case(cuda, "paged", [70, 9, 300], tokens, heads=heads, kv=torch.float16, q=torch.float32, w=w, seed=5)
+    large(c, what, up)
+    for variant in (2, 1):
+        c.check(variant, (what, up, variant))
