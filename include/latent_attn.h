@@ -443,7 +443,8 @@ typedef struct la_weigh_args {
    * s * seq_len + p (equal regions), seq_offsets[s] + p, or s *
    * blocks_per_seq * block_size + p (paged). Entries past a sequence's rows
    * are left as they are. A row that is not finite makes its own sequence's
-   * weights NaN. */
+   * weights NaN (or gets nothing, where all its scores are -infinity), a query
+   * that is not those of the rows that its token sees. */
   float* weights;
   la_mla_config cfg;
   void* workspace; /* la_weigh_kv_workspace_size bytes; NULL: taken stream-ordered (not under capture) */

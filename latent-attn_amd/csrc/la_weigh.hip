@@ -524,6 +524,7 @@ __global__ __launch_bounds__(64 * kW, 2) void weigh_scores_kernel(WeighProblem p
 __global__ __launch_bounds__(256) void weigh_sum_kernel(WeighProblem p, int row_blocks) {
   __shared__ float lse[kWeighRows];
   __shared__ f32x4 part[4][8];
+  __shared__ int bad[2];  // whether a row's sum is not a number (of a segment, and the next)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const Spans sp{p};
   const int T_all = sp.total(), W = min((int)gridDim.x, T_all), W1 = min(p.spans, T_all), w = blockIdx.x;
@@ -533,10 +534,12 @@ __global__ __launch_bounds__(256) void weigh_sum_kernel(WeighProblem p, int row_
   int i, first, n;
   if (!sp.find(t, &i, &first, &n)) return;
   const int rows = p.count;
-  while (true) {
+  if (threadIdx.x == 0) bad[0] = 0;
+  for (int turn = 0;; turn ^= 1) {
     const int s = p.seq0 + i, len = source_rows(p.src, s), end = min(t_end, first + n);
     const int c0 = Spans::of(first, T_all, W1), c1 = Spans::of(min(first + n, T_all) - 1, T_all, W1);
     __syncthreads();
+    if (threadIdx.x == 0) bad[turn ^ 1] = 0;
     for (int r = threadIdx.x; r < 32 * row_blocks; r += 256) {
       float m = kNoScore, l = 0.f;
       constexpr int kOnce = 8;  // partial sums whose loads go out together
@@ -558,27 +561,35 @@ __global__ __launch_bounds__(256) void weigh_sum_kernel(WeighProblem p, int row_
         }
       // rows past the last, and tokens that see nothing, give nothing
       lse[r] = l == 0.f ? INFINITY : m + log2f(l);
+      if (l != l) bad[turn] = 1;
     }
     __syncthreads();
+    const bool strict = bad[turn];
     // a tile per wave, or (many rows) a quarter of a tile's row blocks
     const bool shared = row_blocks >= 8;
     const int b0 = shared ? wave : 0, db = shared ? 4 : 1;
     for (int u = shared ? t : t + wave; u < end; u += shared ? 1 : 4) {
       const float* const from = p.scores + (int64_t)u * row_blocks * 1024 + 4 * lane;
       f32x4 sum = {};
+      // hidden rows' scores are -infinity: they get nothing also from a token whose sum is not a number
+      auto add = [&](auto strict) {
 #pragma unroll 4
-      for (int b = b0; b < row_blocks; b += db) {
-        f32x4 v[4];
+        for (int b = b0; b < row_blocks; b += db) {
+          f32x4 v[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const f32x4*>(from + 1024 * b + 256 * q);
+          for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const f32x4*>(from + 1024 * b + 256 * q);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int r = 32 * b + 8 * q + (lane >> 3);
-          const float e = lse[r];
+          for (int q = 0; q < 4; ++q) {
+            const int r = 32 * b + 8 * q + (lane >> 3);
+            const float e = lse[r];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) sum[k] += r < rows ? __builtin_amdgcn_exp2f(v[q][k] - e) : 0.f;
+            for (int k = 0; k < 4; ++k)
+              sum[k] += r < rows && (!strict.value || v[q][k] != -INFINITY) ? __builtin_amdgcn_exp2f(v[q][k] - e) : 0.f;
+          }
         }
-      }
+      };
+      if (strict) add(std::true_type());
+      else add(std::false_type());
 #pragma unroll
       for (int o = 8; o < 64; o <<= 1)
 #pragma unroll

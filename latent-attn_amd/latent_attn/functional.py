@@ -502,7 +502,9 @@ def weigh_kv(
         rotate_q:    q_rope is not rotated yet
         kernel_variant: 0 = automatic, 1 = plain kernels, 2 = matrix cores
 
-    A row that is not finite makes its own sequence's weights NaN.
+    A row that is not finite makes its own sequence's weights NaN (or gets
+    nothing, where all its scores are -infinity), a query that is not those of
+    the rows that its token sees.
     """
     _C = _load_ext()
     _C.weigh_kv_forward(weights, kv_cache, q_nope, q_rope, W_UK, rope_cos, rope_sin, seq_offsets, *_cfg_args(cfg),

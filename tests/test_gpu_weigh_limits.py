@@ -1,5 +1,5 @@
 """weigh_kv at the edges of its arguments' ranges: offsets that are not in order, rooms far wider than their rows,
-queries outside fp16's range over an fp16 cache."""
+queries outside fp16's range over an fp16 cache, queries that are not finite."""
 
 from __future__ import annotations
 
@@ -8,7 +8,7 @@ import ctypes
 import pytest
 import torch
 
-from draft_cases import places
+from draft_cases import places, weight_places
 from prompt_cases import tables, weights
 from test_gpu_weigh import Case
 
@@ -126,3 +126,23 @@ def test_large_queries_over_an_fp16_cache(cuda, what, up, tokens, heads, w):
     large(c, what, up)
     for variant in (2, 1):
         c.check(variant, (what, up, variant))
+
+
+@pytest.mark.parametrize("variant", [1, 2])
+@pytest.mark.parametrize("kv", [torch.bfloat16, torch.float16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("part", [slice(5, 6), slice(150, 151), slice(0, 192)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("tokens,heads", [(3, 16), (40, 16), (5, 128)])
+def test_a_query_that_is_not_finite_stays_with_the_rows_it_sees(cuda, variant, kv, part, bad, tokens, heads):
+    """One head of one token, in a sequence between two others: the rows behind the token get what the others give them."""
+    c = Case(cuda, "paged", [50, 130, 70], tokens, heads=heads, kv=kv, seed=7)
+    c.q[tokens + 1, heads // 2, part] = bad  # the second token of the second sequence: it sees rows 0 to 130 - tokens + 1
+    w = torch.zeros_like(c.weights)
+    c.run(w, kernel_variant=variant)
+    got = w.cpu().double().view(-1)
+    ref, bounds, _ = c.reference()
+    for s, (r, b) in enumerate(zip(ref, bounds)):
+        at = weight_places(c.layout, s, len(r))
+        seen = torch.arange(len(r)) < (130 - tokens + 2 if s == 1 else 0)
+        assert got[at][seen].isnan().all() and r[~seen].isfinite().all()
+        assert ((got[at] - r).abs()[~seen] <= b[~seen]).all()
