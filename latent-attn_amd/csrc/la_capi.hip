@@ -1565,7 +1565,7 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
     }
     if (mfma) {
       q_prep = v.take(2 * prep_elems * 2);
-      if (a->kv_dtype == LA_DTYPE_F16) p.most = static_cast<uint8_t*>(v.take(kMostRow * prep_rows));
+      if (weigh_f16(a->kv_dtype)) p.most = static_cast<uint8_t*>(v.take(kMostRow * prep_rows));
       p.scores = static_cast<float*>(v.take(weigh_score_bytes(most_tiles, p.count)));
       p.part = static_cast<float*>(v.take(weigh_part_bytes(p.spans, p.seqs, p.count)));
     } else {
@@ -1584,7 +1584,7 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
   hipError_t e = hipSuccess;
   if (direct) {
     const AbsorbQueries x{q, p.src, nullptr, p.low, p.most};
-    e = launch_absorb_any(x, a->W_UK, a->w_uk_dtype, q_prep, a->kv_dtype == LA_DTYPE_F16 ? 2 : 1, weigh_query_scale(p), nh, stream, cu_count());
+    e = launch_absorb_any(x, a->W_UK, a->w_uk_dtype, q_prep, weigh_f16(a->kv_dtype) ? 2 : 1, weigh_query_scale(p), nh, stream, cu_count());
   } else {
     t.q = q;
     t.src = p.src;

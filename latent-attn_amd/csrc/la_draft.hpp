@@ -120,6 +120,7 @@ hipError_t launch_weigh_plain(const WeighProblem& p, hipStream_t stream);
 // by the tiles (of 32 rows) that its sequences have room for.
 bool weigh_mfma_supported(const WeighProblem& p);
 constexpr int kWeighKeys = 32, kWeighRows = 4096;  // keys per tile; (token, head) rows of a piece at most
+inline bool weigh_f16(int kv_dtype) { return kv_dtype != LA_DTYPE_BF16; }  // the products' type: fp16, or bf16
 float weigh_query_scale(const WeighProblem& p);
 hipError_t launch_weigh_queries(const WeighProblem& p, hipStream_t stream);  // q_prep from q_abs and q_rope
 int weigh_spans(int rows, int ncu);

@@ -240,10 +240,10 @@ __device__ inline void stage_store(const Staged<kFp8, kW>& x, lchar* L, int wave
   for (int i = 0; i < S::kS; ++i) {
     u32x4 y;
     if constexpr (kFp8) {
-      y[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.c[i][0], 1.f, false));
-      y[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.c[i][0], 1.f, true));
-      y[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.c[i][1], 1.f, false));
-      y[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.c[i][1], 1.f, true));
+      y[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x.c[i][0], 1.f, false));
+      y[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x.c[i][0], 1.f, true));
+      y[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x.c[i][1], 1.f, false));
+      y[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x.c[i][1], 1.f, true));
     } else {
       y = x.c[i];
     }
@@ -287,7 +287,7 @@ __device__ inline void stage_store(const Staged<kFp8, kW>& x, lchar* L, int wave
 //
 // Precision: a score has to hold fp32's worth, since weights are compared with each
 // other; fp32 matrix instructions have a sixteenth of the 16-bit ones' rate.
-// Cache rows are 16-bit numbers (8-bit ones widen exactly), so the queries go in as
+// Cache rows are 16-bit numbers (8-bit ones widen exactly to fp16), so the queries go in as
 // two 16-bit parts, hi and what is left, whose products with a row are exact and
 // summed in fp32: 2 products for the latent part, 3 for the rope part, whose
 // rotated keys have two parts as well. bf16 leaves 2^-18 of an operand, fp16 less.
@@ -673,12 +673,12 @@ __global__ __launch_bounds__(256) void weigh_queries_kernel(WeighProblem p, int6
 }  // namespace
 
 float weigh_query_scale(const WeighProblem& p) {
-  return p.scale_log2 * (p.src.kv_dtype == LA_DTYPE_F16 ? Mm<__half>::kUp : Mm<__hip_bfloat16>::kUp);
+  return p.scale_log2 * (weigh_f16(p.src.kv_dtype) ? Mm<__half>::kUp : Mm<__hip_bfloat16>::kUp);
 }
 
 hipError_t launch_weigh_queries(const WeighProblem& p, hipStream_t stream) {
   const int64_t n = (int64_t)p.src.num_seqs * p.tokens * p.nh * (kQPrepRow / 8);
-  const auto k = p.src.kv_dtype == LA_DTYPE_F16 ? weigh_queries_kernel<__half> : weigh_queries_kernel<__hip_bfloat16>;
+  const auto k = weigh_f16(p.src.kv_dtype) ? weigh_queries_kernel<__half> : weigh_queries_kernel<__hip_bfloat16>;
   return in_grids((n + 255) / 256, most_blocks(256), [&](int64_t first, unsigned blocks) {
     hipLaunchKernelGGL(k, dim3(blocks), dim3(256), 0, stream, p, first);
   });
@@ -713,7 +713,7 @@ int weigh_spans(int rows, int ncu) {  // as many workgroups as run at once
 
 hipError_t launch_weigh_mfma(const WeighProblem& p, hipStream_t stream, int ncu) {
   const int row_blocks = (p.count + 31) / 32;
-  hipError_t e = p.src.kv_dtype == LA_DTYPE_FP8_E4M3 ? scores_w<__hip_bfloat16, true>(p, row_blocks, stream)
+  hipError_t e = p.src.kv_dtype == LA_DTYPE_FP8_E4M3 ? scores_w<__half, true>(p, row_blocks, stream)
                  : p.src.kv_dtype == LA_DTYPE_BF16   ? scores_w<__hip_bfloat16, false>(p, row_blocks, stream)
                                                      : scores_w<__half, false>(p, row_blocks, stream);
   if (e != hipSuccess) return e;

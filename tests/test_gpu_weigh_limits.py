@@ -1,5 +1,6 @@
 """weigh_kv at the edges of its arguments' ranges: offsets that are not in order, rooms far wider than their rows,
-queries outside fp16's range over an fp16 cache, queries that are not finite."""
+queries outside fp16's range over an fp16 cache, queries that are not finite;
+and what two fp16 parts keep."""
 
 from __future__ import annotations
 
@@ -146,3 +147,20 @@ def test_a_query_that_is_not_finite_stays_with_the_rows_it_sees(cuda, variant, k
         seen = torch.arange(len(r)) < (130 - tokens + 2 if s == 1 else 0)
         assert got[at][seen].isnan().all() and r[~seen].isfinite().all()
         assert ((got[at] - r).abs()[~seen] <= b[~seen]).all()
+
+
+@pytest.mark.parametrize("kv", [torch.float8_e4m3fn, torch.float16])
+@pytest.mark.parametrize("tokens,heads", [(1, 16), (1, 64), (1, 128), (16, 16)])
+@pytest.mark.parametrize("w", [torch.bfloat16, torch.float32])
+def test_fp16_parts_keep_as_much_as_fp32(cuda, kv, tokens, heads, w):
+    """Over fp16 and 8-bit rows, which fp16 holds exactly, two fp16 parts of a query are off by 2^-23 of it (11 bits each), a
+    score of about B = 1 (the root of its terms' squares) by no more; its fp32 sum of some 80 steps by 9 half steps of 2^-24
+    (roundings are independent), 2^-22 together with the exponential's. A weight moves by twice that, its exponent's and its
+    sum's: 2 (2^-23 + 2^-22) < 2^-20. Two bf16 parts left 2^-18 of a query."""
+    c = Case(cuda, "paged", [300, 1500], tokens, heads=heads, kv=kv, q=torch.float32, w=w, seed=9)
+    weight = torch.zeros_like(c.weights)
+    c.run(weight, kernel_variant=2)
+    got = weight.cpu().double().view(-1)
+    for s, r in enumerate(c.reference()[0]):
+        at = weight_places(c.layout, s, len(r))
+        assert (got[at] - r).norm() <= 2.0 ** -20 * r.norm()
