@@ -1058,14 +1058,13 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeProblem& p, int gro
       asm volatile("" : "+v"(blk_cur));
     }
 
-    // what this lane's head sees: on its way before the copies, so it has landed with them
-    uint64_t seen = 0;
+    // what the wave's heads see, half a head's word per lane, to LDS: before the copies, so it has landed with them
     if constexpr (kTree) {
-      const int wblk = min(32 * wave, (hg_heads - 1) & ~31), r = min(lane_id() & 31, hg_heads - 1 - wblk);
+      const int ln = lane_id(), wblk = min(32 * wave, (hg_heads - 1) & ~31), r = min(ln >> 1, hg_heads - 1 - wblk);
       uint32_t nh = (uint32_t)p.nh;
       asm volatile("" : "+s"(nh));  // (its reciprocal, made before the loop, was spilled)
       const uint64_t* from = tree.seen + (int64_t)s * p.qps + (uint32_t)(group * kHG + wblk + r) / nh;
-      asm volatile("global_load_dwordx2 %0, %1, off" : "=v"(seen) : "v"(from));
+      __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint32_t*>(from) + (ln & 1), (lds_void*)(L + kSeenOff + 256 * wave), 4, 0, 0);
     }
 
     // tile 1 rides along iteration -1; a fresh lane index keeps the per-lane
@@ -1114,9 +1113,6 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeProblem& p, int gro
     rotate_rows<KT, kFp8>(L, 0, wave, lane_id());  // fresh lane index: no spilled addresses
     if constexpr (kFp8) expand_rows(L, 0, wave, lane_id());
     if constexpr (kTree) {
-      asm volatile("" : "+v"(seen));
-      const int ln = lane_id();
-      if (ln < 32) lds_st(L, kSeenOff + 8 * (32 * wave + ln), seen);
       if (kT > sg.node0) check_rows<KT>(L, 0, wave, lane_id());
     }
     LA_STAMP(5);

@@ -71,6 +71,8 @@ def _dead_high_half_read(instrs: list, n: int, pending: set) -> bool:
     is the high half of its 64-bit addend and whose result's high half is
     overwritten (next in program text) before anything reads it: the low 32 bits of a*b + c depend
     only on the low 32 bits of c, so the stale high half cannot reach a use.
+    An LDS read overwrites it as a VALU result does (what uses the read's own
+    result too early is reported as such).
     (The compiler forms such 64-bit addends from a 32-bit value and whatever
     the next register holds when it only keeps the low half of the sum.)"""
     ins = instrs[n]
@@ -97,8 +99,10 @@ def _dead_high_half_read(instrs: list, n: int, pending: set) -> bool:
             reads |= _regs(o)
         if hi in reads:
             return False
-        if lops and hi in _regs(lops[0]) and not op.startswith(("ds_", "global_", "buffer_")):
-            return True  # overwritten by a VALU result before any read
+        if lops and hi in _regs(lops[0]) and op.startswith(("ds_write", "global_store", "buffer_store")):
+            return False  # an address, or stored data
+        if lops and hi in _regs(lops[0]) and (op.startswith("ds_read") or not op.startswith(("ds_", "global_", "buffer_"))):
+            return True  # overwritten by a VALU result or an LDS read before any read
     return False
 
 
