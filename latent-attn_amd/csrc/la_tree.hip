@@ -184,7 +184,8 @@ __global__ __launch_bounds__(256) void plain_tree_kernel(PlainTree p, int64_t fi
     acc[i] = 0.f;
   }
   float m = kNoScore, l = 0.f;
-  for (int k = wave; k < L; k += 4) {
+  for (int64_t k64 = wave; k64 < L; k64 += 4) {  // (up to 2^31 - 1 rows)
+    const int k = (int)k64;
     int64_t at = k;
     if (k >= before) {
       if (!(seen >> (k - before) & 1)) continue;

@@ -46,8 +46,8 @@ __global__ __launch_bounds__(256) void plain_lse_kernel(WeighProblem p, int64_t 
   const int keys = source_rows(p.src, s) - p.tokens + j + 1;
   float q[16], m = kNoScore, l = 0.f;
   plain_query(p, item, lane, q);
-  for (int k = wave; k < keys; k += 4) {
-    const float x = plain_score(p, q, p.q_rope + item * (int64_t)p.dR, s, k, lane), up = fmaxf(m, x);
+  for (int64_t k = wave; k < keys; k += 4) {  // (up to 2^31 - 1 rows)
+    const float x = plain_score(p, q, p.q_rope + item * (int64_t)p.dR, s, (int)k, lane), up = fmaxf(m, x);
     l = l * exp2f(m - up) + exp2f(x - up);
     m = up;
   }
