@@ -404,8 +404,11 @@ typedef struct la_accept_args {
    * int32, num_seqs * nodes) lists the accepted nodes from the top down, each
    * larger than the one before it; the first entry that is not, or is no node,
    * ends it. Node path[i]'s row moves to row L - nodes + i and the length
-   * becomes L - nodes + (nodes listed). A sequence with fewer rows than nodes
-   * is left unchanged. */
+   * becomes L - nodes + (nodes listed). A sequence with fewer rows than nodes,
+   * or more than its region holds, is left unchanged. Row weights
+   * (la_weigh_args) are not known here: rows are weighed after their path is
+   * accepted, so that those of dropped ones are still what appended ones start
+   * at. */
   int32_t nodes;
   const int32_t* path;
   la_mla_config cfg;
@@ -426,7 +429,10 @@ typedef struct la_weigh_args {
   int32_t blocks_per_seq;
   /* queries of every sequence's last tokens_per_seq rows (num_seqs *
    * tokens_per_seq, num_heads, .), as in la_prefill_args: token j of n of a
-   * sequence with L rows is at position L - n + j and sees the rows up to its own */
+   * sequence with L rows is at position L - n + j and sees the rows up to its
+   * own. One number for all sequences: where accepted paths differ in length,
+   * the newest token of each, or a call per length (num_seqs 1 of the same
+   * cache: the region, or the row of the block table, of one sequence) */
   int32_t tokens_per_seq;
   const void* q_nope;
   const void* q_rope;
@@ -442,7 +448,8 @@ typedef struct la_weigh_args {
   /* fp32, one per row of the sequences' regions: position p of sequence s at
    * s * seq_len + p (equal regions), seq_offsets[s] + p, or s *
    * blocks_per_seq * block_size + p (paged). Entries past a sequence's rows
-   * are left as they are. A row that is not finite makes its own sequence's
+   * are left as they are: what rows appended there start at (a caller that
+   * shortens a sequence zeroes those it drops). A row that is not finite makes its own sequence's
    * weights NaN (or gets nothing, where all its scores are -infinity), a query
    * that is not those of the rows that its token sees. */
   float* weights;

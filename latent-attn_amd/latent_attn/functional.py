@@ -452,13 +452,15 @@ def accept_kv(
     block_size: int = 0,
 ) -> None:
     """Keeps the rows of a tree's accepted path: they become the sequence's
-    last ones, the tree's others are dropped.
+    last ones, the tree's others are dropped. Row weights (``weigh_kv``) are
+    not moved: weigh rows after their path is accepted.
 
     Args:
         kv_cache, seq_offsets, block_table, block_size: as in ``append_kv``
         seq_lens:    int32 (batch,) device tensor: the rows with the trees'
                      among them; set in place to those that stay. A sequence with
-                     fewer than ``nodes`` is left unchanged.
+                     fewer than ``nodes``, or more than its region holds, is left
+                     unchanged.
         nodes:       rows of each tree, 1 to 64
         path:        int32 (batch, nodes) device tensor: the accepted nodes from
                      the top down, ended by -1 (or anything that is not a later
@@ -492,13 +494,17 @@ def weigh_kv(
         weights:     float32 device tensor, changed in place: (batch, capacity),
                      (batch, blocks_per_seq * block_size) for a paged cache,
                      (total_rows,) with ``seq_offsets``. Entries past a
-                     sequence's rows are left as they are (rows appended later
-                     start at what these hold: zeros).
+                     sequence's rows are left as they are: rows appended later
+                     start at what these hold, zeros (zero them where weighed
+                     rows are dropped by other means than ``evict_kv``).
         kv_cache, seq_offsets, seq_lens, block_table, block_size: as in
                      ``mla_prefill``
         q_nope, q_rope: (batch * n, num_heads, .), as in ``mla_prefill``, of the
                      sequences' last n rows: token j of n of a sequence with L
-                     rows is at position L - n + j and sees the rows up to its own
+                     rows is at position L - n + j and sees the rows up to its own.
+                     One n for all sequences: where accepted paths differ in
+                     length, each one's newest token, or a call per sequence
+                     (``kv[s:s + 1]`` or ``block_table[s:s + 1]``, and so on)
         rotate_q:    q_rope is not rotated yet
         kernel_variant: 0 = automatic, 1 = plain kernels, 2 = matrix cores
 
