@@ -27,7 +27,7 @@ __device__ inline float plain_score(const WeighProblem& p, const float (&q)[16],
     const float cs = p.src.cos[rk + i], sn = p.src.sin[rk + i];
     d += qr[i] * (k0 * cs - k1 * sn) + qr[i + half] * (k0 * sn + k1 * cs);
   }
-  return wave_sum(d) * p.scale_log2;
+  return scaled_score(wave_sum(d), p.scale_log2);
 }
 __device__ inline void plain_query(const WeighProblem& p, int64_t item, int lane, float (&q)[16]) {
 #pragma unroll
