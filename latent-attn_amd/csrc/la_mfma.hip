@@ -229,7 +229,7 @@ constexpr int kSeenOff = kLdsBytes;
 constexpr int kTreeLdsBytes = kSeenOff + 8 * kHG;
 constexpr int kBadOff = kCtBytes;
 static_assert(kSeenOff % 8 == 0 && kTreeLdsBytes <= 160 * 1024 && kBadOff + 4 <= kRopeOff && kBadOff % 4 == 0, "tree LDS");
-constexpr float kNoScore = -1e30f;  // a tree's running maximum before the first row that its head sees
+constexpr float kNoScore = -3.402823466e38f;  // a tree's running maximum before the first row that its head sees: no finite score is below
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));

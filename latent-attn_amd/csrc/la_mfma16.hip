@@ -48,7 +48,7 @@
 namespace la {
 namespace {
 
-constexpr float kNoScore = -1e30f;  // trees: a head may see no row of a tile
+constexpr float kNoScore = -3.402823466e38f;  // trees: a head may see no row of a tile; no finite score is below
 constexpr int kDc = 512;
 constexpr int kDr = 64;
 constexpr int kRowElems = kDc + kDr;

@@ -10,7 +10,7 @@
 namespace la {
 namespace {
 
-constexpr float kNoScore = -1e30f;
+constexpr float kNoScore = -3.402823466e38f;  // no finite score is below
 
 __device__ inline uint64_t shfl64(uint64_t v, int lane) {
   const uint32_t lo = __shfl((int)(uint32_t)v, lane, 64), hi = __shfl((int)(uint32_t)(v >> 32), lane, 64);

@@ -10,7 +10,7 @@
 namespace la {
 namespace {
 
-constexpr float kNoScore = -1e30f;
+constexpr float kNoScore = -3.402823466e38f;  // no finite score is below
 constexpr int kLatent = 1024;  // kv_lora_rank at most: 16 elements per lane
 
 // One row's score against one query, by a wave: q (lane + 64 i) and the row's elements in the lanes.

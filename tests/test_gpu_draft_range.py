@@ -1,4 +1,5 @@
-"""Scores of any size in mla_decode_tree and weigh_kv: the largest of them gets the whole weight where they are far apart."""
+"""Scores of any size in mla_decode_tree and weigh_kv: the largest of them gets the whole weight where they are far apart. The
+running maximum starts below every finite one."""
 
 from __future__ import annotations
 
@@ -33,7 +34,7 @@ def queries(c, by):
     return c
 
 
-BY = [1e9, 1e20, -1e20]
+BY = [1e9, 1e20, -1e20, 1e34, -1e34]
 
 
 @pytest.mark.parametrize("n,heads,lengths", [(7, 16, [30, 57]), (64, 128, [70, 64, 99]), (4, 3, [20, 60])])
