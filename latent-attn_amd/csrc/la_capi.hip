@@ -1594,8 +1594,11 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
     t.vec = queries_vec(q);
     if (t.q_nope || t.q_rope) e = launch_tokens(t, stream);
     if (e != hipSuccess) return scratch.finish(record_hip(e));
-    const int st = la_absorb_q(nope_as_is ? static_cast<const float*>(a->q_nope) : t.q_nope, a->W_UK, a->w_uk_dtype, q_abs,
-                               (int)q.tokens, &c, stream_v);
+    const float* const nope = nope_as_is ? static_cast<const float*>(a->q_nope) : t.q_nope;
+    // fp16 weights have la_absorb_q take queries as fp16 parts, which those of a wider type may not fit
+    const bool wide = a->w_uk_dtype == LA_DTYPE_F16 && a->q_dtype != LA_DTYPE_F16;
+    const int st = wide ? status_of(launch_absorb(nope, a->W_UK, a->w_uk_dtype, q_abs, (int)q.tokens, nh, c.qk_nope_head_dim, c.kv_lora_rank, stream))
+                        : la_absorb_q(nope, a->W_UK, a->w_uk_dtype, q_abs, (int)q.tokens, &c, stream_v);
     if (st != LA_SUCCESS) return scratch.finish(st);
     p.q_abs = q_abs;
     p.q_rope = rope_as_is ? static_cast<const float*>(a->q_rope) : t.q_rope;

@@ -328,6 +328,16 @@ __device__ inline void shared_barrier() {
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
+// A value from another lane of the row, as the control word has it.
+template <int kCtrl>
+__device__ inline float quad_swap(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, 0xF, 0xF, true));
+}
+// Maximum of a lane's group of four.
+__device__ inline float quad_max(float v) {
+  v = fmaxf(v, quad_swap<0xB1>(v));    // quad_perm 1 0 3 2
+  return fmaxf(v, quad_swap<0x4E>(v));  // quad_perm 2 3 0 1
+}
 // Eight elements as loaded (in two halves: 16-bit ones are aligned to four), and as values.
 template <typename QT>
 struct Eight {
@@ -339,7 +349,8 @@ struct Eight {
   }
   __device__ float at(int e) const { return (float)v[e >> 2][e & 3]; }
 };
-// kFit: any.most.
+// kFit: any.most. fp16 weights take the queries as two fp16 parts too: those of a wider type
+// are divided by a power of two per token and head (fit_f16 of all 128 elements, found through LDS).
 template <typename WT, typename QT, bool kFit>
 __global__ __launch_bounds__(kAbsThreads, 4) void absorb_any_kernel(AbsorbQueries any, const WT* __restrict__ W,
                                                                     void* __restrict__ out, int out_mode, float scale,
@@ -349,6 +360,9 @@ __global__ __launch_bounds__(kAbsThreads, 4) void absorb_any_kernel(AbsorbQuerie
   typedef typename M::vec vec;
   __shared__ __attribute__((aligned(16))) char wt[128 * kAbsRowBytes];
   __shared__ __attribute__((aligned(16))) char qs[2 * 8 * 2 * 64 * 16];  // [token half][k-step][hi|lo][lane] 16 B
+  constexpr bool kWide = std::is_same<WT, __half>::value && !std::is_same<QT, _Float16>::value;
+  constexpr bool kLate = kWide && kFit && sizeof(QT) == 4;  // loads when they are due: no registers to hold them before
+  __shared__ uint32_t most[2][kWide ? kAnyTokens : 1];  // bits of the tokens' largest elements; of the next 64, zeros
   // (share, 8 heads) groups of 32 workgroups on one XCD each: a 128-B line of q_prep has
   // 8 heads' slots, and the column blocks of a head read the same queries
   constexpr int ncb = 512 / kAbsCols, gb = 8 * ncb;
@@ -371,12 +385,28 @@ __global__ __launch_bounds__(kAbsThreads, 4) void absorb_any_kernel(AbsorbQuerie
       q[i].load(nope + min(t0 + 32 * i + (lane & 31), tokens - 1) * any.q.nope_stride);
     }
   };
+  int turn = 0;
+  // the exponent that token t's queries (of the 64) are divided by
+  auto wide = [&](int t) { return fit_f16((int)(most[turn][t] >> 23)); };
   auto put_q = [&](int t0) {
+    if constexpr (kWide) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float m = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(q[i].at(e)));
+        const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, m), __builtin_bit_cast(uint32_t, m), false, false);
+        if (lane < 32) atomicMax(&most[turn][32 * i + lane], __builtin_bit_cast(uint32_t, fmaxf(f_of(both[0]), f_of(both[1]))));
+      }
+      shared_barrier();
+      if (tid < kAnyTokens) most[turn ^ 1][tid] = 0;
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
+      const float by = kWide ? power_of_2(-wide(32 * i + (lane & 31))) : 1.f;
       float v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = q[i].at(e);
+      for (int e = 0; e < 8; ++e) v[e] = q[i].at(e) * by;
       vec hi, lo;
       split8<WT>(v, hi, lo);
       *reinterpret_cast<vec*>(qs + 16384 * i + 2 * wave * 1024 + 16 * lane) = hi;
@@ -384,7 +414,7 @@ __global__ __launch_bounds__(kAbsThreads, 4) void absorb_any_kernel(AbsorbQuerie
     }
   };
   int t0 = kAnyTokens * share;
-  load_q(t0);
+  if constexpr (!kLate) load_q(t0);
   constexpr int kWLoads = 128 * 16 / kAbsThreads;
   i16x8 wv[kWLoads];
 #pragma unroll
@@ -403,7 +433,8 @@ __global__ __launch_bounds__(kAbsThreads, 4) void absorb_any_kernel(AbsorbQuerie
     own.load(from + rj);
     other.load(from + (rj ^ 32));
   };
-  if (cb == 0) load_rope(t0);
+  if (!kLate && cb == 0) load_rope(t0);
+  if (kWide && tid < kAnyTokens) most[0][tid] = 0;
 #pragma unroll
   for (int i = 0; i < kWLoads; ++i) {
     const int e = tid + kAbsThreads * i;
@@ -441,10 +472,11 @@ __global__ __launch_bounds__(kAbsThreads, 4) void absorb_any_kernel(AbsorbQuerie
   };
   auto row_of = [&](int t) { return (int64_t)(t / qps) * qprep_rows_per_seq(qps * nh) + (int64_t)(t % qps) * nh + h; };
   for (; t0 < tokens; t0 += kAnyTokens * shares) {
+    if constexpr (kLate) load_q(t0);
     put_q(t0);
     shared_barrier();
     const int next = t0 + kAnyTokens * shares;
-    if (next < tokens) load_q(next);
+    if (!kLate && next < tokens) load_q(next);
     const char* const mine = qs + 16384 * (wave >> 2) + 16 * lane;
     f32x16 acc_hi = {}, acc_lo = {};
 #pragma unroll
@@ -455,14 +487,15 @@ __global__ __launch_bounds__(kAbsThreads, 4) void absorb_any_kernel(AbsorbQuerie
     // register 4 q + r: column 32 (wave % 4) + 8 q + 4 (lane / 32) + r of token lane % 32
     const int tt = t0 + 32 * (wave >> 2) + (lane & 31);
     const int64_t to = row_of(tt);
+    const float back = kWide ? scale * power_of_2(wide(32 * (wave >> 2) + (lane & 31))) : scale;
     float fit = 1.f;
     if constexpr (kFit) {  // of the wave's 32 columns, by both halves' lanes
       float m = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf((acc_hi[r] + acc_lo[r] * (1.f / M::kLoScale)) * scale));
+      for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf((acc_hi[r] + acc_lo[r] * (1.f / M::kLoScale)) * back));
       const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, m), __builtin_bit_cast(uint32_t, m), false, false);
       const int e = exponent_of(fmaxf(f_of(both[0]), f_of(both[1])));
-      if (tt < tokens && lane < 32) any.most[to * kMostRow + 4 * cb + (wave & 3)] = (uint8_t)e;
+      if (tt < tokens && lane < 32) any.most[to * kMostRow + 4 * cb + (__builtin_amdgcn_readfirstlane(wave) & 3)] = (uint8_t)e;
       fit = power_of_2(-fit_f16(e));
     }
 #pragma unroll
@@ -470,8 +503,8 @@ __global__ __launch_bounds__(kAbsThreads, 4) void absorb_any_kernel(AbsorbQuerie
       float v[8];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float a = (acc_hi[4 * q2 + r] + acc_lo[4 * q2 + r] * (1.f / M::kLoScale)) * scale * fit;
-        const float b = (acc_hi[4 * q2 + 4 + r] + acc_lo[4 * q2 + 4 + r] * (1.f / M::kLoScale)) * scale * fit;
+        const float a = (acc_hi[4 * q2 + r] + acc_lo[4 * q2 + r] * (1.f / M::kLoScale)) * back * fit;
+        const float b = (acc_hi[4 * q2 + 4 + r] + acc_lo[4 * q2 + 4 + r] * (1.f / M::kLoScale)) * back * fit;
         const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
         v[r] = f_of(both[0]), v[4 + r] = f_of(both[1]);
       }
@@ -482,10 +515,13 @@ __global__ __launch_bounds__(kAbsThreads, 4) void absorb_any_kernel(AbsorbQuerie
       }
     }
     if (cb == 0) {
+      if constexpr (kLate) load_rope(t0);
       const int tr = t0 + (tid >> 3);
+      int r = rj;
+      asm volatile("" : "+v"(r));  // (addresses with it, held through the loop, were spilled)
       f32x4 cs[2], sn[2];
       if (any.q.rotate) {
-        const int64_t at = source_rope_row(any.src, pos) * 32 + (rj & 31);
+        const int64_t at = source_rope_row(any.src, pos) * 32 + (r & 31);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           cs[i] = *reinterpret_cast<const f32x4*>(any.src.cos + at + 4 * i);
@@ -505,21 +541,22 @@ __global__ __launch_bounds__(kAbsThreads, 4) void absorb_any_kernel(AbsorbQuerie
         float m = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[e] *= kUpRope));
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        m = quad_max(m);
+        m = fmaxf(m, quad_swap<0x141>(m));  // the other quad of the eight
         if (tr < tokens && rj == 0) any.most[row_of(tr) * kMostRow + kMostPieces - 1] = (uint8_t)exponent_of(m);
         const float fit = power_of_2(-fit_f16(exponent_of(m)));
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= fit;
       }
       if (tr < tokens) {
-        const int64_t at = qprep_index(row_of(tr), 512 + rj);
+        const int64_t at = qprep_index(row_of(tr), 512 + r);
         if (out_mode == 1) slot(__bf16(), v, at);
         else slot(_Float16(), v, at);
       }
-      if (next < tokens) load_rope(next);
+      if (!kLate && next < tokens) load_rope(next);
     }
     shared_barrier();  // the operands have been read
+    if constexpr (kWide) turn ^= 1;
   }
 }
 
@@ -1151,15 +1188,7 @@ __global__ __launch_bounds__(kMPWaves * 64, 4) void merge_join_kernel(JoinProble
 // call over one sequence of 30,000 rows and 15 of 300, 16 x 128 heads 293 and 319 us, 4 x 64
 // heads 67 and 84; 16 of 500, 2 x 128 heads 45 and 47; 2 of 2000, 25 x 64 heads 57 and 56.
 constexpr int kMSSlots = 4;
-template <int kCtrl>
-__device__ inline float quad_swap(float v) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, 0xF, 0xF, true));
-}
-// Maximum and sum of a lane's group of four.
-__device__ inline float quad_max(float v) {
-  v = fmaxf(v, quad_swap<0xB1>(v));    // quad_perm 1 0 3 2
-  return fmaxf(v, quad_swap<0x4E>(v));  // quad_perm 2 3 0 1
-}
+// Sum of a lane's group of four.
 __device__ inline float quad_sum(float v) {
   v += quad_swap<0xB1>(v);
   return v + quad_swap<0x4E>(v);

@@ -164,3 +164,36 @@ def test_fp16_parts_keep_as_much_as_fp32(cuda, kv, tokens, heads, w):
     for s, r in enumerate(c.reference()[0]):
         at = weight_places(c.layout, s, len(r))
         assert (got[at] - r).norm() <= 2.0 ** -20 * r.norm()
+
+
+@pytest.mark.parametrize("q", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("up", [1.0, 2.0 ** 14, 2.0 ** 20, 2.0 ** -14])
+@pytest.mark.parametrize("kv", [torch.float16, torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("tokens,heads,some", [(1, 16, False), (3, 128, False), (70, 16, True)])
+def test_large_queries_with_fp16_weights(cuda, q, up, kv, tokens, heads, some):
+    """Queries that fp16 does not hold against an fp16 W_UK whose columns are as much smaller (2^-14 at least: fp16's own
+    range; the rope part is as it was). some: of every other token alone, whose scores grow."""
+    c = Case(cuda, "capacity", [70 + tokens, 9, 200], tokens, heads=heads, kv=kv, q=q, w=torch.float16, seed=5)
+    c.q[:: 2 if some else 1, :, :128] *= up
+    if not some:
+        c.W_UK = (c.W_UK.float() / min(max(up, 2.0 ** -10), 2.0 ** 10)).half()
+        if up > 2.0 ** 10:
+            c.q[..., :128:2] = 0  # (the scores grow by what the weights cannot take back)
+    for variant in (2, 1):
+        if some and up > 2.0 ** 14:
+            # scores of 10^6, whose error leaves open which of two close ones is the larger (the bound of a weight is without
+            # limit, and not a number where the weight is 0): each token's and head's weights still add up to 1, in sums of as
+            # many terms as there are tokens, heads and rows, and each is 0 or more
+            w = torch.zeros_like(c.weights)
+            c.run(w, kernel_variant=variant)
+            for s, r in enumerate(c.rows):
+                got = w[s, :len(r)].double()
+                ones = heads * min(tokens, len(r))
+                assert (got >= 0).all() and abs(float(got.sum()) - ones) <= (ones + len(r) + 16) * 2.0 ** -24 * ones
+        else:
+            c.check(variant, (up, variant))
+    if not some:  # queries out of line: absorbed apart
+        pad = torch.zeros(*c.q.shape[:2], c.q.shape[2] + 1, dtype=q, device=cuda)
+        pad[..., 1:] = c.q
+        c.q = pad[..., 1:]
+        c.check(2, (up, "out of line"))
