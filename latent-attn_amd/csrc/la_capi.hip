@@ -1569,7 +1569,7 @@ int weigh(const la_weigh_args* a, void* stream_v, bool run_it, size_t* need) {
       p.scores = static_cast<float*>(v.take(weigh_score_bytes(most_tiles, p.count)));
       p.part = static_cast<float*>(v.take(weigh_part_bytes(p.spans, p.seqs, p.count)));
     } else {
-      p.lse = static_cast<float*>(v.take((size_t)rows * sizeof(float)));
+      p.sums = static_cast<float*>(v.take((size_t)rows * 2 * sizeof(float)));
     }
     return v.total();
   };

@@ -109,7 +109,7 @@ struct WeighProblem {
   const float* q_rope;  // (num_seqs * tokens, nh, dR)
   float scale_log2;
   float* weights;
-  float* lse;  // plain form: (num_seqs * tokens, nh), base 2
+  float* sums;  // plain form: (num_seqs * tokens, nh, 2), rows' maxima and what their exponentials' sums divide by
   // matrix form: the queries' operands (qprep_index, weigh_query_scale), what their
   // rounding left `low` elements on, and one piece of the call, `seqs` sequences from seq0 on and of
   // each `count` of its (token, head) rows from row0 on (a multiple of 32)

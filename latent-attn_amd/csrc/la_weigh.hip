@@ -1,8 +1,9 @@
 // The attention weight that cache rows get (la_weigh_kv):
-//   w[s, p] += sum_{t, h} 2^(x[t, h, p] - lse[t, h]),  x = scale log2(e) (q_abs . c_t[p] + q_rope . RoPE(k_rope[p], p)),
-// over the sequence's last tokens t (causal) and all heads h, lse the base-2
-// log-sum-exp of a row of x. The weights are sums over many steps that rank rows
-// against each other, so they and the scores are kept to fp32.
+//   w[s, p] += sum_{t, h} 2^(x[t, h, p] - m[t, h]) / l[t, h],  x = scale log2(e) (q_abs . c_t[p] + q_rope . RoPE(k_rope[p], p)),
+// over the sequence's last tokens t (causal) and all heads h, m the maximum of a
+// row of x and l the sum of its 2^(x - m). The weights are sums over many steps that rank rows
+// against each other, so they and the scores are kept to fp32. (m and l stay apart: m + log2 l has only
+// what m's size leaves of l, nothing where m passes 2^24.)
 #include "la_draft.hpp"
 
 #include <type_traits>
@@ -35,10 +36,10 @@ __device__ inline void plain_query(const WeighProblem& p, int64_t item, int lane
 }
 
 // The plain form, for any type and head shape: a workgroup of 4 waves per
-// (token, head) for the log-sum-exps, then a wave per row that goes through
+// (token, head) for maxima and sums, then a wave per row that goes through
 // all (token, head) again. Sums in a fixed order. Bound by the rows' and the
 // queries' way from the L2.
-__global__ __launch_bounds__(256) void plain_lse_kernel(WeighProblem p, int64_t first) {
+__global__ __launch_bounds__(256) void plain_sums_kernel(WeighProblem p, int64_t first) {
   __shared__ float ml[4][2];
   const uint32_t item = (uint32_t)first + blockIdx.x;
   const int token = (int)(item / p.nh), s = token / p.tokens, j = token % p.tokens;
@@ -60,7 +61,8 @@ __global__ __launch_bounds__(256) void plain_lse_kernel(WeighProblem p, int64_t 
     float top = kNoScore, total = 0.f;
     for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w][0]);
     for (int w = 0; w < 4; ++w) total += ml[w][1] * exp2f(ml[w][0] - top);
-    p.lse[item] = keys > 0 ? top + log2f(total) : INFINITY;  // no row gets anything of a token that sees none
+    p.sums[2 * (int64_t)item] = keys > 0 ? top : INFINITY;  // no row gets anything of a token that sees none
+    p.sums[2 * (int64_t)item + 1] = keys > 0 ? 1.f / total : 0.f;
   }
 }
 __global__ __launch_bounds__(256) void plain_weigh_kernel(WeighProblem p, int s, int64_t first) {
@@ -72,7 +74,7 @@ __global__ __launch_bounds__(256) void plain_weigh_kernel(WeighProblem p, int s,
   for (int64_t item = ((int64_t)s * p.tokens + j0) * p.nh; item < (int64_t)(s + 1) * p.tokens * p.nh; ++item) {
     float q[16];
     plain_query(p, item, lane, q);
-    sum += exp2f(plain_score(p, q, p.q_rope + item * p.dR, s, (int)k, lane) - p.lse[item]);
+    sum += exp2f(plain_score(p, q, p.q_rope + item * p.dR, s, (int)k, lane) - p.sums[2 * item]) * p.sums[2 * item + 1];
   }
   const int64_t at = (p.src.offsets ? source_begin(p.src, s) : (int64_t)s * p.src.region) + k;
   if (lane == 0) p.weights[at] += sum;
@@ -518,11 +520,13 @@ __global__ __launch_bounds__(64 * kW, 2) void weigh_scores_kernel(WeighProblem p
   }
 }
 
-// The second kernel: rows' log-sum-exps from their partial sums, then a wave per
+// The second kernel: rows' maxima and sums from their parts, then a wave per
 // tile adds the exponentials of its scores over the rows, in their order. Bound by
 // the scores' way back (32 x 8192 rows, 128 heads: 134 MB in 29 us, 4.6 TB/s).
 __global__ __launch_bounds__(256) void weigh_sum_kernel(WeighProblem p, int row_blocks) {
-  __shared__ float lse[kWeighRows];
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  extern __shared__ __attribute__((aligned(8))) char weigh_sums_lds[];
+  f32x2* const all = reinterpret_cast<f32x2*>(weigh_sums_lds);  // of every row its maximum, and 1 / its sum
   __shared__ f32x4 part[4][8];
   __shared__ int bad[2];  // whether a row's sum is not a number (of a segment, and the next)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -560,7 +564,7 @@ __global__ __launch_bounds__(256) void weigh_sum_kernel(WeighProblem p, int row_
           m = up;
         }
       // rows past the last, and tokens that see nothing, give nothing
-      lse[r] = l == 0.f ? INFINITY : m + log2f(l);
+      all[r] = l == 0.f ? f32x2{INFINITY, 0.f} : f32x2{m, 1.f / l};
       if (l != l) bad[turn] = 1;
     }
     __syncthreads();
@@ -581,10 +585,10 @@ __global__ __launch_bounds__(256) void weigh_sum_kernel(WeighProblem p, int row_
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int r = 32 * b + 8 * q + (lane >> 3);
-            const float e = lse[r];
+            const f32x2 e = all[r];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              sum[k] += r < rows && (!strict.value || v[q][k] != -INFINITY) ? __builtin_amdgcn_exp2f(v[q][k] - e) : 0.f;
+              sum[k] += r < rows && (!strict.value || v[q][k] != -INFINITY) ? __builtin_amdgcn_exp2f(v[q][k] - e[0]) * e[1] : 0.f;
           }
         }
       };
@@ -688,7 +692,7 @@ hipError_t launch_weigh_plain(const WeighProblem& p, hipStream_t stream) {
   const int64_t items = (int64_t)p.src.num_seqs * p.tokens * p.nh;
   if (items > INT32_MAX || p.dc > kLatent) return hipErrorInvalidValue;
   hipError_t e = in_grids(items, most_blocks(256), [&](int64_t first, unsigned blocks) {
-    hipLaunchKernelGGL(plain_lse_kernel, dim3(blocks), dim3(256), 0, stream, p, first);
+    hipLaunchKernelGGL(plain_sums_kernel, dim3(blocks), dim3(256), 0, stream, p, first);
   });
   const int64_t most = p.src.offsets ? p.src.total_rows : p.src.region;
   for (int s = 0; s < p.src.num_seqs && e == hipSuccess; ++s)
@@ -718,7 +722,8 @@ hipError_t launch_weigh_mfma(const WeighProblem& p, hipStream_t stream, int ncu)
                                                      : scores_w<__half, false>(p, row_blocks, stream);
   if (e != hipSuccess) return e;
   const int64_t items = row_blocks >= 8 ? p.tiles : ((int64_t)p.tiles + 3) / 4, blocks = items < 8LL * ncu ? items : 8LL * ncu;
-  hipLaunchKernelGGL(weigh_sum_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p, row_blocks);
+  static_assert(8 * kWeighRows <= 64 * 1024, "LDS of a launch");
+  hipLaunchKernelGGL(weigh_sum_kernel, dim3((unsigned)blocks), dim3(256), 8 * 32 * row_blocks, stream, p, row_blocks);
   return hipGetLastError();
 }
 

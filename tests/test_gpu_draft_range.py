@@ -60,3 +60,28 @@ def test_weights(cuda, tokens, heads, kv, variant, by):
     for s, r in enumerate(c.reference()[0]):
         assert float(r.sum()) == heads * tokens and (r == r.round()).all()  # one row per token
         assert torch.equal(got[weight_places(c.layout, s, len(r))], r)
+
+
+@pytest.mark.parametrize("tokens,heads", [(1, 16), (3, 16), (2, 128), (3, 7)])
+@pytest.mark.parametrize("kv", [torch.bfloat16, torch.float16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("variant", [1, 2])
+@pytest.mark.parametrize("by", [1.0, 1e4, 1e9])
+def test_large_scores_that_are_alike(cuda, tokens, heads, kv, variant, by):
+    """Rows that are one and the same share a token's weight evenly, whatever their score: its sum is the number of rows that the
+    token sees, which a maximum of 10^8 that it was added to as a logarithm would swallow."""
+    lengths = [300, 33, tokens]
+    g = torch.Generator().manual_seed(tokens)
+    row = torch.randn(1, 576, generator=g).to(kv).float()
+    row[:, 512:] = 0
+    c = Weigh(cuda, "paged", lengths, tokens, heads=heads, kv=kv, q=torch.float32, rotate_q=False,
+              data=[row.expand(n, -1).contiguous() for n in lengths])
+    c.q *= by
+    w = torch.zeros_like(c.weights)
+    c.run(w, kernel_variant=variant)
+    got = w.cpu().double().view(-1)
+    for s, n in enumerate(lengths):
+        sees = torch.arange(tokens) + n - tokens + 1
+        want = torch.tensor([heads * float((1.0 / sees[sees > k]).sum()) for k in range(n)], dtype=torch.float64)
+        off = (got[weight_places(c.layout, s, n)] - want).abs()
+        # the exponentials are 1; a reciprocal, its sums over tokens and heads
+        assert (off <= (tokens * heads + 4) * 2.0 ** -24 * want).all()
