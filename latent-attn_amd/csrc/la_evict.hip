@@ -171,7 +171,7 @@ __global__ __launch_bounds__(64 * kW) void evict_select_kernel(EvictProblem p, i
       const uint64_t all = __builtin_amdgcn_ballot_w64(stay);
       const uint32_t i = i0 + 64 * e, mine = to + __popcll(all & before);
       to += __popcll(all);
-      if (stay) {
+      if (stay && mine < keep) {
         kept[mine] = (int32_t)i;
         from[mine] = (uint32_t)moved_index(p.rows, s, begin, (int)i);
         if (mine != i) {
@@ -180,6 +180,12 @@ __global__ __launch_bounds__(64 * kW) void evict_select_kernel(EvictProblem p, i
         }
       }
     }
+  }
+  // Weights that another sequence moves meanwhile (offsets that overlap) are other ones at every look: the rows that
+  // stay are then not as many as they should be, and every entry still has to name a row.
+  for (uint32_t i = done + tid; i < keep; i += kThreads) {
+    kept[i] = (int32_t)i;
+    from[i] = (uint32_t)moved_index(p.rows, s, begin, (int)i);
   }
   if (moves < p.keep) atomicMin(&moved, moves);
   __syncthreads();
