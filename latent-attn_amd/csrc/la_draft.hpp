@@ -6,13 +6,6 @@
 
 namespace la {
 
-// A score from its sum. Fused with a subtraction of the same score, rounded (its row's maximum), the product would leave
-// its rounding there, past 2^24 more than an exponent: the row's largest weight was infinite.
-__device__ inline float scaled_score(float sum, float scale) {
-#pragma clang fp contract(off)
-  return sum * scale;
-}
-
 constexpr int kTreeNodes = LA_TREE_MAX_NODES;
 static_assert(kTreeNodes == 64, "a node's ancestors are the bits of one word, a tree's nodes the lanes of one wave");
 

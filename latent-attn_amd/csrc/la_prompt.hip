@@ -511,7 +511,7 @@ __global__ __launch_bounds__(256) void generic_prompt_kernel(GenericPrompt p, in
       const float cs = p.src.cos[rk + i], sn = p.src.sin[rk + i];
       d += q_l[i] * (k0 * cs - k1 * sn) + q_l[i + half] * (k0 * sn + k1 * cs);
     }
-    const float x = wave_sum(d) * p.scale_log2;
+    const float x = scaled_score(wave_sum(d), p.scale_log2);
     const float up = fmaxf(m, x), a = exp2f(m - up), w = exp2f(x - up);
     m = up;
     l = l * a + w;

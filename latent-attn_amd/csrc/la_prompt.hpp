@@ -322,6 +322,13 @@ struct AbsorbQueries {
   int64_t low;         // > 0: also what the rounded rows leave, in a second array so many elements on
   uint8_t* most;       // fp16 parts of any queries: (rows, kMostRow), exponents of the pieces' largest numbers (fit_f16); or nullptr
 };
+// A score from its sum. Fused with a subtraction of the same score, rounded (its row's maximum), the product would leave
+// its rounding there, past 2^24 more than an exponent: the row's largest weight was infinite.
+__device__ inline float scaled_score(float sum, float scale) {
+#pragma clang fp contract(off)
+  return sum * scale;
+}
+
 // Two fp16 parts of a row of queries. Its pieces of 32 latent columns, and its rope part (which comes doubled, for keys in
 // halves), are each divided by a power of two that goes by their largest number m (as exponent_of has it): 1 for m from
 // 2^-6 on below 2^15, where two parts hold it to 2^-19 or better (and where it is not finite), else the one that brings it to
