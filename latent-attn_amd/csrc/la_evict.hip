@@ -17,10 +17,9 @@
 // waits for another. A few sequences have too few stripes for that; their rows go
 // through a copy, two launches over all compute units.
 //
-// What bounds it (bf16): 32 sequences of 8192 rows cut to 2048, 48 us: selection 18, five
-// rounds of barriers over registers on 32 compute units; movement 30 to 49 (from the
-// caches or HBM), 147 MB. One of 32,768 to 16,384: 66 us through the copy, 529 in stripes;
-// 1001 to 512: 21, latency.
+// What bounds it (bf16): 32 sequences of 8192 rows cut to 2048, 67 us in the two kernels: selection 18, five
+// rounds of barriers over registers on 32 compute units; movement 49 for 147 MB from HBM, 3.0 TB/s (37 from
+// the caches, where the same inputs come again and again). 1001 rows of one to 512: 20 us, latency.
 #include "la_draft.hpp"
 
 #include <algorithm>
@@ -277,6 +276,13 @@ hipError_t move_t(const EvictProblem& p, hipStream_t stream) {
 
 }  // namespace
 
+// Two launches over all compute units against stripes, whose time goes by the rows kept. A call over 576 bf16
+// elements a row (9 stripes, so up to 14 sequences take the copy), us, stripes / copy:
+//   1 sequence, 1001 rows to 512 17.2 / 19.3, 8192 to 512 23.8 / 25.6, to 2048 30.3 / 26.5, 32,768 to 512 54.5 / 56.5,
+//     to 2048 62.1 / 57.8, to 16,384 123 / 65.4
+//   4 of 1001 to 512 17.7 / 20.0, 8192 to 2048 31.8 / 29.7, 32,768 to 16,384 152 / 101
+//   13 of 1001 to 512 18.6 / 22.6, 8192 to 2048 35.6 / 42.5; 16 of 8192 to 2048 38.0 / 49.4; 32 58.3 / 73.5
+// The lengths are on the device and most of a copy's gain is where much is kept: a few us lost below, 50 gained above.
 bool evict_staged(const EvictProblem& p, int ncu) {
   const int unit = moved_unit(p.rows);
   return p.rows.num_seqs * ((p.rows.row_bytes / unit + kLanes - 1) / kLanes) < ncu / 2;

@@ -45,7 +45,8 @@ __device__ inline int tree_rows(const TreeQueries& p, int s) {
 // (a segment's fixed part: its queries, its first tiles' way, its partial rows), own
 // chunks for the shorter last ones: the smaller estimate of the longest chunk is taken.
 // (16 trees of 16 behind 500 to 6000 rows, 128 heads, 16 chunks: own chunks 404 us a call, even
-// ones 328.)
+// ones 328. With 4, 8, 16 or 32 tiles for kSegment calls differ where it decides: 12 trees of 8 behind 200 to
+// 9000 rows, 128 heads 163, 162, 153, 154; 20 of 16 behind 500 to 8000, 64 heads 231, 231, 231, 240; 16 of 16 and 4 of 64 the same.)
 constexpr int kSegment = 8;
 __device__ inline void plan_spans(const TreeQueries& p) {
   const int lane = wave_lane(), seqs = p.q.num_seqs;

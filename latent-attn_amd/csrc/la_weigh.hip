@@ -299,13 +299,14 @@ __device__ inline void stage_store(const Staged<kFp8, kW>& x, lchar* L, int wave
 // contraction, summed through LDS. So all matrix cores work whatever the rows, and
 // a SIMD has two waves (256 registers each), one's other work under the other's
 // products: up to 64 rows in two workgroups of 4 waves per CU, more in one of 8, whose
-// tiles serve 128 rows (32 x 8192 rows, 128 heads: a call 154 us; in the form of 64 rows,
+// tiles serve 128 rows (32 x 8192 rows, 128 heads: a call 154 us when they were compared; in the form of 64 rows,
 // which loads and stages every tile twice, 171). Tiles go HBM -> registers -> LDS, the
 // next one on its way during the products; a buffer of its own for it and for the sums
 // leaves one barrier a tile (with two 158).
 // What bounds it: at 128 rows the round of staging, products, sums and exponentials of a
 // tile, 114 us for those 302 MB and 82 GFLOP (hi and lo): 2.7 TB/s and 0.72 PFLOP/s, each
-// half of its rate. With 16 rows (64 x 300 to 4000 8-bit rows) 26 us, 2.7 TB/s of rows, the
+// half of its rate (fp16 rows, with their queries' and keys' scaling, 145 a call for 141, 8-bit ones 134 for 128 as
+// bf16). With 16 rows (64 x 300 to 4000 8-bit rows) 27 us, 2.7 TB/s of rows, the
 // same round with a quarter of the products; 1001 rows of one sequence 11 us, a few round trips.
 constexpr int weigh_sums(int kWR, int kW) { return (kW / kWR == 2 ? 2048 : 4096) * kW; }
 template <typename T, bool kFp8, int kWR, int kW>
@@ -522,7 +523,7 @@ __global__ __launch_bounds__(64 * kW, 2) void weigh_scores_kernel(WeighProblem p
 
 // The second kernel: rows' maxima and sums from their parts, then a wave per
 // tile adds the exponentials of its scores over the rows, in their order. Bound by
-// the scores' way back (32 x 8192 rows, 128 heads: 134 MB in 29 us, 4.6 TB/s).
+// the scores' way back (32 x 8192 rows, 128 heads: 134 MB in 30 us, 4.5 TB/s).
 __global__ __launch_bounds__(256) void weigh_sum_kernel(WeighProblem p, int row_blocks) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   extern __shared__ __attribute__((aligned(8))) char weigh_sums_lds[];
