@@ -197,3 +197,23 @@ def test_large_queries_with_fp16_weights(cuda, q, up, kv, tokens, heads, some):
         pad[..., 1:] = c.q
         c.q = pad[..., 1:]
         c.check(2, (up, "out of line"))
+
+
+@pytest.mark.parametrize("variant", [1, 2])
+@pytest.mark.parametrize("kv", [torch.bfloat16, torch.float16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("part", [slice(300, 301), slice(540, 541), slice(575, 576)])
+def test_one_element_of_a_row_that_is_not_a_number(cuda, variant, kv, part):
+    """Of every type, in the latent or the rope part: its own sequence's weights, and no other's."""
+    c = Case(cuda, "paged", [50, 60, 70], 3, kv=kv, seed=3)
+    ref, bounds, _ = c.reference()
+    flat = c.layout.kv.view(-1, 576)
+    where = places(c.layout, 1, 60)[20]
+    row = flat[where].float()
+    row[part] = float("nan")
+    flat[where] = row.to(kv)
+    w = torch.zeros_like(c.weights)
+    c.run(w, kernel_variant=variant)
+    got = w.cpu().double().view(-1)
+    assert got[weight_places(c.layout, 1, 60)].isnan().all()
+    for s in (0, 2):
+        assert ((got[weight_places(c.layout, s, len(ref[s]))] - ref[s]).abs() <= bounds[s]).all()
